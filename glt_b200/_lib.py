@@ -78,7 +78,20 @@ class GltMlpSaved(C.Structure):
     _fields_ = [("x_ffn", _vp), ("variance", _vp), ("energy_sq", _vp), ("delta_down", _vp)]
 
 
+class GltKv8Cache(C.Structure):
+    """ctypes mirror of GltKv8Cache (include/glt_graft.h)."""
+    _fields_ = [("format", _i32), ("block_tokens", _i32), ("num_kv_heads", _i32), ("head_dim", _i32),
+                ("num_blocks", C.c_int64), ("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp)]
+
+
+class GltKv8Batch(C.Structure):
+    """ctypes mirror of GltKv8Batch (include/glt_graft.h)."""
+    _fields_ = [("num_seqs", _i32), ("max_blocks", _i32), ("rows", _i32), ("max_new", _i32),
+                ("block_table", _vp), ("lengths", _vp), ("row_start", _vp)]
+
+
 _cfgp = C.POINTER(GltModelConfig)
+_kcp, _kbp = C.POINTER(GltKv8Cache), C.POINTER(GltKv8Batch)
 _gwp = C.POINTER(GltGraftWeights)
 _svp = C.POINTER(GltMlpSaved)
 _fp = C.POINTER(C.c_void_p)
@@ -172,6 +185,20 @@ SIGNATURES: dict[str, tuple] = {
     "glt_model_save_checkpoint": (_i32, [_vp, C.c_char_p, C.c_char_p, _i32]),
     "glt_model_load_checkpoint": (_i32, [_vp, C.c_char_p, C.c_char_p, _i32]),
     "glt_load_bin": (_i32, [C.c_char_p, C.POINTER(_i32), C.POINTER(_i32), _vp, _i64]),
+    "glt_kv8_append": (_i32, [_kcp, _kbp, _vp, _i64, _vp, _i64, _vp]),
+    "glt_kv8_attention_workspace": (_i32, [_kcp, _kbp, _i32, C.POINTER(_i64)]),
+    "glt_kv8_attention": (_i32, [_kcp, _kbp, _vp, _i64, _vp, _i64, _vp, _i32, _f32, _i32, _vp, _i64, _vp,
+                                 _i64, _vp]),
+    "glt_kv8_read": (_i32, [_kcp, _kbp, _vp, _i32, _vp, _vp, _vp]),
+    "glt_w4_packed_bytes": (_i32, [_i32, _i32, _i32, _i32, C.POINTER(_i64)]),
+    "glt_w4_quantize": (_i32, [_vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "glt_w4_pack": (_i32, [_vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp]),
+    "glt_w4_unpack": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
+    "glt_w4_linear": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp, _i64, _i32, _vp, _i64, _i32, _vp, _i64, _vp]),
+    "glt_token_logprobs": (_i32, [_vp, _i32, _i64, _i32, _i32, _vp, _f32, _i32, _vp, _vp, _vp, _vp, _vp,
+                                  _vp]),
+    "glt_token_logprobs_bwd": (_i32, [_vp, _i32, _i64, _i32, _i32, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _i64,
+                                      _vp]),
     "glt_batch_walk_start": (_i32, [_u64, _i32, _i32, C.POINTER(_i32), C.POINTER(_i32)]),
     "glt_batch_step": (_i32, [_vp, _i32, _vp, _i32, _i32, _i32, C.POINTER(_i32), C.POINTER(_i32),
                               _vp, _vp]),

@@ -97,6 +97,13 @@ __device__ __forceinline__ uint32_t pack_bf16x2_rn(float a, float b) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
   return r;
 }
+// One float to bf16 bits with the same conversion (a NaN stays a NaN, which the
+// bias trick of f32_to_bf16_bits does not promise).
+__device__ __forceinline__ uint16_t bf16_bits_rn(float a) {
+  uint16_t r;
+  asm("cvt.rn.bf16.f32 %0, %1;" : "=h"(r) : "f"(a));
+  return r;
+}
 // 2^x on the special-function unit (PTX ex2.approx.ftz.f32).
 __device__ __forceinline__ float ex2_approx(float x) {
   float r;

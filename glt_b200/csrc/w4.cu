@@ -1,0 +1,290 @@
+// Products with 4-bit weights and group scales (glt_w4_*).
+//
+// Packed layout of W [N, K]: rows in tiles of 16, columns in chunks of 64 (the last
+// ones filled up with zero scales).  A chunk of a tile is 128 words of eight codes,
+// in the order the A fragments of mma.m16n8k16 want them: lane 4g + c of a warp owns
+// words 4 * lane + s, s = 0..3, and word s holds, for the k-step s of the chunk, rows
+// g and g + 8 at columns col(c, s, 0..3) = (s / 2) * 32 + c * 8 + (s % 2) * 4 + 0..3.
+// So a warp reads a chunk as one 16-byte load a lane, 512 contiguous bytes, and each
+// 32-column half of the chunk (the smallest group) is two whole k-steps.
+// Register i of the fragment (row half i % 2, column pair i / 2) takes its two codes
+// from bits 4i + 3 .. 4i + 6 and 16 further up (modulo 32): a rotation by 4i brings
+// them to mantissa bits 3..6 of two bf16 numbers 1 + code / 16, exactly.
+#include <math.h>
+
+#include "common.cuh"
+#include "gemm.cuh"
+
+namespace glt {
+namespace {
+
+__host__ __device__ inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
+
+// Offsets of the three parts of a packed matrix.
+struct W4Layout {
+  int N, K, group, asym;
+  int tiles, chunks, groups;  // groups: of the filled-up columns
+  int64_t scale_off, zero_off, bytes;
+  W4Layout(int N_, int K_, int group_, int asym_) : N(N_), K(K_), group(group_), asym(asym_) {
+    tiles = (N + 15) / 16;
+    chunks = (K + 63) / 64;
+    groups = static_cast<int>(up(static_cast<int64_t>(chunks) * 64, group) / group);
+    scale_off = up(static_cast<int64_t>(tiles) * chunks * 512, 256);
+    // [tile][group][g][row half] bf16, then the zeros as bytes in the same order
+    zero_off = up(scale_off + static_cast<int64_t>(tiles) * groups * 32, 256);
+    bytes = zero_off + (asym ? up(static_cast<int64_t>(tiles) * groups * 16, 256) : 0);
+  }
+};
+
+int check_shape(int N, int K, int group) {
+  if (group != 32 && group != 64 && group != 128) return fail(GLT_EINVAL, "w4: group %d (32, 64 or 128)", group);
+  if (N < 1 || K < 1 || K % group) return fail(GLT_EINVAL, "w4: N %d, K %d (a positive multiple of the group %d)", N, K, group);
+  return GLT_OK;
+}
+
+__device__ __forceinline__ float finite_or_zero(float x) { return fabsf(x) < INFINITY ? x : 0.f; }
+
+// One warp a group: the group's largest magnitude (or range), then its codes.
+__global__ void __launch_bounds__(256) w4_quantize_kernel(const uint16_t* __restrict__ w, int64_t ld, int N,
+                                                          int K, int group, int asym, uint8_t* __restrict__ codes,
+                                                          uint16_t* __restrict__ scales, uint8_t* __restrict__ zeros) {
+  const int lane = threadIdx.x & 31;
+  const int ng = K / group;
+  const int64_t total = static_cast<int64_t>(N) * ng;
+  for (int64_t u = blockIdx.x * 8ll + (threadIdx.x >> 5); u < total; u += gridDim.x * 8ll) {
+    const int64_t n = u / ng;
+    const int k0 = static_cast<int>(u - n * ng) * group;
+    float x[4];
+    float lo = 0.f, hi = 0.f;
+    for (int j = 0; j < group / 32; ++j) {
+      x[j] = bf16_bits_to_f32(w[n * ld + k0 + j * 32 + lane]);
+      const float f = finite_or_zero(x[j]);
+      lo = fminf(lo, f);
+      hi = fmaxf(hi, f);
+    }
+    lo = -warp_max(-lo);
+    hi = warp_max(hi);
+    const uint16_t sb = bf16_bits_rn(asym ? (hi - lo) / 15.f : fmaxf(hi, -lo) / 7.f);
+    const float s = bf16_bits_to_f32(sb);
+    const float z = !asym ? 8.f : s > 0.f ? fminf(fmaxf(rintf(-lo / s), 0.f), 15.f) : 0.f;
+    if (lane == 0) {
+      scales[u] = sb;
+      if (asym) zeros[u] = static_cast<uint8_t>(z);
+    }
+    for (int j = 0; j < group / 32; ++j) {
+      // a NaN (or a group of zeros) takes the code of 0
+      const float q = s > 0.f && x[j] == x[j] ? rintf(x[j] / s) : 0.f;
+      codes[n * K + k0 + j * 32 + lane] = static_cast<uint8_t>(fminf(fmaxf(q + z, 0.f), 15.f));
+    }
+  }
+}
+
+__device__ __forceinline__ int chunk_col(int c, int s, int e) { return (s >> 1) * 32 + c * 8 + (s & 1) * 4 + e; }
+__device__ __forceinline__ int code_bit(int i, int h) { return (3 + 16 * h + 4 * i) & 31; }
+
+__global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t* __restrict__ codes,
+                                                      const uint16_t* __restrict__ scales,
+                                                      const uint8_t* __restrict__ zeros, W4Layout L,
+                                                      uint8_t* __restrict__ packed) {
+  const int ng = L.K / L.group;
+  const int64_t words = static_cast<int64_t>(L.tiles) * L.chunks * 128;
+  const int64_t scs = static_cast<int64_t>(L.tiles) * L.groups * 16;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
+  const int64_t first = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
+  for (int64_t q = first; q < words; q += step) {
+    const int s = q & 3, lane = (q >> 2) & 31;
+    const int64_t tc = q >> 7;
+    const int64_t tile = tc / L.chunks;
+    const int chunk = static_cast<int>(tc - tile * L.chunks);
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t n = tile * 16 + (lane >> 2) + 8 * (i & 1);
+        const int k = chunk * 64 + chunk_col(lane & 3, s, 2 * (i >> 1) + h);
+        const uint32_t u = n < L.N && k < L.K ? codes[n * L.K + k] & 15u : 0u;
+        const int b = code_bit(i, h);
+        word |= b <= 28 ? u << b : (u << b) | (u >> (32 - b));
+      }
+    reinterpret_cast<uint32_t*>(packed)[q] = word;
+  }
+  for (int64_t q = first; q < scs; q += step) {
+    const int64_t tg = q >> 4;
+    const int64_t tile = tg / L.groups;
+    const int grp = static_cast<int>(tg - tile * L.groups);
+    const int64_t n = tile * 16 + ((q >> 1) & 7) + 8 * (q & 1);
+    const bool in = n < L.N && grp < ng;
+    reinterpret_cast<uint16_t*>(packed + L.scale_off)[q] = in ? scales[n * ng + grp] : 0;
+    if (L.asym) packed[L.zero_off + q] = in ? zeros[n * ng + grp] & 15u : 0;
+  }
+}
+
+__global__ void __launch_bounds__(256) w4_unpack_kernel(const uint8_t* __restrict__ packed, W4Layout L,
+                                                        uint16_t* __restrict__ w, int64_t ld) {
+  const int64_t total = static_cast<int64_t>(L.N) * L.K;
+  for (int64_t q = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; q < total;
+       q += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t n = q / L.K;
+    const int k = static_cast<int>(q - n * L.K);
+    const int r = n & 15, kk = k & 63;
+    const int s = (kk >> 5) * 2 + ((kk >> 2) & 1), c = (kk >> 3) & 3, e = kk & 3;
+    const int64_t word = (((n >> 4) * L.chunks + (k >> 6)) * 32 + (r & 7) * 4 + c) * 4 + s;
+    const int b = code_bit((r >> 3) + 2 * (e >> 1), e & 1);
+    const uint32_t v = reinterpret_cast<const uint32_t*>(packed)[word];
+    const float u = static_cast<float>(__funnelshift_r(v, v, b) & 15u);
+    const int64_t sc = ((n >> 4) * L.groups + k / L.group) * 16 + (r & 7) * 2 + (r >> 3);
+    const float z = L.asym ? static_cast<float>(packed[L.zero_off + sc]) : 8.f;
+    w[n * ld + k] = bf16_bits_rn((u - z) * bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(packed + L.scale_off)[sc]));
+  }
+}
+
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// y = x . W^T for 8 rows of x: a warp takes one tile of 16 weight rows and walks its chunks.
+__global__ void __launch_bounds__(128) w4_linear_kernel(const uint8_t* __restrict__ packed, W4Layout L,
+                                                        const uint16_t* __restrict__ x, int64_t ld_x, int M,
+                                                        void* __restrict__ y, int64_t ld_y, int y_bf16,
+                                                        const uint16_t* __restrict__ resid, int64_t ld_r) {
+  const int64_t tile = blockIdx.x * 4ll + (threadIdx.x >> 5);
+  if (tile >= L.tiles) return;
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+  const int m = blockIdx.y * 8 + g;
+  const uint4* cw = reinterpret_cast<const uint4*>(packed) + tile * L.chunks * 32 + lane;
+  const uint32_t* sw = reinterpret_cast<const uint32_t*>(packed + L.scale_off) + tile * L.groups * 8 + g;
+  const uint16_t* zw = reinterpret_cast<const uint16_t*>(packed + L.zero_off) + tile * L.groups * 8 + g;
+  float acc[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int ch = 0; ch < L.chunks; ++ch) {
+    const uint4 v = cw[ch * 32];
+    const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int k = ch * 64 + half * 32;
+      if (k >= L.K) break;
+      uint4 xv = make_uint4(0, 0, 0, 0);
+      if (m < M) xv = *reinterpret_cast<const uint4*>(x + m * ld_x + k + c * 8);
+      const uint32_t b[4] = {xv.x, xv.y, xv.z, xv.w};
+      const int grp = k / L.group;
+      const uint32_t sc = sw[grp * 8];
+      // 1 + zero / 16 of rows g and g + 8, twice each
+      uint32_t z0 = 0x3FC03FC0u, z1 = 0x3FC03FC0u;
+      if (L.asym) {
+        const uint32_t z = zw[grp * 8];
+        z0 = (0x3F80u | ((z & 15u) << 3)) * 0x10001u;
+        z1 = (0x3F80u | (((z >> 8) & 15u) << 3)) * 0x10001u;
+      }
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        uint32_t a[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t t = __funnelshift_r(word[half * 2 + s], word[half * 2 + s], 4 * i);
+          a[i] = sub_bf16x2((t & 0x00780078u) | 0x3F803F80u, (i & 1) ? z1 : z0);
+        }
+        mma_bf16(part, a, b[2 * s], b[2 * s + 1]);
+      }
+      const float s0 = 16.f * bf16_lo(sc), s1 = 16.f * bf16_hi(sc);
+      acc[0] += s0 * part[0];
+      acc[1] += s0 * part[1];
+      acc[2] += s1 * part[2];
+      acc[3] += s1 * part[3];
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int64_t n = tile * 16 + g + 8 * (q >> 1), row = blockIdx.y * 8 + 2 * c + (q & 1);
+    if (n >= L.N || row >= M) continue;
+    const float o = acc[q] + (resid ? bf16_bits_to_f32(resid[row * ld_r + n]) : 0.f);
+    if (y_bf16)
+      static_cast<uint16_t*>(y)[row * ld_y + n] = bf16_bits_rn(o);
+    else
+      static_cast<float*>(y)[row * ld_y + n] = o;
+  }
+}
+
+int grid_for(int64_t units, int per_cta) {
+  const int64_t b = (units + per_cta - 1) / per_cta, cap = static_cast<int64_t>(num_sms()) * 16;
+  return static_cast<int>(b < 1 ? 1 : b < cap ? b : cap);
+}
+
+}  // namespace
+}  // namespace glt
+
+using glt::W4Layout;
+
+extern "C" int glt_w4_packed_bytes(int N, int K, int group, int asym, int64_t* bytes) {
+  if (!bytes) return glt::fail(GLT_EINVAL, "null argument");
+  GLT_TRY(glt::check_shape(N, K, group));
+  *bytes = W4Layout(N, K, group, asym).bytes;
+  return GLT_OK;
+}
+
+extern "C" int glt_w4_quantize(const uint16_t* w, int64_t ld_w, int N, int K, int group, int asym,
+                               uint8_t* codes, uint16_t* scales, uint8_t* zeros, void* stream) {
+  if (!w || !codes || !scales || (asym && !zeros)) return glt::fail(GLT_EINVAL, "null argument");
+  GLT_TRY(glt::check_shape(N, K, group));
+  if (ld_w < K) return glt::fail(GLT_EINVAL, "w4: row stride %lld below K %d", (long long)ld_w, K);
+  const int64_t units = static_cast<int64_t>(N) * (K / group);
+  glt::w4_quantize_kernel<<<glt::grid_for(units, 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      w, ld_w, N, K, group, asym, codes, scales, zeros);
+  GLT_LAUNCH_CHECK();
+  return GLT_OK;
+}
+
+extern "C" int glt_w4_pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int N,
+                           int K, int group, void* packed, void* stream) {
+  if (!codes || !scales || !packed) return glt::fail(GLT_EINVAL, "null argument");
+  GLT_TRY(glt::check_shape(N, K, group));
+  if (!glt::aligned16(packed)) return glt::fail(GLT_EINVAL, "w4: packed weights must be 16-byte aligned");
+  const W4Layout L(N, K, group, zeros != nullptr);
+  glt::w4_pack_kernel<<<glt::grid_for(static_cast<int64_t>(L.tiles) * L.chunks * 128, 256), 256, 0,
+                        static_cast<cudaStream_t>(stream)>>>(codes, scales, zeros, L, static_cast<uint8_t*>(packed));
+  GLT_LAUNCH_CHECK();
+  return GLT_OK;
+}
+
+extern "C" int glt_w4_unpack(const void* packed, int N, int K, int group, int asym, uint16_t* w,
+                             int64_t ld_w, void* stream) {
+  if (!packed || !w) return glt::fail(GLT_EINVAL, "null argument");
+  GLT_TRY(glt::check_shape(N, K, group));
+  if (ld_w < K) return glt::fail(GLT_EINVAL, "w4: row stride %lld below K %d", (long long)ld_w, K);
+  if (!glt::aligned16(packed)) return glt::fail(GLT_EINVAL, "w4: packed weights must be 16-byte aligned");
+  glt::w4_unpack_kernel<<<glt::grid_for(static_cast<int64_t>(N) * K, 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      static_cast<const uint8_t*>(packed), W4Layout(N, K, group, asym), w, ld_w);
+  GLT_LAUNCH_CHECK();
+  return GLT_OK;
+}
+
+extern "C" int glt_w4_linear(const void* packed, int N, int K, int group, int asym, const uint16_t* x,
+                             int64_t ld_x, int M, void* y, int64_t ld_y, int y_dtype,
+                             const uint16_t* resid, int64_t ld_r, void* stream) {
+  GLT_TRY(glt::check_shape(N, K, group));
+  if (!packed || (M > 0 && (!x || !y))) return glt::fail(GLT_EINVAL, "null argument");
+  if (M < 0) return glt::fail(GLT_EINVAL, "w4: negative rows");
+  if (y_dtype != 0 && y_dtype != 1) return glt::fail(GLT_EINVAL, "w4: output type %d (0 fp32, 1 bf16)", y_dtype);
+  if (ld_x < K || ld_x % 8 || !glt::aligned16(x))
+    return glt::fail(GLT_EINVAL, "w4: x needs 16-byte aligned rows (row stride a multiple of 8, at least K)");
+  if (ld_y < N || (resid && ld_r < N)) return glt::fail(GLT_EINVAL, "w4: output or residual row stride below N %d", N);
+  if (!glt::aligned16(packed)) return glt::fail(GLT_EINVAL, "w4: packed weights must be 16-byte aligned");
+  if (M == 0) return GLT_OK;
+  const W4Layout L(N, K, group, asym);
+  for (int m0 = 0; m0 < M; m0 += 8 * 65535) {   // grid.y limit
+    const int rows = M - m0 < 8 * 65535 ? M - m0 : 8 * 65535;
+    glt::w4_linear_kernel<<<dim3((L.tiles + 3) / 4, (rows + 7) / 8), 128, 0, static_cast<cudaStream_t>(stream)>>>(
+        static_cast<const uint8_t*>(packed), L, x + static_cast<int64_t>(m0) * ld_x, ld_x, rows,
+        static_cast<uint8_t*>(y) + static_cast<int64_t>(m0) * ld_y * (y_dtype ? 2 : 4), ld_y, y_dtype,
+        resid ? resid + static_cast<int64_t>(m0) * ld_r : nullptr, ld_r);
+    GLT_LAUNCH_CHECK();
+  }
+  return GLT_OK;
+}

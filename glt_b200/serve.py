@@ -1,0 +1,273 @@
+"""Decoding and scoring with a (baked) model, over the C ABI.
+
+``Kv8Cache`` / ``Kv8Batch``: a key/value cache in 8 bits with one scale for each block of
+tokens and head, and the attention that reads it; ``W4Weight``: products with 4-bit weights
+and group scales; ``token_logprobs`` / ``token_logprobs_bwd``: log probabilities of given
+tokens, entropy, the most likely tokens, and the gradient.  Every call runs on the current
+stream of its tensors' device, allocates its outputs with torch and does not synchronise.
+``include/glt_graft.h`` states the formulas, ranges and errors.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple
+
+import torch
+
+from ._lib import GltKv8Batch as _CBatch, GltKv8Cache as _CCache, check, lib
+
+FORMATS = {"int8": 0, "e4m3": 1}
+
+
+def _stream(t: torch.Tensor) -> int:
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _need(ok: bool, msg: str) -> None:
+    if not ok:
+        raise ValueError(msg)
+
+
+def _int32(t: torch.Tensor, name: str) -> torch.Tensor:
+    _need(t.is_cuda and t.dtype == torch.int32 and t.is_contiguous(), f"{name} must be a contiguous int32 CUDA tensor")
+    return t
+
+
+def _rows(t: torch.Tensor, heads: int, hd: int, name: str) -> int:
+    """Row stride of a bf16 [rows, heads, hd] tensor whose rows are dense."""
+    _need(t.is_cuda and t.dtype == torch.bfloat16 and tuple(t.shape[1:]) == (heads, hd),
+          f"{name} must be a bf16 CUDA tensor [rows, {heads}, {hd}], got {t.dtype} {tuple(t.shape)}")
+    _need(t.stride(2) == 1 and t.stride(1) == hd or t.numel() == 0, f"{name}: a row's heads must be contiguous")
+    return t.stride(0) if t.shape[0] > 1 else heads * hd
+
+
+class Kv8Batch:
+    """One step of a batch of sequences, shared by all layers (GltKv8Batch).
+
+    block_table int32 [num_seqs, max_blocks]; lengths int32 [num_seqs], the tokens held
+    before this step; rows, the step's new rows in all; row_start int32 [num_seqs + 1] when the
+    sequences bring different numbers of rows; max_new, the most any of them brings."""
+
+    def __init__(self, block_table: torch.Tensor, lengths: torch.Tensor, rows: int,
+                 row_start: torch.Tensor | None = None, max_new: int | None = None):
+        _need(block_table.dim() == 2 and lengths.shape == block_table.shape[:1],
+              "block_table [num_seqs, max_blocks] and lengths [num_seqs]")
+        n = block_table.shape[0]
+        _need(row_start is None or row_start.shape == (n + 1,), "row_start [num_seqs + 1]")
+        if max_new is None:
+            max_new = rows if row_start is not None else rows // max(n, 1)
+        self.block_table, self.lengths = _int32(block_table, "block_table"), _int32(lengths, "lengths")
+        self.row_start = None if row_start is None else _int32(row_start, "row_start")
+        self.num_seqs, self.max_blocks, self.rows = n, block_table.shape[1], rows
+        self._c = _CBatch(n, self.max_blocks, rows, max_new, block_table.data_ptr(), lengths.data_ptr(),
+                          None if row_start is None else row_start.data_ptr())
+        self._p = C.byref(self._c)
+
+
+class Kv8Cache:
+    """One layer's key/value cache in 8 bits (GltKv8Cache)."""
+
+    def __init__(self, num_blocks: int, block_tokens: int, num_kv_heads: int, head_dim: int, fmt: str = "int8",
+                 device="cuda"):
+        shape = (num_blocks, num_kv_heads, block_tokens, head_dim)
+        self._bind(torch.empty(shape, dtype=torch.uint8, device=device),
+                   torch.empty(shape, dtype=torch.uint8, device=device),
+                   torch.empty(shape[:2], device=device), torch.empty(shape[:2], device=device), fmt)
+
+    @classmethod
+    def from_buffers(cls, k, v, k_scale, v_scale, fmt: str = "int8") -> "Kv8Cache":
+        """A cache over the caller's buffers: codes uint8 [num_blocks, num_kv_heads, block_tokens,
+        head_dim], scales fp32 [num_blocks, num_kv_heads]."""
+        self = cls.__new__(cls)
+        self._bind(k, v, k_scale, v_scale, fmt)
+        return self
+
+    def _bind(self, k, v, k_scale, v_scale, fmt):
+        _need(fmt in FORMATS, f"format {fmt!r} (one of {sorted(FORMATS)})")
+        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype == torch.uint8,
+              "codes must be uint8 [num_blocks, num_kv_heads, block_tokens, head_dim]")
+        _need(k_scale.shape == v_scale.shape == k.shape[:2] and k_scale.dtype == v_scale.dtype == torch.float32,
+              "scales must be fp32 [num_blocks, num_kv_heads]")
+        _need(all(t.is_cuda and t.is_contiguous() for t in (k, v, k_scale, v_scale)),
+              "cache buffers must be contiguous CUDA tensors")
+        self.k, self.v, self.k_scale, self.v_scale, self.fmt = k, v, k_scale, v_scale, fmt
+        self.num_blocks, self.num_kv_heads, self.block_tokens, self.head_dim = k.shape
+        self._c = _CCache(FORMATS[fmt], self.block_tokens, self.num_kv_heads, self.head_dim, self.num_blocks,
+                          k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        self._p = C.byref(self._c)
+
+    def append(self, batch: Kv8Batch, k: torch.Tensor, v: torch.Tensor) -> None:
+        """Write the step's keys and values, bf16 [rows, num_kv_heads, head_dim] (views into packed rows are fine)."""
+        _need(k.shape[0] == v.shape[0] == batch.rows, f"k and v must have {batch.rows} rows")
+        ld_k = _rows(k, self.num_kv_heads, self.head_dim, "k")
+        ld_v = _rows(v, self.num_kv_heads, self.head_dim, "v")
+        check(lib.glt_kv8_append(self._p, batch._p, k.data_ptr(), ld_k, v.data_ptr(), ld_v, _stream(k)))
+
+    def attention(self, batch: Kv8Batch, q: torch.Tensor, scale: float = 0.0, window: int = 0,
+                  token_mask: torch.Tensor | None = None, out: torch.Tensor | None = None):
+        """Attention of the step's queries, bf16 [rows, num_heads, head_dim], after ``append``.
+        Returns (o like q, dense; lse fp32 [rows, num_heads])."""
+        _need(q.dim() == 3 and q.shape[0] == batch.rows, f"q must be [{batch.rows}, num_heads, head_dim]")
+        nh = q.shape[1]
+        ld_q = _rows(q, nh, self.head_dim, "q")
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _need(out.shape == q.shape, "out must have q's shape")
+        ld_o = _rows(out, nh, self.head_dim, "out")
+        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        ld_m = 0
+        if token_mask is not None:
+            _need(token_mask.is_cuda and token_mask.dtype in (torch.uint8, torch.bool) and token_mask.dim() == 2
+                  and token_mask.shape[0] == batch.num_seqs and token_mask.stride(1) == 1
+                  and token_mask.shape[1] >= batch.max_blocks * self.block_tokens,
+                  "token_mask must be bytes [num_seqs, at least max_blocks * block_tokens]")
+            ld_m = token_mask.stride(0) if token_mask.shape[0] > 1 else token_mask.shape[1]
+        need = C.c_int64()
+        check(lib.glt_kv8_attention_workspace(self._p, batch._p, nh, C.byref(need)))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
+        check(lib.glt_kv8_attention(self._p, batch._p, q.data_ptr(), ld_q, out.data_ptr(), ld_o, lse.data_ptr(), nh,
+                                    scale, window, None if token_mask is None else token_mask.data_ptr(), ld_m,
+                                    ws.data_ptr(), need.value, _stream(q)))
+        return out, lse
+
+    def read(self, batch: Kv8Batch, start: torch.Tensor | None, count: int):
+        """Cached values of positions [start[b], start[b] + count): two fp32 tensors
+        [num_seqs, count, num_kv_heads, head_dim]."""
+        if start is not None:
+            _need(_int32(start, "start").shape == (batch.num_seqs,), "start [num_seqs]")
+        shape = (batch.num_seqs, count, self.num_kv_heads, self.head_dim)
+        k, v = (torch.empty(shape, device=self.k.device) for _ in range(2))
+        check(lib.glt_kv8_read(self._p, batch._p, None if start is None else start.data_ptr(), count, k.data_ptr(),
+                               v.data_ptr(), _stream(self.k)))
+        return k, v
+
+
+class W4Weight:
+    """A weight matrix [N, K] in 4 bits with group scales, packed for ``linear``."""
+
+    def __init__(self, packed: torch.Tensor, N: int, K: int, group: int, asym: bool):
+        self.packed, self.N, self.K, self.group, self.asym = packed, N, K, group, bool(asym)
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None) -> "W4Weight":
+        """codes uint8 [N, K] (0..15), scales bf16 [N, K / group], zeros uint8 like the scales or None (8)."""
+        N, K = codes.shape
+        _need(scales.dim() == 2 and scales.shape[0] == N and scales.shape[1] > 0 and K % scales.shape[1] == 0,
+              "scales must be [N, K / group]")
+        group = K // scales.shape[1]
+        _need(codes.dtype == torch.uint8 and scales.dtype == torch.bfloat16, "codes uint8, scales bf16")
+        _need(zeros is None or (zeros.dtype == torch.uint8 and zeros.shape == scales.shape), "zeros uint8 like scales")
+        codes, scales = codes.contiguous(), scales.contiguous()
+        zeros = None if zeros is None else zeros.contiguous()
+        need = C.c_int64()
+        check(lib.glt_w4_packed_bytes(N, K, group, int(zeros is not None), C.byref(need)))
+        packed = torch.empty(need.value, dtype=torch.uint8, device=codes.device)
+        check(lib.glt_w4_pack(codes.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), N, K,
+                              group, packed.data_ptr(), _stream(codes)))
+        return cls(packed, N, K, group, zeros is not None)
+
+    @classmethod
+    def quantize(cls, w: torch.Tensor, group: int = 128, asym: bool = False) -> "W4Weight":
+        """Round a bf16 [N, K] matrix to 4 bits."""
+        return cls.from_codes(*quantize_w4(w, group, asym))
+
+    def unpack(self) -> torch.Tensor:
+        """The weights the codes stand for, bf16 [N, K]."""
+        w = torch.empty(self.N, self.K, dtype=torch.bfloat16, device=self.packed.device)
+        check(lib.glt_w4_unpack(self.packed.data_ptr(), self.N, self.K, self.group, int(self.asym), w.data_ptr(),
+                                self.K, _stream(self.packed)))
+        return w
+
+    def linear(self, x: torch.Tensor, resid: torch.Tensor | None = None,
+               out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
+        """x . W^T (+ resid): x bf16 [M, K], result [M, N] in bf16 or fp32."""
+        M = x.shape[0]
+        _need(x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and x.shape[1] == self.K and x.stride(1) == 1,
+              f"x must be a bf16 CUDA tensor [M, {self.K}] with dense rows")
+        if out is None:
+            _need(out_dtype in (torch.bfloat16, torch.float32), "out_dtype must be bfloat16 or float32")
+            out = torch.empty(M, self.N, dtype=out_dtype, device=x.device)
+        _need(out.shape == (M, self.N) and out.dtype in (torch.bfloat16, torch.float32) and out.stride(1) == 1,
+              f"out must be [{M}, {self.N}] with dense rows")
+        if resid is not None:
+            _need(resid.is_cuda and resid.dtype == torch.bfloat16 and resid.shape == (M, self.N) and
+                  resid.stride(1) == 1, f"resid must be a bf16 CUDA tensor [{M}, {self.N}] with dense rows")
+        check(lib.glt_w4_linear(self.packed.data_ptr(), self.N, self.K, self.group, int(self.asym), x.data_ptr(),
+                                x.stride(0) if M > 1 else self.K, M, out.data_ptr(),
+                                out.stride(0) if M > 1 else self.N, int(out.dtype == torch.bfloat16),
+                                None if resid is None else resid.data_ptr(),
+                                0 if resid is None else resid.stride(0) if M > 1 else self.N, _stream(x)))
+        return out
+
+
+def quantize_w4(w: torch.Tensor, group: int = 128, asym: bool = False):
+    """(codes uint8 [N, K], scales bf16 [N, K / group], zeros uint8 or None) of a bf16 matrix."""
+    _need(w.is_cuda and w.dtype == torch.bfloat16 and w.dim() == 2 and w.stride(1) == 1, "w must be a bf16 CUDA matrix")
+    N, K = w.shape
+    codes = torch.empty(N, K, dtype=torch.uint8, device=w.device)
+    scales = torch.empty(N, K // group, dtype=torch.bfloat16, device=w.device)
+    zeros = torch.empty(N, K // group, dtype=torch.uint8, device=w.device) if asym else None
+    check(lib.glt_w4_quantize(w.data_ptr(), w.stride(0) if N > 1 else K, N, K, group, int(asym), codes.data_ptr(),
+                              scales.data_ptr(), None if zeros is None else zeros.data_ptr(), _stream(w)))
+    return codes, scales, zeros
+
+
+class TokenLogprobs(NamedTuple):
+    logp: torch.Tensor | None      # fp32 [rows], None without targets
+    entropy: torch.Tensor          # fp32 [rows]
+    lse: torch.Tensor              # fp32 [rows]
+    top_ids: torch.Tensor | None   # int32 [rows, top], None with top = 0
+    top_logp: torch.Tensor | None  # fp32 [rows, top]
+    scale: float
+
+
+def _logits(x: torch.Tensor) -> tuple[int, int]:
+    _need(x.is_cuda and x.dim() == 2 and x.dtype in (torch.bfloat16, torch.float32) and
+          (x.stride(1) == 1 or x.shape[1] == 1), "logits must be a bf16 or fp32 CUDA tensor [rows, V] with dense rows")
+    return int(x.dtype == torch.bfloat16), x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, scale: float = 1.0,
+                   top: int = 0) -> TokenLogprobs:
+    """Log probabilities of ``targets`` (int32 [rows], negative: none) under softmax(scale * logits),
+    the entropy, and the ``top`` most likely tokens."""
+    dt, ld = _logits(logits)
+    R, V = logits.shape
+    dev = logits.device
+    if targets is not None:
+        _need(_int32(targets, "targets").shape == (R,), "targets [rows]")
+    stats = torch.empty(3, R, device=dev)
+    ids = torch.empty(R, top, dtype=torch.int32, device=dev) if top else None
+    vals = torch.empty(R, top, device=dev) if top else None
+    logp = stats[0] if targets is not None else None
+    check(lib.glt_token_logprobs(logits.data_ptr(), dt, ld, R, V, None if targets is None else targets.data_ptr(),
+                                 scale, top, None if targets is None else logp.data_ptr(), stats[1].data_ptr(),
+                                 stats[2].data_ptr(), ids.data_ptr() if top else None,
+                                 vals.data_ptr() if top else None, _stream(logits)))
+    return TokenLogprobs(logp, stats[1], stats[2], ids, vals, scale)
+
+
+def token_logprobs_bwd(logits: torch.Tensor, targets: torch.Tensor | None, fwd: TokenLogprobs,
+                       d_logp: torch.Tensor | None = None, d_entropy: torch.Tensor | None = None,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of the logits from those of ``fwd.logp`` and ``fwd.entropy`` (fp32 [rows], None = 0);
+    ``out`` may be the logits themselves."""
+    dt, ld = _logits(logits)
+    R, V = logits.shape
+    if targets is not None:
+        _need(_int32(targets, "targets").shape == (R,), "targets [rows]")
+    for t, name in ((d_logp, "d_logp"), (d_entropy, "d_entropy")):
+        _need(t is None or (t.is_cuda and t.dtype == torch.float32 and t.shape == (R,) and t.is_contiguous()),
+              f"{name} must be a contiguous fp32 CUDA tensor [{R}]")
+    if out is None:
+        out = torch.empty(R, V, dtype=logits.dtype, device=logits.device)
+    _need(out.shape == logits.shape and out.dtype == logits.dtype, "out must have the logits' shape and dtype")
+    ld_o = _logits(out)[1]
+
+    def ptr(t):
+        return None if t is None else t.data_ptr()
+
+    check(lib.glt_token_logprobs_bwd(logits.data_ptr(), dt, ld, R, V, ptr(targets), fwd.scale, fwd.lse.data_ptr(),
+                                     fwd.entropy.data_ptr(), ptr(d_logp), ptr(d_entropy), out.data_ptr(), ld_o,
+                                     _stream(logits)))
+    return out

@@ -241,6 +241,130 @@ GLT_API int glt_rmsnorm_bwd(const float* dy, const uint16_t* x, const uint16_t* 
                             float eps, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Decoding with the baked model.  The reference stops at whole-sequence    */
+/* forwards (grafting.hip:224-271, 446-713); these operators carry a baked   */
+/* model through single-token steps: a key/value cache in 8 bits, products   */
+/* with 4-bit weights, and probabilities of tokens with their gradient.      */
+/* All calls are stream-ordered, allocate nothing and do not synchronise.    */
+/* ------------------------------------------------------------------------ */
+
+/* Key/value cache in 8 bits, one layer.  Token t of sequence b lies in block
+ * table[b][t / block_tokens] at row t % block_tokens.  The value of a code is
+ * scale * (code - 128) (GLT_KV8_INT8, codes 1..255) or scale * e4m3(code)
+ * (GLT_KV8_E4M3), with one fp32 scale for each block and KV head.
+ * block_tokens: 16, 32, 64 or 128; head_dim: 64 or 128; pools 16-byte
+ * aligned.  The buffers are the caller's and need no initial contents. */
+#define GLT_KV8_INT8 0
+#define GLT_KV8_E4M3 1
+typedef struct GltKv8Cache {
+  int format, block_tokens, num_kv_heads, head_dim;
+  int64_t num_blocks;
+  uint8_t* k;      /* dev [num_blocks, num_kv_heads, block_tokens, head_dim] */
+  uint8_t* v;
+  float* k_scale;  /* dev [num_blocks, num_kv_heads] */
+  float* v_scale;
+} GltKv8Cache;
+
+/* One step of a batch of sequences, shared by all layers.  Sequence b holds
+ * lengths[b] tokens from earlier steps and brings rows [row_start[b],
+ * row_start[b+1]) of this step's packed rows (row_start = NULL: rows /
+ * num_seqs rows each); its new token i is at position lengths[b] + i.  The
+ * calls leave `lengths` as it is: the caller advances it once all layers are
+ * done.  max_new bounds the new rows of any sequence.  A sequence whose
+ * lengths, rows or table do not fit (negative, beyond rows, max_new or
+ * max_blocks * block_tokens) is left out, and a block id outside the pool is
+ * skipped; both set code 2 of the device error word (glt_device_error). */
+typedef struct GltKv8Batch {
+  int num_seqs, max_blocks, rows, max_new;
+  const int32_t* block_table; /* dev [num_seqs, max_blocks] */
+  const int32_t* lengths;     /* dev [num_seqs] */
+  const int32_t* row_start;   /* dev [num_seqs + 1] or NULL */
+} GltKv8Batch;
+
+/* Writes this step's keys and values (bf16 rows of num_kv_heads * head_dim,
+ * row strides ld_k / ld_v elements, multiples of 8, 16-byte aligned) into the
+ * cache.  A block's scale is the largest finite magnitude its tokens of this
+ * and earlier steps had, over 127 (int8) or 448 (e4m3); a code is the nearest
+ * to x / scale, ties to even.  When a new token raises the scale of a block that
+ * already holds tokens, their codes are rounded once more to the new scale.
+ * Infinities saturate, NaN is stored as 0. */
+GLT_API int glt_kv8_append(const GltKv8Cache* cache, const GltKv8Batch* batch, const uint16_t* k,
+                           int64_t ld_k, const uint16_t* v, int64_t ld_v, void* stream);
+/* Attention of this step's queries over the cache, after glt_kv8_append.
+ * q, o: bf16 rows of num_heads * head_dim (row strides ld_q, ld_o, multiples of
+ * 8, 16-byte aligned); query head h reads KV head h / (num_heads / num_kv_heads).
+ * The query at position p sees tokens t <= p with, if window > 0, t > p - window
+ * and, if token_mask is given (dev bytes, row b at b * ld_mask, one byte a
+ * position), a nonzero byte.  scale = 0 means 1/sqrt(head_dim).  lse (NULL or
+ * [rows, num_heads] fp32): natural log-sum-exp of the scaled scores.  A query
+ * that sees no token gets o = 0, lse = -inf.  workspace: at least
+ * glt_kv8_attention_workspace bytes, 16-byte aligned, used by one call at a
+ * time; its contents do not matter. */
+GLT_API int glt_kv8_attention_workspace(const GltKv8Cache* cache, const GltKv8Batch* batch,
+                                        int num_heads, int64_t* bytes);
+GLT_API int glt_kv8_attention(const GltKv8Cache* cache, const GltKv8Batch* batch, const uint16_t* q,
+                              int64_t ld_q, uint16_t* o, int64_t ld_o, float* lse, int num_heads,
+                              float scale, int window, const uint8_t* token_mask, int64_t ld_mask,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+/* The cached values of positions [start[b], start[b] + count) of each sequence
+ * as fp32 [num_seqs, count, num_kv_heads, head_dim] (start = NULL: from 0);
+ * positions the sequence does not hold after this step read as 0. */
+GLT_API int glt_kv8_read(const GltKv8Cache* cache, const GltKv8Batch* batch, const int32_t* start,
+                         int count, float* k, float* v, void* stream);
+
+/* 4-bit weights W [N, K] in groups of `group` (32, 64 or 128, dividing K)
+ * columns: w = scale * (code - zero), code 0..15, scale bf16, zero 8 (asym = 0)
+ * or a stored 0..15 (asym = 1).
+ * glt_w4_quantize: codes (one byte each, [N, K]), scales [N, K/group] bf16 and,
+ *   with asym, zeros [N, K/group] bytes of bf16 weights (row stride ld_w).
+ *   asym = 0: scale = bf16(max|w| / 7); asym = 1: scale = bf16((max - min) / 15)
+ *   over the group with 0 included, zero = nearest to -min / scale.  Codes are
+ *   the nearest, ties to even.  Infinities saturate, NaN counts as 0.
+ * glt_w4_pack: the above (or a checkpoint's own codes) into the layout the
+ *   products read, glt_w4_packed_bytes bytes, 16-byte aligned.  zeros = NULL: asym = 0.
+ * glt_w4_unpack: the bf16 (nearest) weights of a packed matrix.
+ * glt_w4_linear: y[M, N] = x[M, K] . W^T (+ resid): x bf16 with row stride ld_x
+ *   (a multiple of 8, 16-byte aligned), y bf16 (y_dtype 1) or fp32 (0), resid bf16
+ *   or NULL; accumulation in fp32.  Made for the few rows of decoding: every 32
+ *   rows read the weights once more. */
+GLT_API int glt_w4_packed_bytes(int N, int K, int group, int asym, int64_t* bytes);
+GLT_API int glt_w4_quantize(const uint16_t* w, int64_t ld_w, int N, int K, int group, int asym,
+                            uint8_t* codes, uint16_t* scales, uint8_t* zeros, void* stream);
+GLT_API int glt_w4_pack(const uint8_t* codes, const uint16_t* scales, const uint8_t* zeros, int N,
+                        int K, int group, void* packed, void* stream);
+GLT_API int glt_w4_unpack(const void* packed, int N, int K, int group, int asym, uint16_t* w,
+                          int64_t ld_w, void* stream);
+GLT_API int glt_w4_linear(const void* packed, int N, int K, int group, int asym, const uint16_t* x,
+                          int64_t ld_x, int M, void* y, int64_t ld_y, int y_dtype,
+                          const uint16_t* resid, int64_t ld_r, void* stream);
+
+/* Log probabilities of given tokens, entropy and the most likely tokens, from
+ * logits [rows, V] (dtype 0 fp32, 1 bf16; row stride ld), z = scale * logit with
+ * scale > 0 (one over the temperature):
+ *   lse[r] = log sum_v exp z_v, logp[r] = z_target - lse (0 for a negative target),
+ *   entropy[r] = -sum_v p_v log p_v (nats), top_ids / top_logp [rows, top]: the `top`
+ *   (0..32, <= V) largest logits in falling order, equal ones by rising index.
+ * targets (int32) and logp are both given or both NULL; entropy may be NULL;
+ * statistics are fp32.  A logit of -inf has probability 0; a row of nothing else gives
+ * lse = logp = -inf and entropy 0.  A row that holds NaN or +inf gives NaN (its top_ids
+ * rank NaN below all numbers).  A target >= V counts as negative and sets code 2 of the
+ * device error word.
+ * glt_token_logprobs_bwd: dlogits (the logits' dtype, row stride ld_d; may be the logits
+ * themselves) from d_logp and d_entropy [rows] (either may be NULL = 0) and the forward's lse and
+ * entropy: scale * (d_logp * ([v = target] - p) - d_entropy * p * (log p + entropy)).
+ * The gradient of a row of -inf is 0.  The reference's loss is the mean cross entropy
+ * of domain tokens alone (grafting.hip:1027-1135). */
+GLT_API int glt_token_logprobs(const void* logits, int dtype, int64_t ld, int rows, int V,
+                               const int32_t* targets, float scale, int top, float* logp,
+                               float* entropy, float* lse, int32_t* top_ids, float* top_logp,
+                               void* stream);
+GLT_API int glt_token_logprobs_bwd(const void* logits, int dtype, int64_t ld, int rows, int V,
+                                   const int32_t* targets, float scale, const float* lse,
+                                   const float* entropy, const float* d_logp,
+                                   const float* d_entropy, void* dlogits, int64_t ld_d,
+                                   void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Configuration                                                            */
 /* Mirrors GraftConfig (src/config.hpp:40-91) plus the CLI-level values of  */
 /* grafting.hip:274-292.  layout selects the graft geometry:                */
