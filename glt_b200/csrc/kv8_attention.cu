@@ -1,4 +1,33 @@
 // Attention of a step's queries over the 8-bit key/value cache (glt_kv8_attention).
+//
+//   o_i = sum_t p_it v_t / sum_t p_it,   p_it = exp(scale q_i.k_t - m_i),   m_i a running maximum
+//
+// A few queries meet a long cache, so the cache's bytes bound the kernel: each is
+// read once for all query heads that share its KV head.
+//
+// Work.  A unit is one KV head of one sequence with up to 8 NT of its query rows
+// (query token x head of the group); its tokens are cut into steps of 32.  The
+// steps of all units, laid end to end, are dealt to the CTAs in equal runs, so a
+// batch of any lengths loads all SMs alike; the four warps of a CTA take the steps
+// of its run in turn, each with its own maximum and sum, and join at the end of a
+// unit.  A unit that crosses CTAs leaves partial results, which a second kernel
+// joins.  All sizes are read on the device: a captured graph follows the lengths.
+//
+// Tensor cores.  Both products have the cache as operand A (16 tokens, or 16
+// channels, by 16) and the few queries as operand B (N = 8), in f16 with 32-bit sums:
+//   S^T = K . Q^T:  8-bit codes become f16 exactly; a query row is brought to f16 by a
+//                   power of two (its bf16 mantissa fits), the block's scale multiplies S.
+//   O^T = V^T . P^T: P is rounded to f16 (11 bits), V's codes are exact, the block's scale
+//                   multiplies the 32-bit sums of a step.  P is taken from the step's own
+//                   maximum times 2^15; a weight still below f16's normal range (2^-29 of
+//                   that maximum) is added in 32 bits on the side, so each weight keeps its
+//                   11 bits, whatever the values it meets.
+// The order of a contraction's index is free, so a lane loads 16 contiguous bytes and
+// uses them for four k-steps of S or eight rows of O.
+//
+// Loads.  Every lane copies the bytes that it will use itself into its own slots of a
+// ring in shared memory (cp.async, 16 bytes), so the ring needs no barrier, and the
+// copies run ahead of the arithmetic across units.
 #include <float.h>
 
 #include "kv8.cuh"
@@ -6,78 +35,723 @@
 namespace glt {
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kStep = 32;   // tokens of a step
+constexpr float kF16Min = 6.103515625e-05f;   // 2^-14, the smallest normal f16
 
-__device__ __forceinline__ float block_max(float v, float* red) {
-  v = warp_max(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-}
-__device__ __forceinline__ float block_add(float v, float* red) {
-  v = warp_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  return red[0] + red[1] + red[2] + red[3];
+__host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+
+struct AttnArgs {
+  GltKv8Cache c;
+  GltKv8Batch b;
+  const uint16_t* q;
+  int64_t ld_q;
+  uint16_t* o;
+  int64_t ld_o;
+  float* lse;
+  int nh, group;
+  float scale;
+  int window;
+  const uint8_t* mask;
+  int64_t ld_mask;
+  float* part;   // [CTA][2] partial results: rows x hd sums, then rows maxima (base 2), rows sums
+  unsigned int* err;
+};
+
+// What one sequence has to do: `steps` steps from token `lo` on, for `units` units.
+struct SeqWork {
+  int past, n, row0, lo, steps, units;
+};
+template <int ROWS>
+__device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int seq, unsigned int* err) {
+  const Kv8Span s = kv8_span(a.b, seq, a.c.block_tokens, err);
+  SeqWork w;
+  w.past = s.past;
+  w.n = s.n;
+  w.row0 = s.row0;
+  w.lo = a.window > 0 ? max(0, s.past - a.window + 1) & ~(kStep - 1) : 0;
+  w.steps = (s.past + s.n - w.lo + kStep - 1) / kStep;
+  w.units = s.n > 0 ? a.c.num_kv_heads * static_cast<int>((static_cast<int64_t>(s.n) * a.group + ROWS - 1) / ROWS) : 0;
+  return w;
 }
 
-// One CTA a (query, head): 128 tokens at a time with a running maximum and sum.
-__global__ void __launch_bounds__(kThreads) kv8_attention_kernel(GltKv8Cache c, GltKv8Batch b,
-                                                                 const uint16_t* __restrict__ q, int64_t ld_q,
-                                                                 uint16_t* __restrict__ o, int64_t ld_o,
-                                                                 float* __restrict__ lse, int nh, float scale,
-                                                                 int window, const uint8_t* __restrict__ mask,
-                                                                 int64_t ld_mask, unsigned int* err) {
-  __shared__ float sq[128], sp[kThreads], red[4];
-  const int seq = blockIdx.y, head = blockIdx.z, kvh = head / (nh / c.num_kv_heads);
-  const bool first = blockIdx.x == 0 && head == 0 && threadIdx.x == 0;
-  const Kv8Span span = kv8_span(b, seq, c.block_tokens, first ? err : nullptr);
-  for (int i = blockIdx.x; i < span.n; i += gridDim.x) {
-    const int64_t row = span.row0 + i;
-    const int pos = span.past + i;
-    __syncthreads();
-    if (threadIdx.x < c.head_dim) sq[threadIdx.x] = bf16_bits_to_f32(q[row * ld_q + head * c.head_dim + threadIdx.x]);
-    __syncthreads();
-    const int t0 = window > 0 ? max(0, pos - window + 1) : 0;
-    float m = -INFINITY, l = 0.f, acc = 0.f;
-    for (int base = t0; base <= pos; base += kThreads) {
-      const int t = base + threadIdx.x;
-      float s = -INFINITY;
-      if (t <= pos && (!mask || mask[seq * ld_mask + t])) {
-        const int64_t id = kv8_block(c, b, seq, t / c.block_tokens, err);
-        if (id >= 0) {
-          const int64_t hb = id * c.num_kv_heads + kvh;
-          const uint8_t* kr = c.k + (hb * c.block_tokens + t % c.block_tokens) * c.head_dim;
-          s = 0.f;
-          for (int d = 0; d < c.head_dim; ++d) s += sq[d] * kv8_decode(kr[d], c.format);
-          s *= c.k_scale[hb] * scale;
+// Finds the sequence that step x of the whole falls into (and the total).  All
+// threads of the CTA call it.
+struct Place {
+  int seq;
+  int64_t base, total;   // first step of the sequence; steps of all sequences
+};
+struct ScanSmem {
+  int64_t warp[kWarps];
+  int64_t base;
+  int seq;
+};
+template <int ROWS, typename Pick>
+__device__ Place find_place(const AttnArgs& a, ScanSmem& sm, bool report, Pick pick) {
+  const int per = (a.b.num_seqs + kThreads - 1) / kThreads;
+  const int first = min(a.b.num_seqs, static_cast<int>(threadIdx.x) * per), last = min(a.b.num_seqs, first + per);
+  int64_t mine = 0;
+  for (int s = first; s < last; ++s) {
+    const SeqWork w = seq_work<ROWS>(a, s, report ? a.err : nullptr);
+    mine += static_cast<int64_t>(w.steps) * w.units;
+  }
+  int64_t scan = mine;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += v;
+  }
+  if (lane == 31) sm.warp[warp] = scan;
+  __syncthreads();
+  Place p;
+  p.total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) scan += sm.warp[w];
+    p.total += sm.warp[w];
+  }
+  const int64_t x = pick(p.total);
+  int64_t base = scan - mine;
+  if (x >= base && x < scan) {
+    for (int s = first; s < last; ++s) {
+      const SeqWork w = seq_work<ROWS>(a, s, nullptr);
+      const int64_t k = static_cast<int64_t>(w.steps) * w.units;
+      if (x < base + k) {
+        sm.seq = s;
+        sm.base = base;
+        break;
+      }
+      base += k;
+    }
+  }
+  __syncthreads();
+  p.seq = sm.seq;
+  p.base = sm.base;
+  return p;
+}
+
+// CTAs that share `total` steps: each has at least one for every warp.
+__device__ __forceinline__ int active_ctas(int64_t total, int grid) {
+  const int64_t n = (total + kWarps - 1) / kWarps;
+  return n < grid ? static_cast<int>(n) : grid;
+}
+__device__ __forceinline__ int64_t share_begin(int64_t total, int ctas, int i) {
+  return total / ctas * i + total % ctas * i / ctas;
+}
+
+// A run of steps, unit by unit.
+template <int ROWS>
+struct Cursor {
+  int seq, unit, s0, s1;
+  int64_t left;   // steps of the run from s0 on
+  SeqWork w;
+  __device__ __forceinline__ void start(const AttnArgs& a, int seq_, int64_t offset, int64_t count) {
+    seq = seq_;
+    left = count;
+    if (left <= 0) return;
+    w = seq_work<ROWS>(a, seq, nullptr);
+    unit = static_cast<int>(offset / w.steps);
+    s0 = static_cast<int>(offset - static_cast<int64_t>(unit) * w.steps);
+    s1 = static_cast<int>(min(static_cast<int64_t>(w.steps), s0 + left));
+  }
+  __device__ __forceinline__ void next(const AttnArgs& a) {
+    left -= s1 - s0;
+    if (left <= 0) return;
+    if (++unit == w.units) {
+      unit = 0;
+      do {
+        if (++seq >= a.b.num_seqs) {   // only if the lengths changed under the kernel
+          left = 0;
+          return;
+        }
+        w = seq_work<ROWS>(a, seq, nullptr);
+      } while (w.units == 0);
+    }
+    s0 = 0;
+    s1 = static_cast<int>(min(static_cast<int64_t>(w.steps), left));
+  }
+  __device__ __forceinline__ bool whole() const { return s0 == 0 && s1 == w.steps; }
+};
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+// Copies of B bytes (zeros where !on); the source address is not read then.
+template <int B>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool on) {
+  if constexpr (B == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(B), "r"(on ? B : 0) : "memory");
+}
+__device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_groups() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+// Bytes 0, 1 (HI = 0) or 2, 3 of a word of codes as two f16 numbers.  An int8 code u
+// in the low mantissa bits of 1024 is 1024 + u; 1152 less is u - 128.
+template <int FMT, int HI>
+__device__ __forceinline__ uint32_t two_codes(uint32_t w) {
+  if constexpr (FMT == GLT_KV8_INT8) {
+    uint32_t r;
+    const uint32_t x = __byte_perm(w, 0x64646464u, HI ? 0x4342 : 0x4140);
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x64806480u));
+    return r;
+  } else {
+    return e4m3x2_to_f16x2(HI ? w >> 16 : w & 0xFFFFu);
+  }
+}
+
+// Four channels of a query row from their sum z, the row's maximum (base 2) and sum of
+// weights.  A row that saw nothing has weight 0 and gives 0; NaN stays NaN.
+__device__ __forceinline__ void write_out(const AttnArgs& a, int row0, int64_t r, int kvh, int hd, int d, float4 z,
+                                          float top, float sum) {
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const int64_t tok = row0 + r / a.group;
+  const int head = kvh * a.group + static_cast<int>(r % a.group);
+  *reinterpret_cast<uint2*>(a.o + tok * a.ld_o + static_cast<int64_t>(head) * hd + d) =
+      make_uint2(pack_bf16x2_rn(z.x * inv, z.y * inv), pack_bf16x2_rn(z.z * inv, z.w * inv));
+  if (a.lse && d == 0) a.lse[tok * a.nh + head] = sum == 0.f ? -INFINITY : top * 0.6931471805599453f + logf(sum);
+}
+// 2^(m - top) for partial results: weights that saw nothing are 0 (or NaN) already.
+__device__ __forceinline__ float join_factor(float m, float top) { return top == -INFINITY ? 1.f : ex2_approx(m - top); }
+
+// Bytes a lane copies for a step: K rows g, g + 8 of each half of 16 tokens, 16 bytes at
+// 16 c (+ 64); V tokens 2c, 2c + 1, 2c + 8, 2c + 9 of each half, hd / 8 bytes at channel g hd / 8.
+template <int HD>
+struct Ring {
+  static constexpr int kStages = HD == 128 ? 2 : 3;
+  static constexpr int kKeys = HD / 16;                  // 16-byte copies of K a lane and step
+  static constexpr int kValueBytes = HD / 8;             // bytes of a copy of V
+  static constexpr int kStage = 32 * (kKeys * 16 + 8 * kValueBytes) + 32;   // + scales, validity
+  static constexpr int kWarp = kStages * kStage;
+};
+template <int HD, int NT>
+constexpr int smem_bytes() {
+  return kWarps * Ring<HD>::kWarp + 2 * 8 * NT * HD * 4 + kWarps * 8 * NT * 8 + static_cast<int>(sizeof(ScanSmem));
+}
+
+template <int HD, int FMT, int NT, bool BT16>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kernel(const __grid_constant__ AttnArgs a) {
+  constexpr int ROWS = 8 * NT, LU = BT16 ? 2 : 1;
+  using R = Ring<HD>;
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* join_o = reinterpret_cast<float*>(smem + kWarps * R::kWarp);            // [2][ROWS][HD]
+  float2* join_ml = reinterpret_cast<float2*>(join_o + 2 * ROWS * HD);           // [warp][ROWS]
+  ScanSmem& scan = *reinterpret_cast<ScanSmem*>(join_ml + kWarps * ROWS);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  int ctas = 0;
+  int64_t begin = 0, end = 0;
+  const Place at = find_place<ROWS>(a, scan, blockIdx.x == 0, [&](int64_t total) {
+    ctas = active_ctas(total, gridDim.x);
+    if (static_cast<int>(blockIdx.x) < ctas) {
+      begin = share_begin(total, ctas, blockIdx.x);
+      end = share_begin(total, ctas, blockIdx.x + 1);
+    }
+    return end > begin ? begin : int64_t{-1};
+  });
+  if (end <= begin) return;
+
+  uint8_t* ring = smem + warp * R::kWarp;
+  const uint32_t ring_k = smem_addr(ring) + lane * 16;
+  const uint32_t ring_v = smem_addr(ring) + 32 * R::kKeys * 16 + lane * R::kValueBytes;
+  constexpr int kScales = 32 * (R::kKeys * 16 + 8 * R::kValueBytes);
+
+  Cursor<ROWS> ld;
+  ld.start(a, at.seq, begin - at.base, end - begin);
+  int ld_step = ld.s0 + warp, ld_stage = 0;
+  // Copies this warp's next step of the run into the next stage (one group, maybe empty).
+  auto issue = [&]() {
+    while (ld.left > 0 && ld_step >= ld.s1) {
+      ld.next(a);
+      ld_step = ld.s0 + warp;
+    }
+    if (ld.left > 0) {
+      const int kvh = ld.unit % a.c.num_kv_heads;
+      const int t0 = ld.w.lo + ld_step * kStep, hi = ld.w.past + ld.w.n;
+      const uint32_t st = ld_stage * R::kStage;
+      int valid = 0;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int t = t0 + 16 * u;
+        int64_t id = -1;
+        if (t < hi) id = kv8_block(a.c, a.b, ld.seq, t / a.c.block_tokens, lane == 0 ? a.err : nullptr);
+        const bool on = id >= 0;
+        valid |= on ? 1 << u : 0;
+        const int64_t hb = on ? id * a.c.num_kv_heads + kvh : 0;
+        const int64_t row = hb * a.c.block_tokens + (t & (a.c.block_tokens - 1));
+        const uint8_t* kp = a.c.k + row * HD;
+        const uint8_t* vp = a.c.v + row * HD;
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int h = 0; h < HD / 64; ++h) {
+            const bool in = on && t + g + 8 * r < hi;
+            copy_async<16>(ring_k + st + ((u * 2 + r) * (HD / 64) + h) * 512,
+                           in ? kp + (g + 8 * r) * HD + h * 64 + c * 16 : a.c.k, in);
+          }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tk = 2 * c + (i & 1) + 8 * (i >> 1);
+          const bool in = on && t + tk < hi;
+          copy_async<R::kValueBytes>(ring_v + st + (u * 4 + i) * 32 * R::kValueBytes,
+                                     in ? vp + tk * HD + g * R::kValueBytes : a.c.v, in);
+        }
+        if (lane < 2) copy_async<4>(smem_addr(ring) + st + kScales + u * 8 + lane * 4, (lane ? a.c.v_scale : a.c.k_scale) + hb, on);
+      }
+      if (lane == 0) *reinterpret_cast<int*>(ring + st + kScales + 16) = valid;
+      ld_step += kWarps;
+    }
+    commit();
+    ld_stage = ld_stage + 1 == R::kStages ? 0 : ld_stage + 1;
+  };
+#pragma unroll 1
+  for (int i = 0; i < R::kStages; ++i) issue();
+
+  Cursor<ROWS> cu;
+  cu.start(a, at.seq, begin - at.base, end - begin);
+  int stage = 0;
+  bool first_segment = true;
+  while (cu.left > 0) {
+    const int kvh = cu.unit % a.c.num_kv_heads, tile = cu.unit / a.c.num_kv_heads;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(ROWS), static_cast<int64_t>(cu.w.n) * a.group - static_cast<int64_t>(tile) * ROWS));
+    // ---- queries: operand B, and the factor that takes S to log2 units
+    uint32_t qb[NT][HD / 16][2];
+    float qs[NT][2];
+    int pos[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int64_t r = static_cast<int64_t>(tile) * ROWS + nt * 8 + g;
+      const bool in = nt * 8 + g < rows;
+      const int64_t tok = r / a.group;
+      const uint16_t* src = a.q + (cu.w.row0 + tok) * a.ld_q + (kvh * a.group + (r - tok * a.group)) * HD;
+      uint4 v[HD / 64][2];
+      float peak = 0.f;
+#pragma unroll
+      for (int h = 0; h < HD / 64; ++h)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          v[h][j] = in ? *reinterpret_cast<const uint4*>(src + h * 64 + c * 16 + j * 8) : make_uint4(0, 0, 0, 0);
+          float f[8];
+          unpack8(v[h][j], f);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) peak = fmaxf(peak, fabsf(f[k]));
+        }
+      peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 1));
+      peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
+      // 2^e takes the largest magnitude to [2^13, 2^14): bf16's 8 bits stay exact in f16 down
+      // to 2^-27 of it, and smaller ones keep an absolute 2^-38 of it
+      int e = 0;
+      if (peak > 0.f && peak <= FLT_MAX) e = 13 - ilogbf(peak);
+      const int e1 = e / 2, e2 = e - e1;   // two factors: 2^e may be out of range
+      const float f1 = exp2f(static_cast<float>(e1)), f2 = exp2f(static_cast<float>(e2));
+#pragma unroll
+      for (int h = 0; h < HD / 64; ++h)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float f[8];
+          unpack8(v[h][j], f);
+#pragma unroll
+          for (int k = 0; k < 8; ++k) f[k] = f[k] * f1 * f2;
+          const int s = h * 4 + j * 2;
+          qb[nt][s][0] = pack_f16x2(f[0], f[1]);
+          qb[nt][s][1] = pack_f16x2(f[2], f[3]);
+          qb[nt][s + 1][0] = pack_f16x2(f[4], f[5]);
+          qb[nt][s + 1][1] = pack_f16x2(f[6], f[7]);
+        }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        // columns 2c, 2c + 1 of S^T: the rows that lanes 8c and 8c + 4 loaded
+        const int ec = __shfl_sync(0xffffffffu, e, 8 * c + 4 * j);
+        qs[nt][j] = a.scale * 1.4426950408889634f * exp2f(static_cast<float>(-(ec / 2))) * exp2f(static_cast<float>(-(ec - ec / 2)));
+        pos[nt][j] = cu.w.past + static_cast<int>((static_cast<int64_t>(tile) * ROWS + nt * 8 + 2 * c + j) / a.group);
+      }
+    }
+    const int pos_lo = cu.w.past + static_cast<int>(static_cast<int64_t>(tile) * ROWS / a.group);
+    const int pos_hi = cu.w.past + static_cast<int>((static_cast<int64_t>(tile) * ROWS + rows - 1) / a.group);
+    float acc[HD / 16][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt][0] = m[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+      for (int j = 0; j < HD / 16; ++j)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) acc[j][nt][k] = 0.f;
+    }
+    const uint8_t* mrow = a.mask ? a.mask + cu.seq * a.ld_mask : nullptr;
+    // the four tokens of a lane in a step: 16 u + 8 r + g
+    auto mask_bits = [&](int step) {
+      uint32_t bits = 0;
+      if (step < cu.s1) {
+        const int t = cu.w.lo + step * kStep + g;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (t + 8 * i <= pos_hi && mrow[t + 8 * i]) bits |= 1u << i;
+      }
+      return bits;
+    };
+    uint32_t seen = mrow ? mask_bits(cu.s0 + warp) : 0;
+
+    for (int step = cu.s0 + warp; step < cu.s1; step += kWarps) {
+      const uint32_t seen_now = seen;
+      if (mrow) seen = mask_bits(step + kWarps);
+      wait_groups<R::kStages - 1>();
+      __syncwarp();   // the scales come from other lanes' copies
+      const uint8_t* sg = ring + stage * R::kStage;
+      const float4 sc = *reinterpret_cast<const float4*>(sg + kScales);   // ks, vs of half 0; of half 1
+      const int valid = *reinterpret_cast<const int*>(sg + kScales + 16);
+      const int t0 = cu.w.lo + step * kStep;
+      // ---- S^T
+      float s[2][NT][4];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) s[u][nt][k] = 0.f;
+#pragma unroll
+        for (int h = 0; h < HD / 64; ++h) {
+          const uint4 r0 = *reinterpret_cast<const uint4*>(sg + ((u * 2 + 0) * (HD / 64) + h) * 512 + lane * 16);
+          const uint4 r1 = *reinterpret_cast<const uint4*>(sg + ((u * 2 + 1) * (HD / 64) + h) * 512 + lane * 16);
+          const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t fa[4] = {two_codes<FMT, 0>(w0[k]), two_codes<FMT, 0>(w1[k]), two_codes<FMT, 1>(w0[k]),
+                                    two_codes<FMT, 1>(w1[k])};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(s[u][nt], fa, qb[nt][h * 4 + k][0], qb[nt][h * 4 + k][1]);
+          }
         }
       }
-      const float mx = fmaxf(m, block_max(s, red));
-      if (mx == -INFINITY) continue;
-      const float corr = expf(m - mx), p = expf(s - mx);
-      m = mx;
-      l = l * corr + block_add(p, red);
-      acc *= corr;
-      __syncthreads();
-      sp[threadIdx.x] = p;
-      __syncthreads();
-      const int n = min(kThreads, pos + 1 - base);
-      if (threadIdx.x < c.head_dim)
-        for (int j = 0; j < n; ++j) {
-          if (sp[j] == 0.f) continue;
-          const int tj = base + j;
-          const int64_t id = kv8_block(c, b, seq, tj / c.block_tokens, nullptr);
-          const int64_t hb = id * c.num_kv_heads + kvh;
-          acc += sp[j] * (c.v_scale[hb] *
-                          kv8_decode(c.v[(hb * c.block_tokens + tj % c.block_tokens) * c.head_dim + threadIdx.x], c.format));
+      // ---- log2 units, masks
+      const bool edge = valid != 3 || mrow || t0 + kStep - 1 > pos_lo || (a.window > 0 && t0 <= pos_hi - a.window);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const float f0 = sc.x * qs[nt][j], f1 = sc.z * qs[nt][j];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[i >> 1][nt][(i & 1) * 2 + j] *= i < 2 ? f0 : f1;
         }
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int t = t0 + 8 * i + g;
+          const bool on = (valid >> (i >> 1) & 1) && (!mrow || (seen_now >> i & 1));
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              if (!(on && t <= pos[nt][j] && (a.window == 0 || t > pos[nt][j] - a.window)))
+                s[i >> 1][nt][(i & 1) * 2 + j] = -INFINITY;
+        }
+      }
+      // A fold unit is what shares a scale of V in this step: its halves with blocks of 16
+      // tokens, else the whole step.  Its weights are taken from its own maximum `peak`
+      // (2^15 at most, in f16's range), and join the running sums by a 32-bit factor.
+      bool moved = false;
+      float peak[LU][NT][2], ref[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float top = m[nt][j];
+#pragma unroll
+          for (int f = 0; f < LU; ++f) {
+            float x = fmaxf(s[f][nt][j], s[f][nt][2 + j]);
+            if (LU == 1) x = fmaxf(x, fmaxf(s[1][nt][j], s[1][nt][2 + j]));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            peak[f][nt][j] = x;
+            top = fmaxf(top, x);
+          }
+          moved |= top > m[nt][j];
+          ref[nt][j] = top;
+        }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float corr = ref[nt][j] == -INFINITY ? 1.f : ex2_approx(m[nt][j] - ref[nt][j]);
+            m[nt][j] = ref[nt][j];
+            l[nt][j] *= corr;
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k) {
+              acc[k][nt][j] *= corr;
+              acc[k][nt][2 + j] *= corr;
+            }
+          }
+      }
+      // ---- P^T as operand B.  Weights below f16's normal range go the 32-bit way below.
+      uint32_t pb[2][NT][2];
+      float fold[LU][NT][2];   // from a unit's sums to the running ones
+      bool small = false;
+#pragma unroll
+      for (int f = 0; f < LU; ++f)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float r = peak[f][nt][j] == -INFINITY ? 0.f : peak[f][nt][j] - 15.f;
+            const float w = peak[f][nt][j] == -INFINITY ? 0.f : ex2_approx(r - m[nt][j]);
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              if (LU == 2 && (i >> 1) != f) continue;
+              float& p = s[i >> 1][nt][(i & 1) * 2 + j];
+              p = ex2_approx(p - r);
+              sum += p;
+              small |= p < kF16Min && p > 0.f;
+            }
+            l[nt][j] = fmaf(sum, w, l[nt][j]);
+            fold[f][nt][j] = w * (f ? sc.w : sc.y);
+          }
+      if (__any_sync(0xffffffffu, small)) {
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {   // tokens 8 i + g of the step
+          const int u = i >> 1;
+          float p[NT][2];
+          bool mine = false;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float x = s[0][nt][j];
+              if (i == 1) x = s[0][nt][2 + j];
+              if (i == 2) x = s[1][nt][j];
+              if (i == 3) x = s[1][nt][2 + j];
+              if (!(x < kF16Min)) x = 0.f;
+              mine |= x > 0.f;
+              p[nt][j] = x * fold[LU == 2 ? u : 0][nt][j];
+            }
+          uint32_t lanes = __ballot_sync(0xffffffffu, mine);
+          while (lanes) {
+            const int tg = (__ffs(lanes) - 1) >> 2;
+            lanes &= ~(0xFu << (4 * tg));
+            const int slot = (u * 4 + (tg & 1) + 2 * (i & 1)) * 32 + g * 4 + (tg >> 1);
+            const uint8_t* vc = sg + 32 * R::kKeys * 16 + slot * R::kValueBytes;
+            float pt[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 2; ++j) pt[nt][j] = __shfl_sync(0xffffffffu, p[nt][j], tg * 4 + c);
+#pragma unroll
+            for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float v = kv8_decode(vc[2 * k + e], FMT);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                  for (int j = 0; j < 2; ++j) acc[k][nt][2 * e + j] = fmaf(pt[nt][j], v, acc[k][nt][2 * e + j]);
+              }
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              if (s[u][nt][k] < kF16Min) s[u][nt][k] = 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          pb[u][nt][0] = transpose_8x8(pack_f16x2(s[u][nt][0], s[u][nt][1]));
+          pb[u][nt][1] = transpose_8x8(pack_f16x2(s[u][nt][2], s[u][nt][3]));
+        }
+      // ---- O^T
+      const uint8_t* sv = sg + 32 * R::kKeys * 16 + lane * R::kValueBytes;
+#pragma unroll
+      for (int jw = 0; jw < HD / 32; ++jw) {   // one word (four channels) of every token: two row tiles
+        float part[LU][2][NT][4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            w[i] = *reinterpret_cast<const uint32_t*>(sv + (u * 4 + i) * 32 * R::kValueBytes + jw * 4);
+          constexpr int kLast = LU - 1;
+          const int f = u < kLast ? u : kLast;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t x = __byte_perm(w[0], w[1], half ? 0x7362 : 0x5140);
+            const uint32_t y = __byte_perm(w[2], w[3], half ? 0x7362 : 0x5140);
+            const uint32_t fa[4] = {two_codes<FMT, 0>(x), two_codes<FMT, 1>(x), two_codes<FMT, 0>(y), two_codes<FMT, 1>(y)};
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              if (LU == 2 || u == 0)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) part[f][half][nt][k] = 0.f;
+              mma_f16(part[f][half][nt], fa, pb[u][nt][0], pb[u][nt][1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+              for (int f = 0; f < LU; ++f) {
+                float& d = acc[jw * 2 + half][nt][k];
+                d = fmaf(part[f][half][nt][k], fold[f][nt][k & 1], d);
+              }
+      }
+      __syncwarp();   // all lanes are done with the stage's scales
+      stage = stage + 1 == R::kStages ? 0 : stage + 1;
+      issue();
     }
-    if (threadIdx.x < c.head_dim)
-      o[row * ld_o + head * c.head_dim + threadIdx.x] = bf16_bits_rn(m == -INFINITY ? 0.f : acc / l);
-    if (lse && threadIdx.x == 0) lse[row * nh + head] = m == -INFINITY ? -INFINITY : m + logf(l);
+
+    // ---- join the warps
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float x = l[nt][j];
+        x += __shfl_xor_sync(0xffffffffu, x, 4);
+        x += __shfl_xor_sync(0xffffffffu, x, 8);
+        x += __shfl_xor_sync(0xffffffffu, x, 16);
+        l[nt][j] = x;
+        if (g == 0) join_ml[warp * ROWS + nt * 8 + 2 * c + j] = make_float2(m[nt][j], x);
+      }
+    __syncthreads();
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, join_ml[w * ROWS + nt * 8 + 2 * c + j].x);
+        const float f = join_factor(m[nt][j], top);
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k) {
+          acc[k][nt][j] *= f;
+          acc[k][nt][2 + j] *= f;
+        }
+      }
+    // O^T tile k, row g (+8) is channel g hd / 8 + 2k (+1); column 2c + j is a query row
+    auto place = [&](int k, int nt, int j) { return (nt * 8 + 2 * c + j) * HD + g * (HD / 8) + 2 * k; };
+    if (warp >= 2) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            *reinterpret_cast<float2*>(join_o + (warp - 2) * ROWS * HD + place(k, nt, j)) =
+                make_float2(acc[k][nt][j], acc[k][nt][2 + j]);
+    }
+    __syncthreads();
+    if (warp < 2) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < HD / 16; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float2* d = reinterpret_cast<float2*>(join_o + warp * ROWS * HD + place(k, nt, j));
+            const float2 x = *d;
+            *d = make_float2(x.x + acc[k][nt][j], x.y + acc[k][nt][2 + j]);
+          }
+    }
+    __syncthreads();
+    const bool whole = cu.whole();
+    float* slot = a.part + (blockIdx.x * 2 + (first_segment ? 0 : 1)) * static_cast<int64_t>(ROWS * HD + 2 * ROWS);
+    for (int i = threadIdx.x; i < rows * (HD / 4); i += kThreads) {
+      const int r = i / (HD / 4), d = i % (HD / 4) * 4;
+      float top = -INFINITY, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, join_ml[w * ROWS + r].x);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) sum += join_ml[w * ROWS + r].y * join_factor(join_ml[w * ROWS + r].x, top);
+      const float4 x = *reinterpret_cast<const float4*>(join_o + r * HD + d);
+      const float4 y = *reinterpret_cast<const float4*>(join_o + (ROWS + r) * HD + d);
+      const float4 z = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+      if (whole) {
+        write_out(a, cu.w.row0, static_cast<int64_t>(tile) * ROWS + r, kvh, HD, d, z, top, sum);
+      } else {
+        *reinterpret_cast<float4*>(slot + r * HD + d) = z;
+        if (d == 0) {
+          slot[ROWS * HD + r] = top;
+          slot[ROWS * HD + ROWS + r] = sum;
+        }
+      }
+    }
+    __syncthreads();   // the join buffers are free again
+    first_segment = false;
+    cu.next(a);
+  }
+  wait_groups<0>();
+}
+
+// One CTA a boundary between two CTAs' shares: joins the unit it cuts, if it is the
+// first boundary inside that unit.
+template <int HD, int NT>
+__global__ void __launch_bounds__(kThreads) kv8_join_kernel(const __grid_constant__ AttnArgs a, int grid) {
+  constexpr int ROWS = 8 * NT;
+  __shared__ ScanSmem scan;
+  const int i = blockIdx.x + 1;
+  int ctas = 0;
+  int64_t cut = 0;
+  const Place at = find_place<ROWS>(a, scan, false, [&](int64_t total) {
+    ctas = active_ctas(total, grid);
+    if (i < ctas) cut = share_begin(total, ctas, i);
+    return i < ctas ? cut : int64_t{-1};
+  });
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (i >= ctas) return;
+  const SeqWork w = seq_work<ROWS>(a, at.seq, nullptr);
+  const int unit = static_cast<int>((cut - at.base) / w.steps);
+  const int64_t u0 = at.base + static_cast<int64_t>(unit) * w.steps, u1 = u0 + w.steps;
+  if (u0 == cut || share_begin(at.total, ctas, i - 1) > u0) return;   // not inside, or not the first
+  int last = i;
+  while (last + 1 < ctas && share_begin(at.total, ctas, last + 1) < u1) ++last;
+  const int kvh = unit % a.c.num_kv_heads, tile = unit / a.c.num_kv_heads;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(ROWS), static_cast<int64_t>(w.n) * a.group - static_cast<int64_t>(tile) * ROWS));
+  constexpr int kSlot = ROWS * HD + 2 * ROWS;
+  // the unit is the first segment of every CTA but maybe the first one
+  const int64_t s0 = (i - 1) * 2 + (share_begin(at.total, ctas, i - 1) < u0 ? 1 : 0);
+  auto slot = [&](int k) { return a.part + (k == i - 1 ? s0 : 2 * static_cast<int64_t>(k)) * kSlot; };
+  for (int e = threadIdx.x; e < rows * (HD / 4); e += kThreads) {
+    const int r = e / (HD / 4), d = e % (HD / 4) * 4;
+    float top = -INFINITY, sum = 0.f;
+    float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = i - 1; k <= last; ++k) top = fmaxf(top, slot(k)[ROWS * HD + r]);
+    for (int k = i - 1; k <= last; ++k) {
+      const float* p = slot(k);
+      const float f = join_factor(p[ROWS * HD + r], top);
+      sum += p[ROWS * HD + ROWS + r] * f;
+      const float4 x = *reinterpret_cast<const float4*>(p + r * HD + d);
+      z.x += x.x * f;
+      z.y += x.y * f;
+      z.z += x.z * f;
+      z.w += x.w * f;
+    }
+    write_out(a, w.row0, static_cast<int64_t>(tile) * ROWS + r, kvh, HD, d, z, top, sum);
   }
 }
 
@@ -88,6 +762,56 @@ int check_heads(const GltKv8Cache* c, const GltKv8Batch* b, int nh) {
   return GLT_OK;
 }
 
+// Row tiles of 8 fill the tensor core's N for up to 8 rows a KV head; more rows go 16 at a
+// time, which reads the cache half as often.
+struct Plan {
+  int nt, grid;
+  int64_t bytes;
+};
+Plan plan(const GltKv8Cache& c, const GltKv8Batch& b, int nh) {
+  Plan p;
+  const int64_t rows = static_cast<int64_t>(b.max_new) * (nh / c.num_kv_heads);
+  p.nt = rows <= 8 ? 1 : 2;
+  // no more CTAs than the fullest cache could feed
+  const int64_t tiles = (rows + 8 * p.nt - 1) / (8 * p.nt);
+  const int64_t steps = (static_cast<int64_t>(b.max_blocks) * c.block_tokens + kStep - 1) / kStep;
+  const double most = static_cast<double>(tiles) * c.num_kv_heads * b.num_seqs * steps / kWarps + 1;
+  p.grid = num_sms() * ctas_per_sm(p.nt);
+  if (most < p.grid) p.grid = static_cast<int>(most);
+  const int64_t r = 8 * p.nt;
+  p.bytes = p.grid * 2 * (r * c.head_dim + 2 * r) * 4;
+  return p;
+}
+
+template <int HD, int FMT, int NT, bool BT16>
+int launch(const AttnArgs& a, int grid, cudaStream_t st) {
+  constexpr int bytes = smem_bytes<HD, NT>();
+  GLT_TRY(ensure_smem_attr(reinterpret_cast<const void*>(&kv8_attention_kernel<HD, FMT, NT, BT16>), bytes));
+  kv8_attention_kernel<HD, FMT, NT, BT16><<<grid, kThreads, bytes, st>>>(a);
+  GLT_LAUNCH_CHECK();
+  if (grid < 2) return GLT_OK;
+  // starts while the first kernel runs, finds its unit, then waits for that kernel's end
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid - 1);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  GLT_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv8_join_kernel<HD, NT>, a, grid));
+  GLT_LAUNCH_CHECK();
+  return GLT_OK;
+}
+
+template <int HD, int FMT>
+int launch_rows(const AttnArgs& a, const Plan& p, cudaStream_t st) {
+  if (a.c.block_tokens == 16)
+    return p.nt == 1 ? launch<HD, FMT, 1, true>(a, p.grid, st) : launch<HD, FMT, 2, true>(a, p.grid, st);
+  return p.nt == 1 ? launch<HD, FMT, 1, false>(a, p.grid, st) : launch<HD, FMT, 2, false>(a, p.grid, st);
+}
+
 }  // namespace
 }  // namespace glt
 
@@ -95,7 +819,7 @@ extern "C" int glt_kv8_attention_workspace(const GltKv8Cache* cache, const GltKv
                                            int num_heads, int64_t* bytes) {
   if (!bytes) return glt::fail(GLT_EINVAL, "null argument");
   GLT_TRY(glt::check_heads(cache, batch, num_heads));
-  *bytes = 0;
+  *bytes = batch->rows > 0 && batch->max_new > 0 ? glt::plan(*cache, *batch, num_heads).bytes : 0;
   return GLT_OK;
 }
 
@@ -113,14 +837,28 @@ extern "C" int glt_kv8_attention(const GltKv8Cache* cache, const GltKv8Batch* ba
   if (window < 0) return glt::fail(GLT_EINVAL, "kv8: negative window");
   if (token_mask && ld_mask < static_cast<int64_t>(batch->max_blocks) * cache->block_tokens)
     return glt::fail(GLT_EINVAL, "kv8: mask row stride below max_blocks * block_tokens");
-  int64_t need = 0;
-  GLT_TRY(glt_kv8_attention_workspace(cache, batch, num_heads, &need));
-  if (workspace_bytes < need || (need > 0 && (!workspace || !glt::aligned16(workspace))))
-    return glt::fail(GLT_EINVAL, "kv8: workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
-  const dim3 grid(batch->max_new < 65535 ? batch->max_new : 65535, batch->num_seqs, num_heads);
-  glt::kv8_attention_kernel<<<grid, glt::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-      *cache, *batch, q, ld_q, o, ld_o, lse, num_heads, scale > 0.f ? scale : 1.f / sqrtf(static_cast<float>(cache->head_dim)),
-      window, token_mask, ld_mask, glt::device_error_word());
-  GLT_LAUNCH_CHECK();
-  return GLT_OK;
+  const glt::Plan p = glt::plan(*cache, *batch, num_heads);
+  if (workspace_bytes < p.bytes || !workspace || !glt::aligned16(workspace))
+    return glt::fail(GLT_EINVAL, "kv8: workspace must be 16-byte aligned and hold %lld bytes", (long long)p.bytes);
+  glt::AttnArgs a;
+  a.c = *cache;
+  a.b = *batch;
+  a.q = q;
+  a.ld_q = ld_q;
+  a.o = o;
+  a.ld_o = ld_o;
+  a.lse = lse;
+  a.nh = num_heads;
+  a.group = num_heads / cache->num_kv_heads;
+  a.scale = scale > 0.f ? scale : 1.f / sqrtf(static_cast<float>(cache->head_dim));
+  a.window = window;
+  a.mask = token_mask;
+  a.ld_mask = ld_mask;
+  a.part = static_cast<float*>(workspace);
+  a.err = glt::device_error_word();
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool int8 = cache->format == GLT_KV8_INT8;
+  if (cache->head_dim == 128)
+    return int8 ? glt::launch_rows<128, GLT_KV8_INT8>(a, p, st) : glt::launch_rows<128, GLT_KV8_E4M3>(a, p, st);
+  return int8 ? glt::launch_rows<64, GLT_KV8_INT8>(a, p, st) : glt::launch_rows<64, GLT_KV8_E4M3>(a, p, st);
 }

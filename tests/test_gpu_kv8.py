@@ -343,3 +343,17 @@ def test_bad_device_values_set_the_error_word():
             assert torch.isfinite(out[1].float()).all() and (out[1] != 7).any()
     c.read(serve.Kv8Batch(i32([[9, 1]]), i32([3]), 0, max_new=0), None, 3)
     assert device_error() == 2
+
+
+def test_nan_queries_give_nan_in_their_rows_only():
+    s = Session("int8", 32, 1, 2, 64, seqs=2, room=400, seed=11)
+    s.step([300, 300], window=1)
+    q = torch.randn(2, 2, 64, device=DEV).to(torch.bfloat16)
+    batch = serve.Kv8Batch(s.table, i32([x - 1 for x in s.lens]), 2)
+    want = s.cache.attention(batch, q)
+    bad = q.clone()
+    bad[0, 1, 3] = math.nan
+    o, lse = s.cache.attention(batch, bad)
+    assert torch.isnan(o[0, 1]).all() and torch.isnan(lse[0, 1])
+    for r, h in ((0, 0), (1, 0), (1, 1)):
+        assert torch.equal(o[r, h], want[0][r, h]) and lse[r, h] == want[1][r, h]
