@@ -30,6 +30,11 @@ int make_tmap_f32_plain(CUtensorMap* tm, const void* base, uint64_t inner, uint6
 int make_tmap_f32_swz128(CUtensorMap* tm, const void* base, uint64_t inner, uint64_t outer,
                          uint64_t ld, uint32_t box_outer);
 
+// 2-D map of dense rows of 64 or 128 bytes (dims {inner, outer}, box {inner,
+// box_outer}), swizzled by its row length: of 128-byte rows, 16-byte chunk c of
+// row r lies at chunk c ^ (r & 7); of 64-byte rows, at c ^ ((r >> 1) & 3).
+int make_tmap_u8(CUtensorMap* tm, const void* base, uint64_t inner, uint64_t outer, uint32_t box_outer);
+
 int num_sms();
 
 // Dynamic tile claiming (GemmShape::tile_ctr) for the GEMMs this host thread

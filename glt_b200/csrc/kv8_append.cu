@@ -14,6 +14,8 @@ int kv8_check(const GltKv8Cache* c, const GltKv8Batch* b) {
   if (c->head_dim != 64 && c->head_dim != 128) return fail(GLT_EINVAL, "kv8: head_dim %d (64 or 128)", c->head_dim);
   if (c->num_kv_heads < 1 || c->num_kv_heads > 4096) return fail(GLT_EINVAL, "kv8: num_kv_heads %d", c->num_kv_heads);
   if (c->num_blocks < 1 || c->num_blocks > INT_MAX) return fail(GLT_EINVAL, "kv8: num_blocks %lld", (long long)c->num_blocks);
+  if (c->num_blocks * c->num_kv_heads * bt > INT_MAX)
+    return fail(GLT_EINVAL, "kv8: a pool of %lld rows (at most 2^31 - 1)", (long long)(c->num_blocks * c->num_kv_heads * bt));
   if (!c->k || !c->v || !c->k_scale || !c->v_scale) return fail(GLT_EINVAL, "kv8: null cache buffer");
   if (!aligned16(c->k) || !aligned16(c->v)) return fail(GLT_EINVAL, "kv8: cache pools must be 16-byte aligned");
   if (b->num_seqs < 0 || b->num_seqs > 65535 || b->rows < 0 || b->max_new < 0)

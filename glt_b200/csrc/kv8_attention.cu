@@ -25,10 +25,13 @@
 // The order of a contraction's index is free, so a lane loads 16 contiguous bytes and
 // uses them for four k-steps of S or eight rows of O.
 //
-// Loads.  Every lane copies the bytes that it will use itself into its own slots of a
-// ring in shared memory (cp.async, 16 bytes), so the ring needs no barrier, and the
-// copies run ahead of the arithmetic across units.
+// Loads.  A warp keeps its own ring of stages in shared memory: one lane starts two TMA
+// copies a step (K and V, 32 rows each, one with blocks of 16 tokens: four), swizzled so
+// that the fragment reads meet no bank twice, and the warp waits on the stage's mbarrier.
+// No warp waits for another inside a unit, and the copies run ahead across units.
 #include <float.h>
+
+#include <type_traits>
 
 #include "kv8.cuh"
 
@@ -145,7 +148,8 @@ __device__ __forceinline__ int64_t share_begin(int64_t total, int ctas, int i) {
 template <int ROWS>
 struct Cursor {
   int seq, unit, s0, s1;
-  int64_t left;   // steps of the run from s0 on
+  int kvh, tile;   // of the unit
+  int64_t left;    // steps of the run from s0 on
   SeqWork w;
   __device__ __forceinline__ void start(const AttnArgs& a, int seq_, int64_t offset, int64_t count) {
     seq = seq_;
@@ -153,14 +157,21 @@ struct Cursor {
     if (left <= 0) return;
     w = seq_work<ROWS>(a, seq, nullptr);
     unit = static_cast<int>(offset / w.steps);
+    tile = unit / a.c.num_kv_heads;
+    kvh = unit - tile * a.c.num_kv_heads;
     s0 = static_cast<int>(offset - static_cast<int64_t>(unit) * w.steps);
     s1 = static_cast<int>(min(static_cast<int64_t>(w.steps), s0 + left));
   }
   __device__ __forceinline__ void next(const AttnArgs& a) {
     left -= s1 - s0;
     if (left <= 0) return;
-    if (++unit == w.units) {
-      unit = 0;
+    ++unit;
+    if (++kvh == a.c.num_kv_heads) {
+      kvh = 0;
+      ++tile;
+    }
+    if (unit == w.units) {
+      unit = kvh = tile = 0;
       do {
         if (++seq >= a.b.num_seqs) {   // only if the lengths changed under the kernel
           left = 0;
@@ -175,14 +186,9 @@ struct Cursor {
   __device__ __forceinline__ bool whole() const { return s0 == 0 && s1 == w.steps; }
 };
 
-__device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
-// Copies of B bytes (zeros where !on); the source address is not read then.
-template <int B>
-__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool on) {
-  if constexpr (B == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(on ? 16 : 0) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(src), "n"(B), "r"(on ? B : 0) : "memory");
+// Copies 4 bytes (zero where !on: the source is not read then).
+__device__ __forceinline__ void copy_async4(void* dst, const void* src, bool on) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(tc::smem_u32(dst)), "l"(src), "r"(on ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -192,6 +198,12 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same from sums of 0.
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   uint32_t r;
@@ -231,31 +243,47 @@ __device__ __forceinline__ void write_out(const AttnArgs& a, int row0, int64_t r
 // 2^(m - top) for partial results: weights that saw nothing are 0 (or NaN) already.
 __device__ __forceinline__ float join_factor(float m, float top) { return top == -INFINITY ? 1.f : ex2_approx(m - top); }
 
-// Bytes a lane copies for a step: K rows g, g + 8 of each half of 16 tokens, 16 bytes at
-// 16 c (+ 64); V tokens 2c, 2c + 1, 2c + 8, 2c + 9 of each half, hd / 8 bytes at channel g hd / 8.
+// One warp's ring: stages of 32 rows of K, then 32 rows of V; scales and flags beside them.
 template <int HD>
 struct Ring {
   static constexpr int kStages = HD == 128 ? 2 : 3;
-  static constexpr int kKeys = HD / 16;                  // 16-byte copies of K a lane and step
-  static constexpr int kValueBytes = HD / 8;             // bytes of a copy of V
-  static constexpr int kStage = 32 * (kKeys * 16 + 8 * kValueBytes) + 32;   // + scales, validity
+  static constexpr int kPart = kStep * HD;          // bytes of K (or V) of a stage
+  static constexpr int kStage = 2 * kPart;
   static constexpr int kWarp = kStages * kStage;
+};
+struct StageNote {
+  float scale[4];   // K, V of the first fold unit; K, V of the second
+  int valid;        // bit u: the block of tokens 16 u .. 16 u + 15 is in the pool
+  int pad[3];
 };
 template <int HD, int NT>
 constexpr int smem_bytes() {
-  return kWarps * Ring<HD>::kWarp + 2 * 8 * NT * HD * 4 + kWarps * 8 * NT * 8 + static_cast<int>(sizeof(ScanSmem));
+  return 1024 /* alignment */ + kWarps * Ring<HD>::kWarp + 2 * 8 * NT * HD * 4 + kWarps * 8 * NT * 8 +
+         kWarps * Ring<HD>::kStages * static_cast<int>(sizeof(StageNote) + 8) + static_cast<int>(sizeof(ScanSmem));
 }
 
 template <int HD, int FMT, int NT, bool BT16>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kernel(const __grid_constant__ AttnArgs a,
+                                                                                   const __grid_constant__ CUtensorMap map_k,
+                                                                                   const __grid_constant__ CUtensorMap map_v) {
   constexpr int ROWS = 8 * NT, LU = BT16 ? 2 : 1;
   using R = Ring<HD>;
-  extern __shared__ __align__(16) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + (-tc::smem_u32(smem_raw) & 1023u);   // the swizzle goes by address
   float* join_o = reinterpret_cast<float*>(smem + kWarps * R::kWarp);            // [2][ROWS][HD]
   float2* join_ml = reinterpret_cast<float2*>(join_o + 2 * ROWS * HD);           // [warp][ROWS]
-  ScanSmem& scan = *reinterpret_cast<ScanSmem*>(join_ml + kWarps * ROWS);
+  StageNote* notes = reinterpret_cast<StageNote*>(join_ml + kWarps * ROWS);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(notes + kWarps * R::kStages);
+  ScanSmem& scan = *reinterpret_cast<ScanSmem*>(bars + kWarps * R::kStages);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
   asm volatile("griddepcontrol.launch_dependents;");
+  uint8_t* ring = smem + warp * R::kWarp;
+  notes += warp * R::kStages;
+  bars += warp * R::kStages;
+  if (lane == 0) {
+    for (int i = 0; i < R::kStages; ++i) tc::mbar_init(bars + i, 1);
+    tc::fence_mbar_init();
+  }
 
   int ctas = 0;
   int64_t begin = 0, end = 0;
@@ -269,68 +297,85 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
   });
   if (end <= begin) return;
 
-  uint8_t* ring = smem + warp * R::kWarp;
-  const uint32_t ring_k = smem_addr(ring) + lane * 16;
-  const uint32_t ring_v = smem_addr(ring) + 32 * R::kKeys * 16 + lane * R::kValueBytes;
-  constexpr int kScales = 32 * (R::kKeys * 16 + 8 * R::kValueBytes);
-
+  // The copies run kStages steps ahead of the arithmetic, and the block ids one step ahead of
+  // the copies: `ld` stands on the next step to copy, whose ids are on their way.
+  const int bt_log = 31 - __clz(a.c.block_tokens);
   Cursor<ROWS> ld;
   ld.start(a, at.seq, begin - at.base, end - begin);
-  int ld_step = ld.s0 + warp, ld_stage = 0;
-  // Copies this warp's next step of the run into the next stage (one group, maybe empty).
-  auto issue = [&]() {
+  int ld_step = ld.s0 + warp, ld_stage = 0, ld_id[LU];
+  auto seek = [&]() {
     while (ld.left > 0 && ld_step >= ld.s1) {
       ld.next(a);
       ld_step = ld.s0 + warp;
     }
     if (ld.left > 0) {
-      const int kvh = ld.unit % a.c.num_kv_heads;
-      const int t0 = ld.w.lo + ld_step * kStep, hi = ld.w.past + ld.w.n;
-      const uint32_t st = ld_stage * R::kStage;
+      const int t = ld.w.lo + ld_step * kStep;
+      const int32_t* ids = a.b.block_table + static_cast<int64_t>(ld.seq) * a.b.max_blocks;
+      ld_id[0] = ids[t >> bt_log];
+      if (LU == 2) ld_id[LU - 1] = t + 16 < ld.w.past + ld.w.n ? ids[(t + 16) >> bt_log] : -1;
+    }
+  };
+  // Copies this warp's next step into the next stage.
+  int issued = 0;
+  auto issue = [&]() {
+    if (ld.left > 0) {
+      const int t0 = ld.w.lo + ld_step * kStep, held = ld.w.past + ld.w.n - t0;   // tokens from t0 on
+      uint64_t* bar = bars + ld_stage;
+      uint8_t* dst = ring + ld_stage * R::kStage;
       int valid = 0;
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int t = t0 + 16 * u;
-        int64_t id = -1;
-        if (t < hi) id = kv8_block(a.c, a.b, ld.seq, t / a.c.block_tokens, lane == 0 ? a.err : nullptr);
-        const bool on = id >= 0;
-        valid |= on ? 1 << u : 0;
-        const int64_t hb = on ? id * a.c.num_kv_heads + kvh : 0;
-        const int64_t row = hb * a.c.block_tokens + (t & (a.c.block_tokens - 1));
-        const uint8_t* kp = a.c.k + row * HD;
-        const uint8_t* vp = a.c.v + row * HD;
-#pragma unroll
-        for (int r = 0; r < 2; ++r)
-#pragma unroll
-          for (int h = 0; h < HD / 64; ++h) {
-            const bool in = on && t + g + 8 * r < hi;
-            copy_async<16>(ring_k + st + ((u * 2 + r) * (HD / 64) + h) * 512,
-                           in ? kp + (g + 8 * r) * HD + h * 64 + c * 16 : a.c.k, in);
-          }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int tk = 2 * c + (i & 1) + 8 * (i >> 1);
-          const bool in = on && t + tk < hi;
-          copy_async<R::kValueBytes>(ring_v + st + (u * 4 + i) * 32 * R::kValueBytes,
-                                     in ? vp + tk * HD + g * R::kValueBytes : a.c.v, in);
-        }
-        if (lane < 2) copy_async<4>(smem_addr(ring) + st + kScales + u * 8 + lane * 4, (lane ? a.c.v_scale : a.c.k_scale) + hb, on);
+      for (int f = 0; f < LU; ++f) {
+        const bool on = ld_id[f] >= 0 && ld_id[f] < a.c.num_blocks;
+        if (on) valid |= LU == 2 ? 1 << f : 3;
+        if (!on && held > 16 * f && lane == 0 && a.err) atomicOr(a.err, GLT_DEVERR_BAD_SHAPE);
+        const int64_t hb = on ? static_cast<int64_t>(ld_id[f]) * a.c.num_kv_heads + ld.kvh : 0;
+        if (lane < 2) copy_async4(notes[ld_stage].scale + f * 2 + lane, (lane ? a.c.v_scale : a.c.k_scale) + hb, on);
       }
-      if (lane == 0) *reinterpret_cast<int*>(ring + st + kScales + 16) = valid;
+      if (lane == 0) {
+        notes[ld_stage].valid = valid;
+        const int units = LU == 2 ? (valid & 1) + (valid >> 1) : valid ? 1 : 0;
+        tc::mbar_arrive_expect_tx(bar, units * (R::kStage / LU));
+#pragma unroll
+        for (int f = 0; f < LU; ++f) {
+          if (!(valid >> f & 1)) continue;
+          const int64_t hb = static_cast<int64_t>(ld_id[f]) * a.c.num_kv_heads + ld.kvh;
+          const int row = static_cast<int>((hb << bt_log) + ((t0 + 16 * f) & (a.c.block_tokens - 1)));
+          tc::tma_load_2d(dst + f * (R::kPart / LU), &map_k, bar, 0, row);
+          tc::tma_load_2d(dst + R::kPart + f * (R::kPart / LU), &map_v, bar, 0, row);
+        }
+      }
       ld_step += kWarps;
+      ++issued;
+      seek();
     }
     commit();
     ld_stage = ld_stage + 1 == R::kStages ? 0 : ld_stage + 1;
   };
+  __syncwarp();   // the barriers are ready
+  seek();
 #pragma unroll 1
   for (int i = 0; i < R::kStages; ++i) issue();
 
   Cursor<ROWS> cu;
   cu.start(a, at.seq, begin - at.base, end - begin);
-  int stage = 0;
-  bool first_segment = true;
+  int stage = 0, taken = 0;
+  uint32_t phase = 0;
+  bool first_segment = true, lost = false;   // lost: a copy did not arrive in time
+  // A lane's fragment bytes in a stage.  K: rows g + 8 r + 16 u, chunk 2c + h (64-byte rows: c);
+  // V: rows 2c + e + 8 r + 16 u, the g-th eighth.
+  int off_k[HD / 64], off_v[2];
+  if (HD == 128) {
+#pragma unroll
+    for (int h = 0; h < HD / 64; ++h) off_k[h] = g * HD + (((2 * c + h) ^ g) << 4);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) off_v[e] = R::kPart + (2 * c + e) * HD + ((g ^ (2 * c + e)) << 4);
+  } else {
+    off_k[0] = g * HD + ((c ^ (g >> 1)) << 4);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) off_v[e] = R::kPart + (2 * c + e) * HD + (((g >> 1) ^ c) << 4) + (g & 1) * 8;
+  }
   while (cu.left > 0) {
-    const int kvh = cu.unit % a.c.num_kv_heads, tile = cu.unit / a.c.num_kv_heads;
+    const int kvh = cu.kvh, tile = cu.tile;
     const int rows = static_cast<int>(min(static_cast<int64_t>(ROWS), static_cast<int64_t>(cu.w.n) * a.group - static_cast<int64_t>(tile) * ROWS));
     // ---- queries: operand B, and the factor that takes S to log2 units
     uint32_t qb[NT][HD / 16][2];
@@ -348,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
       for (int h = 0; h < HD / 64; ++h)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          v[h][j] = in ? *reinterpret_cast<const uint4*>(src + h * 64 + c * 16 + j * 8) : make_uint4(0, 0, 0, 0);
+          v[h][j] = in ? *reinterpret_cast<const uint4*>(src + (HD == 128 ? 2 * c + h : c) * 16 + j * 8) : make_uint4(0, 0, 0, 0);
           float f[8];
           unpack8(v[h][j], f);
 #pragma unroll
@@ -413,49 +458,56 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
     for (int step = cu.s0 + warp; step < cu.s1; step += kWarps) {
       const uint32_t seen_now = seen;
       if (mrow) seen = mask_bits(step + kWarps);
+      if (lost) continue;
       wait_groups<R::kStages - 1>();
-      __syncwarp();   // the scales come from other lanes' copies
-      const uint8_t* sg = ring + stage * R::kStage;
-      const float4 sc = *reinterpret_cast<const float4*>(sg + kScales);   // ks, vs of half 0; of half 1
-      const int valid = *reinterpret_cast<const int*>(sg + kScales + 16);
+      __syncwarp();   // the note comes from other lanes
+      if (!__all_sync(0xffffffffu, tc::mbar_wait(bars + stage, phase, a.err))) {
+        lost = true;
+        continue;
+      }
+      ++taken;
+      uint8_t* sg = ring + stage * R::kStage;
+      const float4 sc = *reinterpret_cast<const float4*>(notes[stage].scale);
+      const int valid = notes[stage].valid;
       const int t0 = cu.w.lo + step * kStep;
       // ---- S^T
       float s[2][NT][4];
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) s[u][nt][k] = 0.f;
-#pragma unroll
         for (int h = 0; h < HD / 64; ++h) {
-          const uint4 r0 = *reinterpret_cast<const uint4*>(sg + ((u * 2 + 0) * (HD / 64) + h) * 512 + lane * 16);
-          const uint4 r1 = *reinterpret_cast<const uint4*>(sg + ((u * 2 + 1) * (HD / 64) + h) * 512 + lane * 16);
+          const uint4 r0 = *reinterpret_cast<const uint4*>(sg + off_k[h] + 16 * u * HD);
+          const uint4 r1 = *reinterpret_cast<const uint4*>(sg + off_k[h] + (16 * u + 8) * HD);
           const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t fa[4] = {two_codes<FMT, 0>(w0[k]), two_codes<FMT, 0>(w1[k]), two_codes<FMT, 1>(w0[k]),
                                     two_codes<FMT, 1>(w1[k])};
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(s[u][nt], fa, qb[nt][h * 4 + k][0], qb[nt][h * 4 + k][1]);
+            for (int nt = 0; nt < NT; ++nt) {
+              if (h == 0 && k == 0)
+                mma_f16_zero(s[u][nt], fa, qb[nt][0][0], qb[nt][0][1]);
+              else
+                mma_f16(s[u][nt], fa, qb[nt][h * 4 + k][0], qb[nt][h * 4 + k][1]);
+            }
           }
         }
       }
-      // ---- log2 units, masks
+      // ---- masks.  z = s * unit is the score in log2 units; the units are kept above 0 so that
+      // a masked -inf stays one
       const bool edge = valid != 3 || mrow || t0 + kStep - 1 > pos_lo || (a.window > 0 && t0 <= pos_hi - a.window);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const float f0 = sc.x * qs[nt][j], f1 = sc.z * qs[nt][j];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[i >> 1][nt][(i & 1) * 2 + j] *= i < 2 ? f0 : f1;
-        }
+      bool cleared = false;
       if (edge) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int t = t0 + 8 * i + g;
-          const bool on = (valid >> (i >> 1) & 1) && (!mrow || (seen_now >> i & 1));
+          const bool on = (valid >> (i >> 1) & 1) && (!mrow || (seen_now >> i & 1)) && t <= pos_hi;
+          if (FMT == GLT_KV8_E4M3 && !on) {
+            // bytes that nobody wrote may be NaN codes, and 0 times NaN is NaN
+            for (int b = 0; b < HD / 4; b += 16)
+              *reinterpret_cast<uint4*>(sg + R::kPart + (8 * i + g) * HD + c * (HD / 4) + b) = make_uint4(0, 0, 0, 0);
+            cleared = true;
+          }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -464,11 +516,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
                 s[i >> 1][nt][(i & 1) * 2 + j] = -INFINITY;
         }
       }
+      if (FMT == GLT_KV8_E4M3 && edge) __syncwarp();   // rows were cleared for other lanes
       // A fold unit is what shares a scale of V in this step: its halves with blocks of 16
       // tokens, else the whole step.  Its weights are taken from its own maximum `peak`
       // (2^15 at most, in f16's range), and join the running sums by a 32-bit factor.
       bool moved = false;
-      float peak[LU][NT][2], ref[NT][2];
+      float peak[LU][NT][2], unit[LU][NT][2], ref[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -476,11 +529,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
           float top = m[nt][j];
 #pragma unroll
           for (int f = 0; f < LU; ++f) {
+            unit[f][nt][j] = fmaxf((f ? sc.z : sc.x) * qs[nt][j], 1e-37f);
             float x = fmaxf(s[f][nt][j], s[f][nt][2 + j]);
             if (LU == 1) x = fmaxf(x, fmaxf(s[1][nt][j], s[1][nt][2 + j]));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+            x *= unit[f][nt][j];
             peak[f][nt][j] = x;
             top = fmaxf(top, x);
           }
@@ -519,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
             for (int i = 0; i < 4; ++i) {
               if (LU == 2 && (i >> 1) != f) continue;
               float& p = s[i >> 1][nt][(i & 1) * 2 + j];
-              p = ex2_approx(p - r);
+              p = ex2_approx(fmaf(p, unit[f][nt][j], -r));
               sum += p;
               small |= p < kF16Min && p > 0.f;
             }
@@ -529,7 +584,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
       if (__any_sync(0xffffffffu, small)) {
 #pragma unroll 1
         for (int i = 0; i < 4; ++i) {   // tokens 8 i + g of the step
-          const int u = i >> 1;
           float p[NT][2];
           bool mine = false;
 #pragma unroll
@@ -542,14 +596,15 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
               if (i == 3) x = s[1][nt][2 + j];
               if (!(x < kF16Min)) x = 0.f;
               mine |= x > 0.f;
-              p[nt][j] = x * fold[LU == 2 ? u : 0][nt][j];
+              p[nt][j] = x * fold[LU == 2 ? i >> 1 : 0][nt][j];
             }
           uint32_t lanes = __ballot_sync(0xffffffffu, mine);
           while (lanes) {
             const int tg = (__ffs(lanes) - 1) >> 2;
             lanes &= ~(0xFu << (4 * tg));
-            const int slot = (u * 4 + (tg & 1) + 2 * (i & 1)) * 32 + g * 4 + (tg >> 1);
-            const uint8_t* vc = sg + 32 * R::kKeys * 16 + slot * R::kValueBytes;
+            // row 8 i + tg, the g-th eighth of its channels
+            const uint8_t* vc = sg + R::kPart + (8 * i + tg) * HD +
+                                (HD == 128 ? (g ^ tg) << 4 : (((g >> 1) ^ (tg >> 1)) << 4) + (g & 1) * 8);
             float pt[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -583,46 +638,43 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
           pb[u][nt][1] = transpose_8x8(pack_f16x2(s[u][nt][2], s[u][nt][3]));
         }
       // ---- O^T
-      const uint8_t* sv = sg + 32 * R::kKeys * 16 + lane * R::kValueBytes;
+      float part[HD / 16][NT][4];
 #pragma unroll
-      for (int jw = 0; jw < HD / 32; ++jw) {   // one word (four channels) of every token: two row tiles
-        float part[LU][2][NT][4];
+      for (int u = 0; u < 2; ++u) {
+        uint32_t w[4][HD / 32];   // four tokens, four channels a word
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            w[i] = *reinterpret_cast<const uint32_t*>(sv + (u * 4 + i) * 32 * R::kValueBytes + jw * 4);
-          constexpr int kLast = LU - 1;
-          const int f = u < kLast ? u : kLast;
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t x = __byte_perm(w[0], w[1], half ? 0x7362 : 0x5140);
-            const uint32_t y = __byte_perm(w[2], w[3], half ? 0x7362 : 0x5140);
-            const uint32_t fa[4] = {two_codes<FMT, 0>(x), two_codes<FMT, 1>(x), two_codes<FMT, 0>(y), two_codes<FMT, 1>(y)};
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              if (LU == 2 || u == 0)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) part[f][half][nt][k] = 0.f;
-              mma_f16(part[f][half][nt], fa, pb[u][nt][0], pb[u][nt][1]);
-            }
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (HD == 128) {
+            const uint4 x = *reinterpret_cast<const uint4*>(sg + off_v[i & 1] + (16 * u + 8 * (i >> 1)) * HD);
+            w[i][0] = x.x, w[i][1] = x.y, w[i][2] = x.z, w[i][3] = x.w;
+          } else {
+            const uint2 x = *reinterpret_cast<const uint2*>(sg + off_v[i & 1] + (16 * u + 8 * (i >> 1)) * HD);
+            w[i][0] = x.x, w[i][1] = x.y;
           }
         }
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
+        for (int k = 0; k < HD / 16; ++k) {
+          const uint32_t x = __byte_perm(w[0][k >> 1], w[1][k >> 1], (k & 1) ? 0x7362 : 0x5140);
+          const uint32_t y = __byte_perm(w[2][k >> 1], w[3][k >> 1], (k & 1) ? 0x7362 : 0x5140);
+          const uint32_t fa[4] = {two_codes<FMT, 0>(x), two_codes<FMT, 1>(x), two_codes<FMT, 0>(y), two_codes<FMT, 1>(y)};
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
+          for (int nt = 0; nt < NT; ++nt) {
+            if (LU == 2 || u == 0)
+              mma_f16_zero(part[k][nt], fa, pb[u][nt][0], pb[u][nt][1]);
+            else
+              mma_f16(part[k][nt], fa, pb[u][nt][0], pb[u][nt][1]);
+            if (LU == 2 || u == 1)
 #pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-              for (int f = 0; f < LU; ++f) {
-                float& d = acc[jw * 2 + half][nt][k];
-                d = fmaf(part[f][half][nt][k], fold[f][nt][k & 1], d);
-              }
+              for (int e = 0; e < 4; ++e) acc[k][nt][e] = fmaf(part[k][nt][e], fold[LU == 2 ? u : 0][nt][e & 1], acc[k][nt][e]);
+          }
+        }
       }
-      __syncwarp();   // all lanes are done with the stage's scales
-      stage = stage + 1 == R::kStages ? 0 : stage + 1;
+      if (FMT == GLT_KV8_E4M3 && cleared) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();   // all lanes are done with the stage
+      if (++stage == R::kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
       issue();
     }
 
@@ -706,6 +758,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
     cu.next(a);
   }
   wait_groups<0>();
+  // after a lost copy: the copies still under way end before the shared memory does
+  for (; taken < issued; ++taken) {
+    tc::mbar_wait(bars + stage, phase, a.err);
+    if (++stage == R::kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
 }
 
 // One CTA a boundary between two CTAs' shares: joins the unit it cuts, if it is the
@@ -787,7 +847,12 @@ template <int HD, int FMT, int NT, bool BT16>
 int launch(const AttnArgs& a, int grid, cudaStream_t st) {
   constexpr int bytes = smem_bytes<HD, NT>();
   GLT_TRY(ensure_smem_attr(reinterpret_cast<const void*>(&kv8_attention_kernel<HD, FMT, NT, BT16>), bytes));
-  kv8_attention_kernel<HD, FMT, NT, BT16><<<grid, kThreads, bytes, st>>>(a);
+  // rows of the pools; a copy is a step's rows, or a block's where blocks are shorter
+  const uint64_t pool_rows = static_cast<uint64_t>(a.c.num_blocks) * a.c.num_kv_heads * a.c.block_tokens;
+  CUtensorMap map_k, map_v;
+  GLT_TRY(make_tmap_u8(&map_k, a.c.k, HD, pool_rows, BT16 ? 16 : kStep));
+  GLT_TRY(make_tmap_u8(&map_v, a.c.v, HD, pool_rows, BT16 ? 16 : kStep));
+  kv8_attention_kernel<HD, FMT, NT, BT16><<<grid, kThreads, bytes, st>>>(a, map_k, map_v);
   GLT_LAUNCH_CHECK();
   if (grid < 2) return GLT_OK;
   // starts while the first kernel runs, finds its unit, then waits for that kernel's end

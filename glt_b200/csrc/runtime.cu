@@ -210,6 +210,23 @@ int make_tmap_f32_swz128(CUtensorMap* tm, const void* base, uint64_t inner, uint
   return GLT_OK;
 }
 
+int make_tmap_u8(CUtensorMap* tm, const void* base, uint64_t inner, uint64_t outer, uint32_t box_outer) {
+  EncodeTiledFn enc = get_encode_fn();
+  if (!enc) return fail(GLT_ECUDA, "cuTensorMapEncodeTiled unavailable");
+  if ((reinterpret_cast<uintptr_t>(base) & 15u) != 0 || (inner != 64 && inner != 128))
+    return fail(GLT_EINVAL, "byte tensor map: base not 16-byte aligned or rows not 64 or 128 bytes");
+  cuuint64_t dims[2] = {inner, outer};
+  cuuint64_t strides[1] = {inner};
+  cuuint32_t box[2] = {static_cast<cuuint32_t>(inner), box_outer};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = enc(tm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE,
+                   inner == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(GLT_ECUDA, "cuTensorMapEncodeTiled (bytes) failed (%d)", (int)r);
+  return GLT_OK;
+}
+
 int make_tmap_bf16(CUtensorMap* tm, const void* base, uint64_t inner, uint64_t outer,
                    uint64_t ld, uint32_t box_outer) {
   EncodeTiledFn enc = get_encode_fn();
