@@ -43,7 +43,8 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kStep = 32;   // tokens of a step
 constexpr float kF16Min = 6.103515625e-05f;   // 2^-14, the smallest normal f16
 
-__host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+constexpr int kCtasPerSm = 2;
+constexpr int kUnitCost = 3;   // what beginning and ending a unit costs a CTA, in steps
 
 struct AttnArgs {
   GltKv8Cache c;
@@ -58,13 +59,14 @@ struct AttnArgs {
   int window;
   const uint8_t* mask;
   int64_t ld_mask;
-  float* part;   // [CTA][2] partial results: rows x hd sums, then rows maxima (base 2), rows sums
+  void* workspace;
   unsigned int* err;
 };
 
 // What one sequence has to do: `steps` steps from token `lo` on, for `units` units.
 struct SeqWork {
   int past, n, row0, lo, steps, units;
+  __device__ __forceinline__ int64_t cost() const { return static_cast<int64_t>(steps + kUnitCost) * units; }
 };
 template <int ROWS>
 __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int seq, unsigned int* err) {
@@ -79,27 +81,52 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int seq, unsigned
   return w;
 }
 
-// Finds the sequence that step x of the whole falls into (and the total).  All
-// threads of the CTA call it.
-struct Place {
+// a / b by the much shorter 32-bit division where that is enough.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
+// How the cost of all sequences, laid end to end, is shared: each of `ctas` CTAs gets
+// `each`, the first `more` of them one more.
+struct Shares {
+  int64_t each;
+  int ctas, more;
+  __device__ __forceinline__ Shares(int64_t total, int grid) {
+    const int64_t n = (total + kWarps - 1) / kWarps;   // at least a step for every warp
+    ctas = n < grid ? static_cast<int>(n) : grid;
+    each = ctas > 0 ? quotient(total, ctas) : 0;
+    more = static_cast<int>(total - each * ctas);
+  }
+  __device__ __forceinline__ int64_t begin(int i) const { return each * i + min(i, more); }
+  __device__ __forceinline__ int owner(int64_t x) const {
+    const int64_t head = (each + 1) * more;
+    return static_cast<int>(x < head ? quotient(x, each + 1) : more + quotient(x - head, each));
+  }
+};
+
+// A CTA's run of the whole: where it begins, and what it costs.
+struct Run {
+  int64_t begin, end;   // in the whole
+  int64_t base;         // of its first sequence
   int seq;
-  int64_t base, total;   // first step of the sequence; steps of all sequences
+  SeqWork w;            // of that sequence
 };
 struct ScanSmem {
   int64_t warp[kWarps];
-  int64_t base;
-  int seq;
+  Run run;
 };
-template <int ROWS, typename Pick>
-__device__ Place find_place(const AttnArgs& a, ScanSmem& sm, bool report, Pick pick) {
+template <int ROWS>
+__device__ __forceinline__ Shares find_run(const AttnArgs& a, ScanSmem& sm) {
   const int per = (a.b.num_seqs + kThreads - 1) / kThreads;
   const int first = min(a.b.num_seqs, static_cast<int>(threadIdx.x) * per), last = min(a.b.num_seqs, first + per);
   int64_t mine = 0;
+  SeqWork w;
   for (int s = first; s < last; ++s) {
-    const SeqWork w = seq_work<ROWS>(a, s, report ? a.err : nullptr);
-    mine += static_cast<int64_t>(w.steps) * w.units;
+    w = seq_work<ROWS>(a, s, blockIdx.x == 0 ? a.err : nullptr);
+    mine += w.cost();
   }
-  int64_t scan = mine;
+  int64_t scan = mine, total = 0;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -108,62 +135,61 @@ __device__ Place find_place(const AttnArgs& a, ScanSmem& sm, bool report, Pick p
   }
   if (lane == 31) sm.warp[warp] = scan;
   __syncthreads();
-  Place p;
-  p.total = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) scan += sm.warp[w];
-    p.total += sm.warp[w];
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < warp) scan += sm.warp[i];
+    total += sm.warp[i];
   }
-  const int64_t x = pick(p.total);
+  const Shares sh(total, gridDim.x);
+  const int64_t begin = static_cast<int>(blockIdx.x) < sh.ctas ? sh.begin(blockIdx.x) : total;
+  const int64_t end = static_cast<int>(blockIdx.x) < sh.ctas ? sh.begin(blockIdx.x + 1) : total;
   int64_t base = scan - mine;
-  if (x >= base && x < scan) {
+  if (begin >= base && begin < scan) {   // one thread's, for begin < total
     for (int s = first; s < last; ++s) {
-      const SeqWork w = seq_work<ROWS>(a, s, nullptr);
-      const int64_t k = static_cast<int64_t>(w.steps) * w.units;
-      if (x < base + k) {
-        sm.seq = s;
-        sm.base = base;
+      if (last - first > 1) w = seq_work<ROWS>(a, s, nullptr);
+      if (begin < base + w.cost()) {
+        sm.run.begin = begin;
+        sm.run.end = end;
+        sm.run.base = base;
+        sm.run.seq = s;
+        sm.run.w = w;
         break;
       }
-      base += k;
+      base += w.cost();
     }
+  } else if (begin == total && threadIdx.x == 0) {
+    sm.run.begin = sm.run.end = total;
   }
   __syncthreads();
-  p.seq = sm.seq;
-  p.base = sm.base;
-  return p;
+  return sh;
 }
 
-// CTAs that share `total` steps: each has at least one for every warp.
-__device__ __forceinline__ int active_ctas(int64_t total, int grid) {
-  const int64_t n = (total + kWarps - 1) / kWarps;
-  return n < grid ? static_cast<int>(n) : grid;
-}
-__device__ __forceinline__ int64_t share_begin(int64_t total, int ctas, int i) {
-  return total / ctas * i + total % ctas * i / ctas;
-}
-
-// A run of steps, unit by unit.
+// Walks a run unit by unit: steps [s0, s1) of each (none where the run only holds a part
+// of the unit's kUnitCost).
 template <int ROWS>
 struct Cursor {
   int seq, unit, s0, s1;
   int kvh, tile;   // of the unit
-  int64_t left;    // steps of the run from s0 on
+  int64_t at, left;   // position in the sequence's unit, rest of the run
   SeqWork w;
-  __device__ __forceinline__ void start(const AttnArgs& a, int seq_, int64_t offset, int64_t count) {
-    seq = seq_;
-    left = count;
+  __device__ __forceinline__ void start(const AttnArgs& a, const Run& r) {
+    seq = r.seq;
+    left = r.end - r.begin;
     if (left <= 0) return;
-    w = seq_work<ROWS>(a, seq, nullptr);
-    unit = static_cast<int>(offset / w.steps);
+    w = r.w;
+    const int64_t offset = r.begin - r.base;
+    unit = static_cast<int>(quotient(offset, w.steps + kUnitCost));
     tile = unit / a.c.num_kv_heads;
     kvh = unit - tile * a.c.num_kv_heads;
-    s0 = static_cast<int>(offset - static_cast<int64_t>(unit) * w.steps);
-    s1 = static_cast<int>(min(static_cast<int64_t>(w.steps), s0 + left));
+    at = offset - static_cast<int64_t>(unit) * (w.steps + kUnitCost);
+    bounds();
+  }
+  __device__ __forceinline__ void bounds() {
+    s0 = max(0, static_cast<int>(at) - kUnitCost);
+    s1 = static_cast<int>(min(static_cast<int64_t>(w.steps), at + left - kUnitCost));
   }
   __device__ __forceinline__ void next(const AttnArgs& a) {
-    left -= s1 - s0;
+    left -= w.steps + kUnitCost - at;
     if (left <= 0) return;
     ++unit;
     if (++kvh == a.c.num_kv_heads) {
@@ -180,10 +206,32 @@ struct Cursor {
         w = seq_work<ROWS>(a, seq, nullptr);
       } while (w.units == 0);
     }
-    s0 = 0;
-    s1 = static_cast<int>(min(static_cast<int64_t>(w.steps), left));
+    at = 0;
+    bounds();
   }
   __device__ __forceinline__ bool whole() const { return s0 == 0 && s1 == w.steps; }
+};
+
+// The workspace: what to join (one task a CTA, that begins a unit it does not end), then two
+// partial results a CTA: rows x hd sums, rows maxima (base 2), rows sums of weights.
+struct JoinTask {
+  int parts;        // CTAs that hold a part: this one and the next parts - 1; 0: nothing to join
+  int first_slot;   // of this CTA; the others used their first
+  int row0, tile, kvh, rows;
+  int pad[2];
+};
+struct Workspace {
+  int* ctas;
+  JoinTask* tasks;
+  float* slots;
+  int64_t bytes;
+  __host__ __device__ Workspace(void* p, int grid, int rows, int hd) {
+    uint8_t* b = static_cast<uint8_t*>(p);
+    ctas = reinterpret_cast<int*>(b);
+    tasks = reinterpret_cast<JoinTask*>(b + 32);
+    slots = reinterpret_cast<float*>(b + 32 + grid * sizeof(JoinTask));
+    bytes = 32 + grid * sizeof(JoinTask) + static_cast<int64_t>(grid) * 2 * (rows * hd + 2 * rows) * 4;
+  }
 };
 
 // Copies 4 bytes (zero where !on: the source is not read then).
@@ -263,10 +311,13 @@ constexpr int smem_bytes() {
 }
 
 template <int HD, int FMT, int NT, bool BT16>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kernel(const __grid_constant__ AttnArgs a,
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(const __grid_constant__ AttnArgs a,
                                                                                    const __grid_constant__ CUtensorMap map_k,
                                                                                    const __grid_constant__ CUtensorMap map_v) {
   constexpr int ROWS = 8 * NT, LU = BT16 ? 2 : 1;
+  // the sums of a step's second half join those of the first, unless each half has its own scale
+  // or (NT = 2) holding them would not leave registers enough
+  constexpr bool kFoldEach = LU == 2 || NT == 2;
   using R = Ring<HD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-tc::smem_u32(smem_raw) & 1023u);   // the swizzle goes by address
@@ -285,23 +336,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
     tc::fence_mbar_init();
   }
 
-  int ctas = 0;
-  int64_t begin = 0, end = 0;
-  const Place at = find_place<ROWS>(a, scan, blockIdx.x == 0, [&](int64_t total) {
-    ctas = active_ctas(total, gridDim.x);
-    if (static_cast<int>(blockIdx.x) < ctas) {
-      begin = share_begin(total, ctas, blockIdx.x);
-      end = share_begin(total, ctas, blockIdx.x + 1);
-    }
-    return end > begin ? begin : int64_t{-1};
-  });
-  if (end <= begin) return;
+  const Shares shares = find_run<ROWS>(a, scan);
+  const Workspace ws(a.workspace, gridDim.x, ROWS, HD);
+  if (blockIdx.x == 0 && threadIdx.x == 0) *ws.ctas = shares.ctas;
+  if (scan.run.end <= scan.run.begin) return;
 
   // The copies run kStages steps ahead of the arithmetic, and the block ids one step ahead of
   // the copies: `ld` stands on the next step to copy, whose ids are on their way.
   const int bt_log = 31 - __clz(a.c.block_tokens);
   Cursor<ROWS> ld;
-  ld.start(a, at.seq, begin - at.base, end - begin);
+  ld.start(a, scan.run);
   int ld_step = ld.s0 + warp, ld_stage = 0, ld_id[LU];
   auto seek = [&]() {
     while (ld.left > 0 && ld_step >= ld.s1) {
@@ -357,10 +401,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
   for (int i = 0; i < R::kStages; ++i) issue();
 
   Cursor<ROWS> cu;
-  cu.start(a, at.seq, begin - at.base, end - begin);
+  cu.start(a, scan.run);
   int stage = 0, taken = 0;
   uint32_t phase = 0;
-  bool first_segment = true, lost = false;   // lost: a copy did not arrive in time
+  bool lost = false;   // a copy did not arrive in time
+  int done = 0;        // units of the run with steps here
+  int64_t base = scan.run.begin - cu.at;   // of the unit in the whole
+  JoinTask task = {};
   // A lane's fragment bytes in a stage.  K: rows g + 8 r + 16 u, chunk 2c + h (64-byte rows: c);
   // V: rows 2c + e + 8 r + 16 u, the g-th eighth.
   int off_k[HD / 64], off_v[2];
@@ -374,7 +421,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
 #pragma unroll
     for (int e = 0; e < 2; ++e) off_v[e] = R::kPart + (2 * c + e) * HD + (((g >> 1) ^ c) << 4) + (g & 1) * 8;
   }
-  while (cu.left > 0) {
+  for (; cu.left > 0; base += cu.w.steps + kUnitCost, cu.next(a)) {
+    if (cu.s1 <= cu.s0) continue;
     const int kvh = cu.kvh, tile = cu.tile;
     const int rows = static_cast<int>(min(static_cast<int64_t>(ROWS), static_cast<int64_t>(cu.w.n) * a.group - static_cast<int64_t>(tile) * ROWS));
     // ---- queries: operand B, and the factor that takes S to log2 units
@@ -496,18 +544,13 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
       // ---- masks.  z = s * unit is the score in log2 units; the units are kept above 0 so that
       // a masked -inf stays one
       const bool edge = valid != 3 || mrow || t0 + kStep - 1 > pos_lo || (a.window > 0 && t0 <= pos_hi - a.window);
-      bool cleared = false;
+      uint32_t live[4] = {};
       if (edge) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int t = t0 + 8 * i + g;
           const bool on = (valid >> (i >> 1) & 1) && (!mrow || (seen_now >> i & 1)) && t <= pos_hi;
-          if (FMT == GLT_KV8_E4M3 && !on) {
-            // bytes that nobody wrote may be NaN codes, and 0 times NaN is NaN
-            for (int b = 0; b < HD / 4; b += 16)
-              *reinterpret_cast<uint4*>(sg + R::kPart + (8 * i + g) * HD + c * (HD / 4) + b) = make_uint4(0, 0, 0, 0);
-            cleared = true;
-          }
+          if (FMT == GLT_KV8_E4M3) live[i] = __ballot_sync(0xffffffffu, on);   // bit 4g: token 8 i + g
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -516,7 +559,6 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
                 s[i >> 1][nt][(i & 1) * 2 + j] = -INFINITY;
         }
       }
-      if (FMT == GLT_KV8_E4M3 && edge) __syncwarp();   // rows were cleared for other lanes
       // A fold unit is what shares a scale of V in this step: its halves with blocks of 16
       // tokens, else the whole step.  Its weights are taken from its own maximum `peak`
       // (2^15 at most, in f16's range), and join the running sums by a 32-bit factor.
@@ -652,6 +694,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
             w[i][0] = x.x, w[i][1] = x.y;
           }
         }
+        if (FMT == GLT_KV8_E4M3 && edge) {
+          // bytes of tokens that no row sees may be NaN codes, and 0 times NaN is NaN
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!(live[2 * u + (i >> 1)] >> (4 * (2 * c + (i & 1))) & 1))
+#pragma unroll
+              for (int k = 0; k < HD / 32; ++k) w[i][k] = 0;
+        }
 #pragma unroll
         for (int k = 0; k < HD / 16; ++k) {
           const uint32_t x = __byte_perm(w[0][k >> 1], w[1][k >> 1], (k & 1) ? 0x7362 : 0x5140);
@@ -659,17 +709,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
           const uint32_t fa[4] = {two_codes<FMT, 0>(x), two_codes<FMT, 1>(x), two_codes<FMT, 0>(y), two_codes<FMT, 1>(y)};
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            if (LU == 2 || u == 0)
+            if (kFoldEach || u == 0)
               mma_f16_zero(part[k][nt], fa, pb[u][nt][0], pb[u][nt][1]);
             else
               mma_f16(part[k][nt], fa, pb[u][nt][0], pb[u][nt][1]);
-            if (LU == 2 || u == 1)
+            if (kFoldEach || u == 1)
 #pragma unroll
               for (int e = 0; e < 4; ++e) acc[k][nt][e] = fmaf(part[k][nt][e], fold[LU == 2 ? u : 0][nt][e & 1], acc[k][nt][e]);
           }
         }
       }
-      if (FMT == GLT_KV8_E4M3 && cleared) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();   // all lanes are done with the stage
       if (++stage == R::kStages) {
         stage = 0;
@@ -732,7 +781,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
     }
     __syncthreads();
     const bool whole = cu.whole();
-    float* slot = a.part + (blockIdx.x * 2 + (first_segment ? 0 : 1)) * static_cast<int64_t>(ROWS * HD + 2 * ROWS);
+    const int slot_index = blockIdx.x * 2 + (done > 0 ? 1 : 0);   // only the first and last unit can be cut
+    float* slot = ws.slots + static_cast<int64_t>(slot_index) * (ROWS * HD + 2 * ROWS);
+    if (!whole && cu.s0 == 0) {
+      task.parts = shares.owner(base + cu.w.steps + kUnitCost - 1) - blockIdx.x + 1;
+      task.first_slot = slot_index;
+      task.row0 = cu.w.row0;
+      task.tile = tile;
+      task.kvh = kvh;
+      task.rows = rows;
+    }
     for (int i = threadIdx.x; i < rows * (HD / 4); i += kThreads) {
       const int r = i / (HD / 4), d = i % (HD / 4) * 4;
       float top = -INFINITY, sum = 0.f;
@@ -754,9 +812,9 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
       }
     }
     __syncthreads();   // the join buffers are free again
-    first_segment = false;
-    cu.next(a);
+    ++done;
   }
+  if (threadIdx.x == 0) ws.tasks[blockIdx.x] = task;
   wait_groups<0>();
   // after a lost copy: the copies still under way end before the shared memory does
   for (; taken < issued; ++taken) {
@@ -768,50 +826,53 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NT)) kv8_attention_kerne
   }
 }
 
-// One CTA a boundary between two CTAs' shares: joins the unit it cuts, if it is the
-// first boundary inside that unit.
+// One CTA a task: joins the parts of a unit.
+constexpr int kJoinBatch = 8;   // parts whose loads are in flight at once
 template <int HD, int NT>
 __global__ void __launch_bounds__(kThreads) kv8_join_kernel(const __grid_constant__ AttnArgs a, int grid) {
-  constexpr int ROWS = 8 * NT;
-  __shared__ ScanSmem scan;
-  const int i = blockIdx.x + 1;
-  int ctas = 0;
-  int64_t cut = 0;
-  const Place at = find_place<ROWS>(a, scan, false, [&](int64_t total) {
-    ctas = active_ctas(total, grid);
-    if (i < ctas) cut = share_begin(total, ctas, i);
-    return i < ctas ? cut : int64_t{-1};
-  });
+  constexpr int ROWS = 8 * NT, kSlot = ROWS * HD + 2 * ROWS;
+  const Workspace ws(a.workspace, grid, ROWS, HD);
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (i >= ctas) return;
-  const SeqWork w = seq_work<ROWS>(a, at.seq, nullptr);
-  const int unit = static_cast<int>((cut - at.base) / w.steps);
-  const int64_t u0 = at.base + static_cast<int64_t>(unit) * w.steps, u1 = u0 + w.steps;
-  if (u0 == cut || share_begin(at.total, ctas, i - 1) > u0) return;   // not inside, or not the first
-  int last = i;
-  while (last + 1 < ctas && share_begin(at.total, ctas, last + 1) < u1) ++last;
-  const int kvh = unit % a.c.num_kv_heads, tile = unit / a.c.num_kv_heads;
-  const int rows = static_cast<int>(min(static_cast<int64_t>(ROWS), static_cast<int64_t>(w.n) * a.group - static_cast<int64_t>(tile) * ROWS));
-  constexpr int kSlot = ROWS * HD + 2 * ROWS;
-  // the unit is the first segment of every CTA but maybe the first one
-  const int64_t s0 = (i - 1) * 2 + (share_begin(at.total, ctas, i - 1) < u0 ? 1 : 0);
-  auto slot = [&](int k) { return a.part + (k == i - 1 ? s0 : 2 * static_cast<int64_t>(k)) * kSlot; };
-  for (int e = threadIdx.x; e < rows * (HD / 4); e += kThreads) {
+  const int ctas = *ws.ctas;
+  const JoinTask task = ws.tasks[blockIdx.x];   // read before it is known to be one: within the workspace
+  if (static_cast<int>(blockIdx.x) >= ctas || task.parts < 2) return;
+  auto slot = [&](int k) {
+    return ws.slots + (k == 0 ? static_cast<int64_t>(task.first_slot) : 2 * (static_cast<int64_t>(blockIdx.x) + k)) * kSlot;
+  };
+  for (int e = threadIdx.x; e < task.rows * (HD / 4); e += kThreads) {
     const int r = e / (HD / 4), d = e % (HD / 4) * 4;
     float top = -INFINITY, sum = 0.f;
     float4 z = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = i - 1; k <= last; ++k) top = fmaxf(top, slot(k)[ROWS * HD + r]);
-    for (int k = i - 1; k <= last; ++k) {
-      const float* p = slot(k);
-      const float f = join_factor(p[ROWS * HD + r], top);
-      sum += p[ROWS * HD + ROWS + r] * f;
-      const float4 x = *reinterpret_cast<const float4*>(p + r * HD + d);
-      z.x += x.x * f;
-      z.y += x.y * f;
-      z.z += x.z * f;
-      z.w += x.w * f;
+    for (int k0 = 0; k0 < task.parts; k0 += kJoinBatch) {
+      float m[kJoinBatch], l[kJoinBatch];
+      float4 x[kJoinBatch];
+      float peak = top;
+#pragma unroll
+      for (int k = 0; k < kJoinBatch; ++k) {
+        const float* p = slot(min(k0 + k, task.parts - 1));
+        m[k] = p[ROWS * HD + r];
+        l[k] = p[ROWS * HD + ROWS + r];
+        x[k] = *reinterpret_cast<const float4*>(p + r * HD + d);
+      }
+#pragma unroll
+      for (int k = 0; k < kJoinBatch; ++k)
+        if (k0 + k < task.parts) peak = fmaxf(peak, m[k]);
+      const float old = join_factor(top, peak);
+      sum *= old;
+      z = make_float4(z.x * old, z.y * old, z.z * old, z.w * old);
+#pragma unroll
+      for (int k = 0; k < kJoinBatch; ++k) {
+        if (k0 + k >= task.parts) continue;
+        const float f = join_factor(m[k], peak);
+        sum = fmaf(l[k], f, sum);
+        z.x = fmaf(x[k].x, f, z.x);
+        z.y = fmaf(x[k].y, f, z.y);
+        z.z = fmaf(x[k].z, f, z.z);
+        z.w = fmaf(x[k].w, f, z.w);
+      }
+      top = peak;
     }
-    write_out(a, w.row0, static_cast<int64_t>(tile) * ROWS + r, kvh, HD, d, z, top, sum);
+    write_out(a, task.row0, static_cast<int64_t>(task.tile) * ROWS + r, task.kvh, HD, d, z, top, sum);
   }
 }
 
@@ -835,11 +896,10 @@ Plan plan(const GltKv8Cache& c, const GltKv8Batch& b, int nh) {
   // no more CTAs than the fullest cache could feed
   const int64_t tiles = (rows + 8 * p.nt - 1) / (8 * p.nt);
   const int64_t steps = (static_cast<int64_t>(b.max_blocks) * c.block_tokens + kStep - 1) / kStep;
-  const double most = static_cast<double>(tiles) * c.num_kv_heads * b.num_seqs * steps / kWarps + 1;
-  p.grid = num_sms() * ctas_per_sm(p.nt);
+  const double most = static_cast<double>(tiles) * c.num_kv_heads * b.num_seqs * (steps + kUnitCost) / kWarps + 1;
+  p.grid = num_sms() * kCtasPerSm;
   if (most < p.grid) p.grid = static_cast<int>(most);
-  const int64_t r = 8 * p.nt;
-  p.bytes = p.grid * 2 * (r * c.head_dim + 2 * r) * 4;
+  p.bytes = Workspace(nullptr, p.grid, 8 * p.nt, c.head_dim).bytes;
   return p;
 }
 
@@ -855,9 +915,9 @@ int launch(const AttnArgs& a, int grid, cudaStream_t st) {
   kv8_attention_kernel<HD, FMT, NT, BT16><<<grid, kThreads, bytes, st>>>(a, map_k, map_v);
   GLT_LAUNCH_CHECK();
   if (grid < 2) return GLT_OK;
-  // starts while the first kernel runs, finds its unit, then waits for that kernel's end
+  // starts while the first kernel runs and waits for its end
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid - 1);
+  cfg.gridDim = dim3(grid - 1);   // the last CTA ends every unit it begins
   cfg.blockDim = dim3(kThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -919,7 +979,7 @@ extern "C" int glt_kv8_attention(const GltKv8Cache* cache, const GltKv8Batch* ba
   a.window = window;
   a.mask = token_mask;
   a.ld_mask = ld_mask;
-  a.part = static_cast<float*>(workspace);
+  a.workspace = workspace;
   a.err = glt::device_error_word();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool int8 = cache->format == GLT_KV8_INT8;
