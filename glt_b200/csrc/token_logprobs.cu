@@ -1,25 +1,112 @@
-// Log probabilities of given tokens, entropy and the most likely tokens of rows
-// of logits, and their gradient (glt_token_logprobs, glt_token_logprobs_bwd).
+// Log probabilities of given tokens, entropy and the most likely tokens of rows of
+// logits, and their gradient (glt_token_logprobs, glt_token_logprobs_bwd).
+//
+// With z = scale x, the running maximum m and the sums s = sum 2^d, t = sum 2^d d of
+// d = (z - m) / ln 2:  lse = m + ln s,  entropy = ln s - ln 2 t / s.  One pass over the
+// logits finds all three, and the maximum that each thread meets on the way decides
+// where the most likely tokens can be: the q-th largest of every warp's 32 maxima,
+// q = ceil(top / warps), taken least over the warps, has `top` logits at or above it,
+// so only the threads' shares whose maximum reaches it are read again (from L2).
+//
+// HBM bounds both kernels: the forward reads the logits once, the backward reads and
+// writes them once.  An element costs the forward about five instructions, one of them
+// on the special-function unit (16 a clock and SM, against the 12 bf16 logits that HBM
+// brings): sums run two at a time (f32x2), maxima and clamps in packed bf16.
+//
+// A row belongs to one CTA; with fewer rows than would fill the SMs, to a cluster of up
+// to eight, joined over distributed shared memory.
+#include <cooperative_groups.h>
 #include <float.h>
 #include <math.h>
 
 #include "common.cuh"
 #include "gemm.cuh"
 
+namespace cg = cooperative_groups;
+
 namespace glt {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
+constexpr int kBatch = 4;            // 16-byte vectors a thread has in flight
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// Logits below this count as probability 0 in the fast path, which is exact there: it runs
+// with a maximum of at least kFloor / 10 and a scale of at least 1e-6.
+constexpr float kFloor = -1e30f;
+
+__device__ __forceinline__ float logit(const float* p) { return *p; }
+__device__ __forceinline__ float logit(const uint16_t* p) { return bf16_bits_to_f32(*p); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(uint16_t* p, float v) { *p = bf16_bits_rn(v); }
+
+// A row as 16-byte vectors, with `head` and `tail` elements outside of them.
+template <typename T>
+struct RowView {
+  static constexpr int kVec = 16 / sizeof(T);
+  const T* x;
+  int V, head, nv, tail;
+  __device__ __forceinline__ RowView(const T* x_, int V_) : x(x_), V(V_) {
+    head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / static_cast<int>(sizeof(T));
+    if (head > V) head = V;
+    nv = (V - head) / kVec;
+    tail = V - head - nv * kVec;
+  }
+  __device__ __forceinline__ const uint4* vec(int v) const { return reinterpret_cast<const uint4*>(x + head) + v; }
+  // index of the e-th element outside of the vectors
+  __device__ __forceinline__ int edge(int e) const { return e < head ? e : V - tail + (e - head); }
+};
 
 template <typename T>
-__device__ __forceinline__ float load_logit(const T* p);
-template <>
-__device__ __forceinline__ float load_logit<float>(const float* p) { return *p; }
-template <>
-__device__ __forceinline__ float load_logit<uint16_t>(const uint16_t* p) { return bf16_bits_to_f32(*p); }
-__device__ __forceinline__ void store_logit(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store_logit(uint16_t* p, float v) { *p = bf16_bits_rn(v); }
+__device__ __forceinline__ void unpack(const uint4& u, float (&f)[16 / sizeof(T)]) {
+  if constexpr (sizeof(T) == 2) {
+    unpack8(u, f);
+  } else {
+    f[0] = __uint_as_float(u.x), f[1] = __uint_as_float(u.y), f[2] = __uint_as_float(u.z), f[3] = __uint_as_float(u.w);
+  }
+}
+
+// Largest element, NaN if any is.
+template <typename T>
+__device__ __forceinline__ float vector_max(const uint4 (&b)[kBatch]) {
+  if constexpr (sizeof(T) == 2) {
+    uint32_t m = b[0].x;
+    auto take = [&](uint32_t w) { asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(m) : "r"(w)); };
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      if (j) take(b[j].x);
+      take(b[j].y), take(b[j].z), take(b[j].w);
+    }
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(bf16_lo(m)), "f"(bf16_hi(m)));
+    return r;
+  } else {
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      for (uint32_t w : {b[j].x, b[j].y, b[j].z, b[j].w}) asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(__uint_as_float(w)));
+    return m;
+  }
+}
+
+// Two floats in one 64-bit register, and sums on them.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 
 // Rank of a logit as a 64-bit key: larger logits first, then lower indices.
 // NaN ranks below every number; -0 equals +0.
@@ -29,99 +116,420 @@ __device__ __forceinline__ uint64_t rank_key(float x, uint32_t index) {
   if (x != x) u = 0;
   return (static_cast<uint64_t>(u) << 32) | (0xFFFFFFFFu - index);
 }
+__device__ __forceinline__ uint32_t key_index(uint64_t k) { return 0xFFFFFFFFu - static_cast<uint32_t>(k); }
 
-template <typename Op, typename V>
-__device__ __forceinline__ V block_reduce(V v, V* red, Op op) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = red[0];
-  for (int w = 1; w < kThreads / 32; ++w) v = op(v, red[w]);
-  return v;
-}
+// Running statistics of some logits: maximum m (a logit), sums to base 2^(a (x - m)).
+struct Stats {
+  float m, s, t;
+  __device__ __forceinline__ void join(float m2, float s2, float t2, float a) {
+    const float top = fmaxf(m, m2);
+    if (top == -INFINITY) return;
+    // the difference before the product: m and m2 may be large and close
+    const float d1 = m == -INFINITY ? 0.f : (m - top) * a, d2 = m2 == -INFINITY ? 0.f : (m2 - top) * a;
+    const float f1 = exp2f(d1), f2 = exp2f(d2);
+    const float u1 = s > 0.f && f1 > 0.f ? f1 * fmaf(s, d1, t) : 0.f, u2 = s2 > 0.f && f2 > 0.f ? f2 * fmaf(s2, d2, t2) : 0.f;
+    s = s * f1 + s2 * f2;
+    t = u1 + u2;
+    m = top;
+  }
+};
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_kernel(
+// The largest keys a warp has seen, one a lane in falling order (0: none).
+struct TopList {
+  uint64_t key = 0;
+  // Takes every lane's candidate (0: none) that ranks above the top-th.
+  __device__ __forceinline__ void take(uint64_t cand, int top, int lane) {
+    uint32_t who = __ballot_sync(0xffffffffu, cand > __shfl_sync(0xffffffffu, key, top - 1));
+    while (who) {
+      const int from = __ffs(who) - 1;
+      who &= who - 1;
+      const uint64_t k = __shfl_sync(0xffffffffu, cand, from);
+      const int at = __popc(__ballot_sync(0xffffffffu, key > k));
+      const uint64_t up = __shfl_up_sync(0xffffffffu, key, 1);
+      if (lane == at) key = k;
+      if (lane > at) key = up;
+    }
+  }
+};
+
+struct RowSmem {
+  Stats stats[kWarps];
+  uint64_t floor[kWarps];
+  uint64_t keys[kWarps][kMaxTop];
+  unsigned char slots[kThreads];   // threads whose share is read again
+  int nslots, bad;
+  // joined over the cluster by its first CTA
+  Stats cta;
+  int cta_bad;
+  uint64_t cta_keys[kMaxTop];
+};
+
+template <typename T, int CLUSTER>
+__global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(
     const T* __restrict__ logits, int64_t ld, int V, const int32_t* __restrict__ targets, float scale,
     int top, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ lse_out,
     int32_t* __restrict__ top_ids, float* __restrict__ top_logp, unsigned int* err) {
-  __shared__ float redf[kThreads / 32];
-  __shared__ unsigned long long redk[kThreads / 32];
-  const int64_t r = blockIdx.x;
-  const T* x = logits + r * ld;
-  auto fmx = [](float a, float b) { return fmaxf(a, b); };
-  auto add = [](float a, float b) { return a + b; };
-  float m = -INFINITY, bad = 0.f;
-  for (int i = threadIdx.x; i < V; i += kThreads) {
-    const float z = load_logit(x + i) * scale;
-    if (!(z < INFINITY)) bad = 1.f;
-    m = fmaxf(m, z);
-  }
-  m = block_reduce(m, redf, fmx);
-  bad = block_reduce(bad, redf, fmx);
-  float s = 0.f, t = 0.f;
-  if (m > -INFINITY)
-    for (int i = threadIdx.x; i < V; i += kThreads) {
-      const float d = load_logit(x + i) * scale - m;
-      const float e = expf(d);
-      s += e;
-      if (e > 0.f) t += e * d;
+  using Row = RowView<T>;
+  constexpr int kVec = Row::kVec;
+  __shared__ RowSmem sm;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t r = blockIdx.x / CLUSTER;
+  const int rank = blockIdx.x % CLUSTER;
+  const Row row(logits + r * ld, V);
+  // this CTA's vectors [v0, v1)
+  const int v0 = static_cast<int>(static_cast<int64_t>(row.nv) * rank / CLUSTER);
+  const int v1 = static_cast<int>(static_cast<int64_t>(row.nv) * (rank + 1) / CLUSTER);
+  const float a = scale * kLog2e;
+  if (threadIdx.x == 0) sm.nslots = sm.bad = 0;
+
+  // ---- one pass
+  Stats st{-INFINITY, 0.f, 0.f};
+  bool bad = false;
+  // first vector of the batch where st.m was met first; -1: no vectors
+  int best = v0 + static_cast<int>(threadIdx.x) < v1 ? v0 + static_cast<int>(threadIdx.x) : -1;
+  uint64_t s2 = 0, t2 = 0;
+  const uint64_t aa = pair(a, a);
+  auto load = [&](uint4 (&b)[kBatch], int v) {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int at = v + j * kThreads;
+      if (at < v1)
+        b[j] = __ldcs(row.vec(at));
+      else if constexpr (sizeof(T) == 2)
+        b[j] = make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u);
+      else
+        b[j] = make_uint4(0xFF800000u, 0xFF800000u, 0xFF800000u, 0xFF800000u);
     }
-  s = block_reduce(s, redf, add);
-  t = block_reduce(t, redf, add);
-  const float lse = bad > 0.f ? NAN : m + logf(s);
-  const bool empty = m == -INFINITY;
-  if (threadIdx.x == 0) {
-    lse_out[r] = empty && bad == 0.f ? -INFINITY : lse;
-    if (entropy) entropy[r] = bad > 0.f ? NAN : empty ? 0.f : logf(s) - t / s;
-    if (targets) {
-      int g = targets[r];
-      if (g >= V) {
-        if (err) atomicOr(err, GLT_DEVERR_BAD_SHAPE);
-        g = -1;
+  };
+  uint4 cur[kBatch], nxt[kBatch];
+  const bool fast_scale = scale >= 1e-6f && scale <= 1e6f;
+  load(nxt, v0 + threadIdx.x);
+  for (int v = v0 + threadIdx.x; v < v1; v += kBatch * kThreads) {
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) cur[j] = nxt[j];
+    load(nxt, v + kBatch * kThreads);
+    const float cm = vector_max<T>(cur);
+    if (!(cm < INFINITY)) bad = true;
+    if (cm > st.m) {
+      if (st.m > -INFINITY) {
+        const float d = (st.m - cm) * a, f = exp2f(d);
+        float s0, s1, t0, t1;
+        unpair(s2, s0, s1);
+        unpair(t2, t0, t1);
+        s2 = pair(s0 * f, s1 * f);
+        t2 = f > 0.f ? pair(f * fmaf(s0, d, t0), f * fmaf(s1, d, t1)) : 0;
       }
-      logp[r] = g < 0 ? 0.f : bad > 0.f ? NAN : empty ? -INFINITY : load_logit(x + g) * scale - lse;
+      st.m = cm;
+      best = v;
+    }
+    const float ma = st.m * a;
+    if (st.m >= kFloor / 10 && fast_scale) {
+      const uint64_t mm = pair(-ma, -ma);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const uint32_t w[4] = {cur[j].x, cur[j].y, cur[j].z, cur[j].w};
+#pragma unroll
+        for (int q = 0; q < (sizeof(T) == 2 ? 4 : 2); ++q) {
+          uint64_t x;
+          if constexpr (sizeof(T) == 2) {
+            uint32_t c;
+            asm("max.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(w[q]), "r"(0xF149F149u));   // -1e30 in bf16
+            x = pair(bf16_lo(c), bf16_hi(c));
+          } else {
+            x = pair(fmaxf(__uint_as_float(w[2 * q]), kFloor), fmaxf(__uint_as_float(w[2 * q + 1]), kFloor));
+          }
+          const uint64_t d = fma2(x, aa, mm);
+          float d0, d1;
+          unpair(d, d0, d1);
+          const uint64_t e = pair(ex2_approx(d0), ex2_approx(d1));
+          s2 = add2(s2, e);
+          t2 = fma2(e, d, t2);
+        }
+      }
+    } else if (st.m > -INFINITY) {
+      float s0, s1, t0, t1;
+      unpair(s2, s0, s1);
+      unpair(t2, t0, t1);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        float f[kVec];
+        unpack<T>(cur[j], f);
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) {
+          const float d = (f[k] - st.m) * a, e = exp2f(d);
+          s0 += e;
+          if (e > 0.f) t0 = fmaf(e, d, t0);
+        }
+      }
+      s2 = pair(s0, s1);
+      t2 = pair(t0, t1);
     }
   }
-  unsigned long long last = ~0ull;
-  for (int j = 0; j < top; ++j) {
-    unsigned long long best = 0;
-    for (int i = threadIdx.x; i < V; i += kThreads) {
-      const unsigned long long k = rank_key(load_logit(x + i), i);
-      if (k < last && k > best) best = k;
+  {
+    float s0, s1, t0, t1;
+    unpair(s2, s0, s1);
+    unpair(t2, t0, t1);
+    st.s = s0 + s1;
+    st.t = t0 + t1;
+  }
+  // what this thread's vectors can rank: at best (its maximum, first index of the batch), surely
+  // no worse than (its maximum, last index)
+  uint64_t upper = 0, lower = 0;
+  if (top > 0 && best >= 0) {
+    const int last = min(best + (kBatch - 1) * kThreads, v1 - 1);
+    upper = rank_key(st.m, row.head + best * kVec);
+    lower = rank_key(st.m, row.head + last * kVec + kVec - 1);
+  }
+  // elements outside of the vectors: one a thread of the first CTA
+  const int edges = rank == 0 ? row.head + row.tail : 0;
+  uint64_t edge_key = 0;
+  if (threadIdx.x < edges) {
+    const int i = row.edge(threadIdx.x);
+    const float x = logit(row.x + i);
+    if (!(x < INFINITY)) bad = true;
+    edge_key = rank_key(x, i);
+    if (x > -INFINITY) st.join(x, 1.f, 0.f, a);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    st.join(__shfl_xor_sync(0xffffffffu, st.m, o), __shfl_xor_sync(0xffffffffu, st.s, o),
+            __shfl_xor_sync(0xffffffffu, st.t, o), a);
+  bad = __any_sync(0xffffffffu, bad);
+  if (lane == 0) sm.stats[warp] = st;
+  uint64_t least = ~0ull;
+  if (top > 0) {
+    // the q-th largest of the warp's lower keys
+    uint64_t left = lower;
+    for (int q = (top + kWarps - 1) / kWarps; q > 0; --q) {
+      least = left;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const uint64_t k = __shfl_xor_sync(0xffffffffu, least, o);
+        if (k > least) least = k;
+      }
+      if (left == least) left = 0;   // keys are distinct, or 0
     }
-    best = block_reduce(best, redk, [](unsigned long long a, unsigned long long b) { return a > b ? a : b; });
-    last = best;
-    if (threadIdx.x == 0) {
-      const int id = static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(best));
-      top_ids[r * top + j] = id;
-      top_logp[r * top + j] = bad > 0.f ? NAN : empty ? -INFINITY : load_logit(x + id) * scale - lse;
+    if (lane == 0) sm.floor[warp] = least;
+  }
+  __syncthreads();
+  if (lane == 0 && bad) sm.bad = 1;
+  if (top > 0) {
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) least = min(least, sm.floor[w]);
+    if (upper >= least && upper > 0) sm.slots[atomicAdd(&sm.nslots, 1)] = threadIdx.x;
+  }
+  __syncthreads();
+  bad = sm.bad;
+
+  // ---- the most likely tokens of this CTA
+  if (top > 0) {
+    TopList list;
+    if (!bad) {
+      for (int i = warp; i < sm.nslots; i += kWarps) {
+        const int slot = sm.slots[i];
+        for (int v = v0 + slot; v < v1; v += 32 * kThreads) {
+          const int at = v + lane * kThreads;
+          float f[kVec];
+          if (at < v1) unpack<T>(*row.vec(at), f);
+#pragma unroll
+          for (int k = 0; k < kVec; ++k) {
+            uint64_t key = at < v1 ? rank_key(f[k], row.head + at * kVec + k) : 0;
+            if (key < least) key = 0;
+            if (__any_sync(0xffffffffu, key > 0)) list.take(key, top, lane);
+          }
+        }
+      }
+    } else {
+      // NaN or +inf: its threads' maxima say nothing, so every vector is read again
+      for (int v = v0 + warp * 32; v < v1; v += kThreads) {
+        const int at = v + lane;
+        float f[kVec];
+        if (at < v1) unpack<T>(*row.vec(at), f);
+        for (int k = 0; k < kVec; ++k) list.take(at < v1 ? rank_key(f[k], row.head + at * kVec + k) : 0, top, lane);
+      }
+    }
+    if (warp == 0) list.take(edge_key, top, lane);   // at most 14, all in the first warp
+    sm.keys[warp][lane] = list.key;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    if (top > 0) {
+      TopList list;
+      list.key = sm.keys[0][lane];
+      for (int w = 1; w < kWarps; ++w) list.take(sm.keys[w][lane], top, lane);
+      sm.cta_keys[lane] = list.key;
+    }
+    if (lane == 0) {
+      Stats all = sm.stats[0];
+      for (int w = 1; w < kWarps; ++w) all.join(sm.stats[w].m, sm.stats[w].s, sm.stats[w].t, a);
+      sm.cta = all;
+      sm.cta_bad = bad;
     }
   }
+  if constexpr (CLUSTER > 1) cg::this_cluster().sync();
+  if (rank == 0 && warp == 0) {
+    __syncwarp();
+    Stats all = sm.cta;
+    TopList list;
+    if (top > 0) list.key = sm.cta_keys[lane];
+    if constexpr (CLUSTER > 1) {
+      for (int c = 1; c < CLUSTER; ++c) {
+        const RowSmem* o = cg::this_cluster().map_shared_rank(&sm, c);
+        all.join(o->cta.m, o->cta.s, o->cta.t, a);
+        if (o->cta_bad) bad = true;
+        if (top > 0) list.take(o->cta_keys[lane], top, lane);
+      }
+    }
+    const bool empty = all.m == -INFINITY;
+    const float ls = logf(all.s);
+    const float lse = bad ? NAN : empty ? -INFINITY : fmaf(all.m, scale, ls);
+    // log probability of a logit: the difference to the maximum first, so that nothing large cancels
+    auto log_p = [&](float x) { return bad ? NAN : empty ? -INFINITY : (x - all.m) * scale - ls; };
+    if (lane == 0) {
+      lse_out[r] = lse;
+      if (entropy) entropy[r] = bad ? NAN : empty ? 0.f : fmaf(-kLn2, all.t / all.s, ls);
+      if (targets) {
+        int g = targets[r];
+        if (g >= V) {
+          if (err) atomicOr(err, GLT_DEVERR_BAD_SHAPE);
+          g = -1;
+        }
+        logp[r] = g < 0 ? 0.f : log_p(logit(row.x + g));
+      }
+    }
+    if (lane < top) {
+      const uint32_t id = key_index(list.key);
+      top_ids[r * top + lane] = static_cast<int32_t>(id);
+      top_logp[r * top + lane] = log_p(logit(row.x + id));
+    }
+  }
+  if constexpr (CLUSTER > 1) cg::this_cluster().sync();   // the others' shared memory was read
+}
+
+// Rows from the last one back: right after the forward, L2 still holds those.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(
+    const T* logits, int64_t ld, int rows, int V, const int32_t* __restrict__ targets, float scale,
+    const float* __restrict__ lse, const float* __restrict__ entropy, const float* __restrict__ d_logp,
+    const float* __restrict__ d_entropy, T* dlogits, int64_t ld_d) {
+  constexpr int kVec = 16 / sizeof(T);
+  const int64_t r = rows - 1 - static_cast<int64_t>(blockIdx.x);
+  const int g = targets ? targets[r] : -1;
+  const bool given = g >= 0 && g < V;
+  const float dl = d_logp && given ? d_logp[r] : 0.f;
+  const float de = d_entropy ? d_entropy[r] : 0.f;
+  const float l = lse[r], h = d_entropy ? entropy[r] : 0.f;
+  const float base = fmaf(de, h, dl);   // dl + de * (log p + H) = base + de * log p
+  // log p = z - lse; 0 where p is (log p may be -inf there)
+  auto grad = [&](float x) {
+    const float lp = fmaf(x, scale, -l);
+    const float p = exp2f(lp * kLog2e);
+    return p == 0.f || l == -INFINITY ? 0.f : -scale * p * fmaf(de, lp, base);
+  };
+  const RowView<T> row(logits + r * ld, V);
+  T* out = dlogits + r * ld_d;
+  const int step = gridDim.y * kThreads;
+  const int first = blockIdx.y * kThreads + threadIdx.x;
+  auto one = [&](int i) { put(out + i, grad(logit(row.x + i)) + (i == g && l != -INFINITY ? scale * dl : 0.f)); };
+  if (((reinterpret_cast<uintptr_t>(row.x) ^ reinterpret_cast<uintptr_t>(out)) & 15) != 0) {
+    for (int i = first; i < V; i += step) one(i);   // no common vectors
+    return;
+  }
+  const int hot = given && l != -INFINITY ? g - row.head : -1;
+  for (int v = first; v < row.nv; v += kBatch * step) {
+    uint4 b[kBatch];
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j)
+      if (v + j * step < row.nv) b[j] = __ldcs(row.vec(v + j * step));
+#pragma unroll
+    for (int j = 0; j < kBatch; ++j) {
+      const int at = v + j * step;
+      if (at >= row.nv) break;
+      float f[kVec];
+      unpack<T>(b[j], f);
+#pragma unroll
+      for (int k = 0; k < kVec; ++k) f[k] = grad(f[k]);
+      if (hot >= 0 && hot / kVec == at)
+#pragma unroll
+        for (int k = 0; k < kVec; ++k)
+          if (hot - at * kVec == k) f[k] += scale * dl;
+      uint4 u;
+      if constexpr (sizeof(T) == 2)
+        u = make_uint4(pack_bf16x2_rn(f[0], f[1]), pack_bf16x2_rn(f[2], f[3]), pack_bf16x2_rn(f[4], f[5]), pack_bf16x2_rn(f[6], f[7]));
+      else
+        u = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+      __stcs(reinterpret_cast<uint4*>(out + row.head) + at, u);
+    }
+  }
+  if (first < row.head + row.tail) one(row.edge(first));
+}
+
+int check(const void* logits, int dtype, int64_t ld, int rows, int V, float scale) {
+  if (dtype != 0 && dtype != 1) return fail(GLT_EINVAL, "token_logprobs: dtype %d (0 fp32, 1 bf16)", dtype);
+  if (rows < 0 || V < 1 || ld < V) return fail(GLT_EINVAL, "token_logprobs: rows %d, V %d, ld %lld", rows, V, (long long)ld);
+  if (!(scale > 0.f) || !(scale <= FLT_MAX)) return fail(GLT_EINVAL, "token_logprobs: scale must be positive and finite");
+  if (reinterpret_cast<uintptr_t>(logits) % (dtype ? 2 : 4)) return fail(GLT_EINVAL, "token_logprobs: logits not aligned to their type");
+  return GLT_OK;
+}
+
+struct Args {
+  const void* logits;
+  int64_t ld;
+  int rows, V;
+  const int32_t* targets;
+  float scale;
+  int top;
+  float *logp, *entropy, *lse;
+  int32_t* top_ids;
+  float* top_logp;
+};
+
+template <typename T, int CLUSTER>
+int launch_forward(const Args& f, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(f.rows) * CLUSTER);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = CLUSTER;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  GLT_CUDA_TRY(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, CLUSTER>, static_cast<const T*>(f.logits), f.ld, f.V,
+                                  f.targets, f.scale, f.top, f.logp, f.entropy, f.lse, f.top_ids, f.top_logp,
+                                  device_error_word()));
+  GLT_LAUNCH_CHECK();
+  return GLT_OK;
+}
+
+// CTAs a row: while the rows alone leave SMs idle, as long as each CTA keeps two batches a thread.
+template <typename T>
+int forward(const Args& f, cudaStream_t st) {
+  const int64_t batch = static_cast<int64_t>(kBatch) * kThreads * 16 / sizeof(T);
+  int c = 1;
+  while (c < 8 && static_cast<int64_t>(f.rows) * c < num_sms() && f.V >= 4 * c * batch) c *= 2;
+  if (c == 8) return launch_forward<T, 8>(f, st);
+  if (c == 4) return launch_forward<T, 4>(f, st);
+  if (c == 2) return launch_forward<T, 2>(f, st);
+  return launch_forward<T, 1>(f, st);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(
-    const T* logits, int64_t ld, int V, const int32_t* __restrict__ targets, float scale,
-    const float* __restrict__ lse, const float* __restrict__ entropy, const float* __restrict__ d_logp,
-    const float* __restrict__ d_entropy, T* dlogits, int64_t ld_d) {
-  const int64_t r = blockIdx.x;
-  const int g = targets ? targets[r] : -1;
-  const float dl = (d_logp && g >= 0 && g < V) ? d_logp[r] : 0.f;
-  const float de = d_entropy ? d_entropy[r] : 0.f;
-  const float l = lse[r], h = d_entropy ? entropy[r] : 0.f;
-  for (int i = threadIdx.x; i < V; i += kThreads) {
-    const float z = load_logit(logits + r * ld + i) * scale;
-    float d = 0.f;
-    if (l != -INFINITY) {
-      const float lp = z - l, p = expf(lp);
-      d = p == 0.f ? 0.f : -p * (dl + de * (lp + h));
-      if (i == g) d += dl;
-    }
-    store_logit(dlogits + r * ld_d + i, d * scale);
-  }
+int backward(const void* logits, int64_t ld, int rows, int V, const int32_t* targets, float scale, const float* lse,
+             const float* entropy, const float* d_logp, const float* d_entropy, void* dlogits, int64_t ld_d, cudaStream_t st) {
+  // CTAs a row: enough for all SMs, each with a batch a thread
+  const int64_t batch = static_cast<int64_t>(kBatch) * kThreads * 16 / sizeof(T);
+  int64_t y = (8ll * num_sms() + rows - 1) / rows;
+  const int64_t most = (V + batch - 1) / batch;
+  if (y > most) y = most;
+  if (y > 65535) y = 65535;
+  token_logprobs_bwd_kernel<T><<<dim3(rows, static_cast<unsigned>(y)), kThreads, 0, st>>>(
+      static_cast<const T*>(logits), ld, rows, V, targets, scale, lse, entropy, d_logp, d_entropy,
+      static_cast<T*>(dlogits), ld_d);
+  GLT_LAUNCH_CHECK();
+  return GLT_OK;
 }
 
 }  // namespace
@@ -132,27 +540,17 @@ extern "C" int glt_token_logprobs(const void* logits, int dtype, int64_t ld, int
                                   float* entropy, float* lse, int32_t* top_ids, float* top_logp,
                                   void* stream) {
   if (rows > 0 && (!logits || !lse)) return glt::fail(GLT_EINVAL, "null argument");
-  if (dtype != 0 && dtype != 1) return glt::fail(GLT_EINVAL, "token_logprobs: dtype %d (0 fp32, 1 bf16)", dtype);
-  if (rows < 0 || V < 1 || ld < V) return glt::fail(GLT_EINVAL, "token_logprobs: rows %d, V %d, ld %lld", rows, V, (long long)ld);
-  if (!(scale > 0.f) || !(scale <= FLT_MAX)) return glt::fail(GLT_EINVAL, "token_logprobs: scale must be positive and finite");
+  GLT_TRY(glt::check(logits, dtype, ld, rows, V, scale));
+  if (rows > INT_MAX / 8) return glt::fail(GLT_EINVAL, "token_logprobs: rows %d (at most %d)", rows, INT_MAX / 8);
   if (top < 0 || top > glt::kMaxTop || top > V)
     return glt::fail(GLT_EINVAL, "token_logprobs: top %d (0..%d, at most V)", top, glt::kMaxTop);
   if (rows > 0 && top > 0 && (!top_ids || !top_logp)) return glt::fail(GLT_EINVAL, "token_logprobs: top without outputs");
   if (rows > 0 && (targets != nullptr) != (logp != nullptr))
     return glt::fail(GLT_EINVAL, "token_logprobs: targets and logp go together");
-  if (reinterpret_cast<uintptr_t>(logits) % (dtype ? 2 : 4))
-    return glt::fail(GLT_EINVAL, "token_logprobs: logits not aligned to their type");
   if (rows == 0) return GLT_OK;
-  unsigned int* err = glt::device_error_word();
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype)
-    glt::token_logprobs_kernel<<<rows, glt::kThreads, 0, st>>>(
-        static_cast<const uint16_t*>(logits), ld, V, targets, scale, top, logp, entropy, lse, top_ids, top_logp, err);
-  else
-    glt::token_logprobs_kernel<<<rows, glt::kThreads, 0, st>>>(
-        static_cast<const float*>(logits), ld, V, targets, scale, top, logp, entropy, lse, top_ids, top_logp, err);
-  GLT_LAUNCH_CHECK();
-  return GLT_OK;
+  const glt::Args f{logits, ld, rows, V, targets, scale, top, logp, entropy, lse, top_ids, top_logp};
+  return dtype ? glt::forward<uint16_t>(f, static_cast<cudaStream_t>(stream))
+               : glt::forward<float>(f, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int glt_token_logprobs_bwd(const void* logits, int dtype, int64_t ld, int rows, int V,
@@ -161,25 +559,16 @@ extern "C" int glt_token_logprobs_bwd(const void* logits, int dtype, int64_t ld,
                                       const float* d_entropy, void* dlogits, int64_t ld_d,
                                       void* stream) {
   if (rows > 0 && (!logits || !lse || !dlogits)) return glt::fail(GLT_EINVAL, "null argument");
-  if (dtype != 0 && dtype != 1) return glt::fail(GLT_EINVAL, "token_logprobs: dtype %d (0 fp32, 1 bf16)", dtype);
-  if (rows < 0 || V < 1 || ld < V || ld_d < V)
-    return glt::fail(GLT_EINVAL, "token_logprobs: rows %d, V %d, ld %lld, ld_d %lld", rows, V, (long long)ld, (long long)ld_d);
-  if (!(scale > 0.f) || !(scale <= FLT_MAX)) return glt::fail(GLT_EINVAL, "token_logprobs: scale must be positive and finite");
+  GLT_TRY(glt::check(logits, dtype, ld, rows, V, scale));
+  if (ld_d < V) return glt::fail(GLT_EINVAL, "token_logprobs: ld_d %lld below V %d", (long long)ld_d, V);
   if (d_logp && !targets) return glt::fail(GLT_EINVAL, "token_logprobs: d_logp without targets");
   if (d_entropy && !entropy) return glt::fail(GLT_EINVAL, "token_logprobs: d_entropy without the forward's entropy");
-  if (reinterpret_cast<uintptr_t>(logits) % (dtype ? 2 : 4) || reinterpret_cast<uintptr_t>(dlogits) % (dtype ? 2 : 4))
-    return glt::fail(GLT_EINVAL, "token_logprobs: buffers not aligned to their type");
+  if (reinterpret_cast<uintptr_t>(dlogits) % (dtype ? 2 : 4))
+    return glt::fail(GLT_EINVAL, "token_logprobs: dlogits not aligned to their type");
   if (logits == dlogits && ld != ld_d) return glt::fail(GLT_EINVAL, "token_logprobs: in place needs ld = ld_d");
   if (rows == 0) return GLT_OK;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype)
-    glt::token_logprobs_bwd_kernel<<<rows, glt::kThreads, 0, st>>>(
-        static_cast<const uint16_t*>(logits), ld, V, targets, scale, lse, entropy, d_logp, d_entropy,
-        static_cast<uint16_t*>(dlogits), ld_d);
-  else
-    glt::token_logprobs_bwd_kernel<<<rows, glt::kThreads, 0, st>>>(
-        static_cast<const float*>(logits), ld, V, targets, scale, lse, entropy, d_logp, d_entropy,
-        static_cast<float*>(dlogits), ld_d);
-  GLT_LAUNCH_CHECK();
-  return GLT_OK;
+    return glt::backward<uint16_t>(logits, ld, rows, V, targets, scale, lse, entropy, d_logp, d_entropy, dlogits, ld_d, st);
+  return glt::backward<float>(logits, ld, rows, V, targets, scale, lse, entropy, d_logp, d_entropy, dlogits, ld_d, st);
 }
