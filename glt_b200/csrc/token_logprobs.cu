@@ -4,9 +4,9 @@
 // With z = scale x, the running maximum m and the sums s = sum 2^d, t = sum 2^d d of
 // d = (z - m) / ln 2:  lse = m + ln s,  entropy = ln s - ln 2 t / s.  One pass over the
 // logits finds all three, and the maximum that each thread meets on the way decides
-// where the most likely tokens can be: the q-th largest of every warp's 32 maxima,
-// q = ceil(top / warps), taken least over the warps, has `top` logits at or above it,
-// so only the threads' shares whose maximum reaches it are read again (from L2).
+// where the most likely tokens can be: the `top`-th largest of the threads' maxima has
+// `top` logits at or above it, so only the shares of the threads whose maximum reaches
+// it (about `top` of 256) are read again, from L2.
 //
 // HBM bounds both kernels: the forward reads the logits once, the backward reads and
 // writes them once.  An element costs the forward about five instructions, one of them
@@ -134,9 +134,30 @@ struct Stats {
   }
 };
 
+// The larger (or smaller) of a lane's key and its partner's.
+__device__ __forceinline__ void exchange(uint64_t& key, int partner, bool larger) {
+  const uint64_t o = __shfl_xor_sync(0xffffffffu, key, partner);
+  if ((o > key) == larger) key = o;
+}
+
 // The largest keys a warp has seen, one a lane in falling order (0: none).
 struct TopList {
   uint64_t key = 0;
+  // Takes another falling list (`other`: this lane's entry).
+  __device__ __forceinline__ void merge(uint64_t other, int lane) {
+    const uint64_t o = __shfl_sync(0xffffffffu, other, 31 - lane);
+    if (o > key) key = o;   // the 32 largest of both, rising then falling
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) exchange(key, d, (lane & d) == 0);
+  }
+  // Takes 32 keys in any order.
+  __device__ __forceinline__ void merge_unsorted(uint64_t other, int lane) {
+#pragma unroll
+    for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+      for (int d = n >> 1; d > 0; d >>= 1) exchange(other, d, ((lane & d) == 0) == ((lane & n) == 0 || n == 32));
+    merge(other, lane);
+  }
   // Takes every lane's candidate (0: none) that ranks above the top-th.
   __device__ __forceinline__ void take(uint64_t cand, int top, int lane) {
     uint32_t who = __ballot_sync(0xffffffffu, cand > __shfl_sync(0xffffffffu, key, top - 1));
@@ -152,12 +173,18 @@ struct TopList {
   }
 };
 
+constexpr int kPick = (kMaxTop + kWarps - 1) / kWarps + 2;   // maxima a warp puts forward
+constexpr int kCand = 256;                                   // logits that reach `least`, before the slow way
 struct RowSmem {
   Stats stats[kWarps];
-  uint64_t floor[kWarps];
-  uint64_t keys[kWarps][kMaxTop];
+  uint64_t least;                  // a key that `top` logits of this CTA reach (0: there may be fewer)
+  union {
+    uint64_t maxima[kWarps * kPick];
+    uint64_t cand[kCand];
+    uint64_t lists[kWarps][32];
+  };
   unsigned char slots[kThreads];   // threads whose share is read again
-  int nslots, bad;
+  int nslots, ncand, bad;
   // joined over the cluster by its first CTA
   Stats cta;
   int cta_bad;
@@ -180,7 +207,10 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(
   const int v0 = static_cast<int>(static_cast<int64_t>(row.nv) * rank / CLUSTER);
   const int v1 = static_cast<int>(static_cast<int64_t>(row.nv) * (rank + 1) / CLUSTER);
   const float a = scale * kLog2e;
-  if (threadIdx.x == 0) sm.nslots = sm.bad = 0;
+  if (threadIdx.x == 0) {
+    sm.nslots = sm.ncand = sm.bad = 0;
+    sm.least = 0;
+  }
 
   // ---- one pass
   Stats st{-INFINITY, 0.f, 0.f};
@@ -194,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(
     for (int j = 0; j < kBatch; ++j) {
       const int at = v + j * kThreads;
       if (at < v1)
-        b[j] = __ldcs(row.vec(at));
+        b[j] = *row.vec(at);
       else if constexpr (sizeof(T) == 2)
         b[j] = make_uint4(0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u, 0xFF80FF80u);
       else
@@ -296,69 +326,82 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(
             __shfl_xor_sync(0xffffffffu, st.t, o), a);
   bad = __any_sync(0xffffffffu, bad);
   if (lane == 0) sm.stats[warp] = st;
-  uint64_t least = ~0ull;
+  // every warp's few largest lower keys
+  const int pick = (top + kWarps - 1) / kWarps + 2;
   if (top > 0) {
-    // the q-th largest of the warp's lower keys
     uint64_t left = lower;
-    for (int q = (top + kWarps - 1) / kWarps; q > 0; --q) {
-      least = left;
+    for (int q = 0; q < pick; ++q) {
+      uint64_t most = left;
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t k = __shfl_xor_sync(0xffffffffu, least, o);
-        if (k > least) least = k;
+        const uint64_t k = __shfl_xor_sync(0xffffffffu, most, o);
+        if (k > most) most = k;
       }
-      if (left == least) left = 0;   // keys are distinct, or 0
+      if (left == most) left = 0;   // keys are distinct, or 0
+      if (lane == 0) sm.maxima[warp * pick + q] = most;
     }
-    if (lane == 0) sm.floor[warp] = least;
   }
   __syncthreads();
   if (lane == 0 && bad) sm.bad = 1;
-  if (top > 0) {
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) least = min(least, sm.floor[w]);
-    if (upper >= least && upper > 0) sm.slots[atomicAdd(&sm.nslots, 1)] = threadIdx.x;
+  if (top > 0 && threadIdx.x < kWarps * pick) {
+    // the one that top - 1 others exceed
+    const uint64_t mine = sm.maxima[threadIdx.x];
+    int above = 0;
+    for (int i = 0; i < kWarps * pick; ++i) above += sm.maxima[i] > mine;
+    if (above == top - 1 && mine > 0) sm.least = mine;
   }
   __syncthreads();
   bad = sm.bad;
 
   // ---- the most likely tokens of this CTA
   if (top > 0) {
-    TopList list;
+    const uint64_t least = sm.least;
+    if (upper >= least && upper > 0) sm.slots[atomicAdd(&sm.nslots, 1)] = threadIdx.x;
+    __syncthreads();
+    auto offer = [&](uint64_t key) {
+      if (key < least) return;
+      const int at = atomicAdd(&sm.ncand, 1);
+      if (at < kCand) sm.cand[at] = key;
+    };
     if (!bad) {
-      for (int i = warp; i < sm.nslots; i += kWarps) {
-        const int slot = sm.slots[i];
-        for (int v = v0 + slot; v < v1; v += 32 * kThreads) {
-          const int at = v + lane * kThreads;
-          float f[kVec];
-          if (at < v1) unpack<T>(*row.vec(at), f);
+      const int per = (v1 - v0 + kThreads - 1) / kThreads;
+      for (int i = threadIdx.x; i < sm.nslots * per; i += kThreads) {
+        const int slot = i / per, at = v0 + sm.slots[slot] + (i - slot * per) * kThreads;
+        if (at >= v1) continue;
+        float f[kVec];
+        unpack<T>(*row.vec(at), f);
 #pragma unroll
-          for (int k = 0; k < kVec; ++k) {
-            uint64_t key = at < v1 ? rank_key(f[k], row.head + at * kVec + k) : 0;
-            if (key < least) key = 0;
-            if (__any_sync(0xffffffffu, key > 0)) list.take(key, top, lane);
-          }
-        }
+        for (int k = 0; k < kVec; ++k) offer(rank_key(f[k], row.head + at * kVec + k));
       }
-    } else {
-      // NaN or +inf: its threads' maxima say nothing, so every vector is read again
+      if (threadIdx.x < edges) offer(edge_key);
+    }
+    __syncthreads();
+    const int n = sm.ncand;
+    if (bad || n > kCand) {
+      // more equal logits than places, or NaN or +inf, where the maxima say nothing: every vector again
+      __syncthreads();   // `lists` takes the place of `cand`
+      TopList list;
       for (int v = v0 + warp * 32; v < v1; v += kThreads) {
         const int at = v + lane;
         float f[kVec];
         if (at < v1) unpack<T>(*row.vec(at), f);
+#pragma unroll
         for (int k = 0; k < kVec; ++k) list.take(at < v1 ? rank_key(f[k], row.head + at * kVec + k) : 0, top, lane);
       }
-    }
-    if (warp == 0) list.take(edge_key, top, lane);   // at most 14, all in the first warp
-    sm.keys[warp][lane] = list.key;
-  }
-  __syncthreads();
-  if (warp == 0) {
-    if (top > 0) {
+      if (warp == 0) list.take(edge_key, top, lane);   // the edges are all in the first warp
+      sm.lists[warp][lane] = list.key;
+      __syncthreads();
+      if (warp == 0) {
+        for (int w = 1; w < kWarps; ++w) list.merge(sm.lists[w][lane], lane);
+        sm.cta_keys[lane] = list.key;
+      }
+    } else if (warp == 0) {
       TopList list;
-      list.key = sm.keys[0][lane];
-      for (int w = 1; w < kWarps; ++w) list.take(sm.keys[w][lane], top, lane);
+      for (int i = 0; i < n; i += 32) list.merge_unsorted(i + lane < n ? sm.cand[i + lane] : 0, lane);
       sm.cta_keys[lane] = list.key;
     }
+  }
+  if (warp == 0) {
     if (lane == 0) {
       Stats all = sm.stats[0];
       for (int w = 1; w < kWarps; ++w) all.join(sm.stats[w].m, sm.stats[w].s, sm.stats[w].t, a);
@@ -373,11 +416,19 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(
     TopList list;
     if (top > 0) list.key = sm.cta_keys[lane];
     if constexpr (CLUSTER > 1) {
+      Stats part[CLUSTER];
+      uint64_t keys[CLUSTER];
+#pragma unroll
       for (int c = 1; c < CLUSTER; ++c) {
         const RowSmem* o = cg::this_cluster().map_shared_rank(&sm, c);
-        all.join(o->cta.m, o->cta.s, o->cta.t, a);
+        part[c] = o->cta;
         if (o->cta_bad) bad = true;
-        if (top > 0) list.take(o->cta_keys[lane], top, lane);
+        keys[c] = top > 0 ? o->cta_keys[lane] : 0;
+      }
+#pragma unroll
+      for (int c = 1; c < CLUSTER; ++c) {
+        all.join(part[c].m, part[c].s, part[c].t, a);
+        if (top > 0) list.merge(keys[c], lane);
       }
     }
     const bool empty = all.m == -INFINITY;
