@@ -10,10 +10,13 @@
 // Register i of the fragment (row half i % 2, column pair i / 2) takes its two codes
 // from bits 4i + 3 .. 4i + 6 and 16 further up (modulo 32): a rotation by 4i brings
 // them to mantissa bits 3..6 of two bf16 numbers 1 + code / 16, exactly.
+#include <cooperative_groups.h>
 #include <math.h>
 
 #include "common.cuh"
 #include "gemm.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace glt {
 namespace {
@@ -144,72 +147,217 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// The same from sums of 0.
+__device__ __forceinline__ void mma_bf16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
   uint32_t r;
   asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
   return r;
 }
 
-// y = x . W^T for 8 rows of x: a warp takes one tile of 16 weight rows and walks its chunks.
-__global__ void __launch_bounds__(128) w4_linear_kernel(const uint8_t* __restrict__ packed, W4Layout L,
-                                                        const uint16_t* __restrict__ x, int64_t ld_x, int M,
-                                                        void* __restrict__ y, int64_t ld_y, int y_bf16,
-                                                        const uint16_t* __restrict__ resid, int64_t ld_r) {
-  const int64_t tile = blockIdx.x * 4ll + (threadIdx.x >> 5);
-  if (tile >= L.tiles) return;
-  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
-  const int m = blockIdx.y * 8 + g;
-  const uint4* cw = reinterpret_cast<const uint4*>(packed) + tile * L.chunks * 32 + lane;
-  const uint32_t* sw = reinterpret_cast<const uint32_t*>(packed + L.scale_off) + tile * L.groups * 8 + g;
-  const uint16_t* zw = reinterpret_cast<const uint16_t*>(packed + L.zero_off) + tile * L.groups * 8 + g;
-  float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int ch = 0; ch < L.chunks; ++ch) {
-    const uint4 v = cw[ch * 32];
-    const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+struct LinearArgs {
+  const uint8_t* packed;
+  W4Layout L;
+  const uint16_t* x;
+  int64_t ld_x;
+  int M;
+  void* y;
+  int64_t ld_y;
+  int y_bf16;
+  const uint16_t* resid;
+  int64_t ld_r;
+};
+
+constexpr int kLinWarps = 4;
+constexpr int kLinThreads = 32 * kLinWarps;
+
+// y = x . W^T for up to 8 NT rows of x: the weights are operand A (16 rows by 16 columns),
+// the rows of x operand B (N = 8).  A cluster of S CTAs takes 16 TILES rows of W; its CTAs
+// split the columns, and a CTA's warps take the chunks of its part in turn, TILES tiles at
+// once so that a fragment of x serves them all.  Partial sums meet in shared memory, then
+// over the cluster, in a fixed order.
+template <int NT, int TILES, bool ASYM, bool G32>
+__global__ void __launch_bounds__(kLinThreads) w4_linear_kernel(const __grid_constant__ LinearArgs a) {
+  constexpr int kAhead = TILES == 1 ? 6 : TILES == 2 ? 3 : 2;   // chunks on their way
+  constexpr int kRows = 16 * TILES, kCols = 8 * NT, kOut = kRows * kCols;
+  extern __shared__ float red[];   // [warp][column][row], then the CTA's sums
+  cg::cluster_group cluster = cg::this_cluster();
+  const int S = cluster.num_blocks(), rank = cluster.block_rank();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const W4Layout& L = a.L;
+  const int tile0 = static_cast<int>(blockIdx.x / S) * TILES;
+  const int m0 = blockIdx.y * kCols;
+  const int ch0 = static_cast<int>(static_cast<int64_t>(L.chunks) * rank / S);
+  const int ch1 = static_cast<int>(static_cast<int64_t>(L.chunks) * (rank + 1) / S);
+  const int group_log = 31 - __clz(L.group);
+
+  // tiles past the last one repeat it; nothing of theirs is written
+  const uint4* cw[TILES];
+  const uint32_t* sw[TILES];
+  const uint16_t* zw[TILES];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int k = ch * 64 + half * 32;
-      if (k >= L.K) break;
-      uint4 xv = make_uint4(0, 0, 0, 0);
-      if (m < M) xv = *reinterpret_cast<const uint4*>(x + m * ld_x + k + c * 8);
-      const uint32_t b[4] = {xv.x, xv.y, xv.z, xv.w};
-      const int grp = k / L.group;
-      const uint32_t sc = sw[grp * 8];
-      // 1 + zero / 16 of rows g and g + 8, twice each
-      uint32_t z0 = 0x3FC03FC0u, z1 = 0x3FC03FC0u;
-      if (L.asym) {
-        const uint32_t z = zw[grp * 8];
-        z0 = (0x3F80u | ((z & 15u) << 3)) * 0x10001u;
-        z1 = (0x3F80u | (((z >> 8) & 15u) << 3)) * 0x10001u;
+  for (int t = 0; t < TILES; ++t) {
+    const int64_t tile = min(tile0 + t, L.tiles - 1);
+    cw[t] = reinterpret_cast<const uint4*>(a.packed) + tile * L.chunks * 32 + lane;
+    sw[t] = reinterpret_cast<const uint32_t*>(a.packed + L.scale_off) + tile * L.groups * 8 + g;
+    zw[t] = reinterpret_cast<const uint16_t*>(a.packed + L.zero_off) + tile * L.groups * 8 + g;
+  }
+  const uint16_t* xr[NT];
+  bool has[NT];
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    has[n] = m0 + n * 8 + g < a.M;
+    xr[n] = a.x + (has[n] ? m0 + n * 8 + g : 0) * a.ld_x + c * 8;
+  }
+
+  constexpr int kHalves = G32 ? 2 : 1;   // groups a chunk touches
+  struct Chunk {
+    uint4 w[TILES];
+    uint32_t sc[TILES][kHalves], z[TILES][kHalves];
+    uint4 x[NT][2];
+  };
+  Chunk ahead[kAhead];
+  auto load = [&](Chunk& k, int ch) {
+    if (ch >= ch1) return;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      k.w[t] = __ldcs(cw[t] + ch * 32);
+#pragma unroll
+      for (int h = 0; h < kHalves; ++h) {
+        const int grp = (ch * 64 + h * 32) >> group_log;
+        k.sc[t][h] = sw[t][grp * 8];
+        if (ASYM) k.z[t][h] = zw[t][grp * 8];
       }
-      float part[4] = {0.f, 0.f, 0.f, 0.f};
+    }
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        uint32_t a[4];
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        k.x[n][h] = has[n] && ch * 64 + h * 32 < L.K ? *reinterpret_cast<const uint4*>(xr[n] + ch * 64 + h * 32)
+                                                     : make_uint4(0, 0, 0, 0);
+  };
+
+  float acc[TILES][NT][4] = {};
+  auto use = [&](const Chunk& k) {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      const uint32_t word[4] = {k.w[t].x, k.w[t].y, k.w[t].z, k.w[t].w};
+      float part[NT][4];
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const int h = G32 ? s >> 1 : 0;
+        // 1 + zero / 16 of rows g and g + 8, twice each
+        uint32_t z0 = 0x3FC03FC0u, z1 = 0x3FC03FC0u;
+        if (ASYM) {
+          z0 = (0x3F80u | ((k.z[t][h] & 15u) << 3)) * 0x10001u;
+          z1 = (0x3F80u | (((k.z[t][h] >> 8) & 15u) << 3)) * 0x10001u;
+        }
+        uint32_t f[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const uint32_t t = __funnelshift_r(word[half * 2 + s], word[half * 2 + s], 4 * i);
-          a[i] = sub_bf16x2((t & 0x00780078u) | 0x3F803F80u, (i & 1) ? z1 : z0);
+          const uint32_t r = __funnelshift_r(word[s], word[s], 4 * i);
+          f[i] = sub_bf16x2((r & 0x00780078u) | 0x3F803F80u, (i & 1) ? z1 : z0);
         }
-        mma_bf16(part, a, b[2 * s], b[2 * s + 1]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const uint4& x = k.x[n][s >> 1];
+          const uint32_t b0 = s & 1 ? x.z : x.x, b1 = s & 1 ? x.w : x.y;
+          if (s == 0 || (G32 && s == 2))
+            mma_bf16_zero(part[n], f, b0, b1);
+          else
+            mma_bf16(part[n], f, b0, b1);
+        }
+        if (s == 3 || (G32 && s == 1)) {
+          const float s0 = bf16_lo(k.sc[t][h]), s1 = bf16_hi(k.sc[t][h]);
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            acc[t][n][0] = fmaf(s0, part[n][0], acc[t][n][0]);
+            acc[t][n][1] = fmaf(s0, part[n][1], acc[t][n][1]);
+            acc[t][n][2] = fmaf(s1, part[n][2], acc[t][n][2]);
+            acc[t][n][3] = fmaf(s1, part[n][3], acc[t][n][3]);
+          }
+        }
       }
-      const float s0 = 16.f * bf16_lo(sc), s1 = 16.f * bf16_hi(sc);
-      acc[0] += s0 * part[0];
-      acc[1] += s0 * part[1];
-      acc[2] += s1 * part[2];
-      acc[3] += s1 * part[3];
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < kAhead; ++d) load(ahead[d], ch0 + warp + d * kLinWarps);
+  for (int ch = ch0 + warp; ch < ch1; ch += kAhead * kLinWarps) {
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) {
+      const int at = ch + d * kLinWarps;
+      if (at >= ch1) break;
+      use(ahead[d]);
+      load(ahead[d], at + kAhead * kLinWarps);
     }
   }
+
+  // ---- join the warps, then the cluster
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int64_t n = tile * 16 + g + 8 * (q >> 1), row = blockIdx.y * 8 + 2 * c + (q & 1);
-    if (n >= L.N || row >= M) continue;
-    const float o = acc[q] + (resid ? bf16_bits_to_f32(resid[row * ld_r + n]) : 0.f);
-    if (y_bf16)
-      static_cast<uint16_t*>(y)[row * ld_y + n] = bf16_bits_rn(o);
+  for (int t = 0; t < TILES; ++t)
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        red[warp * kOut + (n * 8 + 2 * c + (q & 1)) * kRows + t * 16 + g + 8 * (q >> 1)] = acc[t][n][q];
+  __syncthreads();
+  for (int e = threadIdx.x; e < kOut; e += kLinThreads)
+    red[e] = (red[e] + red[kOut + e]) + (red[2 * kOut + e] + red[3 * kOut + e]);
+  if (S > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  const int e0 = kOut * rank / S, e1 = kOut * (rank + 1) / S;
+  for (int e = e0 + threadIdx.x; e < e1; e += kLinThreads) {
+    const int m = m0 + e / kRows;
+    const int64_t n = static_cast<int64_t>(tile0) * 16 + e % kRows;
+    float o = 0.f;
+    for (int r = 0; r < S; ++r) o += S > 1 ? cluster.map_shared_rank(red, r)[e] : red[e];
+    if (m >= a.M || n >= L.N) continue;
+    o *= 16.f;   // the products are of code / 16
+    if (a.resid) o += bf16_bits_to_f32(a.resid[m * a.ld_r + n]);
+    if (a.y_bf16)
+      static_cast<uint16_t*>(a.y)[m * a.ld_y + n] = bf16_bits_rn(o);
     else
-      static_cast<float*>(y)[row * ld_y + n] = o;
+      static_cast<float*>(a.y)[m * a.ld_y + n] = o;
   }
+  if (S > 1) cluster.sync();   // the others have read this CTA's sums
+}
+
+template <int NT, int TILES, bool ASYM, bool G32>
+int launch_linear(const LinearArgs& a, cudaStream_t st) {
+  const auto kernel = w4_linear_kernel<NT, TILES, ASYM, G32>;
+  constexpr int bytes = kLinWarps * 16 * TILES * 8 * NT * 4;
+  const int groups = (a.L.tiles + TILES - 1) / TILES, blocks = (a.M + 8 * NT - 1) / (8 * NT);
+  // CTAs a group of tiles: until the SMs hold six each, while every warp keeps two chunks
+  int S = 1;
+  while (S < 8 && static_cast<int64_t>(groups) * blocks * S < 6ll * num_sms() && a.L.chunks >= 4 * S * kLinWarps) S *= 2;
+  if (blocks > 65535) return fail(GLT_EINVAL, "w4: %d rows", a.M);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(groups) * S, blocks);
+  cfg.blockDim = dim3(kLinThreads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = S;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  GLT_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
+  GLT_LAUNCH_CHECK();
+  return GLT_OK;
+}
+
+template <int NT, int TILES>
+int launch_linear_as(const LinearArgs& a, cudaStream_t st) {
+  if (a.L.group == 32) return a.L.asym ? launch_linear<NT, TILES, true, true>(a, st) : launch_linear<NT, TILES, false, true>(a, st);
+  return a.L.asym ? launch_linear<NT, TILES, true, false>(a, st) : launch_linear<NT, TILES, false, false>(a, st);
 }
 
 int grid_for(int64_t units, int per_cta) {
@@ -277,14 +425,12 @@ extern "C" int glt_w4_linear(const void* packed, int N, int K, int group, int as
   if (ld_y < N || (resid && ld_r < N)) return glt::fail(GLT_EINVAL, "w4: output or residual row stride below N %d", N);
   if (!glt::aligned16(packed)) return glt::fail(GLT_EINVAL, "w4: packed weights must be 16-byte aligned");
   if (M == 0) return GLT_OK;
-  const W4Layout L(N, K, group, asym);
-  for (int m0 = 0; m0 < M; m0 += 8 * 65535) {   // grid.y limit
-    const int rows = M - m0 < 8 * 65535 ? M - m0 : 8 * 65535;
-    glt::w4_linear_kernel<<<dim3((L.tiles + 3) / 4, (rows + 7) / 8), 128, 0, static_cast<cudaStream_t>(stream)>>>(
-        static_cast<const uint8_t*>(packed), L, x + static_cast<int64_t>(m0) * ld_x, ld_x, rows,
-        static_cast<uint8_t*>(y) + static_cast<int64_t>(m0) * ld_y * (y_dtype ? 2 : 4), ld_y, y_dtype,
-        resid ? resid + static_cast<int64_t>(m0) * ld_r : nullptr, ld_r);
-    GLT_LAUNCH_CHECK();
-  }
-  return GLT_OK;
+  const glt::LinearArgs a{static_cast<const uint8_t*>(packed), W4Layout(N, K, group, asym), x, ld_x, M, y, ld_y,
+                          y_dtype, resid, ld_r};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (M <= 2) return glt::launch_linear_as<1, 1>(a, st);
+  if (M <= 8) return glt::launch_linear_as<1, 2>(a, st);
+  if (M <= 16) return glt::launch_linear_as<2, 2>(a, st);
+  if (M <= 24) return glt::launch_linear_as<3, 4>(a, st);
+  return glt::launch_linear_as<4, 4>(a, st);
 }
