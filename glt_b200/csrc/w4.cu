@@ -180,7 +180,7 @@ constexpr int kLinThreads = 32 * kLinWarps;
 // split the columns, and a CTA's warps take the chunks of its part in turn, TILES tiles at
 // once so that a fragment of x serves them all.  Partial sums meet in shared memory, then
 // over the cluster, in a fixed order.
-template <int NT, int TILES, bool ASYM, bool G32>
+template <int NT, int TILES, bool ASYM, int GROUP>
 __global__ void __launch_bounds__(kLinThreads) w4_linear_kernel(const __grid_constant__ LinearArgs a) {
   constexpr int kAhead = TILES == 1 ? 6 : TILES == 2 ? 3 : 2;   // chunks on their way
   constexpr int kRows = 16 * TILES, kCols = 8 * NT, kOut = kRows * kCols;
@@ -193,52 +193,62 @@ __global__ void __launch_bounds__(kLinThreads) w4_linear_kernel(const __grid_con
   const int m0 = blockIdx.y * kCols;
   const int ch0 = static_cast<int>(static_cast<int64_t>(L.chunks) * rank / S);
   const int ch1 = static_cast<int>(static_cast<int64_t>(L.chunks) * (rank + 1) / S);
-  const int group_log = 31 - __clz(L.group);
-
-  // tiles past the last one repeat it; nothing of theirs is written
+  // A warp's chunks are ch0 + warp + kLinWarps j; in step j everything it reads moves on by a
+  // fixed number of bytes.  Tiles past the last one repeat it, rows of x past the last one the
+  // first: nothing of theirs is written.
+  constexpr int kGroups = GROUP == 32 ? 2 : 1;                       // groups a chunk touches
+  constexpr int kGroupStep = kLinWarps * 64 / GROUP;                 // groups from step to step
+  const int first = ch0 + warp;
   const uint4* cw[TILES];
   const uint32_t* sw[TILES];
   const uint16_t* zw[TILES];
 #pragma unroll
   for (int t = 0; t < TILES; ++t) {
     const int64_t tile = min(tile0 + t, L.tiles - 1);
-    cw[t] = reinterpret_cast<const uint4*>(a.packed) + tile * L.chunks * 32 + lane;
-    sw[t] = reinterpret_cast<const uint32_t*>(a.packed + L.scale_off) + tile * L.groups * 8 + g;
-    zw[t] = reinterpret_cast<const uint16_t*>(a.packed + L.zero_off) + tile * L.groups * 8 + g;
+    const int64_t grp = (tile * L.groups + first * 64 / GROUP) * 8 + g;
+    cw[t] = reinterpret_cast<const uint4*>(a.packed) + (tile * L.chunks + first) * 32 + lane;
+    sw[t] = reinterpret_cast<const uint32_t*>(a.packed + L.scale_off) + grp;
+    zw[t] = reinterpret_cast<const uint16_t*>(a.packed + L.zero_off) + grp;
   }
   const uint16_t* xr[NT];
-  bool has[NT];
 #pragma unroll
-  for (int n = 0; n < NT; ++n) {
-    has[n] = m0 + n * 8 + g < a.M;
-    xr[n] = a.x + (has[n] ? m0 + n * 8 + g : 0) * a.ld_x + c * 8;
-  }
+  for (int n = 0; n < NT; ++n)
+    xr[n] = a.x + (m0 + n * 8 + g < a.M ? m0 + n * 8 + g : 0) * a.ld_x + first * 64 + c * 8;
 
-  constexpr int kHalves = G32 ? 2 : 1;   // groups a chunk touches
   struct Chunk {
     uint4 w[TILES];
-    uint32_t sc[TILES][kHalves], z[TILES][kHalves];
+    uint32_t sc[TILES][kGroups], z[TILES][kGroups];
     uint4 x[NT][2];
   };
   Chunk ahead[kAhead];
-  auto load = [&](Chunk& k, int ch) {
-    if (ch >= ch1) return;
+  // Loads the chunk `d` steps on from where the pointers stand.
+  auto load = [&](Chunk& k, int d, bool second_half) {
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
-      k.w[t] = __ldcs(cw[t] + ch * 32);
+      k.w[t] = __ldcs(cw[t] + d * kLinWarps * 32);
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        const int grp = (ch * 64 + h * 32) >> group_log;
-        k.sc[t][h] = sw[t][grp * 8];
-        if (ASYM) k.z[t][h] = zw[t][grp * 8];
+      for (int h = 0; h < kGroups; ++h) {
+        k.sc[t][h] = sw[t][(d * kGroupStep + h) * 8];
+        if (ASYM) k.z[t][h] = zw[t][(d * kGroupStep + h) * 8];
       }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        k.x[n][h] = has[n] && ch * 64 + h * 32 < L.K ? *reinterpret_cast<const uint4*>(xr[n] + ch * 64 + h * 32)
-                                                     : make_uint4(0, 0, 0, 0);
+      for (int h = 0; h < 2; ++h) {
+        k.x[n][h] = make_uint4(0, 0, 0, 0);
+        if (h == 0 || second_half) k.x[n][h] = *reinterpret_cast<const uint4*>(xr[n] + d * kLinWarps * 64 + h * 32);
+      }
+  };
+  auto advance = [&](int d) {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      cw[t] += d * kLinWarps * 32;
+      sw[t] += d * kGroupStep * 8;
+      if (ASYM) zw[t] += d * kGroupStep * 8;
+    }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) xr[n] += d * kLinWarps * 64;
   };
 
   float acc[TILES][NT][4] = {};
@@ -249,7 +259,7 @@ __global__ void __launch_bounds__(kLinThreads) w4_linear_kernel(const __grid_con
       float part[NT][4];
 #pragma unroll
       for (int s = 0; s < 4; ++s) {
-        const int h = G32 ? s >> 1 : 0;
+        const int h = GROUP == 32 ? s >> 1 : 0;
         // 1 + zero / 16 of rows g and g + 8, twice each
         uint32_t z0 = 0x3FC03FC0u, z1 = 0x3FC03FC0u;
         if (ASYM) {
@@ -266,12 +276,12 @@ __global__ void __launch_bounds__(kLinThreads) w4_linear_kernel(const __grid_con
         for (int n = 0; n < NT; ++n) {
           const uint4& x = k.x[n][s >> 1];
           const uint32_t b0 = s & 1 ? x.z : x.x, b1 = s & 1 ? x.w : x.y;
-          if (s == 0 || (G32 && s == 2))
+          if (s == 0 || (GROUP == 32 && s == 2))
             mma_bf16_zero(part[n], f, b0, b1);
           else
             mma_bf16(part[n], f, b0, b1);
         }
-        if (s == 3 || (G32 && s == 1)) {
+        if (s == 3 || (GROUP == 32 && s == 1)) {
           const float s0 = bf16_lo(k.sc[t][h]), s1 = bf16_hi(k.sc[t][h]);
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
@@ -284,16 +294,30 @@ __global__ void __launch_bounds__(kLinThreads) w4_linear_kernel(const __grid_con
       }
     }
   };
+  // Steps of this warp; those before `full` need no check (a last chunk of 32 columns does).
+  const int steps = first < ch1 ? (ch1 - first + kLinWarps - 1) / kLinWarps : 0;
+  const int full_end = min(ch1, L.K / 64);
+  const int full = first < full_end ? (full_end - first + kLinWarps - 1) / kLinWarps : 0;
 #pragma unroll
-  for (int d = 0; d < kAhead; ++d) load(ahead[d], ch0 + warp + d * kLinWarps);
-  for (int ch = ch0 + warp; ch < ch1; ch += kAhead * kLinWarps) {
+  for (int d = 0; d < kAhead; ++d)
+    if (d < steps) load(ahead[d], d, d < full);
+  int j = 0;
+  for (; j + 2 * kAhead <= full; j += kAhead) {
 #pragma unroll
     for (int d = 0; d < kAhead; ++d) {
-      const int at = ch + d * kLinWarps;
-      if (at >= ch1) break;
       use(ahead[d]);
-      load(ahead[d], at + kAhead * kLinWarps);
+      load(ahead[d], kAhead + d, true);
     }
+    advance(kAhead);
+  }
+  for (; j < steps; j += kAhead) {
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) {
+      if (j + d >= steps) break;
+      use(ahead[d]);
+      if (j + kAhead + d < steps) load(ahead[d], kAhead + d, j + kAhead + d < full);
+    }
+    advance(kAhead);
   }
 
   // ---- join the warps, then the cluster
@@ -328,9 +352,9 @@ __global__ void __launch_bounds__(kLinThreads) w4_linear_kernel(const __grid_con
   if (S > 1) cluster.sync();   // the others have read this CTA's sums
 }
 
-template <int NT, int TILES, bool ASYM, bool G32>
+template <int NT, int TILES, bool ASYM, int GROUP>
 int launch_linear(const LinearArgs& a, cudaStream_t st) {
-  const auto kernel = w4_linear_kernel<NT, TILES, ASYM, G32>;
+  const auto kernel = w4_linear_kernel<NT, TILES, ASYM, GROUP>;
   constexpr int bytes = kLinWarps * 16 * TILES * 8 * NT * 4;
   const int groups = (a.L.tiles + TILES - 1) / TILES, blocks = (a.M + 8 * NT - 1) / (8 * NT);
   // CTAs a group of tiles: until the SMs hold six each, while every warp keeps two chunks
@@ -356,8 +380,12 @@ int launch_linear(const LinearArgs& a, cudaStream_t st) {
 
 template <int NT, int TILES>
 int launch_linear_as(const LinearArgs& a, cudaStream_t st) {
-  if (a.L.group == 32) return a.L.asym ? launch_linear<NT, TILES, true, true>(a, st) : launch_linear<NT, TILES, false, true>(a, st);
-  return a.L.asym ? launch_linear<NT, TILES, true, false>(a, st) : launch_linear<NT, TILES, false, false>(a, st);
+  if (a.L.asym) {
+    if (a.L.group == 32) return launch_linear<NT, TILES, true, 32>(a, st);
+    return a.L.group == 64 ? launch_linear<NT, TILES, true, 64>(a, st) : launch_linear<NT, TILES, true, 128>(a, st);
+  }
+  if (a.L.group == 32) return launch_linear<NT, TILES, false, 32>(a, st);
+  return a.L.group == 64 ? launch_linear<NT, TILES, false, 64>(a, st) : launch_linear<NT, TILES, false, 128>(a, st);
 }
 
 int grid_for(int64_t units, int per_cta) {
