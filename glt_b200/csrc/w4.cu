@@ -13,6 +13,8 @@
 #include <cooperative_groups.h>
 #include <math.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "gemm.cuh"
 
@@ -33,9 +35,9 @@ struct W4Layout {
     chunks = (K + 63) / 64;
     groups = static_cast<int>(up(static_cast<int64_t>(chunks) * 64, group) / group);
     scale_off = up(static_cast<int64_t>(tiles) * chunks * 512, 256);
-    // [tile][group][g][row half] bf16, then the zeros as bytes in the same order
+    // [tile][group][g][row half] bf16, then the zeros as bf16 1 + zero / 16 in the same order
     zero_off = up(scale_off + static_cast<int64_t>(tiles) * groups * 32, 256);
-    bytes = zero_off + (asym ? up(static_cast<int64_t>(tiles) * groups * 16, 256) : 0);
+    bytes = zero_off + (asym ? up(static_cast<int64_t>(tiles) * groups * 32, 256) : 0);
   }
 };
 
@@ -119,7 +121,8 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t* __restrict_
     const int64_t n = tile * 16 + ((q >> 1) & 7) + 8 * (q & 1);
     const bool in = n < L.N && grp < ng;
     reinterpret_cast<uint16_t*>(packed + L.scale_off)[q] = in ? scales[n * ng + grp] : 0;
-    if (L.asym) packed[L.zero_off + q] = in ? zeros[n * ng + grp] & 15u : 0;
+    if (L.asym)
+      reinterpret_cast<uint16_t*>(packed + L.zero_off)[q] = 0x3F80u | (in ? (zeros[n * ng + grp] & 15u) << 3 : 0u);
   }
 }
 
@@ -137,7 +140,7 @@ __global__ void __launch_bounds__(256) w4_unpack_kernel(const uint8_t* __restric
     const uint32_t v = reinterpret_cast<const uint32_t*>(packed)[word];
     const float u = static_cast<float>(__funnelshift_r(v, v, b) & 15u);
     const int64_t sc = ((n >> 4) * L.groups + k / L.group) * 16 + (r & 7) * 2 + (r >> 3);
-    const float z = L.asym ? static_cast<float>(packed[L.zero_off + sc]) : 8.f;
+    const float z = L.asym ? static_cast<float>((reinterpret_cast<const uint16_t*>(packed + L.zero_off)[sc] >> 3) & 15u) : 8.f;
     w[n * ld + k] = bf16_bits_rn((u - z) * bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(packed + L.scale_off)[sc]));
   }
 }
@@ -147,11 +150,12 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// The same from sums of 0.
-__device__ __forceinline__ void mma_bf16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+// The same from other sums.
+__device__ __forceinline__ void mma_bf16_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                              float c0, float c1, float c2, float c3) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 __device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -177,12 +181,23 @@ constexpr int kLinThreads = 32 * kLinWarps;
 
 // y = x . W^T for up to 8 NT rows of x: the weights are operand A (16 rows by 16 columns),
 // the rows of x operand B (N = 8).  A cluster of S CTAs takes 16 TILES rows of W; its CTAs
-// split the columns, and a CTA's warps take the chunks of its part in turn, TILES tiles at
-// once so that a fragment of x serves them all.  Partial sums meet in shared memory, then
+// split the columns, and a CTA's warps take the pieces of its part in turn, TILES tiles at
+// once so that a fragment of x serves them all.  A piece is a chunk, or two with groups of
+// 128, so that a group's sums meet its scale once.  Partial sums meet in shared memory, then
 // over the cluster, in a fixed order.
+//
+// Half a byte a weight leaves about 22 cycles of an SM for a tile's chunk, so instructions
+// count.  A register of two weights takes a rotation (three in four) and one AND-OR to become
+// 1 + code / 16.  Taking 1 + zero / 16 off costs one more; with the constant zero 8 it is left
+// to the tensor core: a product with -1.5 everywhere gives -1.5 sum x, from which the sums of
+// every tile start.  (Then |x| counts 1.5 to 1.94 times in 32-bit sums instead of about 0.25
+// times.)  Infinities would not survive that, so a piece of x whose sum is not finite goes
+// the exact way.
 template <int NT, int TILES, bool ASYM, int GROUP>
 __global__ void __launch_bounds__(kLinThreads) w4_linear_kernel(const __grid_constant__ LinearArgs a) {
-  constexpr int kAhead = TILES == 1 ? 6 : TILES == 2 ? 3 : 2;   // chunks on their way
+  constexpr int kSub = GROUP == 128 ? 2 : 1;                    // chunks of a piece
+  constexpr int kGroups = GROUP == 32 ? 2 : 1;                  // groups of a piece
+  constexpr int kAhead = NT == 1 ? 4 / kSub : NT == 2 ? 2 : 1;  // pieces on their way
   constexpr int kRows = 16 * TILES, kCols = 8 * NT, kOut = kRows * kCols;
   extern __shared__ float red[];   // [warp][column][row], then the CTA's sums
   cg::cluster_group cluster = cg::this_cluster();
@@ -191,133 +206,161 @@ __global__ void __launch_bounds__(kLinThreads) w4_linear_kernel(const __grid_con
   const W4Layout& L = a.L;
   const int tile0 = static_cast<int>(blockIdx.x / S) * TILES;
   const int m0 = blockIdx.y * kCols;
-  const int ch0 = static_cast<int>(static_cast<int64_t>(L.chunks) * rank / S);
-  const int ch1 = static_cast<int>(static_cast<int64_t>(L.chunks) * (rank + 1) / S);
-  // A warp's chunks are ch0 + warp + kLinWarps j; in step j everything it reads moves on by a
-  // fixed number of bytes.  Tiles past the last one repeat it, rows of x past the last one the
-  // first: nothing of theirs is written.
-  constexpr int kGroups = GROUP == 32 ? 2 : 1;                       // groups a chunk touches
-  constexpr int kGroupStep = kLinWarps * 64 / GROUP;                 // groups from step to step
-  const int first = ch0 + warp;
+  const int pieces = L.chunks / kSub;   // K is a multiple of the group
+  const int p0 = static_cast<int>(static_cast<int64_t>(pieces) * rank / S);
+  const int p1 = static_cast<int>(static_cast<int64_t>(pieces) * (rank + 1) / S);
+
+  // A warp's pieces are p0 + warp + kLinWarps j; from j to j + 1 everything it reads moves on
+  // by a fixed number of bytes.  Tiles past the last one repeat it, rows of x past the last one
+  // the first: nothing of theirs is written.
+  const int first = p0 + warp;
+  const int steps = first < p1 ? (p1 - first + kLinWarps - 1) / kLinWarps : 0;
   const uint4* cw[TILES];
-  const uint32_t* sw[TILES];
-  const uint16_t* zw[TILES];
+  const uint32_t *sw[TILES], *zw[TILES];
 #pragma unroll
   for (int t = 0; t < TILES; ++t) {
     const int64_t tile = min(tile0 + t, L.tiles - 1);
-    const int64_t grp = (tile * L.groups + first * 64 / GROUP) * 8 + g;
-    cw[t] = reinterpret_cast<const uint4*>(a.packed) + (tile * L.chunks + first) * 32 + lane;
+    const int64_t grp = (tile * L.groups + first * kGroups) * 8 + g;
+    cw[t] = reinterpret_cast<const uint4*>(a.packed) + (tile * L.chunks + first * kSub) * 32 + lane;
     sw[t] = reinterpret_cast<const uint32_t*>(a.packed + L.scale_off) + grp;
-    zw[t] = reinterpret_cast<const uint16_t*>(a.packed + L.zero_off) + grp;
+    zw[t] = reinterpret_cast<const uint32_t*>(a.packed + L.zero_off) + grp;
   }
   const uint16_t* xr[NT];
 #pragma unroll
   for (int n = 0; n < NT; ++n)
-    xr[n] = a.x + (m0 + n * 8 + g < a.M ? m0 + n * 8 + g : 0) * a.ld_x + first * 64 + c * 8;
+    xr[n] = a.x + (m0 + n * 8 + g < a.M ? m0 + n * 8 + g : 0) * a.ld_x + static_cast<int64_t>(first) * kSub * 64 + c * 8;
 
-  struct Chunk {
-    uint4 w[TILES];
+  struct Piece {
+    uint4 w[TILES][kSub];
     uint32_t sc[TILES][kGroups], z[TILES][kGroups];
-    uint4 x[NT][2];
+    uint4 x[NT][2 * kSub];
   };
-  Chunk ahead[kAhead];
-  // Loads the chunk `d` steps on from where the pointers stand.
-  auto load = [&](Chunk& k, int d, bool second_half) {
+  Piece ahead[kAhead];
+  // Loads the piece `d` steps on from where the pointers stand; half: only 32 of its 64 columns
+  // exist (the last of a K that is an odd multiple of 32).
+  auto load = [&](Piece& k, int d, bool half) {
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
-      k.w[t] = __ldcs(cw[t] + d * kLinWarps * 32);
+#pragma unroll
+      for (int i = 0; i < kSub; ++i) k.w[t][i] = __ldcs(cw[t] + (d * kLinWarps * kSub + i) * 32);
 #pragma unroll
       for (int h = 0; h < kGroups; ++h) {
-        k.sc[t][h] = sw[t][(d * kGroupStep + h) * 8];
-        if (ASYM) k.z[t][h] = zw[t][(d * kGroupStep + h) * 8];
+        k.sc[t][h] = sw[t][(d * kLinWarps * kGroups + h) * 8];
+        if (ASYM) k.z[t][h] = zw[t][(d * kLinWarps * kGroups + h) * 8];
       }
     }
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        k.x[n][h] = make_uint4(0, 0, 0, 0);
-        if (h == 0 || second_half) k.x[n][h] = *reinterpret_cast<const uint4*>(xr[n] + d * kLinWarps * 64 + h * 32);
+      for (int h = 0; h < 2 * kSub; ++h) {
+        if (GROUP == 32 && h == 1 && half)
+          k.x[n][h] = make_uint4(0, 0, 0, 0);
+        else
+          k.x[n][h] = *reinterpret_cast<const uint4*>(xr[n] + d * kLinWarps * kSub * 64 + h * 32);
       }
   };
-  auto advance = [&](int d) {
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-      cw[t] += d * kLinWarps * 32;
-      sw[t] += d * kGroupStep * 8;
-      if (ASYM) zw[t] += d * kGroupStep * 8;
-    }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) xr[n] += d * kLinWarps * 64;
-  };
+  const int odd_step = GROUP == 32 && (L.K & 32) && p1 == pieces && steps > 0 && first + (steps - 1) * kLinWarps == pieces - 1
+                           ? steps - 1 : -1;
 
   float acc[TILES][NT][4] = {};
-  auto use = [&](const Chunk& k) {
+  // The k-steps of a group: `start` what its sums begin with, SUB whether zeros are taken off.
+  auto group_of = [&](const Piece& k, int h, const float (&start)[NT][2], auto sub) {
+    constexpr int kSteps = GROUP / 16;
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
-      const uint32_t word[4] = {k.w[t].x, k.w[t].y, k.w[t].z, k.w[t].w};
       float part[NT][4];
+      uint32_t z0 = 0x3FC03FC0u, z1 = 0x3FC03FC0u;
+      if (ASYM) {
+        z0 = __byte_perm(k.z[t][h], 0, 0x1010);
+        z1 = __byte_perm(k.z[t][h], 0, 0x3232);
+      }
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const int h = GROUP == 32 ? s >> 1 : 0;
-        // 1 + zero / 16 of rows g and g + 8, twice each
-        uint32_t z0 = 0x3FC03FC0u, z1 = 0x3FC03FC0u;
-        if (ASYM) {
-          z0 = (0x3F80u | ((k.z[t][h] & 15u) << 3)) * 0x10001u;
-          z1 = (0x3F80u | (((k.z[t][h] >> 8) & 15u) << 3)) * 0x10001u;
-        }
+      for (int i = 0; i < kSteps; ++i) {
+        const int s = h * kSteps + i;   // k-step of the piece
+        const uint4& wv = k.w[t][s >> 2];
+        const uint32_t word = (s & 3) == 0 ? wv.x : (s & 3) == 1 ? wv.y : (s & 3) == 2 ? wv.z : wv.w;
         uint32_t f[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t r = __funnelshift_r(word[s], word[s], 4 * i);
-          f[i] = sub_bf16x2((r & 0x00780078u) | 0x3F803F80u, (i & 1) ? z1 : z0);
+        for (int r = 0; r < 4; ++r) {
+          f[r] = (__funnelshift_r(word, word, 4 * r) & 0x00780078u) | 0x3F803F80u;
+          if (decltype(sub)::value) f[r] = sub_bf16x2(f[r], (r & 1) ? z1 : z0);
         }
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const uint4& x = k.x[n][s >> 1];
           const uint32_t b0 = s & 1 ? x.z : x.x, b1 = s & 1 ? x.w : x.y;
-          if (s == 0 || (GROUP == 32 && s == 2))
-            mma_bf16_zero(part[n], f, b0, b1);
+          if (i == 0)
+            mma_bf16_from(part[n], f, b0, b1, start[n][0], start[n][1], start[n][0], start[n][1]);
           else
             mma_bf16(part[n], f, b0, b1);
         }
-        if (s == 3 || (GROUP == 32 && s == 1)) {
-          const float s0 = bf16_lo(k.sc[t][h]), s1 = bf16_hi(k.sc[t][h]);
+      }
+      const float s0 = bf16_lo(k.sc[t][h]), s1 = bf16_hi(k.sc[t][h]);
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            acc[t][n][0] = fmaf(s0, part[n][0], acc[t][n][0]);
-            acc[t][n][1] = fmaf(s0, part[n][1], acc[t][n][1]);
-            acc[t][n][2] = fmaf(s1, part[n][2], acc[t][n][2]);
-            acc[t][n][3] = fmaf(s1, part[n][3], acc[t][n][3]);
-          }
-        }
+      for (int n = 0; n < NT; ++n) {
+        acc[t][n][0] = fmaf(s0, part[n][0], acc[t][n][0]);
+        acc[t][n][1] = fmaf(s0, part[n][1], acc[t][n][1]);
+        acc[t][n][2] = fmaf(s1, part[n][2], acc[t][n][2]);
+        acc[t][n][3] = fmaf(s1, part[n][3], acc[t][n][3]);
       }
     }
   };
-  // Steps of this warp; those before `full` need no check (a last chunk of 32 columns does).
-  const int steps = first < ch1 ? (ch1 - first + kLinWarps - 1) / kLinWarps : 0;
-  const int full_end = min(ch1, L.K / 64);
-  const int full = first < full_end ? (full_end - first + kLinWarps - 1) / kLinWarps : 0;
+  auto use = [&](const Piece& k) {
+#pragma unroll
+    for (int h = 0; h < kGroups; ++h) {
+      float start[NT][2] = {};
+      bool exact = ASYM;
+      if (!ASYM) {
+        const uint32_t minus[4] = {0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u};   // -1.5
+        float sum[NT][4];
+#pragma unroll
+        for (int i = 0; i < GROUP / 16; ++i)
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const int s = h * (GROUP / 16) + i;
+            const uint4& x = k.x[n][s >> 1];
+            const uint32_t b0 = s & 1 ? x.z : x.x, b1 = s & 1 ? x.w : x.y;
+            if (i == 0)
+              mma_bf16_from(sum[n], minus, b0, b1, 0.f, 0.f, 0.f, 0.f);
+            else
+              mma_bf16(sum[n], minus, b0, b1);
+          }
+        float big = 0.f;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          start[n][0] = sum[n][0];
+          start[n][1] = sum[n][1];
+          big = fmaf(sum[n][0], 0.f, fmaf(sum[n][1], 0.f, big));   // 0, or NaN
+        }
+        exact = __any_sync(0xffffffffu, big != 0.f);
+      }
+      if (exact) {
+        const float none[NT][2] = {};
+        group_of(k, h, none, std::true_type());
+      } else {
+        group_of(k, h, start, std::false_type());
+      }
+    }
+  };
 #pragma unroll
   for (int d = 0; d < kAhead; ++d)
-    if (d < steps) load(ahead[d], d, d < full);
-  int j = 0;
-  for (; j + 2 * kAhead <= full; j += kAhead) {
+    if (d < steps) load(ahead[d], d, d == odd_step);
+  for (int j = 0; j < steps; j += kAhead) {
 #pragma unroll
     for (int d = 0; d < kAhead; ++d) {
-      use(ahead[d]);
-      load(ahead[d], kAhead + d, true);
+      if (j + d < steps) {
+        use(ahead[d]);
+        if (j + d + kAhead < steps) load(ahead[d], d + kAhead, j + d + kAhead == odd_step);
+      }
     }
-    advance(kAhead);
-  }
-  for (; j < steps; j += kAhead) {
 #pragma unroll
-    for (int d = 0; d < kAhead; ++d) {
-      if (j + d >= steps) break;
-      use(ahead[d]);
-      if (j + kAhead + d < steps) load(ahead[d], kAhead + d, j + kAhead + d < full);
+    for (int t = 0; t < TILES; ++t) {
+      cw[t] += kAhead * kLinWarps * kSub * 32;
+      sw[t] += kAhead * kLinWarps * kGroups * 8;
+      if (ASYM) zw[t] += kAhead * kLinWarps * kGroups * 8;
     }
-    advance(kAhead);
+#pragma unroll
+    for (int n = 0; n < NT; ++n) xr[n] += kAhead * kLinWarps * kSub * 64;
   }
 
   // ---- join the warps, then the cluster
@@ -456,9 +499,8 @@ extern "C" int glt_w4_linear(const void* packed, int N, int K, int group, int as
   const glt::LinearArgs a{static_cast<const uint8_t*>(packed), W4Layout(N, K, group, asym), x, ld_x, M, y, ld_y,
                           y_dtype, resid, ld_r};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (M <= 2) return glt::launch_linear_as<1, 1>(a, st);
   if (M <= 8) return glt::launch_linear_as<1, 2>(a, st);
   if (M <= 16) return glt::launch_linear_as<2, 2>(a, st);
-  if (M <= 24) return glt::launch_linear_as<3, 4>(a, st);
-  return glt::launch_linear_as<4, 4>(a, st);
+  if (M <= 24) return glt::launch_linear_as<3, 2>(a, st);
+  return glt::launch_linear_as<4, 2>(a, st);
 }
