@@ -1,19 +1,17 @@
 // Products with 4-bit weights and group scales (glt_w4_*).
 //
-// Packed layout of W [N, K]: rows in tiles of 16, columns in chunks of 64 (the last
-// ones filled up with zero scales).  A chunk of a tile is 128 words of eight codes,
-// in the order the A fragments of mma.m16n8k16 want them: lane 4g + c of a warp owns
-// words 4 * lane + s, s = 0..3, and word s holds, for the k-step s of the chunk, rows
-// g and g + 8 at columns col(c, s, 0..3) = (s / 2) * 32 + c * 8 + (s % 2) * 4 + 0..3.
-// So a warp reads a chunk as one 16-byte load a lane, 512 contiguous bytes, and each
-// 32-column half of the chunk (the smallest group) is two whole k-steps.
-// Register i of the fragment (row half i % 2, column pair i / 2) takes its two codes
-// from bits 4i + 3 .. 4i + 6 and 16 further up (modulo 32): a rotation by 4i brings
-// them to mantissa bits 3..6 of two bf16 numbers 1 + code / 16, exactly.
+// Packed layout of W [N, K]: rows in tiles of 16, columns in blocks of 128 (the last
+// one filled up with zero scales).  A block of a tile is one record, a tile's records follow
+// one another.  A record: two chunks of 64 columns, 128 words of eight codes each, then the
+// scales of the block's groups, [group][g][row half] bf16, then with asym the zeros alike.
+// Lane 4g + c of a warp owns words 4 * lane + s, s = 0..3, of a chunk; byte b of word s holds
+// the codes of row g (low nibble) and row g + 8 (high nibble) at column
+// (s / 2) * 32 + 8 c + (s % 2) * 4 + b.  So one AND (and a shift) makes four codes a register
+// of operand A of mma.m16n8k32 on bytes.
 #include <cooperative_groups.h>
 #include <math.h>
 
-#include <type_traits>
+#include <climits>
 
 #include "common.cuh"
 #include "gemm.cuh"
@@ -23,23 +21,26 @@ namespace cg = cooperative_groups;
 namespace glt {
 namespace {
 
-__host__ __device__ inline int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b * b; }
-
-// Offsets of the three parts of a packed matrix.
 struct W4Layout {
   int N, K, group, asym;
-  int tiles, chunks, groups;  // groups: of the filled-up columns
-  int64_t scale_off, zero_off, bytes;
-  W4Layout(int N_, int K_, int group_, int asym_) : N(N_), K(K_), group(group_), asym(asym_) {
+  int tiles, blocks;
+  int per_block;   // groups of a block
+  int record;      // bytes
+  int64_t bytes;
+  W4Layout(int N_, int K_, int group_, int asym_) : N(N_), K(K_), group(group_), asym(asym_ != 0) {
     tiles = (N + 15) / 16;
-    chunks = (K + 63) / 64;
-    groups = static_cast<int>(up(static_cast<int64_t>(chunks) * 64, group) / group);
-    scale_off = up(static_cast<int64_t>(tiles) * chunks * 512, 256);
-    // [tile][group][g][row half] bf16, then the zeros as bf16 1 + zero / 16 in the same order
-    zero_off = up(scale_off + static_cast<int64_t>(tiles) * groups * 32, 256);
-    bytes = zero_off + (asym ? up(static_cast<int64_t>(tiles) * groups * 32, 256) : 0);
+    blocks = (K + 127) / 128;
+    per_block = 128 / group;
+    record = 1024 + per_block * 32 * (1 + asym);
+    bytes = static_cast<int64_t>(tiles) * blocks * record;
   }
 };
+
+// a / b by the much shorter 32-bit division where that is enough.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
 
 int check_shape(int N, int K, int group) {
   if (group != 32 && group != 64 && group != 128) return fail(GLT_EINVAL, "w4: group %d (32, 64 or 128)", group);
@@ -84,46 +85,53 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const uint16_t* __rest
   }
 }
 
-__device__ __forceinline__ int chunk_col(int c, int s, int e) { return (s >> 1) * 32 + c * 8 + (s & 1) * 4 + e; }
-__device__ __forceinline__ int code_bit(int i, int h) { return (3 + 16 * h + 4 * i) & 31; }
-
 __global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t* __restrict__ codes,
                                                       const uint16_t* __restrict__ scales,
                                                       const uint8_t* __restrict__ zeros, W4Layout L,
                                                       uint8_t* __restrict__ packed) {
-  const int ng = L.K / L.group;
-  const int64_t words = static_cast<int64_t>(L.tiles) * L.chunks * 128;
-  const int64_t scs = static_cast<int64_t>(L.tiles) * L.groups * 16;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * blockDim.x;
-  const int64_t first = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x;
-  for (int64_t q = first; q < words; q += step) {
-    const int s = q & 3, lane = (q >> 2) & 31;
-    const int64_t tc = q >> 7;
-    const int64_t tile = tc / L.chunks;
-    const int chunk = static_cast<int>(tc - tile * L.chunks);
+  const int ng = L.K / L.group, words = L.record / 4;
+  const int64_t total = static_cast<int64_t>(L.tiles) * L.blocks * words;
+  for (int64_t q = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; q < total;
+       q += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+    const int64_t rec = q / words;
+    const int i = static_cast<int>(q - rec * words);
+    const int64_t tile = rec / L.blocks;
+    const int block = static_cast<int>(rec - tile * L.blocks);
     uint32_t word = 0;
+    if (i < 256) {
+      const int s = i & 3, lane = (i >> 2) & 31;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t n = tile * 16 + (lane >> 2) + 8 * (i & 1);
-        const int k = chunk * 64 + chunk_col(lane & 3, s, 2 * (i >> 1) + h);
-        const uint32_t u = n < L.N && k < L.K ? codes[n * L.K + k] & 15u : 0u;
-        const int b = code_bit(i, h);
-        word |= b <= 28 ? u << b : (u << b) | (u >> (32 - b));
+      for (int e = 0; e < 8; ++e) {   // nibble e: byte e / 2, row half e % 2
+        const int64_t n = tile * 16 + (lane >> 2) + 8 * (e & 1);
+        const int k = block * 128 + (i >> 7) * 64 + (s >> 1) * 32 + (lane & 3) * 8 + (s & 1) * 4 + (e >> 1);
+        word |= (n < L.N && k < L.K ? codes[n * L.K + k] & 15u : 0u) << (4 * e);
       }
+    } else {
+      const int j = (i - 256) % (L.per_block * 8);
+      const bool zero = i - 256 >= L.per_block * 8;
+      const int grp = block * L.per_block + (j >> 3);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int64_t n = tile * 16 + (j & 7) + 8 * e;
+        if (n >= L.N || grp >= ng) continue;
+        const uint32_t v = zero ? bf16_bits_rn(static_cast<float>(zeros[n * ng + grp] & 15u)) : scales[n * ng + grp];
+        word |= v << (16 * e);
+      }
+    }
     reinterpret_cast<uint32_t*>(packed)[q] = word;
   }
-  for (int64_t q = first; q < scs; q += step) {
-    const int64_t tg = q >> 4;
-    const int64_t tile = tg / L.groups;
-    const int grp = static_cast<int>(tg - tile * L.groups);
-    const int64_t n = tile * 16 + ((q >> 1) & 7) + 8 * (q & 1);
-    const bool in = n < L.N && grp < ng;
-    reinterpret_cast<uint16_t*>(packed + L.scale_off)[q] = in ? scales[n * ng + grp] : 0;
-    if (L.asym)
-      reinterpret_cast<uint16_t*>(packed + L.zero_off)[q] = 0x3F80u | (in ? (zeros[n * ng + grp] & 15u) << 3 : 0u);
-  }
+}
+
+// code - zero and scale of one weight.
+__device__ __forceinline__ float w4_code(const uint8_t* packed, const W4Layout& L, int64_t n, int k, float* scale) {
+  const uint8_t* rec = packed + ((n >> 4) * L.blocks + (k >> 7)) * L.record;
+  const int r = n & 15, kk = k & 63;
+  const int s = (kk >> 5) * 2 + ((kk >> 2) & 1), c = (kk >> 3) & 3;
+  const int word = ((k >> 6) & 1) * 128 + ((r & 7) * 4 + c) * 4 + s;
+  const uint32_t u = reinterpret_cast<const uint32_t*>(rec)[word] >> (8 * (kk & 3) + 4 * (r >> 3)) & 15u;
+  const uint16_t* sc = reinterpret_cast<const uint16_t*>(rec + 1024) + ((k & 127) / L.group) * 16 + (r & 7) * 2 + (r >> 3);
+  *scale = bf16_bits_to_f32(sc[0]);
+  return static_cast<float>(u) - (L.asym ? bf16_bits_to_f32(sc[L.per_block * 16]) : 8.f);
 }
 
 __global__ void __launch_bounds__(256) w4_unpack_kernel(const uint8_t* __restrict__ packed, W4Layout L,
@@ -133,34 +141,134 @@ __global__ void __launch_bounds__(256) w4_unpack_kernel(const uint8_t* __restric
        q += static_cast<int64_t>(gridDim.x) * blockDim.x) {
     const int64_t n = q / L.K;
     const int k = static_cast<int>(q - n * L.K);
-    const int r = n & 15, kk = k & 63;
-    const int s = (kk >> 5) * 2 + ((kk >> 2) & 1), c = (kk >> 3) & 3, e = kk & 3;
-    const int64_t word = (((n >> 4) * L.chunks + (k >> 6)) * 32 + (r & 7) * 4 + c) * 4 + s;
-    const int b = code_bit((r >> 3) + 2 * (e >> 1), e & 1);
-    const uint32_t v = reinterpret_cast<const uint32_t*>(packed)[word];
-    const float u = static_cast<float>(__funnelshift_r(v, v, b) & 15u);
-    const int64_t sc = ((n >> 4) * L.groups + k / L.group) * 16 + (r & 7) * 2 + (r >> 3);
-    const float z = L.asym ? static_cast<float>((reinterpret_cast<const uint16_t*>(packed + L.zero_off)[sc] >> 3) & 15u) : 8.f;
-    w[n * ld + k] = bf16_bits_rn((u - z) * bf16_bits_to_f32(reinterpret_cast<const uint16_t*>(packed + L.scale_off)[sc]));
+    float scale;
+    const float u = w4_code(packed, L, n, k, &scale);
+    w[n * ld + k] = bf16_bits_rn(u * scale);
   }
 }
 
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+__device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.u8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// The same from other sums.
-__device__ __forceinline__ void mma_bf16_from(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
-                                              float c0, float c1, float c2, float c3) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
-      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
-}
-__device__ __forceinline__ uint32_t sub_bf16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-  return r;
+
+// ---- operand B.  Within a group of columns a row of x becomes fixed-point numbers
+// v = round(x 2^a), with a such that the largest fills 16 bits (LIMBS = 2) or 24 (LIMBS = 3), and
+// v its signed bytes, one column of operand B each.  Products with the codes are then exact
+// integers.  bf16 has 8 bits, so v is x exactly down to 2^-8 of the group's largest magnitude
+// (2^-16 with three bytes), and off by at most 2^-16 (2^-24) of it below: two bytes for results
+// in bf16, three for results in fp32.
+// (On the tensor core, k = 32 of bytes costs what k = 16 of bf16 does, 8 cycles, and the codes need
+// two thirds of an instruction for four where bf16 needs seven; e4m3 is no faster than f16 here.)
+// A tile of N = 8 columns holds 8 / LIMBS rows of x at 2 (or 4, the last empty) columns a row, high
+// byte first.  Image: [chunk of 64][tile of rows][lane][16 bytes], lane 4g + c the column g at the
+// k of operand A's lanes c.
+constexpr int kMagic = 0x4B400000;   // 1.5 2^23 as a float: kMagic + i is the float 1.5 2^23 + i
+// What lane c needs at the ends of a group: what its two columns' sums begin with, kMagic - 8 times
+// the sum of the bytes (asym: minus that sum), and 2^-a of its row.
+struct __align__(16) GroupNote {
+  int start[2];
+  float factor;
+  int pad;
+};
+template <int LIMBS>
+struct XImage {
+  static constexpr int kCols = LIMBS == 2 ? 2 : 4, kRows = 8 / kCols;   // columns a row, rows a tile
+  int per_cta;   // tiles of rows of x that a CTA takes
+  int tiles, chunks, groups;   // tiles filled up to per_cta's multiple; chunks and groups to the end of the last block
+  int64_t notes, finite, bytes;   // offsets in the workspace, after the image
+  __host__ __device__ XImage(const W4Layout& L, int M) {
+    const int need = (M + kRows - 1) / kRows;
+    per_cta = need <= 2 ? need : need <= 5 ? 5 : 8;
+    tiles = (need + per_cta - 1) / per_cta * per_cta;
+    chunks = L.blocks * 2;
+    groups = L.blocks * L.per_block;
+    notes = static_cast<int64_t>(chunks) * tiles * 512;
+    // notes: [group][tile][lane c]
+    finite = notes + static_cast<int64_t>(groups) * tiles * 4 * sizeof(GroupNote);
+    // finite: per row of x, its number of groups that are not finite
+    bytes = (finite + static_cast<int64_t>(M) * 4 + 15) / 16 * 16;
+  }
+};
+
+constexpr int kPrepThreads = 256;
+// A thread takes eight columns of a row, the threads of a group are neighbours.
+template <int LIMBS, int GROUP>
+__global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const uint16_t* __restrict__ x, int64_t ld_x, int M,
+                                                                  W4Layout L, uint8_t* __restrict__ ws) {
+  using Image = XImage<LIMBS>;
+  const Image I(L, M);
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int m = blockIdx.y;
+  const int v = blockIdx.x * kPrepThreads + threadIdx.x;   // of chunks * 8 = blocks * 16
+  const bool in = v < I.chunks * 8;
+  uint4 u = make_uint4(0, 0, 0, 0);
+  if (in && v * 8 < L.K) u = *reinterpret_cast<const uint4*>(x + m * ld_x + v * 8);
+  float f[8];
+  unpack8(u, f);
+  float peak = 0.f;
+  bool bad = false;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    if (fabsf(f[k]) < INFINITY)
+      peak = fmaxf(peak, fabsf(f[k]));
+    else
+      bad = true;
+  }
+  constexpr int kLanes = GROUP / 8;
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+  // the largest to [2^14, 2^15) or [2^22, 2^23), one less for the one mantissa whose high byte would be 128
+  int a = 0;
+  if (peak > 0.f) {
+    const int e = ilogbf(peak);
+    const bool top = (__float_as_uint(peak) >> 16 & 0x7F) == 0x7F && e > -127;
+    a = (LIMBS == 2 ? 14 : 22) - e - (top ? 1 : 0);
+  }
+  // in two factors: 2^a may be out of range
+  const float a0 = exp2f(static_cast<float>(a / 2)), a1 = exp2f(static_cast<float>(a - a / 2));
+  uint32_t limb[LIMBS][2] = {};
+  int sum[LIMBS] = {};
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    int i = fabsf(f[k]) < INFINITY ? __float2int_rn(f[k] * a0 * a1) : 0;
+#pragma unroll
+    for (int l = LIMBS - 1; l >= 0; --l) {
+      const int up = l > 0 ? (i + 128) >> 8 : 0;   // what the next higher byte takes
+      const int b = i - up * 256;
+      limb[l][k >> 2] |= (static_cast<uint32_t>(b) & 0xFFu) << (8 * (k & 3));
+      sum[l] += b;
+      i = up;
+    }
+  }
+#pragma unroll
+  for (int o = 1; o < kLanes; o <<= 1)
+#pragma unroll
+    for (int l = 0; l < LIMBS; ++l) sum[l] += __shfl_xor_sync(0xffffffffu, sum[l], o);
+  if (!in) return;
+  const int chunk = v >> 3, step = (v >> 2) & 1, c = v & 3, tile = m / Image::kRows, row = m % Image::kRows;
+  uint8_t* dst = ws + ((static_cast<int64_t>(chunk) * I.tiles + tile) * 32 + row * Image::kCols * 4 + c) * 16 + step * 8;
+#pragma unroll
+  for (int l = 0; l < LIMBS; ++l) *reinterpret_cast<uint2*>(dst + l * 64) = make_uint2(limb[l][0], limb[l][1]);
+  if (LIMBS == 3) *reinterpret_cast<uint2*>(dst + 192) = make_uint2(0, 0);
+  if (v % kLanes == 0) {
+    GroupNote* note = reinterpret_cast<GroupNote*>(ws + I.notes) +
+                      (static_cast<int64_t>(v / kLanes) * I.tiles + tile) * 4 + row * Image::kCols / 2;
+#pragma unroll
+    for (int j = 0; j < Image::kCols / 2; ++j) {
+      GroupNote n;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int b = 2 * j + e < LIMBS ? sum[2 * j + e < LIMBS ? 2 * j + e : 0] : 0;
+        n.start[e] = L.asym ? -b : kMagic - 8 * b;
+      }
+      n.factor = exp2f(static_cast<float>(-a));
+      n.pad = 0;
+      note[j] = n;
+    }
+  }
+  if (bad) atomicAdd(reinterpret_cast<int*>(ws + I.finite) + m, 1);   // zeroed before
 }
 
 struct LinearArgs {
@@ -174,261 +282,385 @@ struct LinearArgs {
   int y_bf16;
   const uint16_t* resid;
   int64_t ld_r;
+  uint8_t* ws;
+  unsigned int* err;
 };
 
-constexpr int kLinWarps = 4;
-constexpr int kLinThreads = 32 * kLinWarps;
+// One contiguous copy (16-byte aligned, a multiple of 16 bytes) into shared memory.
+__device__ __forceinline__ void copy_bulk(void* dst, const void* src, int bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
+               : "memory");
+}
 
-// y = x . W^T for up to 8 NT rows of x: the weights are operand A (16 rows by 16 columns),
-// the rows of x operand B (N = 8).  A cluster of S CTAs takes 16 TILES rows of W; its CTAs
-// split the columns, and a CTA's warps take the pieces of its part in turn, TILES tiles at
-// once so that a fragment of x serves them all.  A piece is a chunk, or two with groups of
-// 128, so that a group's sums meet its scale once.  Partial sums meet in shared memory, then
-// over the cluster, in a fixed order.
+// One product the plain way, for rows of x that are not finite.
+__device__ __noinline__ float plain_product(const LinearArgs& a, int64_t n, int m) {
+  float sum = 0.f;
+  for (int k = 0; k < a.L.K; ++k) {
+    float scale;
+    const float u = w4_code(a.packed, a.L, n, k, &scale);
+    sum = fmaf(bf16_bits_to_f32(a.x[m * a.ld_x + k]) * scale, u, sum);
+  }
+  return sum;
+}
+
+// y = x . W^T for up to NT tiles of rows of x: the weights are operand A (16 rows by 32
+// columns), the image of x operand B.
+//
+// Work.  One CTA a SM.  A unit is TILES tiles of 16 rows of W, all fed by a load of the
+// image.  A cluster of S CTAs takes a run of units, and its warps equal runs of their blocks,
+// laid end to end.  Each warp has a ring of stages, filled by TMA with a record (of every
+// tile) a stage, that runs ahead across units.  A unit that one warp holds whole is written from
+// registers; the parts of a unit that warps share go through shared memory (the cluster's) to
+// the warp that begins it, which adds them in order.
 //
 // Half a byte a weight leaves about 22 cycles of an SM for a tile's chunk, so instructions
-// count.  A register of two weights takes a rotation (three in four) and one AND-OR to become
-// 1 + code / 16.  Taking 1 + zero / 16 off costs one more; with the constant zero 8 it is left
-// to the tensor core: a product with -1.5 everywhere gives -1.5 sum x, from which the sums of
-// every tile start.  (Then |x| counts 1.5 to 1.94 times in 32-bit sums instead of about 0.25
-// times.)  Infinities would not survive that, so a piece of x whose sum is not finite goes
-// the exact way.
-template <int NT, int TILES, bool ASYM, int GROUP>
-__global__ void __launch_bounds__(kLinThreads) w4_linear_kernel(const __grid_constant__ LinearArgs a) {
-  constexpr int kSub = GROUP == 128 ? 2 : 1;                    // chunks of a piece
-  constexpr int kGroups = GROUP == 32 ? 2 : 1;                  // groups of a piece
-  constexpr int kAhead = NT == 1 ? 4 / kSub : NT == 2 ? 2 : 1;  // pieces on their way
-  constexpr int kRows = 16 * TILES, kCols = 8 * NT, kOut = kRows * kCols;
-  extern __shared__ float red[];   // [warp][column][row], then the CTA's sums
+// count: 12 integer ones make the codes' fragments (8 AND, 4 shifts), two products do the
+// rest for four rows of x.  Zeros: sum v (u - z) = sum v u - z sum v, the second part, and the
+// number that turns the integer into a float, being what a group's sums begin with.
+__host__ __device__ constexpr int linear_warps(int nt) { return nt <= 2 ? 16 : 8; }
+constexpr int kStages = 4;
+
+template <int NT, int TILES, bool ASYM, int GROUP>   // the same for both numbers of bytes
+struct LinearSmem {
+  static constexpr int kWarps = linear_warps(NT);
+  static constexpr int kRecord = 1024 + 128 / GROUP * 32 * (ASYM ? 2 : 1);
+  static constexpr int kBlocks = TILES == 1 ? 2 : 1;           // of a stage: with one tile they lie side by side
+  static constexpr int kStage = kBlocks * TILES * kRecord;
+  static constexpr int kRing = kStages * kStage;               // a warp's
+  static constexpr int kPart = TILES * NT * 2 * 32;            // floats of a part of a unit
+  static constexpr int kBytes = kWarps * (kRing + 2 * kPart * 4 + kStages * 8);
+};
+
+template <int LIMBS, int NT, int TILES, bool ASYM, int GROUP>
+__global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(const __grid_constant__ LinearArgs a) {
+  using Smem = LinearSmem<NT, TILES, ASYM, GROUP>;
+  constexpr int kWarps = Smem::kWarps, kRecord = Smem::kRecord, kPart = Smem::kPart;
+  using Image = XImage<LIMBS>;
+  constexpr int kPer = 128 / GROUP, kSteps = GROUP / 32;        // groups of a block, k-steps of a group
+  constexpr int kLeast = 2;                                     // shorter runs cost more to join than to read
+  extern __shared__ __align__(128) uint8_t smem[];
+  float* parts = reinterpret_cast<float*>(smem + kWarps * Smem::kRing);   // [warp][the unit it continues, the one it only begins]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(parts + kWarps * 2 * kPart);
   cg::cluster_group cluster = cg::this_cluster();
   const int S = cluster.num_blocks(), rank = cluster.block_rank();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, local = threadIdx.x >> 5;
+  const int warp = local * S + rank;    // of the cluster
   const W4Layout& L = a.L;
-  const int tile0 = static_cast<int>(blockIdx.x / S) * TILES;
-  const int m0 = blockIdx.y * kCols;
-  const int pieces = L.chunks / kSub;   // K is a multiple of the group
-  const int p0 = static_cast<int>(static_cast<int64_t>(pieces) * rank / S);
-  const int p1 = static_cast<int>(static_cast<int64_t>(pieces) * (rank + 1) / S);
-
-  // A warp's pieces are p0 + warp + kLinWarps j; from j to j + 1 everything it reads moves on
-  // by a fixed number of bytes.  Tiles past the last one repeat it, rows of x past the last one
-  // the first: nothing of theirs is written.
-  const int first = p0 + warp;
-  const int steps = first < p1 ? (p1 - first + kLinWarps - 1) / kLinWarps : 0;
-  const uint4* cw[TILES];
-  const uint32_t *sw[TILES], *zw[TILES];
-#pragma unroll
-  for (int t = 0; t < TILES; ++t) {
-    const int64_t tile = min(tile0 + t, L.tiles - 1);
-    const int64_t grp = (tile * L.groups + first * kGroups) * 8 + g;
-    cw[t] = reinterpret_cast<const uint4*>(a.packed) + (tile * L.chunks + first * kSub) * 32 + lane;
-    sw[t] = reinterpret_cast<const uint32_t*>(a.packed + L.scale_off) + grp;
-    zw[t] = reinterpret_cast<const uint32_t*>(a.packed + L.zero_off) + grp;
+  const Image I(L, a.M);
+  const int P = L.blocks;
+  const int units = (L.tiles + TILES - 1) / TILES;
+  const int clusters = gridDim.x / S, cl = blockIdx.x / S;
+  const int u0 = static_cast<int>(quotient(static_cast<int64_t>(units) * cl, clusters));
+  const int u1 = static_cast<int>(quotient(static_cast<int64_t>(units) * (cl + 1), clusters));
+  const int64_t all = static_cast<int64_t>(u1 - u0) * P;
+  const int warps = static_cast<int>(min(static_cast<int64_t>(S * kWarps), (all + kLeast - 1) / kLeast));
+  const int64_t each = quotient(all, warps), more = all - each * warps;
+  auto begin_of = [&](int w) { return each * w + min(static_cast<int64_t>(w), more); };
+  const int64_t begin = warp < warps ? begin_of(warp) : all, end = warp < warps ? begin_of(warp + 1) : all;
+  const int count = static_cast<int>(end - begin);
+  int unit = u0, piece = 0;
+  if (count > 0) {
+    const int64_t u = quotient(begin, P);
+    unit += static_cast<int>(u);
+    piece = static_cast<int>(begin - u * P);
   }
-  const uint16_t* xr[NT];
-#pragma unroll
-  for (int n = 0; n < NT; ++n)
-    xr[n] = a.x + (m0 + n * 8 + g < a.M ? m0 + n * 8 + g : 0) * a.ld_x + static_cast<int64_t>(first) * kSub * 64 + c * 8;
 
-  struct Piece {
-    uint4 w[TILES][kSub];
-    uint32_t sc[TILES][kGroups], z[TILES][kGroups];
-    uint4 x[NT][2 * kSub];
-  };
-  Piece ahead[kAhead];
-  // Loads the piece `d` steps on from where the pointers stand; half: only 32 of its 64 columns
-  // exist (the last of a K that is an odd multiple of 32).
-  auto load = [&](Piece& k, int d, bool half) {
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-#pragma unroll
-      for (int i = 0; i < kSub; ++i) k.w[t][i] = __ldcs(cw[t] + (d * kLinWarps * kSub + i) * 32);
-#pragma unroll
-      for (int h = 0; h < kGroups; ++h) {
-        k.sc[t][h] = sw[t][(d * kLinWarps * kGroups + h) * 8];
-        if (ASYM) k.z[t][h] = zw[t][(d * kLinWarps * kGroups + h) * 8];
-      }
+  // ---- the ring
+  uint8_t* ring = smem + local * Smem::kRing;
+  bars += local * kStages;
+  if (lane == 0) {
+    for (int i = 0; i < kStages; ++i) tc::mbar_init(bars + i, 1);
+    tc::fence_mbar_init();
+  }
+  __syncwarp();
+  int to_issue = count, ld_piece = piece, ld_unit = unit;
+  const uint8_t* src = a.packed + (static_cast<int64_t>(unit) * TILES * P + piece) * kRecord;
+  auto issue = [&](int stage) {
+    if (to_issue <= 0) return;
+    const int n = min(to_issue, Smem::kBlocks);
+    if (lane == 0) {
+      tc::mbar_arrive_expect_tx(bars + stage, n * TILES * kRecord);
+      uint8_t* dst = ring + stage * Smem::kStage;
+      copy_bulk(dst, src, n * kRecord, bars + stage);
+      if (TILES == 2)   // a tile past the last one repeats it: nothing of it is written
+        copy_bulk(dst + kRecord, ld_unit * 2 + 1 < L.tiles ? src + static_cast<int64_t>(P) * kRecord : src, kRecord, bars + stage);
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int h = 0; h < 2 * kSub; ++h) {
-        if (GROUP == 32 && h == 1 && half)
-          k.x[n][h] = make_uint4(0, 0, 0, 0);
-        else
-          k.x[n][h] = *reinterpret_cast<const uint4*>(xr[n] + d * kLinWarps * kSub * 64 + h * 32);
-      }
+    to_issue -= n;
+    src += n * kRecord;
+    if (TILES == 2 && ++ld_piece == P) {
+      ld_piece = 0;
+      ++ld_unit;
+      src += static_cast<int64_t>(P) * kRecord;
+    }
   };
-  const int odd_step = GROUP == 32 && (L.K & 32) && p1 == pieces && steps > 0 && first + (steps - 1) * kLinWarps == pieces - 1
-                           ? steps - 1 : -1;
+#pragma unroll 1
+  for (int i = 0; i < kStages; ++i) issue(i);
 
-  float acc[TILES][NT][4] = {};
-  // The k-steps of a group: `start` what its sums begin with, SUB whether zeros are taken off.
-  auto group_of = [&](const Piece& k, int h, const float (&start)[NT][2], auto sub) {
-    constexpr int kSteps = GROUP / 16;
+  // ---- the image and its notes, one chunk and one group ahead
+  const int image_chunk = I.tiles * 32, note_group = I.tiles * 4;   // strides, in elements
+  const uint4* image = reinterpret_cast<const uint4*>(a.ws) + blockIdx.y * NT * 32 + lane;
+  const uint4* notes = reinterpret_cast<const uint4*>(a.ws + I.notes) + blockIdx.y * NT * 4 + c;
+  auto load_image = [&](uint4 (&x)[NT], int chunk) {
+    const uint4* p = image + chunk * image_chunk;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) x[n] = p[n * 32];
+  };
+  auto load_note = [&](uint4 (&x)[NT], int group) {   // a GroupNote
+    const uint4* p = notes + group * note_group;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) x[n] = p[n * 4];
+  };
+  // a lane's two columns: the bytes of a row, or (three bytes) half of them
+  const float high = LIMBS == 2 ? 256.f : c & 1 ? 1.f : 65536.f, low = LIMBS == 2 ? 1.f : c & 1 ? 0.f : 256.f;
+
+  float acc[TILES][NT][2] = {};   // rows g, g + 8 of W by a row of a tile of x
+  int part[TILES][NT][4];
+  // k-step s of the record(s) at `rec`, with the image's chunk x and the group's note.
+  auto step = [&](const uint8_t* rec, int s, const uint4 (&x)[NT], const uint4 (&note)[NT]) {
+    const int grp = s / kSteps;
+    const bool first = s % kSteps == 0, last = s % kSteps == kSteps - 1;
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
-      float part[NT][4];
-      uint32_t z0 = 0x3FC03FC0u, z1 = 0x3FC03FC0u;
-      if (ASYM) {
-        z0 = __byte_perm(k.z[t][h], 0, 0x1010);
-        z1 = __byte_perm(k.z[t][h], 0, 0x3232);
+      const uint8_t* sc = rec + t * kRecord + 1024 + grp * 32 + g * 4;
+      const uint2 w = *reinterpret_cast<const uint2*>(rec + t * kRecord + (s >> 1) * 512 + lane * 16 + (s & 1) * 8);
+      const uint32_t f[4] = {w.x & 0x0F0F0F0Fu, (w.x >> 4) & 0x0F0F0F0Fu, w.y & 0x0F0F0F0Fu, (w.y >> 4) & 0x0F0F0F0Fu};
+      int z0 = 0, z1 = 0;
+      if (ASYM && first) {
+        const uint32_t z = *reinterpret_cast<const uint32_t*>(sc + kPer * 32);
+        z0 = static_cast<int>(bf16_lo(z));
+        z1 = static_cast<int>(bf16_hi(z));
       }
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        const int s = h * kSteps + i;   // k-step of the piece
-        const uint4& wv = k.w[t][s >> 2];
-        const uint32_t word = (s & 3) == 0 ? wv.x : (s & 3) == 1 ? wv.y : (s & 3) == 2 ? wv.z : wv.w;
-        uint32_t f[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          f[r] = (__funnelshift_r(word, word, 4 * r) & 0x00780078u) | 0x3F803F80u;
-          if (decltype(sub)::value) f[r] = sub_bf16x2(f[r], (r & 1) ? z1 : z0);
-        }
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const uint4& x = k.x[n][s >> 1];
-          const uint32_t b0 = s & 1 ? x.z : x.x, b1 = s & 1 ? x.w : x.y;
-          if (i == 0)
-            mma_bf16_from(part[n], f, b0, b1, start[n][0], start[n][1], start[n][0], start[n][1]);
-          else
-            mma_bf16(part[n], f, b0, b1);
-        }
-      }
-      const float s0 = bf16_lo(k.sc[t][h]), s1 = bf16_hi(k.sc[t][h]);
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        acc[t][n][0] = fmaf(s0, part[n][0], acc[t][n][0]);
-        acc[t][n][1] = fmaf(s0, part[n][1], acc[t][n][1]);
-        acc[t][n][2] = fmaf(s1, part[n][2], acc[t][n][2]);
-        acc[t][n][3] = fmaf(s1, part[n][3], acc[t][n][3]);
-      }
-    }
-  };
-  auto use = [&](const Piece& k) {
-#pragma unroll
-    for (int h = 0; h < kGroups; ++h) {
-      float start[NT][2] = {};
-      bool exact = ASYM;
-      if (!ASYM) {
-        const uint32_t minus[4] = {0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u};   // -1.5
-        float sum[NT][4];
-#pragma unroll
-        for (int i = 0; i < GROUP / 16; ++i)
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const int s = h * (GROUP / 16) + i;
-            const uint4& x = k.x[n][s >> 1];
-            const uint32_t b0 = s & 1 ? x.z : x.x, b1 = s & 1 ? x.w : x.y;
-            if (i == 0)
-              mma_bf16_from(sum[n], minus, b0, b1, 0.f, 0.f, 0.f, 0.f);
-            else
-              mma_bf16(sum[n], minus, b0, b1);
-          }
-        float big = 0.f;
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          start[n][0] = sum[n][0];
-          start[n][1] = sum[n][1];
-          big = fmaf(sum[n][0], 0.f, fmaf(sum[n][1], 0.f, big));   // 0, or NaN
+        if (first) {
+          const int s0 = static_cast<int>(note[n].x), s1 = static_cast<int>(note[n].y);
+          part[t][n][0] = ASYM ? kMagic + z0 * s0 : s0;
+          part[t][n][1] = ASYM ? kMagic + z0 * s1 : s1;
+          part[t][n][2] = ASYM ? kMagic + z1 * s0 : s0;
+          part[t][n][3] = ASYM ? kMagic + z1 * s1 : s1;
         }
-        exact = __any_sync(0xffffffffu, big != 0.f);
+        mma_u8s8(part[t][n], f, s & 1 ? x[n].z : x[n].x, s & 1 ? x[n].w : x[n].y);
       }
-      if (exact) {
-        const float none[NT][2] = {};
-        group_of(k, h, none, std::true_type());
-      } else {
-        group_of(k, h, start, std::false_type());
+      if (last) {
+        const uint32_t two = *reinterpret_cast<const uint32_t*>(sc);
+        const float s0 = bf16_lo(two), s1 = bf16_hi(two);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const float h = __int_as_float(part[t][n][2 * q]) - 12582912.f, l = __int_as_float(part[t][n][2 * q + 1]) - 12582912.f;
+            const float v = LIMBS == 2 ? fmaf(h, 256.f, l) : fmaf(h, high, l * low);
+            acc[t][n][q] = fmaf(v * (q ? s1 : s0), __uint_as_float(note[n].z), acc[t][n][q]);
+          }
       }
     }
   };
+  auto write = [&](int u) {
 #pragma unroll
-  for (int d = 0; d < kAhead; ++d)
-    if (d < steps) load(ahead[d], d, d == odd_step);
-  for (int j = 0; j < steps; j += kAhead) {
+    for (int n = 0; n < NT; ++n) {
+      const int m = (static_cast<int>(blockIdx.y) * NT + n) * Image::kRows + c * Image::kRows / 4;
+      float o[TILES][2];
 #pragma unroll
-    for (int d = 0; d < kAhead; ++d) {
-      if (j + d < steps) {
-        use(ahead[d]);
-        if (j + d + kAhead < steps) load(ahead[d], d + kAhead, j + d + kAhead == odd_step);
+      for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          o[t][q] = acc[t][n][q];
+          if (LIMBS == 3) o[t][q] += __shfl_xor_sync(0xffffffffu, o[t][q], 1);   // the other bytes' lane
+        }
+      if (m >= a.M || (LIMBS == 3 && (c & 1))) continue;
+      const bool plain = reinterpret_cast<const int*>(a.ws + I.finite)[m] != 0;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int64_t row = (static_cast<int64_t>(u) * TILES + t) * 16 + g + 8 * q;
+          if (row >= L.N) continue;
+          float y = plain ? plain_product(a, row, m) : o[t][q];
+          if (a.resid) y += bf16_bits_to_f32(a.resid[m * a.ld_r + row]);
+          if (a.y_bf16)
+            static_cast<uint16_t*>(a.y)[m * a.ld_y + row] = bf16_bits_rn(y);
+          else
+            static_cast<float*>(a.y)[m * a.ld_y + row] = y;
+        }
+    }
+  };
+  float* mine = parts + local * 2 * kPart + lane;
+  auto clear = [&]() {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) acc[t][n][0] = acc[t][n][1] = 0.f;
+  };
+  auto leave = [&](int slot) {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) mine[slot * kPart + ((t * NT + n) * 2 + q) * 32] = acc[t][n][q];
+    clear();
+  };
+
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // the image is ready
+  bool begun = piece == 0;   // this warp holds its unit's first block
+  bool lost = false;         // a copy did not arrive in time
+  int stage = 0, left = count;
+  uint32_t phase = 0;
+  uint4 x0[NT], x1[NT], note[2][NT];
+  if (count > 0) {
+    load_image(x0, piece * 2);
+    load_note(note[0], piece * kPer);
+  }
+#pragma unroll 1
+  while (left > 0) {
+    if (!__all_sync(0xffffffffu, tc::mbar_wait(bars + stage, phase, a.err))) {
+      lost = true;
+      break;
+    }
+#pragma unroll
+    for (int b = 0; b < Smem::kBlocks; ++b) {
+      if (b > 0 && left <= 0) break;
+      const uint8_t* rec = ring + stage * Smem::kStage + b * kRecord;
+      const int after = piece + 1 == P ? 0 : piece + 1;
+      load_image(x1, piece * 2 + 1);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        // note[..] of group i of the block: with one group a block they change places from block to block
+        const int i = s / kSteps, at = kPer == 1 ? b & 1 : i & 1;
+        if (s % kSteps == 0) load_note(note[at ^ 1], i + 1 < kPer ? piece * kPer + i + 1 : after * kPer);
+        step(rec, s, s < 2 ? x0 : x1, note[at]);
+        if (s == 1) load_image(x0, after * 2);
+      }
+      if (kPer == 1 && Smem::kBlocks == 1) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) note[0][n] = note[1][n];
+      }
+      --left;
+      piece = after;
+      if (piece == 0) {
+        if (begun) {
+          write(unit);
+          clear();
+        } else {
+          leave(0);
+        }
+        ++unit;
+        begun = true;
       }
     }
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-      cw[t] += kAhead * kLinWarps * kSub * 32;
-      sw[t] += kAhead * kLinWarps * kGroups * 8;
-      if (ASYM) zw[t] += kAhead * kLinWarps * kGroups * 8;
+    __syncwarp();   // all lanes are done with the stage
+    issue(stage);
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1;
     }
-#pragma unroll
-    for (int n = 0; n < NT; ++n) xr[n] += kAhead * kLinWarps * kSub * 64;
   }
-
-  // ---- join the warps, then the cluster
-#pragma unroll
-  for (int t = 0; t < TILES; ++t)
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int q = 0; q < 4; ++q)
-        red[warp * kOut + (n * 8 + 2 * c + (q & 1)) * kRows + t * 16 + g + 8 * (q >> 1)] = acc[t][n][q];
-  __syncthreads();
-  for (int e = threadIdx.x; e < kOut; e += kLinThreads)
-    red[e] = (red[e] + red[kOut + e]) + (red[2 * kOut + e] + red[3 * kOut + e]);
+  // after a lost copy: the copies still under way end before the shared memory does
+  for (int under_way = lost ? (left - to_issue + Smem::kBlocks - 1) / Smem::kBlocks : 0; under_way > 0; --under_way) {
+    tc::mbar_wait(bars + stage, phase, a.err);
+    if (++stage == kStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+  // a unit that goes on in the next warp: one that this warp begins, or only passes through
+  const bool joins = piece > 0 && begun && count > 0;
+  if (piece > 0 && count > 0) leave(begun ? 1 : 0);
   if (S > 1)
     cluster.sync();
   else
     __syncthreads();
-  const int e0 = kOut * rank / S, e1 = kOut * (rank + 1) / S;
-  for (int e = e0 + threadIdx.x; e < e1; e += kLinThreads) {
-    const int m = m0 + e / kRows;
-    const int64_t n = static_cast<int64_t>(tile0) * 16 + e % kRows;
-    float o = 0.f;
-    for (int r = 0; r < S; ++r) o += S > 1 ? cluster.map_shared_rank(red, r)[e] : red[e];
-    if (m >= a.M || n >= L.N) continue;
-    o *= 16.f;   // the products are of code / 16
-    if (a.resid) o += bf16_bits_to_f32(a.resid[m * a.ld_r + n]);
-    if (a.y_bf16)
-      static_cast<uint16_t*>(a.y)[m * a.ld_y + n] = bf16_bits_rn(o);
-    else
-      static_cast<float*>(a.y)[m * a.ld_y + n] = o;
+  if (joins) {
+    const int64_t unit_end = static_cast<int64_t>(unit - u0 + 1) * P;
+    auto add = [&](const float* from) {
+#pragma unroll
+      for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) acc[t][n][q] += from[((t * NT + n) * 2 + q) * 32];
+    };
+    add(mine + kPart);
+#pragma unroll 4
+    for (int w = warp + 1; w < warps && begin_of(w) < unit_end; ++w)
+      add(cluster.map_shared_rank(parts + w / S * 2 * kPart + lane, w % S));
+    write(unit);
   }
-  if (S > 1) cluster.sync();   // the others have read this CTA's sums
+  if (S > 1) cluster.sync();   // the others have read this CTA's parts
 }
 
-template <int NT, int TILES, bool ASYM, int GROUP>
+// CTAs of a cluster: what leaves the fullest cluster the least to do for each of its CTAs
+// (28672 rows: 13 tiles a CTA alone, 12.5 in pairs), of the sizes whose clusters fit at once.
+int cluster_size(const void* kernel, int threads, int bytes, int units, int* size, int* clusters) {
+  double least = 0;
+  for (int S = 1; S <= 8; S *= 2) {
+    int have = num_sms();
+    if (S > 1) GLT_TRY(max_active_clusters(kernel, threads, bytes, S, &have));
+    const int use = units < have ? units : have;
+    const double load = static_cast<double>((units + use - 1) / use) / S;
+    if (S == 1 || load < least * 0.97) {
+      *size = S;
+      least = load;
+      *clusters = use;
+    }
+  }
+  return GLT_OK;
+}
+
+template <int LIMBS, int NT, int TILES, bool ASYM, int GROUP>
 int launch_linear(const LinearArgs& a, cudaStream_t st) {
-  const auto kernel = w4_linear_kernel<NT, TILES, ASYM, GROUP>;
-  constexpr int bytes = kLinWarps * 16 * TILES * 8 * NT * 4;
-  const int groups = (a.L.tiles + TILES - 1) / TILES, blocks = (a.M + 8 * NT - 1) / (8 * NT);
-  // CTAs a group of tiles: until the SMs hold six each, while every warp keeps two chunks
-  int S = 1;
-  while (S < 8 && static_cast<int64_t>(groups) * blocks * S < 6ll * num_sms() && a.L.chunks >= 4 * S * kLinWarps) S *= 2;
-  if (blocks > 65535) return fail(GLT_EINVAL, "w4: %d rows", a.M);
+  using Image = XImage<LIMBS>;
+  const auto kernel = w4_linear_kernel<LIMBS, NT, TILES, ASYM, GROUP>;
+  constexpr int bytes = LinearSmem<NT, TILES, ASYM, GROUP>::kBytes;
+  const Image I(a.L, a.M);
+  const int blocks = I.tiles / NT;
+  if (blocks > 65535 || a.M > 65535) return fail(GLT_EINVAL, "w4: %d rows (at most 65535)", a.M);
+  int clusters = 1, S = 1;
+  GLT_TRY(ensure_smem_attr(reinterpret_cast<const void*>(kernel), bytes));
+  GLT_TRY(cluster_size(reinterpret_cast<const void*>(kernel), 32 * linear_warps(NT), bytes,
+                       (a.L.tiles + TILES - 1) / TILES, &S, &clusters));
+  GLT_CUDA_TRY(cudaMemsetAsync(a.ws + I.finite, 0, sizeof(int) * a.M, st));
+  w4_prepare_kernel<LIMBS, GROUP><<<dim3((I.chunks * 8 + kPrepThreads - 1) / kPrepThreads, a.M), kPrepThreads, 0, st>>>(
+      a.x, a.ld_x, a.M, a.L, a.ws);
+  GLT_LAUNCH_CHECK();
+  // starts beside the preparation and waits for its end after the first loads of weights
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(groups) * S, blocks);
-  cfg.blockDim = dim3(kLinThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(clusters) * S, blocks);
+  cfg.blockDim = dim3(32 * linear_warps(NT));
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = S;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   GLT_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
   GLT_LAUNCH_CHECK();
   return GLT_OK;
 }
 
-template <int NT, int TILES>
+template <int LIMBS, int NT, int TILES>
 int launch_linear_as(const LinearArgs& a, cudaStream_t st) {
   if (a.L.asym) {
-    if (a.L.group == 32) return launch_linear<NT, TILES, true, 32>(a, st);
-    return a.L.group == 64 ? launch_linear<NT, TILES, true, 64>(a, st) : launch_linear<NT, TILES, true, 128>(a, st);
+    if (a.L.group == 32) return launch_linear<LIMBS, NT, TILES, true, 32>(a, st);
+    return a.L.group == 64 ? launch_linear<LIMBS, NT, TILES, true, 64>(a, st) : launch_linear<LIMBS, NT, TILES, true, 128>(a, st);
   }
-  if (a.L.group == 32) return launch_linear<NT, TILES, false, 32>(a, st);
-  return a.L.group == 64 ? launch_linear<NT, TILES, false, 64>(a, st) : launch_linear<NT, TILES, false, 128>(a, st);
+  if (a.L.group == 32) return launch_linear<LIMBS, NT, TILES, false, 32>(a, st);
+  return a.L.group == 64 ? launch_linear<LIMBS, NT, TILES, false, 64>(a, st) : launch_linear<LIMBS, NT, TILES, false, 128>(a, st);
+}
+
+template <int LIMBS>
+int launch_rows(const LinearArgs& a, cudaStream_t st) {
+  const int n = XImage<LIMBS>(a.L, a.M).per_cta;
+  if (n == 1) return launch_linear_as<LIMBS, 1, 1>(a, st);
+  if (n == 2) return launch_linear_as<LIMBS, 2, 1>(a, st);
+  if (n == 5) return launch_linear_as<LIMBS, 5, 2>(a, st);
+  return launch_linear_as<LIMBS, 8, 2>(a, st);
 }
 
 int grid_for(int64_t units, int per_cta) {
@@ -466,7 +698,7 @@ extern "C" int glt_w4_pack(const uint8_t* codes, const uint16_t* scales, const u
   GLT_TRY(glt::check_shape(N, K, group));
   if (!glt::aligned16(packed)) return glt::fail(GLT_EINVAL, "w4: packed weights must be 16-byte aligned");
   const W4Layout L(N, K, group, zeros != nullptr);
-  glt::w4_pack_kernel<<<glt::grid_for(static_cast<int64_t>(L.tiles) * L.chunks * 128, 256), 256, 0,
+  glt::w4_pack_kernel<<<glt::grid_for(L.bytes / 4, 256), 256, 0,
                         static_cast<cudaStream_t>(stream)>>>(codes, scales, zeros, L, static_cast<uint8_t*>(packed));
   GLT_LAUNCH_CHECK();
   return GLT_OK;
@@ -484,9 +716,20 @@ extern "C" int glt_w4_unpack(const void* packed, int N, int K, int group, int as
   return GLT_OK;
 }
 
+extern "C" int glt_w4_linear_workspace(int M, int N, int K, int group, int y_dtype, int64_t* bytes) {
+  if (!bytes) return glt::fail(GLT_EINVAL, "null argument");
+  GLT_TRY(glt::check_shape(N, K, group));
+  if (M < 0) return glt::fail(GLT_EINVAL, "w4: negative rows");
+  if (y_dtype != 0 && y_dtype != 1) return glt::fail(GLT_EINVAL, "w4: output type %d (0 fp32, 1 bf16)", y_dtype);
+  const W4Layout L(N, K, group, 0);
+  *bytes = M == 0 ? 0 : y_dtype ? glt::XImage<2>(L, M).bytes : glt::XImage<3>(L, M).bytes;
+  return GLT_OK;
+}
+
 extern "C" int glt_w4_linear(const void* packed, int N, int K, int group, int asym, const uint16_t* x,
                              int64_t ld_x, int M, void* y, int64_t ld_y, int y_dtype,
-                             const uint16_t* resid, int64_t ld_r, void* stream) {
+                             const uint16_t* resid, int64_t ld_r, void* workspace,
+                             int64_t workspace_bytes, void* stream) {
   GLT_TRY(glt::check_shape(N, K, group));
   if (!packed || (M > 0 && (!x || !y))) return glt::fail(GLT_EINVAL, "null argument");
   if (M < 0) return glt::fail(GLT_EINVAL, "w4: negative rows");
@@ -496,11 +739,13 @@ extern "C" int glt_w4_linear(const void* packed, int N, int K, int group, int as
   if (ld_y < N || (resid && ld_r < N)) return glt::fail(GLT_EINVAL, "w4: output or residual row stride below N %d", N);
   if (!glt::aligned16(packed)) return glt::fail(GLT_EINVAL, "w4: packed weights must be 16-byte aligned");
   if (M == 0) return GLT_OK;
-  const glt::LinearArgs a{static_cast<const uint8_t*>(packed), W4Layout(N, K, group, asym), x, ld_x, M, y, ld_y,
-                          y_dtype, resid, ld_r};
+  const W4Layout L(N, K, group, asym);
+  const int64_t need = y_dtype ? glt::XImage<2>(L, M).bytes : glt::XImage<3>(L, M).bytes;
+  if (workspace_bytes < need || !workspace || !glt::aligned16(workspace))
+    return glt::fail(GLT_EINVAL, "w4: workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
+  if (need / 4 > INT_MAX) return glt::fail(GLT_EINVAL, "w4: %d rows of %d columns", M, K);
+  const glt::LinearArgs a{static_cast<const uint8_t*>(packed), L, x, ld_x, M, y, ld_y, y_dtype, resid, ld_r,
+                          static_cast<uint8_t*>(workspace), glt::device_error_word()};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (M <= 8) return glt::launch_linear_as<1, 2>(a, st);
-  if (M <= 16) return glt::launch_linear_as<2, 2>(a, st);
-  if (M <= 24) return glt::launch_linear_as<3, 2>(a, st);
-  return glt::launch_linear_as<4, 2>(a, st);
+  return y_dtype ? glt::launch_rows<2>(a, st) : glt::launch_rows<3>(a, st);
 }

@@ -192,11 +192,15 @@ class W4Weight:
         if resid is not None:
             _need(resid.is_cuda and resid.dtype == torch.bfloat16 and resid.shape == (M, self.N) and
                   resid.stride(1) == 1, f"resid must be a bf16 CUDA tensor [{M}, {self.N}] with dense rows")
+        need = C.c_int64()
+        check(lib.glt_w4_linear_workspace(M, self.N, self.K, self.group, int(out.dtype == torch.bfloat16), C.byref(need)))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)
         check(lib.glt_w4_linear(self.packed.data_ptr(), self.N, self.K, self.group, int(self.asym), x.data_ptr(),
                                 x.stride(0) if M > 1 else self.K, M, out.data_ptr(),
                                 out.stride(0) if M > 1 else self.N, int(out.dtype == torch.bfloat16),
                                 None if resid is None else resid.data_ptr(),
-                                0 if resid is None else resid.stride(0) if M > 1 else self.N, _stream(x)))
+                                0 if resid is None else resid.stride(0) if M > 1 else self.N, ws.data_ptr(), need.value,
+                                _stream(x)))
         return out
 
 

@@ -325,8 +325,11 @@ GLT_API int glt_kv8_read(const GltKv8Cache* cache, const GltKv8Batch* batch, con
  * glt_w4_unpack: the bf16 (nearest) weights of a packed matrix.
  * glt_w4_linear: y[M, N] = x[M, K] . W^T (+ resid): x bf16 with row stride ld_x
  *   (a multiple of 8, 16-byte aligned), y bf16 (y_dtype 1) or fp32 (0), resid bf16
- *   or NULL; accumulation in fp32.  Made for the few rows of decoding: every 32
- *   rows read the weights once more. */
+ *   or NULL.  Made for the few rows of decoding: every 32 rows read the weights
+ *   once more (every 16 for fp32).  Sums of a group are exact integers, of groups fp32;
+ *   of an element of x, what lies below 2^-16 (fp32 results: 2^-24) of its group's
+ *   largest is rounded off.  At most 65535 rows.  workspace: at least glt_w4_linear_workspace bytes,
+ *   16-byte aligned, used by one call at a time; its contents do not matter. */
 GLT_API int glt_w4_packed_bytes(int N, int K, int group, int asym, int64_t* bytes);
 GLT_API int glt_w4_quantize(const uint16_t* w, int64_t ld_w, int N, int K, int group, int asym,
                             uint8_t* codes, uint16_t* scales, uint8_t* zeros, void* stream);
@@ -336,7 +339,9 @@ GLT_API int glt_w4_unpack(const void* packed, int N, int K, int group, int asym,
                           int64_t ld_w, void* stream);
 GLT_API int glt_w4_linear(const void* packed, int N, int K, int group, int asym, const uint16_t* x,
                           int64_t ld_x, int M, void* y, int64_t ld_y, int y_dtype,
-                          const uint16_t* resid, int64_t ld_r, void* stream);
+                          const uint16_t* resid, int64_t ld_r, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+GLT_API int glt_w4_linear_workspace(int M, int N, int K, int group, int y_dtype, int64_t* bytes);
 
 /* Log probabilities of given tokens, entropy and the most likely tokens, from
  * logits [rows, V] (dtype 0 fp32, 1 bf16; row stride ld), z = scale * logit with

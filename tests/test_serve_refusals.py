@@ -95,11 +95,12 @@ def test_w4_shapes(N, K, group):
     refused(lib.glt_w4_quantize(P, max(K, 1), N, K, group, 0, P, P, None, None), "w4")
     refused(lib.glt_w4_pack(P, P, None, N, K, group, P, None), "w4")
     refused(lib.glt_w4_unpack(P, N, K, group, 0, P, max(K, 1), None), "w4")
-    refused(lib.glt_w4_linear(P, N, K, group, 0, P, max(K, 8), 1, P, 64, 1, None, 0, None), "w4")
+    refused(lib.glt_w4_linear(P, N, K, group, 0, P, max(K, 8), 1, P, 64, 1, None, 0, P, 1 << 40, None), "w4")
+    refused(lib.glt_w4_linear_workspace(1, N, K, group, 1, C.byref(need)), "w4")
 
 
-def linear(x=P, ld_x=128, M=2, y=P, ld_y=40, yt=1, r=None, ld_r=0, packed=P):
-    return lib.glt_w4_linear(packed, 40, 128, 32, 0, x, ld_x, M, y, ld_y, yt, r, ld_r, None)
+def linear(x=P, ld_x=128, M=2, y=P, ld_y=40, yt=1, r=None, ld_r=0, packed=P, ws=P, n=1 << 40):
+    return lib.glt_w4_linear(packed, 40, 128, 32, 0, x, ld_x, M, y, ld_y, yt, r, ld_r, ws, n, None)
 
 
 def test_w4_arguments():
@@ -112,7 +113,14 @@ def test_w4_arguments():
     refused(linear(ld_y=39), "stride")
     refused(linear(r=P, ld_r=39), "stride")
     refused(linear(packed=P + 8), "aligned")
-    assert linear(M=0) == OK
+    need = C.c_int64()
+    assert lib.glt_w4_linear_workspace(2, 40, 128, 32, 1, C.byref(need)) == OK and need.value > 0
+    refused(linear(n=need.value - 1), "workspace")
+    refused(linear(ws=None), "workspace")
+    refused(linear(ws=P + 8), "workspace")
+    refused(lib.glt_w4_linear_workspace(-1, 40, 128, 32, 1, C.byref(need)), "rows")
+    refused(lib.glt_w4_linear_workspace(2, 40, 128, 32, 1, None), "null")
+    assert linear(M=0) == OK and linear(M=0, x=None, y=None, ws=None, n=0) == OK
     refused(lib.glt_w4_quantize(P, 128, 4, 128, 32, 1, P, P, None, None), "null")
     refused(lib.glt_w4_quantize(P, 127, 4, 128, 32, 0, P, P, None, None), "stride")
     refused(lib.glt_w4_packed_bytes(4, 128, 32, 0, None), "null")
