@@ -3,7 +3,8 @@
 // Packed layout of W [N, K]: rows in tiles of 16, columns in blocks of 128 (the last
 // one filled up with zero scales).  A block of a tile is one record, a tile's records follow
 // one another.  A record: two chunks of 64 columns, 128 words of eight codes each, then the
-// scales of the block's groups, [group][g][row half] bf16, then with asym the zeros alike.
+// scales of the block's groups, [group][g][row half] bf16, then with asym 15 - zero alike, as bytes
+// of a 32-bit word (row g, row g + 8, 0, 0).
 // Lane 4g + c of a warp owns words 4 * lane + s, s = 0..3, of a chunk; byte b of word s holds
 // the codes of row g (low nibble) and row g + 8 (high nibble) at column
 // (s / 2) * 32 + 8 c + (s % 2) * 4 + b.  So one AND (and a shift) makes four codes a register
@@ -114,8 +115,7 @@ __global__ void __launch_bounds__(256) w4_pack_kernel(const uint8_t* __restrict_
       for (int e = 0; e < 2; ++e) {
         const int64_t n = tile * 16 + (j & 7) + 8 * e;
         if (n >= L.N || grp >= ng) continue;
-        const uint32_t v = zero ? bf16_bits_rn(static_cast<float>(zeros[n * ng + grp] & 15u)) : scales[n * ng + grp];
-        word |= v << (16 * e);
+        word |= zero ? (15u - (zeros[n * ng + grp] & 15u)) << (8 * e) : static_cast<uint32_t>(scales[n * ng + grp]) << (16 * e);
       }
     }
     reinterpret_cast<uint32_t*>(packed)[q] = word;
@@ -131,7 +131,8 @@ __device__ __forceinline__ float w4_code(const uint8_t* packed, const W4Layout& 
   const uint32_t u = reinterpret_cast<const uint32_t*>(rec)[word] >> (8 * (kk & 3) + 4 * (r >> 3)) & 15u;
   const uint16_t* sc = reinterpret_cast<const uint16_t*>(rec + 1024) + ((k & 127) / L.group) * 16 + (r & 7) * 2 + (r >> 3);
   *scale = bf16_bits_to_f32(sc[0]);
-  return static_cast<float>(u) - (L.asym ? bf16_bits_to_f32(sc[L.per_block * 16]) : 8.f);
+  const int zero = L.asym ? 15 - rec[1024 + L.per_block * 32 + ((k & 127) / L.group) * 32 + (r & 7) * 4 + (r >> 3)] : 8;
+  return static_cast<float>(static_cast<int>(u) - zero);
 }
 
 __global__ void __launch_bounds__(256) w4_unpack_kernel(const uint8_t* __restrict__ packed, W4Layout L,
@@ -153,10 +154,10 @@ __device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], ui
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// ---- operand B.  Within a group of columns a row of x becomes fixed-point numbers
+// ---- operand B.  Within a block of 128 columns a row of x becomes fixed-point numbers
 // v = round(x 2^a), with a such that the largest fills 16 bits (LIMBS = 2) or 24 (LIMBS = 3), and
 // v its signed bytes, one column of operand B each.  Products with the codes are then exact
-// integers.  bf16 has 8 bits, so v is x exactly down to 2^-8 of the group's largest magnitude
+// integers.  bf16 has 8 bits, so v is x exactly down to 2^-8 of the block's largest magnitude
 // (2^-16 with three bytes), and off by at most 2^-16 (2^-24) of it below: two bytes for results
 // in bf16, three for results in fp32.
 // (On the tensor core, k = 32 of bytes costs what k = 16 of bf16 does, 8 cycles, and the codes need
@@ -164,9 +165,10 @@ __device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], ui
 // A tile of N = 8 columns holds 8 / LIMBS rows of x at 2 (or 4, the last empty) columns a row, high
 // byte first.  Image: [chunk of 64][tile of rows][lane][16 bytes], lane 4g + c the column g at the
 // k of operand A's lanes c.
+constexpr int kPrepThreads = 256;
 constexpr int kMagic = 0x4B400000;   // 1.5 2^23 as a float: kMagic + i is the float 1.5 2^23 + i
-// What lane c needs at the ends of a group: what its two columns' sums begin with, kMagic - 8 times
-// the sum of the bytes (asym: minus that sum), and 2^-a of its row.
+// What lane c needs at the ends of a group: what its two columns' sums begin with, kMagic - 8 (asym: 15)
+// times the sum of the bytes, and 2^-a of its row.
 struct __align__(16) GroupNote {
   int start[2];
   float factor;
@@ -177,6 +179,7 @@ struct XImage {
   static constexpr int kCols = LIMBS == 2 ? 2 : 4, kRows = 8 / kCols;   // columns a row, rows a tile
   int per_cta;   // tiles of rows of x that a CTA takes
   int tiles, chunks, groups;   // tiles filled up to per_cta's multiple; chunks and groups to the end of the last block
+  int slots;
   int64_t notes, finite, bytes;   // offsets in the workspace, after the image
   __host__ __device__ XImage(const W4Layout& L, int M) {
     const int need = (M + kRows - 1) / kRows;
@@ -187,12 +190,12 @@ struct XImage {
     notes = static_cast<int64_t>(chunks) * tiles * 512;
     // notes: [group][tile][lane c]
     finite = notes + static_cast<int64_t>(groups) * tiles * 4 * sizeof(GroupNote);
-    // finite: per row of x, its number of groups that are not finite
-    bytes = (finite + static_cast<int64_t>(M) * 4 + 15) / 16 * 16;
+    // finite: per row of x and CTA of the preparation, 0 where all is
+    slots = (chunks * 8 + kPrepThreads - 1) / kPrepThreads;
+    bytes = (finite + static_cast<int64_t>(M) * slots * 4 + 15) / 16 * 16;
   }
 };
 
-constexpr int kPrepThreads = 256;
 // A thread takes eight columns of a row, the threads of a group are neighbours.
 template <int LIMBS, int GROUP>
 __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const uint16_t* __restrict__ x, int64_t ld_x, int M,
@@ -216,9 +219,9 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const uint16_t
     else
       bad = true;
   }
-  constexpr int kLanes = GROUP / 8;
+  constexpr int kLanes = GROUP / 8;   // of a group; 16 of a block
 #pragma unroll
-  for (int o = 1; o < kLanes; o <<= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+  for (int o = 1; o < 16; o <<= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
   // the largest to [2^14, 2^15) or [2^22, 2^23), one less for the one mantissa whose high byte would be 128
   int a = 0;
   if (peak > 0.f) {
@@ -246,6 +249,8 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const uint16_t
   for (int o = 1; o < kLanes; o <<= 1)
 #pragma unroll
     for (int l = 0; l < LIMBS; ++l) sum[l] += __shfl_xor_sync(0xffffffffu, sum[l], o);
+  bad = __syncthreads_or(bad);
+  if (threadIdx.x == 0) reinterpret_cast<int*>(ws + I.finite)[m * I.slots + blockIdx.x] = bad;
   if (!in) return;
   const int chunk = v >> 3, step = (v >> 2) & 1, c = v & 3, tile = m / Image::kRows, row = m % Image::kRows;
   uint8_t* dst = ws + ((static_cast<int64_t>(chunk) * I.tiles + tile) * 32 + row * Image::kCols * 4 + c) * 16 + step * 8;
@@ -261,14 +266,13 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const uint16_t
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int b = 2 * j + e < LIMBS ? sum[2 * j + e < LIMBS ? 2 * j + e : 0] : 0;
-        n.start[e] = L.asym ? -b : kMagic - 8 * b;
+        n.start[e] = kMagic - (L.asym ? 15 : 8) * b;
       }
       n.factor = exp2f(static_cast<float>(-a));
       n.pad = 0;
       note[j] = n;
     }
   }
-  if (bad) atomicAdd(reinterpret_cast<int*>(ws + I.finite) + m, 1);   // zeroed before
 }
 
 struct LinearArgs {
@@ -316,8 +320,9 @@ __device__ __noinline__ float plain_product(const LinearArgs& a, int64_t n, int 
 //
 // Half a byte a weight leaves about 22 cycles of an SM for a tile's chunk, so instructions
 // count: 12 integer ones make the codes' fragments (8 AND, 4 shifts), two products do the
-// rest for four rows of x.  Zeros: sum v (u - z) = sum v u - z sum v, the second part, and the
-// number that turns the integer into a float, being what a group's sums begin with.
+// rest for four rows of x.  Zeros: sum v (u - 8) = sum v u - 8 sum v, the second part, and the
+// number that turns the integer into a float, being what a group's sums begin with; with stored
+// zeros the codes become u + (15 - z), 0..30, by one addition a register, and 15 takes the place of 8.
 __host__ __device__ constexpr int linear_warps(int nt) { return nt <= 2 ? 16 : 8; }
 constexpr int kStages = 4;
 
@@ -416,6 +421,7 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
 
   float acc[TILES][NT][2] = {};   // rows g, g + 8 of W by a row of a tile of x
   int part[TILES][NT][4];
+  float sum[TILES][NT][2];        // of a block's groups
   // k-step s of the record(s) at `rec`, with the image's chunk x and the group's note.
   auto step = [&](const uint8_t* rec, int s, const uint4 (&x)[NT], const uint4 (&note)[NT]) {
     const int grp = s / kSteps;
@@ -424,21 +430,17 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
     for (int t = 0; t < TILES; ++t) {
       const uint8_t* sc = rec + t * kRecord + 1024 + grp * 32 + g * 4;
       const uint2 w = *reinterpret_cast<const uint2*>(rec + t * kRecord + (s >> 1) * 512 + lane * 16 + (s & 1) * 8);
-      const uint32_t f[4] = {w.x & 0x0F0F0F0Fu, (w.x >> 4) & 0x0F0F0F0Fu, w.y & 0x0F0F0F0Fu, (w.y >> 4) & 0x0F0F0F0Fu};
-      int z0 = 0, z1 = 0;
-      if (ASYM && first) {
+      uint32_t f[4] = {w.x & 0x0F0F0F0Fu, (w.x >> 4) & 0x0F0F0F0Fu, w.y & 0x0F0F0F0Fu, (w.y >> 4) & 0x0F0F0F0Fu};
+      if (ASYM) {
         const uint32_t z = *reinterpret_cast<const uint32_t*>(sc + kPer * 32);
-        z0 = static_cast<int>(bf16_lo(z));
-        z1 = static_cast<int>(bf16_hi(z));
+        const uint32_t z0 = __byte_perm(z, 0, 0x0000), z1 = __byte_perm(z, 0, 0x1111);
+        f[0] += z0, f[1] += z1, f[2] += z0, f[3] += z1;
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         if (first) {
-          const int s0 = static_cast<int>(note[n].x), s1 = static_cast<int>(note[n].y);
-          part[t][n][0] = ASYM ? kMagic + z0 * s0 : s0;
-          part[t][n][1] = ASYM ? kMagic + z0 * s1 : s1;
-          part[t][n][2] = ASYM ? kMagic + z1 * s0 : s0;
-          part[t][n][3] = ASYM ? kMagic + z1 * s1 : s1;
+          part[t][n][0] = part[t][n][2] = static_cast<int>(note[n].x);
+          part[t][n][1] = part[t][n][3] = static_cast<int>(note[n].y);
         }
         mma_u8s8(part[t][n], f, s & 1 ? x[n].z : x[n].x, s & 1 ? x[n].w : x[n].y);
       }
@@ -451,7 +453,13 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
           for (int q = 0; q < 2; ++q) {
             const float h = __int_as_float(part[t][n][2 * q]) - 12582912.f, l = __int_as_float(part[t][n][2 * q + 1]) - 12582912.f;
             const float v = LIMBS == 2 ? fmaf(h, 256.f, l) : fmaf(h, high, l * low);
-            acc[t][n][q] = fmaf(v * (q ? s1 : s0), __uint_as_float(note[n].z), acc[t][n][q]);
+            // the row's 2^-a belongs to the block: its groups' sums meet it together
+            if (kPer == 1) {
+              acc[t][n][q] = fmaf(v * (q ? s1 : s0), __uint_as_float(note[n].z), acc[t][n][q]);
+            } else {
+              sum[t][n][q] = grp == 0 ? v * (q ? s1 : s0) : fmaf(v, q ? s1 : s0, sum[t][n][q]);
+              if (grp == kPer - 1) acc[t][n][q] = fmaf(sum[t][n][q], __uint_as_float(note[n].z), acc[t][n][q]);
+            }
           }
       }
     }
@@ -469,7 +477,8 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
           if (LIMBS == 3) o[t][q] += __shfl_xor_sync(0xffffffffu, o[t][q], 1);   // the other bytes' lane
         }
       if (m >= a.M || (LIMBS == 3 && (c & 1))) continue;
-      const bool plain = reinterpret_cast<const int*>(a.ws + I.finite)[m] != 0;
+      bool plain = false;
+      for (int i = 0; i < I.slots; ++i) plain |= reinterpret_cast<const int*>(a.ws + I.finite)[m * I.slots + i] != 0;
 #pragma unroll
       for (int t = 0; t < TILES; ++t)
 #pragma unroll
@@ -620,8 +629,7 @@ int launch_linear(const LinearArgs& a, cudaStream_t st) {
   GLT_TRY(ensure_smem_attr(reinterpret_cast<const void*>(kernel), bytes));
   GLT_TRY(cluster_size(reinterpret_cast<const void*>(kernel), 32 * linear_warps(NT), bytes,
                        (a.L.tiles + TILES - 1) / TILES, &S, &clusters));
-  GLT_CUDA_TRY(cudaMemsetAsync(a.ws + I.finite, 0, sizeof(int) * a.M, st));
-  w4_prepare_kernel<LIMBS, GROUP><<<dim3((I.chunks * 8 + kPrepThreads - 1) / kPrepThreads, a.M), kPrepThreads, 0, st>>>(
+  w4_prepare_kernel<LIMBS, GROUP><<<dim3(I.slots, a.M), kPrepThreads, 0, st>>>(
       a.x, a.ld_x, a.M, a.L, a.ws);
   GLT_LAUNCH_CHECK();
   // starts beside the preparation and waits for its end after the first loads of weights
