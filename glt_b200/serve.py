@@ -17,10 +17,31 @@ import torch
 from ._lib import GltKv8Batch as _CBatch, GltKv8Cache as _CCache, check, lib
 
 FORMATS = {"int8": 0, "e4m3": 1}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # the handle without a Stream object around it
+_capturing = torch.cuda.is_current_stream_capturing
+_BF16, _F32, _I32, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
 
 
 def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+    """The current stream of a tensor's device."""
+    i = t.get_device()
+    return _raw_stream(i) if _raw_stream is not None else torch.cuda.current_stream(i).cuda_stream
+
+
+class _Scratch:
+    """Workspaces of one object, one a stream: work on a stream runs in order, so its calls may share
+    one.  A call under capture gets its own, since graphs may replay side by side."""
+
+    def __init__(self):
+        self._held: dict[int, torch.Tensor] = {}
+
+    def get(self, nbytes: int, like: torch.Tensor, stream: int) -> torch.Tensor:
+        ws = self._held.get(stream)
+        if ws is None or ws.numel() < nbytes or ws.device != like.device or _capturing():
+            ws = torch.empty(max(nbytes, 16), dtype=_U8, device=like.device)
+            if not _capturing():
+                self._held[stream] = ws
+        return ws
 
 
 def _need(ok: bool, msg: str) -> None:
@@ -29,16 +50,19 @@ def _need(ok: bool, msg: str) -> None:
 
 
 def _int32(t: torch.Tensor, name: str) -> torch.Tensor:
-    _need(t.is_cuda and t.dtype == torch.int32 and t.is_contiguous(), f"{name} must be a contiguous int32 CUDA tensor")
+    if not (t.is_cuda and t.dtype is _I32 and t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous int32 CUDA tensor")
     return t
 
 
-def _rows(t: torch.Tensor, heads: int, hd: int, name: str) -> int:
+def _rows(t: torch.Tensor, rows: int, heads: int, hd: int, name: str) -> int:
     """Row stride of a bf16 [rows, heads, hd] tensor whose rows are dense."""
-    _need(t.is_cuda and t.dtype == torch.bfloat16 and tuple(t.shape[1:]) == (heads, hd),
-          f"{name} must be a bf16 CUDA tensor [rows, {heads}, {hd}], got {t.dtype} {tuple(t.shape)}")
-    _need(t.stride(2) == 1 and t.stride(1) == hd or t.numel() == 0, f"{name}: a row's heads must be contiguous")
-    return t.stride(0) if t.shape[0] > 1 else heads * hd
+    if not (t.is_cuda and t.dtype is _BF16 and t.shape == (rows, heads, hd)):
+        raise ValueError(f"{name} must be a bf16 CUDA tensor [{rows}, {heads}, {hd}], got {t.dtype} {tuple(t.shape)}")
+    s = t.stride()
+    if (s[2] != 1 or (s[1] != hd and heads > 1)) and t.numel():
+        raise ValueError(f"{name}: a row's heads must be contiguous")
+    return s[0] if rows > 1 else heads * hd
 
 
 class Kv8Batch:
@@ -62,6 +86,7 @@ class Kv8Batch:
         self._c = _CBatch(n, self.max_blocks, rows, max_new, block_table.data_ptr(), lengths.data_ptr(),
                           None if row_start is None else row_start.data_ptr())
         self._p = C.byref(self._c)
+        self._ws_bytes: dict[tuple, int] = {}   # attention's workspace by what it depends on
 
 
 class Kv8Cache:
@@ -95,39 +120,51 @@ class Kv8Cache:
         self._c = _CCache(FORMATS[fmt], self.block_tokens, self.num_kv_heads, self.head_dim, self.num_blocks,
                           k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
         self._p = C.byref(self._c)
+        self._scratch = _Scratch()
 
     def append(self, batch: Kv8Batch, k: torch.Tensor, v: torch.Tensor) -> None:
         """Write the step's keys and values, bf16 [rows, num_kv_heads, head_dim] (views into packed rows are fine)."""
-        _need(k.shape[0] == v.shape[0] == batch.rows, f"k and v must have {batch.rows} rows")
-        ld_k = _rows(k, self.num_kv_heads, self.head_dim, "k")
-        ld_v = _rows(v, self.num_kv_heads, self.head_dim, "v")
-        check(lib.glt_kv8_append(self._p, batch._p, k.data_ptr(), ld_k, v.data_ptr(), ld_v, _stream(k)))
+        ld_k = _rows(k, batch.rows, self.num_kv_heads, self.head_dim, "k")
+        ld_v = _rows(v, batch.rows, self.num_kv_heads, self.head_dim, "v")
+        st = lib.glt_kv8_append(self._p, batch._p, k.data_ptr(), ld_k, v.data_ptr(), ld_v, _stream(k))
+        if st:
+            check(st)
 
     def attention(self, batch: Kv8Batch, q: torch.Tensor, scale: float = 0.0, window: int = 0,
                   token_mask: torch.Tensor | None = None, out: torch.Tensor | None = None):
         """Attention of the step's queries, bf16 [rows, num_heads, head_dim], after ``append``.
         Returns (o like q, dense; lse fp32 [rows, num_heads])."""
-        _need(q.dim() == 3 and q.shape[0] == batch.rows, f"q must be [{batch.rows}, num_heads, head_dim]")
-        nh = q.shape[1]
-        ld_q = _rows(q, nh, self.head_dim, "q")
+        if q.dim() != 3:
+            raise ValueError("q must be [rows, num_heads, head_dim]")
+        rows, nh = batch.rows, q.shape[1]
+        ld_q = _rows(q, rows, nh, self.head_dim, "q")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _need(out.shape == q.shape, "out must have q's shape")
-        ld_o = _rows(out, nh, self.head_dim, "out")
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-        ld_m = 0
+            out = torch.empty(q.shape, dtype=_BF16, device=q.device)
+            ld_o = nh * self.head_dim
+        else:
+            ld_o = _rows(out, rows, nh, self.head_dim, "out")
+        lse = torch.empty((rows, nh), dtype=_F32, device=q.device)
+        mask, ld_m = None, 0
         if token_mask is not None:
-            _need(token_mask.is_cuda and token_mask.dtype in (torch.uint8, torch.bool) and token_mask.dim() == 2
-                  and token_mask.shape[0] == batch.num_seqs and token_mask.stride(1) == 1
-                  and token_mask.shape[1] >= batch.max_blocks * self.block_tokens,
-                  "token_mask must be bytes [num_seqs, at least max_blocks * block_tokens]")
+            width = batch.max_blocks * self.block_tokens
+            if not (token_mask.is_cuda and token_mask.dtype in (torch.uint8, torch.bool) and token_mask.dim() == 2
+                    and token_mask.shape[0] == batch.num_seqs and token_mask.stride(1) == 1
+                    and token_mask.shape[1] >= width):
+                raise ValueError(f"token_mask must be bytes [{batch.num_seqs}, at least {width}]")
+            mask = token_mask.data_ptr()
             ld_m = token_mask.stride(0) if token_mask.shape[0] > 1 else token_mask.shape[1]
-        need = C.c_int64()
-        check(lib.glt_kv8_attention_workspace(self._p, batch._p, nh, C.byref(need)))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=q.device)
-        check(lib.glt_kv8_attention(self._p, batch._p, q.data_ptr(), ld_q, out.data_ptr(), ld_o, lse.data_ptr(), nh,
-                                    scale, window, None if token_mask is None else token_mask.data_ptr(), ld_m,
-                                    ws.data_ptr(), need.value, _stream(q)))
+        key = (nh, self.num_kv_heads, self.block_tokens, self.head_dim)
+        need = batch._ws_bytes.get(key)
+        if need is None:
+            n = C.c_int64()
+            check(lib.glt_kv8_attention_workspace(self._p, batch._p, nh, C.byref(n)))
+            need = batch._ws_bytes[key] = n.value
+        stream = _stream(q)
+        ws = self._scratch.get(need, q, stream)
+        st = lib.glt_kv8_attention(self._p, batch._p, q.data_ptr(), ld_q, out.data_ptr(), ld_o, lse.data_ptr(), nh,
+                                   scale, window, mask, ld_m, ws.data_ptr(), need, stream)
+        if st:
+            check(st)
         return out, lse
 
     def read(self, batch: Kv8Batch, start: torch.Tensor | None, count: int):
@@ -136,9 +173,12 @@ class Kv8Cache:
         if start is not None:
             _need(_int32(start, "start").shape == (batch.num_seqs,), "start [num_seqs]")
         shape = (batch.num_seqs, count, self.num_kv_heads, self.head_dim)
-        k, v = (torch.empty(shape, device=self.k.device) for _ in range(2))
-        check(lib.glt_kv8_read(self._p, batch._p, None if start is None else start.data_ptr(), count, k.data_ptr(),
-                               v.data_ptr(), _stream(self.k)))
+        k = torch.empty(shape, dtype=_F32, device=self.k.device)
+        v = torch.empty(shape, dtype=_F32, device=self.k.device)
+        st = lib.glt_kv8_read(self._p, batch._p, None if start is None else start.data_ptr(), count, k.data_ptr(),
+                              v.data_ptr(), _stream(self.k))
+        if st:
+            check(st)
         return k, v
 
 
@@ -147,6 +187,8 @@ class W4Weight:
 
     def __init__(self, packed: torch.Tensor, N: int, K: int, group: int, asym: bool):
         self.packed, self.N, self.K, self.group, self.asym = packed, N, K, group, bool(asym)
+        self._ws_bytes: dict[tuple, int] = {}
+        self._scratch = _Scratch()
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None) -> "W4Weight":
@@ -181,26 +223,34 @@ class W4Weight:
     def linear(self, x: torch.Tensor, resid: torch.Tensor | None = None,
                out_dtype: torch.dtype = torch.bfloat16, out: torch.Tensor | None = None) -> torch.Tensor:
         """x . W^T (+ resid): x bf16 [M, K], result [M, N] in bf16 or fp32."""
+        N, K = self.N, self.K
+        if not (x.is_cuda and x.dtype is _BF16 and x.dim() == 2 and x.shape[1] == K and x.stride(1) == 1):
+            raise ValueError(f"x must be a bf16 CUDA tensor [M, {K}] with dense rows")
         M = x.shape[0]
-        _need(x.is_cuda and x.dtype == torch.bfloat16 and x.dim() == 2 and x.shape[1] == self.K and x.stride(1) == 1,
-              f"x must be a bf16 CUDA tensor [M, {self.K}] with dense rows")
+        one = M <= 1
         if out is None:
-            _need(out_dtype in (torch.bfloat16, torch.float32), "out_dtype must be bfloat16 or float32")
-            out = torch.empty(M, self.N, dtype=out_dtype, device=x.device)
-        _need(out.shape == (M, self.N) and out.dtype in (torch.bfloat16, torch.float32) and out.stride(1) == 1,
-              f"out must be [{M}, {self.N}] with dense rows")
-        if resid is not None:
-            _need(resid.is_cuda and resid.dtype == torch.bfloat16 and resid.shape == (M, self.N) and
-                  resid.stride(1) == 1, f"resid must be a bf16 CUDA tensor [{M}, {self.N}] with dense rows")
-        need = C.c_int64()
-        check(lib.glt_w4_linear_workspace(M, self.N, self.K, self.group, int(out.dtype == torch.bfloat16), C.byref(need)))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)
-        check(lib.glt_w4_linear(self.packed.data_ptr(), self.N, self.K, self.group, int(self.asym), x.data_ptr(),
-                                x.stride(0) if M > 1 else self.K, M, out.data_ptr(),
-                                out.stride(0) if M > 1 else self.N, int(out.dtype == torch.bfloat16),
-                                None if resid is None else resid.data_ptr(),
-                                0 if resid is None else resid.stride(0) if M > 1 else self.N, ws.data_ptr(), need.value,
-                                _stream(x)))
+            if out_dtype is not _BF16 and out_dtype is not _F32:
+                raise ValueError("out_dtype must be bfloat16 or float32")
+            out = torch.empty((M, N), dtype=out_dtype, device=x.device)
+        elif not (out.is_cuda and out.shape == (M, N) and out.dtype in (_BF16, _F32) and out.stride(1) == 1):
+            raise ValueError(f"out must be a bf16 or fp32 CUDA tensor [{M}, {N}] with dense rows")
+        bf16 = out.dtype is _BF16
+        if resid is not None and not (resid.is_cuda and resid.dtype is _BF16 and resid.shape == (M, N) and
+                                      resid.stride(1) == 1):
+            raise ValueError(f"resid must be a bf16 CUDA tensor [{M}, {N}] with dense rows")
+        need = self._ws_bytes.get((M, bf16))
+        if need is None:
+            n = C.c_int64()
+            check(lib.glt_w4_linear_workspace(M, N, K, self.group, bf16, C.byref(n)))
+            need = self._ws_bytes[M, bf16] = n.value
+        stream = _stream(x)
+        ws = self._scratch.get(need, x, stream)
+        st = lib.glt_w4_linear(self.packed.data_ptr(), N, K, self.group, self.asym, x.data_ptr(),
+                               K if one else x.stride(0), M, out.data_ptr(), N if one else out.stride(0), bf16,
+                               None if resid is None else resid.data_ptr(),
+                               0 if resid is None else N if one else resid.stride(0), ws.data_ptr(), need, stream)
+        if st:
+            check(st)
         return out
 
 
@@ -225,10 +275,21 @@ class TokenLogprobs(NamedTuple):
     scale: float
 
 
-def _logits(x: torch.Tensor) -> tuple[int, int]:
-    _need(x.is_cuda and x.dim() == 2 and x.dtype in (torch.bfloat16, torch.float32) and
-          (x.stride(1) == 1 or x.shape[1] == 1), "logits must be a bf16 or fp32 CUDA tensor [rows, V] with dense rows")
-    return int(x.dtype == torch.bfloat16), x.stride(0) if x.shape[0] > 1 else x.shape[1]
+def _logits(x: torch.Tensor, name: str = "logits") -> tuple[bool, int]:
+    """(whether bf16, row stride) of a [rows, V] tensor."""
+    if not (x.is_cuda and x.dim() == 2 and (x.dtype is _BF16 or x.dtype is _F32) and
+            (x.stride(1) == 1 or x.shape[1] == 1)):
+        raise ValueError(f"{name} must be a bf16 or fp32 CUDA tensor [rows, V] with dense rows")
+    return x.dtype is _BF16, x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _per_row(t: torch.Tensor | None, rows: int, dtype: torch.dtype, name: str) -> int | None:
+    """Address of a contiguous [rows] tensor, None for None."""
+    if t is None:
+        return None
+    if not (t.is_cuda and t.dtype is dtype and t.shape == (rows,) and t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous {dtype} CUDA tensor [{rows}]")
+    return t.data_ptr()
 
 
 def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, scale: float = 1.0,
@@ -237,18 +298,20 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor | None = None, sc
     the entropy, and the ``top`` most likely tokens."""
     dt, ld = _logits(logits)
     R, V = logits.shape
-    dev = logits.device
-    if targets is not None:
-        _need(_int32(targets, "targets").shape == (R,), "targets [rows]")
-    stats = torch.empty(3, R, device=dev)
-    ids = torch.empty(R, top, dtype=torch.int32, device=dev) if top else None
-    vals = torch.empty(R, top, device=dev) if top else None
-    logp = stats[0] if targets is not None else None
-    check(lib.glt_token_logprobs(logits.data_ptr(), dt, ld, R, V, None if targets is None else targets.data_ptr(),
-                                 scale, top, None if targets is None else logp.data_ptr(), stats[1].data_ptr(),
-                                 stats[2].data_ptr(), ids.data_ptr() if top else None,
-                                 vals.data_ptr() if top else None, _stream(logits)))
-    return TokenLogprobs(logp, stats[1], stats[2], ids, vals, scale)
+    t = _per_row(targets, R, _I32, "targets")
+    stats = torch.empty((3, R), dtype=_F32, device=logits.device)
+    at = stats.data_ptr()
+    ids = vals = ids_at = vals_at = None
+    if top > 0:
+        ids = torch.empty((R, top), dtype=_I32, device=logits.device)
+        vals = torch.empty((R, top), dtype=_F32, device=logits.device)
+        ids_at, vals_at = ids.data_ptr(), vals.data_ptr()
+    st = lib.glt_token_logprobs(logits.data_ptr(), dt, ld, R, V, t, scale, top, None if t is None else at, at + 4 * R,
+                                at + 8 * R, ids_at, vals_at, _stream(logits))
+    if st:
+        check(st)
+    logp, entropy, lse = stats.unbind()
+    return TokenLogprobs(None if targets is None else logp, entropy, lse, ids, vals, scale)
 
 
 def token_logprobs_bwd(logits: torch.Tensor, targets: torch.Tensor | None, fwd: TokenLogprobs,
@@ -258,20 +321,17 @@ def token_logprobs_bwd(logits: torch.Tensor, targets: torch.Tensor | None, fwd: 
     ``out`` may be the logits themselves."""
     dt, ld = _logits(logits)
     R, V = logits.shape
-    if targets is not None:
-        _need(_int32(targets, "targets").shape == (R,), "targets [rows]")
-    for t, name in ((d_logp, "d_logp"), (d_entropy, "d_entropy")):
-        _need(t is None or (t.is_cuda and t.dtype == torch.float32 and t.shape == (R,) and t.is_contiguous()),
-              f"{name} must be a contiguous fp32 CUDA tensor [{R}]")
     if out is None:
-        out = torch.empty(R, V, dtype=logits.dtype, device=logits.device)
-    _need(out.shape == logits.shape and out.dtype == logits.dtype, "out must have the logits' shape and dtype")
-    ld_o = _logits(out)[1]
-
-    def ptr(t):
-        return None if t is None else t.data_ptr()
-
-    check(lib.glt_token_logprobs_bwd(logits.data_ptr(), dt, ld, R, V, ptr(targets), fwd.scale, fwd.lse.data_ptr(),
-                                     fwd.entropy.data_ptr(), ptr(d_logp), ptr(d_entropy), out.data_ptr(), ld_o,
-                                     _stream(logits)))
+        out = torch.empty((R, V), dtype=logits.dtype, device=logits.device)
+        ld_o = V
+    else:
+        if out.shape != logits.shape or out.dtype is not logits.dtype:
+            raise ValueError("out must have the logits' shape and dtype")
+        ld_o = _logits(out, "out")[1]
+    st = lib.glt_token_logprobs_bwd(logits.data_ptr(), dt, ld, R, V, _per_row(targets, R, _I32, "targets"), fwd.scale,
+                                    _per_row(fwd.lse, R, _F32, "fwd.lse"), _per_row(fwd.entropy, R, _F32, "fwd.entropy"),
+                                    _per_row(d_logp, R, _F32, "d_logp"), _per_row(d_entropy, R, _F32, "d_entropy"),
+                                    out.data_ptr(), ld_o, _stream(logits))
+    if st:
+        check(st)
     return out
