@@ -36,12 +36,59 @@ int kv8_check(const GltKv8Cache* c, const GltKv8Batch* b) {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kMaxVec = 128 * 128 / 8 / kThreads;  // 8-value vectors a thread holds of one block
+
+// Eight codes of x / s, exactly: s, or 1 / s, may be out of the fast way's range, x not finite.
+__device__ __forceinline__ uint2 codes_exact(const float (&x)[8], float s, int format) {
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    const float y = s > 0.f && x[q] == x[q] ? x[q] / s : 0.f;
+    w[q >> 2] |= kv8_encode(y, format) << (8 * (q & 3));
+  }
+  return make_uint2(w[0], w[1]);
+}
+
+// The same by products with the two neighbours r (1 -+ 2^-21) of 1 / s.  The quotient, rounded,
+// lies between the two products, and rounding to a code keeps order, so equal codes are the
+// quotient's; where they differ (a code's boundary is that near: one element in some thousands)
+// the division decides.  A division an element took 25 us where this takes 10 (12.6 M elements).
+template <int FMT>
+__device__ __forceinline__ uint2 codes_fast(const float (&x)[8], float s, float lo, float hi) {
+  uint32_t w[2], differ = 0;
+  if constexpr (FMT == GLT_KV8_INT8) {
+    // x r + 1.5 2^23 is rounded to an integer, whose low byte is the code less its offset
+    uint32_t a[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      a[q] = __float_as_uint(fmaf(x[q], lo, 12582912.f));
+      differ |= a[q] ^ __float_as_uint(fmaf(x[q], hi, 12582912.f));
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      w[h] = __byte_perm(__byte_perm(a[4 * h], a[4 * h + 1], 0x0040), __byte_perm(a[4 * h + 2], a[4 * h + 3], 0x0040), 0x5410) ^ 0x80808080u;
+  } else {
+    uint16_t a[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint16_t b;
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a[q]) : "f"(x[2 * q + 1] * lo), "f"(x[2 * q] * lo));
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b) : "f"(x[2 * q + 1] * hi), "f"(x[2 * q] * hi));
+      differ |= a[q] ^ b;
+    }
+    w[0] = a[0] | static_cast<uint32_t>(a[1]) << 16;
+    w[1] = a[2] | static_cast<uint32_t>(a[3]) << 16;
+  }
+  if (differ) return codes_exact(x, s, FMT);
+  return make_uint2(w[0], w[1]);
+}
 
 // One CTA: the part of one sequence's new tokens that falls into one block, for
 // one KV head, keys (z = 0) or values (z = 1).  The rows are read once and kept
-// in registers between the scale and the codes.
-__global__ void __launch_bounds__(kThreads) kv8_append_kernel(GltKv8Cache c, GltKv8Batch b,
+// in registers between the scale and the codes.  HBM bounds prompts, the chain length ->
+// table -> scale bounds single tokens, so all that can be is loaded before the maximum.
+// VECS: vectors of eight values a thread holds of a whole block.
+template <int FMT, int VECS>
+__global__ void __launch_bounds__(kThreads, VECS <= 4 ? 5 : 3) kv8_append_kernel(GltKv8Cache c, GltKv8Batch b,
                                                               const uint16_t* __restrict__ k, int64_t ld_k,
                                                               const uint16_t* __restrict__ v, int64_t ld_v,
                                                               unsigned int* err) {
@@ -55,99 +102,127 @@ __global__ void __launch_bounds__(kThreads) kv8_append_kernel(GltKv8Cache c, Glt
   if (lo >= hi) return;
   const int64_t id = kv8_block(c, b, seq, index, blockIdx.z == 0 && threadIdx.x == 0 ? err : nullptr);
   if (id < 0) return;
-  const int vecs = c.head_dim >> 3;
+  const int vec_log = c.head_dim == 128 ? 4 : 3;   // vectors of eight values in a row
   const int64_t slab = (id * c.num_kv_heads + head) * c.block_tokens * c.head_dim;
-  uint8_t* codes = (is_v ? c.v : c.k) + slab;
+  uint2* codes = reinterpret_cast<uint2*>((is_v ? c.v : c.k) + slab);
   float* scale = (is_v ? c.v_scale : c.k_scale) + id * c.num_kv_heads + head;
   const int64_t ld = is_v ? ld_v : ld_k;
   const uint16_t* src = (is_v ? v : k) + (sp.row0 + static_cast<int64_t>(base + lo - sp.past)) * ld + head * c.head_dim;
-  const int n = (hi - lo) * vecs;
-  uint4 x[kMaxVec];
-  float peak = 0.f;
+  const int n = (hi - lo) << vec_log, held = lo << vec_log;
+  // the block's own tokens of earlier steps keep its scale from falling
+  const float before = lo > 0 ? *scale : 0.f;
+  uint4 x[VECS];
+  uint2 old[VECS];
 #pragma unroll
-  for (int j = 0; j < kMaxVec; ++j) {
+  for (int j = 0; j < VECS; ++j) {
     const int i = threadIdx.x + j * kThreads;
-    if (i >= n) break;
-    x[j] = *reinterpret_cast<const uint4*>(src + (i / vecs) * ld + (i % vecs) * 8);
+    if (i < n) x[j] = *reinterpret_cast<const uint4*>(src + (i >> vec_log) * ld + (i & ((1 << vec_log) - 1)) * 8);
+    if (i < held) old[j] = codes[i];
+  }
+  float peak = 0.f;
+  bool odd = false;   // something not finite among this thread's values
+#pragma unroll
+  for (int j = 0; j < VECS; ++j) {
+    if (threadIdx.x + j * kThreads >= n) break;
     float f[8];
     unpack8(x[j], f);
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
       const float a = fabsf(f[q]);
-      if (a <= FLT_MAX) peak = fmaxf(peak, a);
+      if (a <= FLT_MAX)
+        peak = fmaxf(peak, a);
+      else
+        odd = true;
     }
   }
   peak = warp_max(peak);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = peak;
-  // the block's own tokens of earlier steps keep its scale from falling
-  const float before = lo > 0 ? *scale : 0.f;
   __syncthreads();
-  for (int w = 0; w < kThreads / 32; ++w) peak = fmaxf(peak, red[w]);
-  const float after = fmaxf(before, peak / kv8_top(c.format));
 #pragma unroll
-  for (int j = 0; j < kMaxVec; ++j) {
+  for (int w = 0; w < kThreads / 32; ++w) peak = fmaxf(peak, red[w]);
+  const float after = fmaxf(before, peak / kv8_top(FMT));
+  const bool fast = !odd && after >= 1e-30f;
+  const float r = 1.f / after, r_lo = r * (1.f - 0x1p-21f), r_hi = r * (1.f + 0x1p-21f);
+#pragma unroll
+  for (int j = 0; j < VECS; ++j) {
     const int i = threadIdx.x + j * kThreads;
     if (i >= n) break;
     float f[8];
     unpack8(x[j], f);
-    uint32_t w[2] = {0, 0};
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const float y = after > 0.f && f[q] == f[q] ? f[q] / after : 0.f;
-      w[q >> 2] |= kv8_encode(y, c.format) << (8 * (q & 3));
-    }
-    *reinterpret_cast<uint2*>(codes + (lo * vecs + i) * 8) = make_uint2(w[0], w[1]);
+    codes[held + i] = fast ? codes_fast<FMT>(f, after, r_lo, r_hi) : codes_exact(f, after, FMT);
   }
   if (after > before) {
-    for (int i = threadIdx.x; i < lo * vecs; i += kThreads) {
-      const uint2 old = *reinterpret_cast<const uint2*>(codes + i * 8);
-      const uint32_t o[2] = {old.x, old.y};
-      uint32_t w[2] = {0, 0};
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const float val = kv8_decode((o[q >> 2] >> (8 * (q & 3))) & 0xFFu, c.format) * before;
-        w[q >> 2] |= kv8_encode(val / after, c.format) << (8 * (q & 3));
-      }
-      *reinterpret_cast<uint2*>(codes + i * 8) = make_uint2(w[0], w[1]);
+    for (int j = 0; j < VECS; ++j) {
+      const int i = threadIdx.x + j * kThreads;
+      if (i >= held) break;
+      const uint32_t o[2] = {old[j].x, old[j].y};
+      float f[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) f[q] = kv8_decode((o[q >> 2] >> (8 * (q & 3))) & 0xFFu, FMT) * before;
+      codes[i] = after >= 1e-30f ? codes_fast<FMT>(f, after, r_lo, r_hi) : codes_exact(f, after, FMT);
     }
   }
-  // every thread has read the old scale (it is behind the barrier above)
-  if (threadIdx.x == 0) *scale = after;
+  // every thread has read the old scale (before the barrier above)
+  if (threadIdx.x == 0 && (lo == 0 || after > before)) *scale = after;
 }
 
-// One CTA a position: 8 values a thread of all heads, keys then values.
+// One CTA: the positions of one sequence that lie in one block, for one KV head, keys (z = 0) or values.
+constexpr int kReadBatch = 8;
 __global__ void __launch_bounds__(kThreads) kv8_read_kernel(GltKv8Cache c, GltKv8Batch b,
                                                             const int32_t* __restrict__ start, int count,
                                                             float* __restrict__ k, float* __restrict__ v,
                                                             unsigned int* err) {
-  const int seq = blockIdx.y;
-  const Kv8Span sp = kv8_span(b, seq, c.block_tokens, blockIdx.x == 0 && threadIdx.x == 0 ? err : nullptr);
-  const int vecs = c.head_dim >> 3, per = c.num_kv_heads * vecs;
-  for (int i = blockIdx.x; i < count; i += gridDim.x) {
-    const int64_t pos = (start ? start[seq] : 0) + static_cast<int64_t>(i);
-    int64_t id = -1;
-    if (pos >= 0 && pos < sp.past + sp.n)
-      id = kv8_block(c, b, seq, static_cast<int>(pos / c.block_tokens), threadIdx.x == 0 ? err : nullptr);
-    const int64_t out = (static_cast<int64_t>(seq) * count + i) * per * 8;
-    for (int u = threadIdx.x; u < 2 * per; u += kThreads) {
-      const bool is_v = u >= per;
-      const int w = is_v ? u - per : u, head = w / vecs;
-      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (id >= 0) {
-        const int64_t hb = id * c.num_kv_heads + head;
-        const float s = (is_v ? c.v_scale : c.k_scale)[hb];
-        const uint2 old = *reinterpret_cast<const uint2*>((is_v ? c.v : c.k) +
-                                                          (hb * c.block_tokens + pos % c.block_tokens) * c.head_dim +
-                                                          (w % vecs) * 8);
-        const uint32_t o[2] = {old.x, old.y};
+  const int seq = blockIdx.y, bt = c.block_tokens;
+  const Kv8Span sp = kv8_span(b, seq, bt, blockIdx.x == 0 && threadIdx.x == 0 ? err : nullptr);
+  const int64_t from = start ? start[seq] : 0;
+  const int64_t end = sp.past + sp.n;
+  // cut at multiples of a block's tokens, below zero too
+  const int64_t cut = (from >= 0 ? from / bt : -((-from + bt - 1) / bt)) + blockIdx.x;
+  const int64_t p0 = max(from, cut * bt), p1 = min(from + count, (cut + 1) * bt);
+  if (p0 >= p1) return;
+  int64_t id = -1;
+  if (p0 >= 0 && p0 < end) id = kv8_block(c, b, seq, static_cast<int>(cut), threadIdx.x == 0 ? err : nullptr);
+  const int vec_log = c.head_dim == 128 ? 5 : 4, vecs = 1 << vec_log;   // of four values
+  const int head = blockIdx.z >> 1, total = static_cast<int>(p1 - p0) << vec_log;
+  const bool is_v = blockIdx.z & 1;
+  const int64_t hb = id * c.num_kv_heads + head;
+  const uint32_t* codes = reinterpret_cast<const uint32_t*>((is_v ? c.v : c.k) + (hb * bt + (p0 - cut * bt)) * c.head_dim);
+  const int held = id >= 0 ? static_cast<int>(min(static_cast<int64_t>(total), (end - p0) << vec_log)) : 0;   // vectors the sequence holds
+  const float s = held > 0 ? (is_v ? c.v_scale : c.k_scale)[hb] : 0.f;
+  float* dst = (is_v ? v : k) + ((static_cast<int64_t>(seq) * count + (p0 - from)) * c.num_kv_heads + head) * c.head_dim;
+  const int64_t row = static_cast<int64_t>(c.num_kv_heads) * c.head_dim;
+  for (int u = threadIdx.x; u < total; u += kReadBatch * kThreads) {
+    uint32_t w[kReadBatch];
 #pragma unroll
-        for (int q = 0; q < 8; ++q) f[q] = kv8_decode((o[q >> 2] >> (8 * (q & 3))) & 0xFFu, c.format) * s;
-      }
-      float* dst = (is_v ? v : k) + out + w * 8;
-      reinterpret_cast<float4*>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
-      reinterpret_cast<float4*>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
+    for (int j = 0; j < kReadBatch; ++j) {
+      const int i = u + j * kThreads;
+      w[j] = c.format == GLT_KV8_INT8 ? 0x80808080u : 0u;   // codes of 0
+      if (i < held) w[j] = codes[i];
+    }
+#pragma unroll
+    for (int j = 0; j < kReadBatch; ++j) {
+      const int i = u + j * kThreads;
+      if (i >= total) break;
+      float f[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) f[q] = kv8_decode((w[j] >> (8 * q)) & 0xFFu, c.format) * s;
+      *reinterpret_cast<float4*>(dst + (i >> vec_log) * row + (i & (vecs - 1)) * 4) = make_float4(f[0], f[1], f[2], f[3]);
     }
   }
+}
+
+template <int FMT>
+int launch_append(const GltKv8Cache& c, const GltKv8Batch& b, const uint16_t* k, int64_t ld_k, const uint16_t* v,
+                  int64_t ld_v, cudaStream_t st) {
+  // blocks a sequence's new tokens can reach into, the first one partly filled
+  const dim3 grid((b.max_new + c.block_tokens - 2) / c.block_tokens + 1, b.num_seqs, 2 * c.num_kv_heads);
+  const int vecs = c.block_tokens * c.head_dim / 8;
+  const auto kernel = vecs <= kThreads ? kv8_append_kernel<FMT, 1> : vecs <= 2 * kThreads ? kv8_append_kernel<FMT, 2>
+                      : vecs <= 4 * kThreads ? kv8_append_kernel<FMT, 4> : kv8_append_kernel<FMT, 8>;
+  kernel<<<grid, kThreads, 0, st>>>(c, b, k, ld_k, v, ld_v, device_error_word());
+  GLT_LAUNCH_CHECK();
+  return GLT_OK;
 }
 
 }  // namespace
@@ -162,13 +237,9 @@ extern "C" int glt_kv8_append(const GltKv8Cache* cache, const GltKv8Batch* batch
   if (ld_k < width || ld_v < width || ld_k % 8 || ld_v % 8 || !glt::aligned16(k) || !glt::aligned16(v))
     return glt::fail(GLT_EINVAL, "kv8: new rows must be 16-byte aligned (strides multiples of 8, at least %lld)", (long long)width);
   if (batch->max_new == 0) return GLT_OK;
-  const int bt = cache->block_tokens;
-  // blocks a sequence's new tokens can reach into, the first one partly filled
-  const dim3 grid((batch->max_new + bt - 2) / bt + 1, batch->num_seqs, 2 * cache->num_kv_heads);
-  glt::kv8_append_kernel<<<grid, glt::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-      *cache, *batch, k, ld_k, v, ld_v, glt::device_error_word());
-  GLT_LAUNCH_CHECK();
-  return GLT_OK;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return cache->format == GLT_KV8_INT8 ? glt::launch_append<GLT_KV8_INT8>(*cache, *batch, k, ld_k, v, ld_v, st)
+                                       : glt::launch_append<GLT_KV8_E4M3>(*cache, *batch, k, ld_k, v, ld_v, st);
 }
 
 extern "C" int glt_kv8_read(const GltKv8Cache* cache, const GltKv8Batch* batch, const int32_t* start,
@@ -178,7 +249,8 @@ extern "C" int glt_kv8_read(const GltKv8Cache* cache, const GltKv8Batch* batch, 
   if (count == 0 || batch->num_seqs == 0) return GLT_OK;
   if (!k || !v) return glt::fail(GLT_EINVAL, "null argument");
   if (!glt::aligned16(k) || !glt::aligned16(v)) return glt::fail(GLT_EINVAL, "kv8: outputs must be 16-byte aligned");
-  const dim3 grid(count < 65535 ? count : 65535, batch->num_seqs);
+  // blocks a range can touch
+  const dim3 grid((count + cache->block_tokens - 2) / cache->block_tokens + 1, batch->num_seqs, 2 * cache->num_kv_heads);
   glt::kv8_read_kernel<<<grid, glt::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
       *cache, *batch, start, count, k, v, glt::device_error_word());
   GLT_LAUNCH_CHECK();
