@@ -140,6 +140,15 @@ __device__ __forceinline__ void exchange(uint64_t& key, int partner, bool larger
   if ((o > key) == larger) key = o;
 }
 
+// A warp's 32 keys in falling order.
+__device__ __forceinline__ uint64_t falling(uint64_t key, int lane) {
+#pragma unroll
+  for (int n = 2; n <= 32; n <<= 1)
+#pragma unroll
+    for (int d = n >> 1; d > 0; d >>= 1) exchange(key, d, ((lane & d) == 0) == ((lane & n) == 0 || n == 32));
+  return key;
+}
+
 // The largest keys a warp has seen, one a lane in falling order (0: none).
 struct TopList {
   uint64_t key = 0;
@@ -151,13 +160,7 @@ struct TopList {
     for (int d = 16; d > 0; d >>= 1) exchange(key, d, (lane & d) == 0);
   }
   // Takes 32 keys in any order.
-  __device__ __forceinline__ void merge_unsorted(uint64_t other, int lane) {
-#pragma unroll
-    for (int n = 2; n <= 32; n <<= 1)
-#pragma unroll
-      for (int d = n >> 1; d > 0; d >>= 1) exchange(other, d, ((lane & d) == 0) == ((lane & n) == 0 || n == 32));
-    merge(other, lane);
-  }
+  __device__ __forceinline__ void merge_unsorted(uint64_t other, int lane) { merge(falling(other, lane), lane); }
   // Takes every lane's candidate (0: none) that ranks above the top-th.
   __device__ __forceinline__ void take(uint64_t cand, int top, int lane) {
     uint32_t who = __ballot_sync(0xffffffffu, cand > __shfl_sync(0xffffffffu, key, top - 1));
@@ -306,7 +309,10 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(
   // no worse than (its maximum, last index)
   uint64_t upper = 0, lower = 0;
   if (top > 0 && best >= 0) {
-    const int last = min(best + (kBatch - 1) * kThreads, v1 - 1);
+    int last = best;   // the thread's own last vector of the batch: no two threads may share a lower key
+#pragma unroll
+    for (int j = 1; j < kBatch; ++j)
+      if (best + j * kThreads < v1) last = best + j * kThreads;
     upper = rank_key(st.m, row.head + best * kVec);
     lower = rank_key(st.m, row.head + last * kVec + kVec - 1);
   }
@@ -329,17 +335,8 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(
   // every warp's few largest lower keys
   const int pick = (top + kWarps - 1) / kWarps + 2;
   if (top > 0) {
-    uint64_t left = lower;
-    for (int q = 0; q < pick; ++q) {
-      uint64_t most = left;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const uint64_t k = __shfl_xor_sync(0xffffffffu, most, o);
-        if (k > most) most = k;
-      }
-      if (left == most) left = 0;   // keys are distinct, or 0
-      if (lane == 0) sm.maxima[warp * pick + q] = most;
-    }
+    const uint64_t sorted = falling(lower, lane);
+    if (lane < pick) sm.maxima[warp * pick + lane] = sorted;
   }
   __syncthreads();
   if (lane == 0 && bad) sm.bad = 1;
@@ -347,6 +344,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(
     // the one that top - 1 others exceed
     const uint64_t mine = sm.maxima[threadIdx.x];
     int above = 0;
+#pragma unroll 8
     for (int i = 0; i < kWarps * pick; ++i) above += sm.maxima[i] > mine;
     if (above == top - 1 && mine > 0) sm.least = mine;
   }
