@@ -196,15 +196,12 @@ struct XImage {
   }
 };
 
-// A thread takes eight columns of a row, the threads of a group are neighbours.
+// Eight columns (vector v) of row m of x into the image at ws; the threads of a block's 16 vectors are
+// neighbours and all here.  Returns whether something is not finite.
 template <int LIMBS, int GROUP>
-__global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const uint16_t* __restrict__ x, int64_t ld_x, int M,
-                                                                  W4Layout L, uint8_t* __restrict__ ws) {
+__device__ __forceinline__ bool prepare_vector(const uint16_t* __restrict__ x, int64_t ld_x, const W4Layout& L,
+                                               const XImage<LIMBS>& I, int m, int v, uint8_t* ws) {
   using Image = XImage<LIMBS>;
-  const Image I(L, M);
-  asm volatile("griddepcontrol.launch_dependents;");
-  const int m = blockIdx.y;
-  const int v = blockIdx.x * kPrepThreads + threadIdx.x;   // of chunks * 8 = blocks * 16
   const bool in = v < I.chunks * 8;
   uint4 u = make_uint4(0, 0, 0, 0);
   if (in && v * 8 < L.K) u = *reinterpret_cast<const uint4*>(x + m * ld_x + v * 8);
@@ -249,9 +246,7 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const uint16_t
   for (int o = 1; o < kLanes; o <<= 1)
 #pragma unroll
     for (int l = 0; l < LIMBS; ++l) sum[l] += __shfl_xor_sync(0xffffffffu, sum[l], o);
-  bad = __syncthreads_or(bad);
-  if (threadIdx.x == 0) reinterpret_cast<int*>(ws + I.finite)[m * I.slots + blockIdx.x] = bad;
-  if (!in) return;
+  if (!in) return bad;
   const int chunk = v >> 3, step = (v >> 2) & 1, c = v & 3, tile = m / Image::kRows, row = m % Image::kRows;
   uint8_t* dst = ws + ((static_cast<int64_t>(chunk) * I.tiles + tile) * 32 + row * Image::kCols * 4 + c) * 16 + step * 8;
 #pragma unroll
@@ -273,6 +268,17 @@ __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const uint16_t
       note[j] = n;
     }
   }
+  return bad;
+}
+
+template <int LIMBS, int GROUP>
+__global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const uint16_t* __restrict__ x, int64_t ld_x, int M,
+                                                                  W4Layout L, uint8_t* __restrict__ ws) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  const XImage<LIMBS> I(L, M);
+  const int m = blockIdx.y;
+  const bool bad = __syncthreads_or(prepare_vector<LIMBS, GROUP>(x, ld_x, L, I, m, blockIdx.x * kPrepThreads + threadIdx.x, ws));
+  if (threadIdx.x == 0) reinterpret_cast<int*>(ws + I.finite)[m * I.slots + blockIdx.x] = bad;
 }
 
 struct LinearArgs {
@@ -337,7 +343,7 @@ struct LinearSmem {
   static constexpr int kBytes = kWarps * (kRing + 2 * kPart * 4 + kStages * 8);
 };
 
-template <int LIMBS, int NT, int TILES, bool ASYM, int GROUP>
+template <int LIMBS, int NT, int TILES, bool ASYM, int GROUP, bool FUSED>
 __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(const __grid_constant__ LinearArgs a) {
   using Smem = LinearSmem<NT, TILES, ASYM, GROUP>;
   constexpr int kWarps = Smem::kWarps, kRecord = Smem::kRecord, kPart = Smem::kPart;
@@ -402,10 +408,23 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
 #pragma unroll 1
   for (int i = 0; i < kStages; ++i) issue(i);
 
-  // ---- the image and its notes, one chunk and one group ahead
+  // ---- the image: the workspace's, or (FUSED) made here, in shared memory, while the ring fills
+  const uint8_t* img = a.ws;
+  if (FUSED) {
+    uint8_t* own = smem + Smem::kBytes;
+    int* flags = reinterpret_cast<int*>(own + I.finite);
+    for (int i = threadIdx.x; i < a.M * I.slots; i += 32 * kWarps) flags[i] = 0;
+    __syncthreads();
+    for (int m = 0; m < a.M; ++m)
+      for (int v = 0; v < I.chunks * 8; v += 32 * kWarps)
+        if (prepare_vector<LIMBS, GROUP>(a.x, a.ld_x, L, I, m, v + threadIdx.x, own)) atomicOr(flags + m * I.slots, 1);
+    __syncthreads();
+    img = own;
+  }
+  // image and notes are read one chunk and one group ahead
   const int image_chunk = I.tiles * 32, note_group = I.tiles * 4;   // strides, in elements
-  const uint4* image = reinterpret_cast<const uint4*>(a.ws) + blockIdx.y * NT * 32 + lane;
-  const uint4* notes = reinterpret_cast<const uint4*>(a.ws + I.notes) + blockIdx.y * NT * 4 + c;
+  const uint4* image = reinterpret_cast<const uint4*>(img) + blockIdx.y * NT * 32 + lane;
+  const uint4* notes = reinterpret_cast<const uint4*>(img + I.notes) + blockIdx.y * NT * 4 + c;
   auto load_image = [&](uint4 (&x)[NT], int chunk) {
     const uint4* p = image + chunk * image_chunk;
 #pragma unroll
@@ -478,7 +497,7 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
         }
       if (m >= a.M || (LIMBS == 3 && (c & 1))) continue;
       bool plain = false;
-      for (int i = 0; i < I.slots; ++i) plain |= reinterpret_cast<const int*>(a.ws + I.finite)[m * I.slots + i] != 0;
+      for (int i = 0; i < I.slots; ++i) plain |= reinterpret_cast<const int*>(img + I.finite)[m * I.slots + i] != 0;
 #pragma unroll
       for (int t = 0; t < TILES; ++t)
 #pragma unroll
@@ -511,7 +530,7 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
     clear();
   };
 
-  asm volatile("griddepcontrol.wait;" ::: "memory");   // the image is ready
+  if (!FUSED) asm volatile("griddepcontrol.wait;" ::: "memory");   // the image is ready
   bool begun = piece == 0;   // this warp holds its unit's first block
   bool lost = false;         // a copy did not arrive in time
   int stage = 0, left = count;
@@ -617,24 +636,16 @@ int cluster_size(const void* kernel, int threads, int bytes, int units, int* siz
   return GLT_OK;
 }
 
-template <int LIMBS, int NT, int TILES, bool ASYM, int GROUP>
-int launch_linear(const LinearArgs& a, cudaStream_t st) {
-  using Image = XImage<LIMBS>;
-  const auto kernel = w4_linear_kernel<LIMBS, NT, TILES, ASYM, GROUP>;
-  constexpr int bytes = LinearSmem<NT, TILES, ASYM, GROUP>::kBytes;
-  const Image I(a.L, a.M);
-  const int blocks = I.tiles / NT;
-  if (blocks > 65535 || a.M > 65535) return fail(GLT_EINVAL, "w4: %d rows (at most 65535)", a.M);
+template <int LIMBS, int NT, int TILES, bool ASYM, int GROUP, bool FUSED>
+int launch_linear_one(const LinearArgs& a, const XImage<LIMBS>& I, cudaStream_t st) {
+  const auto kernel = w4_linear_kernel<LIMBS, NT, TILES, ASYM, GROUP, FUSED>;
+  const int bytes = LinearSmem<NT, TILES, ASYM, GROUP>::kBytes + (FUSED ? static_cast<int>(I.bytes) : 0);
   int clusters = 1, S = 1;
   GLT_TRY(ensure_smem_attr(reinterpret_cast<const void*>(kernel), bytes));
   GLT_TRY(cluster_size(reinterpret_cast<const void*>(kernel), 32 * linear_warps(NT), bytes,
                        (a.L.tiles + TILES - 1) / TILES, &S, &clusters));
-  w4_prepare_kernel<LIMBS, GROUP><<<dim3(I.slots, a.M), kPrepThreads, 0, st>>>(
-      a.x, a.ld_x, a.M, a.L, a.ws);
-  GLT_LAUNCH_CHECK();
-  // starts beside the preparation and waits for its end after the first loads of weights
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(clusters) * S, blocks);
+  cfg.gridDim = dim3(static_cast<unsigned>(clusters) * S, I.tiles / NT);
   cfg.blockDim = dim3(32 * linear_warps(NT));
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
@@ -646,10 +657,24 @@ int launch_linear(const LinearArgs& a, cudaStream_t st) {
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 2;
+  cfg.numAttrs = FUSED ? 1 : 2;   // with a preparation: starts beside it and waits for its end after the first copies
   GLT_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
   GLT_LAUNCH_CHECK();
   return GLT_OK;
+}
+
+template <int LIMBS, int NT, int TILES, bool ASYM, int GROUP>
+int launch_linear(const LinearArgs& a, cudaStream_t st) {
+  const XImage<LIMBS> I(a.L, a.M);
+  if (I.tiles / NT > 65535 || a.M > 65535) return fail(GLT_EINVAL, "w4: %d rows (at most 65535)", a.M);
+  // A small x is turned into its image by every CTA for itself: one launch less, but 1.5 us more for each
+  // 16384 elements than reading the image that a launch before made.
+  if constexpr (NT == 1)
+    if (static_cast<int64_t>(a.M) * a.L.K <= 16384 && LinearSmem<NT, TILES, ASYM, GROUP>::kBytes + I.bytes <= 227 * 1024)
+      return launch_linear_one<LIMBS, NT, TILES, ASYM, GROUP, true>(a, I, st);
+  w4_prepare_kernel<LIMBS, GROUP><<<dim3(I.slots, a.M), kPrepThreads, 0, st>>>(a.x, a.ld_x, a.M, a.L, a.ws);
+  GLT_LAUNCH_CHECK();
+  return launch_linear_one<LIMBS, NT, TILES, ASYM, GROUP, false>(a, I, st);
 }
 
 template <int LIMBS, int NT, int TILES>
