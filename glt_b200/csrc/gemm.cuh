@@ -36,8 +36,6 @@ int make_tmap_f32_swz128(CUtensorMap* tm, const void* base, uint64_t inner, uint
 int make_tmap_u8(CUtensorMap* tm, const void* base, uint64_t inner, uint64_t outer, uint32_t box_outer);
 
 int num_sms();
-// Clusters of `size` CTAs of a kernel that can be resident at once (they need SMs of one GPC).
-int max_active_clusters(const void* func, int threads, int smem, int size, int* clusters);
 
 // Dynamic tile claiming (GemmShape::tile_ctr) for the GEMMs this host thread
 // launches: a device int[2], zero at rest, used by one stream at a time.

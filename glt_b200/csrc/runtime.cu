@@ -13,7 +13,6 @@
 #include <map>
 #include <mutex>
 #include <set>
-#include <tuple>
 #include <unordered_map>
 #include <utility>
 
@@ -130,39 +129,6 @@ int max_active_pairs(const void* func, int threads, int smem, int* pairs) {
   }
   done[key] = n;
   *pairs = n;
-  return GLT_OK;
-}
-
-int max_active_clusters(const void* func, int threads, int smem, int size, int* clusters) {
-  int dev = 0;
-  GLT_CUDA_TRY(cudaGetDevice(&dev));
-  static std::map<std::tuple<int, const void*, int, int, int>, int> done;
-  std::lock_guard<std::mutex> lk(g_mu);
-  const auto key = std::make_tuple(dev, func, threads, smem, size);
-  auto it = done.find(key);
-  if (it != done.end()) {
-    *clusters = it->second;
-    return GLT_OK;
-  }
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(size * 1024);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = size;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  int n = 0;
-  cudaError_t e = cudaOccupancyMaxActiveClusters(&n, func, &cfg);
-  if (e != cudaSuccess || n <= 0) {
-    cudaGetLastError();
-    return fail(GLT_ECUDA, "cudaOccupancyMaxActiveClusters(%d): %s (%d)", size, cudaGetErrorString(e), n);
-  }
-  done[key] = n;
-  *clusters = n;
   return GLT_OK;
 }
 

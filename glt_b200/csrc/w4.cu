@@ -9,15 +9,12 @@
 // the codes of row g (low nibble) and row g + 8 (high nibble) at column
 // (s / 2) * 32 + 8 c + (s % 2) * 4 + b.  So one AND (and a shift) makes four codes a register
 // of operand A of mma.m16n8k32 on bytes.
-#include <cooperative_groups.h>
 #include <math.h>
 
 #include <climits>
 
 #include "common.cuh"
 #include "gemm.cuh"
-
-namespace cg = cooperative_groups;
 
 namespace glt {
 namespace {
@@ -318,11 +315,12 @@ __device__ __noinline__ float plain_product(const LinearArgs& a, int64_t n, int 
 // columns), the image of x operand B.
 //
 // Work.  One CTA a SM.  A unit is TILES tiles of 16 rows of W, all fed by a load of the
-// image.  A cluster of S CTAs takes a run of units, and its warps equal runs of their blocks,
-// laid end to end.  Each warp has a ring of stages, filled by TMA with a record (of every
-// tile) a stage, that runs ahead across units.  A unit that one warp holds whole is written from
-// registers; the parts of a unit that warps share go through shared memory (the cluster's) to
-// the warp that begins it, which adds them in order.
+// image.  A CTA takes a run of units, and its warps equal runs of their blocks, laid end to
+// end.  Each warp has a ring of stages, filled by TMA with a record (of every tile) a stage,
+// that runs ahead across units.  A unit that one warp holds whole is written from registers;
+// the parts of a unit that warps share go through shared memory to the warp that begins
+// it, which adds them in order.  (Clusters that split a unit's columns over SMs balance better
+// on paper, 12.25 tiles a CTA for 13 at 28672 rows, and measured 14.2 us for 13.6.)
 //
 // Half a byte a weight leaves about 22 cycles of an SM for a tile's chunk, so instructions
 // count: 12 integer ones make the codes' fragments (8 AND, 4 shifts), two products do the
@@ -349,23 +347,19 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
   constexpr int kWarps = Smem::kWarps, kRecord = Smem::kRecord, kPart = Smem::kPart;
   using Image = XImage<LIMBS>;
   constexpr int kPer = 128 / GROUP, kSteps = GROUP / 32;        // groups of a block, k-steps of a group
-  constexpr int kLeast = 2;                                     // shorter runs cost more to join than to read
+  constexpr int kLeast = 4;                                     // blocks: shorter runs cost more to join than to read
   extern __shared__ __align__(128) uint8_t smem[];
   float* parts = reinterpret_cast<float*>(smem + kWarps * Smem::kRing);   // [warp][the unit it continues, the one it only begins]
   uint64_t* bars = reinterpret_cast<uint64_t*>(parts + kWarps * 2 * kPart);
-  cg::cluster_group cluster = cg::this_cluster();
-  const int S = cluster.num_blocks(), rank = cluster.block_rank();
-  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, local = threadIdx.x >> 5;
-  const int warp = local * S + rank;    // of the cluster
+  const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, warp = threadIdx.x >> 5;
   const W4Layout& L = a.L;
   const Image I(L, a.M);
   const int P = L.blocks;
   const int units = (L.tiles + TILES - 1) / TILES;
-  const int clusters = gridDim.x / S, cl = blockIdx.x / S;
-  const int u0 = static_cast<int>(quotient(static_cast<int64_t>(units) * cl, clusters));
-  const int u1 = static_cast<int>(quotient(static_cast<int64_t>(units) * (cl + 1), clusters));
+  const int u0 = static_cast<int>(quotient(static_cast<int64_t>(units) * blockIdx.x, gridDim.x));
+  const int u1 = static_cast<int>(quotient(static_cast<int64_t>(units) * (blockIdx.x + 1), gridDim.x));
   const int64_t all = static_cast<int64_t>(u1 - u0) * P;
-  const int warps = static_cast<int>(min(static_cast<int64_t>(S * kWarps), (all + kLeast - 1) / kLeast));
+  const int warps = static_cast<int>(min(static_cast<int64_t>(kWarps), (all + kLeast - 1) / kLeast));
   const int64_t each = quotient(all, warps), more = all - each * warps;
   auto begin_of = [&](int w) { return each * w + min(static_cast<int64_t>(w), more); };
   const int64_t begin = warp < warps ? begin_of(warp) : all, end = warp < warps ? begin_of(warp + 1) : all;
@@ -378,8 +372,8 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
   }
 
   // ---- the ring
-  uint8_t* ring = smem + local * Smem::kRing;
-  bars += local * kStages;
+  uint8_t* ring = smem + warp * Smem::kRing;
+  bars += warp * kStages;
   if (lane == 0) {
     for (int i = 0; i < kStages; ++i) tc::mbar_init(bars + i, 1);
     tc::fence_mbar_init();
@@ -513,7 +507,7 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
         }
     }
   };
-  float* mine = parts + local * 2 * kPart + lane;
+  float* mine = parts + warp * 2 * kPart + lane;
   auto clear = [&]() {
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
@@ -595,10 +589,7 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
   // a unit that goes on in the next warp: one that this warp begins, or only passes through
   const bool joins = piece > 0 && begun && count > 0;
   if (piece > 0 && count > 0) leave(begun ? 1 : 0);
-  if (S > 1)
-    cluster.sync();
-  else
-    __syncthreads();
+  __syncthreads();
   if (joins) {
     const int64_t unit_end = static_cast<int64_t>(unit - u0 + 1) * P;
     auto add = [&](const float* from) {
@@ -612,52 +603,27 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
     add(mine + kPart);
 #pragma unroll 4
     for (int w = warp + 1; w < warps && begin_of(w) < unit_end; ++w)
-      add(cluster.map_shared_rank(parts + w / S * 2 * kPart + lane, w % S));
+      add(parts + w * 2 * kPart + lane);
     write(unit);
   }
-  if (S > 1) cluster.sync();   // the others have read this CTA's parts
-}
-
-// CTAs of a cluster: what leaves the fullest cluster the least to do for each of its CTAs
-// (28672 rows: 13 tiles a CTA alone, 12.5 in pairs), of the sizes whose clusters fit at once.
-int cluster_size(const void* kernel, int threads, int bytes, int units, int* size, int* clusters) {
-  double least = 0;
-  for (int S = 1; S <= 8; S *= 2) {
-    int have = num_sms();
-    if (S > 1) GLT_TRY(max_active_clusters(kernel, threads, bytes, S, &have));
-    const int use = units < have ? units : have;
-    const double load = static_cast<double>((units + use - 1) / use) / S;
-    if (S == 1 || load < least * 0.97) {
-      *size = S;
-      least = load;
-      *clusters = use;
-    }
-  }
-  return GLT_OK;
 }
 
 template <int LIMBS, int NT, int TILES, bool ASYM, int GROUP, bool FUSED>
 int launch_linear_one(const LinearArgs& a, const XImage<LIMBS>& I, cudaStream_t st) {
   const auto kernel = w4_linear_kernel<LIMBS, NT, TILES, ASYM, GROUP, FUSED>;
   const int bytes = LinearSmem<NT, TILES, ASYM, GROUP>::kBytes + (FUSED ? static_cast<int>(I.bytes) : 0);
-  int clusters = 1, S = 1;
   GLT_TRY(ensure_smem_attr(reinterpret_cast<const void*>(kernel), bytes));
-  GLT_TRY(cluster_size(reinterpret_cast<const void*>(kernel), 32 * linear_warps(NT), bytes,
-                       (a.L.tiles + TILES - 1) / TILES, &S, &clusters));
+  const int units = (a.L.tiles + TILES - 1) / TILES;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(clusters) * S, I.tiles / NT);
+  cfg.gridDim = dim3(units < num_sms() ? units : num_sms(), I.tiles / NT);
   cfg.blockDim = dim3(32 * linear_warps(NT));
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = S;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = FUSED ? 1 : 2;   // with a preparation: starts beside it and waits for its end after the first copies
+  cfg.numAttrs = FUSED ? 0 : 1;   // with a preparation: starts beside it and waits for its end after the first copies
   GLT_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a));
   GLT_LAUNCH_CHECK();
   return GLT_OK;
