@@ -165,7 +165,8 @@ __device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], ui
 constexpr int kPrepThreads = 256;
 constexpr int kMagic = 0x4B400000;   // 1.5 2^23 as a float: kMagic + i is the float 1.5 2^23 + i
 // What lane c needs at the ends of a group: what its two columns' sums begin with, kMagic - 8 (asym: 15)
-// times the sum of the bytes, and 2^-a of its row.
+// times the sum of the bytes, and 2^-a of its row's block: NaN where the block holds something
+// that is not finite, and such a row's products are then done the plain way.
 struct __align__(16) GroupNote {
   int start[2];
   float factor;
@@ -176,27 +177,23 @@ struct XImage {
   static constexpr int kCols = LIMBS == 2 ? 2 : 4, kRows = 8 / kCols;   // columns a row, rows a tile
   int per_cta;   // tiles of rows of x that a CTA takes
   int tiles, chunks, groups;   // tiles filled up to per_cta's multiple; chunks and groups to the end of the last block
-  int slots;
-  int64_t notes, finite, bytes;   // offsets in the workspace, after the image
+  int64_t notes, bytes;   // offset in the workspace, after the image; of both
   __host__ __device__ XImage(const W4Layout& L, int M) {
     const int need = (M + kRows - 1) / kRows;
-    per_cta = need <= 2 ? need : need <= 5 ? 5 : 8;
+    per_cta = need <= 5 ? need : 8;
     tiles = (need + per_cta - 1) / per_cta * per_cta;
     chunks = L.blocks * 2;
     groups = L.blocks * L.per_block;
     notes = static_cast<int64_t>(chunks) * tiles * 512;
     // notes: [group][tile][lane c]
-    finite = notes + static_cast<int64_t>(groups) * tiles * 4 * sizeof(GroupNote);
-    // finite: per row of x and CTA of the preparation, 0 where all is
-    slots = (chunks * 8 + kPrepThreads - 1) / kPrepThreads;
-    bytes = (finite + static_cast<int64_t>(M) * slots * 4 + 15) / 16 * 16;
+    bytes = notes + static_cast<int64_t>(groups) * tiles * 4 * sizeof(GroupNote);
   }
 };
 
 // Eight columns (vector v) of row m of x into the image at ws; the threads of a block's 16 vectors are
-// neighbours and all here.  Returns whether something is not finite.
+// neighbours and all here.
 template <int LIMBS, int GROUP>
-__device__ __forceinline__ bool prepare_vector(const uint16_t* __restrict__ x, int64_t ld_x, const W4Layout& L,
+__device__ __forceinline__ void prepare_vector(const uint16_t* __restrict__ x, int64_t ld_x, const W4Layout& L,
                                                const XImage<LIMBS>& I, int m, int v, uint8_t* ws) {
   using Image = XImage<LIMBS>;
   const bool in = v < I.chunks * 8;
@@ -205,20 +202,14 @@ __device__ __forceinline__ bool prepare_vector(const uint16_t* __restrict__ x, i
   float f[8];
   unpack8(u, f);
   float peak = 0.f;
-  bool bad = false;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    if (fabsf(f[k]) < INFINITY)
-      peak = fmaxf(peak, fabsf(f[k]));
-    else
-      bad = true;
-  }
+  for (int k = 0; k < 8; ++k) peak = fabsf(f[k]) <= peak ? peak : fabsf(f[k]) < INFINITY ? fabsf(f[k]) : INFINITY;
   constexpr int kLanes = GROUP / 8;   // of a group; 16 of a block
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
   // the largest to [2^14, 2^15) or [2^22, 2^23), one less for the one mantissa whose high byte would be 128
   int a = 0;
-  if (peak > 0.f) {
+  if (peak > 0.f && peak < INFINITY) {
     const int e = ilogbf(peak);
     const bool top = (__float_as_uint(peak) >> 16 & 0x7F) == 0x7F && e > -127;
     a = (LIMBS == 2 ? 14 : 22) - e - (top ? 1 : 0);
@@ -229,7 +220,7 @@ __device__ __forceinline__ bool prepare_vector(const uint16_t* __restrict__ x, i
   int sum[LIMBS] = {};
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    int i = fabsf(f[k]) < INFINITY ? __float2int_rn(f[k] * a0 * a1) : 0;
+    int i = peak < INFINITY ? __float2int_rn(f[k] * a0 * a1) : 0;
 #pragma unroll
     for (int l = LIMBS - 1; l >= 0; --l) {
       const int up = l > 0 ? (i + 128) >> 8 : 0;   // what the next higher byte takes
@@ -243,7 +234,7 @@ __device__ __forceinline__ bool prepare_vector(const uint16_t* __restrict__ x, i
   for (int o = 1; o < kLanes; o <<= 1)
 #pragma unroll
     for (int l = 0; l < LIMBS; ++l) sum[l] += __shfl_xor_sync(0xffffffffu, sum[l], o);
-  if (!in) return bad;
+  if (!in) return;
   const int chunk = v >> 3, step = (v >> 2) & 1, c = v & 3, tile = m / Image::kRows, row = m % Image::kRows;
   uint8_t* dst = ws + ((static_cast<int64_t>(chunk) * I.tiles + tile) * 32 + row * Image::kCols * 4 + c) * 16 + step * 8;
 #pragma unroll
@@ -260,22 +251,18 @@ __device__ __forceinline__ bool prepare_vector(const uint16_t* __restrict__ x, i
         const int b = 2 * j + e < LIMBS ? sum[2 * j + e < LIMBS ? 2 * j + e : 0] : 0;
         n.start[e] = kMagic - (L.asym ? 15 : 8) * b;
       }
-      n.factor = exp2f(static_cast<float>(-a));
+      n.factor = peak < INFINITY ? exp2f(static_cast<float>(-a)) : NAN;
       n.pad = 0;
       note[j] = n;
     }
   }
-  return bad;
 }
 
 template <int LIMBS, int GROUP>
 __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const uint16_t* __restrict__ x, int64_t ld_x, int M,
                                                                   W4Layout L, uint8_t* __restrict__ ws) {
   asm volatile("griddepcontrol.launch_dependents;");
-  const XImage<LIMBS> I(L, M);
-  const int m = blockIdx.y;
-  const bool bad = __syncthreads_or(prepare_vector<LIMBS, GROUP>(x, ld_x, L, I, m, blockIdx.x * kPrepThreads + threadIdx.x, ws));
-  if (threadIdx.x == 0) reinterpret_cast<int*>(ws + I.finite)[m * I.slots + blockIdx.x] = bad;
+  prepare_vector<LIMBS, GROUP>(x, ld_x, L, XImage<LIMBS>(L, M), blockIdx.y, blockIdx.x * kPrepThreads + threadIdx.x, ws);
 }
 
 struct LinearArgs {
@@ -327,30 +314,47 @@ __device__ __noinline__ float plain_product(const LinearArgs& a, int64_t n, int 
 // rest for four rows of x.  Zeros: sum v (u - 8) = sum v u - 8 sum v, the second part, and the
 // number that turns the integer into a float, being what a group's sums begin with; with stored
 // zeros the codes become u + (15 - z), 0..30, by one addition a register, and 15 takes the place of 8.
-__host__ __device__ constexpr int linear_warps(int nt) { return nt <= 2 ? 16 : 8; }
-constexpr int kStages = 4;
+//
+// With up to two tiles of rows of x a warp reads the image and its notes into registers, one
+// chunk and one group ahead; with more they come by the ring (kRingX), since there are neither
+// the registers nor the warps to hide their latency (32 rows by 4096 x 4096: 19.2 us in registers, 13.4
+// by the ring).  As many warps as have the registers and two stages: with five tiles 11 warps take
+// 28.8 us for 19 rows by 4096 x 14336 in groups of 32 with zeros, 10 take 30.9.
+//
+// Measured, back to back, with the preparation: one row by 28672 x 4096 13.3 us (4.5 TB/s of packed
+// weights), by 4096 x 4096 5.8, 16 rows by 4096 x 4096 9.1, 32 rows 13.4.  One row is bound by the
+// copies and the launch; many rows by the integers' way to floats, four instructions for two rows of W by a row
+// of x and group, beside the 8 cycles of a matrix instruction.
+__host__ __device__ constexpr int linear_warps(int nt) { return nt <= 2 ? 16 : nt <= 4 ? 12 : nt <= 5 ? 11 : 7; }
 
 template <int NT, int TILES, bool ASYM, int GROUP>   // the same for both numbers of bytes
 struct LinearSmem {
   static constexpr int kWarps = linear_warps(NT);
+  static constexpr bool kRingX = NT > 2;
   static constexpr int kRecord = 1024 + 128 / GROUP * 32 * (ASYM ? 2 : 1);
   static constexpr int kBlocks = TILES == 1 ? 2 : 1;           // of a stage: with one tile they lie side by side
-  static constexpr int kStage = kBlocks * TILES * kRecord;
-  static constexpr int kRing = kStages * kStage;               // a warp's
+  static constexpr int kImage = kBlocks * TILES * kRecord;     // where a stage's part of the image begins,
+  static constexpr int kNotes = kImage + (kRingX ? NT * 1024 : 0);   // and its notes
+  static constexpr int kStage = kNotes + (kRingX ? 128 / GROUP * NT * 64 : 0);
   static constexpr int kPart = TILES * NT * 2 * 32;            // floats of a part of a unit
-  static constexpr int kBytes = kWarps * (kRing + 2 * kPart * 4 + kStages * 8);
+  static constexpr int kFit = (227 * 1024 / kWarps - kPart * 4 - 32) / kStage;
+  static constexpr int kStages = kFit < 4 ? kFit : 4;
+  static_assert(kStages >= 2, "a warp needs two stages");
+  static constexpr int kRing = kStages * kStage;               // a warp's
+  static constexpr int kBytes = (kWarps * (kRing + kPart * 4 + kStages * 8) + 127) / 128 * 128;
 };
 
 template <int LIMBS, int NT, int TILES, bool ASYM, int GROUP, bool FUSED>
 __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(const __grid_constant__ LinearArgs a) {
   using Smem = LinearSmem<NT, TILES, ASYM, GROUP>;
-  constexpr int kWarps = Smem::kWarps, kRecord = Smem::kRecord, kPart = Smem::kPart;
+  constexpr int kWarps = Smem::kWarps, kRecord = Smem::kRecord, kPart = Smem::kPart, kStages = Smem::kStages;
+  constexpr bool kRingX = Smem::kRingX;
   using Image = XImage<LIMBS>;
   constexpr int kPer = 128 / GROUP, kSteps = GROUP / 32;        // groups of a block, k-steps of a group
   constexpr int kLeast = 4;                                     // blocks: shorter runs cost more to join than to read
   extern __shared__ __align__(128) uint8_t smem[];
-  float* parts = reinterpret_cast<float*>(smem + kWarps * Smem::kRing);   // [warp][the unit it continues, the one it only begins]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(parts + kWarps * 2 * kPart);
+  float* parts = reinterpret_cast<float*>(smem + kWarps * Smem::kRing);   // [warp], of the unit that it goes on with
+  uint64_t* bars = reinterpret_cast<uint64_t*>(parts + kWarps * kPart);
   const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3, warp = threadIdx.x >> 5;
   const W4Layout& L = a.L;
   const Image I(L, a.M);
@@ -385,8 +389,19 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
     if (to_issue <= 0) return;
     const int n = min(to_issue, Smem::kBlocks);
     if (lane == 0) {
-      tc::mbar_arrive_expect_tx(bars + stage, n * TILES * kRecord);
+      tc::mbar_arrive_expect_tx(bars + stage, n * TILES * kRecord + Smem::kStage - Smem::kImage);
       uint8_t* dst = ring + stage * Smem::kStage;
+      if (kRingX) {
+        // of one block: its two chunks of the image, its groups' notes, NT tiles of each
+        const int first = blockIdx.y * NT, at_once = I.tiles == NT ? 1 : 0;
+        for (int h = 0; h < 2; h += 1 + at_once)
+          copy_bulk(dst + Smem::kImage + h * NT * 512, a.ws + (static_cast<int64_t>(ld_piece * 2 + h) * I.tiles + first) * 512,
+                    NT * 512 << at_once, bars + stage);
+        for (int h = 0; h < kPer; h += at_once ? kPer : 1)
+          copy_bulk(dst + Smem::kNotes + h * NT * 64,
+                    a.ws + I.notes + (static_cast<int64_t>(ld_piece * kPer + h) * I.tiles + first) * 64,
+                    at_once ? kPer * NT * 64 : NT * 64, bars + stage);
+      }
       copy_bulk(dst, src, n * kRecord, bars + stage);
       if (TILES == 2)   // a tile past the last one repeats it: nothing of it is written
         copy_bulk(dst + kRecord, ld_unit * 2 + 1 < L.tiles ? src + static_cast<int64_t>(P) * kRecord : src, kRecord, bars + stage);
@@ -399,6 +414,7 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
       src += static_cast<int64_t>(P) * kRecord;
     }
   };
+  if (kRingX) asm volatile("griddepcontrol.wait;" ::: "memory");   // the image is ready
 #pragma unroll 1
   for (int i = 0; i < kStages; ++i) issue(i);
 
@@ -406,12 +422,9 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
   const uint8_t* img = a.ws;
   if (FUSED) {
     uint8_t* own = smem + Smem::kBytes;
-    int* flags = reinterpret_cast<int*>(own + I.finite);
-    for (int i = threadIdx.x; i < a.M * I.slots; i += 32 * kWarps) flags[i] = 0;
-    __syncthreads();
     for (int m = 0; m < a.M; ++m)
       for (int v = 0; v < I.chunks * 8; v += 32 * kWarps)
-        if (prepare_vector<LIMBS, GROUP>(a.x, a.ld_x, L, I, m, v + threadIdx.x, own)) atomicOr(flags + m * I.slots, 1);
+        prepare_vector<LIMBS, GROUP>(a.x, a.ld_x, L, I, m, v + threadIdx.x, own);
     __syncthreads();
     img = own;
   }
@@ -431,13 +444,13 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
   };
   // a lane's two columns: the bytes of a row, or (three bytes) half of them
   const float high = LIMBS == 2 ? 256.f : c & 1 ? 1.f : 65536.f, low = LIMBS == 2 ? 1.f : c & 1 ? 0.f : 256.f;
+  const float back = -12582912.f * (high + low);
 
   float acc[TILES][NT][2] = {};   // rows g, g + 8 of W by a row of a tile of x
   int part[TILES][NT][4];
   float sum[TILES][NT][2];        // of a block's groups
-  // k-step s of the record(s) at `rec`, with the image's chunk x and the group's note.
-  auto step = [&](const uint8_t* rec, int s, const uint4 (&x)[NT], const uint4 (&note)[NT]) {
-    const int grp = s / kSteps;
+  // k-step s, of group grp, of the record(s) at `rec`, with the image's chunk x and the group's note.
+  auto step = [&](const uint8_t* rec, int grp, int s, const uint4 (&x)[NT], const uint4 (&note)[NT]) {
     const bool first = s % kSteps == 0, last = s % kSteps == kSteps - 1;
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
@@ -452,54 +465,83 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         if (first) {
-          part[t][n][0] = part[t][n][2] = static_cast<int>(note[n].x);
-          part[t][n][1] = part[t][n][3] = static_cast<int>(note[n].y);
+          int2 start = make_int2(static_cast<int>(note[n].x), static_cast<int>(note[n].y));
+          if (kRingX) start = *reinterpret_cast<const int2*>(rec + Smem::kNotes + (grp * NT + n) * 64 + c * 16);
+          part[t][n][0] = part[t][n][2] = start.x;
+          part[t][n][1] = part[t][n][3] = start.y;
         }
-        mma_u8s8(part[t][n], f, s & 1 ? x[n].z : x[n].x, s & 1 ? x[n].w : x[n].y);
+        uint2 b = s & 1 ? make_uint2(x[n].z, x[n].w) : make_uint2(x[n].x, x[n].y);
+        if (kRingX)
+          b = *reinterpret_cast<const uint2*>(rec + Smem::kImage + ((s >> 1) * NT + n) * 512 + lane * 16 + (s & 1) * 8);
+        mma_u8s8(part[t][n], f, b.x, b.y);
       }
       if (last) {
         const uint32_t two = *reinterpret_cast<const uint32_t*>(sc);
-        const float s0 = bf16_lo(two), s1 = bf16_hi(two);
+        const float w[2] = {bf16_lo(two), bf16_hi(two)};
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
           for (int q = 0; q < 2; ++q) {
-            const float h = __int_as_float(part[t][n][2 * q]) - 12582912.f, l = __int_as_float(part[t][n][2 * q + 1]) - 12582912.f;
-            const float v = LIMBS == 2 ? fmaf(h, 256.f, l) : fmaf(h, high, l * low);
-            // the row's 2^-a belongs to the block: its groups' sums meet it together
-            if (kPer == 1) {
-              acc[t][n][q] = fmaf(v * (q ? s1 : s0), __uint_as_float(note[n].z), acc[t][n][q]);
-            } else {
-              sum[t][n][q] = grp == 0 ? v * (q ? s1 : s0) : fmaf(v, q ? s1 : s0, sum[t][n][q]);
-              if (grp == kPer - 1) acc[t][n][q] = fmaf(sum[t][n][q], __uint_as_float(note[n].z), acc[t][n][q]);
-            }
+            // high h + low l of the floats 1.5 2^23 + h and + l: the first product and its constant are
+            // multiples of `high`, and exact
+            const float v = fmaf(__int_as_float(part[t][n][2 * q + 1]), low, fmaf(__int_as_float(part[t][n][2 * q]), high, back));
+            sum[t][n][q] = fmaf(v, w[q], sum[t][n][q]);
           }
       }
     }
   };
-  auto write = [&](int u) {
+  auto begin_block = [&]() {
+#pragma unroll
+    for (int t = 0; t < TILES; ++t)
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sum[t][n][0] = sum[t][n][1] = 0.f;
+  };
+  // the row's 2^-a belongs to the block: its groups' sums meet it together
+  auto end_block = [&](const uint8_t* rec, const uint4 (&note)[NT]) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int m = (static_cast<int>(blockIdx.y) * NT + n) * Image::kRows + c * Image::kRows / 4;
-      float o[TILES][2];
+      float factor = __uint_as_float(note[n].z);
+      if (kRingX) factor = *reinterpret_cast<const float*>(rec + Smem::kNotes + n * 64 + c * 16 + 8);
 #pragma unroll
       for (int t = 0; t < TILES; ++t)
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          o[t][q] = acc[t][n][q];
-          if (LIMBS == 3) o[t][q] += __shfl_xor_sync(0xffffffffu, o[t][q], 1);   // the other bytes' lane
+          acc[t][n][q] = fmaf(sum[t][n][q], factor, acc[t][n][q]);
         }
-      if (m >= a.M || (LIMBS == 3 && (c & 1))) continue;
-      bool plain = false;
-      for (int i = 0; i < I.slots; ++i) plain |= reinterpret_cast<const int*>(img + I.finite)[m * I.slots + i] != 0;
+    }
+  };
+  auto write = [&](int u) {
+    const int m0 = static_cast<int>(blockIdx.y) * NT * Image::kRows + c * Image::kRows / 4;
+    const int64_t row0 = static_cast<int64_t>(u) * TILES * 16 + g;
+    float resid[NT][TILES][2];   // all on their way before the first store, which may be to the same place
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int t = 0; t < TILES; ++t)
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
-          const int64_t row = (static_cast<int64_t>(u) * TILES + t) * 16 + g + 8 * q;
+          const int m = m0 + n * Image::kRows;
+          const int64_t row = row0 + t * 16 + 8 * q;
+          resid[n][t][q] = a.resid && m < a.M && row < L.N ? bf16_bits_to_f32(a.resid[m * a.ld_r + row]) : 0.f;
+        }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int m = m0 + n * Image::kRows;
+      if (LIMBS == 3) {
+#pragma unroll
+        for (int t = 0; t < TILES; ++t)
+#pragma unroll
+          for (int q = 0; q < 2; ++q) acc[t][n][q] += __shfl_xor_sync(0xffffffffu, acc[t][n][q], 1);   // the other bytes' lane
+      }
+      if (m >= a.M || (LIMBS == 3 && (c & 1))) continue;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const int64_t row = row0 + t * 16 + 8 * q;
           if (row >= L.N) continue;
-          float y = plain ? plain_product(a, row, m) : o[t][q];
-          if (a.resid) y += bf16_bits_to_f32(a.resid[m * a.ld_r + row]);
+          const float v = acc[t][n][q];
+          const float y = (fabsf(v) < INFINITY ? v : plain_product(a, row, m)) + resid[n][t][q];
           if (a.y_bf16)
             static_cast<uint16_t*>(a.y)[m * a.ld_y + row] = bf16_bits_rn(y);
           else
@@ -507,30 +549,30 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
         }
     }
   };
-  float* mine = parts + warp * 2 * kPart + lane;
+  float* mine = parts + warp * kPart + lane;
   auto clear = [&]() {
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
 #pragma unroll
       for (int n = 0; n < NT; ++n) acc[t][n][0] = acc[t][n][1] = 0.f;
   };
-  auto leave = [&](int slot) {
+  auto leave = [&]() {
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) mine[slot * kPart + ((t * NT + n) * 2 + q) * 32] = acc[t][n][q];
+        for (int q = 0; q < 2; ++q) mine[((t * NT + n) * 2 + q) * 32] = acc[t][n][q];
     clear();
   };
 
-  if (!FUSED) asm volatile("griddepcontrol.wait;" ::: "memory");   // the image is ready
+  if (!FUSED && !kRingX) asm volatile("griddepcontrol.wait;" ::: "memory");   // the image is ready
   bool begun = piece == 0;   // this warp holds its unit's first block
   bool lost = false;         // a copy did not arrive in time
   int stage = 0, left = count;
   uint32_t phase = 0;
   uint4 x0[NT], x1[NT], note[2][NT];
-  if (count > 0) {
+  if (!kRingX && count > 0) {
     load_image(x0, piece * 2);
     load_note(note[0], piece * kPer);
   }
@@ -545,18 +587,28 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
       if (b > 0 && left <= 0) break;
       const uint8_t* rec = ring + stage * Smem::kStage + b * kRecord;
       const int after = piece + 1 == P ? 0 : piece + 1;
-      load_image(x1, piece * 2 + 1);
+      if (!kRingX) load_image(x1, piece * 2 + 1);
+      begin_block();
+      if constexpr (kRingX) {
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        // note[..] of group i of the block: with one group a block they change places from block to block
-        const int i = s / kSteps, at = kPer == 1 ? b & 1 : i & 1;
-        if (s % kSteps == 0) load_note(note[at ^ 1], i + 1 < kPer ? piece * kPer + i + 1 : after * kPer);
-        step(rec, s, s < 2 ? x0 : x1, note[at]);
-        if (s == 1) load_image(x0, after * 2);
-      }
-      if (kPer == 1 && Smem::kBlocks == 1) {
+        for (int i = 0; i < kPer; ++i)
 #pragma unroll
-        for (int n = 0; n < NT; ++n) note[0][n] = note[1][n];
+          for (int s = 0; s < kSteps; ++s) step(rec, i, i * kSteps + s, x0, note[0]);
+        end_block(rec, note[0]);
+      } else {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          // note[..] of group i of the block: with one group a block they change places from block to block
+          const int i = s / kSteps, at = kPer == 1 ? b & 1 : i & 1;
+          if (s % kSteps == 0) load_note(note[at ^ 1], i + 1 < kPer ? piece * kPer + i + 1 : after * kPer);
+          step(rec, i, s, s < 2 ? x0 : x1, note[at]);
+          if (s == 1) load_image(x0, after * 2);
+          if (s == 3) end_block(rec, note[at]);
+        }
+        if (kPer == 1 && Smem::kBlocks == 1) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) note[0][n] = note[1][n];
+        }
       }
       --left;
       piece = after;
@@ -565,7 +617,7 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
           write(unit);
           clear();
         } else {
-          leave(0);
+          leave();
         }
         ++unit;
         begun = true;
@@ -586,9 +638,9 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
       phase ^= 1;
     }
   }
-  // a unit that goes on in the next warp: one that this warp begins, or only passes through
-  const bool joins = piece > 0 && begun && count > 0;
-  if (piece > 0 && count > 0) leave(begun ? 1 : 0);
+  // A unit goes on in the next warp: this one keeps what it began, and leaves what it only goes on with.
+  const bool goes_on = piece > 0 && count > 0, joins = goes_on && begun;
+  if (goes_on && !begun) leave();
   __syncthreads();
   if (joins) {
     const int64_t unit_end = static_cast<int64_t>(unit - u0 + 1) * P;
@@ -600,10 +652,9 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
 #pragma unroll
           for (int q = 0; q < 2; ++q) acc[t][n][q] += from[((t * NT + n) * 2 + q) * 32];
     };
-    add(mine + kPart);
 #pragma unroll 4
     for (int w = warp + 1; w < warps && begin_of(w) < unit_end; ++w)
-      add(parts + w * 2 * kPart + lane);
+      add(parts + w * kPart + lane);
     write(unit);
   }
 }
@@ -638,7 +689,7 @@ int launch_linear(const LinearArgs& a, cudaStream_t st) {
   if constexpr (NT == 1)
     if (static_cast<int64_t>(a.M) * a.L.K <= 16384 && LinearSmem<NT, TILES, ASYM, GROUP>::kBytes + I.bytes <= 227 * 1024)
       return launch_linear_one<LIMBS, NT, TILES, ASYM, GROUP, true>(a, I, st);
-  w4_prepare_kernel<LIMBS, GROUP><<<dim3(I.slots, a.M), kPrepThreads, 0, st>>>(a.x, a.ld_x, a.M, a.L, a.ws);
+  w4_prepare_kernel<LIMBS, GROUP><<<dim3((I.chunks * 8 + kPrepThreads - 1) / kPrepThreads, a.M), kPrepThreads, 0, st>>>(a.x, a.ld_x, a.M, a.L, a.ws);
   GLT_LAUNCH_CHECK();
   return launch_linear_one<LIMBS, NT, TILES, ASYM, GROUP, false>(a, I, st);
 }
@@ -658,6 +709,8 @@ int launch_rows(const LinearArgs& a, cudaStream_t st) {
   const int n = XImage<LIMBS>(a.L, a.M).per_cta;
   if (n == 1) return launch_linear_as<LIMBS, 1, 1>(a, st);
   if (n == 2) return launch_linear_as<LIMBS, 2, 1>(a, st);
+  if (n == 3) return launch_linear_as<LIMBS, 3, 2>(a, st);
+  if (n == 4) return launch_linear_as<LIMBS, 4, 2>(a, st);
   if (n == 5) return launch_linear_as<LIMBS, 5, 2>(a, st);
   return launch_linear_as<LIMBS, 8, 2>(a, st);
 }
