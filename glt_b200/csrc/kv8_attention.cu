@@ -308,7 +308,7 @@ struct StageNote {
 };
 template <int HD, int NT>
 constexpr int smem_bytes() {
-  return 1024 /* alignment */ + kWarps * Ring<HD>::kWarp + 2 * 8 * NT * HD * 4 + kWarps * 8 * NT * 8 +
+  return 1024 /* alignment */ + kWarps * Ring<HD>::kWarp + 2 * 8 * NT * (HD + 4) * 4 + kWarps * 8 * NT * 8 +
          kWarps * Ring<HD>::kStages * static_cast<int>(sizeof(StageNote) + 8) + static_cast<int>(sizeof(ScanSmem));
 }
 
@@ -316,15 +316,15 @@ template <int HD, int FMT, int NT, bool BT16>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(const __grid_constant__ AttnArgs a,
                                                                                    const __grid_constant__ CUtensorMap map_k,
                                                                                    const __grid_constant__ CUtensorMap map_v) {
-  constexpr int ROWS = 8 * NT, LU = BT16 ? 2 : 1;
+  constexpr int ROWS = 8 * NT, LU = BT16 ? 2 : 1, kJoinRow = HD + 4;
   // the sums of a step's second half join those of the first, unless each half has its own scale
   // or (NT = 2) holding them would not leave registers enough
   constexpr bool kFoldEach = LU == 2 || NT == 2;
   using R = Ring<HD>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-tc::smem_u32(smem_raw) & 1023u);   // the swizzle goes by address
-  float* join_o = reinterpret_cast<float*>(smem + kWarps * R::kWarp);            // [2][ROWS][HD]
-  float2* join_ml = reinterpret_cast<float2*>(join_o + 2 * ROWS * HD);           // [warp][ROWS]
+  float* join_o = reinterpret_cast<float*>(smem + kWarps * R::kWarp);            // [2][ROWS][kJoinRow]
+  float2* join_ml = reinterpret_cast<float2*>(join_o + 2 * ROWS * kJoinRow);     // [warp][ROWS]
   StageNote* notes = reinterpret_cast<StageNote*>(join_ml + kWarps * ROWS);
   uint64_t* bars = reinterpret_cast<uint64_t*>(notes + kWarps * R::kStages);
   ScanSmem& scan = *reinterpret_cast<ScanSmem*>(bars + kWarps * R::kStages);
@@ -789,8 +789,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
           acc[k][nt][2 + j] *= f;
         }
       }
-    // O^T tile k, row g (+8) is channel g hd / 8 + 2k (+1); column 2c + j is a query row
-    auto place = [&](int k, int nt, int j) { return (nt * 8 + 2 * c + j) * HD + g * (HD / 8) + 2 * k; };
+    // O^T tile k, row g (+8) is channel g hd / 8 + 2k (+1); column 2c + j is a query row.  Two channels
+    // lie where neither this nor the reading below meets a bank twice: rows are 4 floats longer
+    // (eight banks from one c to the next), and tiles 2i and 2i + 1 share 32, turned by 8i.
+    auto turned = [](int k, int g) { return (k >> 1) * 32 + (((k & 1) * 16 + 2 * g + 8 * (k >> 1)) & 31); };
+    auto place = [&](int k, int nt, int j) { return (nt * 8 + 2 * c + j) * kJoinRow + turned(k, g); };
     if (warp >= 2) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -798,7 +801,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
         for (int k = 0; k < HD / 16; ++k)
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            *reinterpret_cast<float2*>(join_o + (warp - 2) * ROWS * HD + place(k, nt, j)) =
+            *reinterpret_cast<float2*>(join_o + (warp - 2) * ROWS * kJoinRow + place(k, nt, j)) =
                 make_float2(acc[k][nt][j], acc[k][nt][2 + j]);
     }
     __syncthreads();
@@ -809,7 +812,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
         for (int k = 0; k < HD / 16; ++k)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            float2* d = reinterpret_cast<float2*>(join_o + warp * ROWS * HD + place(k, nt, j));
+            float2* d = reinterpret_cast<float2*>(join_o + warp * ROWS * kJoinRow + place(k, nt, j));
             const float2 x = *d;
             *d = make_float2(x.x + acc[k][nt][j], x.y + acc[k][nt][2 + j]);
           }
@@ -823,9 +826,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, join_ml[w * ROWS + r].x);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) sum += join_ml[w * ROWS + r].y * join_factor(join_ml[w * ROWS + r].x, top);
-      const float4 x = *reinterpret_cast<const float4*>(join_o + r * HD + d);
-      const float4 y = *reinterpret_cast<const float4*>(join_o + (ROWS + r) * HD + d);
-      const float4 z = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
+      float4 z;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float* from = join_o + r * kJoinRow + turned((d % (HD / 8)) / 2 + h, d / (HD / 8));
+        const float2 x = *reinterpret_cast<const float2*>(from), y = *reinterpret_cast<const float2*>(from + ROWS * kJoinRow);
+        (h ? z.z : z.x) = x.x + y.x;
+        (h ? z.w : z.y) = x.y + y.y;
+      }
       if (whole) {
         write_out(a, row0, tile * ROWS + r, kvh, HD, d, z, top, sum);
       } else {
