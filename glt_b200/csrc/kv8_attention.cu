@@ -509,23 +509,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
         for (int k = 0; k < 4; ++k) acc[j][nt][k] = 0.f;
     }
     const uint8_t* mrow = a.mask ? a.mask + cu.seq * a.ld_mask : nullptr;
-    // the four tokens of a lane in a step: 16 u + 8 r + g
-    auto mask_bits = [&](int step) {
-      uint32_t bits = 0;
-      if (step < cu.s1) {
-        const int t = cu.w.lo + step * kStep + g;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (t + 8 * i <= pos_hi && mrow[t + 8 * i]) bits |= 1u << i;
-      }
-      return bits;
+    // A lane's token of a step, read a step early and looked at only then.
+    auto mask_byte = [&](int step) {
+      const int t = cu.w.lo + step * kStep + lane;
+      return step < cu.s1 && t <= pos_hi ? mrow[t] : static_cast<uint8_t>(0);
     };
-    uint32_t seen = mrow ? mask_bits(cu.s0 + warp) : 0;
+    uint8_t ahead = mrow ? mask_byte(cu.s0 + warp) : 0;
 
     for (int step = cu.s0 + warp; step < cu.s1; step += kWarps) {
-      const uint32_t seen_now = seen;
-      if (mrow) seen = mask_bits(step + kWarps);
       if (lost) continue;
+      uint32_t seen = 0xFFFFFFFFu;   // bit: a token of the step
+      if (mrow) {
+        seen = __ballot_sync(0xffffffffu, ahead != 0);
+        ahead = mask_byte(step + kWarps);
+      }
       wait_groups<R::kStages - 1>();
       __syncwarp();   // the note comes from other lanes
       if (!__all_sync(0xffffffffu, tc::mbar_wait(bars + stage, phase, a.err))) {
@@ -568,7 +565,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int t = t0 + 8 * i + g;
-          const bool on = (valid >> (i >> 1) & 1) && (!mrow || (seen_now >> i & 1)) && t <= pos_hi;
+          const bool on = (valid >> (i >> 1) & 1) && (seen >> (8 * i + g) & 1) && t <= pos_hi;
           if (FMT == GLT_KV8_E4M3) live[i] = __ballot_sync(0xffffffffu, on);   // bit 4g: token 8 i + g
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
