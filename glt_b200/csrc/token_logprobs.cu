@@ -29,6 +29,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
+constexpr int kCtasPerSm = 4;
 constexpr int kMaxTop = 32;
 constexpr int kBatch = 4;            // 16-byte vectors a thread has in flight
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -195,10 +196,10 @@ struct RowSmem {
 };
 
 template <typename T, int CLUSTER>
-__global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) token_logprobs_kernel(
     const T* __restrict__ logits, int64_t ld, int V, const int32_t* __restrict__ targets, float scale,
     int top, float* __restrict__ logp, float* __restrict__ entropy, float* __restrict__ lse_out,
-    int32_t* __restrict__ top_ids, float* __restrict__ top_logp, unsigned int* err) {
+    int32_t* __restrict__ top_ids, float* __restrict__ top_logp, int ahead, unsigned int* err) {
   using Row = RowView<T>;
   constexpr int kVec = Row::kVec;
   __shared__ RowSmem sm;
@@ -297,6 +298,13 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(
       s2 = pair(s0, s1);
       t2 = pair(t0, t1);
     }
+  }
+  // While this row's sums are joined, the two first batches of the row that one of the SM's CTAs takes
+  // next come to L2 (4096 x 128256 bf16: 188 us without, 186 with; 2047 with the gradient: 286 and 280).
+  if (CLUSTER == 1 && threadIdx.x == 0 && r + ahead < gridDim.x) {
+    const Row next(logits + (r + ahead) * ld, V);
+    const int bytes = min(next.nv, 2 * kBatch * kThreads) * 16;
+    if (bytes > 0) asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(next.vec(0)), "r"(bytes));
   }
   {
     float s0, s1, t0, t1;
@@ -548,7 +556,7 @@ int launch_forward(const Args& f, cudaStream_t st) {
   cfg.numAttrs = 1;
   GLT_CUDA_TRY(cudaLaunchKernelEx(&cfg, token_logprobs_kernel<T, CLUSTER>, static_cast<const T*>(f.logits), f.ld, f.V,
                                   f.targets, f.scale, f.top, f.logp, f.entropy, f.lse, f.top_ids, f.top_logp,
-                                  device_error_word()));
+                                  kCtasPerSm * num_sms(), device_error_word()));
   GLT_LAUNCH_CHECK();
   return GLT_OK;
 }
