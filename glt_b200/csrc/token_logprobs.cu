@@ -477,11 +477,13 @@ __global__ void __launch_bounds__(kThreads) token_logprobs_bwd_kernel(
   const float de = d_entropy ? d_entropy[r] : 0.f;
   const float l = lse[r], h = d_entropy ? entropy[r] : 0.f;
   const float base = fmaf(de, h, dl);   // dl + de * (log p + H) = base + de * log p
-  // log p = z - lse; 0 where p is (log p may be -inf there)
+  // log p = z - lse.  Below -200 (it may be -inf) p is 0 in 32 bits, and the floor keeps the product with
+  // it 0; NaN stays NaN.
+  const float w = -scale * de, w0 = -scale * base, from = l == -INFINITY ? 0.f : -l;
   auto grad = [&](float x) {
-    const float lp = fmaf(x, scale, -l);
-    const float p = exp2f(lp * kLog2e);
-    return p == 0.f || l == -INFINITY ? 0.f : -scale * p * fmaf(de, lp, base);
+    float lp = fmaf(x, scale, from);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(lp) : "f"(-200.f));
+    return ex2_approx(lp * kLog2e) * fmaf(w, lp, w0);
   };
   const RowView<T> row(logits + r * ld, V);
   T* out = dlogits + r * ld_d;
