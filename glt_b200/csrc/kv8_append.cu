@@ -100,23 +100,27 @@ __global__ void __launch_bounds__(kThreads, VECS <= 4 ? 5 : 3) kv8_append_kernel
   const int base = index * c.block_tokens;
   const int lo = max(sp.past, base) - base, hi = min(sp.past + sp.n, base + c.block_tokens) - base;
   if (lo >= hi) return;
-  const int64_t id = kv8_block(c, b, seq, index, blockIdx.z == 0 && threadIdx.x == 0 ? err : nullptr);
-  if (id < 0) return;
   const int vec_log = c.head_dim == 128 ? 4 : 3;   // vectors of eight values in a row
-  const int64_t slab = (id * c.num_kv_heads + head) * c.block_tokens * c.head_dim;
-  uint2* codes = reinterpret_cast<uint2*>((is_v ? c.v : c.k) + slab);
-  float* scale = (is_v ? c.v_scale : c.k_scale) + id * c.num_kv_heads + head;
   const int64_t ld = is_v ? ld_v : ld_k;
   const uint16_t* src = (is_v ? v : k) + (sp.row0 + static_cast<int64_t>(base + lo - sp.past)) * ld + head * c.head_dim;
   const int n = (hi - lo) << vec_log, held = lo << vec_log;
-  // the block's own tokens of earlier steps keep its scale from falling
-  const float before = lo > 0 ? *scale : 0.f;
-  uint4 x[VECS];
-  uint2 old[VECS];
+  uint4 x[VECS];   // on its way beside the block's id
 #pragma unroll
   for (int j = 0; j < VECS; ++j) {
     const int i = threadIdx.x + j * kThreads;
     if (i < n) x[j] = *reinterpret_cast<const uint4*>(src + (i >> vec_log) * ld + (i & ((1 << vec_log) - 1)) * 8);
+  }
+  const int64_t id = kv8_block(c, b, seq, index, blockIdx.z == 0 && threadIdx.x == 0 ? err : nullptr);
+  if (id < 0) return;
+  const int64_t slab = (id * c.num_kv_heads + head) * c.block_tokens * c.head_dim;
+  uint2* codes = reinterpret_cast<uint2*>((is_v ? c.v : c.k) + slab);
+  float* scale = (is_v ? c.v_scale : c.k_scale) + id * c.num_kv_heads + head;
+  // the block's own tokens of earlier steps keep its scale from falling
+  const float before = lo > 0 ? *scale : 0.f;
+  uint2 old[VECS];
+#pragma unroll
+  for (int j = 0; j < VECS; ++j) {
+    const int i = threadIdx.x + j * kThreads;
     if (i < held) old[j] = codes[i];
   }
   float peak = 0.f;
