@@ -60,6 +60,23 @@ __device__ __forceinline__ float kv8_decode(uint32_t code, int format) {
   asm("{.reg .b16 lo, hi; mov.b32 {lo, hi}, %1; cvt.f32.f16 %0, lo;}" : "=f"(f) : "r"(h));
   return f;
 }
+// The four codes of a word.
+template <int FMT>
+__device__ __forceinline__ void kv8_decode4(uint32_t w, float (&f)[4]) {
+  if constexpr (FMT == GLT_KV8_INT8) {
+    // a code in the low mantissa bits of 2^23
+#pragma unroll
+    for (int q = 0; q < 4; ++q) f[q] = __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440 + q)) - 8388736.f;
+  } else {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t two = e4m3x2_to_f16x2(h ? w >> 16 : w & 0xFFFFu);
+      asm("{.reg .b16 lo, hi; mov.b32 {lo, hi}, %2; cvt.f32.f16 %0, lo; cvt.f32.f16 %1, hi;}"
+          : "=f"(f[2 * h]), "=f"(f[2 * h + 1])
+          : "r"(two));
+    }
+  }
+}
 // Largest code magnitude of a format.
 __device__ __forceinline__ float kv8_top(int format) { return format == GLT_KV8_INT8 ? 127.f : 448.f; }
 // Nearest code of a value already divided by its scale (ties to even), saturating.

@@ -88,7 +88,7 @@ __device__ __forceinline__ uint2 codes_fast(const float (&x)[8], float s, float 
 // table -> scale bounds single tokens, so all that can be is loaded before the maximum.
 // VECS: vectors of eight values a thread holds of a whole block.
 template <int FMT, int VECS>
-__global__ void __launch_bounds__(kThreads, VECS <= 4 ? 5 : 3) kv8_append_kernel(GltKv8Cache c, GltKv8Batch b,
+__global__ void __launch_bounds__(kThreads, VECS <= 4 ? 4 : 3) kv8_append_kernel(GltKv8Cache c, GltKv8Batch b,
                                                               const uint16_t* __restrict__ k, int64_t ld_k,
                                                               const uint16_t* __restrict__ v, int64_t ld_v,
                                                               unsigned int* err) {
@@ -123,20 +123,27 @@ __global__ void __launch_bounds__(kThreads, VECS <= 4 ? 5 : 3) kv8_append_kernel
     const int i = threadIdx.x + j * kThreads;
     if (i < held) old[j] = codes[i];
   }
-  float peak = 0.f;
-  bool odd = false;   // something not finite among this thread's values
+  // magnitudes of bf16 order like their bits, two at a time
+  uint32_t two = 0;
 #pragma unroll
   for (int j = 0; j < VECS; ++j) {
     if (threadIdx.x + j * kThreads >= n) break;
-    float f[8];
-    unpack8(x[j], f);
+    const uint32_t w[4] = {x[j].x, x[j].y, x[j].z, x[j].w};
 #pragma unroll
-    for (int q = 0; q < 8; ++q) {
-      const float a = fabsf(f[q]);
-      if (a <= FLT_MAX)
-        peak = fmaxf(peak, a);
-      else
-        odd = true;
+    for (int q = 0; q < 4; ++q) asm("max.u16x2 %0, %0, %1;" : "+r"(two) : "r"(w[q] & 0x7FFF7FFFu));
+  }
+  float peak = __uint_as_float(max(two >> 16, two & 0xFFFFu) << 16);
+  const bool odd = !(peak <= FLT_MAX);   // something not finite among this thread's values
+  if (odd) {
+    peak = 0.f;
+#pragma unroll
+    for (int j = 0; j < VECS; ++j) {
+      if (threadIdx.x + j * kThreads >= n) break;
+      float f[8];
+      unpack8(x[j], f);
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        if (fabsf(f[q]) <= FLT_MAX) peak = fmaxf(peak, fabsf(f[q]));
     }
   }
   peak = warp_max(peak);
@@ -163,7 +170,12 @@ __global__ void __launch_bounds__(kThreads, VECS <= 4 ? 5 : 3) kv8_append_kernel
       const uint32_t o[2] = {old[j].x, old[j].y};
       float f[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) f[q] = kv8_decode((o[q >> 2] >> (8 * (q & 3))) & 0xFFu, FMT) * before;
+      for (int h = 0; h < 2; ++h) {
+        float d[4];
+        kv8_decode4<FMT>(o[h], d);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) f[4 * h + q] = d[q] * before;
+      }
       codes[i] = after >= 1e-30f ? codes_fast<FMT>(f, after, r_lo, r_hi) : codes_exact(f, after, FMT);
     }
   }
@@ -173,6 +185,7 @@ __global__ void __launch_bounds__(kThreads, VECS <= 4 ? 5 : 3) kv8_append_kernel
 
 // One CTA: the positions of one sequence that lie in one block, for one KV head, keys (z = 0) or values.
 constexpr int kReadBatch = 8;
+template <int FMT>
 __global__ void __launch_bounds__(kThreads) kv8_read_kernel(GltKv8Cache c, GltKv8Batch b,
                                                             const int32_t* __restrict__ start, int count,
                                                             float* __restrict__ k, float* __restrict__ v,
@@ -201,7 +214,7 @@ __global__ void __launch_bounds__(kThreads) kv8_read_kernel(GltKv8Cache c, GltKv
 #pragma unroll
     for (int j = 0; j < kReadBatch; ++j) {
       const int i = u + j * kThreads;
-      w[j] = c.format == GLT_KV8_INT8 ? 0x80808080u : 0u;   // codes of 0
+      w[j] = FMT == GLT_KV8_INT8 ? 0x80808080u : 0u;   // codes of 0
       if (i < held) w[j] = codes[i];
     }
 #pragma unroll
@@ -209,9 +222,8 @@ __global__ void __launch_bounds__(kThreads) kv8_read_kernel(GltKv8Cache c, GltKv
       const int i = u + j * kThreads;
       if (i >= total) break;
       float f[4];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) f[q] = kv8_decode((w[j] >> (8 * q)) & 0xFFu, c.format) * s;
-      *reinterpret_cast<float4*>(dst + (i >> vec_log) * row + (i & (vecs - 1)) * 4) = make_float4(f[0], f[1], f[2], f[3]);
+      kv8_decode4<FMT>(w[j], f);
+      *reinterpret_cast<float4*>(dst + (i >> vec_log) * row + (i & (vecs - 1)) * 4) = make_float4(f[0] * s, f[1] * s, f[2] * s, f[3] * s);
     }
   }
 }
@@ -255,8 +267,9 @@ extern "C" int glt_kv8_read(const GltKv8Cache* cache, const GltKv8Batch* batch, 
   if (!glt::aligned16(k) || !glt::aligned16(v)) return glt::fail(GLT_EINVAL, "kv8: outputs must be 16-byte aligned");
   // blocks a range can touch
   const dim3 grid((count + cache->block_tokens - 2) / cache->block_tokens + 1, batch->num_seqs, 2 * cache->num_kv_heads);
-  glt::kv8_read_kernel<<<grid, glt::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(
-      *cache, *batch, start, count, k, v, glt::device_error_word());
+  const auto kernel = cache->format == GLT_KV8_INT8 ? glt::kv8_read_kernel<GLT_KV8_INT8> : glt::kv8_read_kernel<GLT_KV8_E4M3>;
+  kernel<<<grid, glt::kThreads, 0, static_cast<cudaStream_t>(stream)>>>(*cache, *batch, start, count, k, v,
+                                                                       glt::device_error_word());
   GLT_LAUNCH_CHECK();
   return GLT_OK;
 }
