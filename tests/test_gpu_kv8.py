@@ -244,6 +244,34 @@ def test_large_and_small_magnitudes():
         s.check_values()
 
 
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+@pytest.mark.parametrize("power", [0, 100, -50, -55, -62, -110])
+def test_codes_are_those_of_a_division(fmt, power):
+    """Every bf16 mantissa under a maximum of every mantissa (a head each), quotients that meet the codes' boundaries
+    among them, and the codes of a block whose scale rises: equal to rounding the 32-bit quotient."""
+    nkv, hd = 128, 64
+    cache = garbage_cache(3, 128, nkv, hd, fmt)
+    table = torch.tensor([[2]], dtype=torch.int32, device=DEV)
+    ref = {s: RefCache(fmt, 128, nkv, hd) for s in "kv"}
+    g = torch.Generator().manual_seed(power + 200)
+    past = 0
+    for n, rise in ((100, 1.0), (28, 1.37)):
+        i = torch.arange(n * hd)
+        x = (1 + (i % 128) / 128) * torch.exp2(-((i // 128) % 14).float() - 1)
+        x = x[torch.randperm(n * hd, generator=g)].view(n, 1, hd) * torch.randint(0, 2, (n, 1, hd), generator=g).mul(2).sub(1)
+        x = x.repeat(1, nkv, 1)
+        x[n // 2, :, 5] = 1 + torch.arange(nkv) / nkv   # the largest magnitude
+        x = (x * rise * 2.0 ** power).to(torch.bfloat16)
+        batch = serve.Kv8Batch(table, i32([past]), n, max_new=n)
+        cache.append(batch, x.to(DEV), -x.to(DEV))
+        ref["k"].append(0, x)
+        ref["v"].append(0, -x)
+        past += n
+        k, v = cache.read(batch, None, past)
+        assert torch.equal(k[0].cpu(), ref["k"].values(0).float())
+        assert torch.equal(v[0].cpu(), ref["v"].values(0).float())
+
+
 def test_non_finite_keys_saturate_and_nan_is_zero():
     for fmt in ("int8", "e4m3"):
         c = garbage_cache(3, 16, 1, 64, fmt)
