@@ -13,6 +13,9 @@
 // on the special-function unit (16 a clock and SM, against the 12 bf16 logits that HBM
 // brings): sums run two at a time (f32x2), maxima and clamps in packed bf16.
 //
+// Measured: 4096 x 128256 bf16 170 us without the most likely tokens (6.2 TB/s), 185 with 5 of them; the gradient of
+// 2047 x 128257 173 us (6.1 TB/s read and written).
+//
 // A row belongs to one CTA; with fewer rows than would fill the SMs, to a cluster of up
 // to eight, joined over distributed shared memory.
 #include <cooperative_groups.h>
