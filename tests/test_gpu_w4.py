@@ -119,6 +119,40 @@ def test_non_finite_inputs_stay_in_their_rows():
     assert y[2, 3] == -math.inf and (y[2, [i for i in range(40) if i != 3]] == math.inf).all()
 
 
+@pytest.mark.parametrize("out", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M", [3, 4, 6, 7, 10, 12, 13, 15, 20, 24])
+def test_every_number_of_row_tiles(M, out):
+    product(M, 2390, 1152, 64, M % 2 == 0, out=out, resid=M % 3 == 0)
+
+
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("M", [1, 6, 11, 19, 40])
+def test_non_finite_rows_with_many_rows_and_units(M, group):
+    """Infinities and NaN in the first and last block of some rows, sums that join over warps, the residual in place."""
+    N, K = 1030, 1216 if group == 32 else 1280
+    g = torch.Generator(device=DEV).manual_seed(M + group)
+    w = serve.W4Weight.quantize((torch.randn(N, K, device=DEV, generator=g) * 0.1).to(torch.bfloat16), group)
+    x = torch.randn(M, K, device=DEV, generator=g).to(torch.bfloat16)
+    x[0, 3] = math.nan
+    if M > 4:
+        x[M // 2, K - 1] = -math.inf
+    y = torch.randn(M, N, device=DEV, generator=g).to(torch.bfloat16)
+    r = y.clone()
+    w.linear(x, resid=y, out=y)
+    u = w.unpack().double()
+    assert torch.isnan(y[0]).all()
+    fine = torch.ones(M, dtype=torch.bool, device=DEV)
+    fine[0] = False
+    if M > 4:
+        fine[M // 2] = False
+        last = -math.inf * torch.sign(u[:, K - 1])   # NaN where the weight is 0
+        assert torch.equal(torch.nan_to_num(y[M // 2].double(), nan=7.0), torch.nan_to_num(last, nan=7.0))
+    ref = x.double() @ u.t() + r.double()
+    # unpacked weights are rounded to bf16
+    tol = (x.double().abs() @ u.abs().t()) * (2.0 ** -9 + 8 * 2.0 ** -22 + (K / 32 + 16) * 2.0 ** -23) + ref.abs() * 2.0 ** -8
+    assert ((y.double() - ref).abs() <= tol)[fine].all()
+
+
 def test_quantized_weight_is_near_the_matrix():
     """Rounding to 4 bits moves a weight by at most half a step (a step's bf16 rounding included)."""
     w = (torch.randn(96, 256, device=DEV) * 0.1).to(torch.bfloat16)
