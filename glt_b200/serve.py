@@ -10,6 +10,7 @@ stream of its tensors' device, allocates its outputs with torch and does not syn
 from __future__ import annotations
 
 import ctypes as C
+import threading
 from typing import NamedTuple
 
 import torch
@@ -28,9 +29,10 @@ def _stream(t: torch.Tensor) -> int:
     return _raw_stream(i) if _raw_stream is not None else torch.cuda.current_stream(i).cuda_stream
 
 
-class _Scratch:
-    """Workspaces of one object, one a stream: work on a stream runs in order, so its calls may share
-    one.  A call under capture gets its own, since graphs may replay side by side."""
+class _Scratch(threading.local):
+    """Workspaces of one host thread, one for each stream.  A call may be two launches that share its
+    workspace: a thread's calls on a stream run in order and may share one too, but another thread's may come
+    between the two.  A call under capture gets its own, since graphs may replay side by side."""
 
     def __init__(self):
         self._held: dict[int, torch.Tensor] = {}
@@ -42,6 +44,9 @@ class _Scratch:
             if not _capturing():
                 self._held[stream] = ws
         return ws
+
+
+_scratch = _Scratch()
 
 
 def _need(ok: bool, msg: str) -> None:
@@ -120,7 +125,6 @@ class Kv8Cache:
         self._c = _CCache(FORMATS[fmt], self.block_tokens, self.num_kv_heads, self.head_dim, self.num_blocks,
                           k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
         self._p = C.byref(self._c)
-        self._scratch = _Scratch()
 
     def append(self, batch: Kv8Batch, k: torch.Tensor, v: torch.Tensor) -> None:
         """Write the step's keys and values, bf16 [rows, num_kv_heads, head_dim] (views into packed rows are fine)."""
@@ -160,7 +164,7 @@ class Kv8Cache:
             check(lib.glt_kv8_attention_workspace(self._p, batch._p, nh, C.byref(n)))
             need = batch._ws_bytes[key] = n.value
         stream = _stream(q)
-        ws = self._scratch.get(need, q, stream)
+        ws = _scratch.get(need, q, stream)
         st = lib.glt_kv8_attention(self._p, batch._p, q.data_ptr(), ld_q, out.data_ptr(), ld_o, lse.data_ptr(), nh,
                                    scale, window, mask, ld_m, ws.data_ptr(), need, stream)
         if st:
@@ -188,7 +192,6 @@ class W4Weight:
     def __init__(self, packed: torch.Tensor, N: int, K: int, group: int, asym: bool):
         self.packed, self.N, self.K, self.group, self.asym = packed, N, K, group, bool(asym)
         self._ws_bytes: dict[tuple, int] = {}
-        self._scratch = _Scratch()
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None) -> "W4Weight":
@@ -244,7 +247,7 @@ class W4Weight:
             check(lib.glt_w4_linear_workspace(M, N, K, self.group, bf16, C.byref(n)))
             need = self._ws_bytes[M, bf16] = n.value
         stream = _stream(x)
-        ws = self._scratch.get(need, x, stream)
+        ws = _scratch.get(need, x, stream)
         st = lib.glt_w4_linear(self.packed.data_ptr(), N, K, self.group, self.asym, x.data_ptr(),
                                K if one else x.stride(0), M, out.data_ptr(), N if one else out.stride(0), bf16,
                                None if resid is None else resid.data_ptr(),
