@@ -186,16 +186,27 @@ class Kv8Cache:
         return k, v
 
 
+def _packed_bytes(N: int, K: int, group: int, asym: bool) -> int:
+    n = C.c_int64()
+    check(lib.glt_w4_packed_bytes(N, K, group, int(asym), C.byref(n)))
+    return n.value
+
+
 class W4Weight:
     """A weight matrix [N, K] in 4 bits with group scales, packed for ``linear``."""
 
     def __init__(self, packed: torch.Tensor, N: int, K: int, group: int, asym: bool):
+        need = _packed_bytes(N, K, group, asym)
+        _need(packed.is_cuda and packed.dtype is _U8 and packed.dim() == 1 and packed.is_contiguous()
+              and packed.numel() >= need, f"packed must be a contiguous uint8 CUDA tensor of at least {need} bytes")
         self.packed, self.N, self.K, self.group, self.asym = packed, N, K, group, bool(asym)
         self._ws_bytes: dict[tuple, int] = {}
 
     @classmethod
     def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None) -> "W4Weight":
         """codes uint8 [N, K] (0..15), scales bf16 [N, K / group], zeros uint8 like the scales or None (8)."""
+        _need(all(t is None or t.is_cuda for t in (codes, scales, zeros)), "codes, scales and zeros must be CUDA tensors")
+        _need(codes.dim() == 2, "codes [N, K]")
         N, K = codes.shape
         _need(scales.dim() == 2 and scales.shape[0] == N and scales.shape[1] > 0 and K % scales.shape[1] == 0,
               "scales must be [N, K / group]")
@@ -204,9 +215,7 @@ class W4Weight:
         _need(zeros is None or (zeros.dtype == torch.uint8 and zeros.shape == scales.shape), "zeros uint8 like scales")
         codes, scales = codes.contiguous(), scales.contiguous()
         zeros = None if zeros is None else zeros.contiguous()
-        need = C.c_int64()
-        check(lib.glt_w4_packed_bytes(N, K, group, int(zeros is not None), C.byref(need)))
-        packed = torch.empty(need.value, dtype=torch.uint8, device=codes.device)
+        packed = torch.empty(_packed_bytes(N, K, group, zeros is not None), dtype=torch.uint8, device=codes.device)
         check(lib.glt_w4_pack(codes.data_ptr(), scales.data_ptr(), None if zeros is None else zeros.data_ptr(), N, K,
                               group, packed.data_ptr(), _stream(codes)))
         return cls(packed, N, K, group, zeros is not None)
@@ -261,6 +270,7 @@ def quantize_w4(w: torch.Tensor, group: int = 128, asym: bool = False):
     """(codes uint8 [N, K], scales bf16 [N, K / group], zeros uint8 or None) of a bf16 matrix."""
     _need(w.is_cuda and w.dtype == torch.bfloat16 and w.dim() == 2 and w.stride(1) == 1, "w must be a bf16 CUDA matrix")
     N, K = w.shape
+    _packed_bytes(N, K, group, asym)   # refuses sizes and groups that do not fit
     codes = torch.empty(N, K, dtype=torch.uint8, device=w.device)
     scales = torch.empty(N, K // group, dtype=torch.bfloat16, device=w.device)
     zeros = torch.empty(N, K // group, dtype=torch.uint8, device=w.device) if asym else None

@@ -1,9 +1,11 @@
 """The host side of the decoding and scoring calls, without a GPU."""
 import threading
 
+import pytest
 import torch
 
 from glt_b200 import serve
+from glt_b200._lib import GltError
 from serve_host import Host, on
 
 
@@ -64,3 +66,36 @@ def test_calls_under_capture_have_workspaces_of_their_own(monkeypatch):
     w.linear(x)
     w.linear(x)
     assert len({args[-3] for _, _, args in host.calls}) == 3
+
+
+def test_weights_of_host_memory_are_refused(monkeypatch):
+    """Codes, scales and zeros as a checkpoint's reader returns them: the kernel would follow host addresses."""
+    host = Host(monkeypatch)
+    parts = (torch.zeros(64, 128, dtype=torch.uint8), torch.zeros(64, 4, dtype=torch.bfloat16),
+             torch.zeros(64, 4, dtype=torch.uint8))
+    for i in range(3):
+        mixed = [t if i == j else on(t) for j, t in enumerate(parts)]
+        with pytest.raises(ValueError, match="CUDA"):
+            serve.W4Weight.from_codes(*mixed)
+    with pytest.raises(ValueError, match="CUDA"):
+        serve.W4Weight.from_codes(*parts[:2])
+    assert not host.calls
+
+
+@pytest.mark.parametrize("packed", [lambda n: torch.zeros(n, dtype=torch.uint8), lambda n: on(torch.zeros(n - 1, dtype=torch.uint8)),
+                                    lambda n: on(torch.zeros(n, dtype=torch.int8)), lambda n: on(torch.zeros(2 * n, dtype=torch.uint8)[::2])])
+def test_packed_weights_that_do_not_hold_the_matrix_are_refused(monkeypatch, packed):
+    """Every read of `linear` and `unpack` lies within the size that N, K and the group ask for."""
+    Host(monkeypatch)
+    need = serve.C.c_int64()
+    serve.check(serve.lib.glt_w4_packed_bytes(64, 128, 32, 0, serve.C.byref(need)))
+    with pytest.raises(ValueError, match="packed"):
+        serve.W4Weight(packed(need.value), 64, 128, 32, False)
+
+
+@pytest.mark.parametrize("group", [0, -32, 48, 256])
+def test_groups_that_do_not_fit_are_refused_before_any_launch(monkeypatch, group):
+    host = Host(monkeypatch)
+    with pytest.raises(GltError):
+        serve.quantize_w4(on(torch.zeros(4, 128, dtype=torch.bfloat16)), group)
+    assert not host.calls
