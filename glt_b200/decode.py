@@ -94,6 +94,10 @@ class Decoder:
 
     def step(self, ids: torch.Tensor) -> torch.Tensor:
         """New tokens ids [seqs, n] of every sequence: fp32 logits [seqs, vocab] after the last one."""
+        with torch.cuda.device(self.embed.device):   # the layer kernels take the current one
+            return self._step(ids)
+
+    def _step(self, ids: torch.Tensor) -> torch.Tensor:
         n, hd = ids.shape[1], self.head_dim
         batch = serve.Kv8Batch(self.table, self.lengths, ids.numel())
         pos = (self.lengths[:, None] + torch.arange(n, device=ids.device)).flatten()

@@ -32,6 +32,8 @@ class Host:
         monkeypatch.setattr(serve, "lib", self)
         monkeypatch.setattr(serve, "_raw_stream", lambda index: self.stream)
         monkeypatch.setattr(serve, "_capturing", lambda: False)
+        monkeypatch.setattr(serve, "_current_device", lambda: self.current, raising=False)
+        monkeypatch.setattr(torch.cuda, "device", lambda index: on_device(self, index))
 
     # -- torch
     def empty(self, *shape, dtype=torch.float32, device=None):
@@ -53,3 +55,16 @@ class Host:
 
     def launched(self, name, args):
         return 0
+
+
+class on_device:
+    """torch.cuda.device for a Host: launches note the device that is current."""
+
+    def __init__(self, host, index):
+        self.host, self.index = host, index
+
+    def __enter__(self):
+        self.before, self.host.current = self.host.current, self.index
+
+    def __exit__(self, *_):
+        self.host.current = self.before
