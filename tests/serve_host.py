@@ -61,7 +61,7 @@ class on_device:
     """torch.cuda.device for a Host: launches note the device that is current."""
 
     def __init__(self, host, index):
-        self.host, self.index = host, index
+        self.host, self.index = host, index if isinstance(index, int) else index.index
 
     def __enter__(self):
         self.before, self.host.current = self.host.current, self.index
