@@ -46,12 +46,13 @@ class Decoder:
     """A decoder over 4-bit projections (the head is the embedding's transpose) and an 8-bit cache.
 
     The cache holds ``seqs`` sequences of up to ``max_tokens`` tokens; ``lengths`` counts the tokens
-    each one has."""
+    each one has on the device, ``held`` on the host.  ``reset`` forgets them."""
 
     def __init__(self, weights: dict, heads: int, kv_heads: int, head_dim: int, seqs: int, max_tokens: int,
                  group: int = 64, block_tokens: int = 64, fmt: str = "int8", rope_theta: float = 1e6,
                  eps: float = 1e-6):
         self.heads, self.kv_heads, self.head_dim, self.seqs, self.eps = heads, kv_heads, head_dim, seqs, eps
+        self.max_tokens, self.held = max_tokens, 0
         self.embed, self.final_norm = weights["embed"], weights["final_norm"]
         dev = self.embed.device
         self.head = serve.W4Weight.quantize(self.embed, group)
@@ -92,10 +93,26 @@ class Decoder:
                                  half, torch.cuda.current_stream().cuda_stream))
         return h
 
+    def reset(self) -> None:
+        """Starts over with empty sequences."""
+        self.lengths.zero_()
+        self.held = 0
+
+    def _fits(self, ids: torch.Tensor, more: int = 0) -> None:
+        """Refuses what the cache and the rotary table have no room for: ids [seqs, n] and `more` tokens after them."""
+        if ids.dim() != 2 or ids.shape[0] != self.seqs or ids.shape[1] < 1 or ids.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"ids must be int32 or int64 [{self.seqs}, at least 1], got {ids.dtype} {tuple(ids.shape)}")
+        n = ids.shape[1] + more
+        if self.held + n > self.max_tokens:
+            raise ValueError(f"{n} tokens after the {self.held} held are more than max_tokens {self.max_tokens}")
+
     def step(self, ids: torch.Tensor) -> torch.Tensor:
         """New tokens ids [seqs, n] of every sequence: fp32 logits [seqs, vocab] after the last one."""
+        self._fits(ids)
         with torch.cuda.device(self.embed.device):   # the layer kernels take the current one
-            return self._step(ids)
+            logits = self._step(ids)
+        self.held += ids.shape[1]
+        return logits
 
     def _step(self, ids: torch.Tensor) -> torch.Tensor:
         n, hd = ids.shape[1], self.head_dim
@@ -116,6 +133,9 @@ class Decoder:
 
     def generate(self, prompt: torch.Tensor, tokens: int):
         """Greedy continuation of prompt [seqs, n]: (ids [seqs, tokens], log probabilities)."""
+        if tokens < 1:
+            raise ValueError(f"{tokens} tokens to generate (at least 1)")
+        self._fits(prompt, tokens - 1)   # the last one is not fed back
         ids, logps = [], []
         logits = self.step(prompt)
         for i in range(tokens):
@@ -133,16 +153,22 @@ def main() -> None:
     ap.add_argument("--prompt", type=int, default=256)
     ap.add_argument("--tokens", type=int, default=64)
     a = ap.parse_args()
+    if min(a.seqs, a.prompt, a.tokens) < 1:
+        ap.error("--seqs, --prompt and --tokens must be at least 1")
     w = random_weights(hidden=896, intermediate=4864, layers=24, heads=14, kv_heads=2, head_dim=64, vocab=151936)
     d = Decoder(w, heads=14, kv_heads=2, head_dim=64, seqs=a.seqs, max_tokens=a.prompt + a.tokens)
     prompt = torch.randint(0, 151936, (a.seqs, a.prompt), device="cuda", dtype=torch.int32)
     d.generate(prompt, 2)   # first calls load their kernels
-    d.lengths.zero_()
+    d.reset()
     torch.cuda.synchronize()
     t = time.perf_counter()
     ids, logps = d.generate(prompt, a.tokens)
     torch.cuda.synchronize()
     t = time.perf_counter() - t
+    code = C.c_uint()
+    check(lib.glt_device_error(C.byref(code)))
+    if code.value:
+        raise RuntimeError(f"device error word {code.value}")
     print(f"{a.seqs} sequences, prompt {a.prompt}: {a.seqs * a.tokens / t:.0f} tokens/s "
           f"({1e3 * t / a.tokens:.2f} ms a step), mean log probability {logps.mean().item():.3f}")
 

@@ -191,5 +191,6 @@ def test_a_decoder_steps_on_its_own_device(monkeypatch):
     host = Host(monkeypatch)
     d = decode.Decoder.__new__(decode.Decoder)
     d.embed = on(torch.zeros(4, 64), 1)
+    d.seqs, d.max_tokens, d.held = 1, 4, 0
     d._step = lambda ids: host.current
-    assert d.step(None) == 1 and host.current == 0
+    assert d.step(torch.zeros(1, 1, dtype=torch.int32)) == 1 and host.current == 0
