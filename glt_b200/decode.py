@@ -73,6 +73,13 @@ class Decoder:
         angle = torch.outer(torch.arange(max_tokens, device=dev, dtype=torch.float32), inv)
         self.cos, self.sin = angle.cos(), angle.sin()
 
+    def _lookup(self, ids: torch.Tensor) -> torch.Tensor:
+        """Rows of the embedding for ids [seqs, n].  A sequence with an id outside the vocabulary gets NaN, which
+        its logits and log probabilities show: the host does not wait to look at the ids."""
+        known = (ids >= 0) & (ids < self.embed.shape[0])
+        rows = self.embed[torch.where(known, ids, 0).flatten()]
+        return rows.masked_fill_(~known.all(1, keepdim=True).expand_as(ids).reshape(-1, 1), float("nan"))
+
     def _norm(self, x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
         y, var = torch.empty_like(x), torch.empty(x.shape[0], device=x.device)
         check(lib.glt_rmsnorm_fwd(_p(x), _p(w), _p(y), _p(var), x.shape[0], x.shape[1], self.eps,
@@ -118,7 +125,7 @@ class Decoder:
         n, hd = ids.shape[1], self.head_dim
         batch = serve.Kv8Batch(self.table, self.lengths, ids.numel())
         pos = (self.lengths[:, None] + torch.arange(n, device=ids.device)).flatten()
-        x = self.embed[ids.flatten()]
+        x = self._lookup(ids)
         for w in self.layers:
             qkv = w["qkv"].linear(self._norm(x, w["in_norm"])).unflatten(1, (-1, hd))
             rotated = self._rope(qkv[:, :self.heads + self.kv_heads], pos)

@@ -75,3 +75,15 @@ def test_the_command_refuses_empty_work(monkeypatch, args):
     monkeypatch.setattr(decode, "random_weights", lambda **k: pytest.fail("weights were made"))
     with pytest.raises(SystemExit):
         decode.main()
+
+
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64])
+def test_ids_outside_the_vocabulary_give_their_sequence_nan(dtype):
+    """An index out of range would end the context, and a negative one would silently count from the end."""
+    d = decode.Decoder.__new__(decode.Decoder)
+    d.embed = torch.randn(7, 64).to(torch.bfloat16)
+    good = torch.tensor([[0, 6, 3]], dtype=dtype)
+    for bad in (7, -1, 2 ** 31 - 1, -2 ** 31):
+        x = d._lookup(torch.cat((good, torch.tensor([[5, bad, 2]], dtype=dtype), good)))
+        assert torch.equal(x[:3], d.embed[[0, 6, 3]]) and torch.equal(x[6:], x[:3])
+        assert torch.isnan(x[3:6]).all() and x.dtype == torch.bfloat16
