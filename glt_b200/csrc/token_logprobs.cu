@@ -36,9 +36,10 @@ constexpr int kCtasPerSm = 4;
 constexpr int kMaxTop = 32;
 constexpr int kBatch = 4;            // 16-byte vectors a thread has in flight
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// Logits below this count as probability 0 in the fast path, which is exact there: it runs
-// with a maximum of at least kFloor / 10 and a scale of at least 1e-6.
-constexpr float kFloor = -1e30f;
+// The fast path takes exponents as a x - a m in one fused sum, for |a m| up to kNear: beyond it a logit's
+// own spacing is 1/8 or more, and further up a m overflows while the logits are finite.
+// Logits below kFloor count as probability 0 there, which is exact: with a scale of 1e-6 or more, m is above -1e12.
+constexpr float kFloor = -1e30f, kNear = 1048576.f;
 
 __device__ __forceinline__ float logit(const float* p) { return *p; }
 __device__ __forceinline__ float logit(const uint16_t* p) { return bf16_bits_to_f32(*p); }
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) token_logprobs_kernel(
       best = v;
     }
     const float ma = st.m * a;
-    if (st.m >= kFloor / 10 && fast_scale) {
+    if (fabsf(ma) <= kNear && fast_scale) {
       const uint64_t mm = pair(-ma, -ma);
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
@@ -443,8 +444,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) token_logprobs_kernel(
     const bool empty = all.m == -INFINITY;
     const float ls = logf(all.s);
     const float lse = bad ? NAN : empty ? -INFINITY : fmaf(all.m, scale, ls);
-    // log probability of a logit: the difference to the maximum first, so that nothing large cancels
-    auto log_p = [&](float x) { return bad ? NAN : empty ? -INFINITY : (x - all.m) * scale - ls; };
+    // log probability of a logit: the difference to the maximum first, so that nothing large cancels,
+    // unless it is beyond the float range and its product with a scale below 1 is not
+    auto log_p = [&](float x) {
+      if (bad) return NAN;
+      if (empty) return -INFINITY;
+      const float d = (x - all.m) * scale;
+      return (d > -INFINITY ? d : fmaf(x, scale, -(all.m * scale))) - ls;
+    };
     if (lane == 0) {
       lse_out[r] = lse;
       if (entropy) entropy[r] = bad ? NAN : empty ? 0.f : fmaf(-kLn2, all.t / all.s, ls);

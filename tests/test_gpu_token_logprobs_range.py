@@ -1,0 +1,81 @@
+"""Token log probabilities of logits far from 0 (glt_token_logprobs) against 64-bit forms.
+
+A row's statistics are taken relative to its maximum, so their error does not grow with it: with d = scale (x - max),
+a term exp(d) is off by 2^-21 and 2^-22 |d| of itself (|d| exp(d) <= 1), and sums of V terms run at most V + 16
+additions deep for V <= 64, V / 64 + 64 for more.  So ls = log sum exp d is off by e below, logp by e + 2^-22 |d|,
+the entropy by 2 e (1 + entropy); only lse = scale max + ls carries the maximum's own 2^-23."""
+
+import pytest
+import torch
+
+from glt_b200 import serve
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def compare(x, scale, top=0):
+    R, V = x.shape
+    d64 = (x.double() - x.double().amax(-1, keepdim=True)) * scale
+    ls = torch.logsumexp(d64, -1)
+    lq = d64 - ls[:, None]
+    p = lq.exp()
+    ent = -torch.where(p > 0, p * lq, torch.zeros_like(p)).sum(-1)
+    lse = x.double().amax(-1) * scale + ls
+    e = (V + 16 if V <= 64 else V / 64 + 64) * 2.0 ** -24 + 2.0 ** -21 + 2.0 ** -22
+    pick = list(range(min(V, 5))) + [V // 2, V - 1] + [int(x[0].float().argmax())]
+    for v in sorted(set(pick)):
+        t = torch.full((R,), v, device=DEV, dtype=torch.int32)
+        f = serve.token_logprobs(x, t, scale=scale, top=top)
+        want = lq[:, v]
+        got = f.logp.double()
+        huge = want < -3.3e38                      # beyond fp32
+        assert (got[huge] < -3e38).all()
+        assert ((got - want).abs() <= e + 2.0 ** -22 * d64[:, v].abs())[~huge].all(), ((got - want).abs()[~huge].max(), e)
+        assert (got <= 0).all()
+    far = lse.abs() > torch.finfo(torch.float32).max * (1 + 2.0 ** -24)
+    assert ((f.lse.double() - lse).abs() <= 2.0 ** -23 * lse.abs() + e)[~far].all() and torch.isinf(f.lse[far]).all()
+    assert ((f.entropy.double() - ent).abs() <= 2 * e * (1 + ent)).all(), (f.entropy.double() - ent).abs().max()
+    if top:
+        ids = torch.sort(x.double(), dim=-1, descending=True, stable=True).indices[:, :top]
+        assert torch.equal(f.top_ids.long(), ids)
+        want = lq.gather(1, ids)
+        ok = want > -3.3e38
+        assert ((f.top_logp.double() - want).abs() <= e + 2.0 ** -22 * d64.gather(1, ids).abs())[ok].all()
+
+
+def spread(R, V, at, step, dtype, seed):
+    """Rows whose maximum is `at`, the others a few multiples of `step` (a multiple of at's spacing) below."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = at - torch.randint(0, 40, (R, V), device=DEV, generator=g).double() * step
+    x[:, V // 3] = at
+    y = x.to(dtype)
+    assert torch.equal(y.double(), x)
+    return y
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.37, 3.0])
+@pytest.mark.parametrize("V", [9, 64, 1000, 20001])
+@pytest.mark.parametrize("at,step", [(float(2 ** 21 + 1), 0.25), (float(2 ** 23 - 1), 0.5),
+                                     (-float(2 ** 22 - 1), 0.5), (float(2 ** 31), 256.0), (2.0 ** 60, 2.0 ** 37)])
+def test_large_maxima_keep_their_differences(at, step, V, scale):
+    compare(spread(3, V, at, step, torch.float32, V), scale, top=min(V, 5))
+
+
+@pytest.mark.parametrize("scale", [1.0, 0.25, 3.0])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("V", [8, 1001, 20000])
+def test_logits_at_the_type_s_ends(V, dtype, scale):
+    top, low = torch.finfo(dtype).max, torch.finfo(dtype).min
+    g = torch.Generator(device=DEV).manual_seed(V)
+    x = torch.empty(6, V, device=DEV, dtype=dtype)
+    x[0] = top                                         # all equal
+    x[1] = low
+    x[1, V // 2] = top                                 # one token
+    x[2] = torch.where(torch.rand(V, device=DEV, generator=g) < 0.5, top, low).to(dtype)
+    x[3] = torch.randn(V, device=DEV, generator=g).to(dtype)
+    x[3, 1] = top
+    x[4] = low
+    x[5] = (torch.rand(V, device=DEV, generator=g) * 2 - 1).to(dtype) * (top / 2)
+    x[2, 0] = top
+    compare(x, scale, top=4)
