@@ -37,9 +37,15 @@ constexpr int kMaxTop = 32;
 constexpr int kBatch = 4;            // 16-byte vectors a thread has in flight
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // The fast path takes exponents as a x - a m in one fused sum, for |a m| up to kNear: beyond it a logit's
-// own spacing is 1/8 or more, and further up a m overflows while the logits are finite.
+// own spacing is 1/8 or more, and further up a m overflows while the logits are finite.  What the rounding
+// of a m adds to every exponent (carried() below) is known exactly and taken off the sums whenever they are
+// compared with others: at a maximum of 1000 it was 1.6e-5 of a log probability.
 // Logits below kFloor count as probability 0 there, which is exact: with a scale of 1e-6 or more, m is above -1e12.
 constexpr float kFloor = -1e30f, kNear = 1048576.f;
+// Exponents a x - fl(a m) are (x - m) a plus this; `near_to` is kNear, or below 0 with a scale that the fast path leaves out.
+__device__ __forceinline__ float carried(float m, float a, float near_to) {
+  return fabsf(m * a) <= near_to ? fmaf(m, a, -(m * a)) : 0.f;
+}
 
 __device__ __forceinline__ float logit(const float* p) { return *p; }
 __device__ __forceinline__ float logit(const uint16_t* p) { return bf16_bits_to_f32(*p); }
@@ -240,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) token_logprobs_kernel(
     }
   };
   uint4 cur[kBatch], nxt[kBatch];
-  const bool fast_scale = scale >= 1e-6f && scale <= 1e6f;
+  const float near_to = scale >= 1e-6f && scale <= 1e6f ? kNear : -1.f;
   load(nxt, v0 + threadIdx.x);
   for (int v = v0 + threadIdx.x; v < v1; v += kBatch * kThreads) {
 #pragma unroll
@@ -250,7 +256,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) token_logprobs_kernel(
     if (!(cm < INFINITY)) bad = true;
     if (cm > st.m) {
       if (st.m > -INFINITY) {
-        const float d = (st.m - cm) * a, f = exp2f(d);
+        // from one rounded product to the other, or as far as one of them is out of the fast path's range
+        const float from = __fmul_rn(st.m, a), to = __fmul_rn(cm, a);
+        float d = from - to;
+        if (!(fmaxf(fabsf(from), fabsf(to)) <= near_to))
+          d = (st.m - cm) * a + (carried(cm, a, near_to) - carried(st.m, a, near_to));
+        const float f = exp2f(d);
         float s0, s1, t0, t1;
         unpair(s2, s0, s1);
         unpair(t2, t0, t1);
@@ -261,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) token_logprobs_kernel(
       best = v;
     }
     const float ma = st.m * a;
-    if (fabsf(ma) <= kNear && fast_scale) {
+    if (fabsf(ma) <= near_to) {
       const uint64_t mm = pair(-ma, -ma);
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
@@ -314,8 +325,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) token_logprobs_kernel(
     float s0, s1, t0, t1;
     unpair(s2, s0, s1);
     unpair(t2, t0, t1);
-    st.s = s0 + s1;
-    st.t = t0 + t1;
+    const float off = carried(st.m, a, near_to), f = 1.f / ex2_approx(off);   // a lone token's sum is this 2^off
+    st.s = f * (s0 + s1);
+    st.t = f * fmaf(-off, s0 + s1, t0 + t1);
   }
   // what this thread's vectors can rank: at best (its maximum, first index of the batch), surely
   // no worse than (its maximum, last index)
@@ -442,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) token_logprobs_kernel(
       }
     }
     const bool empty = all.m == -INFINITY;
-    const float ls = logf(all.s);
+    const float ls = logf(fmaxf(all.s, 1.f));   // the maximum's own term is 1
     const float lse = bad ? NAN : empty ? -INFINITY : fmaf(all.m, scale, ls);
     // log probability of a logit: the difference to the maximum first, so that nothing large cancels,
     // unless it is beyond the float range and its product with a scale below 1 is not

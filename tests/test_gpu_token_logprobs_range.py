@@ -4,6 +4,7 @@ A row's statistics are taken relative to its maximum, so their error does not gr
 a term exp(d) is off by 2^-21 and 2^-22 |d| of itself (|d| exp(d) <= 1), and sums of V terms run at most V + 16
 additions deep for V <= 64, V / 64 + 64 for more.  So ls = log sum exp d is off by e below, logp by e + 2^-22 |d|,
 the entropy by 2 e (1 + entropy); only lse = scale max + ls carries the maximum's own 2^-23."""
+import math
 
 import pytest
 import torch
@@ -56,7 +57,7 @@ def spread(R, V, at, step, dtype, seed):
 
 @pytest.mark.parametrize("scale", [1.0, 0.37, 3.0])
 @pytest.mark.parametrize("V", [9, 64, 1000, 20001])
-@pytest.mark.parametrize("at,step", [(float(2 ** 21 + 1), 0.25), (float(2 ** 23 - 1), 0.5),
+@pytest.mark.parametrize("at,step", [(float(2 ** 20 + 3), 0.125), (float(2 ** 21 + 1), 0.25), (float(2 ** 23 - 1), 0.5),
                                      (-float(2 ** 22 - 1), 0.5), (float(2 ** 31), 256.0), (2.0 ** 60, 2.0 ** 37)])
 def test_large_maxima_keep_their_differences(at, step, V, scale):
     compare(spread(3, V, at, step, torch.float32, V), scale, top=min(V, 5))
@@ -79,3 +80,28 @@ def test_logits_at_the_type_s_ends(V, dtype, scale):
     x[5] = (torch.rand(V, device=DEV, generator=g) * 2 - 1).to(dtype) * (top / 2)
     x[2, 0] = top
     compare(x, scale, top=4)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("at", [20.3, 37.7, 61.1, 1003.0, 3.3e4, 7.1e5])
+def test_one_likely_token_has_probability_one(at, dtype):
+    """log p of the only token is 0, and no log probability is above it."""
+    g = torch.Generator(device=DEV).manual_seed(int(at))
+    for V in (8, 515, 20001):
+        x = torch.full((16, V), -math.inf, device=DEV, dtype=dtype)
+        m = (at * (1 + torch.rand(16, device=DEV, generator=g) / 2)).to(dtype)
+        x[:, V // 2] = m
+        x[8:] = torch.maximum(x[8:], (m[8:, None] - 200 - at / 2).to(dtype))   # too far below to count
+        t = torch.full((16,), V // 2, device=DEV, dtype=torch.int32)
+        for scale in (1.0, 0.7, 1.9):
+            f = serve.token_logprobs(x, t, scale=scale)
+            assert (f.logp == 0).all() and (f.entropy.abs() <= 2.0 ** -21).all()
+            want = m.double() * scale
+            assert ((f.lse.double() - want).abs() <= 2.0 ** -23 * want).all()
+
+
+@pytest.mark.parametrize("at,step", [(24.0, 0.125), (60.5, 0.25), (1000.0, 0.5), (32768.0, 0.25), (524288.0, 0.25)])
+@pytest.mark.parametrize("V", [8, 33, 1000, 20001])
+def test_confident_rows_keep_their_digits(at, step, V):
+    for seed in range(4):
+        compare(spread(5, V, at + seed * step, step, torch.float32, seed), 1.0 if seed % 2 else 0.77)
