@@ -8,10 +8,12 @@
 // Lane 4g + c of a warp owns words 4 * lane + s, s = 0..3, of a chunk; byte b of word s holds
 // the codes of row g (low nibble) and row g + 8 (high nibble) at column
 // (s / 2) * 32 + 8 c + (s % 2) * 4 + b.  So one AND (and a shift) makes four codes a register
-// of operand A of mma.m16n8k32 on bytes.
+// of operand A of mma.m16n8k32 on bytes, and a word is operand A of mma.m16n8k16 on f16, columns
+// b = 0, 2 and b = 1, 3 side by side.
 #include <math.h>
 
 #include <climits>
+#include <type_traits>
 
 #include "common.cuh"
 #include "gemm.cuh"
@@ -150,52 +152,89 @@ __device__ __forceinline__ void mma_u8s8(int (&d)[4], const uint32_t (&a)[4], ui
       : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// The same from sums of 0.
+__device__ __forceinline__ void mma_f16_zero(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+}
+// Both halves of a register as f16 numbers.
+__device__ __forceinline__ uint32_t sub_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// 2^n for -149 <= n <= 127.
+__device__ __forceinline__ float power_of_two(int n) { return __int_as_float(n >= -126 ? (n + 127) << 23 : 1 << (n + 149)); }
 
-// ---- operand B.  Within a block of 128 columns a row of x becomes fixed-point numbers
-// v = round(x 2^a), with a such that the largest fills 16 bits (LIMBS = 2) or 24 (LIMBS = 3), and
-// v its signed bytes, one column of operand B each.  Products with the codes are then exact
-// integers.  bf16 has 8 bits, so v is x exactly down to 2^-8 of the block's largest magnitude
-// (2^-16 with three bytes), and off by at most 2^-16 (2^-24) of it below: two bytes for results
-// in bf16, three for results in fp32.
-// (On the tensor core, k = 32 of bytes costs what k = 16 of bf16 does, 8 cycles, and the codes need
-// two thirds of an instruction for four where bf16 needs seven; e4m3 is no faster than f16 here.)
-// A tile of N = 8 columns holds 8 / LIMBS rows of x at 2 (or 4, the last empty) columns a row, high
-// byte first.  Image: [chunk of 64][tile of rows][lane][16 bytes], lane 4g + c the column g at the
-// k of operand A's lanes c.
+// ---- operand B: the image of x.  Within a block of 128 columns a row of x is multiplied by a power of two,
+// 2^a, that its largest magnitude chooses, and held in one of two forms.  Both keep every bf16 number down to
+// 2^-22 of that magnitude exactly, and round off only what lies below 2^-30 of it: outliers a million times
+// the other columns cost these nothing, also where an outlier's own weight is 0.
+//
+// HALF: one f16 number a value, the largest in [2^15, 2^16): 8 rows of x are a tile of N = 8 columns.  Codes
+// less their zero are f16 too, exactly; products are exact and sums in 32 bits.
+//
+// Bytes: fixed-point numbers v = round(x 2^a), the largest in [2^30, 2^31), as four signed bytes, a column of
+// operand B each: 2 rows are a tile.  Products with the codes are exact integers until a group's end.
+//
+// Which.  A matrix instruction of bytes takes twice the columns of one of f16 at the same cost, and eight codes
+// need three instructions where f16 needs nine; but a row takes four columns, and a group's end six instructions
+// for two rows of W where f16 takes two.  So bytes for up to 4 rows, with groups of 32 for up to 2 (28672 x 4096,
+// us, bytes and f16: groups of 128, 1 row 14.8 and 18.6, 4 rows 18.3 and 20.8; of 32, 1 row 16.7 and 19.8,
+// 4 rows 23.8 and 22.4).
+//
+// Image: [chunk of 64][tile of rows] with, for bytes, [lane][16 bytes], high byte first, and for f16
+// [half][lane][16 bytes]; lane 4g + c holds column g at the k of operand A's lanes c.
 constexpr int kPrepThreads = 256;
 constexpr int kMagic = 0x4B400000;   // 1.5 2^23 as a float: kMagic + i is the float 1.5 2^23 + i
-// What lane c needs at the ends of a group: what its two columns' sums begin with, kMagic - 8 (asym: 15)
-// times the sum of the bytes, and 2^-a of its row's block: NaN where the block holds something
-// that is not finite, and such a row's products are then done the plain way.
+// Bytes: what lane c needs at the ends of a group: what its two columns' sums begin with, kMagic - 8 (asym: 15)
+// times the sum of the bytes, and 2^-a of its row's block.  (f16: two factors 2^-a a lane and block.)
+// A factor is NaN where the block holds something that is not finite; such a row's products are then done the
+// plain way.
 struct __align__(16) GroupNote {
   int start[2];
   float factor;
   int pad;
 };
-template <int LIMBS>
+template <bool HALF>
 struct XImage {
-  static constexpr int kCols = LIMBS == 2 ? 2 : 4, kRows = 8 / kCols;   // columns a row, rows a tile
+  static constexpr int kRows = HALF ? 8 : 2;          // a tile's
+  static constexpr int kChunk = HALF ? 1024 : 512;    // bytes of a tile's chunk,
+  static constexpr int kNote = HALF ? 32 : 64;        // of its notes
   int per_cta;   // tiles of rows of x that a CTA takes
-  int tiles, chunks, groups;   // tiles filled up to per_cta's multiple; chunks and groups to the end of the last block
+  int tiles, chunks, noted;   // tiles filled up to per_cta's multiple; chunks and blocks (bytes: groups) to the end of the last block
   int64_t notes, bytes;   // offset in the workspace, after the image; of both
   __host__ __device__ XImage(const W4Layout& L, int M) {
-    const int need = (M + kRows - 1) / kRows;
-    per_cta = need <= 5 ? need : 8;
-    tiles = (need + per_cta - 1) / per_cta * per_cta;
+    const int need = (M + kRows - 1) / kRows, ctas = (need + kMaxTiles - 1) / kMaxTiles;
+    per_cta = (need + ctas - 1) / ctas;
+    tiles = per_cta * ctas;
     chunks = L.blocks * 2;
-    groups = L.blocks * L.per_block;
-    notes = static_cast<int64_t>(chunks) * tiles * 512;
-    // notes: [group][tile][lane c]
-    bytes = notes + static_cast<int64_t>(groups) * tiles * 4 * sizeof(GroupNote);
+    noted = HALF ? L.blocks : L.blocks * L.per_block;
+    notes = static_cast<int64_t>(chunks) * tiles * kChunk;
+    bytes = notes + static_cast<int64_t>(noted) * tiles * kNote;   // [block or group][tile][lane c]
   }
+  static constexpr int kMaxTiles = 4;
 };
+bool half_image(const W4Layout& L, int M) { return M > (L.group == 32 ? 2 : 4); }
+int64_t image_bytes(const W4Layout& L, int M) { return half_image(L, M) ? XImage<true>(L, M).bytes : XImage<false>(L, M).bytes; }
 
 // Eight columns (vector v) of row m of x into the image at ws; the threads of a block's 16 vectors are
 // neighbours and all here.
-template <int LIMBS, int GROUP>
+template <bool HALF, int GROUP>
 __device__ __forceinline__ void prepare_vector(const uint16_t* __restrict__ x, int64_t ld_x, const W4Layout& L,
-                                               const XImage<LIMBS>& I, int m, int v, uint8_t* ws) {
-  using Image = XImage<LIMBS>;
+                                               const XImage<HALF>& I, int m, int v, uint8_t* ws) {
+  using Image = XImage<HALF>;
   const bool in = v < I.chunks * 8;
   uint4 u = make_uint4(0, 0, 0, 0);
   if (in && v * 8 < L.K) u = *reinterpret_cast<const uint4*>(x + m * ld_x + v * 8);
@@ -204,65 +243,70 @@ __device__ __forceinline__ void prepare_vector(const uint16_t* __restrict__ x, i
   float peak = 0.f;
 #pragma unroll
   for (int k = 0; k < 8; ++k) peak = fabsf(f[k]) <= peak ? peak : fabsf(f[k]) < INFINITY ? fabsf(f[k]) : INFINITY;
-  constexpr int kLanes = GROUP / 8;   // of a group; 16 of a block
 #pragma unroll
   for (int o = 1; o < 16; o <<= 1) peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, o));
-  // the largest to [2^14, 2^15) or [2^22, 2^23), one less for the one mantissa whose high byte would be 128
+  const bool finite = peak < INFINITY;
+  const int chunk = v >> 3, step = (v >> 2) & 1, c = v & 3, tile = m / Image::kRows, row = m % Image::kRows;
   int a = 0;
-  if (peak > 0.f && peak < INFINITY) {
+  if (HALF) {
+    if (peak > 0.f && finite) a = 15 - ilogbf(peak);
+  } else if (peak > 0.f && finite) {
+    // one less for the one mantissa whose high byte would be 128; 2^149 makes every number an integer, and its
+    // reciprocal is the smallest float
     const int e = ilogbf(peak);
     const bool top = (__float_as_uint(peak) >> 16 & 0x7F) == 0x7F && e > -127;
-    a = (LIMBS == 2 ? 14 : 22) - e - (top ? 1 : 0);
+    a = min(30 - e - (top ? 1 : 0), 149);
   }
   // in two factors: 2^a may be out of range
-  const float a0 = exp2f(static_cast<float>(a / 2)), a1 = exp2f(static_cast<float>(a - a / 2));
-  uint32_t limb[LIMBS][2] = {};
-  int sum[LIMBS] = {};
+  const float a0 = power_of_two(a / 2), a1 = power_of_two(a - a / 2);
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    int i = peak < INFINITY ? __float2int_rn(f[k] * a0 * a1) : 0;
+  for (int k = 0; k < 8; ++k) f[k] = finite ? f[k] * a0 * a1 : 0.f;
+  const float factor = finite ? power_of_two(-a) : NAN;
+  if constexpr (HALF) {
+    if (!in) return;
+    uint8_t* dst = ws + (static_cast<int64_t>(chunk) * I.tiles + tile) * Image::kChunk + step * 512 + (row * 4 + c) * 16;
+    *reinterpret_cast<uint4*>(dst) =
+        make_uint4(pack_f16x2(f[0], f[2]), pack_f16x2(f[1], f[3]), pack_f16x2(f[4], f[6]), pack_f16x2(f[5], f[7]));
+    if (v % 16 == 0)   // of the block: two rows a lane
+      reinterpret_cast<float*>(ws + I.notes + (static_cast<int64_t>(v / 16) * I.tiles + tile) * Image::kNote)[row] = factor;
+  } else {
+    constexpr int kLanes = GROUP / 8;   // of a group; 16 of a block
+    uint32_t limb[4][2] = {};
+    int sum[4] = {};
 #pragma unroll
-    for (int l = LIMBS - 1; l >= 0; --l) {
-      const int up = l > 0 ? (i + 128) >> 8 : 0;   // what the next higher byte takes
-      const int b = i - up * 256;
-      limb[l][k >> 2] |= (static_cast<uint32_t>(b) & 0xFFu) << (8 * (k & 3));
-      sum[l] += b;
-      i = up;
-    }
-  }
+    for (int k = 0; k < 8; ++k) {
+      int i = __float2int_rn(f[k]);
 #pragma unroll
-  for (int o = 1; o < kLanes; o <<= 1)
-#pragma unroll
-    for (int l = 0; l < LIMBS; ++l) sum[l] += __shfl_xor_sync(0xffffffffu, sum[l], o);
-  if (!in) return;
-  const int chunk = v >> 3, step = (v >> 2) & 1, c = v & 3, tile = m / Image::kRows, row = m % Image::kRows;
-  uint8_t* dst = ws + ((static_cast<int64_t>(chunk) * I.tiles + tile) * 32 + row * Image::kCols * 4 + c) * 16 + step * 8;
-#pragma unroll
-  for (int l = 0; l < LIMBS; ++l) *reinterpret_cast<uint2*>(dst + l * 64) = make_uint2(limb[l][0], limb[l][1]);
-  if (LIMBS == 3) *reinterpret_cast<uint2*>(dst + 192) = make_uint2(0, 0);
-  if (v % kLanes == 0) {
-    GroupNote* note = reinterpret_cast<GroupNote*>(ws + I.notes) +
-                      (static_cast<int64_t>(v / kLanes) * I.tiles + tile) * 4 + row * Image::kCols / 2;
-#pragma unroll
-    for (int j = 0; j < Image::kCols / 2; ++j) {
-      GroupNote n;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int b = 2 * j + e < LIMBS ? sum[2 * j + e < LIMBS ? 2 * j + e : 0] : 0;
-        n.start[e] = kMagic - (L.asym ? 15 : 8) * b;
+      for (int l = 3; l >= 0; --l) {
+        const int up = l > 0 ? (i + 128) >> 8 : 0;   // what the next higher byte takes
+        const int b = i - up * 256;
+        limb[l][k >> 2] |= (static_cast<uint32_t>(b) & 0xFFu) << (8 * (k & 3));
+        sum[l] += b;
+        i = up;
       }
-      n.factor = peak < INFINITY ? exp2f(static_cast<float>(-a)) : NAN;
-      n.pad = 0;
-      note[j] = n;
+    }
+#pragma unroll
+    for (int o = 1; o < kLanes; o <<= 1)
+#pragma unroll
+      for (int l = 0; l < 4; ++l) sum[l] += __shfl_xor_sync(0xffffffffu, sum[l], o);
+    if (!in) return;
+    uint8_t* dst = ws + (static_cast<int64_t>(chunk) * I.tiles + tile) * Image::kChunk + (row * 16 + c) * 16 + step * 8;
+#pragma unroll
+    for (int l = 0; l < 4; ++l) *reinterpret_cast<uint2*>(dst + l * 64) = make_uint2(limb[l][0], limb[l][1]);
+    if (v % kLanes == 0) {
+      GroupNote* note = reinterpret_cast<GroupNote*>(ws + I.notes + (static_cast<int64_t>(v / kLanes) * I.tiles + tile) * Image::kNote) + row * 2;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+        note[j] = GroupNote{{kMagic - (L.asym ? 15 : 8) * sum[2 * j], kMagic - (L.asym ? 15 : 8) * sum[2 * j + 1]}, factor, 0};
     }
   }
 }
 
-template <int LIMBS, int GROUP>
+template <bool HALF, int GROUP>
 __global__ void __launch_bounds__(kPrepThreads) w4_prepare_kernel(const uint16_t* __restrict__ x, int64_t ld_x, int M,
                                                                   W4Layout L, uint8_t* __restrict__ ws) {
   asm volatile("griddepcontrol.launch_dependents;");
-  prepare_vector<LIMBS, GROUP>(x, ld_x, L, XImage<LIMBS>(L, M), blockIdx.y, blockIdx.x * kPrepThreads + threadIdx.x, ws);
+  prepare_vector<HALF, GROUP>(x, ld_x, L, XImage<HALF>(L, M), blockIdx.y, blockIdx.x * kPrepThreads + threadIdx.x, ws);
 }
 
 struct LinearArgs {
@@ -278,6 +322,9 @@ struct LinearArgs {
   int64_t ld_r;
   uint8_t* ws;
   unsigned int* err;
+  // 1024 twice in f16.  An argument, since the compiler makes two instructions of an AND and an OR with constants
+  // and one where one of them is in a register.
+  uint32_t f16_1024;
 };
 
 // One contiguous copy (16-byte aligned, a multiple of 16 bytes) into shared memory.
@@ -298,8 +345,8 @@ __device__ __noinline__ float plain_product(const LinearArgs& a, int64_t n, int 
   return sum;
 }
 
-// y = x . W^T for up to NT tiles of rows of x: the weights are operand A (16 rows by 32
-// columns), the image of x operand B.
+// y = x . W^T for up to NT tiles of rows of x: the weights are operand A (16 rows by 32 columns, or twice 16),
+// the image of x operand B.
 //
 // Work.  One CTA a SM.  A unit is TILES tiles of 16 rows of W, all fed by a load of the
 // image.  A CTA takes a run of units, and its warps equal runs of their blocks, laid end to
@@ -310,33 +357,35 @@ __device__ __noinline__ float plain_product(const LinearArgs& a, int64_t n, int 
 // on paper, 12.25 tiles a CTA for 13 at 28672 rows, and measured 14.2 us for 13.6.)
 //
 // Half a byte a weight leaves about 22 cycles of an SM for a tile's chunk, so instructions
-// count: 12 integer ones make the codes' fragments (8 AND, 4 shifts), two products do the
-// rest for four rows of x.  Zeros: sum v (u - 8) = sum v u - 8 sum v, the second part, and the
-// number that turns the integer into a float, being what a group's sums begin with; with stored
-// zeros the codes become u + (15 - z), 0..30, by one addition a register, and 15 takes the place of 8.
+// count.  Bytes: 12 integer ones make a chunk's fragments (8 AND, 4 shifts).  Zeros: sum v (u - 8) = sum v u - 8 sum v,
+// the second part, and the number that turns the integer into a float, being what a group's sums begin with; with
+// stored zeros the codes become u + (15 - z), 0..30, by one addition a register, and 15 takes the place of 8.
+// f16: a code in the low mantissa bits of 1024 is 1024 + u, four bits further up 1024 + 16 u; one f16 instruction
+// takes off the zero, exactly, so that a weight of 0 is 0 whatever x it meets.
 //
-// With up to two tiles of rows of x a warp reads the image and its notes into registers, one
-// chunk and one group ahead; with more they come by the ring (kRingX), since there are neither
-// the registers nor the warps to hide their latency (32 rows by 4096 x 4096: 19.2 us in registers, 13.4
-// by the ring).  As many warps as have the registers and two stages: with five tiles 11 warps take
-// 28.8 us for 19 rows by 4096 x 14336 in groups of 32 with zeros, 10 take 30.9.
+// Bytes, and one tile of f16, a warp reads with its notes into registers, one chunk and one group ahead; more tiles
+// come by the ring (kRingX), since there are neither the registers nor the warps to hide their latency.  As many warps
+// as have the registers and two stages: two tiles, 16 rows by 28672 x 4096, 10, 12 and 14 warps 30.1, 26.3 and 27.9 us;
+// four tiles, 32 rows by 4096 x 4096, 6 and 8 warps 13.4 and 12.5; three tiles, 24 rows, 8 and 11 warps 10.6 either way.
 //
-// Measured, back to back, with the preparation: one row by 28672 x 4096 13.3 us (4.5 TB/s of packed
-// weights), by 4096 x 4096 5.8, 16 rows by 4096 x 4096 9.1, 32 rows 13.4.  One row is bound by the
-// copies and the launch; many rows by the integers' way to floats, four instructions for two rows of W by a row
-// of x and group, beside the 8 cycles of a matrix instruction.
-__host__ __device__ constexpr int linear_warps(int nt) { return nt <= 2 ? 16 : nt <= 4 ? 12 : nt <= 5 ? 11 : 7; }
+// Measured, in a graph whose calls use different weights (more than L2 holds together): one row by 28672 x 4096 14.8 us,
+// 4.1 TB/s of packed weights, by 4096 x 4096 6.7; 8 rows by 4096 x 4096 7.3, 16 rows 9.1, 32 rows 12.5; 19 rows by
+// 4096 x 14336 in groups of 32 with zeros 23.7.  One row is bound by the copies and the launch; many rows by the
+// codes' way to f16 and the latency of the image, which each warp copies for itself.
+__host__ __device__ constexpr int linear_warps(bool half, int nt) { return !half || nt == 1 ? 16 : nt == 2 ? 12 : nt == 3 ? 11 : 8; }
 
-template <int NT, int TILES, bool ASYM, int GROUP>   // the same for both numbers of bytes
+template <bool HALF, int NT, int TILES, bool ASYM, int GROUP>
 struct LinearSmem {
-  static constexpr int kWarps = linear_warps(NT);
-  static constexpr bool kRingX = NT > 2;
+  using Image = XImage<HALF>;
+  static constexpr int kWarps = linear_warps(HALF, NT);
+  static constexpr bool kRingX = HALF && NT > 1;
   static constexpr int kRecord = 1024 + 128 / GROUP * 32 * (ASYM ? 2 : 1);
   static constexpr int kBlocks = TILES == 1 ? 2 : 1;           // of a stage: with one tile they lie side by side
   static constexpr int kImage = kBlocks * TILES * kRecord;     // where a stage's part of the image begins,
-  static constexpr int kNotes = kImage + (kRingX ? NT * 1024 : 0);   // and its notes
-  static constexpr int kStage = kNotes + (kRingX ? 128 / GROUP * NT * 64 : 0);
-  static constexpr int kPart = TILES * NT * 2 * 32;            // floats of a part of a unit
+  static constexpr int kNotes = kImage + (kRingX ? NT * 2 * Image::kChunk : 0);   // and its notes
+  static constexpr int kStage = kNotes + (kRingX ? NT * Image::kNote : 0);
+  static constexpr int kSums = HALF ? 4 : 2;                   // of a lane, tile of W and tile of x
+  static constexpr int kPart = TILES * NT * kSums * 32;        // floats of a part of a unit
   static constexpr int kFit = (227 * 1024 / kWarps - kPart * 4 - 32) / kStage;
   static constexpr int kStages = kFit < 4 ? kFit : 4;
   static_assert(kStages >= 2, "a warp needs two stages");
@@ -344,13 +393,14 @@ struct LinearSmem {
   static constexpr int kBytes = (kWarps * (kRing + kPart * 4 + kStages * 8) + 127) / 128 * 128;
 };
 
-template <int LIMBS, int NT, int TILES, bool ASYM, int GROUP, bool FUSED>
-__global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(const __grid_constant__ LinearArgs a) {
-  using Smem = LinearSmem<NT, TILES, ASYM, GROUP>;
-  constexpr int kWarps = Smem::kWarps, kRecord = Smem::kRecord, kPart = Smem::kPart, kStages = Smem::kStages;
+template <bool HALF, int NT, int TILES, bool ASYM, int GROUP, bool FUSED>
+__global__ void __launch_bounds__(32 * linear_warps(HALF, NT), 1) w4_linear_kernel(const __grid_constant__ LinearArgs a) {
+  using Smem = LinearSmem<HALF, NT, TILES, ASYM, GROUP>;
+  constexpr int kWarps = Smem::kWarps, kRecord = Smem::kRecord, kPart = Smem::kPart, kStages = Smem::kStages, kSums = Smem::kSums;
   constexpr bool kRingX = Smem::kRingX;
-  using Image = XImage<LIMBS>;
-  constexpr int kPer = 128 / GROUP, kSteps = GROUP / 32;        // groups of a block, k-steps of a group
+  using Image = XImage<HALF>;
+  constexpr int kPer = 128 / GROUP, kSteps = GROUP / 32;        // groups of a block, steps of 32 columns of a group
+  constexpr int kVecs = HALF ? 2 : 1;                           // 16-byte vectors of a lane, tile and chunk of the image
   constexpr int kLeast = 4;                                     // blocks: shorter runs cost more to join than to read
   extern __shared__ __align__(128) uint8_t smem[];
   float* parts = reinterpret_cast<float*>(smem + kWarps * Smem::kRing);   // [warp], of the unit that it goes on with
@@ -392,15 +442,14 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
       tc::mbar_arrive_expect_tx(bars + stage, n * TILES * kRecord + Smem::kStage - Smem::kImage);
       uint8_t* dst = ring + stage * Smem::kStage;
       if (kRingX) {
-        // of one block: its two chunks of the image, its groups' notes, NT tiles of each
+        // of one block: its two chunks of the image, NT tiles of each, and their notes
         const int first = blockIdx.y * NT, at_once = I.tiles == NT ? 1 : 0;
         for (int h = 0; h < 2; h += 1 + at_once)
-          copy_bulk(dst + Smem::kImage + h * NT * 512, a.ws + (static_cast<int64_t>(ld_piece * 2 + h) * I.tiles + first) * 512,
-                    NT * 512 << at_once, bars + stage);
-        for (int h = 0; h < kPer; h += at_once ? kPer : 1)
-          copy_bulk(dst + Smem::kNotes + h * NT * 64,
-                    a.ws + I.notes + (static_cast<int64_t>(ld_piece * kPer + h) * I.tiles + first) * 64,
-                    at_once ? kPer * NT * 64 : NT * 64, bars + stage);
+          copy_bulk(dst + Smem::kImage + h * NT * Image::kChunk,
+                    a.ws + (static_cast<int64_t>(ld_piece * 2 + h) * I.tiles + first) * Image::kChunk,
+                    NT * Image::kChunk << at_once, bars + stage);
+        copy_bulk(dst + Smem::kNotes, a.ws + I.notes + (static_cast<int64_t>(ld_piece) * I.tiles + first) * Image::kNote,
+                  NT * Image::kNote, bars + stage);
       }
       copy_bulk(dst, src, n * kRecord, bars + stage);
       if (TILES == 2)   // a tile past the last one repeats it: nothing of it is written
@@ -424,68 +473,98 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
     uint8_t* own = smem + Smem::kBytes;
     for (int m = 0; m < a.M; ++m)
       for (int v = 0; v < I.chunks * 8; v += 32 * kWarps)
-        prepare_vector<LIMBS, GROUP>(a.x, a.ld_x, L, I, m, v + threadIdx.x, own);
+        prepare_vector<HALF, GROUP>(a.x, a.ld_x, L, I, m, v + threadIdx.x, own);
     __syncthreads();
     img = own;
   }
-  // image and notes are read one chunk and one group ahead
-  const int image_chunk = I.tiles * 32, note_group = I.tiles * 4;   // strides, in elements
-  const uint4* image = reinterpret_cast<const uint4*>(img) + blockIdx.y * NT * 32 + lane;
-  const uint4* notes = reinterpret_cast<const uint4*>(img + I.notes) + blockIdx.y * NT * 4 + c;
-  auto load_image = [&](uint4 (&x)[NT], int chunk) {
+  // image and notes are read one chunk and one group (f16: one block) ahead
+  const int image_chunk = I.tiles * (Image::kChunk / 16), note_stride = I.tiles * Image::kNote;
+  const uint4* image = reinterpret_cast<const uint4*>(img) + blockIdx.y * NT * (Image::kChunk / 16) + lane;
+  const uint8_t* notes = img + I.notes + blockIdx.y * NT * Image::kNote + c * (Image::kNote / 4);
+  using Note = typename std::conditional<HALF, float2, uint4>::type;
+  auto load_image = [&](uint4 (&x)[NT][kVecs], int chunk) {
     const uint4* p = image + chunk * image_chunk;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) x[n] = p[n * 32];
-  };
-  auto load_note = [&](uint4 (&x)[NT], int group) {   // a GroupNote
-    const uint4* p = notes + group * note_group;
+    for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int n = 0; n < NT; ++n) x[n] = p[n * 4];
+      for (int j = 0; j < kVecs; ++j) x[n][j] = p[(n * kVecs + j) * 32];
   };
-  // a lane's two columns: the bytes of a row, or (three bytes) half of them
-  const float high = LIMBS == 2 ? 256.f : c & 1 ? 1.f : 65536.f, low = LIMBS == 2 ? 1.f : c & 1 ? 0.f : 256.f;
-  const float back = -12582912.f * (high + low);
+  auto load_note = [&](Note (&x)[NT], int at) {
+    const uint8_t* p = notes + static_cast<int64_t>(at) * note_stride;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) x[n] = *reinterpret_cast<const Note*>(p + n * Image::kNote);
+  };
+  // bytes: a lane's two columns are the high or the low half of a row's four
+  const float high = c & 1 ? 256.f : 16777216.f, low = c & 1 ? 1.f : 65536.f, back = -12582912.f * (high + low);
 
-  float acc[TILES][NT][2] = {};   // rows g, g + 8 of W by a row of a tile of x
-  int part[TILES][NT][4];
-  float sum[TILES][NT][2];        // of a block's groups
-  // k-step s, of group grp, of the record(s) at `rec`, with the image's chunk x and the group's note.
-  auto step = [&](const uint8_t* rec, int grp, int s, const uint4 (&x)[NT], const uint4 (&note)[NT]) {
+  float acc[TILES][NT][kSums] = {};   // rows g, g + 8 of W by a row (f16: two rows) of a tile of x
+  float sum[TILES][NT][kSums];        // of a block's groups
+  using Part = typename std::conditional<HALF, float, int>::type;
+  Part part[TILES][NT][4];
+  // Step s of 32 columns, of group grp, of the record(s) at `rec`, with the image's chunk x and (bytes) the group's note.
+  auto step = [&](const uint8_t* rec, int grp, int s, const uint4 (&x)[NT][kVecs], const Note (&note)[NT]) {
     const bool first = s % kSteps == 0, last = s % kSteps == kSteps - 1;
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
       const uint8_t* sc = rec + t * kRecord + 1024 + grp * 32 + g * 4;
       const uint2 w = *reinterpret_cast<const uint2*>(rec + t * kRecord + (s >> 1) * 512 + lane * 16 + (s & 1) * 8);
-      uint32_t f[4] = {w.x & 0x0F0F0F0Fu, (w.x >> 4) & 0x0F0F0F0Fu, w.y & 0x0F0F0F0Fu, (w.y >> 4) & 0x0F0F0F0Fu};
-      if (ASYM) {
-        const uint32_t z = *reinterpret_cast<const uint32_t*>(sc + kPer * 32);
-        const uint32_t z0 = __byte_perm(z, 0, 0x0000), z1 = __byte_perm(z, 0, 0x1111);
-        f[0] += z0, f[1] += z1, f[2] += z0, f[3] += z1;
-      }
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if (first) {
-          int2 start = make_int2(static_cast<int>(note[n].x), static_cast<int>(note[n].y));
-          if (kRingX) start = *reinterpret_cast<const int2*>(rec + Smem::kNotes + (grp * NT + n) * 64 + c * 16);
-          part[t][n][0] = part[t][n][2] = start.x;
-          part[t][n][1] = part[t][n][3] = start.y;
+      const uint32_t z = ASYM ? *reinterpret_cast<const uint32_t*>(sc + kPer * 32) : 0;   // 15 - zero of rows g, g + 8
+      if constexpr (HALF) {
+        // 1024 + zero and 1024 + 16 zero, twice each
+        uint32_t z0 = 0x64086408u, z1 = 0x64806480u;
+        if (ASYM) {
+          z0 = (__byte_perm(z, 0, 0x4040) ^ 0x000F000Fu) | 0x64006400u;
+          z1 = ((__byte_perm(z, 0, 0x4141) ^ 0x000F000Fu) << 4) | 0x64006400u;
         }
-        uint2 b = s & 1 ? make_uint2(x[n].z, x[n].w) : make_uint2(x[n].x, x[n].y);
-        if (kRingX)
-          b = *reinterpret_cast<const uint2*>(rec + Smem::kImage + ((s >> 1) * NT + n) * 512 + lane * 16 + (s & 1) * 8);
-        mma_u8s8(part[t][n], f, b.x, b.y);
+        const uint32_t words[2] = {w.x, w.y};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t lo = words[h], hi = words[h] >> 8;
+          const uint32_t f[4] = {sub_f16x2((lo & 0x000F000Fu) | a.f16_1024, z0), sub_f16x2((lo & 0x00F000F0u) | a.f16_1024, z1),
+                                 sub_f16x2((hi & 0x000F000Fu) | a.f16_1024, z0), sub_f16x2((hi & 0x00F000F0u) | a.f16_1024, z1)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            uint4 b = x[n][kRingX ? 0 : s & 1];
+            if (kRingX)
+              b = *reinterpret_cast<const uint4*>(rec + Smem::kImage + ((s >> 1) * NT + n) * Image::kChunk + (s & 1) * 512 + lane * 16);
+            if (first && h == 0)
+              mma_f16_zero(part[t][n], f, b.x, b.y);
+            else
+              mma_f16(part[t][n], f, h ? b.z : b.x, h ? b.w : b.y);
+          }
+        }
+      } else {
+        uint32_t f[4] = {w.x & 0x0F0F0F0Fu, (w.x >> 4) & 0x0F0F0F0Fu, w.y & 0x0F0F0F0Fu, (w.y >> 4) & 0x0F0F0F0Fu};
+        if (ASYM) {
+          const uint32_t z0 = __byte_perm(z, 0, 0x0000), z1 = __byte_perm(z, 0, 0x1111);
+          f[0] += z0, f[1] += z1, f[2] += z0, f[3] += z1;
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          if (first) {
+            part[t][n][0] = part[t][n][2] = static_cast<int>(note[n].x);
+            part[t][n][1] = part[t][n][3] = static_cast<int>(note[n].y);
+          }
+          if (s & 1)
+            mma_u8s8(part[t][n], f, x[n][0].z, x[n][0].w);
+          else
+            mma_u8s8(part[t][n], f, x[n][0].x, x[n][0].y);
+        }
       }
       if (last) {
         const uint32_t two = *reinterpret_cast<const uint32_t*>(sc);
-        const float w[2] = {bf16_lo(two), bf16_hi(two)};
+        const float w2[2] = {bf16_lo(two), HALF ? bf16_hi(two) * 0.0625f : bf16_hi(two)};
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            // high h + low l of the floats 1.5 2^23 + h and + l: the first product and its constant are
-            // multiples of `high`, and exact
-            const float v = fmaf(__int_as_float(part[t][n][2 * q + 1]), low, fmaf(__int_as_float(part[t][n][2 * q]), high, back));
-            sum[t][n][q] = fmaf(v, w[q], sum[t][n][q]);
+          for (int q = 0; q < kSums; ++q) {
+            float v;
+            if constexpr (HALF)
+              v = part[t][n][q];
+            else   // high h + low l of the floats 1.5 2^23 + h and + l: the first product and its constant are
+                   // multiples of `high`, and exact
+              v = fmaf(__int_as_float(part[t][n][2 * q + 1]), low, fmaf(__int_as_float(part[t][n][2 * q]), high, back));
+            sum[t][n][q] = fmaf(v, w2[q / (kSums / 2)], sum[t][n][q]);
           }
       }
     }
@@ -494,52 +573,61 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) sum[t][n][0] = sum[t][n][1] = 0.f;
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int q = 0; q < kSums; ++q) sum[t][n][q] = 0.f;
   };
   // the row's 2^-a belongs to the block: its groups' sums meet it together
-  auto end_block = [&](const uint8_t* rec, const uint4 (&note)[NT]) {
+  auto end_block = [&](const uint8_t* rec, const Note (&note)[NT]) {
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      float factor = __uint_as_float(note[n].z);
-      if (kRingX) factor = *reinterpret_cast<const float*>(rec + Smem::kNotes + n * 64 + c * 16 + 8);
+      float factor[2];
+      if constexpr (HALF) {
+        float2 two = note[n];
+        if (kRingX) two = *reinterpret_cast<const float2*>(rec + Smem::kNotes + n * Image::kNote + c * 8);
+        factor[0] = two.x, factor[1] = two.y;
+      } else {
+        factor[0] = factor[1] = __uint_as_float(note[n].z);
+      }
 #pragma unroll
       for (int t = 0; t < TILES; ++t)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          acc[t][n][q] = fmaf(sum[t][n][q], factor, acc[t][n][q]);
-        }
+        for (int q = 0; q < kSums; ++q) acc[t][n][q] = fmaf(sum[t][n][q], factor[q & 1], acc[t][n][q]);
     }
   };
+  // Sum q of a lane: row g (+ 8) of W by row `col` of a tile of x.
+  auto row_of = [](int q) { return q / (kSums / 2) * 8; };
+  auto col_of = [&](int q) { return HALF ? 2 * c + (q & 1) : c >> 1; };
   auto write = [&](int u) {
-    const int m0 = static_cast<int>(blockIdx.y) * NT * Image::kRows + c * Image::kRows / 4;
+    const int m0 = static_cast<int>(blockIdx.y) * NT * Image::kRows;
     const int64_t row0 = static_cast<int64_t>(u) * TILES * 16 + g;
-    float resid[NT][TILES][2];   // all on their way before the first store, which may be to the same place
+    float resid[NT][TILES][kSums];   // all on their way before the first store, which may be to the same place
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int t = 0; t < TILES; ++t)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int m = m0 + n * Image::kRows;
-          const int64_t row = row0 + t * 16 + 8 * q;
+        for (int q = 0; q < kSums; ++q) {
+          const int m = m0 + n * Image::kRows + col_of(q);
+          const int64_t row = row0 + t * 16 + row_of(q);
           resid[n][t][q] = a.resid && m < a.M && row < L.N ? bf16_bits_to_f32(a.resid[m * a.ld_r + row]) : 0.f;
         }
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int m = m0 + n * Image::kRows;
-      if (LIMBS == 3) {
+      if (!HALF) {
 #pragma unroll
         for (int t = 0; t < TILES; ++t)
 #pragma unroll
-          for (int q = 0; q < 2; ++q) acc[t][n][q] += __shfl_xor_sync(0xffffffffu, acc[t][n][q], 1);   // the other bytes' lane
+          for (int q = 0; q < kSums; ++q) acc[t][n][q] += __shfl_xor_sync(0xffffffffu, acc[t][n][q], 1);   // the other bytes' lane
+        if (c & 1) continue;
       }
-      if (m >= a.M || (LIMBS == 3 && (c & 1))) continue;
 #pragma unroll
       for (int t = 0; t < TILES; ++t)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const int64_t row = row0 + t * 16 + 8 * q;
-          if (row >= L.N) continue;
+        for (int q = 0; q < kSums; ++q) {
+          const int m = m0 + n * Image::kRows + col_of(q);
+          const int64_t row = row0 + t * 16 + row_of(q);
+          if (m >= a.M || row >= L.N) continue;
           const float v = acc[t][n][q];
           const float y = (fabsf(v) < INFINITY ? v : plain_product(a, row, m)) + resid[n][t][q];
           if (a.y_bf16)
@@ -554,7 +642,9 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
 #pragma unroll
     for (int t = 0; t < TILES; ++t)
 #pragma unroll
-      for (int n = 0; n < NT; ++n) acc[t][n][0] = acc[t][n][1] = 0.f;
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int q = 0; q < kSums; ++q) acc[t][n][q] = 0.f;
   };
   auto leave = [&]() {
 #pragma unroll
@@ -562,7 +652,7 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) mine[((t * NT + n) * 2 + q) * 32] = acc[t][n][q];
+        for (int q = 0; q < kSums; ++q) mine[((t * NT + n) * kSums + q) * 32] = acc[t][n][q];
     clear();
   };
 
@@ -571,10 +661,12 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
   bool lost = false;         // a copy did not arrive in time
   int stage = 0, left = count;
   uint32_t phase = 0;
-  uint4 x0[NT], x1[NT], note[2][NT];
+  uint4 x0[NT][kVecs], x1[NT][kVecs];
+  Note note[2][NT];
+  constexpr int kNotesPer = HALF ? 1 : kPer;   // of a block
   if (!kRingX && count > 0) {
     load_image(x0, piece * 2);
-    load_note(note[0], piece * kPer);
+    load_note(note[0], piece * kNotesPer);
   }
 #pragma unroll 1
   while (left > 0) {
@@ -598,17 +690,15 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
       } else {
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          // note[..] of group i of the block: with one group a block they change places from block to block
-          const int i = s / kSteps, at = kPer == 1 ? b & 1 : i & 1;
-          if (s % kSteps == 0) load_note(note[at ^ 1], i + 1 < kPer ? piece * kPer + i + 1 : after * kPer);
+          // note[..] of group i of the block: with one note a block they change places from block to block
+          const int i = s / kSteps, k = kNotesPer == 1 ? 0 : i, at = kNotesPer == 1 ? b & 1 : i & 1;
+          if (kNotesPer == 1 ? s == 0 : s % kSteps == 0)
+            load_note(note[at ^ 1], k + 1 < kNotesPer ? piece * kNotesPer + k + 1 : after * kNotesPer);
           step(rec, i, s, s < 2 ? x0 : x1, note[at]);
           if (s == 1) load_image(x0, after * 2);
           if (s == 3) end_block(rec, note[at]);
         }
-        if (kPer == 1 && Smem::kBlocks == 1) {
-#pragma unroll
-          for (int n = 0; n < NT; ++n) note[0][n] = note[1][n];
-        }
+        static_assert(kNotesPer > 1 || Smem::kBlocks == 2, "notes change places from block to block");
       }
       --left;
       piece = after;
@@ -650,7 +740,7 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int q = 0; q < 2; ++q) acc[t][n][q] += from[((t * NT + n) * 2 + q) * 32];
+          for (int q = 0; q < kSums; ++q) acc[t][n][q] += from[((t * NT + n) * kSums + q) * 32];
     };
 #pragma unroll 4
     for (int w = warp + 1; w < warps && begin_of(w) < unit_end; ++w)
@@ -659,15 +749,15 @@ __global__ void __launch_bounds__(32 * linear_warps(NT), 1) w4_linear_kernel(con
   }
 }
 
-template <int LIMBS, int NT, int TILES, bool ASYM, int GROUP, bool FUSED>
-int launch_linear_one(const LinearArgs& a, const XImage<LIMBS>& I, cudaStream_t st) {
-  const auto kernel = w4_linear_kernel<LIMBS, NT, TILES, ASYM, GROUP, FUSED>;
-  const int bytes = LinearSmem<NT, TILES, ASYM, GROUP>::kBytes + (FUSED ? static_cast<int>(I.bytes) : 0);
+template <bool HALF, int NT, int TILES, bool ASYM, int GROUP, bool FUSED>
+int launch_linear_one(const LinearArgs& a, const XImage<HALF>& I, cudaStream_t st) {
+  const auto kernel = w4_linear_kernel<HALF, NT, TILES, ASYM, GROUP, FUSED>;
+  const int bytes = LinearSmem<HALF, NT, TILES, ASYM, GROUP>::kBytes + (FUSED ? static_cast<int>(I.bytes) : 0);
   GLT_TRY(ensure_smem_attr(reinterpret_cast<const void*>(kernel), bytes));
   const int units = (a.L.tiles + TILES - 1) / TILES;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(units < num_sms() ? units : num_sms(), I.tiles / NT);
-  cfg.blockDim = dim3(32 * linear_warps(NT));
+  cfg.blockDim = dim3(32 * linear_warps(HALF, NT));
   cfg.dynamicSmemBytes = bytes;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
@@ -680,39 +770,36 @@ int launch_linear_one(const LinearArgs& a, const XImage<LIMBS>& I, cudaStream_t 
   return GLT_OK;
 }
 
-template <int LIMBS, int NT, int TILES, bool ASYM, int GROUP>
+template <bool HALF, int NT, int TILES, bool ASYM, int GROUP>
 int launch_linear(const LinearArgs& a, cudaStream_t st) {
-  const XImage<LIMBS> I(a.L, a.M);
+  const XImage<HALF> I(a.L, a.M);
   if (I.tiles / NT > 65535 || a.M > 65535) return fail(GLT_EINVAL, "w4: %d rows (at most 65535)", a.M);
   // A small x is turned into its image by every CTA for itself: one launch less, but 1.5 us more for each
   // 16384 elements than reading the image that a launch before made.
   if constexpr (NT == 1)
-    if (static_cast<int64_t>(a.M) * a.L.K <= 16384 && LinearSmem<NT, TILES, ASYM, GROUP>::kBytes + I.bytes <= 227 * 1024)
-      return launch_linear_one<LIMBS, NT, TILES, ASYM, GROUP, true>(a, I, st);
-  w4_prepare_kernel<LIMBS, GROUP><<<dim3((I.chunks * 8 + kPrepThreads - 1) / kPrepThreads, a.M), kPrepThreads, 0, st>>>(a.x, a.ld_x, a.M, a.L, a.ws);
+    if (static_cast<int64_t>(a.M) * a.L.K <= 16384 && LinearSmem<HALF, NT, TILES, ASYM, GROUP>::kBytes + I.bytes <= 227 * 1024)
+      return launch_linear_one<HALF, NT, TILES, ASYM, GROUP, true>(a, I, st);
+  w4_prepare_kernel<HALF, GROUP><<<dim3((I.chunks * 8 + kPrepThreads - 1) / kPrepThreads, a.M), kPrepThreads, 0, st>>>(a.x, a.ld_x, a.M, a.L, a.ws);
   GLT_LAUNCH_CHECK();
-  return launch_linear_one<LIMBS, NT, TILES, ASYM, GROUP, false>(a, I, st);
+  return launch_linear_one<HALF, NT, TILES, ASYM, GROUP, false>(a, I, st);
 }
 
-template <int LIMBS, int NT, int TILES>
+template <bool HALF, int NT, int TILES>
 int launch_linear_as(const LinearArgs& a, cudaStream_t st) {
   if (a.L.asym) {
-    if (a.L.group == 32) return launch_linear<LIMBS, NT, TILES, true, 32>(a, st);
-    return a.L.group == 64 ? launch_linear<LIMBS, NT, TILES, true, 64>(a, st) : launch_linear<LIMBS, NT, TILES, true, 128>(a, st);
+    if (a.L.group == 32) return launch_linear<HALF, NT, TILES, true, 32>(a, st);
+    return a.L.group == 64 ? launch_linear<HALF, NT, TILES, true, 64>(a, st) : launch_linear<HALF, NT, TILES, true, 128>(a, st);
   }
-  if (a.L.group == 32) return launch_linear<LIMBS, NT, TILES, false, 32>(a, st);
-  return a.L.group == 64 ? launch_linear<LIMBS, NT, TILES, false, 64>(a, st) : launch_linear<LIMBS, NT, TILES, false, 128>(a, st);
+  if (a.L.group == 32) return launch_linear<HALF, NT, TILES, false, 32>(a, st);
+  return a.L.group == 64 ? launch_linear<HALF, NT, TILES, false, 64>(a, st) : launch_linear<HALF, NT, TILES, false, 128>(a, st);
 }
 
-template <int LIMBS>
 int launch_rows(const LinearArgs& a, cudaStream_t st) {
-  const int n = XImage<LIMBS>(a.L, a.M).per_cta;
-  if (n == 1) return launch_linear_as<LIMBS, 1, 1>(a, st);
-  if (n == 2) return launch_linear_as<LIMBS, 2, 1>(a, st);
-  if (n == 3) return launch_linear_as<LIMBS, 3, 2>(a, st);
-  if (n == 4) return launch_linear_as<LIMBS, 4, 2>(a, st);
-  if (n == 5) return launch_linear_as<LIMBS, 5, 2>(a, st);
-  return launch_linear_as<LIMBS, 8, 2>(a, st);
+  if (!half_image(a.L, a.M)) return a.M <= 2 ? launch_linear_as<false, 1, 1>(a, st) : launch_linear_as<false, 2, 1>(a, st);
+  const int n = XImage<true>(a.L, a.M).per_cta;
+  if (n == 1) return launch_linear_as<true, 1, 1>(a, st);
+  if (n == 2) return launch_linear_as<true, 2, 2>(a, st);
+  return n == 3 ? launch_linear_as<true, 3, 2>(a, st) : launch_linear_as<true, 4, 2>(a, st);
 }
 
 int grid_for(int64_t units, int per_cta) {
@@ -774,7 +861,7 @@ extern "C" int glt_w4_linear_workspace(int M, int N, int K, int group, int y_dty
   if (M < 0) return glt::fail(GLT_EINVAL, "w4: negative rows");
   if (y_dtype != 0 && y_dtype != 1) return glt::fail(GLT_EINVAL, "w4: output type %d (0 fp32, 1 bf16)", y_dtype);
   const W4Layout L(N, K, group, 0);
-  *bytes = M == 0 ? 0 : y_dtype ? glt::XImage<2>(L, M).bytes : glt::XImage<3>(L, M).bytes;
+  *bytes = M == 0 ? 0 : glt::image_bytes(L, M);
   return GLT_OK;
 }
 
@@ -792,12 +879,12 @@ extern "C" int glt_w4_linear(const void* packed, int N, int K, int group, int as
   if (!glt::aligned16(packed)) return glt::fail(GLT_EINVAL, "w4: packed weights must be 16-byte aligned");
   if (M == 0) return GLT_OK;
   const W4Layout L(N, K, group, asym);
-  const int64_t need = y_dtype ? glt::XImage<2>(L, M).bytes : glt::XImage<3>(L, M).bytes;
+  const int64_t need = glt::image_bytes(L, M);
   if (workspace_bytes < need || !workspace || !glt::aligned16(workspace))
     return glt::fail(GLT_EINVAL, "w4: workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
   if (need / 4 > INT_MAX) return glt::fail(GLT_EINVAL, "w4: %d rows of %d columns", M, K);
   const glt::LinearArgs a{static_cast<const uint8_t*>(packed), L, x, ld_x, M, y, ld_y, y_dtype, resid, ld_r,
-                          static_cast<uint8_t*>(workspace), glt::device_error_word()};
+                          static_cast<uint8_t*>(workspace), glt::device_error_word(), 0x64006400u};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return y_dtype ? glt::launch_rows<2>(a, st) : glt::launch_rows<3>(a, st);
+  return glt::launch_rows(a, st);
 }

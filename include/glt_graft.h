@@ -326,9 +326,9 @@ GLT_API int glt_kv8_read(const GltKv8Cache* cache, const GltKv8Batch* batch, con
  * glt_w4_linear: y[M, N] = x[M, K] . W^T (+ resid): x bf16 with row stride ld_x
  *   (a multiple of 8, 16-byte aligned), y bf16 (y_dtype 1) or fp32 (0), resid bf16
  *   or NULL.  Made for the few rows of decoding: every 32 rows read the weights
- *   once more (every 16 for fp32).  Sums of a group are exact integers, of groups fp32;
- *   of an element of x, what lies below 2^-16 (fp32 results: 2^-24) of the largest
- *   of its 128 columns is rounded off.  At most 65535 rows.  workspace: at least glt_w4_linear_workspace bytes,
+ *   once more.  Weights are exact, sums are in 32 bits (a group's in integers or fp32), and an element of x
+ *   is exact down to 2^-22 of the largest magnitude of its 128 columns: what lies below 2^-30 of that is
+ *   rounded off.  At most 65535 rows.  workspace: at least glt_w4_linear_workspace bytes,
  *   16-byte aligned, used by one call at a time; its contents do not matter. */
 GLT_API int glt_w4_packed_bytes(int N, int K, int group, int asym, int64_t* bytes);
 GLT_API int glt_w4_quantize(const uint16_t* w, int64_t ld_w, int N, int K, int group, int asym,
