@@ -353,6 +353,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
   Cursor<ROWS> ld;
   ld.start(a, scan.run);
   int ld_step = ld.s0 + warp, ld_stage = 0, ld_id[LU];
+  bool ld_on[LU];   // some query may see tokens of it
   auto seek = [&]() {
     while (ld.left > 0 && ld_step >= ld.s1) {
       ld.next(a);
@@ -361,15 +362,18 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
     if (ld.left > 0) {
       const int t = ld.w.lo + ld_step * kStep;
       const int32_t* ids = a.b.block_table + static_cast<int64_t>(ld.seq) * a.b.max_blocks;
-      ld_id[0] = ids[t >> bt_log];
-      if (LU == 2) ld_id[LU - 1] = t + 16 < ld.w.past + ld.w.n ? ids[(t + 16) >> bt_log] : -1;
+      // of a step's two blocks of 16 the first may lie before the window, and the last beyond the tokens
+      ld_on[0] = LU == 1 || a.window == 0 || t + 15 > ld.w.past - a.window;
+      if (LU == 2) ld_on[LU - 1] = t + 16 < ld.w.past + ld.w.n;
+#pragma unroll
+      for (int f = 0; f < LU; ++f) ld_id[f] = ld_on[f] ? ids[(t + 16 * f) >> bt_log] : -1;
     }
   };
   // Copies this warp's next step into the next stage.
   int issued = 0;
   auto issue = [&]() {
     if (ld.left > 0) {
-      const int t0 = ld.w.lo + ld_step * kStep, held = ld.w.past + ld.w.n - t0;   // tokens from t0 on
+      const int t0 = ld.w.lo + ld_step * kStep;
       uint64_t* bar = bars + ld_stage;
       uint8_t* dst = ring + ld_stage * R::kStage;
       int valid = 0;
@@ -377,7 +381,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
       for (int f = 0; f < LU; ++f) {
         const bool on = ld_id[f] >= 0 && ld_id[f] < a.c.num_blocks;
         if (on) valid |= LU == 2 ? 1 << f : 3;
-        if (!on && held > 16 * f && lane == 0 && a.err) atomicOr(a.err, GLT_DEVERR_BAD_SHAPE);
+        if (!on && ld_on[f] && lane == 0 && a.err) atomicOr(a.err, GLT_DEVERR_BAD_SHAPE);
         const int64_t hb = on ? static_cast<int64_t>(ld_id[f]) * a.c.num_kv_heads + ld.kvh : 0;
         if (lane < 2) copy_async4(notes[ld_stage].scale + f * 2 + lane, (lane ? a.c.v_scale : a.c.k_scale) + hb, on);
       }
@@ -502,6 +506,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
     }
     const int pos_lo = cu.w.past + tile * ROWS / a.group;
     const int pos_hi = cu.w.past + (tile * ROWS + rows - 1) / a.group;
+    const int before = a.window > 0 ? pos_lo - a.window : -1;   // the last token before every query's window
     float acc[HD / 16][NT][4], m[NT][2], l[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -569,7 +574,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int t = t0 + 8 * i + g;
-          const bool on = (valid >> (i >> 1) & 1) && (seen >> (8 * i + g) & 1) && t <= pos_hi;
+          // a query of the tile sees it
+          const bool on = (valid >> (i >> 1) & 1) && (seen >> (8 * i + g) & 1) && t <= pos_hi && t > before;
           if (FMT == GLT_KV8_E4M3) live[i] = __ballot_sync(0xffffffffu, on);   // bit 4g: token 8 i + g
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -641,7 +647,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
               small |= p < kF16Min && p > 0.f;
             }
             l[nt][j] = fmaf(sum, w, l[nt][j]);
-            fold[f][nt][j] = w * (f ? sc.w : sc.y);
+            // a unit that the row sees nothing of may have any scale
+            fold[f][nt][j] = peak[f][nt][j] == -INFINITY ? 0.f : w * (f ? sc.w : sc.y);
           }
       if (__any_sync(0xffffffffu, small)) {
 #pragma unroll 1

@@ -297,7 +297,9 @@ GLT_API int glt_kv8_append(const GltKv8Cache* cache, const GltKv8Batch* batch, c
  * and, if token_mask is given (dev bytes, row b at b * ld_mask, one byte a
  * position), a nonzero byte.  scale = 0 means 1/sqrt(head_dim).  lse (NULL or
  * [rows, num_heads] fp32): natural log-sum-exp of the scaled scores.  A query
- * that sees no token gets o = 0, lse = -inf.  workspace: at least
+ * that sees no token gets o = 0, lse = -inf.  What no query sees may hold anything, scales and codes
+ * that are NaN among it; table entries of blocks wholly before the window of a
+ * sequence's first query are not looked at.  workspace: at least
  * glt_kv8_attention_workspace bytes, 16-byte aligned, used by one call at a
  * time; its contents do not matter. */
 GLT_API int glt_kv8_attention_workspace(const GltKv8Cache* cache, const GltKv8Batch* batch,
