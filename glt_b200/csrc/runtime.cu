@@ -43,6 +43,9 @@ static std::atomic<unsigned long long> g_launches{0};
 
 void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 
+// Each device's copy comes, zeroed, with the library's code: a device's first call allocates nothing and may be captured.
+__device__ unsigned int g_error_word;
+
 unsigned int* device_error_word() {
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return nullptr;
@@ -50,11 +53,9 @@ unsigned int* device_error_word() {
   std::lock_guard<std::mutex> lk(g_mu);
   auto it = words.find(dev);
   if (it != words.end()) return it->second;
-  unsigned int* p = nullptr;
-  if (cudaMalloc(&p, sizeof(unsigned int)) != cudaSuccess) return nullptr;
-  if (cudaMemset(p, 0, sizeof(unsigned int)) != cudaSuccess) return nullptr;
-  words[dev] = p;
-  return p;
+  void* p = nullptr;
+  if (cudaGetSymbolAddress(&p, g_error_word) != cudaSuccess) return nullptr;
+  return words[dev] = static_cast<unsigned int*>(p);
 }
 
 int num_sms() {
