@@ -70,7 +70,9 @@ __global__ void __launch_bounds__(256) w4_quantize_kernel(const uint16_t* __rest
     }
     lo = -warp_max(-lo);
     hi = warp_max(hi);
-    const uint16_t sb = bf16_bits_rn(asym ? (hi - lo) / 15.f : fmaxf(hi, -lo) / 7.f);
+    float step = asym ? (hi - lo) / 15.f : fmaxf(hi, -lo) / 7.f;
+    if (!(step < INFINITY)) step = hi / 15.f - lo / 15.f;   // the range is beyond a float, a step of it is not
+    const uint16_t sb = bf16_bits_rn(step);
     const float s = bf16_bits_to_f32(sb);
     const float z = !asym ? 8.f : s > 0.f ? fminf(fmaxf(rintf(-lo / s), 0.f), 15.f) : 0.f;
     if (lane == 0) {
