@@ -11,6 +11,13 @@ namespace glt {
 // Host checks shared by every call on a cache.
 int kv8_check(const GltKv8Cache* c, const GltKv8Batch* b);
 
+// The most new rows a sequence can bring: max_new is the caller's bound, and may say less than the others.
+inline int kv8_most_new(const GltKv8Cache& c, const GltKv8Batch& b) {
+  const int64_t room = static_cast<int64_t>(b.max_blocks) * c.block_tokens;
+  const int most = b.max_new < b.rows ? b.max_new : b.rows;
+  return most < room ? most : static_cast<int>(room);
+}
+
 // Where sequence b stands in this step: `past` tokens held before it, new rows
 // [row0, row0 + n).  n = 0 for a sequence without new rows and for one that
 // does not fit the batch's bounds (which also sets the device error word when

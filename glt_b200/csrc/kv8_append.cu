@@ -231,7 +231,7 @@ template <int FMT>
 int launch_append(const GltKv8Cache& c, const GltKv8Batch& b, const uint16_t* k, int64_t ld_k, const uint16_t* v,
                   int64_t ld_v, cudaStream_t st) {
   // blocks a sequence's new tokens can reach into, the first one partly filled
-  const dim3 grid((b.max_new + c.block_tokens - 2) / c.block_tokens + 1, b.num_seqs, 2 * c.num_kv_heads);
+  const dim3 grid((kv8_most_new(c, b) + c.block_tokens - 2) / c.block_tokens + 1, b.num_seqs, 2 * c.num_kv_heads);
   const int vecs = c.block_tokens * c.head_dim / 8;
   const auto kernel = vecs <= kThreads ? kv8_append_kernel<FMT, 1> : vecs <= 2 * kThreads ? kv8_append_kernel<FMT, 2>
                       : vecs <= 4 * kThreads ? kv8_append_kernel<FMT, 4> : kv8_append_kernel<FMT, 8>;

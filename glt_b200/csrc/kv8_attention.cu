@@ -923,8 +923,8 @@ int check_heads(const GltKv8Cache* c, const GltKv8Batch* b, int nh) {
   GLT_TRY(kv8_check(c, b));
   if (nh < 1 || nh % c->num_kv_heads || nh > 65535)
     return fail(GLT_EINVAL, "kv8: num_heads %d must be a multiple of num_kv_heads %d", nh, c->num_kv_heads);
-  if (static_cast<int64_t>(b->max_new) * nh > INT_MAX / 2)
-    return fail(GLT_EINVAL, "kv8: max_new %d with %d heads", b->max_new, nh);
+  if (static_cast<int64_t>(kv8_most_new(*c, *b)) * nh > INT_MAX / 2)
+    return fail(GLT_EINVAL, "kv8: %d new rows of a sequence with %d heads", kv8_most_new(*c, *b), nh);
   return GLT_OK;
 }
 
@@ -937,7 +937,7 @@ struct Plan {
 };
 Plan plan(const GltKv8Cache& c, const GltKv8Batch& b, int nh) {
   Plan p;
-  const int64_t rows = static_cast<int64_t>(b.max_new) * (nh / c.num_kv_heads);
+  const int64_t rows = static_cast<int64_t>(kv8_most_new(c, b)) * (nh / c.num_kv_heads);
   p.nt = rows <= 8 ? 1 : 2;
   // no more CTAs than the fullest cache could feed
   const int64_t tiles = (rows + 8 * p.nt - 1) / (8 * p.nt);
