@@ -776,9 +776,10 @@ template <bool HALF, int NT, int TILES, bool ASYM, int GROUP>
 int launch_linear(const LinearArgs& a, cudaStream_t st) {
   const XImage<HALF> I(a.L, a.M);
   if (I.tiles / NT > 65535 || a.M > 65535) return fail(GLT_EINVAL, "w4: %d rows (at most 65535)", a.M);
-  // A small x is turned into its image by every CTA for itself: one launch less, but 1.5 us more for each
-  // 16384 elements than reading the image that a launch before made.
-  if constexpr (NT == 1)
+  // A small x of one tile is turned into its bytes by every CTA for itself: one launch less, 2.1 us of the host's time.
+  // On the device one row by 28672 x 4096 takes 14.5 us so and 15.6 with a launch before, by 896 x 4864 6.6 and 5.9;
+  // two rows by 896 x 4864 8.8 and 5.9.  Its f16 image takes longer to make (8 rows by 4864 x 896 10.1 us and 5.2).
+  if constexpr (!HALF && NT == 1)
     if (static_cast<int64_t>(a.M) * a.L.K <= 16384 && LinearSmem<HALF, NT, TILES, ASYM, GROUP>::kBytes + I.bytes <= 227 * 1024)
       return launch_linear_one<HALF, NT, TILES, ASYM, GROUP, true>(a, I, st);
   w4_prepare_kernel<HALF, GROUP><<<dim3((I.chunks * 8 + kPrepThreads - 1) / kPrepThreads, a.M), kPrepThreads, 0, st>>>(a.x, a.ld_x, a.M, a.L, a.ws);
