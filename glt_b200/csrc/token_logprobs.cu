@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) token_logprobs_kernel(
       if (bad) return NAN;
       if (empty) return -INFINITY;
       const float d = (x - all.m) * scale;
-      return (d > -INFINITY ? d : fmaf(x, scale, -(all.m * scale))) - ls;
+      return (d > -INFINITY || x == -INFINITY ? d : fmaf(x, scale, -(all.m * scale))) - ls;
     };
     if (lane == 0) {
       lse_out[r] = lse;

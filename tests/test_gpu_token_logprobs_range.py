@@ -105,3 +105,19 @@ def test_one_likely_token_has_probability_one(at, dtype):
 def test_confident_rows_keep_their_digits(at, step, V):
     for seed in range(4):
         compare(spread(5, V, at + seed * step, step, torch.float32, seed), 1.0 if seed % 2 else 0.77)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("scale", [0.5, 1.0, 3.0])
+def test_forbidden_tokens_below_a_very_low_maximum(dtype, scale):
+    """A logit of -inf has log probability -inf also where the maximum times the scale is beyond the float range."""
+    low = torch.finfo(dtype).min
+    x = torch.full((2, 700), -math.inf, device=DEV, dtype=dtype)
+    x[:, 5], x[1, 600] = low, low
+    for v, want in ((5, [0.0, -math.log(2)]), (3, [-math.inf] * 2), (600, [-math.inf, -math.log(2)])):
+        f = serve.token_logprobs(x, torch.full((2,), v, device=DEV, dtype=torch.int32), scale=scale, top=3)
+        want = torch.tensor(want, device=DEV)
+        assert torch.equal(torch.isinf(f.logp), torch.isinf(want)) and not torch.isnan(f.logp).any()
+        fin = torch.isfinite(want)
+        assert ((f.logp - want).abs()[fin] <= 2.0 ** -20).all()
+        assert (f.top_logp[0, 1:] == -math.inf).all() and (f.top_logp[1, 2] == -math.inf)
