@@ -76,9 +76,9 @@ class Decoder:
     def _lookup(self, ids: torch.Tensor) -> torch.Tensor:
         """Rows of the embedding for ids [seqs, n].  A sequence with an id outside the vocabulary gets NaN, which
         its logits and log probabilities show: the host does not wait to look at the ids."""
-        known = (ids >= 0) & (ids < self.embed.shape[0])
-        rows = self.embed[torch.where(known, ids, 0).flatten()]
-        return rows.masked_fill_(~known.all(1, keepdim=True).expand_as(ids).reshape(-1, 1), float("nan"))
+        held = ids.clamp(0, self.embed.shape[0] - 1)
+        unknown = (held != ids).any(1, keepdim=True).expand_as(ids).reshape(-1, 1)
+        return self.embed[held.flatten()].masked_fill_(unknown, float("nan"))
 
     def _norm(self, x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
         y, var = torch.empty_like(x), torch.empty(x.shape[0], device=x.device)
