@@ -30,9 +30,10 @@
 // that the fragment reads meet no bank twice, and the warp waits on the stage's mbarrier.
 // No warp waits for another inside a unit, and the copies run ahead across units.
 //
-// Measured (32 heads over 8, head_dim 128): 4 sequences of 65537 tokens e4m3 90.6 us, 5.9 TB/s of cache; 32 ragged
+// Measured (32 heads over 8, head_dim 128): 4 sequences of 65537 tokens e4m3 91.4 us, 5.9 TB/s of cache; 32 ragged
 // sequences of up to 8191 tokens int8 62 us, 5.0 TB/s, the ends of units being the difference.  Many query rows (5 new
-// tokens x 8 heads a KV head) are bound by the instructions and their latency: 37.5 us for 12 sequences, 0.85 TB/s.
+// tokens x 8 heads a KV head) are bound by the instructions and their latency: 39 us for 12 sequences, 0.8 TB/s; the
+// kernels for 16 query rows of 128 channels hold all 255 registers and spill 188 to 284 bytes a thread.
 #include <float.h>
 
 #include <type_traits>
@@ -929,7 +930,7 @@ int check_heads(const GltKv8Cache* c, const GltKv8Batch* b, int nh) {
 }
 
 // Row tiles of 8 fill the tensor core's N for up to 8 rows a KV head; more rows go 16 at a
-// time, which reads and decodes the cache half as often (40 rows: 44.6 us against 46.1, at the
+// time, which reads and decodes the cache half as often (40 rows, when measured: 44.6 us against 46.1, at the
 // price of 16 rows' sums, which leave no registers).
 struct Plan {
   int nt, grid;

@@ -13,8 +13,8 @@
 // on the special-function unit (16 a clock and SM, against the 12 bf16 logits that HBM
 // brings): sums run two at a time (f32x2), maxima and clamps in packed bf16.
 //
-// Measured: 4096 x 128256 bf16 170 us without the most likely tokens (6.2 TB/s), 185 with 5 of them; the gradient of
-// 2047 x 128257 173 us (6.1 TB/s read and written).
+// Measured: 4096 x 128256 bf16 170 us without the most likely tokens (6.2 TB/s), 188 with 5 of them; the gradient of
+// 2047 x 128257 176 us (6.0 TB/s read and written).
 //
 // A row belongs to one CTA; with fewer rows than would fill the SMs, to a cluster of up
 // to eight, joined over distributed shared memory.
@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) token_logprobs_kernel(
     }
   }
   // While this row's sums are joined, the two first batches of the row that one of the SM's CTAs takes
-  // next come to L2 (4096 x 128256 bf16: 188 us without, 186 with; 2047 with the gradient: 286 and 280).
+  // next come to L2 (4096 x 128256 bf16, when it was brought in: 188 us without, 185 with; 2047 with the gradient: 286 and 280).
   if (CLUSTER == 1 && threadIdx.x == 0 && r + ahead < gridDim.x) {
     const Row next(logits + (r + ahead) * ld, V);
     const int bytes = min(next.nv, 2 * kBatch * kThreads) * 16;

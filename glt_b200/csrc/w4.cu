@@ -370,7 +370,7 @@ __device__ __noinline__ float plain_product(const LinearArgs& a, int64_t n, int 
 // as have the registers and two stages: two tiles, 16 rows by 28672 x 4096, 10, 12 and 14 warps 30.1, 26.3 and 27.9 us;
 // four tiles, 32 rows by 4096 x 4096, 6 and 8 warps 13.4 and 12.5; three tiles, 24 rows, 8 and 11 warps 10.6 either way.
 //
-// Measured, in a graph whose calls use different weights (more than L2 holds together): one row by 28672 x 4096 14.8 us,
+// Measured, in a graph whose calls use different weights (more than L2 holds together): one row by 28672 x 4096 14.7 us,
 // 4.1 TB/s of packed weights, by 4096 x 4096 6.7; 8 rows by 4096 x 4096 7.3, 16 rows 9.1, 32 rows 12.5; 19 rows by
 // 4096 x 14336 in groups of 32 with zeros 23.7.  One row is bound by the copies and the launch; many rows by the
 // codes' way to f16 and the latency of the image, which each warp copies for itself.
