@@ -339,11 +339,12 @@ __device__ __forceinline__ void copy_bulk(void* dst, const void* src, int bytes,
 // One product the plain way, for rows of x that are not finite.
 __device__ __noinline__ float plain_product(const LinearArgs& a, int64_t n, int m) {
   float sum = 0.f;
-  for (int k = 0; k < a.L.K; ++k) {
-    float scale;
-    const float u = w4_code(a.packed, a.L, n, k, &scale);
-    sum = fmaf(bf16_bits_to_f32(a.x[m * a.ld_x + k]) * scale, u, sum);
-  }
+  for (int k0 = 0; k0 < a.L.K && sum == sum; k0 += 32)   // a sum that is NaN stays so; a group is 32 columns at least
+    for (int k = k0; k < k0 + 32; ++k) {
+      float scale;
+      const float u = w4_code(a.packed, a.L, n, k, &scale);
+      sum = fmaf(bf16_bits_to_f32(a.x[m * a.ld_x + k]) * scale, u, sum);
+    }
   return sum;
 }
 
