@@ -197,6 +197,11 @@ SIGNATURES: dict[str, tuple] = {
     "glt_w4_linear": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp, _i64, _i32, _vp, _i64, _i32, _vp, _i64, _vp,
                              _i64, _vp]),
     "glt_w4_linear_workspace": (_i32, [_i32, _i32, _i32, _i32, _i32, C.POINTER(_i64)]),
+    "glt_w8_quantize_rows": (_i32, [_vp, _i64, _i32, _i32, _vp, _f32, _vp, _i64, _vp, _vp]),
+    "glt_w8_linear_rows": (_i32, [_vp, _i64, _vp, _i32, _vp, _i64, _vp, _i32, _i32, _vp, _i64, _i32, _vp, _i64, _vp]),
+    "glt_w8_linear_workspace": (_i32, [_i32, _i32, C.POINTER(_i64)]),
+    "glt_w8_linear": (_i32, [_vp, _i64, _i32, _vp, _f32, _vp, _i64, _vp, _i32, _i32, _vp, _i64, _i32, _vp, _i64, _vp,
+                             _i64, _vp]),
     "glt_token_logprobs": (_i32, [_vp, _i32, _i64, _i32, _i32, _vp, _f32, _i32, _vp, _vp, _vp, _vp, _vp,
                                   _vp]),
     "glt_token_logprobs_bwd": (_i32, [_vp, _i32, _i64, _i32, _i32, _vp, _f32, _vp, _vp, _vp, _vp, _vp, _i64,

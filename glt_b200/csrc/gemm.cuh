@@ -112,8 +112,8 @@ constexpr int pair_stages() {
 
 // The same contraction on CTA pairs: 256 x 256 output tiles, each CTA of a
 // pair staging 128 rows of A and 128 rows of B per k-block.  group_m counts
-// 256-row tiles.  Static round-robin schedule over clusters.
-template <bool A_MN, bool B_MN, class Epi>
+// 256-row tiles.  With Mma = PairS8 the operands are bytes, and K and the strides count pairs of them.  Static round-robin schedule over clusters.
+template <bool A_MN, bool B_MN, class Mma = tc::PairBf16, class Epi>
 int launch_gemm_pair(const Operand& A, const Operand& B, int M, int N, int K, const Epi& epi,
                      cudaStream_t stream, int k_splits, const Operand* A2, int a2_n_tile,
                      int group_m, const int* m_dev, int m_off, unsigned int* err, uint64_t timeout_ns) {
@@ -158,7 +158,7 @@ int launch_gemm_pair(const Operand& A, const Operand& B, int M, int N, int K, co
   if (!shape.err) return fail(GLT_ECUDA, "device error word unavailable");
   shape.timeout_ns = timeout_ns;
   shape.selftest_skip_first_load = 0;
-  auto kern = tc_gemm_pair_kernel<STAGES, A_MN, B_MN, Epi>;
+  auto kern = tc_gemm_pair_kernel<STAGES, A_MN, B_MN, Epi, Mma>;
   constexpr int smem = gemm_pair_smem_bytes<STAGES, Epi>();
   constexpr int threads = gemm_threads<Epi>();
   GLT_TRY(ensure_smem_attr(reinterpret_cast<const void*>(kern), smem));

@@ -126,6 +126,36 @@ __host__ __device__ constexpr uint32_t make_idesc_pair(bool a_mn, bool b_mn) {
          ((static_cast<uint32_t>(PAIR_BN) >> 3) << 17) | ((static_cast<uint32_t>(PAIR_BM) >> 4) << 24);
 }
 
+// What the pair kernel multiplies.  PairBf16: bf16, 32-bit float sums.  PairS8: signed bytes, 32-bit
+// integer sums (the accumulator's bits are int32); every size, stride and coordinate along K then
+// counts pairs of bytes, since a k-block is 128 bytes and an instruction 32 bytes in both.
+struct PairBf16 {
+  template <bool A_MN, bool B_MN>
+  static constexpr uint32_t idesc() { return make_idesc_pair(A_MN, B_MN); }
+  static __device__ __forceinline__ void issue(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    umma_bf16_pair(d, a, b, idesc, acc);
+  }
+};
+// Instruction descriptor, kind::i8: s8 x s8 -> s32, both operands K-major.
+__host__ __device__ constexpr uint32_t make_idesc_s8(int m, int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((static_cast<uint32_t>(n) >> 3) << 17) |
+         ((static_cast<uint32_t>(m) >> 4) << 24);
+}
+struct PairS8 {
+  template <bool A_MN, bool B_MN>
+  static constexpr uint32_t idesc() {
+    static_assert(!A_MN && !B_MN, "bytes are K-major");
+    return make_idesc_s8(PAIR_BM, PAIR_BN);
+  }
+  static __device__ __forceinline__ void issue(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc));
+  }
+};
+
 template <int STAGES>
 struct PairSmemLayout {
   static constexpr uint32_t A_BYTES = TileBytes<BM>::value;         // 128 rows of A
@@ -146,7 +176,7 @@ constexpr uint32_t gemm_pair_smem_bytes() {
              : 1024 + L::SCRATCH_OFF + 4 * EpiParts<Epi>::value * EpiScratch<Epi>::value;
 }
 
-template <int STAGES, bool A_MN, bool B_MN, class Epi>
+template <int STAGES, bool A_MN, bool B_MN, class Epi, class Mma = PairBf16>
 __global__ void __launch_bounds__(gemm_threads<Epi>(), 1)
     tc_gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA,
                         const __grid_constant__ CUtensorMap tmA2,
@@ -158,7 +188,7 @@ __global__ void __launch_bounds__(gemm_threads<Epi>(), 1)
   static_assert(PARTS == 1 || PARTS == 2, "kParts");
   static_assert(gemm_pair_smem_bytes<STAGES, Epi>() <= 232448 - 64, "shared memory");
   constexpr uint32_t TMEM_COLS = 2 * BN;   // two accumulators of 256 columns
-  constexpr uint32_t IDESC = make_idesc_pair(A_MN, B_MN);
+  constexpr uint32_t IDESC = Mma::template idesc<A_MN, B_MN>();
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -320,7 +350,7 @@ __global__ void __launch_bounds__(gemm_threads<Epi>(), 1)
           for (int k = 0; k < BK / UMMA_K; ++k) {
             const uint64_t ad = A_MN ? desc_mnmajor(a_addr, k) : desc_kmajor(a_addr, k);
             const uint64_t bd = B_MN ? desc_mnmajor(b_addr, k) : desc_kmajor(b_addr, k);
-            umma_bf16_pair(d_tmem, ad, bd, IDESC, acc);
+            Mma::issue(d_tmem, ad, bd, IDESC, acc);
             acc = 1;
           }
           umma_commit_pair_both(&empty_bar[s]);   // frees the stage in both CTAs

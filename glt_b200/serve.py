@@ -2,7 +2,8 @@
 
 ``Kv8Cache`` / ``Kv8Batch``: a key/value cache in 8 bits with one scale for each block of
 tokens and head, and the attention that reads it; ``W4Weight``: products with 4-bit weights
-and group scales; ``token_logprobs`` / ``token_logprobs_bwd``: log probabilities of given
+and group scales; ``W8Weight`` / ``quantize_rows``: products in 8-bit integers with a scale for each
+token and channel; ``token_logprobs`` / ``token_logprobs_bwd``: log probabilities of given
 tokens, entropy, the most likely tokens, and the gradient.  Every call runs on the device that its
 tensors share (which need not be the current one), on its current stream, allocates its outputs
 with torch and does not synchronise.
@@ -22,7 +23,7 @@ FORMATS = {"int8": 0, "e4m3": 1}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # the handle without a Stream object around it
 _capturing = torch.cuda.is_current_stream_capturing
 _current_device = torch.cuda.current_device
-_BF16, _F32, _I32, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8
+_BF16, _F32, _I32, _U8, _I8 = torch.bfloat16, torch.float32, torch.int32, torch.uint8, torch.int8
 
 
 def _stream(i: int) -> int:
@@ -323,6 +324,138 @@ def quantize_w4(w: torch.Tensor, group: int = 128, asym: bool = False):
     check(lib.glt_w4_quantize(w.data_ptr(), w.stride(0) if N > 1 else K, N, K, group, int(asym), codes.data_ptr(),
                               scales.data_ptr(), None if zeros is None else zeros.data_ptr(), _stream(dev)))
     return codes, scales, zeros
+
+
+class W8Rows(NamedTuple):
+    """Rows in 8 bits: codes int8 [rows, K], a view whose rows lie a multiple of 16 bytes apart with zeros between
+    them, and scales fp32 [rows]."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def _bf16_rows(t: torch.Tensor, device: int, rows: int | None, K: int, name: str) -> int:
+    """Row stride of a bf16 [rows, K] tensor of the device whose rows are dense."""
+    if not (t.get_device() == device and t.dtype is _BF16 and t.dim() == 2 and t.shape[1] == K and
+            (rows is None or t.shape[0] == rows) and (t.stride(1) == 1 or K == 1)):
+        raise ValueError(f"{name} must be a bf16 tensor [{'M' if rows is None else rows}, {K}] on cuda:{device} with dense rows")
+    return t.stride(0) if t.shape[0] > 1 else K
+
+
+def _norm_weight(norm: torch.Tensor | None, device: int, K: int) -> int | None:
+    if norm is None:
+        return None
+    if not (norm.get_device() == device and norm.dtype is _BF16 and norm.shape == (K,) and norm.is_contiguous()):
+        raise ValueError(f"norm must be a contiguous bf16 tensor [{K}] on cuda:{device}")
+    return norm.data_ptr()
+
+
+def quantize_rows(x: torch.Tensor, norm: torch.Tensor | None = None, eps: float = 1e-6) -> W8Rows:
+    """Rows of bf16 x [rows, K] in 8 bits, each with its own scale; with ``norm`` (bf16 [K]) of its RMSNorm."""
+    _need(x.is_cuda and x.dim() == 2 and x.shape[1] > 0, "x must be a bf16 CUDA tensor [rows, K]")
+    dev = x.get_device()
+    if dev != _current_device():
+        with torch.cuda.device(dev):
+            return quantize_rows(x, norm, eps)
+    rows, K = x.shape
+    ld_x, norm_at = _bf16_rows(x, dev, rows, K, "x"), _norm_weight(norm, dev, K)
+    codes = torch.empty((rows, (K + 15) // 16 * 16), dtype=_I8, device=x.device)
+    scales = torch.empty((rows,), dtype=_F32, device=x.device)
+    check(lib.glt_w8_quantize_rows(x.data_ptr(), ld_x, rows, K, norm_at, eps, codes.data_ptr(), codes.shape[1],
+                                   scales.data_ptr(), _stream(dev)))
+    return W8Rows(codes[:, :K], scales)
+
+
+class W8Weight:
+    """A weight matrix [N, K] in 8-bit integers with a scale for each output channel."""
+
+    def __init__(self, rows: W8Rows):
+        codes, scales = rows
+        _need(codes.is_cuda and codes.dtype is _I8 and codes.dim() == 2 and codes.shape[0] > 0 and codes.shape[1] > 0,
+              "codes must be an int8 CUDA tensor [N, K]")
+        self.N, self.K = codes.shape
+        self._device = codes.get_device()
+        _need(scales.get_device() == self._device and scales.dtype is _F32 and scales.shape == (self.N,)
+              and scales.is_contiguous(), f"scales must be a contiguous fp32 tensor [{self.N}] on the codes' device")
+        self._ld = codes.stride(0) if self.N > 1 else (self.K + 15) // 16 * 16
+        if (codes.stride(1) != 1 and self.K > 1) or self._ld % 16 or self._ld < (self.K + 15) // 16 * 16:
+            raise ValueError("rows of codes must be dense and lie a multiple of 16 bytes apart (from_codes lays any out)")
+        self.codes, self.scales = codes, scales
+        self._ws_bytes: dict[int, int] = {}
+
+    @classmethod
+    def from_codes(cls, codes: torch.Tensor, scales: torch.Tensor) -> "W8Weight":
+        """codes int8 [N, K], scales fp32 [N]: the weight is codes * scales[:, None].  The codes are laid out anew."""
+        _need(codes.is_cuda and codes.dtype is _I8 and codes.dim() == 2, "codes must be an int8 CUDA tensor [N, K]")
+        _one_device(codes=codes, scales=scales)
+        _need(scales.dtype is _F32, "scales must be fp32")
+        N, K = codes.shape
+        laid = torch.empty((N, (K + 15) // 16 * 16), dtype=_I8, device=codes.device)
+        laid[:, :K] = codes
+        laid[:, K:] = 0
+        return cls(W8Rows(laid[:, :K], scales.contiguous()))
+
+    @classmethod
+    def quantize(cls, w: torch.Tensor) -> "W8Weight":
+        """Round a bf16 [N, K] matrix to 8 bits, a scale for each row."""
+        return cls(quantize_rows(w))
+
+    def linear(self, x: torch.Tensor, resid: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
+               out: torch.Tensor | None = None, norm: torch.Tensor | None = None, eps: float = 1e-6) -> torch.Tensor:
+        """x . W^T (+ resid), x bf16 [M, K] rounded to 8 bits a row (after its RMSNorm with weight ``norm``);
+        result [M, N] in bf16 or fp32."""
+        K, dev = self.K, self._device
+        if dev != _current_device():
+            with torch.cuda.device(dev):
+                return self.linear(x, resid, out_dtype, out, norm, eps)
+        ld_x, norm_at = _bf16_rows(x, dev, None, K, "x"), _norm_weight(norm, dev, K)
+        M = x.shape[0]
+        out, ld_y, r, ld_r = self._outputs(M, resid, out_dtype, out)
+        need = self._ws_bytes.get(M)
+        if need is None:
+            n = C.c_int64()
+            check(lib.glt_w8_linear_workspace(M, K, C.byref(n)))
+            need = self._ws_bytes[M] = n.value
+        stream = _stream(dev)
+        ws = _scratch.get(need, dev, stream)
+        st = lib.glt_w8_linear(x.data_ptr(), ld_x, M, norm_at, eps, self.codes.data_ptr(), self._ld, self.scales.data_ptr(),
+                               self.N, K, out.data_ptr(), ld_y, out.dtype is _BF16, r, ld_r, ws.data_ptr(), need, stream)
+        if st:
+            check(st)
+        return out
+
+    def linear_rows(self, rows: W8Rows, resid: torch.Tensor | None = None, out_dtype: torch.dtype = torch.bfloat16,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+        """``linear`` of rows that ``quantize_rows`` gave, for weights that share their input."""
+        K, dev = self.K, self._device
+        if dev != _current_device():
+            with torch.cuda.device(dev):
+                return self.linear_rows(rows, resid, out_dtype, out)
+        codes, scales = rows
+        M = codes.shape[0]
+        ld = codes.stride(0) if M > 1 else (K + 15) // 16 * 16
+        if not (codes.get_device() == dev == scales.get_device() and codes.dtype is _I8 and codes.shape == (M, K) and
+                (codes.stride(1) == 1 or K == 1) and scales.dtype is _F32 and scales.shape == (M,) and scales.is_contiguous()):
+            raise ValueError(f"rows must be those quantize_rows gives of [M, {K}] on cuda:{dev}")
+        out, ld_y, r, ld_r = self._outputs(M, resid, out_dtype, out)
+        check(lib.glt_w8_linear_rows(codes.data_ptr(), ld, scales.data_ptr(), M, self.codes.data_ptr(), self._ld,
+                                     self.scales.data_ptr(), self.N, K, out.data_ptr(), ld_y, out.dtype is _BF16, r, ld_r,
+                                     _stream(dev)))
+        return out
+
+    def _outputs(self, M: int, resid, out_dtype, out):
+        """(out, its row stride, resid's address, its row stride)"""
+        N, dev = self.N, self._device
+        if out is None:
+            if out_dtype is not _BF16 and out_dtype is not _F32:
+                raise ValueError("out_dtype must be bfloat16 or float32")
+            out = torch.empty((M, N), dtype=out_dtype, device=self.codes.device)
+        elif not (out.get_device() == dev and out.shape == (M, N) and out.dtype in (_BF16, _F32) and
+                  (out.stride(1) == 1 or N == 1)):
+            raise ValueError(f"out must be a bf16 or fp32 tensor [{M}, {N}] on cuda:{dev} with dense rows")
+        r = ld_r = 0
+        if resid is not None:
+            ld_r, r = _bf16_rows(resid, dev, M, N, "resid"), resid.data_ptr()
+        return out, out.stride(0) if M > 1 else N, r or None, ld_r
 
 
 class TokenLogprobs(NamedTuple):

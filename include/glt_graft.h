@@ -345,6 +345,28 @@ GLT_API int glt_w4_linear(const void* packed, int N, int K, int group, int asym,
                           int64_t workspace_bytes, void* stream);
 GLT_API int glt_w4_linear_workspace(int M, int N, int K, int group, int y_dtype, int64_t* bytes);
 
+/* Products in 8-bit integers with a scale for each token and each channel.
+ * glt_w8_quantize_rows: rows of bf16 x [rows, K] (row stride ld_x) to codes [rows, K] (row stride ld_codes,
+ *   a multiple of 16, 16-byte aligned; the bytes from K to the next multiple of 16 are set to 0) and
+ *   scales [rows] fp32: scale = max|x| / 127 over the row, code = nearest to x / scale (both quotients rounded to 32 bits),
+ *   ties to even.  With norm (bf16 [K]) the row is first x / sqrt(mean(x^2) + eps) * norm, in 32 bits.
+ *   A row of zeros has scale 0; one that holds an infinity or NaN has scale NaN and codes 0.  Weights
+ *   [N, K] are quantised by the same call, a channel a row.
+ * glt_w8_linear_rows: y[M, N] = scale[m] * w_scale[n] * sum_k code[m, k] * w[n, k] (+ resid[m, n]), y bf16 (y_dtype 1) or
+ *   fp32 (0), resid bf16 or NULL.  Codes are -128..127, laid out as above with zeros behind K.  Sums are exact.
+ * glt_w8_linear: both, the codes of x in the workspace: glt_w8_linear_workspace bytes, 16-byte aligned,
+ *   used by one call at a time; its contents do not matter.  K at most 131071. */
+GLT_API int glt_w8_quantize_rows(const uint16_t* x, int64_t ld_x, int rows, int K, const uint16_t* norm,
+                                 float eps, int8_t* codes, int64_t ld_codes, float* scales, void* stream);
+GLT_API int glt_w8_linear_rows(const int8_t* codes, int64_t ld_codes, const float* scales, int M,
+                               const int8_t* w, int64_t ld_w, const float* w_scales, int N, int K, void* y,
+                               int64_t ld_y, int y_dtype, const uint16_t* resid, int64_t ld_r, void* stream);
+GLT_API int glt_w8_linear_workspace(int M, int K, int64_t* bytes);
+GLT_API int glt_w8_linear(const uint16_t* x, int64_t ld_x, int M, const uint16_t* norm, float eps,
+                          const int8_t* w, int64_t ld_w, const float* w_scales, int N, int K, void* y,
+                          int64_t ld_y, int y_dtype, const uint16_t* resid, int64_t ld_r, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+
 /* Log probabilities of given tokens, entropy and the most likely tokens, from
  * logits [rows, V] (dtype 0 fp32, 1 bf16; row stride ld), z = scale * logit with
  * scale > 0 (one over the temperature):
