@@ -90,8 +90,13 @@ class GltKv8Batch(C.Structure):
                 ("block_table", _vp), ("lengths", _vp), ("row_start", _vp)]
 
 
+class GltKv8Prefix(C.Structure):
+    """ctypes mirror of GltKv8Prefix (include/glt_graft.h)."""
+    _fields_ = [("num_blocks", _i32), ("block_ids", _vp), ("length", _vp)]
+
+
 _cfgp = C.POINTER(GltModelConfig)
-_kcp, _kbp = C.POINTER(GltKv8Cache), C.POINTER(GltKv8Batch)
+_kcp, _kbp, _kpp = C.POINTER(GltKv8Cache), C.POINTER(GltKv8Batch), C.POINTER(GltKv8Prefix)
 _gwp = C.POINTER(GltGraftWeights)
 _svp = C.POINTER(GltMlpSaved)
 _fp = C.POINTER(C.c_void_p)
@@ -189,6 +194,11 @@ SIGNATURES: dict[str, tuple] = {
     "glt_kv8_attention_workspace": (_i32, [_kcp, _kbp, _i32, C.POINTER(_i64)]),
     "glt_kv8_attention": (_i32, [_kcp, _kbp, _vp, _i64, _vp, _i64, _vp, _i32, _f32, _i32, _vp, _i64, _vp,
                                  _i64, _vp]),
+    "glt_kv8_window_attention": (_i32, [_kcp, _kbp, _vp, _i64, _vp, _i64, _vp, _i32, _f32, _i32, _i32, _vp, _i64, _vp,
+                                        _i64, _vp]),
+    "glt_kv8_prefix_attention_workspace": (_i32, [_kcp, _kbp, _kpp, _i32, C.POINTER(_i64)]),
+    "glt_kv8_prefix_attention": (_i32, [_kcp, _kbp, _kpp, _vp, _i64, _vp, _i64, _vp, _i32, _f32, _vp, _i64, _vp, _i64,
+                                        _vp]),
     "glt_kv8_read": (_i32, [_kcp, _kbp, _vp, _i32, _vp, _vp, _vp]),
     "glt_w4_packed_bytes": (_i32, [_i32, _i32, _i32, _i32, C.POINTER(_i64)]),
     "glt_w4_quantize": (_i32, [_vp, _i64, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),

@@ -1,0 +1,559 @@
+// Attention of a batch of sequences that share a long prefix (glt_kv8_prefix_attention).
+//
+//   o = (sum over the prefix + sum over own tokens of p v) / (the same of p)
+//
+// Every query of the batch sees the whole prefix, so its cache is read once for all of them: the queries
+// that share a KV head are the rows of tcgen05 products with it.
+//
+// A CTA (see kv8_prefix.cuh for its share of the work) goes through steps of 128 tokens:
+//   warps 8-15  copy the codes of the next step to registers, turn them into bf16, which holds codes exactly (8 bits of
+//               int8, 4 of e4m3), and lay K and V into shared memory as the products read them.
+//   warp 16     issues the products: S = Q K^T, and O += P V with P in TMEM, as P was written over S.
+//   warps 0-7   softmax, a thread a query row, in two lanes of 128 rows with an S and an O each: the tensor core works
+//               for one lane while the other's softmax runs.  With more than 128 rows a KV head the lanes are two
+//               tiles of rows at the same tokens; else every second step of the same rows.
+// Q is bf16 as it came.  K's scale multiplies S in 32 bits.  V's scale multiplies the weight p in 32 bits, and what comes of it
+// is split into two bf16 numbers, p = hi + lo, of 16 bits together and the exponents of a float: whatever the scales of
+// different blocks are, each weight keeps its 16 bits.  It costs one product more than rounding p.
+// The sums of a row move to a new maximum only when it has grown by more than 2^8.
+#include <float.h>
+
+#include "kv8_attention.cuh"
+
+namespace glt {
+namespace {
+
+constexpr int kSoftmaxWarps = 8, kDecodeWarps = 8;
+constexpr int kPrefixThreads = 32 * (kSoftmaxWarps + kDecodeWarps + 1);
+constexpr int kDecodeThreads = 32 * kDecodeWarps;
+constexpr float kSlack = 8.f;   // base 2: how far weights may exceed 1
+
+struct PrefixArgs {
+  GltKv8Cache c;
+  const int32_t* block_ids;
+  const uint16_t* q;
+  int64_t ld_q;
+  int rows, group;   // query rows a KV head: rows = tokens * group
+  float scale;
+  PrefixParts parts;
+  unsigned int* err;
+};
+
+// Scales of a stage's groups of 16 tokens.  A block that is not in the pool has k = -1.
+struct PrefixNote {
+  float k[8], v[8];
+};
+
+template <int HD, int LANES>
+struct PrefixSmem {
+  static constexpr int kQ = kPrefixRows * HD * 2;
+  static constexpr int kPart = kPrefixStep * HD * 2;   // K (or V) of a stage
+  static constexpr int kStage = 2 * kPart;
+  static constexpr int kStages = LANES == 2 ? 2 : 3;
+  static constexpr int kBars = 2 * kStages + 2 + 2 + 3;
+  static constexpr int kOffStages = LANES * kQ;
+  static constexpr int kOffNotes = kOffStages + kStages * kStage;
+  static constexpr int kOffBars = kOffNotes + kStages * static_cast<int>(sizeof(PrefixNote));
+  static constexpr int kTotal = 1024 + kOffBars + kBars * 8 + 16;
+};
+static_assert(PrefixSmem<128, 1>::kTotal <= 232448 && PrefixSmem<128, 2>::kTotal <= 232448, "shared memory");
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st32f(uint32_t taddr, const float (&v)[32]) {
+  uint32_t u[16];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[16 * h + i]);
+    tmem_st16(taddr + 16 * h, u);
+  }
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// O (+)= P . V with P in TMEM.
+__device__ __forceinline__ void umma_p(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc));
+}
+
+// Bytes 0, 1 (HI = 0) or 2, 3 of a word of codes as two bf16 numbers, exactly.  A byte c of two's complement is
+// (128 + its low seven bits) - (256 if negative, else 128), and both are bf16 numbers whose bits hold the byte's.
+template <int FMT, int HI>
+__device__ __forceinline__ uint32_t two_bf16(uint32_t w) {
+  uint32_t r;
+  if constexpr (FMT == GLT_KV8_INT8) {
+    const uint32_t x = __byte_perm(w ^ 0x80808080u, 0x43434343u, HI ? 0x4342 : 0x4140);
+    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x & 0xFF7FFF7Fu), "r"(x & 0xFF80FF80u));
+  } else {
+    const uint32_t h = e4m3x2_to_f16x2(HI ? w >> 16 : w & 0xFFFFu);
+    asm("{.reg .b16 lo, hi; .reg .f32 a, b; mov.b32 {lo, hi}, %1; cvt.f32.f16 a, lo; cvt.f32.f16 b, hi;"
+        " cvt.rn.bf16x2.f32 %0, b, a;}"
+        : "=r"(r)
+        : "r"(h));
+  }
+  return r;
+}
+
+// Walks a CTA's run: unit `unit`, steps [s0, s1) of it.
+struct PrefixRun {
+  int64_t at, end;
+  int steps, unit, s0, s1;
+  __device__ __forceinline__ PrefixRun(const PrefixShares& sh, int cta)
+      : at(cta < sh.ctas ? sh.begin(cta) : 0), end(cta < sh.ctas ? sh.begin(cta + 1) : 0), steps(sh.steps) {
+    if (at < end) {
+      unit = static_cast<int>(at / steps);
+      s0 = static_cast<int>(at - static_cast<int64_t>(unit) * steps);
+      s1 = static_cast<int>(min(static_cast<int64_t>(steps), s0 + (end - at)));
+    }
+  }
+  __device__ __forceinline__ bool on() const { return at < end; }
+  __device__ __forceinline__ void next() {
+    at += s1 - s0;
+    ++unit;
+    s0 = 0;
+    s1 = static_cast<int>(min(static_cast<int64_t>(steps), end - at));
+  }
+};
+
+template <int HD, int FMT, int LANES>
+__global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __grid_constant__ PrefixArgs a) {
+  using L = PrefixSmem<HD, LANES>;
+  constexpr uint32_t kIdescS = tc::make_idesc(kPrefixStep, false, false), kIdescO = tc::make_idesc(HD, false, true);
+  constexpr uint32_t kColO = 256;   // TMEM: S of lane 0, of lane 1 (128 columns each), O of lane 0, of lane 1
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + (-tc::smem_u32(smem_raw) & 1023u);   // the swizzle goes by address
+  PrefixNote* notes = reinterpret_cast<PrefixNote*>(smem + L::kOffNotes);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBars);   // a stage is laid out
+  uint64_t* empty = full + L::kStages;                                // a stage's products are done
+  uint64_t* s_full = empty + L::kStages;                              // [lane] S is there
+  uint64_t* p_full = s_full + 2;                                      // [lane] P is there
+  uint64_t* q_full = p_full + 2;                                      // the unit's queries are laid out
+  uint64_t* unit_done = q_full + 1;                                   // all products of the unit are done
+  uint64_t* drain = unit_done + 1;
+  uint32_t* slot = reinterpret_cast<uint32_t*>(drain + 1);
+  __shared__ int abort_storage;
+  volatile int& abort = abort_storage;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::kStages; ++i) {
+      tc::mbar_init(full + i, kDecodeWarps);
+      tc::mbar_init(empty + i, 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(s_full + i, 1);
+      tc::mbar_init(p_full + i, 4);
+    }
+    tc::mbar_init(q_full, kSoftmaxWarps);
+    tc::mbar_init(unit_done, 1);
+    tc::mbar_init(drain, 1);
+    abort = 0;
+    tc::fence_mbar_init();
+  }
+  if (warp == 16) {
+    tc::tmem_alloc(slot, 512);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *slot;
+  const int tokens = a.parts.tokens(blockIdx.x == 0 && threadIdx.x == 0 ? a.err : nullptr);
+  const PrefixShares shares(a.parts, tokens);
+  PrefixRun run(shares, blockIdx.x);
+
+  if (warp < kSoftmaxWarps) {
+    // ------------------------------- softmax -------------------------------
+    const int mine = warp >> 2;                            // lane of the pipeline
+    const int r = (warp & 3) * 32 + lane;                  // query row in the tile
+    const uint32_t at = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
+    const uint32_t s_at = at + mine * 128, o_at = at + kColO + mine * 128;
+    const float unit_q = a.scale * 1.4426950408889634f;
+    uint32_t s_phase = 0;
+    int seg = 0, base = 0;   // steps before the unit's
+    for (; run.on() && !abort; run.next(), ++seg) {
+      const int kvh = run.unit % a.parts.kv_heads, pair = run.unit / a.parts.kv_heads;
+      // ---- queries.  LANES = 2: a thread its row; else two threads a row
+      {
+        const int row = LANES == 2 ? r : static_cast<int>(threadIdx.x) >> 1;
+        const int rho = (LANES == 2 ? pair * 2 + mine : pair) * kPrefixRows + row;
+        const int tok = rho / a.group;
+        const uint16_t* src = a.q + static_cast<int64_t>(tok) * a.ld_q + (kvh * a.group + rho - tok * a.group) * HD;
+        uint8_t* dst = smem + (LANES == 2 ? mine * L::kQ : 0) + row * 128;
+        const int first = LANES == 2 ? 0 : (threadIdx.x & 1) * (HD / 16), count = LANES == 2 ? HD / 8 : HD / 16;
+#pragma unroll
+        for (int i = 0; i < count; ++i) {
+          const int c = first + i;   // 8 channels
+          const uint4 x = rho < a.rows ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(dst + (c >> 3) * (kPrefixRows * 128) + (((c & 7) ^ (row & 7)) << 4)) = x;
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(q_full);
+      }
+      float m = -INFINITY, l = 0.f;
+      bool any = false;
+      const int n = run.s1 - run.s0;
+      for (int i = LANES == 2 ? 0 : mine; i < n; i += LANES == 2 ? 1 : 2) {
+        const int st = (base + i) % L::kStages;
+        // (the stage is long laid out when S is there: waited for so that its note is seen)
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(s_full + mine, s_phase, a.err, &abort) &&
+                                         tc::mbar_wait(full + st, ((base + i) / L::kStages) & 1, a.err, &abort))) {
+          abort = 1;
+          break;
+        }
+        s_phase ^= 1;
+        tc::tc_fence_after();
+        const PrefixNote& note = notes[st];
+        const int left = tokens - (run.s0 + i) * kPrefixStep;   // tokens of the step
+        float uk[8];
+        bool bad = false;
+#pragma unroll
+        for (int g = 0; g < 8; ++g) {
+          const float k = note.k[g];
+          bad |= k < 0.f;
+          uk[g] = fmaxf(k * unit_q, 1e-37f);   // above 0, so that a masked -inf stays one
+        }
+        const bool edge = bad || left < kPrefixStep;
+        // a masked score, of columns c .. c + 31
+        auto mask = [&](float (&v)[32], int c) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (c + j >= left || note.k[(c + j) >> 4] < 0.f) v[j] = -INFINITY;
+        };
+        float peak = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) {
+          float v[32];
+          tc::tmem_ld32(s_at + c, v);
+          if (edge) mask(v, c);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float x[4] = {v[16 * h], v[16 * h + 1], v[16 * h + 2], v[16 * h + 3]};
+#pragma unroll
+            for (int j = 4; j < 16; ++j) x[j & 3] = fmaxf(x[j & 3], v[16 * h + j]);
+            peak = fmaxf(peak, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * uk[c / 16 + h]);
+          }
+        }
+        const bool grow = peak > m + kSlack || (m == -INFINITY && peak > m);
+        if (__any_sync(0xffffffffu, grow)) {
+          // S of this step came after the products of the lane's last: O is at rest
+          const float f = grow ? (m == -INFINITY ? 0.f : ex2_approx(m - peak)) : 1.f;
+          if (any) {
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 32) {
+              float o[32];
+              tc::tmem_ld32(o_at + c, o);
+#pragma unroll
+              for (int j = 0; j < 32; ++j) o[j] *= f;
+              tmem_st32f(o_at + c, o);
+            }
+          }
+          if (grow) {
+            l *= f;
+            m = peak;
+          }
+        }
+        any = true;
+        const float ref = m == -INFINITY ? 0.f : m;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 128; c += 32) {
+          float v[32];
+          tc::tmem_ld32(s_at + c, v);
+          if (edge) mask(v, c);
+          uint32_t hi[16], lo[16];
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float sv = note.v[(c + j) >> 4];
+            const float p0 = ex2_approx(fmaf(v[j], uk[(c + j) >> 4], -ref));
+            const float p1 = ex2_approx(fmaf(v[j + 1], uk[(c + j) >> 4], -ref));
+            sum[j & 2] += p0;
+            sum[(j & 2) + 1] += p1;
+            const float w0 = p0 * sv, w1 = p1 * sv;
+            const uint32_t h = pack_bf16x2_rn(w0, w1);
+            hi[j >> 1] = h;
+            lo[j >> 1] = pack_bf16x2_rn(w0 - bf16_lo(h), w1 - bf16_hi(h));
+          }
+          tmem_st16(s_at + c, hi);        // over the scores just read: hi of 32 tokens, then lo
+          tmem_st16(s_at + c + 16, lo);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_wait_st();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(p_full + mine);
+      }
+      // ---- the unit's result
+      if (abort || !__all_sync(0xffffffffu, tc::mbar_wait(unit_done, seg & 1, a.err, &abort))) {
+        abort = 1;
+        break;
+      }
+      tc::tc_fence_after();
+      float* out = a.parts.slots + (static_cast<int64_t>(run.unit) + blockIdx.x) * PrefixParts::slot_floats(HD);
+      const int row = mine * kPrefixRows + r;
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 32) {
+        float o[32];
+        if (any) {
+          tc::tmem_ld32(o_at + c, o);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) o[j] = 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < 32; j += 4)
+          *reinterpret_cast<float4*>(out + row * HD + c + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+      }
+      out[2 * kPrefixRows * HD + row] = m;
+      out[2 * kPrefixRows * (HD + 1) + row] = l;
+      tc::tc_fence_before();   // the next unit's products write O once P of its first step has come
+      base += n;
+    }
+  } else if (warp < kSoftmaxWarps + kDecodeWarps) {
+    // ------------------------------- codes ---------------------------------
+    constexpr int kChunks = HD / 16;                                    // 16 channels of a token
+    constexpr int kMine = kPrefixStep * kChunks / kDecodeThreads;       // of a thread, of K and of V
+    constexpr int kTokenStep = kDecodeThreads / kChunks;                // tokens between two of them
+    const int tid = threadIdx.x - 32 * kSoftmaxWarps;
+    const int tok0 = tid / kChunks, chunk = tid % kChunks;
+    const int bt = a.c.block_tokens, bt_log = 31 - __clz(bt);
+    int step = run.on() ? run.s0 : 0;
+    // block ids are loaded a step before the codes, the codes a step before they are laid out
+    int ids[kMine], note_id = -1;
+    auto load_ids = [&](const PrefixRun& at, int s) {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int t = s * kPrefixStep + tok0 + i * kTokenStep;
+        ids[i] = at.on() && t < tokens ? a.block_ids[t >> bt_log] : -1;
+      }
+      if (tid < 8) {
+        const int t = s * kPrefixStep + tid * 16;
+        note_id = at.on() && t < tokens ? a.block_ids[t >> bt_log] : -2;
+      }
+    };
+    uint4 k[kMine], v[kMine];
+    float note_k = 0.f, note_v = 0.f;
+    auto address = [&](const PrefixRun& at, int s, int i) {
+      const int t = s * kPrefixStep + tok0 + i * kTokenStep;
+      return ((static_cast<int64_t>(ids[i]) * a.c.num_kv_heads + at.unit % a.parts.kv_heads) * bt + (t & (bt - 1))) * HD + chunk * 16;
+    };
+    auto load = [&](const PrefixRun& at, int s, uint4 (&x)[kMine], const uint8_t* pool) {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i)
+        x[i] = ids[i] >= 0 && ids[i] < a.c.num_blocks
+                   ? *reinterpret_cast<const uint4*>(pool + address(at, s, i))
+                   : (FMT == GLT_KV8_INT8 ? make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u) : make_uint4(0, 0, 0, 0));
+    };
+    auto load_note = [&](const PrefixRun& at) {
+      if (tid >= 8) return;
+      const bool in = note_id >= 0 && note_id < a.c.num_blocks;
+      const int64_t hb = static_cast<int64_t>(in ? note_id : 0) * a.c.num_kv_heads + at.unit % a.parts.kv_heads;
+      note_k = in ? a.c.k_scale[hb] : note_id == -2 ? 0.f : -1.f;
+      note_v = in ? a.c.v_scale[hb] : 0.f;
+      if (!in && note_id != -2 && at.on() && a.err) atomicOr(a.err, GLT_DEVERR_BAD_SHAPE);
+    };
+    auto lay = [&](const uint4 (&x)[kMine], uint8_t* dst) {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int tok = tok0 + i * kTokenStep;
+        uint8_t* row = dst + (chunk >> 2) * (kPrefixStep * 128) + tok * 128;
+        const int c = 2 * (chunk & 3);
+        *reinterpret_cast<uint4*>(row + ((c ^ (tok & 7)) << 4)) = make_uint4(
+            two_bf16<FMT, 0>(x[i].x), two_bf16<FMT, 1>(x[i].x), two_bf16<FMT, 0>(x[i].y), two_bf16<FMT, 1>(x[i].y));
+        *reinterpret_cast<uint4*>(row + (((c + 1) ^ (tok & 7)) << 4)) = make_uint4(
+            two_bf16<FMT, 0>(x[i].z), two_bf16<FMT, 1>(x[i].z), two_bf16<FMT, 0>(x[i].w), two_bf16<FMT, 1>(x[i].w));
+      }
+    };
+    auto advance = [&]() {
+      if (++step == run.s1) {
+        run.next();
+        step = run.on() ? run.s0 : 0;
+      }
+    };
+    if (run.on()) {
+      load_ids(run, step);
+      load(run, step, k, a.c.k);
+      load(run, step, v, a.c.v);
+      load_note(run);
+      for (int it = 0; !abort; ++it) {
+        // on to the next step, whose ids come now
+        advance();
+        load_ids(run, step);
+        const int st = it % L::kStages;
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(empty + st, ((it / L::kStages) & 1) ^ 1, a.err, &abort))) {
+          abort = 1;
+          break;
+        }
+        uint8_t* dst = smem + L::kOffStages + st * L::kStage;
+        if (tid < 8) {
+          notes[st].k[tid] = note_k;
+          notes[st].v[tid] = note_v;
+        }
+        lay(k, dst);
+        if (run.on()) load(run, step, k, a.c.k);
+        lay(v, dst + L::kPart);
+        if (run.on()) {
+          load(run, step, v, a.c.v);
+          load_note(run);
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(full + st);
+        if (!run.on()) break;
+      }
+    }
+  } else if (lane == 0) {
+    // ------------------------------- products ------------------------------
+    uint32_t p_phase[2] = {0, 0};
+    bool ok = true;
+    int base = 0;   // steps before the unit's
+    const uint32_t q_at = tc::smem_u32(smem), st_at = tc::smem_u32(smem + L::kOffStages);
+    for (int seg = 0; ok && run.on() && !abort; run.next(), ++seg) {
+      const int steps = run.s1 - run.s0, n = LANES * steps;   // products of a lane and a step
+      ok = tc::mbar_wait(q_full, seg & 1, a.err, &abort);
+      auto scores = [&](int i) {
+        const int step = base + (LANES == 2 ? i >> 1 : i), ln = i & 1, st = step % L::kStages;
+        if (LANES == 1 || ln == 0) {
+          if (!tc::mbar_wait(full + st, (step / L::kStages) & 1, a.err, &abort)) return false;
+        }
+        tc::tc_fence_after();
+        const uint32_t q = q_at + (LANES == 2 ? ln * L::kQ : 0), kk = st_at + st * L::kStage;
+#pragma unroll
+        for (int j = 0; j < HD / 16; ++j)
+          tc::umma_bf16(tmem + ln * 128, tc::desc_kmajor(q + (j >> 2) * (kPrefixRows * 128), j & 3),
+                        tc::desc_kmajor(kk + (j >> 2) * (kPrefixStep * 128), j & 3), kIdescS, j > 0);
+        tc::umma_commit(s_full + ln);
+        return true;
+      };
+      auto values = [&](int i) {
+        const int step = base + (LANES == 2 ? i >> 1 : i), ln = i & 1, st = step % L::kStages;
+        if (!tc::mbar_wait(p_full + ln, p_phase[ln], a.err, &abort)) return false;
+        p_phase[ln] ^= 1;
+        tc::tc_fence_after();
+        const uint32_t vv = st_at + st * L::kStage + L::kPart, p = tmem + ln * 128, o = tmem + kColO + ln * 128;
+        const bool first = i < 2;
+#pragma unroll
+        for (int j = 0; j < kPrefixStep / 16; ++j) {
+          const uint64_t b = tc::make_sdesc(vv + j * 2048, kPrefixStep * 128, 1024);
+          const uint32_t pj = p + (j >> 1) * 32 + (j & 1) * 8;
+          umma_p(o, pj, b, kIdescO, !(first && j == 0));
+          umma_p(o, pj + 16, b, kIdescO, 1);
+        }
+        if (LANES == 1 || ln == 1) tc::umma_commit(empty + st);
+        return true;
+      };
+      for (int i = 0; ok && i <= n; ++i) {
+        if (i < n) ok = scores(i);
+        if (ok && i > 0) ok = values(i - 1);
+      }
+      if (ok) tc::umma_commit(unit_done);
+      base += steps;
+    }
+    if (!ok) abort = 1;
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  if (warp == 16) {
+    tc::tc_fence_after();
+    if (abort) {
+      // no product may still write TMEM when it is given back
+      if (lane == 0) {
+        tc::umma_commit(drain);
+        tc::mbar_wait(drain, 0, a.err);
+      }
+      __syncwarp();
+    }
+    tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int HD, int FMT>
+int launch_prefix(const PrefixArgs& a, cudaStream_t st) {
+  auto go = [&](auto kern, int bytes) {
+    GLT_TRY(ensure_smem_attr(reinterpret_cast<const void*>(kern), bytes));
+    kern<<<a.parts.grid, kPrefixThreads, bytes, st>>>(a);
+    GLT_LAUNCH_CHECK();
+    return static_cast<int>(GLT_OK);
+  };
+  return a.parts.lanes == 2 ? go(kv8_prefix_kernel<HD, FMT, 2>, PrefixSmem<HD, 2>::kTotal)
+                            : go(kv8_prefix_kernel<HD, FMT, 1>, PrefixSmem<HD, 1>::kTotal);
+}
+
+int check_prefix(const GltKv8Cache* c, const GltKv8Prefix* p) {
+  if (!p) return fail(GLT_EINVAL, "null argument");
+  if (p->num_blocks < 0 || static_cast<int64_t>(p->num_blocks) * c->block_tokens > INT_MAX - 4096)
+    return fail(GLT_EINVAL, "kv8: a prefix of %d blocks", p->num_blocks);
+  if (!p->length || (p->num_blocks > 0 && !p->block_ids)) return fail(GLT_EINVAL, "kv8: null prefix length or block ids");
+  return GLT_OK;
+}
+
+// The shares of the prefix; `slots` is left to the caller.
+PrefixParts plan_prefix(const GltKv8Cache& c, const GltKv8Batch& b, const GltKv8Prefix& p, int nh) {
+  PrefixParts s = {};
+  s.length = p.length;
+  s.capacity = p.num_blocks * c.block_tokens;
+  s.kv_heads = c.num_kv_heads;
+  const int64_t rows = static_cast<int64_t>(b.rows) * (nh / c.num_kv_heads);
+  s.tiles = static_cast<int>((rows + kPrefixRows - 1) / kPrefixRows);
+  s.lanes = s.tiles > 1 ? 2 : 1;
+  const int64_t most = static_cast<int64_t>(s.units()) * ((s.capacity + kPrefixStep - 1) / kPrefixStep);
+  s.grid = num_sms();
+  if (most < s.grid) s.grid = static_cast<int>(most);
+  return s;
+}
+int64_t align16(int64_t n) { return (n + 15) / 16 * 16; }
+
+}  // namespace
+}  // namespace glt
+
+extern "C" int glt_kv8_prefix_attention_workspace(const GltKv8Cache* cache, const GltKv8Batch* batch,
+                                                  const GltKv8Prefix* prefix, int num_heads, int64_t* bytes) {
+  if (!bytes) return glt::fail(GLT_EINVAL, "null argument");
+  GLT_TRY(glt::check_heads(cache, batch, num_heads));
+  GLT_TRY(glt::check_prefix(cache, prefix));
+  *bytes = batch->rows > 0 && batch->max_new > 0
+               ? glt::align16(glt::plan(*cache, *batch, num_heads).bytes) +
+                     glt::plan_prefix(*cache, *batch, *prefix, num_heads).bytes(cache->head_dim)
+               : 0;
+  return GLT_OK;
+}
+
+extern "C" int glt_kv8_prefix_attention(const GltKv8Cache* cache, const GltKv8Batch* batch, const GltKv8Prefix* prefix,
+                                        const uint16_t* q, int64_t ld_q, uint16_t* o, int64_t ld_o, float* lse,
+                                        int num_heads, float scale, const uint8_t* token_mask, int64_t ld_mask,
+                                        void* workspace, int64_t workspace_bytes, void* stream) {
+  GLT_TRY(glt::check_heads(cache, batch, num_heads));
+  GLT_TRY(glt::check_prefix(cache, prefix));
+  if (batch->rows == 0 || batch->max_new == 0) return GLT_OK;
+  if (static_cast<int64_t>(batch->rows) * num_heads > INT_MAX / 2)
+    return glt::fail(GLT_EINVAL, "kv8: %d rows of %d heads", batch->rows, num_heads);
+  glt::AttnArgs a;
+  glt::Plan p;
+  GLT_TRY(glt::prepare(cache, batch, q, ld_q, o, ld_o, lse, num_heads, scale, 0, token_mask, ld_mask, workspace,
+                       workspace_bytes, &a, &p));
+  a.parts = glt::plan_prefix(*cache, *batch, *prefix, num_heads);
+  const int64_t own = glt::align16(p.bytes), need = own + a.parts.bytes(cache->head_dim);
+  if (workspace_bytes < need)
+    return glt::fail(GLT_EINVAL, "kv8: workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
+  a.parts.slots = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + own);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a.parts.grid > 0) {
+    const glt::PrefixArgs x = {*cache, prefix->block_ids, q, ld_q, batch->rows * a.group, a.group, a.scale, a.parts, a.err};
+    const bool int8 = cache->format == GLT_KV8_INT8;
+    if (cache->head_dim == 128)
+      GLT_TRY((int8 ? glt::launch_prefix<128, GLT_KV8_INT8>(x, st) : glt::launch_prefix<128, GLT_KV8_E4M3>(x, st)));
+    else
+      GLT_TRY((int8 ? glt::launch_prefix<64, GLT_KV8_INT8>(x, st) : glt::launch_prefix<64, GLT_KV8_E4M3>(x, st)));
+  }
+  return glt::launch_all<glt::Mode::kPrefix>(a, p, st);
+}

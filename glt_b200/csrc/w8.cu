@@ -66,15 +66,17 @@ __device__ __forceinline__ float norm_factor(float sum, int K, float eps, bool s
 }
 __device__ __forceinline__ float square_scaled(float x) { return (x * 0x1p-64f) * (x * 0x1p-64f); }
 
-// Codes of eight values.  Common: q = fl(y inv) with inv = fl(1 / s) is at most an ulp off, and one correction by the
-// exact remainder gives the correctly rounded quotient (Markstein); 1.5 * 2^23 added to it leaves the
+// Codes of eight values.  Common: y inv with inv = fl(1 / s) is within two units in the last place of the quotient, one
+// correction by the remainder brings it within one, and a second gives the quotient rounded to nearest
+// (Markstein's theorem, IBM Journal of Research and Development 34, 1990); 1.5 * 2^23 added to it leaves the
 // nearest integer, ties to even, in the low bits.  |q| <= 127 (1 + 2^-23), so nothing needs a clamp.
 __device__ __forceinline__ uint2 encode8(const float (&y)[8], float s, float inv, bool common) {
   uint32_t c[8];
   if (common) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float q = y[i] * inv;
+      float q = y[i] * inv;
+      q = fmaf(fmaf(-q, s, y[i]), inv, q);
       c[i] = __float_as_uint(fmaf(fmaf(-q, s, y[i]), inv, q) + 12582912.f);
     }
   } else {   // a scale of 0 (or one that is no number), or so small that its reciprocal or the remainders leave the float range

@@ -17,7 +17,7 @@ from typing import NamedTuple
 
 import torch
 
-from ._lib import GltKv8Batch as _CBatch, GltKv8Cache as _CCache, check, lib
+from ._lib import GltKv8Batch as _CBatch, GltKv8Cache as _CCache, GltKv8Prefix as _CPrefix, check, lib
 
 FORMATS = {"int8": 0, "e4m3": 1}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # the handle without a Stream object around it
@@ -107,6 +107,19 @@ class Kv8Batch:
         self._ws_bytes: dict[tuple, int] = {}   # attention's workspace by what it depends on
 
 
+class Kv8Prefix:
+    """A prefix that all sequences of a batch share, for all layers (GltKv8Prefix).
+
+    blocks int32 [n], the blocks of the cache that hold it; length int32 [1], its tokens (read on the device)."""
+
+    def __init__(self, blocks: torch.Tensor, length: torch.Tensor):
+        _need(blocks.dim() == 1 and length.shape == (1,), "blocks [n] and length [1]")
+        self.blocks, self.length = _int32(blocks, "blocks"), _int32(length, "length")
+        self._device = _one_device(blocks=blocks, length=length)
+        self._c = _CPrefix(blocks.shape[0], blocks.data_ptr(), length.data_ptr())
+        self._p = C.byref(self._c)
+
+
 class Kv8Cache:
     """One layer's key/value cache in 8 bits (GltKv8Cache)."""
 
@@ -157,17 +170,9 @@ class Kv8Cache:
         if st:
             check(st)
 
-    def attention(self, batch: Kv8Batch, q: torch.Tensor, scale: float = 0.0, window: int = 0,
-                  token_mask: torch.Tensor | None = None, out: torch.Tensor | None = None):
-        """Attention of the step's queries, bf16 [rows, num_heads, head_dim], after ``append``.
-        Returns (o like q, dense; lse fp32 [rows, num_heads])."""
-        if q.dim() != 3:
-            raise ValueError("q must be [rows, num_heads, head_dim]")
-        dev = self._batch_device(batch)
-        if dev != _current_device():
-            with torch.cuda.device(dev):
-                return self.attention(batch, q, scale, window, token_mask, out)
-        rows, nh = batch.rows, q.shape[1]
+    def _step(self, batch: Kv8Batch, q: torch.Tensor, token_mask: torch.Tensor | None, out: torch.Tensor | None):
+        """Checks what every form of attention takes: (ld_q, out, ld_o, lse, mask's address, its row stride)."""
+        dev, rows, nh = self._device, batch.rows, q.shape[1]
         ld_q = _rows(q, dev, rows, nh, self.head_dim, "q")
         if out is None:
             out = torch.empty(q.shape, dtype=_BF16, device=q.device)
@@ -184,6 +189,21 @@ class Kv8Cache:
                 raise ValueError(f"token_mask must be bytes [{batch.num_seqs}, at least {width}] on cuda:{dev}")
             mask = token_mask.data_ptr()
             ld_m = token_mask.stride(0) if token_mask.shape[0] > 1 else token_mask.shape[1]
+        return ld_q, out, ld_o, lse, mask, ld_m
+
+    def attention(self, batch: Kv8Batch, q: torch.Tensor, scale: float = 0.0, window: int = 0,
+                  token_mask: torch.Tensor | None = None, out: torch.Tensor | None = None, sinks: int = 0):
+        """Attention of the step's queries, bf16 [rows, num_heads, head_dim], after ``append``.  With a window, the
+        first ``sinks`` tokens of a sequence stay visible behind it.
+        Returns (o like q, dense; lse fp32 [rows, num_heads])."""
+        if q.dim() != 3:
+            raise ValueError("q must be [rows, num_heads, head_dim]")
+        dev = self._batch_device(batch)
+        if dev != _current_device():
+            with torch.cuda.device(dev):
+                return self.attention(batch, q, scale, window, token_mask, out, sinks)
+        nh = q.shape[1]
+        ld_q, out, ld_o, lse, mask, ld_m = self._step(batch, q, token_mask, out)
         key = (nh, self.num_kv_heads, self.block_tokens, self.head_dim)
         need = batch._ws_bytes.get(key)
         if need is None:
@@ -192,8 +212,40 @@ class Kv8Cache:
             need = batch._ws_bytes[key] = n.value
         stream = _stream(dev)
         ws = _scratch.get(need, dev, stream)
-        st = lib.glt_kv8_attention(self._p, batch._p, q.data_ptr(), ld_q, out.data_ptr(), ld_o, lse.data_ptr(), nh,
-                                   scale, window, mask, ld_m, ws.data_ptr(), need, stream)
+        if sinks:
+            st = lib.glt_kv8_window_attention(self._p, batch._p, q.data_ptr(), ld_q, out.data_ptr(), ld_o, lse.data_ptr(),
+                                              nh, scale, window, sinks, mask, ld_m, ws.data_ptr(), need, stream)
+        else:
+            st = lib.glt_kv8_attention(self._p, batch._p, q.data_ptr(), ld_q, out.data_ptr(), ld_o, lse.data_ptr(), nh,
+                                       scale, window, mask, ld_m, ws.data_ptr(), need, stream)
+        if st:
+            check(st)
+        return out, lse
+
+    def prefix_attention(self, batch: Kv8Batch, prefix: Kv8Prefix, q: torch.Tensor, scale: float = 0.0,
+                         token_mask: torch.Tensor | None = None, out: torch.Tensor | None = None):
+        """``attention`` in which every sequence of the batch is the prefix followed by its own tokens, which alone the
+        batch's tables and lengths (and ``token_mask``) describe."""
+        if q.dim() != 3:
+            raise ValueError("q must be [rows, num_heads, head_dim]")
+        dev = self._batch_device(batch)
+        if prefix._device != dev:
+            raise ValueError(f"the cache lies on cuda:{dev}, the prefix on cuda:{prefix._device}")
+        if dev != _current_device():
+            with torch.cuda.device(dev):
+                return self.prefix_attention(batch, prefix, q, scale, token_mask, out)
+        nh = q.shape[1]
+        ld_q, out, ld_o, lse, mask, ld_m = self._step(batch, q, token_mask, out)
+        key = (nh, self.num_kv_heads, self.block_tokens, self.head_dim, prefix.blocks.shape[0])
+        need = batch._ws_bytes.get(key)
+        if need is None:
+            n = C.c_int64()
+            check(lib.glt_kv8_prefix_attention_workspace(self._p, batch._p, prefix._p, nh, C.byref(n)))
+            need = batch._ws_bytes[key] = n.value
+        stream = _stream(dev)
+        ws = _scratch.get(need, dev, stream)
+        st = lib.glt_kv8_prefix_attention(self._p, batch._p, prefix._p, q.data_ptr(), ld_q, out.data_ptr(), ld_o,
+                                          lse.data_ptr(), nh, scale, mask, ld_m, ws.data_ptr(), need, stream)
         if st:
             check(st)
         return out, lse

@@ -308,6 +308,34 @@ GLT_API int glt_kv8_attention(const GltKv8Cache* cache, const GltKv8Batch* batch
                               int64_t ld_q, uint16_t* o, int64_t ld_o, float* lse, int num_heads,
                               float scale, int window, const uint8_t* token_mask, int64_t ld_mask,
                               void* workspace, int64_t workspace_bytes, void* stream);
+/* The same with a window (> 0) and `sinks` first tokens that stay visible behind it: the query at position p sees
+ * tokens t <= p with t < sinks or t > p - window.  window = 0 or sinks = 0 is glt_kv8_attention.  Table entries of
+ * blocks of which no query sees a token are not looked at, so that a long sequence may give back
+ * the blocks between its first tokens and its window.  Workspace: that of glt_kv8_attention. */
+GLT_API int glt_kv8_window_attention(const GltKv8Cache* cache, const GltKv8Batch* batch, const uint16_t* q,
+                                     int64_t ld_q, uint16_t* o, int64_t ld_o, float* lse, int num_heads,
+                                     float scale, int window, int sinks, const uint8_t* token_mask,
+                                     int64_t ld_mask, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* A prefix that all sequences of a batch share: `length` (dev [1], read on the device) tokens in blocks block_ids
+ * (dev [num_blocks]) of the same cache.  A length outside 0 .. num_blocks * block_tokens counts as 0, and a
+ * block id outside the pool is skipped; both set code 2 of the device error word.
+ * glt_kv8_prefix_attention: attention in which each sequence of the batch is the prefix followed by its own tokens
+ * (batch->lengths and block_table hold and count only those): a query sees the whole prefix and, of its own
+ * tokens, those that glt_kv8_attention without a window shows it (token_mask is for own tokens).
+ * The prefix's cache is read once for every 256 rows (token x head of a group) of a KV head, not once a sequence.
+ * workspace: glt_kv8_prefix_attention_workspace bytes, else as there. */
+typedef struct GltKv8Prefix {
+  int num_blocks;
+  const int32_t* block_ids; /* dev [num_blocks] */
+  const int32_t* length;    /* dev [1] */
+} GltKv8Prefix;
+GLT_API int glt_kv8_prefix_attention_workspace(const GltKv8Cache* cache, const GltKv8Batch* batch,
+                                               const GltKv8Prefix* prefix, int num_heads, int64_t* bytes);
+GLT_API int glt_kv8_prefix_attention(const GltKv8Cache* cache, const GltKv8Batch* batch, const GltKv8Prefix* prefix,
+                                     const uint16_t* q, int64_t ld_q, uint16_t* o, int64_t ld_o, float* lse,
+                                     int num_heads, float scale, const uint8_t* token_mask, int64_t ld_mask,
+                                     void* workspace, int64_t workspace_bytes, void* stream);
 /* The cached values of positions [start[b], start[b] + count) of each sequence
  * as fp32 [num_seqs, count, num_kv_heads, head_dim] (start = NULL: from 0);
  * positions the sequence does not hold after this step read as 0. */
