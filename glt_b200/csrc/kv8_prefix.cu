@@ -6,16 +6,19 @@
 // that share a KV head are the rows of tcgen05 products with it.
 //
 // A CTA (see kv8_prefix.cuh for its share of the work) goes through steps of 128 tokens:
-//   warps 8-15  copy the codes of the next step to registers, turn them into bf16, which holds codes exactly (8 bits of
-//               int8, 4 of e4m3), and lay K and V into shared memory as the products read them.
+//   warps 8-15  copy the codes of the next step to registers, turn them into f16, which holds codes exactly, and lay K
+//               and V into shared memory as the products read them.
 //   warp 16     issues the products: S = Q K^T, and O += P V with P in TMEM, as P was written over S.
 //   warps 0-7   softmax, a thread a query row, in two lanes of 128 rows with an S and an O each: the tensor core works
 //               for one lane while the other's softmax runs.  With more than 128 rows a KV head the lanes are two
 //               tiles of rows at the same tokens; else every second step of the same rows.
-// Q is bf16 as it came.  K's scale multiplies S in 32 bits.  V's scale multiplies the weight p in 32 bits, and what comes of it
-// is split into two bf16 numbers, p = hi + lo, of 16 bits together and the exponents of a float: whatever the scales of
-// different blocks are, each weight keeps its 16 bits.  It costs one product more than rounding p.
-// The sums of a row move to a new maximum only when it has grown by more than 2^8.
+// A query row is brought to f16 by a power of two, as in kv8_attention.cuh.  The scale of K multiplies S in 32 bits.  The
+// scale of V joins the exponent: a token counts 2^(s + log2 scale - ref) in the sum of values, ref a running
+// maximum of that exponent, so that f16 has what one token can add at most near its top whatever the scales of the blocks
+// are: 11 bits down to 2^-29 of the row's largest summand, and below an absolute 2^-40 of it.  (P as the sum
+// of two bf16 numbers needs no such reference, but half as many products and instructions again: 306 us where
+// this took XXX, 512 rows a KV head, 65537 tokens.)  Over 1 / scale, in 32 bits, the same numbers make the sum of weights.
+// The reference moves only when the maximum has grown by more than 2^8.
 #include <float.h>
 
 #include "kv8_attention.cuh"
@@ -26,7 +29,9 @@ namespace {
 constexpr int kSoftmaxWarps = 8, kDecodeWarps = 8;
 constexpr int kPrefixThreads = 32 * (kSoftmaxWarps + kDecodeWarps + 1);
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
-constexpr float kSlack = 8.f;   // base 2: how far weights may exceed 1
+// Base 2: how far summands may exceed the reference, and how far below f16's top (2^16) they stay with that.
+constexpr float kSlack = 8.f, kLift = 7.f;
+constexpr float kLeastScale = 0x1p-120f;   // of V: smaller ones count as 0, and weigh as 2^-60
 
 struct PrefixArgs {
   GltKv8Cache c;
@@ -39,9 +44,10 @@ struct PrefixArgs {
   unsigned int* err;
 };
 
-// Scales of a stage's groups of 16 tokens.  A block that is not in the pool has k = -1.
-struct PrefixNote {
-  float k[8], v[8];
+// Scales of a stage's groups of 16 tokens.  flags: bit g, the group's block is not in the pool; bit 8 + g, its values are 0.
+struct alignas(16) PrefixNote {
+  float k[8], log_v[8], inv_v[8];
+  int flags, pad[3];
 };
 
 template <int HD, int LANES>
@@ -85,22 +91,11 @@ __device__ __forceinline__ void umma_p(uint32_t d, uint32_t a_tmem, uint64_t b, 
       "r"(a_tmem), "l"(b), "r"(idesc), "r"(acc));
 }
 
-// Bytes 0, 1 (HI = 0) or 2, 3 of a word of codes as two bf16 numbers, exactly.  A byte c of two's complement is
-// (128 + its low seven bits) - (256 if negative, else 128), and both are bf16 numbers whose bits hold the byte's.
-template <int FMT, int HI>
-__device__ __forceinline__ uint32_t two_bf16(uint32_t w) {
-  uint32_t r;
-  if constexpr (FMT == GLT_KV8_INT8) {
-    const uint32_t x = __byte_perm(w ^ 0x80808080u, 0x43434343u, HI ? 0x4342 : 0x4140);
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x & 0xFF7FFF7Fu), "r"(x & 0xFF80FF80u));
-  } else {
-    const uint32_t h = e4m3x2_to_f16x2(HI ? w >> 16 : w & 0xFFFFu);
-    asm("{.reg .b16 lo, hi; .reg .f32 a, b; mov.b32 {lo, hi}, %1; cvt.f32.f16 a, lo; cvt.f32.f16 b, hi;"
-        " cvt.rn.bf16x2.f32 %0, b, a;}"
-        : "=r"(r)
-        : "r"(h));
-  }
-  return r;
+// Sixteen codes as f16 numbers, in two vectors.
+template <int FMT>
+__device__ __forceinline__ void sixteen_f16(const uint4& x, uint4& a, uint4& b) {
+  a = make_uint4(two_codes<FMT, 0>(x.x), two_codes<FMT, 1>(x.x), two_codes<FMT, 0>(x.y), two_codes<FMT, 1>(x.y));
+  b = make_uint4(two_codes<FMT, 0>(x.z), two_codes<FMT, 1>(x.z), two_codes<FMT, 0>(x.w), two_codes<FMT, 1>(x.w));
 }
 
 // Walks a CTA's run: unit `unit`, steps [s0, s1) of it.
@@ -127,7 +122,8 @@ struct PrefixRun {
 template <int HD, int FMT, int LANES>
 __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __grid_constant__ PrefixArgs a) {
   using L = PrefixSmem<HD, LANES>;
-  constexpr uint32_t kIdescS = tc::make_idesc(kPrefixStep, false, false), kIdescO = tc::make_idesc(HD, false, true);
+  constexpr uint32_t kBf16 = (1u << 7) | (1u << 10);   // operand types of a descriptor: f16 is 0
+  constexpr uint32_t kIdescS = tc::make_idesc(kPrefixStep, false, false) & ~kBf16, kIdescO = tc::make_idesc(HD, false, true) & ~kBf16;
   constexpr uint32_t kColO = 256;   // TMEM: S of lane 0, of lane 1 (128 columns each), O of lane 0, of lane 1
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-tc::smem_u32(smem_raw) & 1023u);   // the swizzle goes by address
@@ -153,7 +149,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
       tc::mbar_init(s_full + i, 1);
       tc::mbar_init(p_full + i, 4);
     }
-    tc::mbar_init(q_full, kSoftmaxWarps);
+    tc::mbar_init(q_full, 4 * LANES);
     tc::mbar_init(unit_done, 1);
     tc::mbar_init(drain, 1);
     abort = 0;
@@ -177,28 +173,45 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
     const int r = (warp & 3) * 32 + lane;                  // query row in the tile
     const uint32_t at = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_at = at + mine * 128, o_at = at + kColO + mine * 128;
-    const float unit_q = a.scale * 1.4426950408889634f;
     uint32_t s_phase = 0;
     int seg = 0, base = 0;   // steps before the unit's
     for (; run.on() && !abort; run.next(), ++seg) {
       const int kvh = run.unit % a.parts.kv_heads, pair = run.unit / a.parts.kv_heads;
-      // ---- queries.  LANES = 2: a thread its row; else two threads a row
+      // ---- queries: a thread its row, which one of the lanes lays out
+      float unit_q;   // takes S to log2 units
       {
-        const int row = LANES == 2 ? r : static_cast<int>(threadIdx.x) >> 1;
-        const int rho = (LANES == 2 ? pair * 2 + mine : pair) * kPrefixRows + row;
+        const int rho = (LANES == 2 ? pair * 2 + mine : pair) * kPrefixRows + r;
+        const bool on = rho < a.rows;
         const int tok = rho / a.group;
-        const uint16_t* src = a.q + static_cast<int64_t>(tok) * a.ld_q + (kvh * a.group + rho - tok * a.group) * HD;
-        uint8_t* dst = smem + (LANES == 2 ? mine * L::kQ : 0) + row * 128;
-        const int first = LANES == 2 ? 0 : (threadIdx.x & 1) * (HD / 16), count = LANES == 2 ? HD / 8 : HD / 16;
+        const uint4* src = reinterpret_cast<const uint4*>(a.q + static_cast<int64_t>(tok) * a.ld_q + (kvh * a.group + rho - tok * a.group) * HD);
+        float peak = 0.f;
+#pragma unroll 4
+        for (int c = 0; c < HD / 8; ++c) {
+          float f[8];
+          unpack8(on ? src[c] : make_uint4(0, 0, 0, 0), f);
 #pragma unroll
-        for (int i = 0; i < count; ++i) {
-          const int c = first + i;   // 8 channels
-          const uint4 x = rho < a.rows ? *reinterpret_cast<const uint4*>(src + c * 8) : make_uint4(0, 0, 0, 0);
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * (kPrefixRows * 128) + (((c & 7) ^ (row & 7)) << 4)) = x;
+          for (int j = 0; j < 8; ++j) peak = fmaxf(peak, fabsf(f[j]));
         }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(q_full);
+        // 2^e takes the largest magnitude to [2^13, 2^14)
+        auto power = [](int e) { return __int_as_float((e + 127) << 23); };   // 2^e, |e| < 127
+        int e = 0;
+        if (peak > 0.f && peak <= FLT_MAX) e = 13 - (static_cast<int>(__float_as_uint(peak) >> 23) - 127);
+        const float f1 = power(e >> 1), f2 = power(e - (e >> 1));   // 2^e may be out of range
+        unit_q = a.scale * 1.4426950408889634f * power(-(e >> 1)) * power(-(e - (e >> 1)));
+        if (LANES == 2 || mine == 0) {
+          uint8_t* dst = smem + (LANES == 2 ? mine * L::kQ : 0) + r * 128;
+#pragma unroll 4
+          for (int c = 0; c < HD / 8; ++c) {
+            float f[8];
+            unpack8(on ? src[c] : make_uint4(0, 0, 0, 0), f);
+            *reinterpret_cast<uint4*>(dst + (c >> 3) * (kPrefixRows * 128) + (((c & 7) ^ (r & 7)) << 4)) =
+                make_uint4(pack_f16x2(f[0] * f1 * f2, f[1] * f1 * f2), pack_f16x2(f[2] * f1 * f2, f[3] * f1 * f2),
+                           pack_f16x2(f[4] * f1 * f2, f[5] * f1 * f2), pack_f16x2(f[6] * f1 * f2, f[7] * f1 * f2));
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(q_full);
+        }
       }
       float m = -INFINITY, l = 0.f;
       bool any = false;
@@ -215,33 +228,35 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
         tc::tc_fence_after();
         const PrefixNote& note = notes[st];
         const int left = tokens - (run.s0 + i) * kPrefixStep;   // tokens of the step
-        float uk[8];
-        bool bad = false;
+        const int flags = note.flags;
+        const bool edge = left < kPrefixStep || flags != 0;
+        // Loops of 32 columns are not unrolled: with all roles' code unrolled, warps waited for instructions more than
+        // for anything else (a step took 10,400 cycles).
+        auto units = [&](int c) {   // of the two groups of 16; above 0, so that a masked -inf stays one
+          const float2 k = *reinterpret_cast<const float2*>(note.k + c / 16);
+          return make_float2(fmaxf(k.x * unit_q, 1e-37f), fmaxf(k.y * unit_q, 1e-37f));
+        };
+        auto scores = [&](int c, float (&v)[32]) {
+          tc::tmem_ld32(s_at + c, v);
+          if (edge) {
+            const int gone = flags >> (c / 16);
 #pragma unroll
-        for (int g = 0; g < 8; ++g) {
-          const float k = note.k[g];
-          bad |= k < 0.f;
-          uk[g] = fmaxf(k * unit_q, 1e-37f);   // above 0, so that a masked -inf stays one
-        }
-        const bool edge = bad || left < kPrefixStep;
-        // a masked score, of columns c .. c + 31
-        auto mask = [&](float (&v)[32], int c) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (c + j >= left || note.k[(c + j) >> 4] < 0.f) v[j] = -INFINITY;
+            for (int j = 0; j < 32; ++j)
+              if (c + j >= left || (gone >> (j / 16) & 1)) v[j] = -INFINITY;
+          }
         };
         float peak = -INFINITY;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < 128; c += 32) {
           float v[32];
-          tc::tmem_ld32(s_at + c, v);
-          if (edge) mask(v, c);
+          scores(c, v);
+          const float2 u = units(c), w = *reinterpret_cast<const float2*>(note.log_v + c / 16);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             float x[4] = {v[16 * h], v[16 * h + 1], v[16 * h + 2], v[16 * h + 3]};
 #pragma unroll
             for (int j = 4; j < 16; ++j) x[j & 3] = fmaxf(x[j & 3], v[16 * h + j]);
-            peak = fmaxf(peak, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) * uk[c / 16 + h]);
+            peak = fmaxf(peak, fmaf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), h ? u.y : u.x, h ? w.y : w.x));
           }
         }
         const bool grow = peak > m + kSlack || (m == -INFINITY && peak > m);
@@ -264,30 +279,33 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
           }
         }
         any = true;
-        const float ref = m == -INFINITY ? 0.f : m;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+        const float ref = kLift - (m == -INFINITY ? 0.f : m);
+#pragma unroll 1
         for (int c = 0; c < 128; c += 32) {
           float v[32];
-          tc::tmem_ld32(s_at + c, v);
-          if (edge) mask(v, c);
-          uint32_t hi[16], lo[16];
+          scores(c, v);
+          const float2 u = units(c), w = *reinterpret_cast<const float2*>(note.log_v + c / 16),
+                       inv = *reinterpret_cast<const float2*>(note.inv_v + c / 16);
+          uint32_t p[16];
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            const float sv = note.v[(c + j) >> 4];
-            const float p0 = ex2_approx(fmaf(v[j], uk[(c + j) >> 4], -ref));
-            const float p1 = ex2_approx(fmaf(v[j + 1], uk[(c + j) >> 4], -ref));
-            sum[j & 2] += p0;
-            sum[(j & 2) + 1] += p1;
-            const float w0 = p0 * sv, w1 = p1 * sv;
-            const uint32_t h = pack_bf16x2_rn(w0, w1);
-            hi[j >> 1] = h;
-            lo[j >> 1] = pack_bf16x2_rn(w0 - bf16_lo(h), w1 - bf16_hi(h));
+          for (int h = 0; h < 2; ++h) {
+            const float uh = h ? u.y : u.x, rh = ref + (h ? w.y : w.x);
+            float sum[2] = {0.f, 0.f};
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+              const float p0 = ex2_approx(fmaf(v[16 * h + j], uh, rh)), p1 = ex2_approx(fmaf(v[16 * h + j + 1], uh, rh));
+              sum[0] += p0;
+              sum[1] += p1;
+              p[8 * h + j / 2] = pack_f16x2(p0, p1);
+            }
+            l = fmaf(sum[0] + sum[1], h ? inv.y : inv.x, l);
+            if (edge && (flags >> (8 + c / 16 + h) & 1)) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) p[8 * h + j] = 0;
+            }
           }
-          tmem_st16(s_at + c, hi);        // over the scores just read: hi of 32 tokens, then lo
-          tmem_st16(s_at + c + 16, lo);
+          tmem_st16(s_at + c / 2, p);   // over scores that are read
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         tmem_wait_st();
         tc::tc_fence_before();
         __syncwarp();
@@ -311,10 +329,12 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
           for (int j = 0; j < 32; ++j) o[j] = 0.f;
         }
 #pragma unroll
-        for (int j = 0; j < 32; j += 4)
-          *reinterpret_cast<float4*>(out + row * HD + c + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+        for (int j = 0; j < 32; j += 8)
+          asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out + row * HD + c + j), "f"(o[j]),
+                       "f"(o[j + 1]), "f"(o[j + 2]), "f"(o[j + 3]), "f"(o[j + 4]), "f"(o[j + 5]), "f"(o[j + 6]), "f"(o[j + 7])
+                       : "memory");
       }
-      out[2 * kPrefixRows * HD + row] = m;
+      out[2 * kPrefixRows * HD + row] = m - kLift;
       out[2 * kPrefixRows * (HD + 1) + row] = l;
       tc::tc_fence_before();   // the next unit's products write O once P of its first step has come
       base += n;
@@ -343,6 +363,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
     };
     uint4 k[kMine], v[kMine];
     float note_k = 0.f, note_v = 0.f;
+    bool note_gone = false;
     auto address = [&](const PrefixRun& at, int s, int i) {
       const int t = s * kPrefixStep + tok0 + i * kTokenStep;
       return ((static_cast<int64_t>(ids[i]) * a.c.num_kv_heads + at.unit % a.parts.kv_heads) * bt + (t & (bt - 1))) * HD + chunk * 16;
@@ -358,9 +379,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
       if (tid >= 8) return;
       const bool in = note_id >= 0 && note_id < a.c.num_blocks;
       const int64_t hb = static_cast<int64_t>(in ? note_id : 0) * a.c.num_kv_heads + at.unit % a.parts.kv_heads;
-      note_k = in ? a.c.k_scale[hb] : note_id == -2 ? 0.f : -1.f;
+      note_k = in ? a.c.k_scale[hb] : 0.f;
       note_v = in ? a.c.v_scale[hb] : 0.f;
-      if (!in && note_id != -2 && at.on() && a.err) atomicOr(a.err, GLT_DEVERR_BAD_SHAPE);
+      note_gone = !in && note_id != -2;
+      if (note_gone && at.on() && a.err) atomicOr(a.err, GLT_DEVERR_BAD_SHAPE);
     };
     auto lay = [&](const uint4 (&x)[kMine], uint8_t* dst) {
 #pragma unroll
@@ -368,10 +390,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
         const int tok = tok0 + i * kTokenStep;
         uint8_t* row = dst + (chunk >> 2) * (kPrefixStep * 128) + tok * 128;
         const int c = 2 * (chunk & 3);
-        *reinterpret_cast<uint4*>(row + ((c ^ (tok & 7)) << 4)) = make_uint4(
-            two_bf16<FMT, 0>(x[i].x), two_bf16<FMT, 1>(x[i].x), two_bf16<FMT, 0>(x[i].y), two_bf16<FMT, 1>(x[i].y));
-        *reinterpret_cast<uint4*>(row + (((c + 1) ^ (tok & 7)) << 4)) = make_uint4(
-            two_bf16<FMT, 0>(x[i].z), two_bf16<FMT, 1>(x[i].z), two_bf16<FMT, 0>(x[i].w), two_bf16<FMT, 1>(x[i].w));
+        uint4 lo, hi;
+        sixteen_f16<FMT>(x[i], lo, hi);
+        *reinterpret_cast<uint4*>(row + ((c ^ (tok & 7)) << 4)) = lo;
+        *reinterpret_cast<uint4*>(row + (((c + 1) ^ (tok & 7)) << 4)) = hi;
       }
     };
     auto advance = [&]() {
@@ -386,30 +408,32 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
       load(run, step, v, a.c.v);
       load_note(run);
       for (int it = 0; !abort; ++it) {
-        // on to the next step, whose ids come now
-        advance();
-        load_ids(run, step);
         const int st = it % L::kStages;
         if (!__all_sync(0xffffffffu, tc::mbar_wait(empty + st, ((it / L::kStages) & 1) ^ 1, a.err, &abort))) {
           abort = 1;
           break;
         }
+        // on to the next step, whose ids come now
+        advance();
+        load_ids(run, step);
         uint8_t* dst = smem + L::kOffStages + st * L::kStage;
         if (tid < 8) {
+          const bool some = !(note_v < kLeastScale);
           notes[st].k[tid] = note_k;
-          notes[st].v[tid] = note_v;
+          notes[st].log_v[tid] = some ? log2f(note_v) : -60.f;
+          notes[st].inv_v[tid] = some ? 1.f / note_v : 0x1p60f;
+          const unsigned gone = __ballot_sync(0xFFu, note_gone), none = __ballot_sync(0xFFu, !some);
+          if (tid == 0) notes[st].flags = static_cast<int>(gone | none << 8);
         }
         lay(k, dst);
-        if (run.on()) load(run, step, k, a.c.k);
         lay(v, dst + L::kPart);
-        if (run.on()) {
-          load(run, step, v, a.c.v);
-          load_note(run);
-        }
-        fence_async_smem();
+        fence_async_smem();   // (it would wait for loads)
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(full + st);
         if (!run.on()) break;
+        load(run, step, k, a.c.k);
+        load(run, step, v, a.c.v);
+        load_note(run);
       }
     }
   } else if (lane == 0) {
@@ -445,9 +469,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
 #pragma unroll
         for (int j = 0; j < kPrefixStep / 16; ++j) {
           const uint64_t b = tc::make_sdesc(vv + j * 2048, kPrefixStep * 128, 1024);
-          const uint32_t pj = p + (j >> 1) * 32 + (j & 1) * 8;
-          umma_p(o, pj, b, kIdescO, !(first && j == 0));
-          umma_p(o, pj + 16, b, kIdescO, 1);
+          umma_p(o, p + 8 * j, b, kIdescO, !(first && j == 0));
         }
         if (LANES == 1 || ln == 1) tc::umma_commit(empty + st);
         return true;
@@ -511,7 +533,7 @@ PrefixParts plan_prefix(const GltKv8Cache& c, const GltKv8Batch& b, const GltKv8
   if (most < s.grid) s.grid = static_cast<int>(most);
   return s;
 }
-int64_t align16(int64_t n) { return (n + 15) / 16 * 16; }
+int64_t align32(int64_t n) { return (n + 31) / 32 * 32; }
 
 }  // namespace
 }  // namespace glt
@@ -522,7 +544,7 @@ extern "C" int glt_kv8_prefix_attention_workspace(const GltKv8Cache* cache, cons
   GLT_TRY(glt::check_heads(cache, batch, num_heads));
   GLT_TRY(glt::check_prefix(cache, prefix));
   *bytes = batch->rows > 0 && batch->max_new > 0
-               ? glt::align16(glt::plan(*cache, *batch, num_heads).bytes) +
+               ? glt::align32(glt::plan(*cache, *batch, num_heads).bytes) +
                      glt::plan_prefix(*cache, *batch, *prefix, num_heads).bytes(cache->head_dim)
                : 0;
   return GLT_OK;
@@ -542,7 +564,7 @@ extern "C" int glt_kv8_prefix_attention(const GltKv8Cache* cache, const GltKv8Ba
   GLT_TRY(glt::prepare(cache, batch, q, ld_q, o, ld_o, lse, num_heads, scale, 0, token_mask, ld_mask, workspace,
                        workspace_bytes, &a, &p));
   a.parts = glt::plan_prefix(*cache, *batch, *prefix, num_heads);
-  const int64_t own = glt::align16(p.bytes), need = own + a.parts.bytes(cache->head_dim);
+  const int64_t own = glt::align32(p.bytes), need = own + a.parts.bytes(cache->head_dim);
   if (workspace_bytes < need)
     return glt::fail(GLT_EINVAL, "kv8: workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
   a.parts.slots = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + own);
