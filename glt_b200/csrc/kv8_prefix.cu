@@ -6,9 +6,9 @@
 // that share a KV head are the rows of tcgen05 products with it.
 //
 // A CTA (see kv8_prefix.cuh for its share of the work) goes through steps of 128 tokens:
-//   warps 8-15  copy the codes of the next step to registers, turn them into f16, which holds codes exactly, and lay K
-//               and V into shared memory as the products read them.
-//   warp 16     issues the products: S = Q K^T, and O += P V with P in TMEM, as P was written over S.
+//   warp 13     looks up the blocks, copies their codes in bulk into a ring of 64 tokens of K or V each, and notes the scales.
+//   warps 8-11  turn codes into f16, which holds them exactly, and lay K and V out as the products read them.
+//   warp 12     issues the products: S = Q K^T, and O += P V with P in TMEM, as P was written over S.
 //   warps 0-7   softmax, a thread a query row, in two lanes of 128 rows with an S and an O each: the tensor core works
 //               for one lane while the other's softmax runs.  With more than 128 rows a KV head the lanes are two
 //               tiles of rows at the same tokens; else every second step of the same rows.
@@ -26,8 +26,9 @@
 namespace glt {
 namespace {
 
-constexpr int kSoftmaxWarps = 8, kDecodeWarps = 8;
-constexpr int kPrefixThreads = 32 * (kSoftmaxWarps + kDecodeWarps + 1);
+constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4, kIssueWarp = kSoftmaxWarps + kDecodeWarps;
+constexpr int kCopyWarp = kIssueWarp + 1;
+constexpr int kPrefixThreads = 32 * (kCopyWarp + 1);
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
 // Base 2: how far summands may exceed the reference, and how far below f16's top (2^16) they stay with that.
 constexpr float kSlack = 8.f, kLift = 7.f;
@@ -50,21 +51,46 @@ struct alignas(16) PrefixNote {
   int flags, pad[3];
 };
 
+constexpr int kRawTokens = 64;   // of K or V, in an element of the ring of codes
+constexpr int kNotes = 8;        // steps whose scales are held: more than can be under way
+
 template <int HD, int LANES>
 struct PrefixSmem {
   static constexpr int kQ = kPrefixRows * HD * 2;
-  static constexpr int kPart = kPrefixStep * HD * 2;   // K (or V) of a stage
-  static constexpr int kStage = 2 * kPart;
-  static constexpr int kStages = LANES == 2 ? 2 : 3;
-  static constexpr int kBars = 2 * kStages + 2 + 2 + 3;
-  static constexpr int kOffStages = LANES * kQ;
-  static constexpr int kOffNotes = kOffStages + kStages * kStage;
-  static constexpr int kOffBars = kOffNotes + kStages * static_cast<int>(sizeof(PrefixNote));
+  static constexpr int kPart = kPrefixStep * HD * 2;   // K (or V) of a step
+  static constexpr int kRaw = kRawTokens * HD;
+  static constexpr int kRaws = LANES == 2 ? 4 : 8;     // a step is four
+  static constexpr int kOffK = LANES * kQ;             // two steps each
+  static constexpr int kOffV = kOffK + 2 * kPart;
+  static constexpr int kOffRaw = kOffV + 2 * kPart;
+  static constexpr int kOffNotes = kOffRaw + kRaws * kRaw;
+  static constexpr int kOffBars = kOffNotes + kNotes * static_cast<int>(sizeof(PrefixNote));
+  static constexpr int kBars = 2 * kRaws + 8 + 4 + 3;
   static constexpr int kTotal = 1024 + kOffBars + kBars * 8 + 16;
 };
 static_assert(PrefixSmem<128, 1>::kTotal <= 232448 && PrefixSmem<128, 2>::kTotal <= 232448, "shared memory");
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+// 64 columns of the thread's lane.
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
+  uint32_t r[64];
+#pragma unroll
+  for (int h = 0; h < 64; h += 32)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[h + 0]), "=r"(r[h + 1]), "=r"(r[h + 2]), "=r"(r[h + 3]), "=r"(r[h + 4]), "=r"(r[h + 5]), "=r"(r[h + 6]),
+          "=r"(r[h + 7]), "=r"(r[h + 8]), "=r"(r[h + 9]), "=r"(r[h + 10]), "=r"(r[h + 11]), "=r"(r[h + 12]),
+          "=r"(r[h + 13]), "=r"(r[h + 14]), "=r"(r[h + 15]), "=r"(r[h + 16]), "=r"(r[h + 17]), "=r"(r[h + 18]),
+          "=r"(r[h + 19]), "=r"(r[h + 20]), "=r"(r[h + 21]), "=r"(r[h + 22]), "=r"(r[h + 23]), "=r"(r[h + 24]),
+          "=r"(r[h + 25]), "=r"(r[h + 26]), "=r"(r[h + 27]), "=r"(r[h + 28]), "=r"(r[h + 29]), "=r"(r[h + 30]),
+          "=r"(r[h + 31])
+        : "r"(taddr + h));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
@@ -82,6 +108,11 @@ __device__ __forceinline__ void tmem_st32f(uint32_t taddr, const float (&v)[32])
   }
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(dst)),
+               "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
+               : "memory");
+}
 // O (+)= P . V with P in TMEM.
 __device__ __forceinline__ void umma_p(uint32_t d, uint32_t a_tmem, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
@@ -128,10 +159,14 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-tc::smem_u32(smem_raw) & 1023u);   // the swizzle goes by address
   PrefixNote* notes = reinterpret_cast<PrefixNote*>(smem + L::kOffNotes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBars);   // a stage is laid out
-  uint64_t* empty = full + L::kStages;                                // a stage's products are done
-  uint64_t* s_full = empty + L::kStages;                              // [lane] S is there
-  uint64_t* p_full = s_full + 2;                                      // [lane] P is there
+  uint64_t* raw_full = reinterpret_cast<uint64_t*>(smem + L::kOffBars);
+  uint64_t* raw_empty = raw_full + L::kRaws;
+  uint64_t* k_full = raw_empty + L::kRaws;   // [2] K of a step is laid out, is read (and so on for V)
+  uint64_t* k_empty = k_full + 2;
+  uint64_t* v_full = k_empty + 2;
+  uint64_t* v_empty = v_full + 2;
+  uint64_t* s_full = v_empty + 2;            // [lane] S is there
+  uint64_t* p_full = s_full + 2;             // [lane] P is there
   uint64_t* q_full = p_full + 2;                                      // the unit's queries are laid out
   uint64_t* unit_done = q_full + 1;                                   // all products of the unit are done
   uint64_t* drain = unit_done + 1;
@@ -141,11 +176,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;");
   if (threadIdx.x == 0) {
-    for (int i = 0; i < L::kStages; ++i) {
-      tc::mbar_init(full + i, kDecodeWarps);
-      tc::mbar_init(empty + i, 1);
+    for (int i = 0; i < L::kRaws; ++i) {
+      tc::mbar_init(raw_full + i, 1);
+      tc::mbar_init(raw_empty + i, kDecodeWarps);
     }
     for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(k_full + i, kDecodeWarps);
+      tc::mbar_init(k_empty + i, 1);
+      tc::mbar_init(v_full + i, kDecodeWarps);
+      tc::mbar_init(v_empty + i, 1);
       tc::mbar_init(s_full + i, 1);
       tc::mbar_init(p_full + i, 4);
     }
@@ -155,7 +194,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
     abort = 0;
     tc::fence_mbar_init();
   }
-  if (warp == 16) {
+  if (warp == kIssueWarp) {
     tc::tmem_alloc(slot, 512);
     tc::tmem_relinquish();
   }
@@ -166,6 +205,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
   const int tokens = a.parts.tokens(blockIdx.x == 0 && threadIdx.x == 0 ? a.err : nullptr);
   const PrefixShares shares(a.parts, tokens);
   PrefixRun run(shares, blockIdx.x);
+  int copied = 0;   // elements of the ring that this thread has armed
 
   if (warp < kSoftmaxWarps) {
     // ------------------------------- softmax -------------------------------
@@ -184,14 +224,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
         const bool on = rho < a.rows;
         const int tok = rho / a.group;
         const uint4* src = reinterpret_cast<const uint4*>(a.q + static_cast<int64_t>(tok) * a.ld_q + (kvh * a.group + rho - tok * a.group) * HD);
-        float peak = 0.f;
-#pragma unroll 4
-        for (int c = 0; c < HD / 8; ++c) {
-          float f[8];
-          unpack8(on ? src[c] : make_uint4(0, 0, 0, 0), f);
+        uint4 x[HD / 8];   // at once: the loads' latency is the unit's
 #pragma unroll
-          for (int j = 0; j < 8; ++j) peak = fmaxf(peak, fabsf(f[j]));
-        }
+        for (int c = 0; c < HD / 8; ++c) x[c] = on ? src[c] : make_uint4(0, 0, 0, 0);
+        uint32_t tops = 0;   // of bf16 numbers without their signs, the larger is the larger integer
+#pragma unroll
+        for (int c = 0; c < HD / 8; ++c)
+          tops = __vmaxu2(tops, __vmaxu2(__vmaxu2(x[c].x & 0x7FFF7FFFu, x[c].y & 0x7FFF7FFFu),
+                                         __vmaxu2(x[c].z & 0x7FFF7FFFu, x[c].w & 0x7FFF7FFFu)));
+        const float peak = fmaxf(bf16_lo(tops), bf16_hi(tops));
         // 2^e takes the largest magnitude to [2^13, 2^14)
         auto power = [](int e) { return __int_as_float((e + 127) << 23); };   // 2^e, |e| < 127
         int e = 0;
@@ -200,10 +241,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
         unit_q = a.scale * 1.4426950408889634f * power(-(e >> 1)) * power(-(e - (e >> 1)));
         if (LANES == 2 || mine == 0) {
           uint8_t* dst = smem + (LANES == 2 ? mine * L::kQ : 0) + r * 128;
-#pragma unroll 4
+#pragma unroll
           for (int c = 0; c < HD / 8; ++c) {
             float f[8];
-            unpack8(on ? src[c] : make_uint4(0, 0, 0, 0), f);
+            unpack8(x[c], f);
             *reinterpret_cast<uint4*>(dst + (c >> 3) * (kPrefixRows * 128) + (((c & 7) ^ (r & 7)) << 4)) =
                 make_uint4(pack_f16x2(f[0] * f1 * f2, f[1] * f1 * f2), pack_f16x2(f[2] * f1 * f2, f[3] * f1 * f2),
                            pack_f16x2(f[4] * f1 * f2, f[5] * f1 * f2), pack_f16x2(f[6] * f1 * f2, f[7] * f1 * f2));
@@ -217,46 +258,51 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
       bool any = false;
       const int n = run.s1 - run.s0;
       for (int i = LANES == 2 ? 0 : mine; i < n; i += LANES == 2 ? 1 : 2) {
-        const int st = (base + i) % L::kStages;
-        // (the stage is long laid out when S is there: waited for so that its note is seen)
+        // (K is long laid out when S is there: waited for so that the step's note is seen)
         if (!__all_sync(0xffffffffu, tc::mbar_wait(s_full + mine, s_phase, a.err, &abort) &&
-                                         tc::mbar_wait(full + st, ((base + i) / L::kStages) & 1, a.err, &abort))) {
+                                         tc::mbar_wait(k_full + ((base + i) & 1), ((base + i) >> 1) & 1, a.err, &abort))) {
           abort = 1;
           break;
         }
         s_phase ^= 1;
         tc::tc_fence_after();
-        const PrefixNote& note = notes[st];
+        const PrefixNote& note = notes[(base + i) % kNotes];
         const int left = tokens - (run.s0 + i) * kPrefixStep;   // tokens of the step
         const int flags = note.flags;
         const bool edge = left < kPrefixStep || flags != 0;
-        // Loops of 32 columns are not unrolled: with all roles' code unrolled, warps waited for instructions more than
+        // Loops of 64 columns are not unrolled: with all roles' code unrolled, warps waited for instructions more than
         // for anything else (a step took 10,400 cycles).
-        auto units = [&](int c) {   // of the two groups of 16; above 0, so that a masked -inf stays one
-          const float2 k = *reinterpret_cast<const float2*>(note.k + c / 16);
-          return make_float2(fmaxf(k.x * unit_q, 1e-37f), fmaxf(k.y * unit_q, 1e-37f));
+        auto four = [](const float* p, float (&f)[4]) {   // of the groups of 16
+          const float4 x = *reinterpret_cast<const float4*>(p);
+          f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w;
         };
-        auto scores = [&](int c, float (&v)[32]) {
-          tc::tmem_ld32(s_at + c, v);
+        auto units = [&](int c, float (&u)[4]) {
+          four(note.k + c / 16, u);
+#pragma unroll
+          for (int h = 0; h < 4; ++h) u[h] = fmaxf(u[h] * unit_q, 1e-37f);   // above 0, so that a masked -inf stays one
+        };
+        auto scores = [&](int c, float (&v)[64]) {
+          tmem_ld64(s_at + c, v);
           if (edge) {
             const int gone = flags >> (c / 16);
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
+            for (int j = 0; j < 64; ++j)
               if (c + j >= left || (gone >> (j / 16) & 1)) v[j] = -INFINITY;
           }
         };
         float peak = -INFINITY;
 #pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
-          float v[32];
+        for (int c = 0; c < 128; c += 64) {
+          float v[64], u[4], w[4];
           scores(c, v);
-          const float2 u = units(c), w = *reinterpret_cast<const float2*>(note.log_v + c / 16);
+          units(c, u);
+          four(note.log_v + c / 16, w);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < 4; ++h) {
             float x[4] = {v[16 * h], v[16 * h + 1], v[16 * h + 2], v[16 * h + 3]};
 #pragma unroll
             for (int j = 4; j < 16; ++j) x[j & 3] = fmaxf(x[j & 3], v[16 * h + j]);
-            peak = fmaxf(peak, fmaf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), h ? u.y : u.x, h ? w.y : w.x));
+            peak = fmaxf(peak, fmaf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), u[h], w[h]));
           }
         }
         const bool grow = peak > m + kSlack || (m == -INFINITY && peak > m);
@@ -281,30 +327,35 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
         any = true;
         const float ref = kLift - (m == -INFINITY ? 0.f : m);
 #pragma unroll 1
-        for (int c = 0; c < 128; c += 32) {
-          float v[32];
+        for (int c = 0; c < 128; c += 64) {
+          float v[64], u[4], w[4], inv[4];
           scores(c, v);
-          const float2 u = units(c), w = *reinterpret_cast<const float2*>(note.log_v + c / 16),
-                       inv = *reinterpret_cast<const float2*>(note.inv_v + c / 16);
-          uint32_t p[16];
+          units(c, u);
+          four(note.log_v + c / 16, w);
+          four(note.inv_v + c / 16, inv);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float uh = h ? u.y : u.x, rh = ref + (h ? w.y : w.x);
-            float sum[2] = {0.f, 0.f};
+          for (int half = 0; half < 2; ++half) {
+            uint32_t p[16];
 #pragma unroll
-            for (int j = 0; j < 16; j += 2) {
-              const float p0 = ex2_approx(fmaf(v[16 * h + j], uh, rh)), p1 = ex2_approx(fmaf(v[16 * h + j + 1], uh, rh));
-              sum[0] += p0;
-              sum[1] += p1;
-              p[8 * h + j / 2] = pack_f16x2(p0, p1);
+            for (int g = 0; g < 2; ++g) {
+              const int h = 2 * half + g;
+              const float uh = u[h], rh = ref + w[h];
+              float sum[2] = {0.f, 0.f};
+#pragma unroll
+              for (int j = 0; j < 16; j += 2) {
+                const float p0 = ex2_approx(fmaf(v[16 * h + j], uh, rh)), p1 = ex2_approx(fmaf(v[16 * h + j + 1], uh, rh));
+                sum[0] += p0;
+                sum[1] += p1;
+                p[8 * g + j / 2] = pack_f16x2(p0, p1);
+              }
+              l = fmaf(sum[0] + sum[1], inv[h], l);
+              if (edge && (flags >> (8 + c / 16 + h) & 1)) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) p[8 * g + j] = 0;
+              }
             }
-            l = fmaf(sum[0] + sum[1], h ? inv.y : inv.x, l);
-            if (edge && (flags >> (8 + c / 16 + h) & 1)) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) p[8 * h + j] = 0;
-            }
+            tmem_st16(s_at + c / 2 + 16 * half, p);   // over scores that are read
           }
-          tmem_st16(s_at + c / 2, p);   // over scores that are read
         }
         tmem_wait_st();
         tc::tc_fence_before();
@@ -339,139 +390,152 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
       tc::tc_fence_before();   // the next unit's products write O once P of its first step has come
       base += n;
     }
-  } else if (warp < kSoftmaxWarps + kDecodeWarps) {
+  } else if (warp < kIssueWarp) {
     // ------------------------------- codes ---------------------------------
-    constexpr int kChunks = HD / 16;                                    // 16 channels of a token
-    constexpr int kMine = kPrefixStep * kChunks / kDecodeThreads;       // of a thread, of K and of V
-    constexpr int kTokenStep = kDecodeThreads / kChunks;                // tokens between two of them
+    constexpr int kChunks = HD / 16;                                   // 16 channels of a token
+    constexpr int kMine = kRawTokens * kChunks / kDecodeThreads;       // of a thread, of an element of the ring
     const int tid = threadIdx.x - 32 * kSoftmaxWarps;
-    const int tok0 = tid / kChunks, chunk = tid % kChunks;
-    const int bt = a.c.block_tokens, bt_log = 31 - __clz(bt);
-    int step = run.on() ? run.s0 : 0;
-    // block ids are loaded a step before the codes, the codes a step before they are laid out
-    int ids[kMine], note_id = -1;
-    auto load_ids = [&](const PrefixRun& at, int s) {
+    const int chunk = tid % kChunks, tok0 = tid / kChunks;
+    int it = 0, raw = 0;
+    uint32_t raw_phase = 0;
+    // The step's K or V; tokens that are not there become 0 (P is 0 there, and 0 times a NaN would not be).
+    auto lay = [&](uint8_t* dst, int left) {
+      int flags = 0;
+#pragma unroll 1
+      for (int u = 0; u < kPrefixStep; u += kRawTokens) {
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(raw_full + raw, raw_phase, a.err, &abort))) return false;
+        if (u == 0) flags = notes[it % kNotes].flags;
+        const uint8_t* src = smem + L::kOffRaw + raw * L::kRaw + tid * 16;
+        uint4 x[kMine];
 #pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int t = s * kPrefixStep + tok0 + i * kTokenStep;
-        ids[i] = at.on() && t < tokens ? a.block_ids[t >> bt_log] : -1;
-      }
-      if (tid < 8) {
-        const int t = s * kPrefixStep + tid * 16;
-        note_id = at.on() && t < tokens ? a.block_ids[t >> bt_log] : -2;
-      }
-    };
-    uint4 k[kMine], v[kMine];
-    float note_k = 0.f, note_v = 0.f;
-    bool note_gone = false;
-    auto address = [&](const PrefixRun& at, int s, int i) {
-      const int t = s * kPrefixStep + tok0 + i * kTokenStep;
-      return ((static_cast<int64_t>(ids[i]) * a.c.num_kv_heads + at.unit % a.parts.kv_heads) * bt + (t & (bt - 1))) * HD + chunk * 16;
-    };
-    auto load = [&](const PrefixRun& at, int s, uint4 (&x)[kMine], const uint8_t* pool) {
+        for (int i = 0; i < kMine; ++i) x[i] = *reinterpret_cast<const uint4*>(src + i * (kDecodeThreads * 16));
 #pragma unroll
-      for (int i = 0; i < kMine; ++i)
-        x[i] = ids[i] >= 0 && ids[i] < a.c.num_blocks
-                   ? *reinterpret_cast<const uint4*>(pool + address(at, s, i))
-                   : (FMT == GLT_KV8_INT8 ? make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u) : make_uint4(0, 0, 0, 0));
-    };
-    auto load_note = [&](const PrefixRun& at) {
-      if (tid >= 8) return;
-      const bool in = note_id >= 0 && note_id < a.c.num_blocks;
-      const int64_t hb = static_cast<int64_t>(in ? note_id : 0) * a.c.num_kv_heads + at.unit % a.parts.kv_heads;
-      note_k = in ? a.c.k_scale[hb] : 0.f;
-      note_v = in ? a.c.v_scale[hb] : 0.f;
-      note_gone = !in && note_id != -2;
-      if (note_gone && at.on() && a.err) atomicOr(a.err, GLT_DEVERR_BAD_SHAPE);
-    };
-    auto lay = [&](const uint4 (&x)[kMine], uint8_t* dst) {
-#pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int tok = tok0 + i * kTokenStep;
-        uint8_t* row = dst + (chunk >> 2) * (kPrefixStep * 128) + tok * 128;
-        const int c = 2 * (chunk & 3);
-        uint4 lo, hi;
-        sixteen_f16<FMT>(x[i], lo, hi);
-        *reinterpret_cast<uint4*>(row + ((c ^ (tok & 7)) << 4)) = lo;
-        *reinterpret_cast<uint4*>(row + (((c + 1) ^ (tok & 7)) << 4)) = hi;
+        for (int i = 0; i < kMine; ++i) {
+          const int tok = u + tok0 + i * (kDecodeThreads / kChunks);
+          uint4 lo, hi;
+          sixteen_f16<FMT>(x[i], lo, hi);
+          if (tok >= left || (flags >> (tok >> 4) & 1)) lo = hi = make_uint4(0, 0, 0, 0);
+          uint8_t* row = dst + (chunk >> 2) * (kPrefixStep * 128) + tok * 128;
+          const int c = 2 * (chunk & 3);
+          *reinterpret_cast<uint4*>(row + ((c ^ (tok & 7)) << 4)) = lo;
+          *reinterpret_cast<uint4*>(row + (((c + 1) ^ (tok & 7)) << 4)) = hi;
+        }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(raw_empty + raw);
+        if (++raw == L::kRaws) {
+          raw = 0;
+          raw_phase ^= 1;
+        }
       }
+      fence_async_smem();
+      __syncwarp();
+      return true;
     };
-    auto advance = [&]() {
-      if (++step == run.s1) {
-        run.next();
-        step = run.on() ? run.s0 : 0;
-      }
-    };
-    if (run.on()) {
-      load_ids(run, step);
-      load(run, step, k, a.c.k);
-      load(run, step, v, a.c.v);
-      load_note(run);
-      for (int it = 0; !abort; ++it) {
-        const int st = it % L::kStages;
-        if (!__all_sync(0xffffffffu, tc::mbar_wait(empty + st, ((it / L::kStages) & 1) ^ 1, a.err, &abort))) {
+    for (; run.on() && !abort; run.next())
+      for (int step = run.s0; step < run.s1; ++step, ++it) {
+        const int slot = it & 1, left = tokens - step * kPrefixStep;
+        const uint32_t free_phase = ((it >> 1) & 1) ^ 1;
+        bool ok = __all_sync(0xffffffffu, tc::mbar_wait(k_empty + slot, free_phase, a.err, &abort)) &&
+                  lay(smem + L::kOffK + slot * L::kPart, left);
+        if (ok && lane == 0) tc::mbar_arrive(k_full + slot);
+        ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(v_empty + slot, free_phase, a.err, &abort)) &&
+             lay(smem + L::kOffV + slot * L::kPart, left);
+        if (ok && lane == 0) tc::mbar_arrive(v_full + slot);
+        if (!ok) {
           abort = 1;
           break;
         }
-        // on to the next step, whose ids come now
-        advance();
-        load_ids(run, step);
-        uint8_t* dst = smem + L::kOffStages + st * L::kStage;
-        if (tid < 8) {
-          const bool some = !(note_v < kLeastScale);
-          notes[st].k[tid] = note_k;
-          notes[st].log_v[tid] = some ? log2f(note_v) : -60.f;
-          notes[st].inv_v[tid] = some ? 1.f / note_v : 0x1p60f;
-          const unsigned gone = __ballot_sync(0xFFu, note_gone), none = __ballot_sync(0xFFu, !some);
-          if (tid == 0) notes[st].flags = static_cast<int>(gone | none << 8);
-        }
-        lay(k, dst);
-        lay(v, dst + L::kPart);
-        fence_async_smem();   // (it would wait for loads)
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(full + st);
-        if (!run.on()) break;
-        load(run, step, k, a.c.k);
-        load(run, step, v, a.c.v);
-        load_note(run);
       }
-    }
-  } else if (lane == 0) {
+  } else if (warp == kCopyWarp) {
+    // ------------------------------- copies --------------------------------
+    const int bt = a.c.block_tokens, bt_log = 31 - __clz(bt);
+    const int piece = min(bt, kRawTokens);   // tokens of a copy
+    int it = 0, raw = 0;
+    uint32_t raw_phase = 1;
+    // lane g < 8: the block of tokens 16 g .. of a step, read a step ahead
+    auto there = [&](int step) { return lane < 8 && step * kPrefixStep + 16 * lane < tokens; };
+    auto block = [&](int step) { return there(step) ? a.block_ids[(step * kPrefixStep + 16 * lane) >> bt_log] : -1; };
+    int id = run.on() ? block(run.s0) : -1;
+    for (; run.on() && !abort; run.next())
+      for (int step = run.s0; step < run.s1; ++step, ++it) {
+        const int kvh = run.unit % a.parts.kv_heads;
+        const bool in = id >= 0 && id < a.c.num_blocks, gone = !in && there(step);
+        const int64_t hb = in ? static_cast<int64_t>(id) * a.c.num_kv_heads + kvh : 0;
+        const float ks = in ? a.c.k_scale[hb] : 0.f, vs = in ? a.c.v_scale[hb] : 0.f;
+        if (gone && a.err) atomicOr(a.err, GLT_DEVERR_BAD_SHAPE);
+        const bool more = step + 1 < run.s1;   // (a following unit begins with step 0)
+        id = more || run.at + (run.s1 - run.s0) < run.end ? block(more ? step + 1 : 0) : -1;
+        bool ok = true;
+        for (int part = 0; ok && part < 4; ++part) {   // K, K, V, V
+          const int u = (part & 1) * kRawTokens;
+          ok = __all_sync(0xffffffffu, tc::mbar_wait(raw_empty + raw, raw_phase, a.err, &abort));
+          if (!ok) break;
+          if (part == 0) {
+            const bool some = !(vs < kLeastScale);
+            const unsigned lost = __ballot_sync(0xffffffffu, gone), none = __ballot_sync(0xffffffffu, lane < 8 && !some);
+            PrefixNote& note = notes[it % kNotes];
+            if (lane < 8) {
+              note.k[lane] = ks;
+              note.log_v[lane] = some ? log2f(vs) : -60.f;
+              note.inv_v[lane] = some ? 1.f / vs : 0x1p60f;
+            }
+            if (lane == 0) note.flags = static_cast<int>(lost | none << 8);
+          }
+          // one lane for each copy: that of the copy's first 16 tokens
+          const int t = 16 * lane - u;   // in the element
+          const bool mine = in && t >= 0 && t < kRawTokens && t % piece == 0;
+          const int copies = __popc(__ballot_sync(0xffffffffu, mine));
+          if (lane == 0) tc::mbar_arrive_expect_tx(raw_full + raw, copies * piece * HD);
+          __syncwarp();
+          if (mine)
+            bulk_load(smem + L::kOffRaw + raw * L::kRaw + t * HD,
+                      (part < 2 ? a.c.k : a.c.v) + ((hb << bt_log) + ((step * kPrefixStep + 16 * lane) & (bt - 1))) * HD, piece * HD,
+                      raw_full + raw);
+          ++copied;
+          if (++raw == L::kRaws) {
+            raw = 0;
+            raw_phase ^= 1;
+          }
+        }
+        if (!ok) {
+          abort = 1;
+          break;
+        }
+      }
+  } else if (warp == kIssueWarp && lane == 0) {
     // ------------------------------- products ------------------------------
     uint32_t p_phase[2] = {0, 0};
     bool ok = true;
     int base = 0;   // steps before the unit's
-    const uint32_t q_at = tc::smem_u32(smem), st_at = tc::smem_u32(smem + L::kOffStages);
+    const uint32_t q_at = tc::smem_u32(smem), k_at = tc::smem_u32(smem + L::kOffK), v_at = tc::smem_u32(smem + L::kOffV);
     for (int seg = 0; ok && run.on() && !abort; run.next(), ++seg) {
       const int steps = run.s1 - run.s0, n = LANES * steps;   // products of a lane and a step
       ok = tc::mbar_wait(q_full, seg & 1, a.err, &abort);
       auto scores = [&](int i) {
-        const int step = base + (LANES == 2 ? i >> 1 : i), ln = i & 1, st = step % L::kStages;
-        if (LANES == 1 || ln == 0) {
-          if (!tc::mbar_wait(full + st, (step / L::kStages) & 1, a.err, &abort)) return false;
-        }
+        const int step = base + (LANES == 2 ? i >> 1 : i), ln = i & 1, slot = step & 1;
+        if ((LANES == 1 || ln == 0) && !tc::mbar_wait(k_full + slot, (step >> 1) & 1, a.err, &abort)) return false;
         tc::tc_fence_after();
-        const uint32_t q = q_at + (LANES == 2 ? ln * L::kQ : 0), kk = st_at + st * L::kStage;
+        const uint32_t q = q_at + (LANES == 2 ? ln * L::kQ : 0), kk = k_at + slot * L::kPart;
 #pragma unroll
         for (int j = 0; j < HD / 16; ++j)
           tc::umma_bf16(tmem + ln * 128, tc::desc_kmajor(q + (j >> 2) * (kPrefixRows * 128), j & 3),
                         tc::desc_kmajor(kk + (j >> 2) * (kPrefixStep * 128), j & 3), kIdescS, j > 0);
         tc::umma_commit(s_full + ln);
+        if (LANES == 1 || ln == 1) tc::umma_commit(k_empty + slot);
         return true;
       };
       auto values = [&](int i) {
-        const int step = base + (LANES == 2 ? i >> 1 : i), ln = i & 1, st = step % L::kStages;
+        const int step = base + (LANES == 2 ? i >> 1 : i), ln = i & 1, slot = step & 1;
+        if ((LANES == 1 || ln == 0) && !tc::mbar_wait(v_full + slot, (step >> 1) & 1, a.err, &abort)) return false;
         if (!tc::mbar_wait(p_full + ln, p_phase[ln], a.err, &abort)) return false;
         p_phase[ln] ^= 1;
         tc::tc_fence_after();
-        const uint32_t vv = st_at + st * L::kStage + L::kPart, p = tmem + ln * 128, o = tmem + kColO + ln * 128;
+        const uint32_t vv = v_at + slot * L::kPart, p = tmem + ln * 128, o = tmem + kColO + ln * 128;
         const bool first = i < 2;
 #pragma unroll
-        for (int j = 0; j < kPrefixStep / 16; ++j) {
-          const uint64_t b = tc::make_sdesc(vv + j * 2048, kPrefixStep * 128, 1024);
-          umma_p(o, p + 8 * j, b, kIdescO, !(first && j == 0));
-        }
-        if (LANES == 1 || ln == 1) tc::umma_commit(empty + st);
+        for (int j = 0; j < kPrefixStep / 16; ++j)
+          umma_p(o, p + 8 * j, tc::make_sdesc(vv + j * 2048, kPrefixStep * 128, 1024), kIdescO, !(first && j == 0));
+        if (LANES == 1 || ln == 1) tc::umma_commit(v_empty + slot);
         return true;
       };
       for (int i = 0; ok && i <= n; ++i) {
@@ -485,7 +549,14 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
   }
   tc::tc_fence_before();
   __syncthreads();
-  if (warp == 16) {
+  if (warp == kCopyWarp && lane == 0 && abort) {
+    // copies still under way end before the shared memory does
+    for (int d = 0; d < L::kRaws && d < copied; ++d) {
+      const int j = copied - 1 - d;
+      tc::mbar_wait(raw_full + j % L::kRaws, (j / L::kRaws) & 1, a.err);
+    }
+  }
+  if (warp == kIssueWarp) {
     tc::tc_fence_after();
     if (abort) {
       // no product may still write TMEM when it is given back
