@@ -43,7 +43,7 @@
 
 #include <type_traits>
 
-#include "kv8_prefix.cuh"
+#include "kv8.cuh"
 
 namespace glt {
 namespace {
@@ -59,7 +59,7 @@ constexpr int kCtasPerSm = 2;   // three, with smaller rings, took 108 us for th
 constexpr int kUnitCost = 12;
 
 // kPlain: all earlier tokens, or those of a window.  kSinks: of a window and the first `sinks` tokens.
-// kPrefix: all earlier tokens, joined with what kv8_prefix_kernel left of the prefix that all sequences share.
+// kPrefix: all earlier tokens, in 32 bits and not divided by the sum of weights, for a join with a prefix's parts.
 enum class Mode { kPlain, kSinks, kPrefix };
 
 struct AttnArgs {
@@ -77,8 +77,8 @@ struct AttnArgs {
   int64_t ld_mask;
   void* workspace;
   unsigned int* err;
-  int sinks;          // kSinks
-  PrefixParts parts;  // kPrefix
+  int sinks;    // kSinks
+  float* own;   // kPrefix: dev [rows, num_heads, head_dim] sums of values, then [rows, num_heads] maxima (base 2) and sums of weights
 };
 
 // What one sequence has to do: `steps` steps from token `lo` on (kSinks: the first `head` of them from token 0 on, the
@@ -311,6 +311,9 @@ __device__ __forceinline__ uint32_t two_codes(uint32_t w) {
   }
 }
 
+// 2^(m - top) for partial results: weights that saw nothing are 0 (or NaN) already.
+__device__ __forceinline__ float join_factor(float m, float top) { return top == -INFINITY ? 1.f : ex2_approx(m - top); }
+
 // Four channels of a query row from their sum z, the row's maximum (base 2) and sum of
 // weights.  A row that saw nothing has weight 0 and gives 0; NaN stays NaN.
 template <Mode M>
@@ -318,7 +321,12 @@ __device__ __forceinline__ void write_out(const AttnArgs& a, int row0, int r, in
                                           float top, float sum) {
   const int i = r / a.group, head = kvh * a.group + r - i * a.group;
   const int64_t tok = row0 + i;
-  if (M == Mode::kPrefix) join_prefix(a.parts, static_cast<int>(tok) * a.group + r - i * a.group, kvh, hd, d, z, top, sum);
+  if (M == Mode::kPrefix) {
+    const int64_t at = tok * a.nh + head;
+    *reinterpret_cast<float4*>(a.own + at * hd + d) = z;
+    if (d == 0) *reinterpret_cast<float2*>(a.own + static_cast<int64_t>(a.b.rows) * a.nh * hd + 2 * at) = make_float2(top, sum);
+    return;
+  }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   *reinterpret_cast<uint2*>(a.o + tok * a.ld_o + static_cast<int64_t>(head) * hd + d) =
       make_uint2(pack_bf16x2_rn(z.x * inv, z.y * inv), pack_bf16x2_rn(z.z * inv, z.w * inv));
@@ -374,7 +382,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
   const Shares shares = find_run<ROWS, M>(a, scan);
   const Workspace ws(a.workspace, gridDim.x, ROWS, HD);
   if (blockIdx.x == 0 && threadIdx.x == 0) *ws.ctas = shares.ctas;
-  if (scan.run.end <= scan.run.begin) return;
+  if (scan.run.end <= scan.run.begin) {
+    if (M == Mode::kPrefix) asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
 
   // The copies run kStages steps ahead of the arithmetic, and the block ids one step ahead of
   // the copies: `ld` stands on the next step to copy, whose ids are on their way.
@@ -860,7 +871,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
           }
     }
     __syncthreads();
-    if (M == Mode::kPrefix) asm volatile("griddepcontrol.wait;" ::: "memory");   // the prefix's parts
     float* slot = ws.slots + static_cast<int64_t>(slot_index) * (ROWS * HD + 2 * ROWS);
     for (int i = threadIdx.x; i < rows * (HD / 4); i += kThreads) {
       const int r = i / (HD / 4), d = i % (HD / 4) * 4;
@@ -890,8 +900,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
     __syncthreads();   // the join buffers are free again
     ++done;
   }
-  // (the join, which waits for this kernel, reads them too)
-  if (M == Mode::kPrefix) asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (M == Mode::kPrefix) asm volatile("griddepcontrol.wait;" ::: "memory");   // who waits for this kernel waits for the prefix's
   if (threadIdx.x == 0) ws.tasks[blockIdx.x] = task;
   wait_groups<0>();
   // after a lost copy: the copies still under way end before the shared memory does
@@ -911,6 +920,7 @@ template <int HD, int NT, Mode M>
 __global__ void __launch_bounds__(kThreads) kv8_join_kernel(const __grid_constant__ AttnArgs a, int grid) {
   constexpr int ROWS = 8 * NT, kSlot = ROWS * HD + 2 * ROWS;
   const Workspace ws(a.workspace, grid, ROWS, HD);
+  if (M == Mode::kPrefix) asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int ctas = *ws.ctas;
   const JoinTask task = ws.tasks[blockIdx.x];   // read before it is known to be one: within the workspace
@@ -1002,7 +1012,7 @@ int launch(const AttnArgs& a, int grid, cudaStream_t st) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  if (M == Mode::kPrefix) {   // starts while the prefix's kernel runs, and waits for its end before it joins
+  if (M == Mode::kPrefix) {   // starts while the prefix's kernel runs
     cfg.gridDim = dim3(grid);
     cfg.dynamicSmemBytes = bytes;
     cfg.numAttrs = 1;

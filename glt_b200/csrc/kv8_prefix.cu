@@ -6,9 +6,10 @@
 // that share a KV head are the rows of tcgen05 products with it.
 //
 // A CTA (see kv8_prefix.cuh for its share of the work) goes through steps of 128 tokens:
-//   warp 13     looks up the blocks, copies their codes in bulk into a ring of 64 tokens of K or V each, and notes the scales.
+//   warp 14     looks up the blocks, copies their codes in bulk into a ring of 64 tokens of K or V each, and notes the scales.
 //   warps 8-11  turn codes into f16, which holds them exactly, and lay K and V out as the products read them.
-//   warp 12     issues the products: S = Q K^T, and O += P V with P in TMEM, as P was written over S.
+//   warps 12-13 issue the products of a lane each: S = Q K^T, and O += P V with P in TMEM, as P was written over S.  (From one
+//               warp, the tensor cores ran dry whenever it went from one barrier to the next.)
 //   warps 0-7   softmax, a thread a query row, in two lanes of 128 rows with an S and an O each: the tensor core works
 //               for one lane while the other's softmax runs.  With more than 128 rows a KV head the lanes are two
 //               tiles of rows at the same tokens; else every second step of the same rows.
@@ -18,20 +19,24 @@
 // are: 11 bits down to 2^-29 of the row's largest summand, and below an absolute 2^-40 of it.  (P as the sum
 // of two bf16 numbers needs no such reference, but half as many products and instructions again: 306 us where
 // this took XXX, 512 rows a KV head, 65537 tokens.)  Over 1 / scale, in 32 bits, the same numbers make the sum of weights.
-// The reference moves only when the maximum has grown by more than 2^8.
+// The reference moves only when the weights come near f16's top.
 #include <float.h>
 
+#include <algorithm>
+
 #include "kv8_attention.cuh"
+#include "kv8_prefix.cuh"
 
 namespace glt {
 namespace {
 
 constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4, kIssueWarp = kSoftmaxWarps + kDecodeWarps;
-constexpr int kCopyWarp = kIssueWarp + 1;
+constexpr int kCopyWarp = kIssueWarp + 2;   // an issuing warp for each lane
 constexpr int kPrefixThreads = 32 * (kCopyWarp + 1);
+constexpr int kHalf = 64;   // tokens of an S
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
-// Base 2: how far summands may exceed the reference, and how far below f16's top (2^16) they stay with that.
-constexpr float kSlack = 8.f, kLift = 7.f;
+constexpr float kLift = 7.f;          // base 2: what the reference counts in f16, whose top is 2^16
+constexpr float kMostSum = 0x1p15f;   // of 16 tokens, before the reference moves
 constexpr float kLeastScale = 0x1p-120f;   // of V: smaller ones count as 0, and weigh as 2^-60
 
 struct PrefixArgs {
@@ -65,7 +70,7 @@ struct PrefixSmem {
   static constexpr int kOffRaw = kOffV + 2 * kPart;
   static constexpr int kOffNotes = kOffRaw + kRaws * kRaw;
   static constexpr int kOffBars = kOffNotes + kNotes * static_cast<int>(sizeof(PrefixNote));
-  static constexpr int kBars = 2 * kRaws + 8 + 4 + 3;
+  static constexpr int kBars = 2 * kRaws + 8 + 8 + 2 + 3;
   static constexpr int kTotal = 1024 + kOffBars + kBars * 8 + 16;
 };
 static_assert(PrefixSmem<128, 1>::kTotal <= 232448 && PrefixSmem<128, 2>::kTotal <= 232448, "shared memory");
@@ -91,6 +96,28 @@ __device__ __forceinline__ void tmem_ld64(uint32_t taddr, float (&v)[64]) {
 #pragma unroll
   for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
+// Two floats in one instruction.
+__device__ __forceinline__ uint64_t two_floats(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float low(uint64_t x) { return __uint_as_float(static_cast<uint32_t>(x)); }
+__device__ __forceinline__ float high(uint64_t x) { return __uint_as_float(static_cast<uint32_t>(x >> 32)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ void four(const float* p, float (&f)[4]) {
+  const float4 x = *reinterpret_cast<const float4*>(p);
+  f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w;
+}
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
@@ -98,14 +125,26 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
       "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32f(uint32_t taddr, const float (&v)[32]) {
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&v)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const float (&v)[16]) {
   uint32_t u[16];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
+  for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[i]);
+  tmem_st16(taddr, u);
+}
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 16; ++i) u[i] = __float_as_uint(v[16 * h + i]);
-    tmem_st16(taddr + 16 * h, u);
-  }
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
@@ -154,8 +193,8 @@ template <int HD, int FMT, int LANES>
 __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __grid_constant__ PrefixArgs a) {
   using L = PrefixSmem<HD, LANES>;
   constexpr uint32_t kBf16 = (1u << 7) | (1u << 10);   // operand types of a descriptor: f16 is 0
-  constexpr uint32_t kIdescS = tc::make_idesc(kPrefixStep, false, false) & ~kBf16, kIdescO = tc::make_idesc(HD, false, true) & ~kBf16;
-  constexpr uint32_t kColO = 256;   // TMEM: S of lane 0, of lane 1 (128 columns each), O of lane 0, of lane 1
+  constexpr uint32_t kIdescS = tc::make_idesc(kHalf, false, false) & ~kBf16, kIdescO = tc::make_idesc(HD, false, true) & ~kBf16;
+  constexpr uint32_t kColO = 256;   // TMEM: two S of lane 0, of lane 1 (64 columns each), O of lane 0, of lane 1 (128 each)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-tc::smem_u32(smem_raw) & 1023u);   // the swizzle goes by address
   PrefixNote* notes = reinterpret_cast<PrefixNote*>(smem + L::kOffNotes);
@@ -165,10 +204,11 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
   uint64_t* k_empty = k_full + 2;
   uint64_t* v_full = k_empty + 2;
   uint64_t* v_empty = v_full + 2;
-  uint64_t* s_full = v_empty + 2;            // [lane] S is there
-  uint64_t* p_full = s_full + 2;             // [lane] P is there
-  uint64_t* q_full = p_full + 2;                                      // the unit's queries are laid out
-  uint64_t* unit_done = q_full + 1;                                   // all products of the unit are done
+  uint64_t* s_full = v_empty + 2;            // [lane][half] S is there
+  uint64_t* p_full = s_full + 4;             // [lane][half] P is there
+  uint64_t* o_full = p_full + 4;             // [lane] O has a P more
+  uint64_t* q_full = o_full + 2;             // the unit's queries are laid out
+  uint64_t* unit_done = q_full + 1;          // all products of the unit are done
   uint64_t* drain = unit_done + 1;
   uint32_t* slot = reinterpret_cast<uint32_t*>(drain + 1);
   __shared__ int abort_storage;
@@ -182,15 +222,18 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
     }
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(k_full + i, kDecodeWarps);
-      tc::mbar_init(k_empty + i, 1);
+      tc::mbar_init(k_empty + i, LANES);
       tc::mbar_init(v_full + i, kDecodeWarps);
-      tc::mbar_init(v_empty + i, 1);
+      tc::mbar_init(v_empty + i, LANES);
+      tc::mbar_init(o_full + i, 1);
+    }
+    for (int i = 0; i < 4; ++i) {
       tc::mbar_init(s_full + i, 1);
       tc::mbar_init(p_full + i, 4);
     }
     tc::mbar_init(q_full, 4 * LANES);
-    tc::mbar_init(unit_done, 1);
-    tc::mbar_init(drain, 1);
+    tc::mbar_init(unit_done, 2);
+    tc::mbar_init(drain, 2);
     abort = 0;
     tc::fence_mbar_init();
   }
@@ -214,41 +257,55 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
     const uint32_t at = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_at = at + mine * 128, o_at = at + kColO + mine * 128;
     uint32_t s_phase = 0;
-    int seg = 0, base = 0;   // steps before the unit's
+    int seg = 0, base = 0, products = 0;   // steps before the unit's, the lane's products with V so far
     for (; run.on() && !abort; run.next(), ++seg) {
       const int kvh = run.unit % a.parts.kv_heads, pair = run.unit / a.parts.kv_heads;
-      // ---- queries: a thread its row, which one of the lanes lays out
-      float unit_q;   // takes S to log2 units
+      // ---- queries: a warp its threads' rows, kPer lanes to a row
+      float unit_q = 0.f;   // takes S to log2 units
       {
-        const int rho = (LANES == 2 ? pair * 2 + mine : pair) * kPrefixRows + r;
-        const bool on = rho < a.rows;
-        const int tok = rho / a.group;
-        const uint4* src = reinterpret_cast<const uint4*>(a.q + static_cast<int64_t>(tok) * a.ld_q + (kvh * a.group + rho - tok * a.group) * HD);
-        uint4 x[HD / 8];   // at once: the loads' latency is the unit's
-#pragma unroll
-        for (int c = 0; c < HD / 8; ++c) x[c] = on ? src[c] : make_uint4(0, 0, 0, 0);
-        uint32_t tops = 0;   // of bf16 numbers without their signs, the larger is the larger integer
-#pragma unroll
-        for (int c = 0; c < HD / 8; ++c)
-          tops = __vmaxu2(tops, __vmaxu2(__vmaxu2(x[c].x & 0x7FFF7FFFu, x[c].y & 0x7FFF7FFFu),
-                                         __vmaxu2(x[c].z & 0x7FFF7FFFu, x[c].w & 0x7FFF7FFFu)));
-        const float peak = fmaxf(bf16_lo(tops), bf16_hi(tops));
-        // 2^e takes the largest magnitude to [2^13, 2^14)
+        constexpr int kPer = HD / 8, kRows = 32 / kPer, kTurns = 32 / kRows;
+        const int c = lane % kPer;
+        const int rho0 = (LANES == 2 ? pair * 2 + mine : pair) * kPrefixRows + (warp & 3) * 32 + lane / kPer;
         auto power = [](int e) { return __int_as_float((e + 127) << 23); };   // 2^e, |e| < 127
-        int e = 0;
-        if (peak > 0.f && peak <= FLT_MAX) e = 13 - (static_cast<int>(__float_as_uint(peak) >> 23) - 127);
-        const float f1 = power(e >> 1), f2 = power(e - (e >> 1));   // 2^e may be out of range
-        unit_q = a.scale * 1.4426950408889634f * power(-(e >> 1)) * power(-(e - (e >> 1)));
-        if (LANES == 2 || mine == 0) {
-          uint8_t* dst = smem + (LANES == 2 ? mine * L::kQ : 0) + r * 128;
+        uint8_t* dst = smem + (LANES == 2 ? mine * L::kQ : 0) + (c >> 3) * (kPrefixRows * 128);
+        constexpr int kBatch = 8;   // rows whose loads are in flight at once: their latency is the unit's
+#pragma unroll 1
+        for (int i0 = 0; i0 < kTurns; i0 += kBatch) {
+        uint4 x[kBatch];
 #pragma unroll
-          for (int c = 0; c < HD / 8; ++c) {
+        for (int k = 0; k < kBatch; ++k) {
+          const int i = i0 + k;
+          const int rho = rho0 + i * kRows, tok = rho / a.group;
+          x[k] = rho < a.rows ? *reinterpret_cast<const uint4*>(a.q + static_cast<int64_t>(tok) * a.ld_q +
+                                                                (kvh * a.group + rho - tok * a.group) * HD + c * 8)
+                              : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const int i = i0 + k;
+          // of bf16 numbers without their signs, the larger is the larger integer
+          uint32_t tops = __vmaxu2(__vmaxu2(x[k].x & 0x7FFF7FFFu, x[k].y & 0x7FFF7FFFu),
+                                   __vmaxu2(x[k].z & 0x7FFF7FFFu, x[k].w & 0x7FFF7FFFu));
+#pragma unroll
+          for (int o = kPer / 2; o > 0; o >>= 1) tops = __vmaxu2(tops, __shfl_xor_sync(0xffffffffu, tops, o));
+          const float peak = fmaxf(bf16_lo(tops), bf16_hi(tops));
+          // 2^e takes the largest magnitude to [2^13, 2^14)
+          int e = 0;
+          if (peak > 0.f && peak <= FLT_MAX) e = 13 - (static_cast<int>(__float_as_uint(peak) >> 23) - 127);
+          const float f1 = power(e >> 1), f2 = power(e - (e >> 1));   // 2^e may be out of range
+          const int e_mine = __shfl_sync(0xffffffffu, e, lane % kRows * kPer);
+          if (lane / kRows == i) unit_q = a.scale * 1.4426950408889634f * power(-(e_mine >> 1)) * power(-(e_mine - (e_mine >> 1)));
+          if (LANES == 2 || mine == 0) {
+            const int row = (warp & 3) * 32 + i * kRows + lane / kPer;
             float f[8];
-            unpack8(x[c], f);
-            *reinterpret_cast<uint4*>(dst + (c >> 3) * (kPrefixRows * 128) + (((c & 7) ^ (r & 7)) << 4)) =
+            unpack8(x[k], f);
+            *reinterpret_cast<uint4*>(dst + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
                 make_uint4(pack_f16x2(f[0] * f1 * f2, f[1] * f1 * f2), pack_f16x2(f[2] * f1 * f2, f[3] * f1 * f2),
                            pack_f16x2(f[4] * f1 * f2, f[5] * f1 * f2), pack_f16x2(f[6] * f1 * f2, f[7] * f1 * f2));
           }
+        }
+        }
+        if (LANES == 2 || mine == 0) {
           fence_async_smem();
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(q_full);
@@ -257,110 +314,105 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
       float m = -INFINITY, l = 0.f;
       bool any = false;
       const int n = run.s1 - run.s0;
-      for (int i = LANES == 2 ? 0 : mine; i < n; i += LANES == 2 ? 1 : 2) {
+      for (int i = LANES == 2 ? 0 : mine; i < n && !abort; i += LANES == 2 ? 1 : 2, s_phase ^= 1) {
+        const PrefixNote& note = notes[(base + i) % kNotes];
         // (K is long laid out when S is there: waited for so that the step's note is seen)
-        if (!__all_sync(0xffffffffu, tc::mbar_wait(s_full + mine, s_phase, a.err, &abort) &&
-                                         tc::mbar_wait(k_full + ((base + i) & 1), ((base + i) >> 1) & 1, a.err, &abort))) {
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(k_full + ((base + i) & 1), ((base + i) >> 1) & 1, a.err, &abort))) {
           abort = 1;
           break;
         }
-        s_phase ^= 1;
-        tc::tc_fence_after();
-        const PrefixNote& note = notes[(base + i) % kNotes];
-        const int left = tokens - (run.s0 + i) * kPrefixStep;   // tokens of the step
         const int flags = note.flags;
-        const bool edge = left < kPrefixStep || flags != 0;
-        // Loops of 64 columns are not unrolled: with all roles' code unrolled, warps waited for instructions more than
-        // for anything else (a step took 10,400 cycles).
-        auto four = [](const float* p, float (&f)[4]) {   // of the groups of 16
-          const float4 x = *reinterpret_cast<const float4*>(p);
-          f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w;
-        };
-        auto units = [&](int c, float (&u)[4]) {
-          four(note.k + c / 16, u);
-#pragma unroll
-          for (int h = 0; h < 4; ++h) u[h] = fmaxf(u[h] * unit_q, 1e-37f);   // above 0, so that a masked -inf stays one
-        };
-        auto scores = [&](int c, float (&v)[64]) {
-          tmem_ld64(s_at + c, v);
-          if (edge) {
-            const int gone = flags >> (c / 16);
-#pragma unroll
-            for (int j = 0; j < 64; ++j)
-              if (c + j >= left || (gone >> (j / 16) & 1)) v[j] = -INFINITY;
-          }
-        };
-        float peak = -INFINITY;
+        const int left = tokens - (run.s0 + i) * kPrefixStep;   // tokens of the step
+        // not unrolled: with all roles' code unrolled, warps waited for instructions more than for anything else
 #pragma unroll 1
-        for (int c = 0; c < 128; c += 64) {
-          float v[64], u[4], w[4];
-          scores(c, v);
-          units(c, u);
-          four(note.log_v + c / 16, w);
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            float x[4] = {v[16 * h], v[16 * h + 1], v[16 * h + 2], v[16 * h + 3]};
-#pragma unroll
-            for (int j = 4; j < 16; ++j) x[j & 3] = fmaxf(x[j & 3], v[16 * h + j]);
-            peak = fmaxf(peak, fmaf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), u[h], w[h]));
+        for (int half = 0; half < 2; ++half) {
+          float u[4], w[4];   // of the groups of 16 tokens
+          four(note.k + 4 * half, u);
+          four(note.log_v + 4 * half, w);
+          if (!__all_sync(0xffffffffu, tc::mbar_wait(s_full + 2 * mine + half, s_phase, a.err, &abort))) {
+            abort = 1;
+            break;
           }
-        }
-        const bool grow = peak > m + kSlack || (m == -INFINITY && peak > m);
-        if (__any_sync(0xffffffffu, grow)) {
-          // S of this step came after the products of the lane's last: O is at rest
-          const float f = grow ? (m == -INFINITY ? 0.f : ex2_approx(m - peak)) : 1.f;
-          if (any) {
+          tc::tc_fence_after();
+          const uint32_t s_half = s_at + half * kHalf;
+          float v[kHalf];
+          tmem_ld64(s_half, v);
+#pragma unroll
+          for (int g = 0; g < 4; ++g) u[g] = fmaxf(u[g] * unit_q, 1e-37f);   // above 0, so that a masked -inf stays one
+          const int gone = flags >> (4 * half);
+          if (left < (half + 1) * kHalf || (gone & 0xF)) {
+#pragma unroll
+            for (int j = 0; j < kHalf; ++j)
+              if (j >= left - half * kHalf || (gone >> (j / 16) & 1)) v[j] = -INFINITY;
+          }
+          // P by the reference as it stands.  A unit's first S moves it, and one whose weights would come near f16's
+          // top, which the sums show: the maximum is taken then, and only then.
+          float sums[4];
+          bool moved = false;
 #pragma unroll 1
-            for (int c = 0; c < HD; c += 32) {
-              float o[32];
-              tc::tmem_ld32(o_at + c, o);
+          while (true) {
+            const float ref = kLift - (m == -INFINITY ? 0.f : m);
 #pragma unroll
-              for (int j = 0; j < 32; ++j) o[j] *= f;
-              tmem_st32f(o_at + c, o);
-            }
-          }
-          if (grow) {
-            l *= f;
-            m = peak;
-          }
-        }
-        any = true;
-        const float ref = kLift - (m == -INFINITY ? 0.f : m);
-#pragma unroll 1
-        for (int c = 0; c < 128; c += 64) {
-          float v[64], u[4], w[4], inv[4];
-          scores(c, v);
-          units(c, u);
-          four(note.log_v + c / 16, w);
-          four(note.inv_v + c / 16, inv);
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            uint32_t p[16];
-#pragma unroll
-            for (int g = 0; g < 2; ++g) {
-              const int h = 2 * half + g;
-              const float uh = u[h], rh = ref + w[h];
-              float sum[2] = {0.f, 0.f};
+            for (int g = 0; g < 4; ++g) {
+              uint32_t p[8];
+              const float r = ref + w[g];
+              const uint64_t u2 = two_floats(u[g], u[g]), r2 = two_floats(r, r);
+              uint64_t sum = 0;
 #pragma unroll
               for (int j = 0; j < 16; j += 2) {
-                const float p0 = ex2_approx(fmaf(v[16 * h + j], uh, rh)), p1 = ex2_approx(fmaf(v[16 * h + j + 1], uh, rh));
-                sum[0] += p0;
-                sum[1] += p1;
-                p[8 * g + j / 2] = pack_f16x2(p0, p1);
+                const uint64_t e = fma2(two_floats(v[16 * g + j], v[16 * g + j + 1]), u2, r2);
+                const float p0 = ex2_approx(low(e)), p1 = ex2_approx(high(e));
+                sum = add2(sum, two_floats(p0, p1));
+                p[j / 2] = pack_f16x2(p0, p1);
               }
-              l = fmaf(sum[0] + sum[1], inv[h], l);
-              if (edge && (flags >> (8 + c / 16 + h) & 1)) {
+              sums[g] = low(sum) + high(sum);
+              tmem_st8(s_half + 8 * g, p);   // over S, which is read
+            }
+            const bool high = fmaxf(fmaxf(sums[0], sums[1]), fmaxf(sums[2], sums[3])) > kMostSum;
+            if (moved || !__any_sync(0xffffffffu, high || m == -INFINITY)) break;
+            moved = true;
+            float peak = -INFINITY;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) p[8 * g + j] = 0;
+            for (int g = 0; g < 4; ++g) {
+              float x[4] = {v[16 * g], v[16 * g + 1], v[16 * g + 2], v[16 * g + 3]};
+#pragma unroll
+              for (int j = 4; j < 16; ++j) x[j & 3] = fmaxf(x[j & 3], v[16 * g + j]);
+              peak = fmaxf(peak, fmaf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), u[g], w[g]));
+            }
+            const bool grow = peak > m;   // rows of the warp that need not move do no harm
+            const float f = grow ? (m == -INFINITY ? 0.f : ex2_approx(m - peak)) : 1.f;
+            if (any) {
+              // the lane's last product with V is done, and the next one waits for this P
+              if (!__all_sync(0xffffffffu, tc::mbar_wait(o_full + mine, (products - 1) & 1, a.err, &abort))) {
+                abort = 1;
+                break;
+              }
+              tc::tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < HD; c += 16) {
+                float o[16];
+                tmem_ld16(o_at + c, o);
+#pragma unroll
+                for (int j = 0; j < 16; ++j) o[j] *= f;
+                tmem_st16(o_at + c, o);
               }
             }
-            tmem_st16(s_at + c / 2 + 16 * half, p);   // over scores that are read
+            if (grow) {
+              l *= f;
+              m = peak;
+            }
           }
+          if (abort) break;
+          any = true;
+          ++products;
+          four(note.inv_v + 4 * half, u);
+#pragma unroll
+          for (int g = 0; g < 4; ++g) l = fmaf(sums[g], u[g], l);
+          tmem_wait_st();
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(p_full + 2 * mine + half);
         }
-        tmem_wait_st();
-        tc::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(p_full + mine);
       }
       // ---- the unit's result
       if (abort || !__all_sync(0xffffffffu, tc::mbar_wait(unit_done, seg & 1, a.err, &abort))) {
@@ -399,12 +451,15 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
     int it = 0, raw = 0;
     uint32_t raw_phase = 0;
     // The step's K or V; tokens that are not there become 0 (P is 0 there, and 0 times a NaN would not be).
-    auto lay = [&](uint8_t* dst, int left) {
+    auto lay = [&](uint8_t* dst, int left, bool values) {
       int flags = 0;
 #pragma unroll 1
       for (int u = 0; u < kPrefixStep; u += kRawTokens) {
         if (!__all_sync(0xffffffffu, tc::mbar_wait(raw_full + raw, raw_phase, a.err, &abort))) return false;
-        if (u == 0) flags = notes[it % kNotes].flags;
+        if (u == 0) {
+          flags = notes[it % kNotes].flags;
+          if (values) flags |= flags >> 8;
+        }
         const uint8_t* src = smem + L::kOffRaw + raw * L::kRaw + tid * 16;
         uint4 x[kMine];
 #pragma unroll
@@ -436,10 +491,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
         const int slot = it & 1, left = tokens - step * kPrefixStep;
         const uint32_t free_phase = ((it >> 1) & 1) ^ 1;
         bool ok = __all_sync(0xffffffffu, tc::mbar_wait(k_empty + slot, free_phase, a.err, &abort)) &&
-                  lay(smem + L::kOffK + slot * L::kPart, left);
+                  lay(smem + L::kOffK + slot * L::kPart, left, false);
         if (ok && lane == 0) tc::mbar_arrive(k_full + slot);
         ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(v_empty + slot, free_phase, a.err, &abort)) &&
-             lay(smem + L::kOffV + slot * L::kPart, left);
+             lay(smem + L::kOffV + slot * L::kPart, left, true);
         if (ok && lane == 0) tc::mbar_arrive(v_full + slot);
         if (!ok) {
           abort = 1;
@@ -502,48 +557,52 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
           break;
         }
       }
-  } else if (warp == kIssueWarp && lane == 0) {
+  } else if (warp < kCopyWarp && lane == 0) {
     // ------------------------------- products ------------------------------
-    uint32_t p_phase[2] = {0, 0};
+    const int mine = warp - kIssueWarp;
+    const uint32_t q = tc::smem_u32(smem) + (LANES == 2 ? mine * L::kQ : 0), k_at = tc::smem_u32(smem + L::kOffK),
+                   v_at = tc::smem_u32(smem + L::kOffV), p = tmem + mine * 128, o = tmem + kColO + mine * 128;
+    uint32_t p_phase = 0;
     bool ok = true;
     int base = 0;   // steps before the unit's
-    const uint32_t q_at = tc::smem_u32(smem), k_at = tc::smem_u32(smem + L::kOffK), v_at = tc::smem_u32(smem + L::kOffV);
     for (int seg = 0; ok && run.on() && !abort; run.next(), ++seg) {
-      const int steps = run.s1 - run.s0, n = LANES * steps;   // products of a lane and a step
+      const int n = run.s1 - run.s0, first = LANES == 2 ? 0 : mine, by = LANES == 2 ? 1 : 2;
       ok = tc::mbar_wait(q_full, seg & 1, a.err, &abort);
-      auto scores = [&](int i) {
-        const int step = base + (LANES == 2 ? i >> 1 : i), ln = i & 1, slot = step & 1;
-        if ((LANES == 1 || ln == 0) && !tc::mbar_wait(k_full + slot, (step >> 1) & 1, a.err, &abort)) return false;
+      // S of half a step runs a step ahead of its P: the other half's softmax has the time between
+      auto scores = [&](int i, int half) {
+        const int step = base + i, slot = step & 1;
+        if (half == 0 && !tc::mbar_wait(k_full + slot, (step >> 1) & 1, a.err, &abort)) return false;
         tc::tc_fence_after();
-        const uint32_t q = q_at + (LANES == 2 ? ln * L::kQ : 0), kk = k_at + slot * L::kPart;
+        const uint32_t kk = k_at + slot * L::kPart + half * kHalf * 128;
 #pragma unroll
         for (int j = 0; j < HD / 16; ++j)
-          tc::umma_bf16(tmem + ln * 128, tc::desc_kmajor(q + (j >> 2) * (kPrefixRows * 128), j & 3),
+          tc::umma_bf16(p + half * kHalf, tc::desc_kmajor(q + (j >> 2) * (kPrefixRows * 128), j & 3),
                         tc::desc_kmajor(kk + (j >> 2) * (kPrefixStep * 128), j & 3), kIdescS, j > 0);
-        tc::umma_commit(s_full + ln);
-        if (LANES == 1 || ln == 1) tc::umma_commit(k_empty + slot);
+        tc::umma_commit(s_full + 2 * mine + half);
+        if (half) tc::umma_commit(k_empty + slot);
         return true;
       };
-      auto values = [&](int i) {
-        const int step = base + (LANES == 2 ? i >> 1 : i), ln = i & 1, slot = step & 1;
-        if ((LANES == 1 || ln == 0) && !tc::mbar_wait(v_full + slot, (step >> 1) & 1, a.err, &abort)) return false;
-        if (!tc::mbar_wait(p_full + ln, p_phase[ln], a.err, &abort)) return false;
-        p_phase[ln] ^= 1;
-        tc::tc_fence_after();
-        const uint32_t vv = v_at + slot * L::kPart, p = tmem + ln * 128, o = tmem + kColO + ln * 128;
-        const bool first = i < 2;
+      for (int half = 0; half < 2; ++half)
+        if (ok && first < n) ok = scores(first, half);
+      for (int i = first; ok && i < n; i += by, p_phase ^= 1) {
+        const int step = base + i, slot = step & 1;
+        ok = tc::mbar_wait(v_full + slot, (step >> 1) & 1, a.err, &abort);
+        for (int half = 0; ok && half < 2; ++half) {
+          ok = tc::mbar_wait(p_full + 2 * mine + half, p_phase, a.err, &abort);
+          if (!ok) break;
+          tc::tc_fence_after();
+          const uint32_t vv = v_at + slot * L::kPart + half * kHalf * 128;
 #pragma unroll
-        for (int j = 0; j < kPrefixStep / 16; ++j)
-          umma_p(o, p + 8 * j, tc::make_sdesc(vv + j * 2048, kPrefixStep * 128, 1024), kIdescO, !(first && j == 0));
-        if (LANES == 1 || ln == 1) tc::umma_commit(v_empty + slot);
-        return true;
-      };
-      for (int i = 0; ok && i <= n; ++i) {
-        if (i < n) ok = scores(i);
-        if (ok && i > 0) ok = values(i - 1);
+          for (int j = 0; j < kHalf / 16; ++j)
+            umma_p(o, p + half * kHalf + 8 * j, tc::make_sdesc(vv + j * 2048, kPrefixStep * 128, 1024), kIdescO,
+                   !(i == first && half == 0 && j == 0));
+          tc::umma_commit(o_full + mine);
+          if (half) tc::umma_commit(v_empty + slot);
+          if (i + by < n) ok = scores(i + by, half);
+        }
       }
       if (ok) tc::umma_commit(unit_done);
-      base += steps;
+      base += n;
     }
     if (!ok) abort = 1;
   }
@@ -556,17 +615,87 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
       tc::mbar_wait(raw_full + j % L::kRaws, (j / L::kRaws) & 1, a.err);
     }
   }
+  if (abort) {
+    // no product may still write TMEM when it is given back
+    if (lane == 0 && (warp == kIssueWarp || warp == kIssueWarp + 1)) {
+      tc::umma_commit(drain);
+      tc::mbar_wait(drain, 0, a.err);
+    }
+    __syncthreads();
+  }
   if (warp == kIssueWarp) {
     tc::tc_fence_after();
-    if (abort) {
-      // no product may still write TMEM when it is given back
-      if (lane == 0) {
-        tc::umma_commit(drain);
-        tc::mbar_wait(drain, 0, a.err);
-      }
-      __syncwarp();
-    }
     tc::tmem_dealloc(tmem, 512);
+  }
+}
+
+// Adds the prefix's parts to four channels (from d on) of a query row: its sum z of values, maximum and sum of weights.
+__device__ __forceinline__ void join_prefix(const PrefixParts& p, int row, int kvh, int hd, int d, float4& z, float& top,
+                                            float& sum) {
+  const int tokens = p.tokens(nullptr);
+  if (tokens == 0) return;
+  const PrefixShares sh(p, tokens);
+  const int tile = row / kPrefixRows, r = row % kPrefixRows;
+  const int unit = tile / p.lanes * p.kv_heads + kvh;
+  const int first = sh.owner(static_cast<int64_t>(unit) * sh.steps);
+  const int last = sh.owner(static_cast<int64_t>(unit + 1) * sh.steps - 1);
+  // the row's results: one a CTA, or two
+  const int lane0 = p.lanes == 2 ? tile & 1 : 0, per = p.lanes == 2 ? 1 : 2;
+  const int parts = (last - first + 1) * per, slot = PrefixParts::slot_floats(hd);
+  const float* base = p.slots + static_cast<int64_t>(unit + first) * slot;
+  constexpr int kBatch = 8;   // parts whose loads are in flight at once
+  for (int k0 = 0; k0 < parts; k0 += kBatch) {
+    float m[kBatch], l[kBatch];
+    float4 x[kBatch];
+    float peak = top;
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      const int i = min(k0 + k, parts - 1);
+      const int cta = per == 2 ? i >> 1 : i, lane = per == 2 ? i & 1 : lane0;
+      const float* s = base + static_cast<int64_t>(cta) * slot;
+      const int at = lane * kPrefixRows + r;
+      x[k] = *reinterpret_cast<const float4*>(s + static_cast<int64_t>(at) * hd + d);
+      m[k] = s[2 * kPrefixRows * hd + at];
+      l[k] = s[2 * kPrefixRows * (hd + 1) + at];
+    }
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k)
+      if (k0 + k < parts) peak = fmaxf(peak, m[k]);
+    const float old = join_factor(top, peak);
+    sum *= old;
+    z = make_float4(z.x * old, z.y * old, z.z * old, z.w * old);
+#pragma unroll
+    for (int k = 0; k < kBatch; ++k) {
+      if (k0 + k >= parts) continue;
+      const float f = join_factor(m[k], peak);
+      sum = fmaf(l[k], f, sum);
+      z.x = fmaf(x[k].x, f, z.x);
+      z.y = fmaf(x[k].y, f, z.y);
+      z.z = fmaf(x[k].z, f, z.z);
+      z.w = fmaf(x[k].w, f, z.w);
+    }
+    top = peak;
+  }
+}
+
+// Joins what the sequences' own tokens and the prefix gave a query row: a thread four channels, blockIdx.y a sequence.
+__global__ void __launch_bounds__(kThreads) kv8_prefix_join_kernel(const __grid_constant__ AttnArgs a,
+                                                                  const __grid_constant__ PrefixParts parts) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const Kv8Span s = kv8_span(a.b, blockIdx.y, a.c.block_tokens, nullptr);
+  const int hd = a.c.head_dim, per = hd / 4;
+  const float* ml = a.own + static_cast<int64_t>(a.b.rows) * a.nh * hd;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < static_cast<int64_t>(s.n) * a.nh * per;
+       i += static_cast<int64_t>(gridDim.x) * kThreads) {
+    const int64_t at = static_cast<int64_t>(s.row0) * a.nh + i / per;   // row and head
+    const int d = static_cast<int>(i % per) * 4;
+    const int64_t tok = at / a.nh;
+    const int head = static_cast<int>(at - tok * a.nh), kvh = head / a.group;
+    float4 z = *reinterpret_cast<const float4*>(a.own + at * hd + d);
+    const float2 own = *reinterpret_cast<const float2*>(ml + 2 * at);
+    float top = own.x, sum = own.y;
+    join_prefix(parts, static_cast<int>(tok) * a.group + head - kvh * a.group, kvh, hd, d, z, top, sum);
+    write_out<Mode::kPlain>(a, static_cast<int>(tok), head - kvh * a.group, kvh, hd, d, z, top, sum);
   }
 }
 
@@ -605,6 +734,24 @@ PrefixParts plan_prefix(const GltKv8Cache& c, const GltKv8Batch& b, const GltKv8
   return s;
 }
 int64_t align32(int64_t n) { return (n + 31) / 32 * 32; }
+int64_t own_bytes(const GltKv8Cache& c, const GltKv8Batch& b, int nh) {
+  return align32(static_cast<int64_t>(b.rows) * nh * (c.head_dim + 2) * 4);
+}
+int launch_join(const AttnArgs& a, const PrefixParts& parts, cudaStream_t st) {
+  const int64_t most = static_cast<int64_t>(kv8_most_new(a.c, a.b)) * a.nh * (a.c.head_dim / 4);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>((most + kThreads - 1) / kThreads, 4096)), a.b.num_seqs);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  GLT_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv8_prefix_join_kernel, a, parts));
+  GLT_LAUNCH_CHECK();
+  return GLT_OK;
+}
 
 }  // namespace
 }  // namespace glt
@@ -616,6 +763,7 @@ extern "C" int glt_kv8_prefix_attention_workspace(const GltKv8Cache* cache, cons
   GLT_TRY(glt::check_prefix(cache, prefix));
   *bytes = batch->rows > 0 && batch->max_new > 0
                ? glt::align32(glt::plan(*cache, *batch, num_heads).bytes) +
+                     glt::own_bytes(*cache, *batch, num_heads) +
                      glt::plan_prefix(*cache, *batch, *prefix, num_heads).bytes(cache->head_dim)
                : 0;
   return GLT_OK;
@@ -634,19 +782,23 @@ extern "C" int glt_kv8_prefix_attention(const GltKv8Cache* cache, const GltKv8Ba
   glt::Plan p;
   GLT_TRY(glt::prepare(cache, batch, q, ld_q, o, ld_o, lse, num_heads, scale, 0, token_mask, ld_mask, workspace,
                        workspace_bytes, &a, &p));
-  a.parts = glt::plan_prefix(*cache, *batch, *prefix, num_heads);
-  const int64_t own = glt::align32(p.bytes), need = own + a.parts.bytes(cache->head_dim);
+  glt::PrefixParts parts = glt::plan_prefix(*cache, *batch, *prefix, num_heads);
+  const int64_t first = glt::align32(p.bytes), second = first + glt::own_bytes(*cache, *batch, num_heads),
+                need = second + parts.bytes(cache->head_dim);
   if (workspace_bytes < need)
-    return glt::fail(GLT_EINVAL, "kv8: workspace must be 16-byte aligned and hold %lld bytes", (long long)need);
-  a.parts.slots = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + own);
+    return glt::fail(GLT_EINVAL, "kv8: workspace must be 32-byte aligned and hold %lld bytes", (long long)need);
+  if (reinterpret_cast<uintptr_t>(workspace) & 31) return glt::fail(GLT_EINVAL, "kv8: workspace must be 32-byte aligned");
+  a.own = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + first);
+  parts.slots = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + second);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a.parts.grid > 0) {
-    const glt::PrefixArgs x = {*cache, prefix->block_ids, q, ld_q, batch->rows * a.group, a.group, a.scale, a.parts, a.err};
+  if (parts.grid > 0) {
+    const glt::PrefixArgs x = {*cache, prefix->block_ids, q, ld_q, batch->rows * a.group, a.group, a.scale, parts, a.err};
     const bool int8 = cache->format == GLT_KV8_INT8;
     if (cache->head_dim == 128)
       GLT_TRY((int8 ? glt::launch_prefix<128, GLT_KV8_INT8>(x, st) : glt::launch_prefix<128, GLT_KV8_E4M3>(x, st)));
     else
       GLT_TRY((int8 ? glt::launch_prefix<64, GLT_KV8_INT8>(x, st) : glt::launch_prefix<64, GLT_KV8_E4M3>(x, st)));
   }
-  return glt::launch_all<glt::Mode::kPrefix>(a, p, st);
+  GLT_TRY(glt::launch_all<glt::Mode::kPrefix>(a, p, st));
+  return glt::launch_join(a, parts, st);
 }

@@ -54,56 +54,4 @@ struct PrefixShares {
   }
 };
 
-// 2^(m - top) for partial results: weights that saw nothing are 0 (or NaN) already.
-__device__ __forceinline__ float join_factor(float m, float top) { return top == -INFINITY ? 1.f : ex2_approx(m - top); }
-
-// Adds the prefix's parts to four channels (from d on) of a query row: its sum z of values, maximum and sum of weights.
-__device__ __forceinline__ void join_prefix(const PrefixParts& p, int row, int kvh, int hd, int d, float4& z, float& top,
-                                            float& sum) {
-  const int tokens = p.tokens(nullptr);
-  if (tokens == 0) return;
-  const PrefixShares sh(p, tokens);
-  const int tile = row / kPrefixRows, r = row % kPrefixRows;
-  const int unit = tile / p.lanes * p.kv_heads + kvh;
-  const int first = sh.owner(static_cast<int64_t>(unit) * sh.steps);
-  const int last = sh.owner(static_cast<int64_t>(unit + 1) * sh.steps - 1);
-  // the row's results: one a CTA, or two
-  const int lane0 = p.lanes == 2 ? tile & 1 : 0, per = p.lanes == 2 ? 1 : 2;
-  const int parts = (last - first + 1) * per, slot = PrefixParts::slot_floats(hd);
-  const float* base = p.slots + static_cast<int64_t>(unit + first) * slot;
-  constexpr int kBatch = 4;   // parts whose loads are in flight at once
-  for (int k0 = 0; k0 < parts; k0 += kBatch) {
-    float m[kBatch], l[kBatch];
-    float4 x[kBatch];
-    float peak = top;
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int i = min(k0 + k, parts - 1);
-      const int cta = per == 2 ? i >> 1 : i, lane = per == 2 ? i & 1 : lane0;
-      const float* s = base + static_cast<int64_t>(cta) * slot;
-      const int at = lane * kPrefixRows + r;
-      x[k] = *reinterpret_cast<const float4*>(s + static_cast<int64_t>(at) * hd + d);
-      m[k] = s[2 * kPrefixRows * hd + at];
-      l[k] = s[2 * kPrefixRows * (hd + 1) + at];
-    }
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k)
-      if (k0 + k < parts) peak = fmaxf(peak, m[k]);
-    const float old = join_factor(top, peak);
-    sum *= old;
-    z = make_float4(z.x * old, z.y * old, z.z * old, z.w * old);
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      if (k0 + k >= parts) continue;
-      const float f = join_factor(m[k], peak);
-      sum = fmaf(l[k], f, sum);
-      z.x = fmaf(x[k].x, f, z.x);
-      z.y = fmaf(x[k].y, f, z.y);
-      z.z = fmaf(x[k].z, f, z.z);
-      z.w = fmaf(x[k].w, f, z.w);
-    }
-    top = peak;
-  }
-}
-
 }  // namespace glt

@@ -324,7 +324,7 @@ GLT_API int glt_kv8_window_attention(const GltKv8Cache* cache, const GltKv8Batch
  * (batch->lengths and block_table hold and count only those): a query sees the whole prefix and, of its own
  * tokens, those that glt_kv8_attention without a window shows it (token_mask is for own tokens).
  * The prefix's cache is read once for every 256 rows (token x head of a group) of a KV head, not once a sequence.
- * workspace: glt_kv8_prefix_attention_workspace bytes, else as there. */
+ * workspace: glt_kv8_prefix_attention_workspace bytes, 32-byte aligned, else as there. */
 typedef struct GltKv8Prefix {
   int num_blocks;
   const int32_t* block_ids; /* dev [num_blocks] */
