@@ -71,7 +71,8 @@ struct PrefixSmem {
   static constexpr int kOffNotes = kOffRaw + kRaws * kRaw;
   static constexpr int kOffBars = kOffNotes + kNotes * static_cast<int>(sizeof(PrefixNote));
   static constexpr int kBars = 2 * kRaws + 8 + 8 + 2 + 3;
-  static constexpr int kTotal = 1024 + kOffBars + kBars * 8 + 16;
+  static constexpr int kOffUnits = kOffBars + (kBars + 2) * 8;
+  static constexpr int kTotal = 1024 + kOffUnits + kPrefixRows * 4;
 };
 static_assert(PrefixSmem<128, 1>::kTotal <= 232448 && PrefixSmem<128, 2>::kTotal <= 232448, "shared memory");
 
@@ -147,6 +148,10 @@ __device__ __forceinline__ void tmem_ld16(uint32_t taddr, float (&v)[16]) {
   for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// Copies 16 bytes (zero where !on: the source is not read then).
+__device__ __forceinline__ void copy_async16(void* dst, const void* src, bool on) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(dst)), "l"(src), "r"(on ? 16 : 0) : "memory");
+}
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(dst)),
                "l"(src), "r"(bytes), "r"(tc::smem_u32(bar))
@@ -168,24 +173,30 @@ __device__ __forceinline__ void sixteen_f16(const uint4& x, uint4& a, uint4& b) 
   b = make_uint4(two_codes<FMT, 0>(x.z), two_codes<FMT, 1>(x.z), two_codes<FMT, 0>(x.w), two_codes<FMT, 1>(x.w));
 }
 
-// Walks a CTA's run: unit `unit`, steps [s0, s1) of it.
+// Walks a CTA's run: steps [s0, s1) of unit `unit`.
 struct PrefixRun {
-  int64_t at, end;
-  int steps, unit, s0, s1;
-  __device__ __forceinline__ PrefixRun(const PrefixShares& sh, int cta)
-      : at(cta < sh.ctas ? sh.begin(cta) : 0), end(cta < sh.ctas ? sh.begin(cta + 1) : 0), steps(sh.steps) {
-    if (at < end) {
-      unit = static_cast<int>(at / steps);
-      s0 = static_cast<int>(at - static_cast<int64_t>(unit) * steps);
-      s1 = static_cast<int>(min(static_cast<int64_t>(steps), s0 + (end - at)));
-    }
+  int64_t left;   // of the run, from the unit's first place here on
+  int steps, place, unit, s0, s1;
+  __device__ __forceinline__ PrefixRun(const PrefixShares& sh, int cta) : left(0), steps(sh.steps) {
+    if (cta >= sh.ctas) return;
+    const int64_t begin = sh.begin(cta);
+    left = sh.begin(cta + 1) - begin;
+    unit = static_cast<int>(PrefixShares::quotient(begin, steps + kPrefixUnitCost));
+    place = static_cast<int>(begin - static_cast<int64_t>(unit) * (steps + kPrefixUnitCost));
+    bounds();
   }
-  __device__ __forceinline__ bool on() const { return at < end; }
+  __device__ __forceinline__ void bounds() {
+    s0 = max(0, place - kPrefixUnitCost);
+    s1 = static_cast<int>(min(static_cast<int64_t>(steps), place + left - kPrefixUnitCost));
+    if (left > 0 && s1 <= s0) next();   // only a part of the unit's cost
+  }
+  __device__ __forceinline__ bool on() const { return left > 0; }
+  __device__ __forceinline__ bool last() const { return left <= steps + kPrefixUnitCost - place + kPrefixUnitCost; }
   __device__ __forceinline__ void next() {
-    at += s1 - s0;
+    left -= steps + kPrefixUnitCost - place;
     ++unit;
-    s0 = 0;
-    s1 = static_cast<int>(min(static_cast<int64_t>(steps), end - at));
+    place = 0;
+    if (left > 0) bounds();
   }
 };
 
@@ -211,6 +222,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
   uint64_t* unit_done = q_full + 1;          // all products of the unit are done
   uint64_t* drain = unit_done + 1;
   uint32_t* slot = reinterpret_cast<uint32_t*>(drain + 1);
+  float* unit_rows = reinterpret_cast<float*>(smem + L::kOffUnits);   // LANES = 1: what lane 0 found for each row
   __shared__ int abort_storage;
   volatile int& abort = abort_storage;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -256,64 +268,73 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
     const int r = (warp & 3) * 32 + lane;                  // query row in the tile
     const uint32_t at = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const uint32_t s_at = at + mine * 128, o_at = at + kColO + mine * 128;
+    // x / group for x < group + 4: the quotient is at most 4, and no multiple lies as near as 2^-32 of it
+    const uint32_t group_inverse = a.group > 1 ? 0xFFFFFFFFu / static_cast<uint32_t>(a.group) + 1 : 0;
     uint32_t s_phase = 0;
     int seg = 0, base = 0, products = 0;   // steps before the unit's, the lane's products with V so far
     for (; run.on() && !abort; run.next(), ++seg) {
       const int kvh = run.unit % a.parts.kv_heads, pair = run.unit / a.parts.kv_heads;
       // ---- queries: a warp its threads' rows, kPer lanes to a row
+      // (one lane for both where they are the same)
+      const int n = run.s1 - run.s0;
       float unit_q = 0.f;   // takes S to log2 units
-      {
+      if (LANES == 2 || mine == 0) {
+        // into their places as they are, a warp its threads' rows, kPer lanes to a row, all at once (the loads' latency is the
+        // unit's); then a thread takes its row to f16
         constexpr int kPer = HD / 8, kRows = 32 / kPer, kTurns = 32 / kRows;
-        const int c = lane % kPer;
-        const int rho0 = (LANES == 2 ? pair * 2 + mine : pair) * kPrefixRows + (warp & 3) * 32 + lane / kPer;
+        const int tile_row = (LANES == 2 ? pair * 2 + mine : pair) * kPrefixRows;
+        uint8_t* q_smem = smem + (LANES == 2 ? mine * L::kQ : 0);
+        auto place = [&](int row, int c) { return q_smem + (c >> 3) * (kPrefixRows * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4); };
+        int row = (warp & 3) * 32 + lane / kPer;
+        int tok = (tile_row + row) / a.group, head = tile_row + row - tok * a.group;   // head of the group
+#pragma unroll 4
+        for (int i = 0; i < kTurns; ++i) {
+          copy_async16(place(row, lane % kPer), a.q + static_cast<int64_t>(tok) * a.ld_q + (kvh * a.group + head) * HD + lane % kPer * 8,
+                       tile_row + row < a.rows);
+          row += kRows;
+          head += kRows;
+          const int more = a.group > 1 ? static_cast<int>(__umulhi(static_cast<uint32_t>(head), group_inverse)) : head;   // head / group
+          tok += more;
+          head -= more * a.group;
+        }
+        commit();
+        wait_groups<0>();
+        __syncwarp();
+        uint32_t tops = 0;   // of bf16 numbers without their signs, the larger is the larger integer
+#pragma unroll 4
+        for (int c = 0; c < HD / 8; ++c) {
+          const uint4 x = *reinterpret_cast<const uint4*>(place(r, c));
+          tops = __vmaxu2(tops, __vmaxu2(__vmaxu2(x.x & 0x7FFF7FFFu, x.y & 0x7FFF7FFFu), __vmaxu2(x.z & 0x7FFF7FFFu, x.w & 0x7FFF7FFFu)));
+        }
+        const float peak = fmaxf(bf16_lo(tops), bf16_hi(tops));
+        // 2^e takes the largest magnitude to [2^13, 2^14)
         auto power = [](int e) { return __int_as_float((e + 127) << 23); };   // 2^e, |e| < 127
-        uint8_t* dst = smem + (LANES == 2 ? mine * L::kQ : 0) + (c >> 3) * (kPrefixRows * 128);
-        constexpr int kBatch = 8;   // rows whose loads are in flight at once: their latency is the unit's
-#pragma unroll 1
-        for (int i0 = 0; i0 < kTurns; i0 += kBatch) {
-        uint4 x[kBatch];
+        int e = 0;
+        if (peak > 0.f && peak <= FLT_MAX) e = 13 - (static_cast<int>(__float_as_uint(peak) >> 23) - 127);
+        const float f1 = power(e >> 1), f2 = power(e - (e >> 1));   // 2^e may be out of range
+        unit_q = a.scale * 1.4426950408889634f * power(-(e >> 1)) * power(-(e - (e >> 1)));
+#pragma unroll 2
+        for (int c = 0; c < HD / 8; ++c) {
+          float f[8];
+          unpack8(*reinterpret_cast<const uint4*>(place(r, c)), f);
 #pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-          const int i = i0 + k;
-          const int rho = rho0 + i * kRows, tok = rho / a.group;
-          x[k] = rho < a.rows ? *reinterpret_cast<const uint4*>(a.q + static_cast<int64_t>(tok) * a.ld_q +
-                                                                (kvh * a.group + rho - tok * a.group) * HD + c * 8)
-                              : make_uint4(0, 0, 0, 0);
+          for (int j = 0; j < 8; ++j) f[j] = f[j] * f1 * f2;
+          *reinterpret_cast<uint4*>(place(r, c)) =
+              make_uint4(pack_f16x2(f[0], f[1]), pack_f16x2(f[2], f[3]), pack_f16x2(f[4], f[5]), pack_f16x2(f[6], f[7]));
         }
-#pragma unroll
-        for (int k = 0; k < kBatch; ++k) {
-          const int i = i0 + k;
-          // of bf16 numbers without their signs, the larger is the larger integer
-          uint32_t tops = __vmaxu2(__vmaxu2(x[k].x & 0x7FFF7FFFu, x[k].y & 0x7FFF7FFFu),
-                                   __vmaxu2(x[k].z & 0x7FFF7FFFu, x[k].w & 0x7FFF7FFFu));
-#pragma unroll
-          for (int o = kPer / 2; o > 0; o >>= 1) tops = __vmaxu2(tops, __shfl_xor_sync(0xffffffffu, tops, o));
-          const float peak = fmaxf(bf16_lo(tops), bf16_hi(tops));
-          // 2^e takes the largest magnitude to [2^13, 2^14)
-          int e = 0;
-          if (peak > 0.f && peak <= FLT_MAX) e = 13 - (static_cast<int>(__float_as_uint(peak) >> 23) - 127);
-          const float f1 = power(e >> 1), f2 = power(e - (e >> 1));   // 2^e may be out of range
-          const int e_mine = __shfl_sync(0xffffffffu, e, lane % kRows * kPer);
-          if (lane / kRows == i) unit_q = a.scale * 1.4426950408889634f * power(-(e_mine >> 1)) * power(-(e_mine - (e_mine >> 1)));
-          if (LANES == 2 || mine == 0) {
-            const int row = (warp & 3) * 32 + i * kRows + lane / kPer;
-            float f[8];
-            unpack8(x[k], f);
-            *reinterpret_cast<uint4*>(dst + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
-                make_uint4(pack_f16x2(f[0] * f1 * f2, f[1] * f1 * f2), pack_f16x2(f[2] * f1 * f2, f[3] * f1 * f2),
-                           pack_f16x2(f[4] * f1 * f2, f[5] * f1 * f2), pack_f16x2(f[6] * f1 * f2, f[7] * f1 * f2));
-          }
+        if (LANES == 1) unit_rows[r] = unit_q;
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(q_full);
+      } else if (n > 1) {   // it has steps
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(q_full, seg & 1, a.err, &abort))) {
+          abort = 1;
+          break;
         }
-        }
-        if (LANES == 2 || mine == 0) {
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(q_full);
-        }
+        unit_q = unit_rows[r];
       }
       float m = -INFINITY, l = 0.f;
       bool any = false;
-      const int n = run.s1 - run.s0;
       for (int i = LANES == 2 ? 0 : mine; i < n && !abort; i += LANES == 2 ? 1 : 2, s_phase ^= 1) {
         const PrefixNote& note = notes[(base + i) % kNotes];
         // (K is long laid out when S is there: waited for so that the step's note is seen)
@@ -519,7 +540,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
         const float ks = in ? a.c.k_scale[hb] : 0.f, vs = in ? a.c.v_scale[hb] : 0.f;
         if (gone && a.err) atomicOr(a.err, GLT_DEVERR_BAD_SHAPE);
         const bool more = step + 1 < run.s1;   // (a following unit begins with step 0)
-        id = more || run.at + (run.s1 - run.s0) < run.end ? block(more ? step + 1 : 0) : -1;
+        id = more || !run.last() ? block(more ? step + 1 : 0) : -1;
         bool ok = true;
         for (int part = 0; ok && part < 4; ++part) {   // K, K, V, V
           const int u = (part & 1) * kRawTokens;
@@ -629,73 +650,128 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
   }
 }
 
-// Adds the prefix's parts to four channels (from d on) of a query row: its sum z of values, maximum and sum of weights.
-__device__ __forceinline__ void join_prefix(const PrefixParts& p, int row, int kvh, int hd, int d, float4& z, float& top,
-                                            float& sum) {
-  const int tokens = p.tokens(nullptr);
-  if (tokens == 0) return;
-  const PrefixShares sh(p, tokens);
-  const int tile = row / kPrefixRows, r = row % kPrefixRows;
-  const int unit = tile / p.lanes * p.kv_heads + kvh;
-  const int first = sh.owner(static_cast<int64_t>(unit) * sh.steps);
-  const int last = sh.owner(static_cast<int64_t>(unit + 1) * sh.steps - 1);
-  // the row's results: one a CTA, or two
-  const int lane0 = p.lanes == 2 ? tile & 1 : 0, per = p.lanes == 2 ? 1 : 2;
-  const int parts = (last - first + 1) * per, slot = PrefixParts::slot_floats(hd);
-  const float* base = p.slots + static_cast<int64_t>(unit + first) * slot;
-  constexpr int kBatch = 8;   // parts whose loads are in flight at once
-  for (int k0 = 0; k0 < parts; k0 += kBatch) {
-    float m[kBatch], l[kBatch];
-    float4 x[kBatch];
-    float peak = top;
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      const int i = min(k0 + k, parts - 1);
-      const int cta = per == 2 ? i >> 1 : i, lane = per == 2 ? i & 1 : lane0;
-      const float* s = base + static_cast<int64_t>(cta) * slot;
-      const int at = lane * kPrefixRows + r;
-      x[k] = *reinterpret_cast<const float4*>(s + static_cast<int64_t>(at) * hd + d);
-      m[k] = s[2 * kPrefixRows * hd + at];
-      l[k] = s[2 * kPrefixRows * (hd + 1) + at];
-    }
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k)
-      if (k0 + k < parts) peak = fmaxf(peak, m[k]);
-    const float old = join_factor(top, peak);
-    sum *= old;
-    z = make_float4(z.x * old, z.y * old, z.z * old, z.w * old);
-#pragma unroll
-    for (int k = 0; k < kBatch; ++k) {
-      if (k0 + k >= parts) continue;
-      const float f = join_factor(m[k], peak);
-      sum = fmaf(l[k], f, sum);
-      z.x = fmaf(x[k].x, f, z.x);
-      z.y = fmaf(x[k].y, f, z.y);
-      z.z = fmaf(x[k].z, f, z.z);
-      z.w = fmaf(x[k].w, f, z.w);
-    }
-    top = peak;
-  }
-}
-
-// Joins what the sequences' own tokens and the prefix gave a query row: a thread four channels, blockIdx.y a sequence.
-__global__ void __launch_bounds__(kThreads) kv8_prefix_join_kernel(const __grid_constant__ AttnArgs a,
-                                                                  const __grid_constant__ PrefixParts parts) {
+// Joins what the prefix and the sequences' own tokens gave the query rows: a lane eight channels of a row, SPLIT warps
+// a share of its parts each.  blockIdx.y is the sequence.
+constexpr int kJoinWarps = 4;
+template <int SPLIT>
+__global__ void __launch_bounds__(32 * kJoinWarps) kv8_prefix_join_kernel(const __grid_constant__ AttnArgs a,
+                                                                         const __grid_constant__ PrefixParts p) {
+  constexpr int kSets = kJoinWarps / SPLIT;   // of rows, of a CTA
+  __shared__ float4 sm_z[kJoinWarps][2][32];
+  __shared__ float2 sm_ml[kJoinWarps][32];
+  const int hd = a.c.head_dim, slot = PrefixParts::slot_floats(hd);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, share = warp % SPLIT;
+  const int per_log = hd == 128 ? 4 : 3, rows = 32 >> per_log;   // of a set
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Kv8Span s = kv8_span(a.b, blockIdx.y, a.c.block_tokens, nullptr);
-  const int hd = a.c.head_dim, per = hd / 4;
-  const float* ml = a.own + static_cast<int64_t>(a.b.rows) * a.nh * hd;
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; i < static_cast<int64_t>(s.n) * a.nh * per;
-       i += static_cast<int64_t>(gridDim.x) * kThreads) {
-    const int64_t at = static_cast<int64_t>(s.row0) * a.nh + i / per;   // row and head
-    const int d = static_cast<int>(i % per) * 4;
-    const int64_t tok = at / a.nh;
-    const int head = static_cast<int>(at - tok * a.nh), kvh = head / a.group;
-    float4 z = *reinterpret_cast<const float4*>(a.own + at * hd + d);
-    const float2 own = *reinterpret_cast<const float2*>(ml + 2 * at);
-    float top = own.x, sum = own.y;
-    join_prefix(parts, static_cast<int>(tok) * a.group + head - kvh * a.group, kvh, hd, d, z, top, sum);
-    write_out<Mode::kPlain>(a, static_cast<int>(tok), head - kvh * a.group, kvh, hd, d, z, top, sum);
+  const PrefixShares sh(p, p.tokens(nullptr));
+  const int count = s.n * a.nh, first_row = s.row0 * a.nh;   // rows of heads: checked on the host
+  const float* own_ml = a.own + static_cast<int64_t>(a.b.rows) * a.nh * hd;
+  const int d = (lane & ((1 << per_log) - 1)) * 8;
+  // (the CTA's warps take as many turns as its first)
+  for (int i0 = blockIdx.x * kSets * rows; i0 < count; i0 += gridDim.x * kSets * rows) {
+    const int i = i0 + warp / SPLIT * rows + (lane >> per_log);
+    const bool on = i < count;
+    const int at = first_row + (on ? i : i0);   // row and head
+    const int tok = at / a.nh, head = at - tok * a.nh, kvh = head / a.group, in_group = head - kvh * a.group;
+    const int rho = tok * a.group + in_group, tile = rho / kPrefixRows, row = rho % kPrefixRows;
+    const int unit = (p.lanes == 2 ? tile >> 1 : tile) * p.kv_heads + kvh;
+    // the row's parts: one a CTA, or two; the last is the sequence's own
+    const int lane0 = p.lanes == 2 ? tile & 1 : 0, twice = p.lanes == 2 ? 0 : 1;
+    int first = 0, parts = 1;
+    if (sh.ctas > 0) {
+      const int64_t begin = static_cast<int64_t>(unit) * (sh.steps + kPrefixUnitCost);
+      first = sh.owner(begin + kPrefixUnitCost);
+      parts = ((sh.owner(begin + sh.steps + kPrefixUnitCost - 1) - first + 1) << twice) + 1;
+    }
+    const float* base = p.slots + static_cast<int64_t>(unit + first) * slot;
+    float z[8] = {}, top = -INFINITY, sum = 0.f;
+    constexpr int kBatch = 3;   // parts whose loads are in flight at once
+    for (int k0 = share; k0 < parts; k0 += kBatch * SPLIT) {
+      float m[kBatch], l[kBatch];
+      float4 x[kBatch][2];
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const int part = k0 + k * SPLIT;
+        m[k] = -INFINITY;
+        l[k] = 0.f;
+        x[k][0] = x[k][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        const float* from;
+        if (part < parts - 1) {
+          const float* part_at = base + static_cast<int64_t>(part >> twice) * slot;
+          const int r = (twice ? part & 1 : lane0) * kPrefixRows + row;
+          from = part_at + r * hd + d;
+          m[k] = part_at[2 * kPrefixRows * hd + r];
+          l[k] = part_at[2 * kPrefixRows * (hd + 1) + r];
+        } else {
+          from = a.own + static_cast<int64_t>(at) * hd + d;
+          if (part == parts - 1) {
+            const float2 ml = *reinterpret_cast<const float2*>(own_ml + 2 * static_cast<int64_t>(at));
+            m[k] = ml.x;
+            l[k] = ml.y;
+          }
+        }
+        if (part < parts) {
+          x[k][0] = reinterpret_cast<const float4*>(from)[0];
+          x[k][1] = reinterpret_cast<const float4*>(from)[1];
+        }
+      }
+      float peak = top;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) peak = fmaxf(peak, m[k]);
+      const float old = join_factor(top, peak);
+      sum *= old;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) z[j] *= old;
+#pragma unroll
+      for (int k = 0; k < kBatch; ++k) {
+        const float f = join_factor(m[k], peak);
+        sum = fmaf(l[k], f, sum);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          z[4 * h] = fmaf(x[k][h].x, f, z[4 * h]);
+          z[4 * h + 1] = fmaf(x[k][h].y, f, z[4 * h + 1]);
+          z[4 * h + 2] = fmaf(x[k][h].z, f, z[4 * h + 2]);
+          z[4 * h + 3] = fmaf(x[k][h].w, f, z[4 * h + 3]);
+        }
+      }
+      top = peak;
+    }
+    if constexpr (SPLIT > 1) {
+      sm_z[warp][0][lane] = make_float4(z[0], z[1], z[2], z[3]);
+      sm_z[warp][1][lane] = make_float4(z[4], z[5], z[6], z[7]);
+      sm_ml[warp][lane] = make_float2(top, sum);
+      __syncthreads();
+      if (share == 0) {
+        float peak = top;
+#pragma unroll
+        for (int w = 1; w < SPLIT; ++w) peak = fmaxf(peak, sm_ml[warp + w][lane].x);
+        const float old = join_factor(top, peak);
+        sum *= old;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) z[j] *= old;
+#pragma unroll
+        for (int w = 1; w < SPLIT; ++w) {
+          const float2 ml = sm_ml[warp + w][lane];
+          const float f = join_factor(ml.x, peak);
+          sum = fmaf(ml.y, f, sum);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float4 x = sm_z[warp + w][h][lane];
+            z[4 * h] = fmaf(x.x, f, z[4 * h]);
+            z[4 * h + 1] = fmaf(x.y, f, z[4 * h + 1]);
+            z[4 * h + 2] = fmaf(x.z, f, z[4 * h + 2]);
+            z[4 * h + 3] = fmaf(x.w, f, z[4 * h + 3]);
+          }
+        }
+        top = peak;
+      }
+    }
+    if (on && share == 0) {
+      write_out<Mode::kPlain>(a, tok, in_group, kvh, hd, d, make_float4(z[0], z[1], z[2], z[3]), top, sum);
+      write_out<Mode::kPlain>(a, tok, in_group, kvh, hd, d + 4, make_float4(z[4], z[5], z[6], z[7]), top, sum);
+    }
+    if (SPLIT > 1) __syncthreads();
   }
 }
 
@@ -737,18 +813,21 @@ int64_t align32(int64_t n) { return (n + 31) / 32 * 32; }
 int64_t own_bytes(const GltKv8Cache& c, const GltKv8Batch& b, int nh) {
   return align32(static_cast<int64_t>(b.rows) * nh * (c.head_dim + 2) * 4);
 }
+template <int SPLIT>
 int launch_join(const AttnArgs& a, const PrefixParts& parts, cudaStream_t st) {
-  const int64_t most = static_cast<int64_t>(kv8_most_new(a.c, a.b)) * a.nh * (a.c.head_dim / 4);
+  const int64_t rows = static_cast<int64_t>(kv8_most_new(a.c, a.b)) * a.nh, set = kJoinWarps / SPLIT * (256 / a.c.head_dim);
+  // as many CTAs as are resident at once go through all rows, if they are enough for a sequence each
+  const int64_t resident = (static_cast<int64_t>(num_sms()) * 8 + a.b.num_seqs - 1) / a.b.num_seqs;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>((most + kThreads - 1) / kThreads, 4096)), a.b.num_seqs);
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(std::min((rows + set - 1) / set, resident)), a.b.num_seqs);
+  cfg.blockDim = dim3(32 * kJoinWarps);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  GLT_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv8_prefix_join_kernel, a, parts));
+  GLT_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv8_prefix_join_kernel<SPLIT>, a, parts));
   GLT_LAUNCH_CHECK();
   return GLT_OK;
 }
@@ -800,5 +879,7 @@ extern "C" int glt_kv8_prefix_attention(const GltKv8Cache* cache, const GltKv8Ba
       GLT_TRY((int8 ? glt::launch_prefix<64, GLT_KV8_INT8>(x, st) : glt::launch_prefix<64, GLT_KV8_E4M3>(x, st)));
   }
   GLT_TRY(glt::launch_all<glt::Mode::kPrefix>(a, p, st));
-  return glt::launch_join(a, parts, st);
+  // rows of more than a few parts go to several warps: with one each, 2048 rows of 20 parts took 10 us where four
+  // take XXX; 18944 rows of 3 parts 60 us with four, XXX with one
+  return (parts.lanes == 2 ? 1 : 2) * parts.grid > 4 * parts.units() ? glt::launch_join<4>(a, parts, st) : glt::launch_join<1>(a, parts, st);
 }

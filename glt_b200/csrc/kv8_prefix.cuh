@@ -2,9 +2,9 @@
 // sequence's own tokens.
 //
 // Query rows (token x head of the group) of one KV head are cut into tiles of 128.  A unit is one KV head with
-// `lanes` neighbouring tiles; its steps of 128 tokens, laid end to end with those of all units, are dealt to
-// the CTAs in equal runs.  A CTA leaves, for each unit it has steps of, unnormalised sums of values, maxima (base 2)
-// and sums of weights in a slot of its own.
+// `lanes` neighbouring tiles; its steps of 128 tokens and what it costs to begin and to end it, laid end to end with
+// those of all units, are dealt to the CTAs in equal runs.  A CTA leaves, for each unit it has steps of,
+// unnormalised sums of values, maxima (base 2) and sums of weights in a slot of its own.
 #pragma once
 
 #include "kv8.cuh"
@@ -13,6 +13,7 @@ namespace glt {
 
 constexpr int kPrefixStep = 128;   // tokens of a step
 constexpr int kPrefixRows = 128;   // query rows of a tile
+constexpr int kPrefixUnitCost = 2;   // what laying out a unit's queries and writing its result cost, in steps
 
 struct PrefixParts {
   const int32_t* length;   // dev [1]
@@ -36,21 +37,26 @@ struct PrefixParts {
   }
 };
 
-// The steps of all units in equal runs, the first `more` of them one longer.
+// The costs of all units (kPrefixUnitCost and the steps) in equal runs, the first `more` of them one longer.
 struct PrefixShares {
   int64_t each;
   int steps, ctas, more;
   __device__ __forceinline__ PrefixShares(const PrefixParts& p, int tokens) {
     steps = (tokens + kPrefixStep - 1) / kPrefixStep;
-    const int64_t total = static_cast<int64_t>(steps) * p.units();
+    const int64_t total = steps > 0 ? static_cast<int64_t>(steps + kPrefixUnitCost) * p.units() : 0;
     ctas = total < p.grid ? static_cast<int>(total) : p.grid;
-    each = ctas > 0 ? total / ctas : 0;
+    each = ctas > 0 ? quotient(total, ctas) : 0;
     more = static_cast<int>(total - each * ctas);
+  }
+  // by the much shorter 32-bit division where that is enough
+  static __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+    if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    return a / b;
   }
   __device__ __forceinline__ int64_t begin(int i) const { return each * i + min(i, more); }
   __device__ __forceinline__ int owner(int64_t x) const {
     const int64_t head = (each + 1) * more;
-    return static_cast<int>(x < head ? x / (each + 1) : more + (x - head) / each);
+    return static_cast<int>(x < head ? quotient(x, each + 1) : more + quotient(x - head, each));
   }
 };
 
