@@ -33,7 +33,7 @@ namespace {
 constexpr int kSoftmaxWarps = 8, kDecodeWarps = 4, kIssueWarp = kSoftmaxWarps + kDecodeWarps;
 constexpr int kCopyWarp = kIssueWarp + 2;   // an issuing warp for each lane
 constexpr int kPrefixThreads = 32 * (kCopyWarp + 1);
-constexpr int kHalf = 64;   // tokens of an S
+constexpr int kAhead = 2;   // steps that K is laid out ahead of V
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
 constexpr float kLift = 7.f;          // base 2: what the reference counts in f16, whose top is 2^16
 constexpr float kMostSum = 0x1p15f;   // of 16 tokens, before the reference moves
@@ -50,29 +50,28 @@ struct PrefixArgs {
   unsigned int* err;
 };
 
-// Scales of a stage's groups of 16 tokens.  flags: bit g, the group's block is not in the pool; bit 8 + g, its values are 0.
+// Scales of a step's groups of 16 tokens.  flags: bit g, the group's block is not in the pool; bit 4 + g, its values are 0.
 struct alignas(16) PrefixNote {
-  float k[8], log_v[8], inv_v[8];
+  float k[4], log_v[4], inv_v[4];
   int flags, pad[3];
 };
-
-constexpr int kRawTokens = 64;   // of K or V, in an element of the ring of codes
-constexpr int kNotes = 8;        // steps whose scales are held: more than can be under way
+constexpr int kNotes = 16;   // steps whose scales are held: more than can be under way
+constexpr int kSlots = 3;    // steps of K, and of V, that are laid out
 
 template <int HD, int LANES>
 struct PrefixSmem {
   static constexpr int kQ = kPrefixRows * HD * 2;
   static constexpr int kPart = kPrefixStep * HD * 2;   // K (or V) of a step
-  static constexpr int kRaw = kRawTokens * HD;
-  static constexpr int kRaws = LANES == 2 ? 4 : 8;     // a step is four
-  static constexpr int kOffK = LANES * kQ;             // two steps each
-  static constexpr int kOffV = kOffK + 2 * kPart;
-  static constexpr int kOffRaw = kOffV + 2 * kPart;
+  static constexpr int kRaw = kPrefixStep * HD;        // its codes
+  static constexpr int kRaws = LANES == 2 ? 8 : 12;
+  static constexpr int kOffK = LANES * kQ;
+  static constexpr int kOffV = kOffK + kSlots * kPart;
+  static constexpr int kOffRaw = kOffV + kSlots * kPart;
   static constexpr int kOffNotes = kOffRaw + kRaws * kRaw;
   static constexpr int kOffBars = kOffNotes + kNotes * static_cast<int>(sizeof(PrefixNote));
-  static constexpr int kBars = 2 * kRaws + 8 + 8 + 2 + 3;
+  static constexpr int kBars = 2 * kRaws + 4 * kSlots + 8 + 2 + 3;
   static constexpr int kOffUnits = kOffBars + (kBars + 2) * 8;
-  static constexpr int kTotal = 1024 + kOffUnits + kPrefixRows * 4;
+  static constexpr int kTotal = 1024 + kOffUnits + (LANES == 1 ? kPrefixRows * 4 : 0);
 };
 static_assert(PrefixSmem<128, 1>::kTotal <= 232448 && PrefixSmem<128, 2>::kTotal <= 232448, "shared memory");
 
@@ -191,7 +190,12 @@ struct PrefixRun {
     if (left > 0 && s1 <= s0) next();   // only a part of the unit's cost
   }
   __device__ __forceinline__ bool on() const { return left > 0; }
-  __device__ __forceinline__ bool last() const { return left <= steps + kPrefixUnitCost - place + kPrefixUnitCost; }
+  // On to the next step.
+  __device__ __forceinline__ void step(int& s) {
+    if (++s < s1) return;
+    next();
+    s = on() ? s0 : 0;
+  }
   __device__ __forceinline__ void next() {
     left -= steps + kPrefixUnitCost - place;
     ++unit;
@@ -204,19 +208,19 @@ template <int HD, int FMT, int LANES>
 __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __grid_constant__ PrefixArgs a) {
   using L = PrefixSmem<HD, LANES>;
   constexpr uint32_t kBf16 = (1u << 7) | (1u << 10);   // operand types of a descriptor: f16 is 0
-  constexpr uint32_t kIdescS = tc::make_idesc(kHalf, false, false) & ~kBf16, kIdescO = tc::make_idesc(HD, false, true) & ~kBf16;
+  constexpr uint32_t kIdescS = tc::make_idesc(kPrefixStep, false, false) & ~kBf16, kIdescO = tc::make_idesc(HD, false, true) & ~kBf16;
   constexpr uint32_t kColO = 256;   // TMEM: two S of lane 0, of lane 1 (64 columns each), O of lane 0, of lane 1 (128 each)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = smem_raw + (-tc::smem_u32(smem_raw) & 1023u);   // the swizzle goes by address
   PrefixNote* notes = reinterpret_cast<PrefixNote*>(smem + L::kOffNotes);
   uint64_t* raw_full = reinterpret_cast<uint64_t*>(smem + L::kOffBars);
   uint64_t* raw_empty = raw_full + L::kRaws;
-  uint64_t* k_full = raw_empty + L::kRaws;   // [2] K of a step is laid out, is read (and so on for V)
-  uint64_t* k_empty = k_full + 2;
-  uint64_t* v_full = k_empty + 2;
-  uint64_t* v_empty = v_full + 2;
-  uint64_t* s_full = v_empty + 2;            // [lane][half] S is there
-  uint64_t* p_full = s_full + 4;             // [lane][half] P is there
+  uint64_t* k_full = raw_empty + L::kRaws;   // K of a step is laid out, is read (and so on for V)
+  uint64_t* k_empty = k_full + kSlots;
+  uint64_t* v_full = k_empty + kSlots;
+  uint64_t* v_empty = v_full + kSlots;
+  uint64_t* s_full = v_empty + kSlots;       // [lane][2] S is there
+  uint64_t* p_full = s_full + 4;             // [lane][2] P is there
   uint64_t* o_full = p_full + 4;             // [lane] O has a P more
   uint64_t* q_full = o_full + 2;             // the unit's queries are laid out
   uint64_t* unit_done = q_full + 1;          // all products of the unit are done
@@ -232,18 +236,18 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
       tc::mbar_init(raw_full + i, 1);
       tc::mbar_init(raw_empty + i, kDecodeWarps);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kSlots; ++i) {
       tc::mbar_init(k_full + i, kDecodeWarps);
       tc::mbar_init(k_empty + i, LANES);
       tc::mbar_init(v_full + i, kDecodeWarps);
       tc::mbar_init(v_empty + i, LANES);
-      tc::mbar_init(o_full + i, 1);
     }
+    for (int i = 0; i < 2; ++i) tc::mbar_init(o_full + i, 1);
     for (int i = 0; i < 4; ++i) {
-      tc::mbar_init(s_full + i, 1);
+      tc::mbar_init(s_full + i, 2);   // the products, and their issuer, who has seen the step's note
       tc::mbar_init(p_full + i, 4);
     }
-    tc::mbar_init(q_full, 4 * LANES);
+    tc::mbar_init(q_full, kSoftmaxWarps);   // both lanes', so that neither falls a unit behind
     tc::mbar_init(unit_done, 2);
     tc::mbar_init(drain, 2);
     abort = 0;
@@ -270,8 +274,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
     const uint32_t s_at = at + mine * 128, o_at = at + kColO + mine * 128;
     // x / group for x < group + 4: the quotient is at most 4, and no multiple lies as near as 2^-32 of it
     const uint32_t group_inverse = a.group > 1 ? 0xFFFFFFFFu / static_cast<uint32_t>(a.group) + 1 : 0;
-    uint32_t s_phase = 0;
-    int seg = 0, base = 0, products = 0;   // steps before the unit's, the lane's products with V so far
+    int seg = 0, base = 0, products = 0;   // steps before the unit's, the lane's steps so far
     for (; run.on() && !abort; run.next(), ++seg) {
       const int kvh = run.unit % a.parts.kv_heads, pair = run.unit / a.parts.kv_heads;
       // ---- queries: a warp its threads' rows, kPer lanes to a row
@@ -326,7 +329,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
         fence_async_smem();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(q_full);
-      } else if (n > 1) {   // it has steps
+      } else {
+        if (lane == 0) tc::mbar_arrive(q_full);
         if (!__all_sync(0xffffffffu, tc::mbar_wait(q_full, seg & 1, a.err, &abort))) {
           abort = 1;
           break;
@@ -335,105 +339,95 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
       }
       float m = -INFINITY, l = 0.f;
       bool any = false;
-      for (int i = LANES == 2 ? 0 : mine; i < n && !abort; i += LANES == 2 ? 1 : 2, s_phase ^= 1) {
-        const PrefixNote& note = notes[(base + i) % kNotes];
-        // (K is long laid out when S is there: waited for so that the step's note is seen)
-        if (!__all_sync(0xffffffffu, tc::mbar_wait(k_full + ((base + i) & 1), ((base + i) >> 1) & 1, a.err, &abort))) {
+      for (int i = LANES == 2 ? 0 : mine; i < n && !abort; i += LANES == 2 ? 1 : 2) {
+        const int it = base + i, buf = products & 1;
+        const PrefixNote& note = notes[it % kNotes];
+        if (!__all_sync(0xffffffffu, tc::mbar_wait(s_full + 2 * mine + buf, products >> 1 & 1, a.err, &abort))) {
           abort = 1;
           break;
         }
-        const int flags = note.flags;
-        const int left = tokens - (run.s0 + i) * kPrefixStep;   // tokens of the step
-        // not unrolled: with all roles' code unrolled, warps waited for instructions more than for anything else
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
-          float u[4], w[4];   // of the groups of 16 tokens
-          four(note.k + 4 * half, u);
-          four(note.log_v + 4 * half, w);
-          if (!__all_sync(0xffffffffu, tc::mbar_wait(s_full + 2 * mine + half, s_phase, a.err, &abort))) {
-            abort = 1;
-            break;
-          }
-          tc::tc_fence_after();
-          const uint32_t s_half = s_at + half * kHalf;
-          float v[kHalf];
-          tmem_ld64(s_half, v);
+        tc::tc_fence_after();
+        float u[4], w[4];   // of the groups of 16 tokens
+        four(note.k, u);
+        four(note.log_v, w);
+        const int flags = note.flags, left = tokens - (run.s0 + i) * kPrefixStep;   // tokens of the step
+        const uint32_t s_buf = s_at + buf * kPrefixStep;
+        float v[kPrefixStep];
+        tmem_ld64(s_buf, v);
 #pragma unroll
-          for (int g = 0; g < 4; ++g) u[g] = fmaxf(u[g] * unit_q, 1e-37f);   // above 0, so that a masked -inf stays one
-          const int gone = flags >> (4 * half);
-          if (left < (half + 1) * kHalf || (gone & 0xF)) {
+        for (int g = 0; g < 4; ++g) u[g] = fmaxf(u[g] * unit_q, 1e-37f);   // above 0, so that a masked -inf stays one
+        if (left < kPrefixStep || (flags & 0xF)) {
 #pragma unroll
-            for (int j = 0; j < kHalf; ++j)
-              if (j >= left - half * kHalf || (gone >> (j / 16) & 1)) v[j] = -INFINITY;
-          }
-          // P by the reference as it stands.  A unit's first S moves it, and one whose weights would come near f16's
-          // top, which the sums show: the maximum is taken then, and only then.
-          float sums[4];
-          bool moved = false;
-#pragma unroll 1
-          while (true) {
-            const float ref = kLift - (m == -INFINITY ? 0.f : m);
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              uint32_t p[8];
-              const float r = ref + w[g];
-              const uint64_t u2 = two_floats(u[g], u[g]), r2 = two_floats(r, r);
-              uint64_t sum = 0;
-#pragma unroll
-              for (int j = 0; j < 16; j += 2) {
-                const uint64_t e = fma2(two_floats(v[16 * g + j], v[16 * g + j + 1]), u2, r2);
-                const float p0 = ex2_approx(low(e)), p1 = ex2_approx(high(e));
-                sum = add2(sum, two_floats(p0, p1));
-                p[j / 2] = pack_f16x2(p0, p1);
-              }
-              sums[g] = low(sum) + high(sum);
-              tmem_st8(s_half + 8 * g, p);   // over S, which is read
-            }
-            const bool high = fmaxf(fmaxf(sums[0], sums[1]), fmaxf(sums[2], sums[3])) > kMostSum;
-            if (moved || !__any_sync(0xffffffffu, high || m == -INFINITY)) break;
-            moved = true;
-            float peak = -INFINITY;
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              float x[4] = {v[16 * g], v[16 * g + 1], v[16 * g + 2], v[16 * g + 3]};
-#pragma unroll
-              for (int j = 4; j < 16; ++j) x[j & 3] = fmaxf(x[j & 3], v[16 * g + j]);
-              peak = fmaxf(peak, fmaf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), u[g], w[g]));
-            }
-            const bool grow = peak > m;   // rows of the warp that need not move do no harm
-            const float f = grow ? (m == -INFINITY ? 0.f : ex2_approx(m - peak)) : 1.f;
-            if (any) {
-              // the lane's last product with V is done, and the next one waits for this P
-              if (!__all_sync(0xffffffffu, tc::mbar_wait(o_full + mine, (products - 1) & 1, a.err, &abort))) {
-                abort = 1;
-                break;
-              }
-              tc::tc_fence_after();
-#pragma unroll 1
-              for (int c = 0; c < HD; c += 16) {
-                float o[16];
-                tmem_ld16(o_at + c, o);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) o[j] *= f;
-                tmem_st16(o_at + c, o);
-              }
-            }
-            if (grow) {
-              l *= f;
-              m = peak;
-            }
-          }
-          if (abort) break;
-          any = true;
-          ++products;
-          four(note.inv_v + 4 * half, u);
-#pragma unroll
-          for (int g = 0; g < 4; ++g) l = fmaf(sums[g], u[g], l);
-          tmem_wait_st();
-          tc::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(p_full + 2 * mine + half);
+          for (int j = 0; j < kPrefixStep; ++j)
+            if (j >= left || (flags >> (j / 16) & 1)) v[j] = -INFINITY;
         }
+        // P by the reference as it stands.  A unit's first S moves it, and one whose weights would come near f16's
+        // top, which the sums show: the maximum is taken then, and only then.
+        float sums[4];
+        bool moved = false;
+#pragma unroll 1
+        while (true) {
+          const float ref = kLift - (m == -INFINITY ? 0.f : m);
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            uint32_t p[8];
+            const float r = ref + w[g];
+            const uint64_t u2 = two_floats(u[g], u[g]), r2 = two_floats(r, r);
+            uint64_t sum = 0;
+#pragma unroll
+            for (int j = 0; j < 16; j += 2) {
+              const uint64_t e = fma2(two_floats(v[16 * g + j], v[16 * g + j + 1]), u2, r2);
+              const float p0 = ex2_approx(low(e)), p1 = ex2_approx(high(e));
+              sum = add2(sum, two_floats(p0, p1));
+              p[j / 2] = pack_f16x2(p0, p1);
+            }
+            sums[g] = low(sum) + high(sum);
+            tmem_st8(s_buf + 8 * g, p);   // over S, which is read
+          }
+          const bool high = fmaxf(fmaxf(sums[0], sums[1]), fmaxf(sums[2], sums[3])) > kMostSum;
+          if (moved || !__any_sync(0xffffffffu, high || m == -INFINITY)) break;
+          moved = true;
+          float peak = -INFINITY;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            float x[4] = {v[16 * g], v[16 * g + 1], v[16 * g + 2], v[16 * g + 3]};
+#pragma unroll
+            for (int j = 4; j < 16; ++j) x[j & 3] = fmaxf(x[j & 3], v[16 * g + j]);
+            peak = fmaxf(peak, fmaf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), u[g], w[g]));
+          }
+          const bool grow = peak > m;   // rows of the warp that need not move do no harm
+          const float f = grow ? (m == -INFINITY ? 0.f : ex2_approx(m - peak)) : 1.f;
+          if (any) {
+            // the lane's last product with V is done, and the next one waits for this P
+            if (!__all_sync(0xffffffffu, tc::mbar_wait(o_full + mine, (products - 1) & 1, a.err, &abort))) {
+              abort = 1;
+              break;
+            }
+            tc::tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 16) {
+              float o[16];
+              tmem_ld16(o_at + c, o);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[j] *= f;
+              tmem_st16(o_at + c, o);
+            }
+          }
+          if (grow) {
+            l *= f;
+            m = peak;
+          }
+        }
+        if (abort) break;
+        any = true;
+        ++products;
+        four(note.inv_v, u);
+#pragma unroll
+        for (int g = 0; g < 4; ++g) l = fmaf(sums[g], u[g], l);
+        tmem_wait_st();
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(p_full + 2 * mine + buf);
       }
       // ---- the unit's result
       if (abort || !__all_sync(0xffffffffu, tc::mbar_wait(unit_done, seg & 1, a.err, &abort))) {
@@ -465,162 +459,186 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
     }
   } else if (warp < kIssueWarp) {
     // ------------------------------- codes ---------------------------------
-    constexpr int kChunks = HD / 16;                                   // 16 channels of a token
-    constexpr int kMine = kRawTokens * kChunks / kDecodeThreads;       // of a thread, of an element of the ring
+    constexpr int kChunks = HD / 16;                                    // 16 channels of a token
+    constexpr int kMine = kPrefixStep * kChunks / kDecodeThreads;       // of a thread, of an element of the ring
     const int tid = threadIdx.x - 32 * kSoftmaxWarps;
     const int chunk = tid % kChunks, tok0 = tid / kChunks;
-    int it = 0, raw = 0;
+    int raw = 0;
     uint32_t raw_phase = 0;
-    // The step's K or V; tokens that are not there become 0 (P is 0 there, and 0 times a NaN would not be).
-    auto lay = [&](uint8_t* dst, int left, bool values) {
-      int flags = 0;
-#pragma unroll 1
-      for (int u = 0; u < kPrefixStep; u += kRawTokens) {
-        if (!__all_sync(0xffffffffu, tc::mbar_wait(raw_full + raw, raw_phase, a.err, &abort))) return false;
-        if (u == 0) {
-          flags = notes[it % kNotes].flags;
-          if (values) flags |= flags >> 8;
-        }
-        const uint8_t* src = smem + L::kOffRaw + raw * L::kRaw + tid * 16;
-        uint4 x[kMine];
+    // The K or V of step `it`; tokens that are not there become 0 (P is 0 there, and 0 times a NaN would not be).
+    auto lay = [&](uint8_t* dst, int it, int left, bool values) {
+      if (!__all_sync(0xffffffffu, tc::mbar_wait(raw_full + raw, raw_phase, a.err, &abort))) return false;
+      int flags = notes[it % kNotes].flags;
+      if (values) flags |= flags >> 4;
+      const uint8_t* src = smem + L::kOffRaw + raw * L::kRaw + tid * 16;
+      uint4 x[kMine];
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) x[i] = *reinterpret_cast<const uint4*>(src + i * (kDecodeThreads * 16));
+      for (int i = 0; i < kMine; ++i) x[i] = *reinterpret_cast<const uint4*>(src + i * (kDecodeThreads * 16));
+      uint8_t* row = dst + (chunk >> 2) * (kPrefixStep * 128) + tok0 * 128;
+      const int c = 2 * (chunk & 3), turn = tok0 & 7;
+      static_assert(kDecodeThreads / kChunks % 8 == 0, "a thread's tokens are swizzled alike");
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-          const int tok = u + tok0 + i * (kDecodeThreads / kChunks);
-          uint4 lo, hi;
-          sixteen_f16<FMT>(x[i], lo, hi);
-          if (tok >= left || (flags >> (tok >> 4) & 1)) lo = hi = make_uint4(0, 0, 0, 0);
-          uint8_t* row = dst + (chunk >> 2) * (kPrefixStep * 128) + tok * 128;
-          const int c = 2 * (chunk & 3);
-          *reinterpret_cast<uint4*>(row + ((c ^ (tok & 7)) << 4)) = lo;
-          *reinterpret_cast<uint4*>(row + (((c + 1) ^ (tok & 7)) << 4)) = hi;
-        }
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(raw_empty + raw);
-        if (++raw == L::kRaws) {
-          raw = 0;
-          raw_phase ^= 1;
-        }
+      for (int i = 0; i < kMine; ++i) {
+        const int tok = tok0 + i * (kDecodeThreads / kChunks);
+        uint4 lo, hi;
+        sixteen_f16<FMT>(x[i], lo, hi);
+        if (tok >= left || (flags >> (tok >> 4) & 1)) lo = hi = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(row + i * (kDecodeThreads / kChunks * 128) + ((c ^ turn) << 4)) = lo;
+        *reinterpret_cast<uint4*>(row + i * (kDecodeThreads / kChunks * 128) + (((c + 1) ^ turn) << 4)) = hi;
       }
       fence_async_smem();
       __syncwarp();
+      if (lane == 0) tc::mbar_arrive(raw_empty + raw);
+      if (++raw == L::kRaws) {
+        raw = 0;
+        raw_phase ^= 1;
+      }
       return true;
     };
-    for (; run.on() && !abort; run.next())
-      for (int step = run.s0; step < run.s1; ++step, ++it) {
-        const int slot = it & 1, left = tokens - step * kPrefixStep;
-        const uint32_t free_phase = ((it >> 1) & 1) ^ 1;
-        bool ok = __all_sync(0xffffffffu, tc::mbar_wait(k_empty + slot, free_phase, a.err, &abort)) &&
-                  lay(smem + L::kOffK + slot * L::kPart, left, false);
-        if (ok && lane == 0) tc::mbar_arrive(k_full + slot);
-        ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(v_empty + slot, free_phase, a.err, &abort)) &&
-             lay(smem + L::kOffV + slot * L::kPart, left, true);
-        if (ok && lane == 0) tc::mbar_arrive(v_full + slot);
-        if (!ok) {
-          abort = 1;
-          break;
-        }
+    int step = run.on() ? run.s0 : 0, left[kAhead + 1] = {};
+    for (int it = 0, end = INT_MAX - kAhead; !abort && it < end + kAhead; ++it) {
+      bool ok = true;
+#pragma unroll
+      for (int i = kAhead; i > 0; --i) left[i] = left[i - 1];
+      if (it < end && !run.on()) end = it;
+      if (it < end) {
+        left[0] = tokens - step * kPrefixStep;
+        run.step(step);
+        ok = __all_sync(0xffffffffu, tc::mbar_wait(k_empty + it % kSlots, (it / kSlots & 1) ^ 1, a.err, &abort)) &&
+             lay(smem + L::kOffK + it % kSlots * L::kPart, it, left[0], false);
+        if (ok && lane == 0) tc::mbar_arrive(k_full + it % kSlots);
       }
+      if (ok && it >= kAhead && it < end + kAhead) {
+        const int v = it - kAhead;
+        ok = __all_sync(0xffffffffu, tc::mbar_wait(v_empty + v % kSlots, (v / kSlots & 1) ^ 1, a.err, &abort)) &&
+             lay(smem + L::kOffV + v % kSlots * L::kPart, v, left[kAhead], true);
+        if (ok && lane == 0) tc::mbar_arrive(v_full + v % kSlots);
+      }
+      if (!ok) abort = 1;
+    }
   } else if (warp == kCopyWarp) {
     // ------------------------------- copies --------------------------------
     const int bt = a.c.block_tokens, bt_log = 31 - __clz(bt);
-    const int piece = min(bt, kRawTokens);   // tokens of a copy
-    int it = 0, raw = 0;
+    const int piece = min(bt, kPrefixStep);   // tokens of a copy
+    int raw = 0;
     uint32_t raw_phase = 1;
-    // lane g < 8: the block of tokens 16 g .. of a step, read a step ahead
-    auto there = [&](int step) { return lane < 8 && step * kPrefixStep + 16 * lane < tokens; };
-    auto block = [&](int step) { return there(step) ? a.block_ids[(step * kPrefixStep + 16 * lane) >> bt_log] : -1; };
-    int id = run.on() ? block(run.s0) : -1;
-    for (; run.on() && !abort; run.next())
-      for (int step = run.s0; step < run.s1; ++step, ++it) {
-        const int kvh = run.unit % a.parts.kv_heads;
-        const bool in = id >= 0 && id < a.c.num_blocks, gone = !in && there(step);
-        const int64_t hb = in ? static_cast<int64_t>(id) * a.c.num_kv_heads + kvh : 0;
-        const float ks = in ? a.c.k_scale[hb] : 0.f, vs = in ? a.c.v_scale[hb] : 0.f;
+    // Lane g < 4 has tokens 16 g .. of a step.  Its block's id is read two steps ahead, its scales one.
+    struct Place {
+      bool on, in;     // the run has the step; its block is in the pool
+      int step, unit;
+      int64_t row;     // id, then block and head in the pool, then token
+      float k, v;
+    };
+    int step = run.on() ? run.s0 : 0;
+    auto read_id = [&]() {
+      Place x = {run.on(), false, step, run.unit, -1, 0.f, 0.f};
+      if (x.on && lane < 4 && step * kPrefixStep + 16 * lane < tokens)
+        x.row = a.block_ids[(step * kPrefixStep + 16 * lane) >> bt_log];
+      if (x.on) run.step(step);
+      return x;
+    };
+    auto read_scales = [&](Place& x) {
+      x.in = x.row >= 0 && x.row < a.c.num_blocks;
+      const int64_t hb = x.in ? x.row * a.c.num_kv_heads + x.unit % a.parts.kv_heads : 0;
+      x.k = x.in ? a.c.k_scale[hb] : 0.f;
+      x.v = x.in ? a.c.v_scale[hb] : 0.f;
+      x.row = (hb << bt_log) + ((x.step * kPrefixStep + 16 * lane) & (bt - 1));
+    };
+    // one lane for each copy: that of the copy's first 16 tokens
+    const bool leads = lane < 4 && 16 * lane % piece == 0;
+    auto copy = [&](const uint8_t* pool, bool in, int64_t row) {
+      const int copies = __popc(__ballot_sync(0xffffffffu, leads && in));
+      if (lane == 0) tc::mbar_arrive_expect_tx(raw_full + raw, copies * piece * HD);
+      __syncwarp();
+      if (leads && in) bulk_load(smem + L::kOffRaw + raw * L::kRaw + 16 * lane * HD, pool + row * HD, piece * HD, raw_full + raw);
+      ++copied;
+      if (++raw == L::kRaws) {
+        raw = 0;
+        raw_phase ^= 1;
+      }
+    };
+    auto free = [&]() { return __all_sync(0xffffffffu, tc::mbar_wait(raw_empty + raw, raw_phase, a.err, &abort)) != 0; };
+    Place now = read_id();
+    read_scales(now);
+    Place next = read_id();
+    bool in_v[kAhead + 1] = {};
+    int64_t row_v[kAhead + 1] = {};
+    for (int it = 0, end = INT_MAX - kAhead; !abort && it < end + kAhead; ++it) {
+      bool ok = true;
+#pragma unroll
+      for (int i = kAhead; i > 0; --i) in_v[i] = in_v[i - 1], row_v[i] = row_v[i - 1];
+      if (it < end && !now.on) end = it;
+      if (it < end) {
+        in_v[0] = now.in;
+        row_v[0] = now.row;
+        const bool gone = lane < 4 && !now.in && now.step * kPrefixStep + 16 * lane < tokens, some = !(now.v < kLeastScale);
         if (gone && a.err) atomicOr(a.err, GLT_DEVERR_BAD_SHAPE);
-        const bool more = step + 1 < run.s1;   // (a following unit begins with step 0)
-        id = more || !run.last() ? block(more ? step + 1 : 0) : -1;
-        bool ok = true;
-        for (int part = 0; ok && part < 4; ++part) {   // K, K, V, V
-          const int u = (part & 1) * kRawTokens;
-          ok = __all_sync(0xffffffffu, tc::mbar_wait(raw_empty + raw, raw_phase, a.err, &abort));
-          if (!ok) break;
-          if (part == 0) {
-            const bool some = !(vs < kLeastScale);
-            const unsigned lost = __ballot_sync(0xffffffffu, gone), none = __ballot_sync(0xffffffffu, lane < 8 && !some);
-            PrefixNote& note = notes[it % kNotes];
-            if (lane < 8) {
-              note.k[lane] = ks;
-              note.log_v[lane] = some ? log2f(vs) : -60.f;
-              note.inv_v[lane] = some ? 1.f / vs : 0x1p60f;
-            }
-            if (lane == 0) note.flags = static_cast<int>(lost | none << 8);
+        const unsigned lost = __ballot_sync(0xffffffffu, gone), none = __ballot_sync(0xffffffffu, lane < 4 && !some);
+        const float ks = now.k, vs = now.v;
+        read_scales(next);
+        now = next;
+        next = read_id();
+        ok = free();
+        if (ok) {
+          PrefixNote& note = notes[it % kNotes];
+          if (lane < 4) {
+            note.k[lane] = ks;
+            note.log_v[lane] = some ? log2f(vs) : -60.f;
+            note.inv_v[lane] = some ? 1.f / vs : 0x1p60f;
           }
-          // one lane for each copy: that of the copy's first 16 tokens
-          const int t = 16 * lane - u;   // in the element
-          const bool mine = in && t >= 0 && t < kRawTokens && t % piece == 0;
-          const int copies = __popc(__ballot_sync(0xffffffffu, mine));
-          if (lane == 0) tc::mbar_arrive_expect_tx(raw_full + raw, copies * piece * HD);
+          if (lane == 0) note.flags = static_cast<int>(lost | none << 4);
           __syncwarp();
-          if (mine)
-            bulk_load(smem + L::kOffRaw + raw * L::kRaw + t * HD,
-                      (part < 2 ? a.c.k : a.c.v) + ((hb << bt_log) + ((step * kPrefixStep + 16 * lane) & (bt - 1))) * HD, piece * HD,
-                      raw_full + raw);
-          ++copied;
-          if (++raw == L::kRaws) {
-            raw = 0;
-            raw_phase ^= 1;
-          }
-        }
-        if (!ok) {
-          abort = 1;
-          break;
+          copy(a.c.k, in_v[0], row_v[0]);
         }
       }
+      if (ok && it >= kAhead && it < end + kAhead) {
+        ok = free();
+        if (ok) copy(a.c.v, in_v[kAhead], row_v[kAhead]);
+      }
+      if (!ok) abort = 1;
+    }
   } else if (warp < kCopyWarp && lane == 0) {
     // ------------------------------- products ------------------------------
     const int mine = warp - kIssueWarp;
     const uint32_t q = tc::smem_u32(smem) + (LANES == 2 ? mine * L::kQ : 0), k_at = tc::smem_u32(smem + L::kOffK),
-                   v_at = tc::smem_u32(smem + L::kOffV), p = tmem + mine * 128, o = tmem + kColO + mine * 128;
-    uint32_t p_phase = 0;
+                   v_at = tc::smem_u32(smem + L::kOffV), s = tmem + mine * 128, o = tmem + kColO + mine * 128;
     bool ok = true;
-    int base = 0;   // steps before the unit's
+    int base = 0, scored = 0, summed = 0;   // steps before the unit's; the lane's S and P so far
     for (int seg = 0; ok && run.on() && !abort; run.next(), ++seg) {
       const int n = run.s1 - run.s0, first = LANES == 2 ? 0 : mine, by = LANES == 2 ? 1 : 2;
       ok = tc::mbar_wait(q_full, seg & 1, a.err, &abort);
-      // S of half a step runs a step ahead of its P: the other half's softmax has the time between
-      auto scores = [&](int i, int half) {
-        const int step = base + i, slot = step & 1;
-        if (half == 0 && !tc::mbar_wait(k_full + slot, (step >> 1) & 1, a.err, &abort)) return false;
+      // S runs two of the lane's steps ahead of its P, so that the softmax of one has the time between
+      auto scores = [&](int i) {
+        const int it = base + i, slot = it % kSlots;
+        if (!tc::mbar_wait(k_full + slot, it / kSlots & 1, a.err, &abort)) return false;
         tc::tc_fence_after();
-        const uint32_t kk = k_at + slot * L::kPart + half * kHalf * 128;
+        const uint32_t kk = k_at + slot * L::kPart, buf = scored++ & 1;
 #pragma unroll
         for (int j = 0; j < HD / 16; ++j)
-          tc::umma_bf16(p + half * kHalf, tc::desc_kmajor(q + (j >> 2) * (kPrefixRows * 128), j & 3),
+          tc::umma_bf16(s + buf * kPrefixStep, tc::desc_kmajor(q + (j >> 2) * (kPrefixRows * 128), j & 3),
                         tc::desc_kmajor(kk + (j >> 2) * (kPrefixStep * 128), j & 3), kIdescS, j > 0);
-        tc::umma_commit(s_full + 2 * mine + half);
-        if (half) tc::umma_commit(k_empty + slot);
+        tc::mbar_arrive(s_full + 2 * mine + buf);
+        tc::umma_commit(s_full + 2 * mine + buf);
+        tc::umma_commit(k_empty + slot);
         return true;
       };
-      for (int half = 0; half < 2; ++half)
-        if (ok && first < n) ok = scores(first, half);
-      for (int i = first; ok && i < n; i += by, p_phase ^= 1) {
-        const int step = base + i, slot = step & 1;
-        ok = tc::mbar_wait(v_full + slot, (step >> 1) & 1, a.err, &abort);
-        for (int half = 0; ok && half < 2; ++half) {
-          ok = tc::mbar_wait(p_full + 2 * mine + half, p_phase, a.err, &abort);
-          if (!ok) break;
-          tc::tc_fence_after();
-          const uint32_t vv = v_at + slot * L::kPart + half * kHalf * 128;
+      if (ok && first < n) ok = scores(first);
+      if (ok && first + by < n) ok = scores(first + by);
+      for (int i = first; ok && i < n; i += by) {
+        const int it = base + i, slot = it % kSlots, buf = summed & 1;
+        ok = tc::mbar_wait(v_full + slot, it / kSlots & 1, a.err, &abort) &&
+             tc::mbar_wait(p_full + 2 * mine + buf, summed >> 1 & 1, a.err, &abort);
+        if (!ok) break;
+        ++summed;
+        tc::tc_fence_after();
+        const uint32_t vv = v_at + slot * L::kPart;
 #pragma unroll
-          for (int j = 0; j < kHalf / 16; ++j)
-            umma_p(o, p + half * kHalf + 8 * j, tc::make_sdesc(vv + j * 2048, kPrefixStep * 128, 1024), kIdescO,
-                   !(i == first && half == 0 && j == 0));
-          tc::umma_commit(o_full + mine);
-          if (half) tc::umma_commit(v_empty + slot);
-          if (i + by < n) ok = scores(i + by, half);
-        }
+        for (int j = 0; j < kPrefixStep / 16; ++j)
+          umma_p(o, s + buf * kPrefixStep + 8 * j, tc::make_sdesc(vv + j * 2048, kPrefixStep * 128, 1024), kIdescO,
+                 !(i == first && j == 0));
+        tc::umma_commit(o_full + mine);
+        tc::umma_commit(v_empty + slot);
+        if (i + 2 * by < n) ok = scores(i + 2 * by);
       }
       if (ok) tc::umma_commit(unit_done);
       base += n;

@@ -2,7 +2,7 @@
 // sequence's own tokens.
 //
 // Query rows (token x head of the group) of one KV head are cut into tiles of 128.  A unit is one KV head with
-// `lanes` neighbouring tiles; its steps of 128 tokens and what it costs to begin and to end it, laid end to end with
+// `lanes` neighbouring tiles; its steps of 64 tokens and what it costs to begin and to end it, laid end to end with
 // those of all units, are dealt to the CTAs in equal runs.  A CTA leaves, for each unit it has steps of,
 // unnormalised sums of values, maxima (base 2) and sums of weights in a slot of its own.
 #pragma once
@@ -11,9 +11,9 @@
 
 namespace glt {
 
-constexpr int kPrefixStep = 128;   // tokens of a step
+constexpr int kPrefixStep = 64;    // tokens of a step
 constexpr int kPrefixRows = 128;   // query rows of a tile
-constexpr int kPrefixUnitCost = 2;   // what laying out a unit's queries and writing its result cost, in steps
+constexpr int kPrefixUnitCost = 4;   // what laying out a unit's queries and writing its result cost, in steps
 
 struct PrefixParts {
   const int32_t* length;   // dev [1]
