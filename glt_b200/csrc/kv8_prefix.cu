@@ -465,56 +465,74 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
     const int chunk = tid % kChunks, tok0 = tid / kChunks;
     int raw = 0;
     uint32_t raw_phase = 0;
-    // The K or V of step `it`; tokens that are not there become 0 (P is 0 there, and 0 times a NaN would not be).
-    auto lay = [&](uint8_t* dst, int it, int left, bool values) {
+    static_assert(kDecodeThreads / kChunks % 8 == 0, "a thread's tokens are swizzled alike");
+    const int c = 2 * (chunk & 3), turn = tok0 & 7;
+    const int off_lo = (chunk >> 2) * (kPrefixStep * 128) + tok0 * 128 + ((c ^ turn) << 4), off_hi = off_lo ^ 16;
+    // The next element of the ring, once it is there.
+    auto take = [&](uint4 (&x)[kMine], int& from) {
       if (!__all_sync(0xffffffffu, tc::mbar_wait(raw_full + raw, raw_phase, a.err, &abort))) return false;
-      int flags = notes[it % kNotes].flags;
-      if (values) flags |= flags >> 4;
       const uint8_t* src = smem + L::kOffRaw + raw * L::kRaw + tid * 16;
-      uint4 x[kMine];
 #pragma unroll
       for (int i = 0; i < kMine; ++i) x[i] = *reinterpret_cast<const uint4*>(src + i * (kDecodeThreads * 16));
-      uint8_t* row = dst + (chunk >> 2) * (kPrefixStep * 128) + tok0 * 128;
-      const int c = 2 * (chunk & 3), turn = tok0 & 7;
-      static_assert(kDecodeThreads / kChunks % 8 == 0, "a thread's tokens are swizzled alike");
-#pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int tok = tok0 + i * (kDecodeThreads / kChunks);
-        uint4 lo, hi;
-        sixteen_f16<FMT>(x[i], lo, hi);
-        if (tok >= left || (flags >> (tok >> 4) & 1)) lo = hi = make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(row + i * (kDecodeThreads / kChunks * 128) + ((c ^ turn) << 4)) = lo;
-        *reinterpret_cast<uint4*>(row + i * (kDecodeThreads / kChunks * 128) + (((c + 1) ^ turn) << 4)) = hi;
-      }
-      fence_async_smem();
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(raw_empty + raw);
+      from = raw;
       if (++raw == L::kRaws) {
         raw = 0;
         raw_phase ^= 1;
       }
       return true;
     };
+    // Tokens that are not there become 0 (P is 0 there, and 0 times a NaN would not be).
+    auto lay = [&](const uint4 (&x)[kMine], uint8_t* dst, int left, int flags) {
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const int tok = tok0 + i * (kDecodeThreads / kChunks);
+        uint4 lo, hi;
+        sixteen_f16<FMT>(x[i], lo, hi);
+        if (tok >= left || (flags >> (tok >> 4) & 1)) lo = hi = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(dst + off_lo + i * (kDecodeThreads / kChunks * 128)) = lo;
+        *reinterpret_cast<uint4*>(dst + off_hi + i * (kDecodeThreads / kChunks * 128)) = hi;
+      }
+    };
     int step = run.on() ? run.s0 : 0, left[kAhead + 1] = {};
+    // K of a step goes with V of the step kAhead before: one turn's latencies for both
     for (int it = 0, end = INT_MAX - kAhead; !abort && it < end + kAhead; ++it) {
-      bool ok = true;
 #pragma unroll
       for (int i = kAhead; i > 0; --i) left[i] = left[i - 1];
       if (it < end && !run.on()) end = it;
-      if (it < end) {
+      const bool with_k = it < end, with_v = it >= kAhead && it < end + kAhead;
+      if (with_k) {
         left[0] = tokens - step * kPrefixStep;
         run.step(step);
-        ok = __all_sync(0xffffffffu, tc::mbar_wait(k_empty + it % kSlots, (it / kSlots & 1) ^ 1, a.err, &abort)) &&
-             lay(smem + L::kOffK + it % kSlots * L::kPart, it, left[0], false);
-        if (ok && lane == 0) tc::mbar_arrive(k_full + it % kSlots);
       }
-      if (ok && it >= kAhead && it < end + kAhead) {
-        const int v = it - kAhead;
-        ok = __all_sync(0xffffffffu, tc::mbar_wait(v_empty + v % kSlots, (v / kSlots & 1) ^ 1, a.err, &abort)) &&
-             lay(smem + L::kOffV + v % kSlots * L::kPart, v, left[kAhead], true);
-        if (ok && lane == 0) tc::mbar_arrive(v_full + v % kSlots);
+      const int v = it - kAhead, slot_k = it % kSlots, slot_v = v % kSlots;
+      uint4 xk[kMine], xv[kMine];
+      int from_k = 0, from_v = 0;
+      bool ok = true;
+      if (with_k)
+        ok = __all_sync(0xffffffffu, tc::mbar_wait(k_empty + slot_k, (it / kSlots & 1) ^ 1, a.err, &abort)) && take(xk, from_k);
+      if (ok && with_v)
+        ok = __all_sync(0xffffffffu, tc::mbar_wait(v_empty + slot_v, (v / kSlots & 1) ^ 1, a.err, &abort)) && take(xv, from_v);
+      if (!ok) {
+        abort = 1;
+        break;
       }
-      if (!ok) abort = 1;
+      if (with_k) lay(xk, smem + L::kOffK + slot_k * L::kPart, left[0], notes[it % kNotes].flags);
+      if (with_v) {
+        const int flags = notes[v % kNotes].flags;
+        lay(xv, smem + L::kOffV + slot_v * L::kPart, left[kAhead], flags | flags >> 4);
+      }
+      fence_async_smem();
+      __syncwarp();
+      if (lane == 0) {
+        if (with_k) {
+          tc::mbar_arrive(k_full + slot_k);
+          tc::mbar_arrive(raw_empty + from_k);
+        }
+        if (with_v) {
+          tc::mbar_arrive(v_full + slot_v);
+          tc::mbar_arrive(raw_empty + from_v);
+        }
+      }
     }
   } else if (warp == kCopyWarp) {
     // ------------------------------- copies --------------------------------
