@@ -27,7 +27,7 @@ namespace {
 struct QuantArgs {
   const uint16_t* x;
   int64_t ld_x;
-  int K;
+  int rows, K;
   const uint16_t* norm;   // NULL: none
   float eps;
   int8_t* codes;
@@ -45,7 +45,7 @@ __device__ __forceinline__ uint4 load_vec(const uint16_t* row, int v, int K, boo
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The largest (or the sum) of all threads' values, in every thread.
+// The largest (or the sum) of all threads' values of a row, in every thread.
 template <int THREADS, bool MAX>
 __device__ __forceinline__ float block_join(float v, float* sm) {
   v = MAX ? warp_max(v) : warp_sum(v);
@@ -90,99 +90,116 @@ __device__ __forceinline__ uint2 encode8(const float (&y)[8], float s, float inv
   return make_uint2(four(c[0], c[1], c[2], c[3]), four(c[4], c[5], c[6], c[7]));
 }
 
-// VECS vectors of eight values a thread; VECS = 0: any length, read again for each pass.
+// VECS vectors of eight values a thread; VECS = 0: any length, read again for each pass.  A CTA takes one row after the
+// other; the next one's loads are under way while a row is worked on, whose values stay in registers from the norm to the
+// codes: for many tokens the instructions bound it (8192 rows of 4096 with their norm: XXX).
 template <int THREADS, int VECS, bool NORM>
-__global__ void __launch_bounds__(THREADS) w8_quantize_kernel(const QuantArgs a) {
+__global__ void __launch_bounds__(THREADS, 1024 / THREADS) w8_quantize_kernel(const QuantArgs a) {
   __shared__ float sm[THREADS / 32];
   asm volatile("griddepcontrol.launch_dependents;");
-  const uint16_t* row = a.x + static_cast<int64_t>(blockIdx.x) * a.ld_x;
-  const bool aligned = (reinterpret_cast<uintptr_t>(row) & 15u) == 0;
-  const bool g_aligned = NORM && (reinterpret_cast<uintptr_t>(a.norm) & 15u) == 0;
   const int vecs = (a.K + 15) / 16 * 2;   // codes are written up to a multiple of 16
-  uint4 held[VECS > 0 ? VECS : 1];
-  auto for_each = [&](auto&& f) {
-    if constexpr (VECS > 0) {
-#pragma unroll
-      for (int i = 0; i < VECS; ++i) {
-        const int v = threadIdx.x + i * THREADS;
-        if (v < vecs) f(v, held[i]);
-      }
-    } else {
-      for (int v = threadIdx.x; v < vecs; v += THREADS) f(v, load_vec(row, v, a.K, aligned));
-    }
-  };
-  if constexpr (VECS > 0) {
+  const bool g_aligned = NORM && (reinterpret_cast<uintptr_t>(a.norm) & 15u) == 0;
+  constexpr int kHeld = VECS > 0 ? VECS : 1;
+  uint4 ahead[kHeld];
+  auto row_of = [&](int64_t r) { return a.x + r * a.ld_x; };
+  auto is_aligned = [&](int64_t r) { return (reinterpret_cast<uintptr_t>(row_of(r)) & 15u) == 0; };
+  auto load = [&](int64_t r) {
+    const bool aligned = is_aligned(r);
 #pragma unroll
     for (int i = 0; i < VECS; ++i) {
       const int v = threadIdx.x + i * THREADS;
-      if (v < vecs) held[i] = load_vec(row, v, a.K, aligned);
-    }
-  }
-  float r = 1.f;
-  if constexpr (NORM) {
-    float sum = 0.f;
-    for_each([&](int, const uint4& u) {
-      float f[8];
-      unpack8(u, f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum = fmaf(f[i], f[i], sum);
-    });
-    sum = block_join<THREADS, false>(sum, sm);
-    const bool scaled = sum == INFINITY;
-    if (scaled) {
-      sum = 0.f;
-      for_each([&](int, const uint4& u) {
-        float f[8];
-        unpack8(u, f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sum += square_scaled(f[i]);
-      });
-      sum = block_join<THREADS, false>(sum, sm);
-    }
-    r = norm_factor(sum, a.K, a.eps, scaled);
-  }
-  auto values = [&](int v, const uint4& u, float (&y)[8]) {
-    unpack8(u, y);
-    if constexpr (NORM) {
-      float g[8];
-      unpack8(load_vec(a.norm, v, a.K, g_aligned), g);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = y[i] * r * g[i];
+      ahead[i] = v < vecs ? load_vec(row_of(r), v, a.K, aligned) : make_uint4(0, 0, 0, 0);
     }
   };
-  float peak = 0.f;
-  bool bad = false;
-  for_each([&](int v, const uint4& u) {
-    float y[8];
-    values(v, u, y);
+  if (VECS > 0) load(blockIdx.x);
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    float y[kHeld][8];
+    if constexpr (VECS > 0) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      peak = fmaxf(peak, fabsf(y[i]));
-      bad |= !(fabsf(y[i]) <= FLT_MAX);
+      for (int i = 0; i < VECS; ++i) unpack8(ahead[i], y[i]);
+      if (r + gridDim.x < a.rows) load(r + gridDim.x);
     }
-  });
-  peak = block_join<THREADS, true>(bad ? INFINITY : peak, sm);
-  // a row that holds an infinity or NaN has no scale: it says so
-  const float s = peak <= FLT_MAX ? __fdiv_rn(peak, 127.f) : __uint_as_float(0x7FC00000u);
-  if (threadIdx.x == 0) a.scales[blockIdx.x] = s;
-  const bool common = s >= 0x1p-100f && s <= 0x1p100f;   // reciprocals and remainders are normal numbers
-  const float inv = __frcp_rn(s);
-  int8_t* out = a.codes + static_cast<int64_t>(blockIdx.x) * a.ld_codes;
-  for_each([&](int v, const uint4& u) {
-    float y[8];
-    values(v, u, y);
-    *reinterpret_cast<uint2*>(out + v * 8) = encode8(y, s, inv, common);
-  });
+    // f(vector's index, its eight values as they stand)
+    float factor = 1.f;
+    bool normed = false;
+    auto for_each = [&](auto&& f) {
+      if constexpr (VECS > 0) {
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) f(threadIdx.x + i * THREADS, y[i]);
+      } else {
+        const bool aligned = is_aligned(r);
+        for (int v = threadIdx.x; v < vecs; v += THREADS) {
+          unpack8(load_vec(row_of(r), v, a.K, aligned), y[0]);
+          if (normed) {
+            float g[8];
+            unpack8(load_vec(a.norm, v, a.K, g_aligned), g);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[0][j] = y[0][j] * factor * g[j];
+          }
+          f(v, y[0]);
+        }
+      }
+    };
+    if constexpr (NORM) {
+      float sum = 0.f;
+      for_each([&](int, float (&f)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum = fmaf(f[j], f[j], sum);
+      });
+      sum = block_join<THREADS, false>(sum, sm);
+      const bool scaled = sum == INFINITY;
+      if (scaled) {
+        sum = 0.f;
+        for_each([&](int, float (&f)[8]) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum += square_scaled(f[j]);
+        });
+        sum = block_join<THREADS, false>(sum, sm);
+      }
+      factor = norm_factor(sum, a.K, a.eps, scaled);
+      normed = true;
+      if constexpr (VECS > 0) {
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) {
+          const int v = threadIdx.x + i * THREADS;
+          float g[8];
+          unpack8(v < vecs ? load_vec(a.norm, v, a.K, g_aligned) : make_uint4(0, 0, 0, 0), g);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) y[i][j] = y[i][j] * factor * g[j];
+        }
+      }
+    }
+    float peak = 0.f, odd = 0.f;   // odd: NaN when a value is NaN or infinite
+    for_each([&](int, float (&f)[8]) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        peak = fmaxf(peak, fabsf(f[j]));
+        odd = fmaf(f[j], 0.f, odd);
+      }
+    });
+    peak = block_join<THREADS, true>(odd == 0.f ? peak : INFINITY, sm);
+    // a row that holds an infinity or NaN has no scale: it says so
+    const float s = peak <= FLT_MAX ? __fdiv_rn(peak, 127.f) : __uint_as_float(0x7FC00000u);
+    if (threadIdx.x == 0) a.scales[r] = s;
+    const bool common = s >= 0x1p-100f && s <= 0x1p100f;   // reciprocals and remainders are normal numbers
+    const float inv = __frcp_rn(s);
+    int8_t* out = a.codes + r * a.ld_codes;
+    for_each([&](int v, float (&f)[8]) {
+      if (v < vecs) *reinterpret_cast<uint2*>(out + v * 8) = encode8(f, s, inv, common);
+    });
+  }
 }
 
 // A row goes to as many threads as hold it with up to four vectors each.
-int quantize(const QuantArgs& a, int rows, cudaStream_t st) {
+int quantize(const QuantArgs& a, cudaStream_t st) {
   auto go = [&](auto threads, auto vecs) {
     constexpr int T = decltype(threads)::value, V = decltype(vecs)::value;
+    const int most = num_sms() * (1024 / T);   // as many as are resident
+    const int grid = a.rows < most ? a.rows : most;
     if (a.norm)
-      w8_quantize_kernel<T, V, true><<<rows, T, 0, st>>>(a);
+      w8_quantize_kernel<T, V, true><<<grid, T, 0, st>>>(a);
     else
-      w8_quantize_kernel<T, V, false><<<rows, T, 0, st>>>(a);
+      w8_quantize_kernel<T, V, false><<<grid, T, 0, st>>>(a);
   };
   if (a.K <= 4096)
     go(std::integral_constant<int, 256>{}, std::integral_constant<int, 2>{});
@@ -207,10 +224,10 @@ struct ProductArgs {
   int M, N;
 };
 
-template <bool BF16>
-__device__ __forceinline__ void put(const ProductArgs& a, int m, int n, int sum, float t, float s) {
+template <bool BF16, bool RESID>
+__device__ __forceinline__ void put(const ProductArgs& a, int m, int n, int sum, float t, float s, uint16_t r) {
   float z = static_cast<float>(sum) * t * s;
-  if (a.resid) z += bf16_bits_to_f32(a.resid[m * a.ld_r + n]);
+  if (RESID) z += bf16_bits_to_f32(r);
   if (BF16)
     static_cast<uint16_t*>(a.y)[m * a.ld_y + n] = bf16_bits_rn(z);
   else
@@ -218,7 +235,7 @@ __device__ __forceinline__ void put(const ProductArgs& a, int m, int n, int sum,
 }
 
 // The pair kernel's epilogue: rows are channels, columns tokens.
-template <bool BF16>
+template <bool BF16, bool RESID>
 struct EpiW8 {
   static constexpr int kParts = 2;
   ProductArgs a;
@@ -228,13 +245,20 @@ struct EpiW8 {
 #pragma unroll 1
     for (int j = c.part * 128; j < c.part * 128 + 128; j += 32) {
       if (c.n0 + j >= a.M) break;
+      const int m0 = c.n0 + j, m1 = min(a.M, m0 + 32) - 1;
       float v[32];
+      uint16_t r[32];   // all reads before the first write, and none behind a branch of its own
+      if (RESID) {
+        const uint16_t* from = a.resid + (on ? c.row : 0);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) r[i] = from[min(m0 + i, m1) * a.ld_r];
+      }
+      const float s = a.x_scales[min(m0 + static_cast<int>(threadIdx.x & 31), m1)];   // a lane's token
       c.load(j, v);
-      if (!on) continue;
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
-        const int m = c.n0 + j + i;
-        if (m < a.M) put<BF16>(a, m, c.row, __float_as_int(v[i]), t, a.x_scales[m]);
+        const float si = __shfl_sync(0xffffffffu, s, i);
+        if (on && m0 + i <= m1) put<BF16, RESID>(a, m0 + i, c.row, __float_as_int(v[i]), t, si, RESID ? r[i] : 0);
       }
     }
   }
@@ -258,18 +282,17 @@ constexpr int kChannels = 128;   // of a CTA of the stream kernel
 constexpr int kStreamThreads = 192;
 constexpr int kMaxShares = 8;    // CTAs of a cluster
 
-// Two CTAs an SM for up to 64 tokens, whose stages are small; else one.
 template <int NT>
 struct Stream {
   static constexpr int kA = kChannels * 128, kB = NT * 128, kStage = kA + kB;
-  static constexpr int kCtasPerSm = NT <= 64 ? 2 : 1;
-  static constexpr int kStages = (kCtasPerSm == 2 ? 110 * 1024 : 220 * 1024) / kStage;
+  static constexpr int kCtasPerSm = 2;
+  static constexpr int kStages = 110 * 1024 / kStage;
   static constexpr int kSmem = 1024 + kStages * kStage + (2 * kStages + 2) * 8 + 16;
   static constexpr int kTmem = NT < 32 ? 32 : NT;
 };
 
 // shares: CTAs of the cluster, blockIdx.x % shares is the CTA's.
-template <int NT, bool BF16>
+template <int NT, bool BF16, bool RESID>
 __global__ void __launch_bounds__(kStreamThreads) w8_stream_kernel(const __grid_constant__ CUtensorMap map_w,
                                                                   const __grid_constant__ CUtensorMap map_x, int blocks,
                                                                   int shares, const ProductArgs a, unsigned int* err) {
@@ -361,7 +384,7 @@ __global__ void __launch_bounds__(kStreamThreads) w8_stream_kernel(const __grid_
   }
   // The cluster's integers.  Each CTA adds up a run of `chunk` tokens and takes the others' parts of it into the
   // memory of its ring, which is free once all its products are done.
-  const int tokens = min(NT, a.M - m0), chunk = (tokens + shares - 1) / shares;
+  const int tokens = min(NT, a.M - m0), chunk = ((tokens + shares - 1) / shares + 7) & ~7;
   bool good = true;
   if (warp >= 2) {
     good = __all_sync(0xffffffffu, tc::mbar_wait(done, 0, err, &abort));
@@ -377,16 +400,17 @@ __global__ void __launch_bounds__(kStreamThreads) w8_stream_kernel(const __grid_
       for (int to = 0; to < shares; ++to) {
         const int c0 = to * chunk, c1 = min(tokens, c0 + chunk);
         if (to == share || c0 >= c1) continue;
-        // part `share` (less one behind the receiver's own) of the receiver's memory: [part][token][channel]
+        // part `share` (less one behind the receiver's own) of the receiver's memory: [part][four tokens][channel][token]
         const uint32_t dst = tc::mapa_shared(
-            tc::smem_u32(smem) + ((share - (share > to ? 1 : 0)) * chunk * kChannels + ch) * 4, static_cast<uint32_t>(to));
-        for (int c = c0 & ~7; c < c1; c += 8) {
+            tc::smem_u32(smem) + ((share - (share > to ? 1 : 0)) * chunk * kChannels + ch * 4) * 4, static_cast<uint32_t>(to));
+        for (int c = c0; c < c1; c += 8) {
           uint32_t v[8];
           tmem_ld8(from + static_cast<uint32_t>(c), v);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (c + i >= c0 && c + i < c1)
-              asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(dst + (c + i - c0) * kChannels * 4), "r"(v[i]) : "memory");
+          for (int i = 0; i < 8; i += 4)
+            asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst + (c + i - c0) * kChannels * 4),
+                         "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3])
+                         : "memory");
         }
       }
     }
@@ -396,17 +420,28 @@ __global__ void __launch_bounds__(kStreamThreads) w8_stream_kernel(const __grid_
   if (warp >= 2 && good) {
     const int c0 = share * chunk, c1 = min(tokens, c0 + chunk);
     const float t = n < a.N ? a.w_scales[n] : 0.f;
-    for (int c = c0 & ~7; c < c1; c += 8) {
+    for (int c = c0; c < c1; c += 8) {
       uint32_t v[8];
-      tmem_ld8(from + static_cast<uint32_t>(c), v);
+      uint16_t r[8] = {};   // (y may be the residual: all reads before the first write)
+      float s[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        if (c + i < c0 || c + i >= c1) continue;
-        int sum = static_cast<int>(v[i]);
-        const int* part = reinterpret_cast<const int*>(smem) + (c + i - c0) * kChannels + ch;
-        for (int p = 0; p < shares - 1; ++p) sum += part[p * chunk * kChannels];
-        if (n < a.N) put<BF16>(a, m0 + c + i, n, sum, t, a.x_scales[m0 + c + i]);
+        const int m = m0 + min(c + i, c1 - 1);
+        s[i] = a.x_scales[m];
+        if (RESID) r[i] = a.resid[m * a.ld_r + min(n, a.N - 1)];
       }
+      tmem_ld8(from + static_cast<uint32_t>(c), v);
+      const int4* part = reinterpret_cast<const int4*>(smem) + (c - c0) / 4 * kChannels + ch;
+      for (int p = 0; p < shares - 1; ++p) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int4 x = part[p * (chunk / 4) * kChannels + h * kChannels];
+          v[4 * h] += x.x, v[4 * h + 1] += x.y, v[4 * h + 2] += x.z, v[4 * h + 3] += x.w;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (n < a.N && c + i < c1) put<BF16, RESID>(a, m0 + c + i, n, static_cast<int>(v[i]), t, s[i], r[i]);
     }
   }
   tc::tc_fence_before();
@@ -436,10 +471,10 @@ struct Codes {
   int64_t ld;
 };
 
-template <int NT, bool BF16>
+template <int NT, bool BF16, bool RESID>
 int launch_stream(const Codes& w, const Codes& x, int K16, const ProductArgs& a, bool after_quantize, cudaStream_t st) {
   using S = Stream<NT>;
-  auto kern = w8_stream_kernel<NT, BF16>;
+  auto kern = w8_stream_kernel<NT, BF16, RESID>;
   GLT_TRY(ensure_smem_attr(reinterpret_cast<const void*>(kern), S::kSmem));
   CUtensorMap map_w, map_x;
   GLT_TRY(make_tmap_bf16(&map_w, w.p, K16 / 2, a.N, w.ld / 2, kChannels));
@@ -448,11 +483,11 @@ int launch_stream(const Codes& w, const Codes& x, int K16, const ProductArgs& a,
   if (!err) return fail(GLT_ECUDA, "device error word unavailable");
   const int blocks = (K16 + 127) / 128;
   const int rows = (a.N + kChannels - 1) / kChannels, cols = (a.M + NT - 1) / NT;
-  // K is shared so that all CTAs are resident at once, each with four blocks of it at least
-  int shares = static_cast<int>(static_cast<int64_t>(num_sms()) * S::kCtasPerSm / (static_cast<int64_t>(rows) * cols));
-  if (shares > kMaxShares) shares = kMaxShares;
-  if (shares > blocks / 4) shares = blocks / 4;
-  if (shares < 1) shares = 1;
+  // K is shared so that all CTAs are resident at once, each with four blocks of it at least.  (Clusters of 6 CTAs
+  // for 48 tiles took 21 us with 64 tokens where XXX.)
+  int shares = kMaxShares;
+  while (shares > 1 && (static_cast<int64_t>(rows) * cols * shares > static_cast<int64_t>(num_sms()) * S::kCtasPerSm || shares > blocks / 4))
+    shares /= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(rows * shares, cols);
   cfg.blockDim = dim3(kStreamThreads);
@@ -472,17 +507,23 @@ int launch_stream(const Codes& w, const Codes& x, int K16, const ProductArgs& a,
   return GLT_OK;
 }
 
-template <bool BF16>
+template <bool BF16, bool RESID>
 int product(const Codes& w, const Codes& x, int K16, const ProductArgs& a, bool after_quantize, cudaStream_t st) {
-  if (a.M <= 16) return launch_stream<16, BF16>(w, x, K16, a, after_quantize, st);
-  if (a.M <= 32) return launch_stream<32, BF16>(w, x, K16, a, after_quantize, st);
-  if (a.M <= 64) return launch_stream<64, BF16>(w, x, K16, a, after_quantize, st);
-  if (a.M <= 128) return launch_stream<128, BF16>(w, x, K16, a, after_quantize, st);
-  if (a.M <= 256) return launch_stream<256, BF16>(w, x, K16, a, after_quantize, st);
+  if (a.M <= 16) return launch_stream<16, BF16, RESID>(w, x, K16, a, after_quantize, st);
+  if (a.M <= 32) return launch_stream<32, BF16, RESID>(w, x, K16, a, after_quantize, st);
+  // more tokens go 64 at a time while all tiles are resident at once
+  const int64_t tiles = static_cast<int64_t>((a.N + kChannels - 1) / kChannels) * ((a.M + 63) / 64);
+  if (tiles <= 2 * num_sms()) return launch_stream<64, BF16, RESID>(w, x, K16, a, after_quantize, st);
   // 16 tiles of 256 channels a raster group: the group's weights stay in L2 while all tokens pass
   return launch_gemm_pair<false, false, tc::PairS8>({w.p, w.ld / 2, false}, {x.p, x.ld / 2, false}, a.N, a.M, K16 / 2,
-                                                    EpiW8<BF16>{a}, st, 1, nullptr, INT_MAX, 16, nullptr, 0, nullptr,
+                                                    EpiW8<BF16, RESID>{a}, st, 1, nullptr, INT_MAX, 16, nullptr, 0, nullptr,
                                                     tc::GLT_MBAR_TIMEOUT_NS);
+}
+
+int product(const Codes& w, const Codes& x, int K16, const ProductArgs& a, int y_dtype, bool after_quantize, cudaStream_t st) {
+  if (a.resid)
+    return y_dtype ? product<true, true>(w, x, K16, a, after_quantize, st) : product<false, true>(w, x, K16, a, after_quantize, st);
+  return y_dtype ? product<true, false>(w, x, K16, a, after_quantize, st) : product<false, false>(w, x, K16, a, after_quantize, st);
 }
 
 int round16(int k) { return (k + 15) / 16 * 16; }
@@ -516,7 +557,7 @@ extern "C" int glt_w8_quantize_rows(const uint16_t* x, int64_t ld_x, int rows, i
   GLT_TRY(glt::check_codes(codes, ld_codes, K, "codes"));
   if (!x || !scales || ld_x < K) return glt::fail(GLT_EINVAL, "w8: null argument, or rows of x closer than %d", K);
   if (norm && !(eps >= 0.f && eps <= FLT_MAX)) return glt::fail(GLT_EINVAL, "w8: eps must be finite and not negative");
-  return glt::quantize({x, ld_x, K, norm, eps, codes, ld_codes, scales}, rows, static_cast<cudaStream_t>(stream));
+  return glt::quantize({x, ld_x, rows, K, norm, eps, codes, ld_codes, scales}, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int glt_w8_linear_rows(const int8_t* codes, int64_t ld_codes, const float* scales, int M, const int8_t* w,
@@ -529,9 +570,7 @@ extern "C" int glt_w8_linear_rows(const int8_t* codes, int64_t ld_codes, const f
   GLT_TRY(glt::check_out(y, ld_y, y_dtype, resid, ld_r, N));
   if (!scales || !w_scales) return glt::fail(GLT_EINVAL, "null argument");
   const glt::ProductArgs a = {scales, w_scales, y, ld_y, resid, ld_r, M, N};
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return y_dtype ? glt::product<true>({w, ld_w}, {codes, ld_codes}, glt::round16(K), a, false, st)
-                 : glt::product<false>({w, ld_w}, {codes, ld_codes}, glt::round16(K), a, false, st);
+  return glt::product({w, ld_w}, {codes, ld_codes}, glt::round16(K), a, y_dtype, false, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int glt_w8_linear_workspace(int M, int K, int64_t* bytes) {
@@ -557,7 +596,5 @@ extern "C" int glt_w8_linear(const uint16_t* x, int64_t ld_x, int M, const uint1
   const int K16 = glt::round16(K);
   GLT_TRY(glt_w8_quantize_rows(x, ld_x, M, K, norm, eps, codes, K16, scales, stream));
   const glt::ProductArgs a = {scales, w_scales, y, ld_y, resid, ld_r, M, N};
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  return y_dtype ? glt::product<true>({w, ld_w}, {codes, K16}, K16, a, true, st)
-                 : glt::product<false>({w, ld_w}, {codes, K16}, K16, a, true, st);
+  return glt::product({w, ld_w}, {codes, K16}, K16, a, y_dtype, true, static_cast<cudaStream_t>(stream));
 }

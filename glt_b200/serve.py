@@ -410,7 +410,7 @@ def quantize_rows(x: torch.Tensor, norm: torch.Tensor | None = None, eps: float 
             return quantize_rows(x, norm, eps)
     rows, K = x.shape
     ld_x, norm_at = _bf16_rows(x, dev, rows, K, "x"), _norm_weight(norm, dev, K)
-    codes = torch.empty((rows, (K + 15) // 16 * 16), dtype=_I8, device=x.device)
+    codes = torch.empty((rows, (K + 127) // 128 * 128), dtype=_I8, device=x.device)   # rows that begin with a line
     scales = torch.empty((rows,), dtype=_F32, device=x.device)
     check(lib.glt_w8_quantize_rows(x.data_ptr(), ld_x, rows, K, norm_at, eps, codes.data_ptr(), codes.shape[1],
                                    scales.data_ptr(), _stream(dev)))
@@ -441,7 +441,7 @@ class W8Weight:
         _one_device(codes=codes, scales=scales)
         _need(scales.dtype is _F32, "scales must be fp32")
         N, K = codes.shape
-        laid = torch.empty((N, (K + 15) // 16 * 16), dtype=_I8, device=codes.device)
+        laid = torch.empty((N, (K + 127) // 128 * 128), dtype=_I8, device=codes.device)   # rows that begin with a line
         laid[:, :K] = codes
         laid[:, K:] = 0
         return cls(W8Rows(laid[:, :K], scales.contiguous()))
