@@ -15,11 +15,20 @@
 //               tiles of rows at the same tokens; else every second step of the same rows.
 // A query row is brought to f16 by a power of two, as in kv8_attention.cuh.  The scale of K multiplies S in 32 bits.  The
 // scale of V joins the exponent: a token counts 2^(s + log2 scale - ref) in the sum of values, ref a running
-// maximum of that exponent, so that f16 has what one token can add at most near its top whatever the scales of the blocks
-// are: 11 bits down to 2^-29 of the row's largest summand, and below an absolute 2^-40 of it.  (P as the sum
-// of two bf16 numbers needs no such reference, but half as many products and instructions again: 306 us where
-// this took XXX, 512 rows a KV head, 65537 tokens.)  Over 1 / scale, in 32 bits, the same numbers make the sum of weights.
+// reference near the maximum of that exponent, so that f16 has what one token can add at most near its top whatever the
+// scales of the blocks are: 11 bits down to 2^-24 of the reference, and below that within 2^-35 of it.  Over 1 / scale,
+// in 32 bits, the same numbers make the sum of weights.  (P as the sum of two bf16 numbers needs no such
+// reference, but half as many products and instructions again: 306 us where f16 took 258, other things equal.)
 // The reference moves only when the weights come near f16's top.
+//
+// What bounds it: 4 rows hd operations a token are 83 us at the measured bf16 rate for 4096 rows (128 sequences, 32 heads over 8,
+// head_dim 128) behind 65537 tokens, of 194 us the call takes.  A step of 64 tokens and 256 rows takes a CTA 2400 cycles
+// where its products need 1300 of the tensor cores and its exponentials 1000 of their units: each of the
+// softmax's two warps a scheduler waits 700 of them for what it has just read or issued, at 0.4 instructions a cycle.  Sixteen
+// softmax warps of half a row each (72 registers) were slower, 234 us.  One result after the other: loops as short as here instead of
+// unrolled code 306 us for 423; scores ahead of the softmax, sums instead of maxima 204 for 258.
+// Few sequences are bound by beginnings and ends: 64 sequences behind 8193 tokens 55 us, of which the units' first loads, the
+// parts' way through memory (19 MB) and the own tokens' kernel are three quarters.
 #include <float.h>
 
 #include <algorithm>
@@ -35,7 +44,7 @@ constexpr int kCopyWarp = kIssueWarp + 2;   // an issuing warp for each lane
 constexpr int kPrefixThreads = 32 * (kCopyWarp + 1);
 constexpr int kAhead = 2;   // steps that K is laid out ahead of V
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
-constexpr float kLift = 7.f;          // base 2: what the reference counts in f16, whose top is 2^16
+constexpr float kLift = 10.f;         // base 2: what the reference counts in f16, whose top is 2^16 and last normal 2^-14
 constexpr float kMostSum = 0x1p15f;   // of 16 tokens, before the reference moves
 constexpr float kLeastScale = 0x1p-120f;   // of V: smaller ones count as 0, and weigh as 2^-60
 
@@ -915,7 +924,7 @@ extern "C" int glt_kv8_prefix_attention(const GltKv8Cache* cache, const GltKv8Ba
       GLT_TRY((int8 ? glt::launch_prefix<64, GLT_KV8_INT8>(x, st) : glt::launch_prefix<64, GLT_KV8_E4M3>(x, st)));
   }
   GLT_TRY(glt::launch_all<glt::Mode::kPrefix>(a, p, st));
-  // rows of more than a few parts go to several warps: with one each, 2048 rows of 20 parts took 10 us where four
-  // take XXX; 18944 rows of 3 parts 60 us with four, XXX with one
-  return (parts.lanes == 2 ? 1 : 2) * parts.grid > 4 * parts.units() ? glt::launch_join<4>(a, parts, st) : glt::launch_join<1>(a, parts, st);
+  // Rows of many parts go to four warps, others to one (the whole call: 2048 rows of 19 parts 54.8 us against 60.6, 42 of
+  // up to 26 16.9 against 21.9; 4096 of 10 197.8 against 194.1, 18944 of 3 128.1 against 111.6).
+  return (parts.lanes == 2 ? 1 : 2) * parts.grid > 12 * parts.units() ? glt::launch_join<4>(a, parts, st) : glt::launch_join<1>(a, parts, st);
 }

@@ -11,10 +11,15 @@
 // Product: weights are operand A of tcgen05.mma kind::i8 (128 or 256 channels), tokens operand B, so that a
 // thread of the epilogue owns a channel, a warp writes 32 neighbouring channels of a token whatever their alignment,
 // and few tokens cost few columns.  Two kernels:
-//   * few tokens: w8_stream_kernel, bound by the weights' bytes.  A CTA takes 128 channels and a share of K; the CTAs
+//   * w8_stream_kernel, bound by the weights' bytes.  A CTA takes 128 channels, up to 64 tokens and a share of K; the CTAs
 //     of a cluster share K and add their integers through distributed shared memory.  It starts
 //     (programmatic dependent launch) while the tokens are quantised and fills its ring with weights.
-//   * many tokens: the CTA-pair kernel of tc_gemm_pair.cuh with byte operands, bound by the tensor cores.
+//     8 tokens by 28672 x 4096: 22.7 us, 5.2 TB/s; 60 tokens by 32001 x 4097: 30.8 us, where every CTA's tokens come through L2 too.
+//   * the CTA-pair kernel of tc_gemm_pair.cuh with byte operands, bound by the tensor cores and, in long runs, the power
+//     limit: 8192 tokens by 28672 x 4096 654 us (2.9e15 operations a second), 2047 by 4096 x 14336 95 us (2.5e15: 128 tiles are
+//     1.7 rounds of 74 pairs).
+// The first goes on while all its tiles are resident at once: 64 / 65 tokens by 28672 x 4096 27.4 / 41.0 us against 33.8 / 34.8 by
+// pairs, 512 by 4096 x 4096 18.9 against 21.7, 400 by 6144 x 4096 30.1 against 21.7.
 #include <float.h>
 #include <limits.h>
 
@@ -92,7 +97,8 @@ __device__ __forceinline__ uint2 encode8(const float (&y)[8], float s, float inv
 
 // VECS vectors of eight values a thread; VECS = 0: any length, read again for each pass.  A CTA takes one row after the
 // other; the next one's loads are under way while a row is worked on, whose values stay in registers from the norm to the
-// codes: for many tokens the instructions bound it (8192 rows of 4096 with their norm: XXX).
+// codes: for many tokens the instructions bound it (8192 rows of 4096 with their norm: 34 us,
+// 0.44 of the copy rate; a warp a row, without barriers, took 64).
 template <int THREADS, int VECS, bool NORM>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) w8_quantize_kernel(const QuantArgs a) {
   __shared__ float sm[THREADS / 32];
@@ -483,8 +489,8 @@ int launch_stream(const Codes& w, const Codes& x, int K16, const ProductArgs& a,
   if (!err) return fail(GLT_ECUDA, "device error word unavailable");
   const int blocks = (K16 + 127) / 128;
   const int rows = (a.N + kChannels - 1) / kChannels, cols = (a.M + NT - 1) / NT;
-  // K is shared so that all CTAs are resident at once, each with four blocks of it at least.  (Clusters of 6 CTAs
-  // for 48 tiles took 21 us with 64 tokens where XXX.)
+  // K is shared so that all CTAs are resident at once, each with four blocks of it at least.  (Clusters of 6
+  // for 48 tiles took 21.2 us with 64 tokens where 4 take 12.6.)
   int shares = kMaxShares;
   while (shares > 1 && (static_cast<int64_t>(rows) * cols * shares > static_cast<int64_t>(num_sms()) * S::kCtasPerSm || shares > blocks / 4))
     shares /= 2;
