@@ -79,6 +79,7 @@ struct AttnArgs {
   unsigned int* err;
   int sinks;    // kSinks
   float* own;   // kPrefix: dev [rows, num_heads, head_dim] sums of values, then [rows, num_heads] maxima (base 2) and sums of weights
+  bool chained; // kPrefix: the launch before is the prefix's, so that this one may start while it runs
 };
 
 // What one sequence has to do: `steps` steps from token `lo` on (kSinks: the first `head` of them from token 0 on, the
@@ -1012,10 +1013,10 @@ int launch(const AttnArgs& a, int grid, cudaStream_t st) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  if (M == Mode::kPrefix) {   // starts while the prefix's kernel runs
+  if (M == Mode::kPrefix) {
     cfg.gridDim = dim3(grid);
     cfg.dynamicSmemBytes = bytes;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = a.chained ? 1 : 0;   // behind any other kernel, its writes would not be awaited
     GLT_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv8_attention_kernel<HD, FMT, NT, BT16, M>, a, map_k, map_v));
   } else {
     kv8_attention_kernel<HD, FMT, NT, BT16, M><<<grid, kThreads, bytes, st>>>(a, map_k, map_v);

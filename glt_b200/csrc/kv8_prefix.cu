@@ -915,7 +915,8 @@ extern "C" int glt_kv8_prefix_attention(const GltKv8Cache* cache, const GltKv8Ba
   a.own = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + first);
   parts.slots = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + second);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (parts.grid > 0) {
+  a.chained = parts.grid > 0;
+  if (a.chained) {
     const glt::PrefixArgs x = {*cache, prefix->block_ids, q, ld_q, batch->rows * a.group, a.group, a.scale, parts, a.err};
     const bool int8 = cache->format == GLT_KV8_INT8;
     if (cache->head_dim == 128)

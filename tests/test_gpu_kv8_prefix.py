@@ -286,6 +286,24 @@ def test_graphs_follow_the_lengths_and_do_not_share():
     assert take_error() == 0
 
 
+def test_a_prefix_without_blocks_waits_for_what_ran_before():
+    """Nothing of the call may start before the kernel that writes its queries has ended."""
+    c = Case("int8", 32, 2, 4, 64, 0, [300] * 64, [1] * 64, seed=16)
+    cache, batch, prefix, _ = c.objects()
+    assert prefix.blocks.numel() == 0
+    want = c.run()
+    c.check(*want)
+    big = torch.zeros(1 << 26, device=DEV, dtype=torch.bfloat16)
+    q = c.q.contiguous()
+    n = q.numel()
+    for _ in range(20):
+        big.zero_()
+        big[-n:].copy_(q.flatten())
+        got = cache.prefix_attention(batch, prefix, big[-n:].view(q.shape))
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert take_error() == 0
+
+
 def test_another_stream():
     c = Case("int8", 16, 2, 7, 64, 500, [33] * 4, [1] * 4, seed=15)
     want = c.run()
