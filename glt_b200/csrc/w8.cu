@@ -535,10 +535,11 @@ int product(const Codes& w, const Codes& x, int K16, const ProductArgs& a, int y
 int round16(int k) { return (k + 15) / 16 * 16; }
 // 131071 products of two bytes stay within 32 bits
 constexpr int kMaxK = 131071;
+constexpr int kMaxRows = INT_MAX - 255;   // rounded up to tiles they are 32-bit numbers still
 
 int check_sizes(int M, int N, int K) {
-  if (M < 0 || N < 1 || K < 1 || K > kMaxK)
-    return fail(GLT_EINVAL, "w8: sizes M %d, N %d, K %d (K at most %d)", M, N, K, kMaxK);
+  if (M < 0 || M > kMaxRows || N < 1 || N > kMaxRows || K < 1 || K > kMaxK)
+    return fail(GLT_EINVAL, "w8: sizes M %d, N %d (at most %d), K %d (at most %d)", M, N, kMaxRows, K, kMaxK);
   return GLT_OK;
 }
 int check_codes(const int8_t* p, int64_t ld, int K, const char* what) {

@@ -385,7 +385,7 @@ GLT_API int glt_w4_linear_workspace(int M, int N, int K, int group, int y_dtype,
  * glt_w8_linear_rows: y[M, N] = scale[m] * w_scale[n] * sum_k code[m, k] * w[n, k] (+ resid[m, n]), y bf16 (y_dtype 1) or
  *   fp32 (0), resid bf16 or NULL.  Codes are -128..127, laid out as above with zeros behind K.  Sums are exact.
  * glt_w8_linear: both, the codes of x in the workspace: glt_w8_linear_workspace bytes, 16-byte aligned,
- *   used by one call at a time; its contents do not matter.  K at most 131071. */
+ *   used by one call at a time; its contents do not matter.  K at most 131071, M and N at most 2^31 - 256. */
 GLT_API int glt_w8_quantize_rows(const uint16_t* x, int64_t ld_x, int rows, int K, const uint16_t* norm,
                                  float eps, int8_t* codes, int64_t ld_codes, float* scales, void* stream);
 GLT_API int glt_w8_linear_rows(const int8_t* codes, int64_t ld_codes, const float* scales, int M,

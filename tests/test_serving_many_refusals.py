@@ -138,6 +138,14 @@ def test_w8_products(call):
     refused(lib.glt_w8_linear_workspace(2, 0, C.byref(need)), "sizes")
 
 
+def test_w8_sizes_that_leave_32_bits_when_rounded_up():
+    top = 2 ** 31 - 255
+    refused(rows(n=top), "sizes")
+    for call in (product, linear):
+        refused(call(M=top), "sizes")
+        refused(call(N=top, ld_y=top), "sizes")
+
+
 # ---- the Python layer, on tensors that only say they lie on a GPU
 
 BF16, I8 = torch.bfloat16, torch.int8
