@@ -46,7 +46,8 @@ constexpr int kAhead = 2;   // steps that K is laid out ahead of V
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
 constexpr float kLift = 10.f;         // base 2: what the reference counts in f16, whose top is 2^16 and last normal 2^-14
 constexpr float kMostSum = 0x1p15f;   // of 16 tokens, before the reference moves
-constexpr float kLeastScale = 0x1p-120f;   // of V: smaller ones count as 0, and weigh as 2^-60
+// Of V: smaller ones count as 0, and weigh as 2^-60.  Over the scale, a weight's 2^10 stay within 32 bits for 2^27 tokens.
+constexpr float kLeastScale = 0x1p-90f;
 
 struct PrefixArgs {
   GltKv8Cache c;

@@ -5,6 +5,7 @@ Tolerance, for scores s (base 2) and weights p of the exact softmax:
   * the exponent s + log2(scale of v) - reference is rounded: (|s| + 150) 2^-23 more, in units of ln 2;
   * a weight is rounded to f16, 2^-11, and below f16's normal range by at most half of 2^-24, where the reference, which
     the row's largest summand reaches, counts 2^10: 2^-35 of that summand a token, times the largest code (512);
+  * values whose scale is below 2^-90 count as 0: what they add, sum p |v| over those, is missing;
   * the result to bf16, eps / 2."""
 import math
 
@@ -111,7 +112,8 @@ class Case:
                 ds = mags * (self.hd + 8) * 2.0 ** -23 + (mags * 1.45 + 150) * 2.0 ** -23
                 spread = torch.einsum("hgt,htd->hgd", p, val.abs())
                 flush = (p * s[:, None]).amax(-1) * key.shape[1] * 512 * 2.0 ** -35
-                tol = 2 * (2.0 ** -11 + 2 * ds)[..., None] * spread + flush[..., None]
+                gone_v = torch.einsum("hgt,htd->hgd", p * (s < 2.0 ** -90)[:, None], val.abs())
+                tol = 2 * (2.0 ** -11 + 2 * ds)[..., None] * spread + flush[..., None] + gone_v
                 tol = tol + torch.finfo(torch.bfloat16).eps / 2 * (want_o.abs() + tol) + 1e-30
                 assert ((got_o - want_o).abs() <= tol).all(), (b, i, ((got_o - want_o).abs() - tol).max().item())
                 tol_l = ds + (8 + key.shape[1] / 32) * 2.0 ** -23 + 2.0 ** -22 * want_l.abs()
@@ -154,6 +156,18 @@ def test_values_of_very_different_scales(fmt, rows):
     c.check(*c.run())
     c.vs[c.blocks.long()] = 0.0
     c.check(*c.run())
+
+
+@pytest.mark.parametrize("rows", [3, 50])
+@pytest.mark.parametrize("power", [-119, -111, -91, -89, -60, 100])
+def test_weights_count_whatever_the_values_scales(rows, power):
+    """Weights over scales of V that are tiny or huge stay within 32 bits: lse does not depend on V."""
+    c = Case("int8", 32, 2, 4, 64, 700, [40] * rows, [1] * rows, seed=17)
+    _, lse = c.run()
+    c.vs.fill_(2.0 ** power)
+    o, got = c.run()
+    c.check(o, got)
+    assert ((got - lse).abs() <= 2.0 ** -15 * (1 + lse.abs())).all()
 
 
 @pytest.mark.parametrize("q_amp", [0.0, 1e-3, 30.0, 1e4])
