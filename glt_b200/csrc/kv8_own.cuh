@@ -10,21 +10,16 @@
 // 11 bits down to 2^-29 of the row's largest summand, and below that within 2^-40 of it.
 //
 // What bounds it: latency, about 0.8 us a step of 16 tokens, of which the next step's codes are on their way during one
-// (fetching four steps ahead to L2 gained nothing).  So it is for short tables; whole calls behind 777 tokens, e4m3, head_dim 128,
-// other kernel / this one in us, by the tokens that a table holds:
-//                                                64             192             256             320
-//   16 sequences, 37 new tokens, 32 heads over 4  78.0 / 49.9     88.3 / 62.8     89.8 / 71.1     97.7 / 79.3
-//   128 sequences, 1 token, 32 heads over 8       43.3 / 31.5     53.7 / 42.9     56.5 / 47.9     62.8 / 54.8
-//   2 sequences, 37 new tokens, 32 heads over 4   33.5 / 24.1     37.0 / 30.0     38.1 / 34.0     40.2 / 37.6
-//   3 sequences, 1 token, 14 heads over 2         20.3 / 18.4     22.4 / 19.1     22.3 / 22.5     21.8 / 25.8
+// (fetching four steps ahead to L2 gained nothing).  So it is for short tables (own_is_short).
 #pragma once
+
+#include <algorithm>
 
 #include "kv8_attention.cuh"
 
 namespace glt {
 namespace {
 
-constexpr int kOwnMost = 256;   // tokens of a table
 constexpr int kOwnWarps = 4;
 constexpr int kOwnRows = 16;
 constexpr int kOwnStep = 16;   // tokens: blocks hold a multiple of them
@@ -226,9 +221,22 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) kv8_own_kernel(const __grid
   asm volatile("griddepcontrol.wait;" ::: "memory");   // who waits for this kernel waits for the prefix's
 }
 
+int own_tiles(const AttnArgs& a) { return (kv8_most_new(a.c, a.b) * a.group + kOwnRows - 1) / kOwnRows; }   // 32 bits: check_heads
+// Whether the sequences' tables hold so few tokens that this kernel is the faster one: the more warps there are, the more the ends of units
+// cost the other.  Whole calls behind 777 tokens, head_dim 128, e4m3, other kernel / this one in us, by the tokens of a table:
+//                                                            256            320            384            512
+//   1 sequence, 1 token, 32 heads over 8: 8 warps        21.9 / 22.5    22.4 / 25.3    22.8 / 28.7    21.7 / 34.7
+//   2 sequences, 37 tokens, 32 heads over 4: 152 warps   37.9 / 33.9    40.2 / 37.6    40.2 / 41.7    42.3 / 49.5
+//   64 sequences, 1 token, 32 heads over 8: 512          38.9 / 32.5    42.3 / 36.9    42.8 / 41.2    47.3 / 49.9
+//   128 sequences: 1024                                  55.4 / 48.4    62.2 / 54.4    64.1 / 59.9    70.5 / 68.2
+//   100 sequences, 5 tokens, 64 heads over 8: 2400       145 / 108      161 / 120      165 / 132      186 / 153
+bool own_is_short(const AttnArgs& a) {
+  const int64_t warps = static_cast<int64_t>(a.b.num_seqs) * a.c.num_kv_heads * own_tiles(a);
+  return static_cast<int64_t>(a.b.max_blocks) * a.c.block_tokens <= std::min<int64_t>(512, 256 + warps / 8);
+}
 template <int HD, int FMT>
 int launch_own(const AttnArgs& a, cudaStream_t st) {
-  const int tiles = (kv8_most_new(a.c, a.b) * a.group + kOwnRows - 1) / kOwnRows;   // 32 bits: check_heads
+  const int tiles = own_tiles(a);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((tiles * a.c.num_kv_heads + kOwnWarps - 1) / kOwnWarps, a.b.num_seqs);
   cfg.blockDim = dim3(32 * kOwnWarps);

@@ -22,7 +22,7 @@
 // The reference moves only when the weights come near f16's top.
 //
 // What bounds it: 4 rows hd operations a token are 83 us at the measured bf16 rate for 4096 rows (128 sequences, 32 heads over 8,
-// head_dim 128) behind 65537 tokens, of 194 us the call takes.  A step of 64 tokens and 256 rows takes a CTA 2400 cycles
+// head_dim 128) behind 65537 tokens, of 191 us the call takes.  A step of 64 tokens and 256 rows takes a CTA 2400 cycles
 // where its products need 1300 of the tensor cores and its exponentials 1000 of their units: each of the
 // softmax's two warps a scheduler waits 700 of them for what it has just read or issued, at 0.4 instructions a cycle.  Sixteen
 // softmax warps of half a row each (72 registers) were slower, 234 us.  One result after the other: loops as short as here instead of
@@ -926,7 +926,7 @@ extern "C" int glt_kv8_prefix_attention(const GltKv8Cache* cache, const GltKv8Ba
     else
       GLT_TRY((int8 ? glt::launch_prefix<64, GLT_KV8_INT8>(x, st) : glt::launch_prefix<64, GLT_KV8_E4M3>(x, st)));
   }
-  if (static_cast<int64_t>(batch->max_blocks) * cache->block_tokens <= glt::kOwnMost)
+  if (glt::own_is_short(a))
     GLT_TRY(glt::launch_own(a, st));
   else
     GLT_TRY(glt::launch_all<glt::Mode::kPrefix>(a, p, st));
