@@ -97,7 +97,7 @@ __device__ __forceinline__ uint2 encode8(const float (&y)[8], float s, float inv
 
 // VECS vectors of eight values a thread; VECS = 0: any length, read again for each pass.  A CTA takes one row after the
 // other; the next one's loads are under way while a row is worked on, whose values stay in registers from the norm to the
-// codes: for many tokens the instructions bound it (8192 rows of 4096 with their norm: 34 us,
+// codes: for many tokens instructions and the latency between barriers bound it (8192 rows of 4096 with their norm: 34 us,
 // 0.44 of the copy rate; a warp a row, without barriers, took 64).
 template <int THREADS, int VECS, bool NORM>
 __global__ void __launch_bounds__(THREADS, 1024 / THREADS) w8_quantize_kernel(const QuantArgs a) {
