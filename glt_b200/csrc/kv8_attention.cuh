@@ -82,13 +82,16 @@ struct AttnArgs {
   bool chained; // kPrefix: the launch before is the prefix's, so that this one may start while it runs
 };
 
-// What one sequence has to do: `steps` steps from token `lo` on (kSinks: the first `head` of them from token 0 on, the
-// others from token lo + 32 head on), for `units` units.
+// Steps that hold a sequence's first tokens.
+__device__ __forceinline__ int sink_steps(const AttnArgs& a) { return a.sinks / kStep + (a.sinks % kStep != 0); }
+
+// What one sequence has to do: `steps` steps from token `lo` on, for `units` units.  kSinks: the first sink_steps of them are from
+// token 0 on, and lo is 0 where the window's follow without a gap.
 struct SeqWork {
-  int past, n, row0, lo, steps, units, head;
+  int past, n, row0, lo, steps, units;
   template <Mode M>
-  __device__ __forceinline__ int token(int step) const {
-    return (M == Mode::kSinks && step < head ? 0 : lo) + step * kStep;
+  __device__ __forceinline__ int token(const AttnArgs& a, int step) const {
+    return (M == Mode::kSinks && step < sink_steps(a) ? 0 : lo) + step * kStep;
   }
   __device__ __forceinline__ int64_t cost() const { return static_cast<int64_t>(steps + kUnitCost) * units; }
 };
@@ -100,17 +103,7 @@ __device__ __forceinline__ SeqWork seq_work(const AttnArgs& a, int seq, unsigned
   w.n = s.n;
   w.row0 = s.row0;
   w.lo = a.window > 0 ? max(0, s.past - a.window + 1) & ~(kStep - 1) : 0;
-  w.head = 0;
-  if (M == Mode::kSinks) {
-    // steps of the first tokens, and then of the window: one run where no step lies between
-    const int head = a.sinks / kStep + (a.sinks % kStep != 0);
-    if (w.lo / kStep > head) {
-      w.head = head;
-      w.lo -= head * kStep;
-    } else {
-      w.lo = 0;
-    }
-  }
+  if (M == Mode::kSinks) w.lo = max(0, w.lo / kStep - sink_steps(a)) * kStep;
   w.steps = (s.past + s.n - w.lo + kStep - 1) / kStep;
   w.units = s.n > 0 ? a.c.num_kv_heads * ((s.n * a.group + ROWS - 1) / ROWS) : 0;   // n * group is checked on the host
   return w;
@@ -401,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
       ld_step = ld.s0 + warp;
     }
     if (ld.left > 0) {
-      const int t = ld.w.template token<M>(ld_step);
+      const int t = ld.w.template token<M>(a, ld_step);
       const int32_t* ids = a.b.block_table + static_cast<int64_t>(ld.seq) * a.b.max_blocks;
       // of a step's two blocks of 16 the first may lie before the window, and the last beyond the tokens
       ld_on[0] = LU == 1 || a.window == 0 || t + 15 > ld.w.past - a.window || (kSinks && t < a.sinks);
@@ -416,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
   int issued = 0;
   auto issue = [&]() {
     if (ld.left > 0) {
-      const int t0 = ld.w.template token<M>(ld_step);
+      const int t0 = ld.w.template token<M>(a, ld_step);
       uint64_t* bar = bars + ld_stage;
       uint8_t* dst = ring + ld_stage * R::kStage;
       int valid = 0;
@@ -563,7 +556,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
     const uint8_t* mrow = a.mask ? a.mask + cu.seq * a.ld_mask : nullptr;
     // A lane's token of a step, read a step early and looked at only then.
     auto mask_byte = [&](int step) {
-      const int t = cu.w.template token<M>(step) + lane;
+      const int t = cu.w.template token<M>(a, step) + lane;
       return step < cu.s1 && t <= pos_hi ? mrow[t] : static_cast<uint8_t>(0);
     };
     uint8_t ahead = mrow ? mask_byte(cu.s0 + warp) : 0;
@@ -585,7 +578,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
       uint8_t* sg = ring + stage * R::kStage;
       const float4 sc = *reinterpret_cast<const float4*>(notes[stage].scale);
       const int valid = notes[stage].valid;
-      const int t0 = cu.w.template token<M>(step);
+      const int t0 = cu.w.template token<M>(a, step);
       // ---- S^T
       float s[2][NT][4];
 #pragma unroll
