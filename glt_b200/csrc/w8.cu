@@ -63,14 +63,6 @@ __device__ __forceinline__ float block_join(float v, float* sm) {
   return r;
 }
 
-// The factor x / sqrt(mean x^2 + eps) of a row.  Sums of squares that leave the float range are taken again from
-// x / 2^64: a row of any finite bf16 has a finite norm.
-__device__ __forceinline__ float norm_factor(float sum, int K, float eps, bool scaled) {
-  if (!scaled) return rsqrtf(sum / K + eps);
-  return rsqrtf(sum / K + eps * 0x1p-128f) * 0x1p-64f;
-}
-__device__ __forceinline__ float square_scaled(float x) { return (x * 0x1p-64f) * (x * 0x1p-64f); }
-
 // Codes of eight values.  Common: y inv with inv = fl(1 / s) is within two units in the last place of the quotient, one
 // correction by the remainder brings it within one, and a second gives the quotient rounded to nearest
 // (Markstein's theorem, IBM Journal of Research and Development 34, 1990); 1.5 * 2^23 added to it leaves the
@@ -126,7 +118,7 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) w8_quantize_kernel(co
       if (r + gridDim.x < a.rows) load(r + gridDim.x);
     }
     // f(vector's index, its eight values as they stand)
-    float factor = 1.f;
+    float factor = 1.f, lift = 1.f;
     bool normed = false;
     auto for_each = [&](auto&& f) {
       if constexpr (VECS > 0) {
@@ -136,6 +128,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) w8_quantize_kernel(co
         const bool aligned = is_aligned(r);
         for (int v = threadIdx.x; v < vecs; v += THREADS) {
           unpack8(load_vec(row_of(r), v, a.K, aligned), y[0]);
+          if (lift != 1.f) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[0][j] *= lift;
+          }
           if (normed) {
             float g[8];
             unpack8(load_vec(a.norm, v, a.K, g_aligned), g);
@@ -147,22 +143,28 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) w8_quantize_kernel(co
       }
     };
     if constexpr (NORM) {
-      float sum = 0.f;
-      for_each([&](int, float (&f)[8]) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum = fmaf(f[j], f[j], sum);
-      });
-      sum = block_join<THREADS, false>(sum, sm);
-      const bool scaled = sum == INFINITY;
-      if (scaled) {
-        sum = 0.f;
+      auto mean_square = [&]() {
+        float sum = 0.f;
         for_each([&](int, float (&f)[8]) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) sum += square_scaled(f[j]);
+          for (int j = 0; j < 8; ++j) sum = fmaf(f[j], f[j], sum);
         });
-        sum = block_join<THREADS, false>(sum, sm);
+        return block_join<THREADS, false>(sum, sm) / a.K;
+      };
+      float mean = mean_square() + a.eps;
+      // A mean that leaves the float range is taken again of x / 2^80, whose squares sum up to 2^(96 + 17) at most, so that a row of
+      // any finite bf16 has its norm; its values stay divided.
+      if (!(mean <= FLT_MAX)) {
+        lift = 0x1p-80f;
+        if constexpr (VECS > 0) {
+#pragma unroll
+          for (int i = 0; i < VECS; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[i][j] *= lift;
+        }
+        mean = mean_square() + a.eps * lift * lift;
       }
-      factor = norm_factor(sum, a.K, a.eps, scaled);
+      factor = rsqrtf(mean);
       normed = true;
       if constexpr (VECS > 0) {
 #pragma unroll
