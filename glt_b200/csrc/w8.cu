@@ -152,10 +152,10 @@ __global__ void __launch_bounds__(THREADS, 1024 / THREADS) w8_quantize_kernel(co
         return block_join<THREADS, false>(sum, sm) / a.K;
       };
       float mean = mean_square() + a.eps;
-      // A mean that leaves the float range is taken again of x / 2^80, whose squares sum up to 2^(96 + 17) at most, so that a row of
-      // any finite bf16 has its norm; its values stay divided.
-      if (!(mean <= FLT_MAX)) {
-        lift = 0x1p-80f;
+      // A mean that leaves the float range is taken again of x / 2^80, whose squares sum up to 2^(96 + 17) at most, and one below
+      // 2^-100, where squares lose bits, of 2^100 x: so a row of any finite bf16 has its norm.  Its values stay multiplied.
+      if (!(mean <= FLT_MAX) || mean < 0x1p-100f) {
+        lift = mean < 0x1p-100f ? 0x1p100f : 0x1p-80f;
         if constexpr (VECS > 0) {
 #pragma unroll
           for (int i = 0; i < VECS; ++i)

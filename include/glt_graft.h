@@ -379,7 +379,8 @@ GLT_API int glt_w4_linear_workspace(int M, int N, int K, int group, int y_dtype,
  * glt_w8_quantize_rows: rows of bf16 x [rows, K] (row stride ld_x) to codes [rows, K] (row stride ld_codes,
  *   a multiple of 16, 16-byte aligned; the bytes from K to the next multiple of 16 are set to 0) and
  *   scales [rows] fp32: scale = max|x| / 127 over the row, code = nearest to x / scale (both quotients rounded to 32 bits),
- *   ties to even.  With norm (bf16 [K]) the row is first x / sqrt(mean(x^2) + eps) * norm, in 32 bits.
+ *   ties to even.  With norm (bf16 [K]) the row is first x / sqrt(mean(x^2) + eps) * norm, in 32 bits
+ *   (a row of zeros with eps = 0 is 0 / 0, NaN).
  *   A row of zeros has scale 0; one that holds an infinity or NaN has scale NaN and codes 0.  Weights
  *   [N, K] are quantised by the same call, a channel a row.
  * glt_w8_linear_rows: y[M, N] = scale[m] * w_scale[n] * sum_k code[m, k] * w[n, k] (+ resid[m, n]), y bf16 (y_dtype 1) or
