@@ -232,9 +232,15 @@ struct ProductArgs {
   int M, N;
 };
 
-template <bool BF16, bool RESID>
+// A sum is below 2^31, so times a channel's scale t below 2^96 it stays within 32 bits; a larger t is multiplied last, so that only a
+// result that leaves the range does.  LARGE: such a t may be among the warp's channels (with the choice for every element in
+// the pair kernel, 8192 tokens by 28672 x 4096 took 688 us for 672).  Underflow takes nothing: a product with an integer is a
+// multiple of the other factor's last place.
+constexpr float kLargeScale = 0x1p96f;
+template <bool BF16, bool RESID, bool LARGE>
 __device__ __forceinline__ void put(const ProductArgs& a, int m, int n, int sum, float t, float s, uint16_t r) {
   float z = static_cast<float>(sum) * t * s;
+  if (LARGE && t >= kLargeScale) z = static_cast<float>(sum) * s * t;
   if (RESID) z += bf16_bits_to_f32(r);
   if (BF16)
     static_cast<uint16_t*>(a.y)[m * a.ld_y + n] = bf16_bits_rn(z);
@@ -250,6 +256,13 @@ struct EpiW8 {
   __device__ __forceinline__ void operator()(const tc::EpiCtx<256>& c) const {
     const bool on = c.row < a.N;
     const float t = on ? a.w_scales[c.row] : 0.f;
+    if (__any_sync(0xffffffffu, t >= kLargeScale))
+      write<true>(c, on, t);
+    else
+      write<false>(c, on, t);
+  }
+  template <bool LARGE>
+  __device__ __forceinline__ void write(const tc::EpiCtx<256>& c, bool on, float t) const {
 #pragma unroll 1
     for (int j = c.part * 128; j < c.part * 128 + 128; j += 32) {
       if (c.n0 + j >= a.M) break;
@@ -266,7 +279,7 @@ struct EpiW8 {
 #pragma unroll
       for (int i = 0; i < 32; ++i) {
         const float si = __shfl_sync(0xffffffffu, s, i);
-        if (on && m0 + i <= m1) put<BF16, RESID>(a, m0 + i, c.row, __float_as_int(v[i]), t, si, RESID ? r[i] : 0);
+        if (on && m0 + i <= m1) put<BF16, RESID, LARGE>(a, m0 + i, c.row, __float_as_int(v[i]), t, si, RESID ? r[i] : 0);
       }
     }
   }
@@ -449,7 +462,7 @@ __global__ void __launch_bounds__(kStreamThreads) w8_stream_kernel(const __grid_
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (n < a.N && c + i < c1) put<BF16, RESID>(a, m0 + c + i, n, static_cast<int>(v[i]), t, s[i], r[i]);
+        if (n < a.N && c + i < c1) put<BF16, RESID, true>(a, m0 + c + i, n, static_cast<int>(v[i]), t, s[i], r[i]);
     }
   }
   tc::tc_fence_before();
