@@ -49,9 +49,12 @@ class Decoder:
     The cache holds ``seqs`` sequences of up to ``max_tokens`` tokens behind a shared prefix of up to
     ``shared_tokens``; ``lengths`` counts the tokens each one has on the device, ``held`` on the host, neither the
     prefix's.  ``reset`` forgets the sequences.  With ``window``, a token sees the last ``window`` tokens and the first
-    ``sinks`` (no prefix then)."""
+    ``sinks`` (no prefix then).
 
-    prefix = None
+    A sequence that was given an id outside the vocabulary gets logits of NaN from then on, until ``reset``: the host
+    does not wait to look at the ids, and the cache holds nothing right of such a token."""
+
+    prefix = unknown = None
     window = sinks = 0
 
     def __init__(self, weights: dict, heads: int, kv_heads: int, head_dim: int, seqs: int, max_tokens: int,
@@ -86,6 +89,7 @@ class Decoder:
         # sequence b owns blocks b, b + seqs, ...
         self.table = torch.arange(seqs * blocks, dtype=torch.int32, device=dev).view(blocks, seqs).t().contiguous()
         self.lengths = torch.zeros(seqs, dtype=torch.int32, device=dev)
+        self.unknown = torch.zeros(seqs, 1, dtype=torch.bool, device=dev)   # sequences with ids outside the vocabulary
         # the prefix the blocks behind them
         self.shared_tokens, self.shared_blocks = shared_tokens, torch.arange(
             seqs * blocks, seqs * blocks + shared, dtype=torch.int32, device=dev)
@@ -94,12 +98,14 @@ class Decoder:
         angle = torch.outer(torch.arange(shared_tokens + max_tokens, device=dev, dtype=torch.float32), inv)
         self.cos, self.sin = angle.cos(), angle.sin()
 
-    def _lookup(self, ids: torch.Tensor) -> torch.Tensor:
-        """Rows of the embedding for ids [seqs, n].  A sequence with an id outside the vocabulary gets NaN, which
-        its logits and log probabilities show: the host does not wait to look at the ids."""
+    def _lookup(self, ids: torch.Tensor, mark: torch.Tensor | None = None) -> torch.Tensor:
+        """Rows of the embedding for ids [seqs, n]: NaN for a sequence with an id outside the vocabulary, which ``mark``
+        [seqs, 1] notes too, since not every layer kernel keeps a NaN."""
         held = ids.clamp(0, self.embed.shape[0] - 1)
-        unknown = (held != ids).any(1, keepdim=True).expand_as(ids).reshape(-1, 1)
-        return self.embed[held.flatten()].masked_fill_(unknown, float("nan"))
+        unknown = (held != ids).any(1, keepdim=True)
+        if mark is not None:
+            mark |= unknown
+        return self.embed[held.flatten()].masked_fill_(unknown.expand_as(ids).reshape(-1, 1), float("nan"))
 
     def _norm(self, x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
         y, var = torch.empty_like(x), torch.empty(x.shape[0], device=x.device)
@@ -146,6 +152,8 @@ class Decoder:
     def reset(self) -> None:
         """Starts over with empty sequences; a shared prefix stays."""
         self.lengths.zero_()
+        if self.unknown is not None:
+            self.unknown.zero_()
         self.held = 0
 
     def _fits(self, ids: torch.Tensor, more: int = 0) -> None:
@@ -169,14 +177,14 @@ class Decoder:
         pos = self.lengths[:, None] + torch.arange(n, device=ids.device)
         if self.prefix is not None:
             pos = pos + self.shared_length
-        x = self._layers(ids, serve.Kv8Batch(self.table, self.lengths, ids.numel()), pos.flatten())
+        x = self._layers(ids, serve.Kv8Batch(self.table, self.lengths, ids.numel()), pos.flatten(), self.unknown)
         self.lengths += n
         last = x.view(self.seqs, n, -1)[:, -1].contiguous()
-        return self._project(self.head, last, self.final_norm, out_dtype=torch.float32)
+        return self._project(self.head, last, self.final_norm, out_dtype=torch.float32).masked_fill_(self.unknown, float("nan"))
 
-    def _layers(self, ids: torch.Tensor, batch: serve.Kv8Batch, pos: torch.Tensor) -> torch.Tensor:
-        """The layers' output [rows, hidden] of the batch's new tokens at positions pos [rows]."""
-        hd, x = self.head_dim, self._lookup(ids)
+    def _layers(self, ids: torch.Tensor, batch: serve.Kv8Batch, pos: torch.Tensor, mark: torch.Tensor | None = None) -> torch.Tensor:
+        """The layers' output [rows, hidden] of the batch's new tokens at positions pos [rows]; ``mark`` as for _lookup."""
+        hd, x = self.head_dim, self._lookup(ids, mark)
         for w in self.layers:
             qkv = self._project(w["qkv"], x, w["in_norm"]).unflatten(1, (-1, hd))
             rotated = self._rope(qkv[:, :self.heads + self.kv_heads], pos)
