@@ -51,8 +51,9 @@ class Decoder:
     prefix's.  ``reset`` forgets the sequences.  With ``window``, a token sees the last ``window`` tokens and the first
     ``sinks`` (no prefix then).
 
-    A sequence that was given an id outside the vocabulary gets logits of NaN from then on, until ``reset``: the host
-    does not wait to look at the ids, and the cache holds nothing right of such a token."""
+    A sequence that was given an id outside the vocabulary gets logits of NaN from then on, until ``reset``, and all of
+    them do behind a shared prefix with one: the host does not wait to look at the ids, and the cache holds nothing
+    right of such a token."""
 
     prefix = unknown = None
     window = sinks = 0
@@ -94,6 +95,7 @@ class Decoder:
         self.shared_tokens, self.shared_blocks = shared_tokens, torch.arange(
             seqs * blocks, seqs * blocks + shared, dtype=torch.int32, device=dev)
         self.shared_length = torch.zeros(1, dtype=torch.int32, device=dev)
+        self.shared_unknown = torch.zeros(1, 1, dtype=torch.bool, device=dev)
         inv = 1.0 / rope_theta ** (torch.arange(0, head_dim, 2, device=dev, dtype=torch.float32) / head_dim)
         angle = torch.outer(torch.arange(shared_tokens + max_tokens, device=dev, dtype=torch.float32), inv)
         self.cos, self.sin = angle.cos(), angle.sin()
@@ -144,8 +146,9 @@ class Decoder:
         with torch.cuda.device(self.embed.device):
             self.prefix = None
             self.shared_length.zero_()
+            self.shared_unknown.zero_()
             self._layers(ids[None], serve.Kv8Batch(self.shared_blocks[None], self.shared_length, ids.numel()),
-                         torch.arange(ids.numel(), device=ids.device))
+                         torch.arange(ids.numel(), device=ids.device), self.shared_unknown)
             self.shared_length += ids.numel()
         self.prefix = serve.Kv8Prefix(self.shared_blocks, self.shared_length)
 
@@ -180,9 +183,10 @@ class Decoder:
         x = self._layers(ids, serve.Kv8Batch(self.table, self.lengths, ids.numel()), pos.flatten(), self.unknown)
         self.lengths += n
         last = x.view(self.seqs, n, -1)[:, -1].contiguous()
-        return self._project(self.head, last, self.final_norm, out_dtype=torch.float32).masked_fill_(self.unknown, float("nan"))
+        unknown = self.unknown if self.prefix is None else self.unknown | self.shared_unknown
+        return self._project(self.head, last, self.final_norm, out_dtype=torch.float32).masked_fill_(unknown, float("nan"))
 
-    def _layers(self, ids: torch.Tensor, batch: serve.Kv8Batch, pos: torch.Tensor, mark: torch.Tensor | None = None) -> torch.Tensor:
+    def _layers(self, ids: torch.Tensor, batch: serve.Kv8Batch, pos: torch.Tensor, mark: torch.Tensor) -> torch.Tensor:
         """The layers' output [rows, hidden] of the batch's new tokens at positions pos [rows]; ``mark`` as for _lookup."""
         hd, x = self.head_dim, self._lookup(ids, mark)
         for w in self.layers:
