@@ -698,9 +698,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
 }
 
 // Joins what the prefix and the sequences' own tokens gave the query rows: a lane eight channels of a row, SPLIT warps
-// a share of its parts each.  blockIdx.y is the sequence.
+// a share of its parts each.  blockIdx.y is the sequence.  REPORT: the prefix has no blocks, and so no kernel that would report
+// a length.
 constexpr int kJoinWarps = 4;
-template <int SPLIT>
+template <int SPLIT, bool REPORT>
 __global__ void __launch_bounds__(32 * kJoinWarps) kv8_prefix_join_kernel(const __grid_constant__ AttnArgs a,
                                                                          const __grid_constant__ PrefixParts p) {
   constexpr int kSets = kJoinWarps / SPLIT;   // of rows, of a CTA
@@ -711,7 +712,7 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv8_prefix_join_kernel(const 
   const int per_log = hd == 128 ? 4 : 3, rows = 32 >> per_log;   // of a set
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Kv8Span s = kv8_span(a.b, blockIdx.y, a.c.block_tokens, nullptr);
-  const PrefixShares sh(p, p.tokens(nullptr));
+  const PrefixShares sh(p, p.tokens(REPORT && (blockIdx.x | blockIdx.y | threadIdx.x) == 0 ? a.err : nullptr));
   const int count = s.n * a.nh, first_row = s.row0 * a.nh;   // rows of heads: checked on the host
   const float* own_ml = a.own + static_cast<int64_t>(a.b.rows) * a.nh * hd;
   const int d = (lane & ((1 << per_log) - 1)) * 8;
@@ -860,7 +861,7 @@ int64_t align32(int64_t n) { return (n + 31) / 32 * 32; }
 int64_t own_bytes(const GltKv8Cache& c, const GltKv8Batch& b, int nh) {
   return align32(static_cast<int64_t>(b.rows) * nh * (c.head_dim + 2) * 4);
 }
-template <int SPLIT>
+template <int SPLIT, bool REPORT>
 int launch_join(const AttnArgs& a, const PrefixParts& parts, cudaStream_t st) {
   const int64_t rows = static_cast<int64_t>(kv8_most_new(a.c, a.b)) * a.nh, set = kJoinWarps / SPLIT * (256 / a.c.head_dim);
   // as many CTAs as are resident at once go through all rows, if they are enough for a sequence each
@@ -874,7 +875,7 @@ int launch_join(const AttnArgs& a, const PrefixParts& parts, cudaStream_t st) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  GLT_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv8_prefix_join_kernel<SPLIT>, a, parts));
+  GLT_CUDA_TRY(cudaLaunchKernelEx(&cfg, kv8_prefix_join_kernel<SPLIT, REPORT>, a, parts));
   GLT_LAUNCH_CHECK();
   return GLT_OK;
 }
@@ -930,7 +931,8 @@ extern "C" int glt_kv8_prefix_attention(const GltKv8Cache* cache, const GltKv8Ba
     GLT_TRY(glt::launch_own(a, st));
   else
     GLT_TRY(glt::launch_all<glt::Mode::kPrefix>(a, p, st));
+  if (parts.grid == 0) return glt::launch_join<1, true>(a, parts, st);
   // Rows of many parts go to four warps, others to one (the whole call when measured: 2048 rows of 19 parts 54.8 us against 60.6, 42 of
   // up to 26 16.9 against 21.9; 4096 of 10 197.8 against 194.1, 18944 of 3 128.1 against 111.6).
-  return (parts.lanes == 2 ? 1 : 2) * parts.grid > 12 * parts.units() ? glt::launch_join<4>(a, parts, st) : glt::launch_join<1>(a, parts, st);
+  return (parts.lanes == 2 ? 1 : 2) * parts.grid > 12 * parts.units() ? glt::launch_join<4, false>(a, parts, st) : glt::launch_join<1, false>(a, parts, st);
 }
