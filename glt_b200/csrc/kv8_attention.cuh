@@ -308,6 +308,23 @@ __device__ __forceinline__ uint32_t two_codes(uint32_t w) {
 // 2^(m - top) for partial results: weights that saw nothing are 0 (or NaN) already.
 __device__ __forceinline__ float join_factor(float m, float top) { return top == -INFINITY ? 1.f : ex2_approx(m - top); }
 
+// Where scales of V join the exponents, a number that leaves 32 bits (below 2^-126, counted 2^10 at least at the reference) has less than
+// 2^-72 of the weight of the token that made the reference, if their scales lie within kLowScale .. kHighScale (values of 0 weigh
+// as the lowest).  Else weights are summed from numbers 2^kWideLift as large, which the largest, 2^15 and some, bear: they have
+// less than 2^-32 of that weight where they leave 32 bits.
+constexpr float kLowScale = 0x1p-60f, kHighScale = 0x1p4f, kWideLift = 108.f;
+// The sum of weights of tokens whose numbers sum up to `lifted`; log_v and inv_v are their scale's.
+__device__ __forceinline__ float wide_weights(float lifted, float log_v, float inv_v) {
+  return log_v < 0.f ? lifted * (inv_v * 0x1p-108f) : lifted * inv_v * 0x1p-108f;
+}
+// 2^d, d <= 0, as two factors, the second 1 down to 2^-120: a sum of weights is taken times both, since where scales of V join the
+// exponents it may be as far above 1 as 2^d is below.
+struct TwoFactors {
+  float a, b;
+  __device__ __forceinline__ explicit TwoFactors(float d)
+      : a(ex2_approx(fmaxf(d, -120.f))), b(ex2_approx(fminf(d + 120.f, 0.f))) {}
+};
+
 // Four channels of a query row from their sum z, the row's maximum (base 2) and sum of
 // weights.  A row that saw nothing has weight 0 and gives 0; NaN stays NaN.
 template <Mode M>

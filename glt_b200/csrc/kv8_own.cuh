@@ -7,7 +7,8 @@
 // the channels is free: a lane loads 16 contiguous bytes of K for four k-steps of S, and 16 of V
 // (8 with head_dim 64) for a column of as many products.  P stays in the registers that S came in.
 // The scale of V joins the exponent, and P is rounded to f16, counted 2^15 at the running maximum of the exponents:
-// 11 bits down to 2^-29 of the row's largest summand, and below that within 2^-40 of it.
+// 11 bits down to 2^-29 of the row's largest summand, and below that within 2^-40 of it.  Over the scale, the same numbers make
+// the sum of weights, unless scales lie far apart (kWideLift).
 //
 // What bounds it: latency, about 0.8 us a step of 16 tokens, of which the next step's codes are on their way during one
 // (fetching four steps ahead to L2 gained nothing).  So it is for short tables (own_is_short).
@@ -128,6 +129,7 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) kv8_own_kernel(const __grid
     };
 
     float acc[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    bool wide = false;   // a scale of V so far was outside kLowScale .. kHighScale
 #pragma unroll
     for (int j = 0; j < HD / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
     Step now, ahead;
@@ -152,6 +154,7 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) kv8_own_kernel(const __grid
         }
       const bool some = !(now.vs < kOwnLeastScale);
       const float log_v = some ? log2f(now.vs) : -60.f, inv_v = some ? 1.f / now.vs : 0x1p60f;
+      wide |= some && !(now.vs >= kLowScale && now.vs <= kHighScale);
       uint32_t p[4];
       float factor[2];
 #pragma unroll
@@ -168,6 +171,7 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) kv8_own_kernel(const __grid
         peak = fmaxf(peak, __shfl_xor_sync(0xffffffffu, peak, 2));
         const float top = fmaxf(m[h], peak), ref = kOwnLift - (top == -INFINITY ? 0.f : top);
         factor[h] = m[h] == -INFINITY ? 1.f : ex2_approx(m[h] - top);   // (without a maximum the sums are 0, or NaN)
+        const float before = m[h];
         m[h] = top;
         float y[4], sum = 0.f;
 #pragma unroll
@@ -175,7 +179,15 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) kv8_own_kernel(const __grid
           y[i] = ex2_approx(x[i] + ref);
           sum += y[i];
         }
-        l[h] = fmaf(sum, inv_v, l[h] * factor[h]);
+        if (wide) {
+          const TwoFactors f(before == -INFINITY ? 0.f : before - top);
+          float lifted = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) lifted += ex2_approx(x[i] + ref + kWideLift);
+          l[h] = l[h] * f.a * f.b + wide_weights(lifted, log_v, inv_v);
+        } else {
+          l[h] = fmaf(sum, inv_v, l[h] * factor[h]);
+        }
         p[h] = pack_f16x2(y[0], y[1]);
         p[2 + h] = pack_f16x2(y[2], y[3]);
       }

@@ -17,7 +17,8 @@
 // scale of V joins the exponent: a token counts 2^(s + log2 scale - ref) in the sum of values, ref a running
 // reference near the maximum of that exponent, so that f16 has what one token can add at most near its top whatever the
 // scales of the blocks are: 11 bits down to 2^-24 of the reference, and below that within 2^-35 of it.  Over 1 / scale,
-// in 32 bits, the same numbers make the sum of weights.  (P as the sum of two bf16 numbers needs no such
+// in 32 bits, the same numbers make the sum of weights; where scales lie so far apart that they would leave 32 bits, larger
+// ones do (kWideLift).  (P as the sum of two bf16 numbers needs no such
 // reference, but half as many products and instructions again: 306 us where f16 took 258, other things equal.)
 // The reference moves only when the weights come near f16's top.
 //
@@ -61,10 +62,14 @@ struct PrefixArgs {
   unsigned int* err;
 };
 
-// Scales of a step's groups of 16 tokens.  flags: bit g, the group's block is not in the pool; bit 4 + g, its values are 0.
+// Scales of a step's groups of 16 tokens, and flags of each: kLost, its block is not in the pool; kNone, its values are 0; kWide, a scale
+// of V so far was outside kLowScale .. kHighScale.
+constexpr int kLost = 1, kNone = 2, kWide = 4, kEach = 0x01010101;
 struct alignas(16) PrefixNote {
   float k[4], log_v[4], inv_v[4];
-  int flags, pad[3];
+  uint8_t flags[4];
+  int pad[3];
+  __device__ __forceinline__ int all_flags() const { return *reinterpret_cast<const int*>(flags); }
 };
 constexpr int kNotes = 16;   // steps whose scales are held: more than can be under way
 constexpr int kSlots = 3;    // steps of K, and of V, that are laid out
@@ -215,6 +220,68 @@ struct PrefixRun {
   }
 };
 
+// A step where scales of V lie far apart (kWide): 16 tokens at a time, by their maximum, P over what is read of S.  done: the barrier of
+// the lane's last product with V, if there was one.  (As a function of its own it made the other steps slower: 65537 tokens,
+// 4096 rows 196 us for 194.)
+struct RowSums {
+  float m, l;   // the reference, the sum of weights
+  bool ok;
+};
+template <int HD>
+__device__ __forceinline__ RowSums wide_step(const PrefixNote& note, int left, float unit_q, float m, float l, uint32_t s_buf,
+                                             uint32_t o_at, uint64_t* done, uint32_t parity, unsigned int* err, volatile int* abort) {
+  const int flags = note.all_flags();
+  auto group = [&](int g, float (&v)[16]) {
+    tmem_ld16(s_buf + 16 * g, v);
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+      if (16 * g + j >= left || (flags >> (8 * g) & kLost)) v[j] = -INFINITY;
+    return fmaxf(note.k[g] * unit_q, 1e-37f);
+  };
+  float peak = m;
+#pragma unroll 1
+  for (int g = 0; g < 4; ++g) {
+    float v[16], top = -INFINITY;
+    const float u = group(g, v);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) top = fmaxf(top, v[j]);
+    peak = fmaxf(peak, fmaf(top, u, note.log_v[g]));
+  }
+  if (__any_sync(0xffffffffu, peak > m)) {
+    const TwoFactors f(peak > m ? m - peak : 0.f);
+    if (done) {
+      if (!__all_sync(0xffffffffu, tc::mbar_wait(done, parity, err, abort))) return {m, l, false};
+      tc::tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 16) {
+        float o[16];
+        tmem_ld16(o_at + c, o);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j] = o[j] * f.a * f.b;
+        tmem_st16(o_at + c, o);
+      }
+    }
+    l = l * f.a * f.b;
+    m = peak;
+  }
+  const float ref = kLift - (m == -INFINITY ? 0.f : m);
+#pragma unroll 1
+  for (int g = 0; g < 4; ++g) {
+    float v[16], lifted = 0.f;
+    uint32_t p[8];
+    const float u = group(g, v), log_v = note.log_v[g], r = ref + log_v;
+#pragma unroll
+    for (int j = 0; j < 16; j += 2) {
+      const float e0 = fmaf(v[j], u, r), e1 = fmaf(v[j + 1], u, r);
+      p[j / 2] = pack_f16x2(ex2_approx(e0), ex2_approx(e1));
+      lifted += ex2_approx(e0 + kWideLift) + ex2_approx(e1 + kWideLift);
+    }
+    tmem_st8(s_buf + 8 * g, p);
+    l += wide_weights(lifted, log_v, note.inv_v[g]);
+  }
+  return {m, l, true};
+}
+
 template <int HD, int FMT, int LANES>
 __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __grid_constant__ PrefixArgs a) {
   using L = PrefixSmem<HD, LANES>;
@@ -361,16 +428,33 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
         float u[4], w[4];   // of the groups of 16 tokens
         four(note.k, u);
         four(note.log_v, w);
-        const int flags = note.flags, left = tokens - (run.s0 + i) * kPrefixStep;   // tokens of the step
+        const int flags = note.all_flags(), left = tokens - (run.s0 + i) * kPrefixStep;   // tokens of the step
         const uint32_t s_buf = s_at + buf * kPrefixStep;
         float v[kPrefixStep];
         tmem_ld64(s_buf, v);
 #pragma unroll
         for (int g = 0; g < 4; ++g) u[g] = fmaxf(u[g] * unit_q, 1e-37f);   // above 0, so that a masked -inf stays one
-        if (left < kPrefixStep || (flags & 0xF)) {
+        if (left < kPrefixStep || (flags & (kLost | kWide) * kEach)) {
+          if (flags & kWide * kEach) {
+            const RowSums x = wide_step<HD>(note, left, unit_q, m, l, s_buf, o_at, any ? o_full + mine : nullptr, (products - 1) & 1,
+                                            a.err, &abort);
+            if (!x.ok) {
+              abort = 1;
+              break;
+            }
+            m = x.m;
+            l = x.l;
+            any = true;
+            ++products;
+            tmem_wait_st();
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(p_full + 2 * mine + buf);
+            continue;
+          }
 #pragma unroll
           for (int j = 0; j < kPrefixStep; ++j)
-            if (j >= left || (flags >> (j / 16) & 1)) v[j] = -INFINITY;
+            if (j >= left || (flags >> (j / 16 * 8) & kLost)) v[j] = -INFINITY;
         }
         // P by the reference as it stands.  A unit's first S moves it, and one whose weights would come near f16's
         // top, which the sums show: the maximum is taken then, and only then.
@@ -499,7 +583,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
         const int tok = tok0 + i * (kDecodeThreads / kChunks);
         uint4 lo, hi;
         sixteen_f16<FMT>(x[i], lo, hi);
-        if (tok >= left || (flags >> (tok >> 4) & 1)) lo = hi = make_uint4(0, 0, 0, 0);
+        if (tok >= left || (flags >> ((tok >> 4) * 8) & 1)) lo = hi = make_uint4(0, 0, 0, 0);
         *reinterpret_cast<uint4*>(dst + off_lo + i * (kDecodeThreads / kChunks * 128)) = lo;
         *reinterpret_cast<uint4*>(dst + off_hi + i * (kDecodeThreads / kChunks * 128)) = hi;
       }
@@ -527,10 +611,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
         abort = 1;
         break;
       }
-      if (with_k) lay(xk, smem + L::kOffK + slot_k * L::kPart, left[0], notes[it % kNotes].flags);
+      if (with_k) lay(xk, smem + L::kOffK + slot_k * L::kPart, left[0], notes[it % kNotes].all_flags());
       if (with_v) {
-        const int flags = notes[v % kNotes].flags;
-        lay(xv, smem + L::kOffV + slot_v * L::kPart, left[kAhead], flags | flags >> 4);
+        const int flags = notes[v % kNotes].all_flags();
+        lay(xv, smem + L::kOffV + slot_v * L::kPart, left[kAhead], flags | flags >> 1);   // kLost or kNone
       }
       fence_async_smem();
       __syncwarp();
@@ -590,6 +674,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
     Place now = read_id();
     read_scales(now);
     Place next = read_id();
+    bool wide = false;   // of the lane's groups
     bool in_v[kAhead + 1] = {};
     int64_t row_v[kAhead + 1] = {};
     for (int it = 0, end = INT_MAX - kAhead; !abort && it < end + kAhead; ++it) {
@@ -602,7 +687,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
         row_v[0] = now.row;
         const bool gone = lane < 4 && !now.in && now.step * kPrefixStep + 16 * lane < tokens, some = !(now.v < kLeastScale);
         if (gone && a.err) atomicOr(a.err, GLT_DEVERR_BAD_SHAPE);
-        const unsigned lost = __ballot_sync(0xffffffffu, gone), none = __ballot_sync(0xffffffffu, lane < 4 && !some);
+        wide |= now.in && some && !(now.v >= kLowScale && now.v <= kHighScale);
         const float ks = now.k, vs = now.v;
         read_scales(next);
         now = next;
@@ -614,8 +699,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
             note.k[lane] = ks;
             note.log_v[lane] = some ? log2f(vs) : -60.f;
             note.inv_v[lane] = some ? 1.f / vs : 0x1p60f;
+            note.flags[lane] = (gone ? kLost : 0) | (some ? 0 : kNone) | (wide ? kWide : 0);
           }
-          if (lane == 0) note.flags = static_cast<int>(lost | none << 4);
           __syncwarp();
           copy(a.c.k, in_v[0], row_v[0]);
         }
@@ -702,7 +787,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
 // a length.
 constexpr int kJoinWarps = 4;
 template <int SPLIT, bool REPORT>
-__global__ void __launch_bounds__(32 * kJoinWarps) kv8_prefix_join_kernel(const __grid_constant__ AttnArgs a,
+__global__ void __launch_bounds__(32 * kJoinWarps, SPLIT > 1 ? 7 : 6) kv8_prefix_join_kernel(const __grid_constant__ AttnArgs a,
                                                                          const __grid_constant__ PrefixParts p) {
   constexpr int kSets = kJoinWarps / SPLIT;   // of rows, of a CTA
   __shared__ float4 sm_z[kJoinWarps][2][32];
@@ -767,20 +852,20 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv8_prefix_join_kernel(const 
       float peak = top;
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) peak = fmaxf(peak, m[k]);
-      const float old = join_factor(top, peak);
-      sum *= old;
+      const TwoFactors old(peak == -INFINITY ? 0.f : top - peak);
+      sum = sum * old.b * old.a;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) z[j] *= old;
+      for (int j = 0; j < 8; ++j) z[j] = z[j] * old.b * old.a;
 #pragma unroll
       for (int k = 0; k < kBatch; ++k) {
-        const float f = join_factor(m[k], peak);
-        sum = fmaf(l[k], f, sum);
+        const TwoFactors f(peak == -INFINITY ? 0.f : m[k] - peak);
+        sum = fmaf(l[k] * f.b, f.a, sum);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          z[4 * h] = fmaf(x[k][h].x, f, z[4 * h]);
-          z[4 * h + 1] = fmaf(x[k][h].y, f, z[4 * h + 1]);
-          z[4 * h + 2] = fmaf(x[k][h].z, f, z[4 * h + 2]);
-          z[4 * h + 3] = fmaf(x[k][h].w, f, z[4 * h + 3]);
+          z[4 * h] = fmaf(x[k][h].x * f.b, f.a, z[4 * h]);
+          z[4 * h + 1] = fmaf(x[k][h].y * f.b, f.a, z[4 * h + 1]);
+          z[4 * h + 2] = fmaf(x[k][h].z * f.b, f.a, z[4 * h + 2]);
+          z[4 * h + 3] = fmaf(x[k][h].w * f.b, f.a, z[4 * h + 3]);
         }
       }
       top = peak;
@@ -794,22 +879,22 @@ __global__ void __launch_bounds__(32 * kJoinWarps) kv8_prefix_join_kernel(const 
         float peak = top;
 #pragma unroll
         for (int w = 1; w < SPLIT; ++w) peak = fmaxf(peak, sm_ml[warp + w][lane].x);
-        const float old = join_factor(top, peak);
-        sum *= old;
+        const TwoFactors old(peak == -INFINITY ? 0.f : top - peak);
+        sum = sum * old.b * old.a;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) z[j] *= old;
+        for (int j = 0; j < 8; ++j) z[j] = z[j] * old.b * old.a;
 #pragma unroll
         for (int w = 1; w < SPLIT; ++w) {
           const float2 ml = sm_ml[warp + w][lane];
-          const float f = join_factor(ml.x, peak);
-          sum = fmaf(ml.y, f, sum);
+          const TwoFactors f(peak == -INFINITY ? 0.f : ml.x - peak);
+          sum = fmaf(ml.y * f.b, f.a, sum);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const float4 x = sm_z[warp + w][h][lane];
-            z[4 * h] = fmaf(x.x, f, z[4 * h]);
-            z[4 * h + 1] = fmaf(x.y, f, z[4 * h + 1]);
-            z[4 * h + 2] = fmaf(x.z, f, z[4 * h + 2]);
-            z[4 * h + 3] = fmaf(x.w, f, z[4 * h + 3]);
+            z[4 * h] = fmaf(x.x * f.b, f.a, z[4 * h]);
+            z[4 * h + 1] = fmaf(x.y * f.b, f.a, z[4 * h + 1]);
+            z[4 * h + 2] = fmaf(x.z * f.b, f.a, z[4 * h + 2]);
+            z[4 * h + 3] = fmaf(x.w * f.b, f.a, z[4 * h + 3]);
           }
         }
         top = peak;

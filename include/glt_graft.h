@@ -325,7 +325,8 @@ GLT_API int glt_kv8_window_attention(const GltKv8Cache* cache, const GltKv8Batch
  * tokens, those that glt_kv8_attention without a window shows it (token_mask is for own tokens).
  * The prefix's cache is read once for every 256 rows (token x head of a group) of a KV head, not once a sequence.
  * What a token adds to a sum is exact to 11 bits down to 2^-24 of the largest such summand of
- * its row, and to 2^-35 of that below; a scale of V below 2^-90 counts as 0.
+ * its row, and to 2^-35 of that below; a scale of V below 2^-90 counts as 0.  Weights count in lse and the divisor whatever the
+ * scales of V, beside another block's too.
  * workspace: glt_kv8_prefix_attention_workspace bytes, 32-byte aligned, else as there. */
 typedef struct GltKv8Prefix {
   int num_blocks;
