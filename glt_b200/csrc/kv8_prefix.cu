@@ -697,7 +697,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
           PrefixNote& note = notes[it % kNotes];
           if (lane < 4) {
             note.k[lane] = ks;
-            note.log_v[lane] = some ? log2f(vs) : -60.f;
+            note.log_v[lane] = (some ? log2f(vs) : -60.f) + ks * 0.f;   // NaN where the scale of K is one (which the softmax drops)
             note.inv_v[lane] = some ? 1.f / vs : 0x1p60f;
             note.flags[lane] = (gone ? kLost : 0) | (some ? 0 : kNone) | (wide ? kWide : 0);
           }
