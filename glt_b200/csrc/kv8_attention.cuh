@@ -691,7 +691,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            const float r = peak[f][nt][j] == -INFINITY ? 0.f : peak[f][nt][j] - 15.f;
+            // (a scale of K that is NaN comes back in here: the units above drop it)
+            const float r = peak[f][nt][j] == -INFINITY ? 0.f : fmaf(f ? sc.z : sc.x, 0.f, peak[f][nt][j] - 15.f);
             const float w = peak[f][nt][j] == -INFINITY ? 0.f : ex2_approx(r - m[nt][j]);
             float sum = 0.f;
 #pragma unroll
