@@ -630,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) kv8_attention_kernel(con
           const int t = t0 + 8 * i + g;
           // a query of the tile sees it
           const bool on = (valid >> (i >> 1) & 1) && (seen >> (8 * i + g) & 1) && t <= pos_hi &&
-                          (t > before || (kSinks && t < a.sinks));
+                          (kSinks ? t > before || t < a.sinks : t > before);
           if (FMT == GLT_KV8_E4M3) live[i] = __ballot_sync(0xffffffffu, on);   // bit 4g: token 8 i + g
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
