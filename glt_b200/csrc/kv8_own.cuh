@@ -242,6 +242,8 @@ int own_tiles(const AttnArgs& a) { return (kv8_most_new(a.c, a.b) * a.group + kO
 //   64 sequences, 1 token, 32 heads over 8: 512          38.9 / 32.5    42.3 / 36.9    42.8 / 41.2    47.3 / 49.9
 //   128 sequences: 1024                                  55.4 / 48.4    62.2 / 54.4    64.1 / 59.9    70.5 / 68.2
 //   100 sequences, 5 tokens, 64 heads over 8: 2400       145 / 108      161 / 120      165 / 132      186 / 153
+// (Next to its bound the rule is off by up to 7 %: 152 warps with 320 tokens, 512 with 384, 1024 with 512.)  It goes by the room of a
+// table, since what the sequences hold is known on the device alone: tables as tight as the lengths allow are the faster ones.
 bool own_is_short(const AttnArgs& a) {
   const int64_t warps = static_cast<int64_t>(a.b.num_seqs) * a.c.num_kv_heads * own_tiles(a);
   return static_cast<int64_t>(a.b.max_blocks) * a.c.block_tokens <= std::min<int64_t>(512, 256 + warps / 8);

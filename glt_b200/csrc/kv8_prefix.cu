@@ -5,8 +5,8 @@
 // Every query of the batch sees the whole prefix, so its cache is read once for all of them: the queries
 // that share a KV head are the rows of tcgen05 products with it.
 //
-// A CTA (see kv8_prefix.cuh for its share of the work) goes through steps of 128 tokens:
-//   warp 14     looks up the blocks, copies their codes in bulk into a ring of 64 tokens of K or V each, and notes the scales.
+// A CTA (see kv8_prefix.cuh for its share of the work) goes through steps of 64 tokens:
+//   warp 14     looks up the blocks, copies their codes in bulk into a ring of K or V of a step each, and notes the scales.
 //   warps 8-11  turn codes into f16, which holds them exactly, and lay K and V out as the products read them.
 //   warps 12-13 issue the products of a lane each: S = Q K^T, and O += P V with P in TMEM, as P was written over S.  (From one
 //               warp, the tensor cores ran dry whenever it went from one barrier to the next.)
@@ -23,12 +23,12 @@
 // The reference moves only when the weights come near f16's top.
 //
 // What bounds it: 4 rows hd operations a token are 83 us at the measured bf16 rate for 4096 rows (128 sequences, 32 heads over 8,
-// head_dim 128) behind 65537 tokens, of 191 us the call takes.  A step of 64 tokens and 256 rows takes a CTA 2400 cycles
+// head_dim 128) behind 65537 tokens, of 194 us the call takes.  A step of 64 tokens and 256 rows takes a CTA 2400 cycles
 // where its products need 1300 of the tensor cores and its exponentials 1000 of their units: each of the
 // softmax's two warps a scheduler waits 700 of them for what it has just read or issued, at 0.4 instructions a cycle.  Sixteen
 // softmax warps of half a row each (72 registers) were slower, 234 us.  One result after the other: loops as short as here instead of
 // unrolled code 306 us for 423; scores ahead of the softmax, sums instead of maxima 204 for 258.
-// Few sequences are bound by beginnings and ends: 64 sequences behind 8193 tokens 55 us, of which the units' first loads, the
+// Few sequences are bound by beginnings and ends: 64 sequences behind 8193 tokens 56 us, of which the units' first loads, the
 // parts' way through memory (19 MB) and the own tokens' kernel are three quarters.
 #include <float.h>
 
@@ -48,7 +48,8 @@ constexpr int kAhead = 2;   // steps that K is laid out ahead of V
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
 constexpr float kLift = 10.f;         // base 2: what the reference counts in f16, whose top is 2^16 and last normal 2^-14
 constexpr float kMostSum = 0x1p15f;   // of 16 tokens, before the reference moves
-// Of V: smaller ones count as 0, and weigh as 2^-60.  Over the scale, a weight's 2^10 stay within 32 bits for 2^27 tokens.
+// Of V: smaller ones count as 0, and weigh as 2^-60.  Over the scale, weights, of 2^11 on average at most before the reference moves,
+// stay within 32 bits for 2^26 tokens.
 constexpr float kLeastScale = 0x1p-90f;
 
 struct PrefixArgs {
@@ -1017,7 +1018,8 @@ extern "C" int glt_kv8_prefix_attention(const GltKv8Cache* cache, const GltKv8Ba
   else
     GLT_TRY(glt::launch_all<glt::Mode::kPrefix>(a, p, st));
   if (parts.grid == 0) return glt::launch_join<1, true>(a, parts, st);
-  // Rows of many parts go to four warps, others to one (the whole call when measured: 2048 rows of 19 parts 54.8 us against 60.6, 42 of
-  // up to 26 16.9 against 21.9; 4096 of 10 197.8 against 194.1, 18944 of 3 128.1 against 111.6).
+  // Rows of many parts go to four warps, others to one (whole calls, four warps / one, in us, by the parts of a unit: 64 sequences of 4
+  // heads over each of 6, 8, 10, 12, 16 and 20 KV heads, 25 parts 51.2 / 57.5, 19 55.9 / 61.0, 15 69.7 / 70.3, 12 76.3 / 75.5, 9 86.8 / 85.4,
+  // 7 102.7 / 98.1; 3 sequences, units of up to 26 parts 14.5 / 17.6; 128 sequences, 10 parts 197 / 195; 18944 rows of 3 107.4 / 87.3).
   return (parts.lanes == 2 ? 1 : 2) * parts.grid > 12 * parts.units() ? glt::launch_join<4, false>(a, parts, st) : glt::launch_join<1, false>(a, parts, st);
 }
