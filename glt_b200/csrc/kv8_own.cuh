@@ -8,7 +8,7 @@
 // (8 with head_dim 64) for a column of as many products.  P stays in the registers that S came in.
 // The scale of V joins the exponent, and P is rounded to f16, counted 2^15 at the running maximum of the exponents:
 // 11 bits down to 2^-29 of the row's largest summand, and below that within 2^-40 of it.  Over the scale, the same numbers make
-// the sum of weights, unless scales lie far apart (kWideLift).
+// the sum of weights, unless scales lie far apart (ScaleWindow).
 //
 // What bounds it: latency, about 0.8 us a step of 16 tokens, of which the next step's codes are on their way during one
 // (fetching four steps ahead to L2 gained nothing).  So it is for short tables (own_is_short).
@@ -25,7 +25,7 @@ constexpr int kOwnWarps = 4;
 constexpr int kOwnRows = 16;
 constexpr int kOwnStep = 16;   // tokens: blocks hold a multiple of them
 constexpr float kOwnLift = 15.f;
-// Of V: smaller ones count as 0, and weigh as 2^-60.  Over the scale, a weight's 2^15 stay within 32 bits.
+// Of V: smaller ones count as 0.  Over the scale, a weight's 2^15 stay within 32 bits.
 constexpr float kOwnLeastScale = 0x1p-90f;
 
 template <int HD, int FMT>
@@ -129,12 +129,13 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) kv8_own_kernel(const __grid
     };
 
     float acc[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    bool wide = false;   // a scale of V so far was outside kLowScale .. kHighScale
+    bool wide = false;   // a scale of V so far was outside the window
 #pragma unroll
     for (int j = 0; j < HD / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
     Step now, ahead;
     int id = id_of(kOwnStep);
     load(0, id_of(0), ahead);
+    const ScaleWindow window(ahead.vs);
 #pragma unroll 1
     for (int t0 = 0; t0 < end; t0 += kOwnStep) {
       now = ahead;
@@ -153,8 +154,8 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) kv8_own_kernel(const __grid
           for (int j = 0; j < 4; ++j) mma_f16(z[n], qa[k * 4 + j], two_codes<FMT, 0>(w[j]), two_codes<FMT, 1>(w[j]));
         }
       const bool some = !(now.vs < kOwnLeastScale);
-      const float log_v = some ? log2f(now.vs) : -60.f, inv_v = some ? 1.f / now.vs : 0x1p60f;
-      wide |= some && !(now.vs >= kLowScale && now.vs <= kHighScale);
+      const float log_v = some ? log2f(now.vs) : window.none_log, inv_v = some ? 1.f / now.vs : window.none_inv;
+      wide |= some && !window.holds(now.vs);
       uint32_t p[4];
       float factor[2];
 #pragma unroll

@@ -18,7 +18,7 @@
 // reference near the maximum of that exponent, so that f16 has what one token can add at most near its top whatever the
 // scales of the blocks are: 11 bits down to 2^-24 of the reference, and below that within 2^-35 of it.  Over 1 / scale,
 // in 32 bits, the same numbers make the sum of weights; where scales lie so far apart that they would leave 32 bits, larger
-// ones do (kWideLift).  (P as the sum of two bf16 numbers needs no such
+// ones do (ScaleWindow).  (P as the sum of two bf16 numbers needs no such
 // reference, but half as many products and instructions again: 306 us where f16 took 258, other things equal.)
 // The reference moves only when the weights come near f16's top.
 //
@@ -48,7 +48,7 @@ constexpr int kAhead = 2;   // steps that K is laid out ahead of V
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
 constexpr float kLift = 10.f;         // base 2: what the reference counts in f16, whose top is 2^16 and last normal 2^-14
 constexpr float kMostSum = 0x1p15f;   // of 16 tokens, before the reference moves
-// Of V: smaller ones count as 0, and weigh as 2^-60.  Over the scale, weights, of 2^11 on average at most before the reference moves,
+// Of V: smaller ones count as 0.  Over the scale, weights, of 2^11 on average at most before the reference moves,
 // stay within 32 bits for 2^26 tokens.
 constexpr float kLeastScale = 0x1p-90f;
 
@@ -64,7 +64,7 @@ struct PrefixArgs {
 };
 
 // Scales of a step's groups of 16 tokens, and flags of each: kLost, its block is not in the pool; kNone, its values are 0; kWide, a scale
-// of V so far was outside kLowScale .. kHighScale.
+// of V so far was outside the run's ScaleWindow.
 constexpr int kLost = 1, kNone = 2, kWide = 4, kEach = 0x01010101;
 struct alignas(16) PrefixNote {
   float k[4], log_v[4], inv_v[4];
@@ -675,6 +675,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
     Place now = read_id();
     read_scales(now);
     Place next = read_id();
+    const ScaleWindow window(__shfl_sync(0xffffffffu, now.v, 0));
     bool wide = false;   // of the lane's groups
     bool in_v[kAhead + 1] = {};
     int64_t row_v[kAhead + 1] = {};
@@ -688,7 +689,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
         row_v[0] = now.row;
         const bool gone = lane < 4 && !now.in && now.step * kPrefixStep + 16 * lane < tokens, some = !(now.v < kLeastScale);
         if (gone && a.err) atomicOr(a.err, GLT_DEVERR_BAD_SHAPE);
-        wide |= now.in && some && !(now.v >= kLowScale && now.v <= kHighScale);
+        wide |= now.in && some && !window.holds(now.v);
         const float ks = now.k, vs = now.v;
         read_scales(next);
         now = next;
@@ -698,8 +699,8 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
           PrefixNote& note = notes[it % kNotes];
           if (lane < 4) {
             note.k[lane] = ks;
-            note.log_v[lane] = (some ? log2f(vs) : -60.f) + ks * 0.f;   // NaN where the scale of K is one (which the softmax drops)
-            note.inv_v[lane] = some ? 1.f / vs : 0x1p60f;
+            note.log_v[lane] = (some ? log2f(vs) : window.none_log) + ks * 0.f;   // NaN where the scale of K is one (which the softmax drops)
+            note.inv_v[lane] = some ? 1.f / vs : window.none_inv;
             note.flags[lane] = (gone ? kLost : 0) | (some ? 0 : kNone) | (wide ? kWide : 0);
           }
           __syncwarp();
