@@ -5,7 +5,8 @@ built from the operators of ``glt_b200.serve`` and the layer kernels of the C AB
 cache for a batch of sequences; ``step`` runs any number of new tokens of each sequence (a
 prompt or one token) and returns the logits of the last one; ``generate`` decodes and returns
 the tokens with their log probabilities.  ``share`` runs a prompt that all sequences begin with once,
-for all of them; with a window, old tokens but a few first ones drop out of sight.
+for all of them; with a window, old tokens but a few first ones drop out of sight (the cache holds
+``max_tokens`` all the same).
 
 Usage:  python -m glt_b200.decode [--seqs N] [--prompt N] [--tokens N] [--bits 4|8] [--shared N] [--window N --sinks N]
 (random weights of the Qwen2.5-0.5B shape; prints tokens per second)
