@@ -310,20 +310,18 @@ __device__ __forceinline__ float join_factor(float m, float top) { return top ==
 
 // Where scales of V join the exponents, a number that leaves 32 bits (below 2^-126, counted 2^10 at least at the reference) has less than
 // 2^-72 of the weight of the token that made the reference, if their scales lie within a window of 2^64: from 2^-52 (not below
-// 2^-90, where values count as 0) to 2^12 of the first one.  Values of 0 weigh as its lowest.
+// 2^-90, where values count as 0) to 2^12 of the first one.  Values of 0 weigh as the least scale, 2^-90, so that no reference is
+// theirs where a summand is near: beside scales up to 2^8 they have less than 2^-38 then.
 // Else weights are summed from numbers 2^kWideLift as large, which the largest, 2^15 and some, bear: they have
-// less than 2^-32 of that weight where they leave 32 bits.  (All steps that way: 4096 rows behind 65537 tokens 367 us for 195.)
+// less than 2^-32 of that weight where they leave 32 bits.  (All steps that way: 4096 rows behind 65537 tokens 367 us for 193.)
+constexpr float kLeastScale = 0x1p-90f, kMostBesideNone = 0x1p8f;
 struct ScaleWindow {
-  float low, high, none_log, none_inv;   // none: base 2, and its reciprocal, what values of 0 weigh as
+  float low, high;
   __device__ __forceinline__ explicit ScaleWindow(float first) {
-    const int e = first >= 0x1p-90f && first <= FLT_MAX ? static_cast<int>(__float_as_uint(first) >> 23) - 127 : -8;
-    const int lo = max(e - 52, -90), hi = min(e + 12, 127);
-    low = __int_as_float((lo + 127) << 23);
-    high = __int_as_float((hi + 127) << 23);
-    none_log = static_cast<float>(lo);
-    none_inv = __int_as_float((127 - lo) << 23);
+    const int e = first >= kLeastScale && first <= FLT_MAX ? static_cast<int>(__float_as_uint(first) >> 23) - 127 : -8;
+    low = __int_as_float((max(e - 52, -90) + 127) << 23);
+    high = __int_as_float((min(e + 12, 127) + 127) << 23);
   }
-  __device__ __forceinline__ bool holds(float scale) const { return scale >= low && scale <= high; }
 };
 constexpr float kWideLift = 108.f;
 // The sum of weights of tokens whose numbers sum up to `lifted`; log_v and inv_v are their scale's.

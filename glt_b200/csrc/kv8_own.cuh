@@ -24,9 +24,7 @@ namespace {
 constexpr int kOwnWarps = 4;
 constexpr int kOwnRows = 16;
 constexpr int kOwnStep = 16;   // tokens: blocks hold a multiple of them
-constexpr float kOwnLift = 15.f;
-// Of V: smaller ones count as 0.  Over the scale, a weight's 2^15 stay within 32 bits.
-constexpr float kOwnLeastScale = 0x1p-90f;
+constexpr float kOwnLift = 15.f;   // (over the least scale, a weight's 2^15 stay within 32 bits)
 
 template <int HD, int FMT>
 __global__ void __launch_bounds__(32 * kOwnWarps, 2) kv8_own_kernel(const __grid_constant__ AttnArgs a, int tiles) {
@@ -153,9 +151,9 @@ __global__ void __launch_bounds__(32 * kOwnWarps, 2) kv8_own_kernel(const __grid
 #pragma unroll
           for (int j = 0; j < 4; ++j) mma_f16(z[n], qa[k * 4 + j], two_codes<FMT, 0>(w[j]), two_codes<FMT, 1>(w[j]));
         }
-      const bool some = !(now.vs < kOwnLeastScale);
-      const float log_v = some ? log2f(now.vs) : window.none_log, inv_v = some ? 1.f / now.vs : window.none_inv;
-      wide |= some && !window.holds(now.vs);
+      const bool some = !(now.vs < kLeastScale);
+      const float vs = some ? now.vs : kLeastScale, log_v = log2f(vs), inv_v = 1.f / vs;
+      wide |= some ? !(now.vs >= window.low && now.vs <= window.high) : window.high > kMostBesideNone;
       uint32_t p[4];
       float factor[2];
 #pragma unroll

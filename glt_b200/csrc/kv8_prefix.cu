@@ -23,12 +23,12 @@
 // The reference moves only when the weights come near f16's top.
 //
 // What bounds it: 4 rows hd operations a token are 83 us at the measured bf16 rate for 4096 rows (128 sequences, 32 heads over 8,
-// head_dim 128) behind 65537 tokens, of 194 us the call takes.  A step of 64 tokens and 256 rows takes a CTA 2400 cycles
+// head_dim 128) behind 65537 tokens, of 193 us the call takes.  A step of 64 tokens and 256 rows takes a CTA 2400 cycles
 // where its products need 1300 of the tensor cores and its exponentials 1000 of their units: each of the
 // softmax's two warps a scheduler waits 700 of them for what it has just read or issued, at 0.4 instructions a cycle.  Sixteen
 // softmax warps of half a row each (72 registers) were slower, 234 us.  One result after the other: loops as short as here instead of
 // unrolled code 306 us for 423; scores ahead of the softmax, sums instead of maxima 204 for 258.
-// Few sequences are bound by beginnings and ends: 64 sequences behind 8193 tokens 56 us, of which the units' first loads, the
+// Few sequences are bound by beginnings and ends: 64 sequences behind 8193 tokens 55 us, of which the units' first loads, the
 // parts' way through memory (19 MB) and the own tokens' kernel are three quarters.
 #include <float.h>
 
@@ -47,10 +47,7 @@ constexpr int kPrefixThreads = 32 * (kCopyWarp + 1);
 constexpr int kAhead = 2;   // steps that K is laid out ahead of V
 constexpr int kDecodeThreads = 32 * kDecodeWarps;
 constexpr float kLift = 10.f;         // base 2: what the reference counts in f16, whose top is 2^16 and last normal 2^-14
-constexpr float kMostSum = 0x1p15f;   // of 16 tokens, before the reference moves
-// Of V: smaller ones count as 0.  Over the scale, weights, of 2^11 on average at most before the reference moves,
-// stay within 32 bits for 2^26 tokens.
-constexpr float kLeastScale = 0x1p-90f;
+constexpr float kMostSum = 0x1p15f;   // of 16 tokens, before the reference moves: over the least scale, 2^26 of them stay within 32 bits
 
 struct PrefixArgs {
   GltKv8Cache c;
@@ -222,15 +219,15 @@ struct PrefixRun {
 };
 
 // A step where scales of V lie far apart (kWide): 16 tokens at a time, by their maximum, P over what is read of S.  done: the barrier of
-// the lane's last product with V, if there was one.  (As a function of its own it made the other steps slower: 65537 tokens,
-// 4096 rows 196 us for 194.)
+// the lane's last product with V, if there was one.  (Not inline: with its code in the loop
+// of ordinary steps 64 sequences behind 8193 tokens took 55.8 us for 54.8, and 128 behind 65537 191.8 for 192.7.)
 struct RowSums {
   float m, l;   // the reference, the sum of weights
   bool ok;
 };
 template <int HD>
-__device__ __forceinline__ RowSums wide_step(const PrefixNote& note, int left, float unit_q, float m, float l, uint32_t s_buf,
-                                             uint32_t o_at, uint64_t* done, uint32_t parity, unsigned int* err, volatile int* abort) {
+__device__ __noinline__ RowSums wide_step(const PrefixNote& note, int left, float unit_q, float m, float l, uint32_t s_buf, uint32_t o_at,
+                                          uint64_t* done, uint32_t parity, unsigned int* err, volatile int* abort) {
   const int flags = note.all_flags();
   auto group = [&](int g, float (&v)[16]) {
     tmem_ld16(s_buf + 16 * g, v);
@@ -643,9 +640,10 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
       int64_t row;     // id, then block and head in the pool, then token
       float k, v;
     };
+    constexpr int64_t kNoTokens = INT64_MIN;   // no group of the step, or one behind the last token
     int step = run.on() ? run.s0 : 0;
     auto read_id = [&]() {
-      Place x = {run.on(), false, step, run.unit, -1, 0.f, 0.f};
+      Place x = {run.on(), false, step, run.unit, kNoTokens, 0.f, 0.f};
       if (x.on && lane < 4 && step * kPrefixStep + 16 * lane < tokens)
         x.row = a.block_ids[(step * kPrefixStep + 16 * lane) >> bt_log];
       if (x.on) run.step(step);
@@ -655,7 +653,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
       x.in = x.row >= 0 && x.row < a.c.num_blocks;
       const int64_t hb = x.in ? x.row * a.c.num_kv_heads + x.unit % a.parts.kv_heads : 0;
       x.k = x.in ? a.c.k_scale[hb] : 0.f;
-      x.v = x.in ? a.c.v_scale[hb] : 0.f;
+      x.v = x.in ? a.c.v_scale[hb] : x.row == kNoTokens ? 0x1p-8f : 0.f;   // (an ordinary one)
       x.row = (hb << bt_log) + ((x.step * kPrefixStep + 16 * lane) & (bt - 1));
     };
     // one lane for each copy: that of the copy's first 16 tokens
@@ -676,7 +674,7 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
     read_scales(now);
     Place next = read_id();
     const ScaleWindow window(__shfl_sync(0xffffffffu, now.v, 0));
-    bool wide = false;   // of the lane's groups
+    int wide = 0;   // kWide, once a scale of the lane's groups was outside the window
     bool in_v[kAhead + 1] = {};
     int64_t row_v[kAhead + 1] = {};
     for (int it = 0, end = INT_MAX - kAhead; !abort && it < end + kAhead; ++it) {
@@ -687,10 +685,22 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
       if (it < end) {
         in_v[0] = now.in;
         row_v[0] = now.row;
-        const bool gone = lane < 4 && !now.in && now.step * kPrefixStep + 16 * lane < tokens, some = !(now.v < kLeastScale);
-        if (gone && a.err) atomicOr(a.err, GLT_DEVERR_BAD_SHAPE);
-        wide |= now.in && some && !window.holds(now.v);
-        const float ks = now.k, vs = now.v;
+        const float ks = now.k;
+        float vs = now.v;
+        int flags = wide;
+        if (!(vs >= window.low && vs <= window.high)) {
+          const bool none = vs < kLeastScale;
+          if (now.in) {
+            if (!none || window.high > kMostBesideNone) flags = wide = kWide;
+          } else if (none) {   // (not a group without tokens)
+            flags |= kLost;
+            if (a.err) atomicOr(a.err, GLT_DEVERR_BAD_SHAPE);
+          }
+          if (none) {
+            flags |= kNone;
+            vs = kLeastScale;
+          }
+        }
         read_scales(next);
         now = next;
         next = read_id();
@@ -699,9 +709,9 @@ __global__ void __launch_bounds__(kPrefixThreads, 1) kv8_prefix_kernel(const __g
           PrefixNote& note = notes[it % kNotes];
           if (lane < 4) {
             note.k[lane] = ks;
-            note.log_v[lane] = (some ? log2f(vs) : window.none_log) + ks * 0.f;   // NaN where the scale of K is one (which the softmax drops)
-            note.inv_v[lane] = some ? 1.f / vs : window.none_inv;
-            note.flags[lane] = (gone ? kLost : 0) | (some ? 0 : kNone) | (wide ? kWide : 0);
+            note.log_v[lane] = log2f(vs) + ks * 0.f;   // NaN where the scale of K is one (which the softmax drops)
+            note.inv_v[lane] = 1.f / vs;
+            note.flags[lane] = static_cast<uint8_t>(flags);
           }
           __syncwarp();
           copy(a.c.k, in_v[0], row_v[0]);
